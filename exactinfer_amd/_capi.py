@@ -23,6 +23,9 @@ EXPORTS = (
     "ei_decode_step", "ei_decode_step_noalloc", "ei_attn_decode_paged", "ei_decode_step_paged", "ei_attn_prefill", "ei_attn_prefill_ws_bytes", "ei_attn_prefill_split", "ei_prefill_step", "ei_prefill_step_paged", "ei_qkv_project", "ei_stream_ceiling", "ei_synth_fill",
     "ei_attn_workspace_status", "ei_decode_status_check", "ei_read_ceiling",
     "ei_qkv_project_max_rows",
+    # include/ei_packed.h
+    "ei_rope_table_scaled", "ei_rope_rows", "ei_packed_plan_bytes", "ei_packed_plan", "ei_packed_ws_bytes",
+    "ei_attn_packed", "ei_attn_packed_paged", "ei_packed_step_paged",
     # include/ei_gguf.h
     "ei_gguf_open", "ei_gguf_close", "ei_gguf_version", "ei_gguf_n_tensors", "ei_gguf_tensor", "ei_gguf_find_tensor",
     "ei_gguf_get_int", "ei_gguf_get_float", "ei_gguf_get_str", "ei_gguf_qwen3_config",
@@ -60,6 +63,16 @@ _SIGS = {
     "ei_prefill_step_paged": ([_vp, _vp, _l, _vp, _vp, _vp, _vp, _i, _i, _vp, _i, _i, _i, _i, _vp, _vp, _vp, _i, _f, _f,
                                _i, _vp, _sz], _i),
     "ei_qkv_project": ([_vp, _vp, _l, _i, _i, _vp, _f, _vp, _i, _i, _vp, _l], _i),
+    "ei_rope_table_scaled": ([_vp, _vp, _i, _i, _d, _vp], _i),
+    "ei_rope_rows": ([_vp, _vp, _l, _vp, _l, _i, _i, _i, _vp, _f, _vp, _i, _vp, _i, _i], _i),
+    "ei_packed_plan_bytes": ([_i, _i, _i, _i], _sz),
+    "ei_packed_plan": ([_vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _sz], _i),
+    "ei_packed_ws_bytes": ([_i, _i, _i], _sz),
+    "ei_attn_packed": ([_vp, _vp, _l, _vp, _vp, _l, _vp, _i, _i, _i, _i, _i, _f, _vp, _sz, _vp, _sz], _i),
+    "ei_attn_packed_paged": ([_vp, _vp, _l, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _f, _vp, _sz, _vp, _sz],
+                             _i),
+    "ei_packed_step_paged": ([_vp, _vp, _l, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _i, _i,
+                              _f, _f, _vp, _sz, _vp, _sz], _i),
     "ei_gguf_open": ([ctypes.c_char_p], _vp),
     "ei_gguf_close": ([_vp], None),
     "ei_gguf_version": ([_vp], _i),
@@ -73,6 +86,14 @@ _SIGS = {
     "ei_stream_ceiling": ([_vp, _vp, _vp, _i, _i, _vp], _i),
     "ei_synth_fill": ([_vp, _vp, _sz, _u64, _u64, _l, _l, _f], _i),
 }
+
+
+class RopeScalingC(ctypes.Structure):
+    """ei_rope_scaling of include/ei_packed.h."""
+
+    _fields_ = [("kind", _i), ("factor", _d), ("n_trained", _i), ("beta_fast", _d), ("beta_slow", _d),
+                ("attn_factor", _d)]
+
 
 _lib = None
 

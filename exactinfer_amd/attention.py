@@ -273,6 +273,242 @@ def prefill_step(qkv: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor, shape: A
     return out
 
 
+# ---------------------------------------------------------------- rotary positions of packed rows
+_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
+_LAYOUTS = {"half": 0, "interleaved": 1}
+
+
+@dataclass(frozen=True)
+class RopeScaling:
+    """How the rotary frequencies are scaled for contexts `factor` times as long as the n_trained
+    positions a model was trained for (include/ei_packed.h): none, linear, ntk or yarn."""
+
+    kind: str = "none"
+    factor: float = 1.0
+    n_trained: int = 0
+    beta_fast: float = 32.0
+    beta_slow: float = 1.0
+    attn_factor: float = 0.0  # yarn: factor on cos and sin, 0: 0.1 ln(factor) + 1
+
+
+def _need_here(name: str, t: torch.Tensor, dtype: torch.dtype, inner: bool = True) -> None:
+    """A tensor of this dtype on the current device, whose stream the call is launched on."""
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a GPU tensor")
+    if t.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.device.index != torch.cuda.current_device():
+        raise ValueError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
+    if inner and t.numel() and t.stride(-1) != 1:
+        raise ValueError(f"{name} must be contiguous in its last dimension")
+
+
+def _need_contiguous(name: str, t: torch.Tensor, dtype: torch.dtype) -> None:
+    _need_here(name, t, dtype, inner=False)
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _need_gamma(name: str, t: torch.Tensor | None) -> None:
+    if t is not None:
+        _need_contiguous(name, t, torch.float32)
+        if t.numel() != HEAD_DIM:
+            raise ValueError(f"{name} must hold {HEAD_DIM} values, got {t.numel()}")
+
+
+def _rows_of(name: str, t: torch.Tensor, rows: int, width: int) -> int:
+    """Row stride of a [>= rows, >= width] matrix (or [>= rows, heads, 128]), after checking it."""
+    _need_here(name, t, torch.float32)
+    if t.dim() == 3 and (t.stride(1) == t.shape[2] or t.shape[1] == 1):
+        have = t.shape[1] * t.shape[2]
+    elif t.dim() == 2:
+        have = t.shape[1]
+    else:
+        raise ValueError(f"{name} must be [rows, values] or [rows, heads, {HEAD_DIM}] with whole rows")
+    if t.shape[0] < rows or have < width:
+        raise ValueError(f"{name} must hold {rows} rows of {width} values, got {tuple(t.shape)}")
+    # (the stride of a single row is whatever the view says, and is not used)
+    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), (have + 3) // 4 * 4)
+
+
+def rope_table_scaled(n_pos: int, rope_dim: int = HEAD_DIM, theta: float = 1e6, scaling: RopeScaling | None = None,
+                      out: torch.Tensor | None = None, device="cuda") -> torch.Tensor:
+    """[n_pos, rope_dim/2, 2] (cos, sin) table made on the GPU, angles in double, for plain or scaled
+    frequencies (ei_rope_table_scaled).  It serves every function that takes a table."""
+    import ctypes
+    sc = scaling or RopeScaling()
+    if sc.kind not in _SCALINGS:
+        raise ValueError(f"scaling kind {sc.kind!r}: one of {', '.join(_SCALINGS)}")
+    if out is None:
+        out = torch.empty((n_pos, rope_dim // 2, 2), dtype=torch.float32, device=device)
+    _need_contiguous("out", out, torch.float32)
+    if out.shape != (n_pos, rope_dim // 2, 2):
+        raise ValueError(f"out must be [{n_pos}, {rope_dim // 2}, 2], got {tuple(out.shape)}")
+    c = _capi.RopeScalingC(_SCALINGS[sc.kind], sc.factor, sc.n_trained, sc.beta_fast, sc.beta_slow, sc.attn_factor)
+    _capi.call("ei_rope_table_scaled", _stream(), out.data_ptr(), n_pos, rope_dim, float(theta), ctypes.byref(c))
+    return out
+
+
+def _table_positions(cs: torch.Tensor, rope_dim: int) -> int:
+    _need_contiguous("cs", cs, torch.float32)
+    if cs.dim() != 3 or cs.shape[1] != rope_dim // 2 or cs.shape[2] != 2:
+        raise ValueError(f"cs must be [positions, {rope_dim // 2}, 2], got {tuple(cs.shape)}")
+    return cs.shape[0]
+
+
+def rope_rows(x: torch.Tensor, n_heads: int, cs: torch.Tensor, pos: torch.Tensor, rope_dim: int = HEAD_DIM,
+              layout: str = "half", gamma: torch.Tensor | None = None, eps: float = 1e-6,
+              out: torch.Tensor | None = None) -> torch.Tensor:
+    """Turns the first n_heads heads of each row of x [rows, >= n_heads*128] to the row's position
+    pos (int32 [rows]), normed first when gamma is given (ei_rope_rows).  Into `out`, which may be x;
+    a row whose position lies outside the table is copied as it is."""
+    if layout not in _LAYOUTS:
+        raise ValueError(f"layout {layout!r}: one of {', '.join(_LAYOUTS)}")
+    _need_contiguous("pos", pos, torch.int32)
+    _need_gamma("gamma", gamma)
+    rows, width = pos.numel(), n_heads * HEAD_DIM
+    xs = _rows_of("x", x, rows, width)
+    if out is None:
+        out = torch.empty((rows, width), dtype=torch.float32, device=x.device)
+    ys, n_pos = _rows_of("out", out, rows, width), _table_positions(cs, rope_dim)
+    if rows:  # (an empty tensor has no address)
+        _capi.call("ei_rope_rows", _stream(), x.data_ptr(), xs, out.data_ptr(), ys, rows, n_heads, HEAD_DIM,
+                   _ptr(gamma), float(eps), cs.data_ptr(), n_pos, pos.data_ptr(), rope_dim, _LAYOUTS[layout])
+    return out
+
+
+# ---------------------------------------------------------------- several sequences' rows in one call
+class PackedBatch:
+    """Plan and workspace of batches of up to max_seq sequences and max_rows new rows
+    (include/ei_packed.h).  plan() lays a batch out from its lengths, once for all layers; the calls
+    that take the batch then run one after another (they share the workspace)."""
+
+    def __init__(self, max_seq: int, max_rows: int, n_head: int, n_head_kv: int, device="cuda"):
+        self.max_seq, self.max_rows, self.n_head, self.n_head_kv = max_seq, max_rows, n_head, n_head_kv
+        self.nbytes = int(_capi.lib().ei_packed_plan_bytes(max_seq, max_rows, n_head, n_head_kv))
+        self.ws_nbytes = int(_capi.lib().ei_packed_ws_bytes(max_rows, n_head, n_head_kv))
+        if self.nbytes == 0 or self.ws_nbytes == 0:
+            raise ValueError("invalid packed batch shape")
+        self.buf = torch.empty(self.nbytes, dtype=torch.uint8, device=device)
+        self.ws = torch.empty(self.ws_nbytes, dtype=torch.uint8, device=device)
+        self.n_seq = 0  # no plan yet
+        self.rows = 0
+        self.prompts = False
+
+    def plan(self, cu_rows: torch.Tensor, rows: int, max_kv: int, kv_len: torch.Tensor | None = None) -> None:
+        """cu_rows int32 [n_seq + 1]: sequence s owns rows cu_rows[s] .. cu_rows[s+1] - 1, of `rows` in
+        all (later ones belong to nobody).  kv_len int32 [n_seq], each at most max_kv: keys after the
+        new rows are appended; None: whole prompts."""
+        _need_contiguous("cu_rows", cu_rows, torch.int32)
+        n_seq = cu_rows.numel() - 1
+        if not 1 <= n_seq <= self.max_seq or not 0 <= rows <= self.max_rows:
+            raise ValueError(f"batch of {n_seq} sequences and {rows} rows: made for 1 to {self.max_seq} sequences and "
+                             f"up to {self.max_rows} rows")
+        if kv_len is not None:
+            _need_contiguous("kv_len", kv_len, torch.int32)
+            if kv_len.numel() != n_seq:
+                raise ValueError(f"kv_len must hold {n_seq} lengths, got {kv_len.numel()}")
+        _capi.call("ei_packed_plan", _stream(), cu_rows.data_ptr(), _ptr(kv_len), n_seq, rows, max_kv, self.n_head,
+                   self.n_head_kv, self.buf.data_ptr(), self.nbytes)
+        self.n_seq, self.rows, self.prompts = n_seq, rows, kv_len is None
+
+    def _check(self, shape: AttnShape) -> None:
+        if self.n_seq == 0:
+            raise ValueError("the batch has no plan yet: call plan() first")
+        if (shape.n_head, shape.n_head_kv) != (self.n_head, self.n_head_kv):
+            raise ValueError(f"the batch was made for {self.n_head}/{self.n_head_kv} heads, the call has "
+                             f"{shape.n_head}/{shape.n_head_kv}")
+
+    def _out(self, out: torch.Tensor | None, device) -> torch.Tensor:
+        if out is None:
+            return torch.empty((self.rows, self.n_head, HEAD_DIM), dtype=torch.float32, device=device)
+        _need_contiguous("out", out, torch.float32)
+        if out.numel() < self.rows * self.n_head * HEAD_DIM:
+            raise ValueError(f"out must hold {self.rows} rows of {self.n_head * HEAD_DIM} values")
+        return out
+
+    def _tail(self) -> tuple:
+        return self.buf.data_ptr(), self.nbytes, self.ws.data_ptr(), self.ws_nbytes
+
+
+def attn_packed(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, batch: PackedBatch, shape: AttnShape,
+                scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of whole prompts packed one after another (ei_attn_packed): q [rows, >= H*128],
+    k and v [rows, >= HKV*128] (normed and turned; views of one buffer are fine), batch planned without
+    kv_len; returns [rows, H, 128]."""
+    batch._check(shape)
+    if not batch.prompts:
+        raise ValueError("the batch is planned over a cache (kv_len): attn_packed takes whole prompts")
+    qs = _rows_of("q", q, batch.rows, shape.n_head * HEAD_DIM)
+    ks, vs = _rows_of("k", k, batch.rows, shape.kd), _rows_of("v", v, batch.rows, shape.kd)
+    if ks != vs:
+        raise ValueError(f"k and v must share a row stride, got {ks} and {vs}")
+    out = batch._out(out, q.device)
+    scale = default_scale() if scale is None else scale
+    if batch.rows == 0:
+        return out
+    _capi.call("ei_attn_packed", _stream(), q.data_ptr(), qs, k.data_ptr(), v.data_ptr(), ks, out.data_ptr(),
+               batch.n_seq, batch.rows, shape.n_head, shape.n_head_kv, shape.head_dim, float(scale), *batch._tail())
+    return out
+
+
+def _pool_args(kc: torch.Tensor, vc: torch.Tensor, block_table: torch.Tensor, block_size: int, batch: PackedBatch,
+               shape: AttnShape) -> tuple:
+    for name, t in (("kc", kc), ("vc", vc)):
+        _need_contiguous(name, t, torch.float32)
+    if kc.numel() != vc.numel() or kc.numel() % shape.kd:
+        raise ValueError(f"kc and vc must be pools of rows of {shape.kd} values, got {tuple(kc.shape)} and "
+                         f"{tuple(vc.shape)}")
+    _need_contiguous("block_table", block_table, torch.int32)
+    if block_table.dim() != 2 or block_table.shape[0] < batch.n_seq:
+        raise ValueError(f"block_table must be [{batch.n_seq}, blocks], got {tuple(block_table.shape)}")
+    if block_size <= 0:
+        raise ValueError(f"block_size {block_size} must be positive")
+    return (kc.data_ptr(), vc.data_ptr(), kc.numel() // shape.kd // block_size, block_table.data_ptr(),
+            block_table.shape[1], block_size)
+
+
+def attn_packed_paged(q: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor, block_table: torch.Tensor, block_size: int,
+                      batch: PackedBatch, shape: AttnShape, scale: float | None = None,
+                      out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of the batch's new rows, q [rows, >= H*128] normed and turned, over each sequence's pages
+    of the pool kc, vc (their new keys already there; block_table int32 [n_seq, blocks]): a chunk of a
+    prompt, draft tokens or a single token each (ei_attn_packed_paged).  Returns [rows, H, 128]."""
+    batch._check(shape)
+    qs = _rows_of("q", q, batch.rows, shape.n_head * HEAD_DIM)
+    pool = _pool_args(kc, vc, block_table, block_size, batch, shape)
+    out = batch._out(out, q.device)
+    scale = default_scale() if scale is None else scale
+    if batch.rows == 0:
+        return out
+    _capi.call("ei_attn_packed_paged", _stream(), q.data_ptr(), qs, out.data_ptr(), *pool, batch.n_seq, batch.rows,
+               shape.n_head, shape.n_head_kv, shape.head_dim, float(scale), *batch._tail())
+    return out
+
+
+def packed_step_paged(qkv: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor, block_table: torch.Tensor,
+                      block_size: int, batch: PackedBatch, shape: AttnShape, q_gamma: torch.Tensor,
+                      k_gamma: torch.Tensor, cs: torch.Tensor, scale: float | None = None,
+                      out: torch.Tensor | None = None) -> torch.Tensor:
+    """The whole step of a batch from raw projections qkv [rows, >= (H+2HKV)*128], which it only reads:
+    QK-norm and rotary positions, K and V appended to the sequences' pages, attention
+    (ei_packed_step_paged).  Returns [rows, H, 128]."""
+    batch._check(shape)
+    rs = _rows_of("qkv", qkv, batch.rows, shape.qkv)
+    pool = _pool_args(kc, vc, block_table, block_size, batch, shape)
+    _need_gamma("q_gamma", q_gamma)
+    _need_gamma("k_gamma", k_gamma)
+    n_pos = _table_positions(cs, shape.rope_dim)
+    out = batch._out(out, qkv.device)
+    scale = default_scale() if scale is None else scale
+    if batch.rows == 0:
+        return out
+    _capi.call("ei_packed_step_paged", _stream(), qkv.data_ptr(), rs, out.data_ptr(), *pool, batch.n_seq, batch.rows,
+               shape.n_head, shape.n_head_kv, shape.head_dim, q_gamma.data_ptr(), k_gamma.data_ptr(), cs.data_ptr(),
+               n_pos, shape.rope_dim, float(shape.eps), float(scale), *batch._tail())
+    return out
+
+
 # ---------------------------------------------------------------- synthetic inputs
 def synth_fill(t: torch.Tensor, seed: int, offset: int = 0, row_len: int = 1, spike_every: int = 0,
                spike_mult: float = 1.0) -> torch.Tensor:
@@ -299,5 +535,6 @@ def decode_bytes(kv_len: int, n_head: int, n_head_kv: int, head_dim: int = HEAD_
 __all__ = [
     "AttnShape", "DecodeWorkspace", "attn_decode", "attn_decode_batched", "attn_prefill", "decode_step",
     "default_scale", "headnorm_rope", "kv_append", "qkv_prepare", "rope_table", "synth_fill", "flops_causal",
-    "decode_bytes",
+    "decode_bytes", "RopeScaling", "rope_table_scaled", "rope_rows", "PackedBatch", "attn_packed",
+    "attn_packed_paged", "packed_step_paged",
 ]

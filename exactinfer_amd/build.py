@@ -15,9 +15,10 @@ PKG = Path(__file__).resolve().parent
 ROOT = PKG.parent
 CSRC = PKG / "csrc"
 LIB = PKG / "libei_attn.so"
-SOURCES = ["csrc/prologue.hip", "csrc/decode.hip", "csrc/prefill.hip", "csrc/project.hip", "csrc/capi.cpp",
+SOURCES = ["csrc/prologue.hip", "csrc/decode.hip", "csrc/prefill.hip", "csrc/project.hip", "csrc/rope.hip",
+           "csrc/packed.hip", "csrc/capi.cpp",
            "host/hip_attention.cpp", "host/gguf_index.cpp", "host/qwen3_schema.cpp"]
-HEADERS = ["common.h", "launch.h"]
+HEADERS = ["common.h", "launch.h", "planes.h"]
 
 HIPCC_FLAGS = [
     "--offload-arch=gfx950",
@@ -55,7 +56,7 @@ def build(verbose: bool = False) -> Path:
 def inputs() -> list[Path]:
     """Every file the library is built from: the sources, the private headers and the ABI header."""
     return ([PKG / s for s in SOURCES] + [CSRC / h for h in HEADERS] + [PKG / "host" / h for h in ("gguf_index.h", "hip_attention.h")] +
-            [ROOT / "include" / h for h in ("ei_attn.h", "ei_gguf.h")])
+            [ROOT / "include" / h for h in ("ei_attn.h", "ei_gguf.h", "ei_packed.h")])
 
 
 def is_stale() -> bool:

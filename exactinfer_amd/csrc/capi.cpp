@@ -12,6 +12,7 @@
 
 #include "../../include/ei_attn.h"
 #include "../../include/ei_gguf.h"
+#include "../../include/ei_packed.h"
 #include "../host/gguf_index.h"
 #include "launch.h"
 
@@ -615,6 +616,234 @@ EI_API int ei_synth_fill(ei_stream_t stream, float* dst, size_t n, uint64_t seed
     return hip_status(ei::launch_synth_fill(static_cast<hipStream_t>(stream), dst, n, seed, offset, row_len,
                                             spike_every, spike_mult),
                       "synth fill launch");
+}
+
+// ------------------------------------------------------------------ packed batches (include/ei_packed.h)
+namespace {
+
+// whether [a, a + a_bytes) and [b, b + b_bytes) share a byte
+bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + b_bytes && y < x + a_bytes;
+}
+// bytes from a matrix's first value to its last
+size_t span_bytes(int rows, long stride, long width) {
+    return rows > 0 ? ((size_t)(rows - 1) * (size_t)stride + (size_t)width) * sizeof(float) : 0;
+}
+
+constexpr int kMaxPackedSeqs = 65535;
+
+bool packed_shape_ok(int n_seq, int rows, int n_head, int n_head_kv) {
+    return n_seq > 0 && n_seq <= kMaxPackedSeqs && rows >= 0 && n_head > 0 && n_head_kv > 0 &&
+           n_head_kv <= kMaxKvHeads && n_head % n_head_kv == 0 && n_head / n_head_kv <= 8 &&
+           prefill_rows_ok(rows, n_head);
+}
+
+int check_packed(int n_seq, int rows, int n_head, int n_head_kv, int head_dim, const void* plan, size_t plan_bytes,
+                 const void* ws, size_t ws_bytes, const float* out) {
+    if (int e = check_heads(n_head, n_head_kv, head_dim)) return e;
+    REQUIRE(n_seq > 0 && n_seq <= kMaxPackedSeqs, "n_seq %d out of range [1, 65535]", n_seq);
+    REQUIRE(rows >= 0 && prefill_rows_ok(rows, n_head),
+            "rows %d x n_head %d: at most 2^20 rows and 2^28 query rows per launch", rows, n_head);
+    const size_t need = ei::packed_plan_bytes(n_seq, rows, n_head, n_head_kv);
+    REQUIRE(plan && aligned16(plan) && plan_bytes >= need,
+            "plan missing, not 16-byte aligned or %zu B < %zu B (ei_packed_plan_bytes)", plan_bytes, need);
+    const size_t ws_need = ei::packed_ws_bytes(rows, n_head, n_head_kv);
+    REQUIRE(ws && aligned16(ws) && ws_bytes >= ws_need,
+            "workspace missing, not 16-byte aligned or %zu B < %zu B (ei_packed_ws_bytes)", ws_bytes, ws_need);
+    REQUIRE(out && aligned16(out), "out missing or not 16-byte aligned");
+    const size_t out_bytes = (size_t)rows * n_head * head_dim * sizeof(float);
+    REQUIRE(!overlap(out, out_bytes, ws, ws_need) && !overlap(out, out_bytes, plan, need) &&
+                !overlap(plan, need, ws, ws_need),
+            "out, plan and workspace overlap");
+    return EI_OK;
+}
+
+int check_pool(const float* kc, const float* vc, int n_blocks, const int* block_table, int max_blocks, int block_size,
+               int* shift) {
+    REQUIRE(kc && vc && block_table, "null pointer argument");
+    REQUIRE(aligned16(kc) && aligned16(vc), "pointers must be 16-byte aligned");
+    REQUIRE(block_size >= 32 && (block_size & (block_size - 1)) == 0,
+            "block_size %d must be a power of two >= 32 (whole 32-key tiles per block)", block_size);
+    REQUIRE(max_blocks > 0 && (long)max_blocks * block_size <= 0x7FFFFFFFL,
+            "max_blocks %d x block_size %d must lie in [1, 2^31 - 1] keys", max_blocks, block_size);
+    REQUIRE(n_blocks > 0, "n_blocks %d must be positive", n_blocks);
+    int s = 0;
+    while ((1 << s) < block_size) ++s;
+    *shift = s;
+    return EI_OK;
+}
+
+}  // namespace
+
+EI_API int ei_rope_table_scaled(ei_stream_t stream, float* cs, int n_pos, int rope_dim, double theta,
+                                const ei_rope_scaling* scaling) {
+    REQUIRE(cs != nullptr && aligned16(cs), "cs missing or not 16-byte aligned");
+    REQUIRE(n_pos > 0, "n_pos %d must be positive", n_pos);
+    REQUIRE(rope_dim > 0 && rope_dim % 2 == 0 && rope_dim <= ei::kHeadDimMax,
+            "rope_dim %d must be even and in (0, %d]", rope_dim, ei::kHeadDimMax);
+    REQUIRE(theta > 0.0 && std::isfinite(theta), "theta must be positive");
+    const int kind = scaling ? scaling->kind : EI_ROPE_NONE;
+    REQUIRE(kind >= EI_ROPE_NONE && kind <= EI_ROPE_YARN, "scaling kind %d", kind);
+    const double s = kind == EI_ROPE_NONE ? 1.0 : scaling->factor;
+    REQUIRE(s >= 1.0 && std::isfinite(s), "scaling factor %g must be >= 1", s);
+    REQUIRE(kind != EI_ROPE_NTK || rope_dim > 2, "rope_dim %d: NTK scaling needs more than one pair", rope_dim);
+    if (kind == EI_ROPE_NTK) theta *= std::pow(s, double(rope_dim) / (rope_dim - 2));
+    ei::RopeFrequencies fr{};
+    fr.m = 1.0;
+    double lo = 0.0, width = 1.0;
+    if (kind == EI_ROPE_YARN) {
+        REQUIRE(scaling->n_trained > 0, "n_trained %d must be positive", scaling->n_trained);
+        REQUIRE(scaling->beta_slow > 0.0 && scaling->beta_fast >= scaling->beta_slow &&
+                    std::isfinite(scaling->beta_fast),
+                "beta_fast %g must be >= beta_slow %g > 0", scaling->beta_fast, scaling->beta_slow);
+        REQUIRE(theta > 1.0, "theta %g: the ramp needs a base above 1", theta);
+        // the pair that makes `turns` turns over the trained positions
+        auto pair = [&](double turns) {
+            return rope_dim * std::log(scaling->n_trained / (turns * 6.283185307179586)) / (2.0 * std::log(theta));
+        };
+        lo = std::fmax(std::floor(pair(scaling->beta_fast)), 0.0);
+        const double hi = std::fmin(std::ceil(pair(scaling->beta_slow)), rope_dim - 1.0);
+        width = std::fmax(hi - lo, 1e-3);
+        fr.m = scaling->attn_factor > 0.0 ? scaling->attn_factor : 0.1 * std::log(s) + 1.0;
+    }
+    for (int i = 0; i < rope_dim / 2; ++i) {
+        const double f = std::pow(theta, -2.0 * i / rope_dim);
+        if (kind == EI_ROPE_LINEAR) fr.f[i] = f / s;
+        else if (kind == EI_ROPE_YARN) {
+            const double ramp = std::fmin(std::fmax((i - lo) / width, 0.0), 1.0);
+            fr.f[i] = f / s * ramp + f * (1.0 - ramp);
+        } else fr.f[i] = f;
+    }
+    return hip_status(ei::launch_rope_table(static_cast<hipStream_t>(stream), cs, n_pos, rope_dim, fr),
+                      "rope table launch");
+}
+
+EI_API int ei_rope_rows(ei_stream_t stream, const float* x, long x_stride, float* y, long y_stride, int rows,
+                        int n_heads, int head_dim, const float* gamma, float eps, const float* cs, int n_pos,
+                        const int* pos, int rope_dim, int layout) {
+    if (head_dim != 128) return fail(EI_ERR_UNSUPPORTED, "head_dim %d: only 128 is built", head_dim);
+    if (int e = check_rope(rope_dim, head_dim)) return e;
+    REQUIRE(layout == EI_ROPE_HALF || layout == EI_ROPE_INTERLEAVED, "layout %d", layout);
+    REQUIRE(x && y && cs && pos, "null pointer argument");
+    REQUIRE(rows >= 0 && n_heads > 0 && n_pos > 0, "rows %d / n_heads %d / n_pos %d", rows, n_heads, n_pos);
+    REQUIRE((long)rows * n_heads <= 0x7FFFFFFFL, "rows %d x n_heads %d above 2^31 - 1", rows, n_heads);
+    const long width = (long)n_heads * head_dim;
+    REQUIRE(x_stride >= width && y_stride >= width && x_stride % 4 == 0 && y_stride % 4 == 0,
+            "strides %ld / %ld must be multiples of 4 and >= n_heads*head_dim", x_stride, y_stride);
+    REQUIRE(aligned16(x) && aligned16(y) && aligned16(cs) && aligned16(gamma), "pointers must be 16-byte aligned");
+    REQUIRE((x == y && x_stride == y_stride) ||
+                !overlap(x, span_bytes(rows, x_stride, width), y, span_bytes(rows, y_stride, width)),
+            "y overlaps x without being x");
+    if (rows == 0) return ok();
+    return hip_status(ei::launch_rope_rows(static_cast<hipStream_t>(stream), x, x_stride, y, y_stride, rows, n_heads,
+                                           gamma, eps, cs, n_pos, pos, rope_dim, layout == EI_ROPE_HALF),
+                      "ei_rope_rows launch");
+}
+
+EI_API size_t ei_packed_plan_bytes(int n_seq, int rows, int n_head, int n_head_kv) {
+    return packed_shape_ok(n_seq, rows, n_head, n_head_kv) ? ei::packed_plan_bytes(n_seq, rows, n_head, n_head_kv) : 0;
+}
+
+EI_API size_t ei_packed_ws_bytes(int rows, int n_head, int n_head_kv) {
+    return packed_shape_ok(1, rows, n_head, n_head_kv) ? ei::packed_ws_bytes(rows, n_head, n_head_kv) : 0;
+}
+
+EI_API int ei_packed_plan(ei_stream_t stream, const int* cu_rows, const int* kv_len, int n_seq, int rows, int max_kv,
+                          int n_head, int n_head_kv, void* plan, size_t plan_bytes) {
+    if (int e = check_heads(n_head, n_head_kv, 128)) return e;
+    REQUIRE(n_seq > 0 && n_seq <= kMaxPackedSeqs, "n_seq %d out of range [1, 65535]", n_seq);
+    REQUIRE(rows >= 0 && prefill_rows_ok(rows, n_head),
+            "rows %d x n_head %d: at most 2^20 rows and 2^28 query rows per launch", rows, n_head);
+    REQUIRE(max_kv >= 0, "max_kv %d", max_kv);
+    REQUIRE(cu_rows != nullptr, "cu_rows is null");
+    const size_t need = ei::packed_plan_bytes(n_seq, rows, n_head, n_head_kv);
+    REQUIRE(plan && aligned16(plan) && plan_bytes >= need,
+            "plan missing, not 16-byte aligned or %zu B < %zu B (ei_packed_plan_bytes)", plan_bytes, need);
+    return hip_status(ei::launch_packed_plan(static_cast<hipStream_t>(stream), cu_rows, kv_len, n_seq, rows, max_kv,
+                                             n_head, n_head_kv, plan),
+                      "packed plan launch");
+}
+
+EI_API int ei_attn_packed(ei_stream_t stream, const float* q, long q_stride, const float* k, const float* v,
+                          long kv_stride, float* out, int n_seq, int rows, int n_head, int n_head_kv, int head_dim,
+                          float scale, const void* plan, size_t plan_bytes, void* ws, size_t ws_bytes) {
+    if (int e = check_packed(n_seq, rows, n_head, n_head_kv, head_dim, plan, plan_bytes, ws, ws_bytes, out)) return e;
+    REQUIRE(q && k && v, "null pointer argument");
+    REQUIRE(aligned16(q) && aligned16(k) && aligned16(v), "pointers must be 16-byte aligned");
+    const long qw = (long)n_head * head_dim, kw = (long)n_head_kv * head_dim;
+    REQUIRE(q_stride >= qw && q_stride % 4 == 0, "q_stride %ld", q_stride);
+    REQUIRE(kv_stride >= kw && kv_stride % 4 == 0 && kv_stride <= (1L << 24), "kv_stride %ld", kv_stride);
+    const size_t ob = span_bytes(rows, qw, qw);
+    REQUIRE(!overlap(out, ob, q, span_bytes(rows, q_stride, qw)) &&
+                !overlap(out, ob, k, span_bytes(rows, kv_stride, kw)) &&
+                !overlap(out, ob, v, span_bytes(rows, kv_stride, kw)),
+            "out overlaps q, k or v");
+    if (rows == 0) return ok();
+    ei::PackedArgs a{};
+    a.q = q, a.q_stride = q_stride;
+    a.k = k, a.v = v, a.kv_stride = kv_stride;
+    a.out = out;
+    a.n_seq = n_seq, a.rows = rows, a.H = n_head, a.HKV = n_head_kv;
+    a.scale = scale;
+    a.plan = static_cast<const char*>(plan);
+    return hip_status(ei::launch_packed(static_cast<hipStream_t>(stream), a, ws), "packed attention launch");
+}
+
+EI_API int ei_attn_packed_paged(ei_stream_t stream, const float* q, long q_stride, float* out, const float* kc,
+                                const float* vc, int n_blocks, const int* block_table, int max_blocks, int block_size,
+                                int n_seq, int rows, int n_head, int n_head_kv, int head_dim, float scale,
+                                const void* plan, size_t plan_bytes, void* ws, size_t ws_bytes) {
+    if (int e = check_packed(n_seq, rows, n_head, n_head_kv, head_dim, plan, plan_bytes, ws, ws_bytes, out)) return e;
+    int shift = 0;
+    if (int e = check_pool(kc, vc, n_blocks, block_table, max_blocks, block_size, &shift)) return e;
+    REQUIRE(q && aligned16(q), "q missing or not 16-byte aligned");
+    const long qw = (long)n_head * head_dim;
+    REQUIRE(q_stride >= qw && q_stride % 4 == 0, "q_stride %ld", q_stride);
+    REQUIRE(!overlap(out, span_bytes(rows, qw, qw), q, span_bytes(rows, q_stride, qw)), "out overlaps q");
+    if (rows == 0) return ok();
+    ei::PackedArgs a{};
+    a.q = q, a.q_stride = q_stride;
+    a.k = kc, a.v = vc, a.kv_stride = (long)n_head_kv * head_dim;
+    a.out = out;
+    a.btab = block_table;
+    a.max_blocks = max_blocks, a.bshift = shift, a.n_blocks = n_blocks;
+    a.n_seq = n_seq, a.rows = rows, a.H = n_head, a.HKV = n_head_kv;
+    a.scale = scale;
+    a.plan = static_cast<const char*>(plan);
+    return hip_status(ei::launch_packed(static_cast<hipStream_t>(stream), a, ws), "packed attention launch");
+}
+
+EI_API int ei_packed_step_paged(ei_stream_t stream, const float* qkv, long row_stride, float* out, float* kc, float* vc,
+                                int n_blocks, const int* block_table, int max_blocks, int block_size, int n_seq,
+                                int rows, int n_head, int n_head_kv, int head_dim, const float* q_gamma,
+                                const float* k_gamma, const float* cs, int n_pos, int rope_dim, float eps, float scale,
+                                const void* plan, size_t plan_bytes, void* ws, size_t ws_bytes) {
+    if (int e = check_packed(n_seq, rows, n_head, n_head_kv, head_dim, plan, plan_bytes, ws, ws_bytes, out)) return e;
+    if (int e = check_rope(rope_dim, head_dim)) return e;
+    int shift = 0;
+    if (int e = check_pool(kc, vc, n_blocks, block_table, max_blocks, block_size, &shift)) return e;
+    REQUIRE(qkv && q_gamma && k_gamma && cs, "null pointer argument");
+    REQUIRE(n_pos > 0, "n_pos %d must be positive", n_pos);
+    const long w = (long)(n_head + 2 * n_head_kv) * head_dim, qw = (long)n_head * head_dim;
+    REQUIRE(row_stride >= w && row_stride % 4 == 0 && aligned16(qkv),
+            "qkv must be 16-byte aligned, row_stride %ld a multiple of 4 and >= (H+2*HKV)*head_dim", row_stride);
+    const size_t in = span_bytes(rows, row_stride, w);
+    REQUIRE(!overlap(out, span_bytes(rows, qw, qw), qkv, in) &&
+                !overlap(ws, ei::packed_ws_bytes(rows, n_head, n_head_kv), qkv, in),
+            "out or workspace overlaps qkv");
+    if (rows == 0) return ok();
+    ei::PackedArgs a{};
+    a.k = kc, a.v = vc, a.kv_stride = (long)n_head_kv * head_dim;
+    a.out = out;
+    a.btab = block_table;
+    a.max_blocks = max_blocks, a.bshift = shift, a.n_blocks = n_blocks;
+    a.n_seq = n_seq, a.rows = rows, a.H = n_head, a.HKV = n_head_kv;
+    a.scale = scale;
+    a.plan = static_cast<const char*>(plan);
+    return hip_status(ei::launch_packed_step(static_cast<hipStream_t>(stream), a, qkv, row_stride, kc, vc, q_gamma,
+                                             k_gamma, cs, n_pos, rope_dim, eps, ws),
+                      "packed step launch");
 }
 
 // ------------------------------------------------------------------ GGUF reader (include/ei_gguf.h)

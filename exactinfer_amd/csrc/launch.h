@@ -9,6 +9,8 @@
 
 namespace ei {
 
+constexpr int kHeadDimMax = 128;
+
 // Workspaces of the decode's split merge are laid out by their size alone, so that
 // calls of any plan on one workspace agree: the status word at the top, below it a zone of
 // arrival counters (one 256-byte line per unit, unit u at (u + 1) lines below the status word;
@@ -143,5 +145,44 @@ hipError_t launch_prefill(hipStream_t st, const float* q, long q_stride, float* 
                           const float* vc, const int* pos_dev, int B, int H, int HKV, float scale, int ksplit,
                           void* ws, const float* q_gamma = nullptr, const float* cs = nullptr, float eps = 0.f,
                           const int* block_table = nullptr, int block_shift = 0, int max_blocks = 0);
+
+// ------------------------------------------------------------------ rope.hip
+struct RopeFrequencies {
+    double f[kHeadDimMax / 2];
+    double m;  // factor on cos and sin
+};
+hipError_t launch_rope_table(hipStream_t st, float* cs, int n_pos, int rope_dim, const RopeFrequencies& fr);
+// half: rotate-half pairs, else interleaved ones
+hipError_t launch_rope_rows(hipStream_t st, const float* x, long x_stride, float* y, long y_stride, int rows,
+                            int n_heads, const float* gamma, float eps, const float* cs, int n_pos, const int* pos,
+                            int rope_dim, bool half);
+
+// ------------------------------------------------------------------ packed.hip
+constexpr int kPackedCus = 256;   // workgroups the plan fills (one per CU)
+constexpr int kPlanMagic = 0x45495031;
+constexpr int kUnitRows = 128;    // flat query rows (token, head of the group) that share K/V tiles
+constexpr int kPartFloats = kUnitRows * (kHeadDimMax + 2);  // an unnormalised part of a unit: O, then (m, l)
+int packed_shares(int HKV);       // workgroups per KV head
+size_t packed_plan_bytes(int n_seq, int rows, int H, int HKV);
+size_t packed_ws_bytes(int rows, int H, int HKV);
+hipError_t launch_packed_plan(hipStream_t st, const int* cu, const int* kv_len, int n_seq, int rows, int max_kv, int H,
+                              int HKV, void* plan);
+struct PackedArgs {
+    const float* q;
+    long q_stride;      // floats between rows
+    const float* k;     // first key of row 0 (packed prompts) or of the pool
+    const float* v;
+    long kv_stride;     // floats between key rows
+    float* out;         // [rows][H][128]
+    const int* btab;    // paged: [n_seq][max_blocks], or null
+    int max_blocks, bshift, n_blocks;
+    int n_seq, rows, H, HKV;
+    float scale;
+    const char* plan;
+};
+hipError_t launch_packed(hipStream_t st, const PackedArgs& a, void* ws);
+hipError_t launch_packed_step(hipStream_t st, PackedArgs a, const float* qkv, long row_stride, float* kc, float* vc,
+                              const float* q_gamma, const float* k_gamma, const float* cs, int n_pos, int rope_dim,
+                              float eps, void* ws);
 
 }  // namespace ei
