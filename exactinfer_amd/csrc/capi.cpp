@@ -755,7 +755,7 @@ EI_API int ei_packed_plan(ei_stream_t stream, const int* cu_rows, const int* kv_
     REQUIRE(n_seq > 0 && n_seq <= kMaxPackedSeqs, "n_seq %d out of range [1, 65535]", n_seq);
     REQUIRE(rows >= 0 && prefill_rows_ok(rows, n_head),
             "rows %d x n_head %d: at most 2^20 rows and 2^28 query rows per launch", rows, n_head);
-    REQUIRE(max_kv >= 0, "max_kv %d", max_kv);
+    REQUIRE(max_kv >= 0 && max_kv <= (1 << 30), "max_kv %d out of range [0, 2^30]", max_kv);
     REQUIRE(cu_rows != nullptr, "cu_rows is null");
     const size_t need = ei::packed_plan_bytes(n_seq, rows, n_head, n_head_kv);
     REQUIRE(plan && aligned16(plan) && plan_bytes >= need,

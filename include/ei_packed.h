@@ -68,7 +68,7 @@ int ei_rope_rows(ei_stream_t stream, const float* x, long x_stride, float* y, lo
  * made once for a batch, it serves every layer, on any stream that the plan's launch comes before.
  * kv_len (device int32 [n_seq]): keys of sequence s after its new rows are appended, so that its
  * row i of n sees keys 0 .. kv_len[s] - n + i; a row that sees none (kv_len[s] < n) gets zeros.
- * kv_len NULL: whole prompts, kv_len[s] = n.  Lengths are taken as lying in [0, max_kv].
+ * kv_len NULL: whole prompts, kv_len[s] = n.  Lengths are taken as lying in [0, max_kv], max_kv <= 2^30.
  * A call of the entry points below whose n_seq, rows, heads differ from the plan's writes nothing, and so
  * does one on a plan whose cu_rows count more rows than `rows`.
  * The plan of n_seq sequences and `rows` rows takes ei_packed_plan_bytes(n_seq, rows, ...) bytes (0
