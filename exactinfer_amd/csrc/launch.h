@@ -161,7 +161,6 @@ hipError_t launch_rope_rows(hipStream_t st, const float* x, long x_stride, float
 constexpr int kPackedCus = 256;   // workgroups the plan fills (one per CU)
 constexpr int kPlanMagic = 0x45495031;
 constexpr int kUnitRows = 128;    // flat query rows (token, head of the group) that share K/V tiles
-constexpr int kPartFloats = kUnitRows * (kHeadDimMax + 2);  // an unnormalised part of a unit: O, then (m, l)
 int packed_shares(int HKV);       // workgroups per KV head
 size_t packed_plan_bytes(int n_seq, int rows, int H, int HKV);
 size_t packed_ws_bytes(int rows, int H, int HKV);

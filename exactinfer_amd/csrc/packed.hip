@@ -9,69 +9,97 @@
 namespace ei {
 
 constexpr int kKT = 32;         // keys per tile
-constexpr int kPassTiles = 5;   // a unit's fixed cost, in tiles
+constexpr int kFewRows = 32;    // units of up to so many rows go to k_packed_few
 
 // ------------------------------------------------------------------ the plan
 // The query rows of a sequence and KV head are taken flat, row f = token * G + head of the group, and
 // cut into units of kUnitRows: a unit shares its K and V tiles, whatever G is and however few tokens
-// there are.  Its cost is its causal key tiles and kPassTiles for everything done once per unit.
+// there are.  A sequence's last unit, if it has at most kFewRows rows (single tokens, drafts, tails of
+// prompts), goes to the list of few-row units and its own kernel, the others to the wide list.
 //
-// `shares` workgroups serve each KV head, all heads alike.  Each takes the same cost: first whole
-// units, dealt out in descending order of tiles and back and forth, round by round, so that the
-// workgroups walk units of about the same keys at the same time (their tiles meet in the XCD's L2);
-// then, of the last units (the smallest: one to two rounds of them, or all if there are fewer), laid
-// end to end on a line, what is missing to an equal share.  The cuts on the line may fall inside a
-// unit: its parts are merged by k_packed_combine.
+// `shares` workgroups serve each KV head, all heads alike, and take the same cost each: a unit's causal key
+// tiles, and something for what is done once per unit.  Few-row units are laid end to end on a line
+// and the line cut evenly.  Of the wide list each workgroup first takes whole units, dealt out in
+// descending order of tiles and back and forth, round by round, so that the workgroups walk units of
+// about the same keys at the same time (their tiles meet in the XCD's L2); the last units (the
+// smallest: one to two rounds of them, or all if there are fewer) form a line, of which each gets what
+// is missing to an equal share.  A cut may fall inside a unit: its parts are merged by k_packed_combine.
 //
 // Order and cuts follow from the lengths alone (no atomics decide them), so a batch planned twice
 // gives the same bits twice.
-struct PlanView {
-    int4* seq;    // first row, rows, keys, first unit (unit numbers run through the sequences)
-    int4* units;  // in the order of the deal: sequence, unit of the sequence, tiles, 0
-    int2* cuts;   // [shares + 1]: on the line, unit and first tile
+struct Unit {
+    int row0, n, len, u;    // the sequence's first row, rows and keys; the unit's number in it
+    int seq, tiles, pad[2];
 };
-__host__ __device__ inline size_t plan_seq_at() { return 256; }
-__host__ __device__ inline size_t plan_units_at(int n_seq) { return plan_seq_at() + (size_t)n_seq * 16; }
-__host__ __device__ inline long plan_max_units(int n_seq, int rows, int G) {
-    return ((long)rows * G) / kUnitRows + n_seq;
+static_assert(sizeof(Unit) == 32, "two 16-byte pieces");
+struct List {      // one kernel's work
+    Unit* units;   // dealt units in the order of the deal, then the line
+    int2* cuts;    // [shares + 1]: on the line, unit and first tile
+};
+struct PlanView {
+    int4* seq;     // first row, rows, keys, wide units before this sequence's
+    List wide, few;
+};
+// header words past the shape: rounds of the deal, units dealt, on the wide line, few-row units
+enum { kHeadRounds = 6, kHeadDealt = 7, kHeadLine = 8, kHeadFew = 9 };
+constexpr size_t kPlanSeqAt = 256;
+__host__ __device__ inline long plan_max_wide(int n_seq, int rows, int G) { return (long)rows * G / kUnitRows + n_seq; }
+__host__ __device__ inline size_t plan_wide_at(int n_seq) { return kPlanSeqAt + (size_t)n_seq * sizeof(int4); }
+__host__ __device__ inline size_t plan_few_at(int n_seq, int rows, int G) {
+    return plan_wide_at(n_seq) + (size_t)plan_max_wide(n_seq, rows, G) * sizeof(Unit);
 }
 __host__ __device__ inline size_t plan_cuts_at(int n_seq, int rows, int G) {
-    return plan_units_at(n_seq) + (size_t)plan_max_units(n_seq, rows, G) * 16;
+    return plan_few_at(n_seq, rows, G) + (size_t)n_seq * sizeof(Unit);
 }
-__device__ __forceinline__ PlanView plan_view(char* plan, int n_seq, int rows, int G) {
-    return {reinterpret_cast<int4*>(plan + plan_seq_at()), reinterpret_cast<int4*>(plan + plan_units_at(n_seq)),
-            reinterpret_cast<int2*>(plan + plan_cuts_at(n_seq, rows, G))};
+__device__ __forceinline__ PlanView plan_view(char* plan, int n_seq, int rows, int G, int shares) {
+    int2* cuts = reinterpret_cast<int2*>(plan + plan_cuts_at(n_seq, rows, G));
+    return {reinterpret_cast<int4*>(plan + kPlanSeqAt),
+            {reinterpret_cast<Unit*>(plan + plan_wide_at(n_seq)), cuts},
+            {reinterpret_cast<Unit*>(plan + plan_few_at(n_seq, rows, G)), cuts + shares + 1}};
 }
 int packed_shares(int HKV) { return kPackedCus / HKV > 1 ? kPackedCus / HKV : 1; }
 size_t packed_plan_bytes(int n_seq, int rows, int H, int HKV) {
-    const size_t b = plan_cuts_at(n_seq, rows, H / HKV) + (size_t)(packed_shares(HKV) + 1) * sizeof(int2);
+    const size_t b = plan_cuts_at(n_seq, rows, H / HKV) + 2 * (size_t)(packed_shares(HKV) + 1) * sizeof(int2);
     return (b + 255) & ~(size_t)255;
 }
 
-constexpr int kPlanThreads = 1024;
-constexpr int kPlanSeqLds = 2048;      // sequences held in LDS (more are read from the plan)
-constexpr int kMinShare = 8;           // the least cost worth a workgroup
-constexpr long kMaxRankWork = 1 << 20;  // units x sequences up to which units are sorted
+constexpr int kPlanThreads = 512;
+constexpr int kPlanSeqLds = 1024;       // sequences held in LDS (more are read from the plan)
+constexpr int kPlanLineLds = 1024;      // units of the line held in LDS (likewise)
+constexpr long kMaxRankWork = 1 << 20;  // wide units x sequences up to which units are sorted
 
-// Exclusive sum over the workgroup; total in every thread.
-__device__ __forceinline__ long long block_scan(long long v, long long* total) {
-    __shared__ long long part[kPlanThreads / 64];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    long long s = v;
+// What the two kernels' work costs, in tiles: `pass` for everything done once per unit; a workgroup is worth
+// `least`; a cut leaves whole turns (the tiles that a workgroup's waves take at a time) on both sides.
+struct ListCost {
+    int pass, least, turn;
+};
+constexpr ListCost kWideCost = {5, 8, 2}, kFewCost = {8, 16, 8};
+
+// Sum over the lanes up to this one.
+__device__ __forceinline__ long long wave_scan(long long v) {
+    const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const long long t = __shfl_up(s, d);
-        if (lane >= d) s += t;
+        const long long t = __shfl_up(v, d);
+        if (lane >= d) v += t;
     }
-    if (lane == 63) part[w] = s;
+    return v;
+}
+// Exclusive sum over the workgroup; total in every thread.
+__device__ __forceinline__ long long block_scan(long long v, long long* total) {
+    constexpr int kN = kPlanThreads / 64;
+    __shared__ long long part[kN];
+    const int w = threadIdx.x >> 6;
+    const long long s = wave_scan(v);
+    __syncthreads();  // the last call's sums have been read
+    if ((threadIdx.x & 63) == 63) part[w] = s;
     __syncthreads();
     long long before = 0, all = 0;
 #pragma unroll
-    for (int i = 0; i < kPlanThreads / 64; ++i) {
+    for (int i = 0; i < kN; ++i) {
         if (i < w) before += part[i];
         all += part[i];
     }
-    __syncthreads();
     *total = all;
     return before + s - v;
 }
@@ -81,13 +109,51 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
                                                               int max_kv, int H, int HKV, int shares,
                                                               char* __restrict__ plan) {
     __shared__ int4 seq_lds[kPlanSeqLds];
+    __shared__ int line_lds[kPlanLineLds];
     __shared__ unsigned long long load[kPackedCus];
     __shared__ long long cut_at[kPackedCus + 1];
     const int tid = threadIdx.x, G = H / HKV;
-    const PlanView pv = plan_view(plan, n_seq, rows, G);
+    const PlanView pv = plan_view(plan, n_seq, rows, G, shares);
+    // keys that rows up to `row` of a sequence of n rows and len keys see, in tiles
+    auto tiles_of = [](int n, int len, int row) { return (max(min(len - n + row + 1, len), 0) + kKT - 1) / kKT; };
+    auto wide_of = [&](int n) { return (int)(((long long)n * G + kUnitRows - 1 - kFewRows) / kUnitRows); };
 
-    // sequences: rows, keys, first unit
-    long long units = 0;
+    // The cuts of a line of `line` units: share j's end where `before` (its and the earlier shares' wants)
+    // falls on the running cost.
+    auto cut_line = [&](const List& list, int dealt, int line, ListCost c, const int* lds, long long want) {
+        long long all;
+        const long long before = block_scan(want, &all);
+        if (tid <= shares) {
+            cut_at[tid] = tid == 0 ? 0 : before;  // (thread `shares` wants nothing: the sum of all)
+            list.cuts[tid] = make_int2(tid == 0 ? 0 : line, 0);
+        }
+        __syncthreads();
+        long long at = 0;
+        for (int base = 0; base < line; base += kPlanThreads) {
+            const int i = base + tid;
+            const int tiles = i >= line ? 0 : lds ? lds[i] : list.units[dealt + i].tiles;
+            const long long cost = i < line ? tiles + c.pass : 0;
+            long long sum;
+            const long long a = at + block_scan(cost, &sum);
+            if (i < line) {
+                int lo = 1, hi = shares + 1;  // the first cut not before a
+                while (lo < hi) {
+                    const int mid = (lo + hi) >> 1;
+                    if (cut_at[mid] >= a) hi = mid;
+                    else lo = mid + 1;
+                }
+                for (; lo <= shares && cut_at[lo] < a + cost; ++lo) {
+                    const long long t = (cut_at[lo] - a) / c.turn * c.turn;
+                    if (lo == shares || t + c.turn > tiles) list.cuts[lo] = make_int2(lo == shares ? line : i + 1, 0);
+                    else list.cuts[lo] = make_int2(i, (int)t);
+                }
+            }
+            at += sum;
+        }
+    };
+
+    // sequences: rows, keys, first wide unit; the few-row units
+    long long units = 0, few = 0, few_cost = 0;
     int bad = 0;
     for (int base = 0; base < n_seq; base += kPlanThreads) {
         const int s = base + tid;
@@ -100,23 +166,38 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
             len = kv_len ? min(max(kv_len[s], 0), max_kv) : min(n, max_kv);
         }
         bad = __syncthreads_or(bad);
-        const long long nu = bad ? 0 : ((long long)n * G + kUnitRows - 1) / kUnitRows;
+        if (bad) n = 0;  // rows outside the batch: no call on this plan does anything
+        const int nw = wide_of(n), is_few = (long long)n * G > (long long)nw * kUnitRows;
+        const int tiles = is_few ? tiles_of(n, len, n - 1) : 0;
         long long all;
-        const long long at = units + block_scan(nu, &all);
+        const long long at = block_scan((long long)nw << 32 | is_few, &all);  // (both sums stay below 2^31)
         if (s < n_seq) {
-            const int4 e = make_int4(lo, n, len, (int)at);
+            const int4 e = make_int4(lo, n, len, (int)(units + (at >> 32)));
             pv.seq[s] = e;
             if (s < kPlanSeqLds) seq_lds[s] = e;
         }
-        units += all;
+        if (is_few) {
+            const int i = (int)(few + (at & 0xFFFFFFFF));
+            pv.few.units[i] = Unit{lo, n, len, nw, s, tiles, {0, 0}};
+            if (i < kPlanLineLds) line_lds[i] = tiles;
+        }
+        units += all >> 32;
+        few += all & 0xFFFFFFFF;
+        block_scan(is_few ? tiles + kFewCost.pass : 0, &all);
+        few_cost += all;
     }
-    if (bad) units = 0;  // rows outside the batch: no call on this plan does anything
+    if (bad) units = few = 0;
+    const int U = (int)units;
     __syncthreads();
+    if (few > 0) {  // uniform
+        const long long share = max((few_cost + shares - 1) / shares, (long long)kFewCost.least);
+        cut_line(pv.few, 0, (int)few, kFewCost, few <= kPlanLineLds ? line_lds : nullptr, tid < shares ? share : 0);
+        __syncthreads();
+    } else if (tid <= shares) pv.few.cuts[tid] = make_int2(0, 0);
+
     const bool in_lds = n_seq <= kPlanSeqLds;
     auto seq_at = [&](int s) { return in_lds ? seq_lds[s] : pv.seq[s]; };
-    const int U = (int)units;
-    auto units_of = [&](const int4& e) { return (int)(((long long)e.y * G + kUnitRows - 1) / kUnitRows); };
-    auto unit = [&](int i) {  // sequence, unit of the sequence, tiles
+    auto unit = [&](int i) {
         int lo = 0, hi = n_seq - 1;
         while (lo < hi) {  // the last sequence whose first unit is not past i
             const int mid = (lo + hi + 1) >> 1;
@@ -125,90 +206,76 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
         }
         const int4 e = seq_at(lo);
         const int u = i - e.w;
-        const int last = min(e.y - 1, (kUnitRows * u + kUnitRows - 1) / G);
-        const int keys = max(min(e.z - e.y + last + 1, e.z), 0);
-        return make_int4(lo, u, (int)(((long long)keys + kKT - 1) / kKT), 0);
+        const int row = min(e.y - 1, (kUnitRows * u + kUnitRows - 1) / G);
+        return Unit{e.x, e.y, e.z, u, lo, tiles_of(e.y, e.z, row), {0, 0}};
     };
-    // units of sequence e with more than t tiles (they are its last ones)
+    // wide units of sequence e with more than t tiles (they are its last ones)
     auto above = [&](const int4& e, int t) {
-        const int nu = units_of(e);
-        if (t < 0) return nu;
+        const int nw = wide_of(e.y);
+        if (t < 0) return nw;
         const long long m = 32LL * t - (e.z - e.y);  // rows that see at most t tiles
-        if (m <= 0) return nu;
-        return m >= e.y ? 0 : nu - min(nu, (int)(m * G / kUnitRows));
+        if (m <= 0) return nw;
+        return m >= e.y ? 0 : nw - min(nw, (int)(m * G / kUnitRows));
     };
-
-    long long mine = 0, total;
-    for (int i = tid; i < U; i += kPlanThreads) mine += unit(i).z + kPassTiles;
-    block_scan(mine, &total);
-    const long long even = (total + shares - 1) / shares;
-    const long long share = even > kMinShare ? even : kMinShare;
-    // (sorting costs units x sequences: where that is much, there is enough work for the order not to matter)
-    const int rounds = (long long)U * n_seq <= kMaxRankWork && U / shares > 1 ? U / shares - 1 : 0;
-    const int dealt = rounds * shares, line = U - dealt;
-    for (int j = tid; j < shares; j += kPlanThreads) load[j] = 0;
-    __syncthreads();
-    for (int i = tid; i < U; i += kPlanThreads) {
-        const int4 x = unit(i);
-        int at = i;
-        if (rounds > 0) {
-            // units before this one: more tiles, or as many in an earlier sequence, or later in its own
-            at = 0;
-            for (int s = 0; s < n_seq; ++s) {
-                const int4 e = seq_at(s);
-                at += s < x.x ? above(e, x.z - 1) : s > x.x ? above(e, x.z) : units_of(e) - 1 - x.y;
-            }
+    if (U > 0) {  // uniform
+        Unit own{};  // this thread's first unit
+        long long mine = 0, total;
+        for (int i = tid; i < U; i += kPlanThreads) {
+            const Unit x = unit(i);
+            if (i == tid) own = x;
+            mine += x.tiles + kWideCost.pass;
         }
-        pv.units[at] = x;
-        if (at < dealt) {
-            const int r = at / shares, j = at - r * shares;
-            atomicAdd(&load[(r & 1) ? shares - 1 - j : j], (unsigned long long)(x.z + kPassTiles));
-        }
-    }
-    __syncthreads();
-    long long all;
-    const long long want = tid < shares ? max(share - (long long)load[tid], 0LL) : 0;
-    const long long before = block_scan(want, &all);
-    if (tid <= shares) cut_at[tid] = tid == 0 ? 0 : before;  // (thread `shares` wants nothing: the sum of all)
-    if (tid <= shares) pv.cuts[tid] = make_int2(tid == 0 ? 0 : line, 0);
-    __syncthreads();
-    // the cuts that fall on each unit of the line
-    long long at = 0;
-    for (int base = 0; base < line; base += kPlanThreads) {
-        const int i = base + tid;
-        const int tiles = i < line ? pv.units[dealt + i].z : 0;
-        const long long cost = i < line ? tiles + kPassTiles : 0;
-        long long sum;
-        const long long a = at + block_scan(cost, &sum);
-        if (i < line) {
-            int lo = 1, hi = shares + 1;  // the first cut not before a
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (cut_at[mid] >= a) hi = mid;
-                else lo = mid + 1;
+        for (int j = tid; j < shares; j += kPlanThreads) load[j] = 0;
+        block_scan(mine, &total);
+        const long long share = max((total + shares - 1) / shares, (long long)kWideCost.least);
+        // (sorting costs units x sequences: where that is much, there is enough work for the order not to matter)
+        const int rounds = (long long)U * n_seq <= kMaxRankWork && U / shares > 1 ? U / shares - 1 : 0;
+        const int dealt = rounds * shares, line = U - dealt;
+        for (int i = tid; i < U; i += kPlanThreads) {
+            const Unit x = i == tid ? own : unit(i);
+            int at = i;
+            if (rounds > 0) {
+                // units before this one: more tiles, or as many in an earlier sequence, or later in its own
+                at = 0;
+                for (int s = 0; s < n_seq; ++s) {
+                    const int4 e = seq_at(s);
+                    at += s < x.seq ? above(e, x.tiles - 1) : s > x.seq ? above(e, x.tiles) : wide_of(e.y) - 1 - x.u;
+                }
             }
-            for (; lo <= shares && cut_at[lo] < a + cost; ++lo) {
-                // an even number of tiles on both sides of a cut (the key groups take turns), or none
-                int t = (int)(cut_at[lo] - a) & ~1;
-                if (lo == shares || t >= tiles - 1) pv.cuts[lo] = make_int2(lo == shares ? line : i + 1, 0);
-                else pv.cuts[lo] = make_int2(i, t);
-            }
+            pv.wide.units[at] = x;
+            if (at < dealt) {
+                const int r = at / shares, j = at - r * shares;
+                atomicAdd(&load[(r & 1) ? shares - 1 - j : j], (unsigned long long)(x.tiles + kWideCost.pass));
+            } else if (at - dealt < kPlanLineLds) line_lds[at - dealt] = x.tiles;
         }
-        at += sum;
+        __syncthreads();
+        const long long want = tid < shares ? max(share - (long long)load[tid], 0LL) : 0;
+        cut_line(pv.wide, dealt, line, kWideCost, line <= kPlanLineLds ? line_lds : nullptr, want);
+        if (tid == 0) {
+            int* h = reinterpret_cast<int*>(plan);
+            h[kHeadRounds] = rounds, h[kHeadDealt] = dealt, h[kHeadLine] = line;
+        }
+    } else {
+        if (tid <= shares) pv.wide.cuts[tid] = make_int2(0, 0);
+        if (tid == 0) {
+            int* h = reinterpret_cast<int*>(plan);
+            h[kHeadRounds] = h[kHeadDealt] = h[kHeadLine] = 0;
+        }
     }
     if (tid == 0) {
         int* h = reinterpret_cast<int*>(plan);
         h[0] = bad ? 0 : kPlanMagic;
         h[1] = n_seq, h[2] = rows, h[3] = H, h[4] = HKV;
         h[5] = kv_len == nullptr;
-        h[6] = rounds, h[7] = dealt, h[8] = line;
+        h[kHeadFew] = (int)few;
     }
 }
 
 // Whether the plan is one of this call's batch (and of whole prompts, where the keys are the rows).
 __device__ __forceinline__ bool plan_fits(const char* plan, int n_seq, int rows, int H, int HKV, bool prompts) {
     const int* h = reinterpret_cast<const int*>(plan);
-    return h[0] == kPlanMagic && h[1] == n_seq && h[2] == rows && h[3] == H && h[4] == HKV && (!prompts || h[5]);
+    return (h[0] == kPlanMagic) & (h[1] == n_seq) & (h[2] == rows) & (h[3] == H) & (h[4] == HKV) &
+           (!prompts | (h[5] != 0));
 }
 
 // The sequence that owns row b: the last whose first row is not past it, if it has that row; else -1.
@@ -230,22 +297,27 @@ __device__ __forceinline__ int row_owner(const int4* seq, int n_seq, int b, int 
 // Both products on v_mfma_f32_32x32x16_bf16 with fp32 operands as three bf16 planes (planes.h), six
 // plane products each, as in prefill.hip, and with its wave layout: a wave holds 32 flat query rows,
 // computes S^T[key][row] = K . Q^T, so that each lane owns one row and 16 of a tile's 32 keys, and
-// O^T[d][row] = V^T . P^T from the same registers.
+// O^T[d][row] = V^T . P^T from the same registers.  The softmax scale is multiplied into q.
 //
-// Workgroup = kGroups key groups x kSlots waves: the unit's 128 rows over the waves of a group, its
-// tiles over the groups in turn (tile kt to group kt % kGroups counted from the pass's first), whose
-// (m, l, O) meet in LDS at the end of the pass.  A pass is a unit, or the part of it between two cuts
-// of the plan's line; a part goes unnormalised to the workspace, its rows as they are numbered in the
-// unit.  Waves without rows (a unit of few) take part in loading the tiles and multiply nothing.
+// A workgroup of eight waves walks its share of a list pass by pass: a pass is a unit, or the part of it
+// between two cuts of the list's line.  A part goes unnormalised to the workspace.
 //
-// The key loop is that of prefill.hip: each wave of a group fetches a quarter of a K or V tile, 16
-// floats per lane, and stores its planes (V transposed) while the group multiplies the other of the
-// two; the groups run half an iteration apart, so that one has matrix work while the other is in its
-// softmax.
+// Wide units (wide_pass): two key groups of four waves; a group's waves hold 32 rows
+// each and share its tiles, which take turns (tile kt to group (kt - first) % 2).  The key loop is that
+// of prefill.hip: each wave of a group fetches a quarter of a K or V tile, 16 floats per lane, and
+// stores its planes in LDS (V transposed) while the group multiplies the other of the two; the groups
+// run half an iteration apart, so that one has matrix work while the other is in its softmax.  Waves
+// without rows repeat the sequence's last one and write nothing (a branch round their products costs the
+// other waves registers).
+//
+// Few-row units (few_pass): every wave holds the same rows and a tile of its own, loaded straight into the
+// operands' registers (more loads in flight, no barrier in the loop); q's planes are in LDS.  (Both kinds
+// in one kernel leave the compiler short of registers in both loops.)
 typedef __amdgpu_buffer_rsrc_t Rsrc;
 constexpr int kQB = 32;                         // flat rows per wave
 constexpr int kSlots = kUnitRows / kQB;         // waves per key group
 constexpr int kGroups = 2;                      // key groups per workgroup
+constexpr int kWaves = kSlots * kGroups;
 constexpr float kLazy = 8.f;                    // lazy-rescale threshold (log2 units)
 constexpr int kXchF = 34;                       // floats per lane exchanged by the merge
 constexpr int kRowF = kHeadDim + 4;             // padded fp32 row of the staging area
@@ -253,49 +325,665 @@ constexpr int kRowF = kHeadDim + 4;             // padded fp32 row of the stagin
 // lane, spread over all LDS banks
 constexpr int kKRowB = 2 * kHeadDim + 16, kKPlane = kKT * kKRowB;  // K plane: [32 keys][128 d] bf16
 constexpr int kVRowB = 2 * kKT + 16, kVPlane = kHeadDim * kVRowB;  // V plane, transposed: [128 d][32 keys]
-// LDS: the K planes of both groups, and the merge's exchange area, from 0; the V planes after it,
-// and over them the staging area of the unit's rows (queries, later outputs)
-constexpr int kStageF = kGroups * kSlots * kXchF * 64;
-constexpr int kLdsF = kStageF + kUnitRows * kRowF;
+// LDS of a wide pass: the K planes of both groups, and the merge's exchange area, from 0; the V planes
+// after it, and over them the staging area of the unit's rows (queries, later outputs).  Of a few-rows
+// pass: q's planes from 0; then, over them, every wave's rows, and their (m, l).
+constexpr int kStageF = kWaves * kXchF * 64;
+constexpr int kWideF = kStageF + kUnitRows * kRowF;
+constexpr int kFewML = kWaves * kQB * kRowF;
+constexpr int kFewF = kFewML + kWaves * kQB * 2;
 static_assert(kGroups * 3 * kKPlane <= kStageF * 4, "K planes below the staging area");
-static_assert(kStageF * 4 + kGroups * 3 * kVPlane <= kLdsF * 4, "V planes within the LDS span");
-static_assert(kLdsF * 4 <= 160 * 1024, "LDS budget");
+static_assert(kStageF * 4 + kGroups * 3 * kVPlane <= kWideF * 4, "V planes within the LDS span");
+static_assert(kWideF * 4 <= 160 * 1024 && kFewF * 4 <= 160 * 1024, "LDS budget");
 
 __device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
+// A pass, all of it wave-uniform.
+struct Pass {
+    int seq, u;            // sequence, unit of the sequence
+    int row0, pos0;        // first row of the sequence and its position (may be negative)
+    int nflat;             // the sequence's flat rows of this KV head
+    int T;                 // keys that the unit's last row sees
+    int kt_lo, nrange;     // tiles [kt_lo, kt_lo + nrange)
+    float* part;           // where its unnormalised rows go, or null: a whole unit
+};
+
+// The visible rows of a tile as a buffer: reads past the last one, and of a missing page, give zeros.
 template <bool kPaged>
-__global__ __launch_bounds__(64 * kSlots * kGroups) void k_packed_attn(PackedArgs a, int shares,
-                                                                       float* __restrict__ parts) {
+__device__ __forceinline__ Rsrc tile_rsrc(const PackedArgs& a, const Pass& p, const float* cache, int t0) {
+    size_t row = (size_t)p.row0 + t0;
+    int there = min(kKT, p.T - t0);
+    if constexpr (kPaged) {
+        const int blk = t0 >> a.bshift;
+        const int phys = blk < a.max_blocks ? a.btab[(size_t)p.seq * a.max_blocks + blk] : -1;
+        const bool ok = phys >= 0 && phys < a.n_blocks;
+        row = ok ? ((size_t)phys << a.bshift) | (size_t)(t0 & ((1 << a.bshift) - 1)) : 0;
+        if (!ok) there = 0;
+    }
+    return __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<float*>(cache) + row * a.kv_stride, 0,
+        there ? (int)((uint32_t)(there - 1) * (uint32_t)(a.kv_stride * 4) + kHeadDim * 4) : 0, kBufferDword3);
+}
+
+// A workgroup's parts in its kernel's share of the workspace: slot 0 of the unit that it goes on with, slot 1
+// of the one that it begins; O rows, then (m, l) of each.
+constexpr size_t kWidePart = kUnitRows * (kHeadDim + 2), kFewPart = kFewRows * (kHeadDim + 2);
+__device__ __forceinline__ size_t part_at(bool few, int block, int slot) {
+    return (size_t)(2 * block + slot) * (few ? kFewPart : kWidePart);
+}
+
+struct Sums {  // of 32 rows, one per lane and its lane ^ 32: O^T, running maximum (log2 units), sum of weights
+    floatx16 o[4];
+    float m, l;
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[db][i] = 0.f;
+        m = -INFINITY;
+        l = 0.f;
+    }
+};
+
+// Scores s of tile kt -> P (in place), the running maximum and sum, O rescaled if the maximum rose by
+// more than kLazy.  Tiles from nfull on cross the diagonal of the wave's rows.
+__device__ __forceinline__ void softmax_tile(Sums& x, floatx16& s, int kt, int nfull, int qpos, int hh) {
+    if (kt >= nfull) {
+        const int k0 = unhoisted(kt * kKT + 4 * hh);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            if (k0 + 8 * (r >> 2) + (r & 3) > qpos) s[r] = -INFINITY;
+    }
+    float mx = s[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+    const float ms = half_max(mx);
+    if (__builtin_amdgcn_ballot_w64(ms > x.m + kLazy)) {  // rare after the first tile
+        const float mn = fmaxf(x.m, ms);
+        const float corr = x.m == mn ? 1.f : __builtin_amdgcn_exp2f(x.m - mn);
+        x.l *= corr;
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x.o[db][r] *= corr;
+        x.m = mn;
+    }
+    const float nb = x.m == -INFINITY ? 0.f : -x.m;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        s[r] = __builtin_amdgcn_exp2f(s[r] + nb);
+        x.l += s[r];
+    }
+}
+
+// The planes of P's half x (registers 8x .. 8x + 7): the B operand of two steps' worth of keys.
+__device__ __forceinline__ Planes split_p(const floatx16& s, int x) {
+    uint32_t h[4], m[4], l[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) split_pair(s[8 * x + 2 * j], s[8 * x + 2 * j + 1], h[j], m[j], l[j]);
+    return {u32x4{h[0], h[1], h[2], h[3]}, u32x4{m[0], m[1], m[2], m[3]}, u32x4{l[0], l[1], l[2], l[3]}};
+}
+
+// Whether planes did not serve a wave's sums (prefill.hip has the same rule): an infinite value, or one
+// past kPlaneMax, in K or V shows as a sum that is not finite.  A V value or a weight below kPlaneMin
+// may have lost bits of its third plane, 2^-134, which shows in no sum from kSmallSum up; with a
+// smaller one the wave looks through its V tiles, in the quarters of the columns with such a sum: it
+// stands if no V value there is below kPlaneMin and the largest one is too small for the weights' 2^-134
+// to show in it.  tile(i) is the wave's i-th tile, at(db, row, quarter piece) the byte offset of four
+// values of column quarter db.
+template <bool kFew, typename Tile>
+__device__ __forceinline__ bool planes_failed(const Sums& x, int n_mine, Tile v_tile, uint32_t row_bytes, int lane) {
+    float z = x.l * 0.f, least[4];
+#pragma unroll
+    for (int db = 0; db < 4; ++db) {
+        least[db] = INFINITY;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            z = __builtin_fmaf(x.o[db][r], 0.f, z);
+            least[db] = fminf(least[db], __builtin_fabsf(x.o[db][r]));
+        }
+    }
+    if (__builtin_amdgcn_ballot_w64(z != 0.f)) return true;
+    const float least_all = fminf(fminf(least[0], least[1]), fminf(least[2], least[3]));
+    // (a lane without a visible key has no sum: m stays -inf)
+    if (!__builtin_amdgcn_ballot_w64(least_all < kSmallSum && x.m != -INFINITY)) return false;
+    uint32_t small = 0xFFFFFFFFu, tiny = 0xFFFFFFFFu;  // the smallest nonzero sum and V value
+    if (x.m != -INFINITY) {
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) small = min(small, magnitude(__float_as_uint(x.o[db][r])));
+    }
+    float most = 0.f;
+#pragma unroll
+    for (int db = 0; db < 4; ++db) {
+        if (!__builtin_amdgcn_ballot_w64(least[db] < kSmallSum && x.m != -INFINITY)) continue;
+        for (int i = 0; i < n_mine; ++i) {
+            const Rsrc rs = v_tile(i);
+            const int ln = unhoisted(lane);
+            // lane: rows ln / 8 + 8j, four of the quarter's 32 values
+            const uint32_t off = (ln >> 3) * row_bytes + (kFew ? 64u * (ln & 7) + 4u * db : 16u * (ln & 7) + 128u * db);
+#pragma unroll
+            for (int j = 0; j < kKT / 8; ++j) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t v = __builtin_amdgcn_raw_buffer_load_b32(
+                        rs, off + 8 * j * row_bytes + (kFew ? 16 : 4) * e, 0, 0);
+                    tiny = min(tiny, magnitude(v));
+                    most = fmaxf(most, __builtin_fabsf(__uint_as_float(v)));
+                }
+            }
+        }
+    }
+    // the sums are off by up to 2^20 2^-134 most; a lane without a nonzero one has nothing to lose
+    const float limit = wave_max(most) * 0x1p-84f;
+    return __builtin_amdgcn_ballot_w64(tiny < kTinyMagnitude || limit > of_magnitude(small)) != 0;
+}
+
+// A wave's tiles again, both products in fp32 from the cache.  In a tile that crosses the diagonal a
+// value that a row does not see must not be multiplied at all (0 times infinity), and the matrix
+// instruction takes every row with every key: P . V goes key by key there, P through p_lds, 32 x 32
+// floats of the wave's own.  Column of sum (db, i): 32 db + i, with kFew 4 i + db.
+template <bool kFew, typename KTile, typename VTile, typename Index>
+__device__ __forceinline__ void redo_fp32(Sums& x, const PackedArgs& a, const Pass& p, const float* q_row, float sl2,
+                                          int n_mine, KTile k_tile, VTile v_tile, Index index, int nfull, int qpos,
+                                          uint32_t row_bytes, float* p_lds, int lane) {
+    const int col = lane & 31, hh = lane >> 5;
+    // values 16t + 8hh .. + 7 of the row
+    float q[64];
+#pragma unroll
+    for (int t = 0; t < 16; ++t) {
+        const float4 v = *reinterpret_cast<const float4*>(q_row + 16 * (t >> 1) + 4 * (t & 1) + 8 * hh);
+        q[4 * t] = v.x * sl2, q[4 * t + 1] = v.y * sl2, q[4 * t + 2] = v.z * sl2, q[4 * t + 3] = v.w * sl2;
+    }
+    x.clear();
+    for (int i = 0; i < n_mine; ++i) {
+        const int kt = index(i);
+        floatx16 s;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 0.f;
+        {
+            const Rsrc rs = k_tile(i);
+            const uint32_t off = unhoisted(col) * row_bytes + 32u * hh;
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {  // d = 16t + 8hh + 2j and the next
+                    const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(rs, off + 64 * t + 8 * j, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(v.x), q[8 * t + 2 * j], s, 0, 0, 0);
+                    s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(v.y), q[8 * t + 2 * j + 1], s, 0, 0, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        softmax_tile(x, s, kt, nfull, qpos, hh);
+        const Rsrc rs = v_tile(i);
+        constexpr uint32_t kI = kFew ? 16 : 4, kDb = kFew ? 4 : 128;
+        if (kt < nfull) {
+            const uint32_t off = unhoisted(4 * hh) * row_bytes + kI * col;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {  // lane half hh: key 8(r/4) + 4hh + r%4
+#pragma unroll
+                for (int db = 0; db < 4; ++db) {
+                    const float v = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+                        rs, off + (8 * (r >> 2) + (r & 3)) * row_bytes + kDb * db, 0, 0));
+                    x.o[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[r], x.o[db], 0, 0, 0);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            continue;
+        }
+        const int ln = unhoisted(lane);
+        float* pw = p_lds + (ln & 31);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) pw[32 * (8 * (r >> 2) + 4 * (ln >> 5) + (r & 3))] = s[r];
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+        for (int key = 0; key < kKT; ++key) {
+            const float pk = pw[32 * key];
+            const uint32_t off = key * row_bytes + 4 * kI * (ln >> 5);
+            if (kt * kKT + key <= qpos) {
+#pragma unroll
+                for (int db = 0; db < 4; ++db) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {  // i = 8(r/4) + 4hh + r%4
+                        const float v = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
+                            rs, off + kDb * db + kI * (8 * (r >> 2) + (r & 3)), 0, 0));
+                        x.o[db][r] = __builtin_fmaf(pk, v, x.o[db][r]);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+        }
+        __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// ---- a wide unit
+template <bool kPaged>
+__device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, int kvh, FastDiv fG, float sl2,
+                                          float* smem) {
     constexpr int D = kHeadDim;
-    extern __shared__ __align__(16) float smem[];
-    if (!plan_fits(a.plan, a.n_seq, a.rows, a.H, a.HKV, !kPaged)) return;
-    const int kvh = blockIdx.x % a.HKV, share = blockIdx.x / a.HKV;  // a KV head's workgroups share an XCD's L2
-    const int H = a.H, G = a.H / a.HKV;
-    const FastDiv fG = fast_div((uint32_t)G);
-    const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    // (what follows from the thread's number is computed in each pass: kept over passes it would spill)
+    const int tid = unhoisted(threadIdx.x), lane = tid & 63, w = tid >> 6;
     const int wu = scalar(w), hw = wu % kSlots, grp = wu / kSlots;
     const int col = lane & 31, hh = lane >> 5;
+    const int G = (int)fG.d;
     const uint32_t row_bytes = (uint32_t)(a.kv_stride * 4);
-    const float* const kbase = a.k + (size_t)kvh * D;
-    const float* const vbase = a.v + (size_t)kvh * D;
     char* const lds = reinterpret_cast<char*>(smem);
     char* const kpl = lds + grp * 3 * kKPlane;
     char* const vpl = lds + kStageF * 4 + grp * 3 * kVPlane;
     float* const stage = smem + kStageF;
-    const float sl2 = a.scale * 1.44269504088896340736f;  // goes into q: scores come out in log2 units
     const uint32_t voff_k = (uint32_t)(8 * hw + (lane >> 3)) * row_bytes + 32u * (lane & 7);
     const uint32_t voff_v =
         (uint32_t)(16 * (lane >> 5) + 4 * ((lane >> 4) & 1)) * row_bytes + 4u * (32 * hw + 2 * (lane & 15));
+    const int f0 = kUnitRows * p.u + kQB * hw;  // this wave's first row
+    const bool live = f0 < p.nflat;
+    const int qpos = p.pos0 + fdiv(min(f0 + col, p.nflat - 1), fG);  // this lane's query
+    const int nfull = max(p.pos0 + fdiv(min(f0, p.nflat - 1), fG) + 1, 0) / kKT;  // tiles below the wave's diagonal
+    const int n_it = (p.nrange + kGroups - 1) / kGroups, n_mine = (p.nrange - grp + kGroups - 1) / kGroups;
+    auto index = [&](int i) { return p.kt_lo + kGroups * i + grp; };
+    auto k_tile = [&](int i) { return tile_rsrc<kPaged>(a, p, a.k + (size_t)kvh * D, index(i) * kKT); };
+    auto v_tile = [&](int i) { return tile_rsrc<kPaged>(a, p, a.v + (size_t)kvh * D, index(i) * kKT); };
 
-    const PlanView pv = plan_view(const_cast<char*>(a.plan), a.n_seq, a.rows, G);
+    // K and V of this group's i-th tile, a quarter per wave:
+    //   K: row 8*hw + lane/8, d = 8c .. 8c+7 and 64 + 8c .. (c = lane%8)
+    //   V: d = 32*hw + 2*(lane%16) and the next, the eight keys of chunk lane/16 (step s = chunk/2,
+    //     half hh = chunk%2 of the P.V operand: keys 16s + 4hh + {0..3, 8..11})
+    float rg[16];
+    auto load_k = [&](int i) {
+        const Rsrc rs = k_tile(i);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(rs, voff_k + 256 * (j >> 1) + 16 * (j & 1), 0, 0);
+            rg[4 * j] = __uint_as_float(v.x), rg[4 * j + 1] = __uint_as_float(v.y);
+            rg[4 * j + 2] = __uint_as_float(v.z), rg[4 * j + 3] = __uint_as_float(v.w);
+        }
+    };
+    auto load_v = [&](int i) {
+        const Rsrc rs = v_tile(i);
+        const uint32_t off = unhoisted(voff_v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(rs, off + (8 * (j >> 2) + (j & 3)) * row_bytes, 0, 0);
+            rg[2 * j] = __uint_as_float(v.x), rg[2 * j + 1] = __uint_as_float(v.y);
+        }
+    };
+    // a value of rg past kPlaneMax turns one of them into NaN, which reaches a sum of every wave that
+    // multiplies it
+    auto check_planes = [&]() {
+        float most = 0.f;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) most = fmaxf(most, __builtin_fabsf(rg[j]));
+        rg[0] = most < kPlaneMax ? rg[0] : __uint_as_float(0xFFFFFFFFu);
+    };
+    // half x of the conversion of rg: eight values, one 16-byte piece of each plane
+    auto conv_k = [&](int x) {
+        uint32_t ch[4], cm[4], cl[4];
+        if (x == 0) check_planes();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) split_pair(rg[8 * x + 2 * j], rg[8 * x + 2 * j + 1], ch[j], cm[j], cl[j]);
+        char* d = kpl + (8 * hw + (lane >> 3)) * kKRowB + 16 * (lane & 7) + 128 * x;
+        *reinterpret_cast<u32x4*>(d) = u32x4{ch[0], ch[1], ch[2], ch[3]};
+        *reinterpret_cast<u32x4*>(d + kKPlane) = u32x4{cm[0], cm[1], cm[2], cm[3]};
+        *reinterpret_cast<u32x4*>(d + 2 * kKPlane) = u32x4{cl[0], cl[1], cl[2], cl[3]};
+    };
+    auto conv_v = [&](int x) {  // d + x
+        uint32_t ch[4], cm[4], cl[4];
+        if (x == 0) check_planes();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) split_pair(rg[4 * j + x], rg[4 * j + 2 + x], ch[j], cm[j], cl[j]);
+        char* d = vpl + (32 * hw + 2 * (lane & 15) + x) * kVRowB + 16 * (lane >> 4);
+        *reinterpret_cast<u32x4*>(d) = u32x4{ch[0], ch[1], ch[2], ch[3]};
+        *reinterpret_cast<u32x4*>(d + kVPlane) = u32x4{cm[0], cm[1], cm[2], cm[3]};
+        *reinterpret_cast<u32x4*>(d + 2 * kVPlane) = u32x4{cl[0], cl[1], cl[2], cl[3]};
+    };
+    auto k_frag = [&](int t, int plane) {  // K[key col][16t + 8hh ..]
+        return *reinterpret_cast<const u32x4*>(kpl + col * kKRowB + 16 * hh + 32 * t + plane * kKPlane);
+    };
+    auto v_frag = [&](int x, int plane) {  // step s = x/4, d = 32 (x%4) + col
+        return *reinterpret_cast<const u32x4*>(vpl + (32 * (x & 3) + col) * kVRowB + 32 * (x >> 2) + 16 * hh +
+                                               plane * kVPlane);
+    };
+
+    // the unit's query rows by LDS DMA, once for both groups: wave wu rows 16*wu .. of the unit
+    // (rows past the sequence repeat its last), 512 contiguous bytes each
+    {
+        int f = min(kUnitRows * p.u + (kQB / 2) * wu, p.nflat - 1);
+        const int t0 = fdiv(f, fG);
+        int g = f - t0 * G;
+        uint64_t sb = (uint64_t)(uintptr_t)(a.q + ((size_t)p.row0 + t0) * a.q_stride + (size_t)(kvh * G + g) * D);
+        const uint64_t next = (uint64_t)((a.q_stride - (long)(G - 1) * D) * 4);
+        const uint32_t lb = scalar((int)lds_addr(stage + (kQB / 2) * wu * kRowF));
+        if (hh == 0) {
+#pragma unroll
+            for (int j = 0; j < kQB / 2; ++j) {
+                dma16_s(sb, 16u * col, lb + j * (kRowF * 4));
+                if (f + 1 < p.nflat) {
+                    ++f;
+                    ++g;
+                    sb += g == G ? next : (uint64_t)(D * 4);
+                    if (g == G) g = 0;
+                }
+            }
+        }
+    }
+    if (n_mine > 0) load_k(0);
+    wait_vmcnt<0>();
+    lds_barrier();
+    Planes qp[8];
+    // a score on planes is off by at most 2^-134 (|q| + |k|) per element, 2^-77 with K below kPlaneMax and
+    // q below 2^50; a wave with a q element past that takes its tiles in fp32 after the key loop
+    uint64_t q_fp32;
+    {
+        const float* qs = stage + (hw * kQB + col) * kRowF + 8 * hh;
+        float most = 0.f;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+            float4 x = *reinterpret_cast<const float4*>(qs + 16 * t);
+            float4 y = *reinterpret_cast<const float4*>(qs + 16 * t + 4);
+            x.x *= sl2, x.y *= sl2, x.z *= sl2, x.w *= sl2, y.x *= sl2, y.y *= sl2, y.z *= sl2, y.w *= sl2;
+#pragma unroll
+            for (const float f : {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w}) most = fmaxf(most, __builtin_fabsf(f));
+            uint32_t h[4], m[4], l[4];
+            split_pair(x.x, x.y, h[0], m[0], l[0]);
+            split_pair(x.z, x.w, h[1], m[1], l[1]);
+            split_pair(y.x, y.y, h[2], m[2], l[2]);
+            split_pair(y.z, y.w, h[3], m[3], l[3]);
+            qp[t] = {u32x4{h[0], h[1], h[2], h[3]}, u32x4{m[0], m[1], m[2], m[3]}, u32x4{l[0], l[1], l[2], l[3]}};
+        }
+        q_fp32 = __builtin_amdgcn_ballot_w64(!(most < 0x1p50f));
+    }
+    if (n_mine > 0) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) conv_k(x);
+        load_v(0);
+    }
+    Sums x;
+    x.clear();
+    lds_barrier();  // every wave has its q (the staging area is free for the V planes); K planes stored
+    if (grp == 1) lds_barrier();
+    for (int i = 0; i < n_it; ++i) {
+        floatx16 s;
+        if (i < n_mine) {
+            // S^T = K . Q^T, while V(i) goes to its planes; then K(i+1) is fetched
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = 0.f;
+            Planes kf;
+            kf.l = k_frag(0, 2), kf.m = k_frag(0, 1), kf.h = k_frag(0, 0);
+#pragma unroll
+            for (int t = 0; t < 8; ++t) {
+                if (t == 4 || t == 6) conv_v(t == 6);
+                mfma_split(kf, qp[t], s, [&](int pl) { return t < 7 ? k_frag(t + 1, pl) : u32x4{}; });
+            }
+            if (i + 1 < n_mine) load_k(i + 1);
+        }
+        lds_barrier();
+        if (i < n_mine) {
+            __builtin_amdgcn_s_setprio(1);
+            softmax_tile(x, s, index(i), nfull, qpos, hh);
+            // O^T += V^T . P^T, while K(i+1) goes to its planes; then V(i+1) is fetched
+            const bool more = i + 1 < n_mine;
+            Planes vf, pp;
+            vf.l = v_frag(0, 2), vf.m = v_frag(0, 1), vf.h = v_frag(0, 0);
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+                if ((y & 3) == 0) pp = split_p(s, y >> 2);
+                if (y == 4 || y == 6) conv_k(y == 6);
+                mfma_split(vf, pp, x.o[y & 3], [&](int pl) { return y < 7 ? v_frag(y + 1, pl) : u32x4{}; });
+            }
+            if (more) load_v(i + 1);
+            __builtin_amdgcn_s_setprio(0);
+        }
+        lds_barrier();
+    }
+    if (grp == 0) lds_barrier();
+
+    if (live && (q_fp32 || planes_failed<false>(x, n_mine, v_tile, row_bytes, lane))) {
+        const int f = min(f0 + col, p.nflat - 1), t0 = fdiv(f, fG);
+        const float* q_row = a.q + ((size_t)p.row0 + t0) * a.q_stride + (size_t)(kvh * G + f - t0 * G) * D;
+        redo_fp32<false>(x, a, p, q_row, sl2, n_mine, k_tile, v_tile, index, nfull, qpos, row_bytes,
+                         smem + w * (kXchF * 64), lane);
+    }
+
+    // ---- the key groups meet through LDS (tile buffers are free after the barrier): group g finishes
+    // output blocks db = 2g, 2g+1 and hands the other two to its partner
+    float* xw = smem + w * (kXchF * 64) + lane;
+    xw[0] = x.m;
+    xw[64] = x.l;
+    // (grp is wave-uniform: selects, not a dynamic register index)
+    const floatx16 give0 = grp ? x.o[0] : x.o[2], give1 = grp ? x.o[1] : x.o[3];
+    const floatx16 keep0 = grp ? x.o[2] : x.o[0], keep1 = grp ? x.o[3] : x.o[1];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        xw[(2 + i) * 64] = give0[i];
+        xw[(18 + i) * 64] = give1[i];
+    }
+    lds_barrier();
+    const float* xp = smem + ((1 - grp) * kSlots + hw) * (kXchF * 64) + lane;
+    const float mp = xp[0], lp = xp[64];
+    const float mt = fmaxf(x.m, mp);  // -inf only when the pass holds no visible key for the row
+    const float c0 = x.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x.m - mt);
+    const float cp = mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mp - mt);
+    const float l = half_sum(x.l * c0 + lp * cp);
+    {
+        // finished rows (normalised; a row that sees no key: zeros), or the part's, to the staging area
+        const float inv = p.part ? 1.f : qpos < 0 ? 0.f : 1.f / l;
+        float* ost = stage + (hw * kQB + col) * kRowF + 64 * grp + 4 * hh;
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            // O^T registers r .. r+3 of block db are d = 32 db + 8(r/4) + 4hh + 0 .. 3
+            float v0[4], v1[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                v0[j] = (keep0[r + j] * c0 + xp[(2 + r + j) * 64] * cp) * inv;
+                v1[j] = (keep1[r + j] * c0 + xp[(18 + r + j) * 64] * cp) * inv;
+            }
+            *reinterpret_cast<float4*>(ost + 2 * r) = make_float4(v0[0], v0[1], v0[2], v0[3]);
+            *reinterpret_cast<float4*>(ost + 32 + 2 * r) = make_float4(v1[0], v1[1], v1[2], v1[3]);
+        }
+        if (p.part && hh == 0 && grp == 0)
+            *reinterpret_cast<float2*>(p.part + kUnitRows * D + 2 * (hw * kQB + col)) = make_float2(mt, l);
+    }
+    lds_barrier();
+    {
+        const int ln = unhoisted(lane), c4 = 4 * (ln & 31);
+#pragma unroll
+        for (int j = 0; j < kQB / 4; ++j) {  // wave wu: rows 16*wu .. of the unit, two per instruction
+            const int jj = (kQB / 2) * wu + 2 * j + (ln >> 5), f = kUnitRows * p.u + jj;
+            const float4 v = *reinterpret_cast<const float4*>(stage + jj * kRowF + c4);
+            const int t0 = fdiv(f, fG);
+            float* dst = p.part ? p.part + jj * D : a.out + (((size_t)p.row0 + t0) * a.H + kvh * G + f - t0 * G) * D;
+            if (f < p.nflat) *reinterpret_cast<float4*>(dst + c4) = v;
+        }
+    }
+}
+
+// ---- a unit of few rows
+template <bool kPaged>
+__device__ __forceinline__ void few_pass(const PackedArgs& a, const Pass& p, int kvh, FastDiv fG, float sl2,
+                                         float* smem) {
+    constexpr int D = kHeadDim;
+    const int tid = unhoisted(threadIdx.x), lane = tid & 63, w = tid >> 6, wu = scalar(w);
+    const int col = lane & 31, hh = lane >> 5;
+    const int G = (int)fG.d;
+    const uint32_t row_bytes = (uint32_t)(a.kv_stride * 4);
+    char* const qpl = reinterpret_cast<char*>(smem);
+    const int f0 = kUnitRows * p.u, last = p.nflat - 1;
+    const int qpos = p.pos0 + fdiv(min(f0 + col, last), fG);
+    const int nfull = max(p.pos0 + fdiv(f0, fG) + 1, 0) / kKT;
+    const int n_mine = (p.nrange - wu + kWaves - 1) / kWaves;
+    auto index = [&](int i) { return p.kt_lo + kWaves * i + wu; };
+    auto k_tile = [&](int i) { return tile_rsrc<kPaged>(a, p, a.k + (size_t)kvh * D, index(i) * kKT); };
+    auto v_tile = [&](int i) { return tile_rsrc<kPaged>(a, p, a.v + (size_t)kvh * D, index(i) * kKT); };
+    // K: lane's key col, d = 16t + 8hh .. + 7 (t of the four of half y), as the operand wants it
+    u32x4 kr[2][8];
+    const uint32_t voff_k = (uint32_t)col * row_bytes + 32u * hh;
+    auto load_k = [&](const Rsrc& rs, int y) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            kr[y][j] = __builtin_amdgcn_raw_buffer_load_b128(rs, voff_k + 256 * y + 64 * (j >> 1) + 16 * (j & 1), 0, 0);
+    };
+    // V: d = 4 col .. + 3, one in each column quarter; step y holds the keys 16y + 4hh + {0..3, 8..11}
+    u32x4 vr[2][8];
+    const uint32_t voff_v = (uint32_t)(4 * hh) * row_bytes + 16u * col;
+    auto load_v = [&](const Rsrc& rs, int y) {
+        const uint32_t off = unhoisted(voff_v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            vr[y][j] = __builtin_amdgcn_raw_buffer_load_b128(
+                rs, off + (uint32_t)(16 * y + 8 * (j >> 2) + (j & 3)) * row_bytes, 0, 0);
+    };
+    if (n_mine > 0) {
+        const Rsrc rk = k_tile(0), rv = v_tile(0);
+        load_k(rk, 0);
+        load_k(rk, 1);
+        load_v(rv, 0);
+        load_v(rv, 1);
+    }
+    // q's planes, 8 values per thread: rows past the last repeat it
+    int q_fp32;
+    {
+        const int row = tid >> 4, d = 8 * (tid & 15), f = min(f0 + row, last), t0 = fdiv(f, fG);
+        const float* src = a.q + ((size_t)p.row0 + t0) * a.q_stride + (size_t)(kvh * G + f - t0 * G) * D + d;
+        float v[8];
+        *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
+        *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(src + 4);
+        float most = 0.f;
+        uint32_t h[4], m[4], l[4];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            v[j] *= sl2;
+            most = fmaxf(most, __builtin_fabsf(v[j]));
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) split_pair(v[2 * j], v[2 * j + 1], h[j], m[j], l[j]);
+        char* dst = qpl + row * kKRowB + 2 * d;
+        *reinterpret_cast<u32x4*>(dst) = u32x4{h[0], h[1], h[2], h[3]};
+        *reinterpret_cast<u32x4*>(dst + kKPlane) = u32x4{m[0], m[1], m[2], m[3]};
+        *reinterpret_cast<u32x4*>(dst + 2 * kKPlane) = u32x4{l[0], l[1], l[2], l[3]};
+        q_fp32 = __syncthreads_or(!(most < 0x1p50f));  // (see wide_pass)
+    }
+    auto q_frag = [&](int t) {
+        const char* q = qpl + col * kKRowB + 16 * hh + 32 * t;
+        return Planes{*reinterpret_cast<const u32x4*>(q), *reinterpret_cast<const u32x4*>(q + kKPlane),
+                      *reinterpret_cast<const u32x4*>(q + 2 * kKPlane)};
+    };
+    auto mul = [&](const Planes& x, const Planes& y, floatx16& c) {
+        c = mfma_bf16(x.l, y.h, c);
+        c = mfma_bf16(x.m, y.m, c);
+        c = mfma_bf16(x.m, y.h, c);
+        c = mfma_bf16(x.h, y.l, c);
+        c = mfma_bf16(x.h, y.m, c);
+        c = mfma_bf16(x.h, y.h, c);
+    };
+    // eight values' planes; one past kPlaneMax turns into NaN, which reaches a sum
+    auto planes_of = [&](const float (&v)[8]) {
+        uint32_t h[4], m[4], l[4];
+        float most = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = fmaxf(most, __builtin_fabsf(v[j]));
+        const float v0 = most < kPlaneMax ? v[0] : __uint_as_float(0xFFFFFFFFu);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) split_pair(j ? v[2 * j] : v0, v[2 * j + 1], h[j], m[j], l[j]);
+        return Planes{u32x4{h[0], h[1], h[2], h[3]}, u32x4{m[0], m[1], m[2], m[3]}, u32x4{l[0], l[1], l[2], l[3]}};
+    };
+    Sums x;
+    x.clear();
+    for (int i = 0; i < n_mine; ++i) {
+        const bool more = i + 1 < n_mine;
+        const Rsrc rk = k_tile(more ? i + 1 : i), rv = v_tile(more ? i + 1 : i);
+        floatx16 s;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(kr[t >> 2][2 * (t & 3) + (j >> 2)][j & 3]);
+            mul(planes_of(v), q_frag(t), s);
+            if (more && (t == 3 || t == 7)) load_k(rk, t >> 2);
+        }
+        softmax_tile(x, s, index(i), nfull, qpos, hh);
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            const Planes pp = split_p(s, y);
+#pragma unroll
+            for (int db = 0; db < 4; ++db) {
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(vr[y][j][db]);
+                mul(planes_of(v), pp, x.o[db]);
+            }
+            if (more) load_v(rv, y);
+        }
+    }
+    lds_barrier();  // q's planes have been read
+    float* const mine = smem + wu * (kQB * kRowF);
+    if (q_fp32 || planes_failed<true>(x, n_mine, v_tile, row_bytes, lane)) {
+        const int f = min(f0 + col, last), t0 = fdiv(f, fG);
+        const float* q_row = a.q + ((size_t)p.row0 + t0) * a.q_stride + (size_t)(kvh * G + f - t0 * G) * D;
+        redo_fp32<true>(x, a, p, q_row, sl2, n_mine, k_tile, v_tile, index, nfull, qpos, row_bytes, mine, lane);
+    }
+    // every wave's rows meet: O^T register r of quarter db is d = 4 (8(r/4) + 4hh + r%4) + db
+#pragma unroll
+    for (int r = 0; r < 16; ++r)
+        *reinterpret_cast<float4*>(mine + col * kRowF + 4 * (8 * (r >> 2) + 4 * hh + (r & 3))) =
+            make_float4(x.o[0][r], x.o[1][r], x.o[2][r], x.o[3][r]);
+    const float l_row = half_sum(x.l);
+    if (hh == 0) *reinterpret_cast<float2*>(smem + kFewML + 2 * (wu * kQB + col)) = make_float2(x.m, l_row);
+    lds_barrier();
+    // two rows per wave and round, a lane four columns
+    const int rows = min(kQB, p.nflat - f0), d = 4 * col;
+    for (int row = 2 * wu + hh; row < rows; row += 2 * kWaves) {
+        float M = -INFINITY, L = 0.f, c[kWaves];
+        float2 ml[kWaves];
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) {
+            ml[i] = *reinterpret_cast<const float2*>(smem + kFewML + 2 * (i * kQB + row));
+            M = fmaxf(M, ml[i].x);
+        }
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) {
+            c[i] = ml[i].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[i].x - M);
+            // (a wave whose every score is NaN keeps m at -inf, and its NaN sum counts)
+            L += ml[i].x == -INFINITY ? ml[i].y : ml[i].y * c[i];
+            const float4 v = *reinterpret_cast<const float4*>(smem + (i * kQB + row) * kRowF + d);
+            o.x = __builtin_fmaf(c[i], v.x, o.x), o.y = __builtin_fmaf(c[i], v.y, o.y);
+            o.z = __builtin_fmaf(c[i], v.z, o.z), o.w = __builtin_fmaf(c[i], v.w, o.w);
+        }
+        const int f = f0 + row, t0 = fdiv(f, fG);
+        float* dst;
+        if (p.part) {
+            dst = p.part + row * D;
+            if (col == 0) *reinterpret_cast<float2*>(p.part + kFewRows * D + 2 * row) = make_float2(M, L);
+        } else {
+            dst = a.out + (((size_t)p.row0 + t0) * a.H + kvh * G + f - t0 * G) * D;
+            const float inv = p.pos0 + t0 < 0 ? 0.f : 1.f / L;  // a row that sees no key: zeros
+            o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
+        }
+        *reinterpret_cast<float4*>(dst + d) = o;
+    }
+}
+
+// Workgroup (share, KV head) walks its part of the wide list, or of the few-row one.
+template <bool kPaged, bool kFew>
+__device__ __forceinline__ void walk_list(const PackedArgs& a, int shares, float* parts, float* smem) {
+    const int kvh = blockIdx.x % a.HKV, share = blockIdx.x / a.HKV;  // a KV head's workgroups share an XCD's L2
+    const FastDiv fG = fast_div((uint32_t)(a.H / a.HKV));
+    const float sl2 = a.scale * 1.44269504088896340736f;  // scores come out in log2 units
+    const PlanView pv = plan_view(const_cast<char*>(a.plan), a.n_seq, a.rows, (int)fG.d, shares);
+    const List list = kFew ? pv.few : pv.wide;
     const int* head = reinterpret_cast<const int*>(a.plan);
-    const int rounds = scalar(head[6]), dealt = scalar(head[7]);
-    const int first = scalar(pv.cuts[share].x), first_tile = scalar(pv.cuts[share].y);
-    const int last = scalar(pv.cuts[share + 1].x), last_tile = scalar(pv.cuts[share + 1].y);
-
+    const int rounds = kFew ? 0 : scalar(head[kHeadRounds]), dealt = kFew ? 0 : scalar(head[kHeadDealt]);
+    const int2 from = list.cuts[share], to = list.cuts[share + 1];
+    if (!plan_fits(a.plan, a.n_seq, a.rows, a.H, a.HKV, !kPaged)) return;
+    const int first = scalar(from.x), first_tile = scalar(from.y), last = scalar(to.x), last_tile = scalar(to.y);
     for (int pass = 0;; ++pass) {
-        // the pass's unit, its tiles [kt_lo, kt_lo + nrange), and where its part goes (-1: whole)
-        int at, kt_lo = 0, cut = -1;
+        int at, cut = -1;
+        Pass p;
+        p.kt_lo = 0;
         if (pass < rounds) {
             at = pass * shares + ((pass & 1) ? shares - 1 - share : share);
         } else {
@@ -303,471 +991,56 @@ __global__ __launch_bounds__(64 * kSlots * kGroups) void k_packed_attn(PackedArg
             if (i > last || (i == last && last_tile == 0)) break;
             at = dealt + i;
             cut = i == last ? last_tile : -1;
-            kt_lo = i == first ? first_tile : 0;
+            p.kt_lo = i == first ? first_tile : 0;
         }
-        const int s = scalar(pv.units[at].x), u = scalar(pv.units[at].y), tiles = scalar(pv.units[at].z);
-        const int nrange = (cut >= 0 ? cut : tiles) - kt_lo;
-        const bool part = kt_lo > 0 || cut >= 0;
-        const int row0 = scalar(pv.seq[s].x), n = scalar(pv.seq[s].y), len = scalar(pv.seq[s].z);
-        const int pos0 = len - n;                 // position of the sequence's first new row (may be negative)
-        const int nflat = n * G;                  // its flat rows of this KV head
-        const int f0 = kUnitRows * u + kQB * hw;  // this wave's first
-        const bool live = f0 < nflat;
-        const int tok = fdiv(min(f0 + col, nflat - 1), fG);
-        const int qpos = pos0 + tok;              // this lane's query
-        const int T = min(max(pos0 + fdiv(min(kUnitRows * u + kUnitRows, nflat) - 1, fG) + 1, 0), len);  // keys seen
-        const int nfull = max(pos0 + fdiv(min(f0, nflat - 1), fG) + 1, 0) / kKT;  // tiles below the wave's diagonal
-        const int n_it = (nrange + kGroups - 1) / kGroups, n_mine = (nrange - grp + kGroups - 1) / kGroups;
-
-        // K and V of this group's i-th tile (kt_lo + kGroups * i + grp), a quarter per wave:
-        //   K: row 8*hw + lane/8, d = 8c .. 8c+7 and 64 + 8c .. (c = lane%8)
-        //   V: d = 32*hw + 2*(lane%16) and the next, the eight keys of chunk lane/16 (step s = chunk/2,
-        //     half hh = chunk%2 of the P.V operand: keys 16s + 4hh + {0..3, 8..11})
-        float rg[16];
-        // the tile's visible rows as a buffer: reads past the last one give zeros
-        auto tile_rsrc = [&](const float* cache, int t0) {
-            size_t row = (size_t)row0 + t0;
-            int there = min(kKT, T - t0);
-            if constexpr (kPaged) {
-                const int blk = t0 >> a.bshift;
-                const int phys = blk < a.max_blocks ? a.btab[(size_t)s * a.max_blocks + blk] : -1;
-                const bool ok = phys >= 0 && phys < a.n_blocks;
-                row = ok ? ((size_t)phys << a.bshift) | (size_t)(t0 & ((1 << a.bshift) - 1)) : 0;
-                if (!ok) there = 0;
-            }
-            return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(cache) + row * a.kv_stride, 0,
-                                                     there ? (int)((uint32_t)(there - 1) * row_bytes + D * 4) : 0,
-                                                     kBufferDword3);
-        };
-        auto load_k = [&](int i) {
-            const Rsrc rs = tile_rsrc(kbase, (kt_lo + kGroups * i + grp) * kKT);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(rs, voff_k + 256 * (j >> 1) + 16 * (j & 1), 0, 0);
-                rg[4 * j] = __uint_as_float(v.x), rg[4 * j + 1] = __uint_as_float(v.y);
-                rg[4 * j + 2] = __uint_as_float(v.z), rg[4 * j + 3] = __uint_as_float(v.w);
-            }
-        };
-        auto load_v = [&](int i) {
-            const Rsrc rs = tile_rsrc(vbase, (kt_lo + kGroups * i + grp) * kKT);
-            const uint32_t off = unhoisted(voff_v);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const u32x2 v =
-                    __builtin_amdgcn_raw_buffer_load_b64(rs, off + (8 * (j >> 2) + (j & 3)) * row_bytes, 0, 0);
-                rg[2 * j] = __uint_as_float(v.x), rg[2 * j + 1] = __uint_as_float(v.y);
-            }
-        };
-        // a value of rg past kPlaneMax turns one of them into NaN, which reaches a sum of every wave that
-        // multiplies it
-        auto check_planes = [&]() {
-            float most = 0.f;
-#pragma unroll
-            for (int j = 0; j < 16; ++j) most = fmaxf(most, __builtin_fabsf(rg[j]));
-            rg[0] = most < kPlaneMax ? rg[0] : __uint_as_float(0xFFFFFFFFu);
-        };
-        // half x of the conversion of rg: eight values, one 16-byte piece of each plane
-        auto conv_k = [&](int x) {
-            uint32_t ch[4], cm[4], cl[4];
-            if (x == 0) check_planes();
-#pragma unroll
-            for (int j = 0; j < 4; ++j) split_pair(rg[8 * x + 2 * j], rg[8 * x + 2 * j + 1], ch[j], cm[j], cl[j]);
-            char* p = kpl + (8 * hw + (lane >> 3)) * kKRowB + 16 * (lane & 7) + 128 * x;
-            *reinterpret_cast<u32x4*>(p) = u32x4{ch[0], ch[1], ch[2], ch[3]};
-            *reinterpret_cast<u32x4*>(p + kKPlane) = u32x4{cm[0], cm[1], cm[2], cm[3]};
-            *reinterpret_cast<u32x4*>(p + 2 * kKPlane) = u32x4{cl[0], cl[1], cl[2], cl[3]};
-        };
-        auto conv_v = [&](int x) {  // d + x
-            uint32_t ch[4], cm[4], cl[4];
-            if (x == 0) check_planes();
-#pragma unroll
-            for (int j = 0; j < 4; ++j) split_pair(rg[4 * j + x], rg[4 * j + 2 + x], ch[j], cm[j], cl[j]);
-            char* p = vpl + (32 * hw + 2 * (lane & 15) + x) * kVRowB + 16 * (lane >> 4);
-            *reinterpret_cast<u32x4*>(p) = u32x4{ch[0], ch[1], ch[2], ch[3]};
-            *reinterpret_cast<u32x4*>(p + kVPlane) = u32x4{cm[0], cm[1], cm[2], cm[3]};
-            *reinterpret_cast<u32x4*>(p + 2 * kVPlane) = u32x4{cl[0], cl[1], cl[2], cl[3]};
-        };
-        auto k_frag = [&](int t, int plane) {  // K[key col][16t + 8hh ..]
-            return *reinterpret_cast<const u32x4*>(kpl + col * kKRowB + 16 * hh + 32 * t + plane * kKPlane);
-        };
-        auto v_frag = [&](int x, int plane) {  // step s = x/4, d = 32 (x%4) + col
-            return *reinterpret_cast<const u32x4*>(vpl + (32 * (x & 3) + col) * kVRowB + 32 * (x >> 2) + 16 * hh +
-                                                   plane * kVPlane);
-        };
-
-        // the unit's query rows by LDS DMA, once for both groups: wave wu rows 16*wu .. of the unit
-        // (rows past the sequence repeat its last), 512 contiguous bytes each
-        if (pass > 0) lds_barrier();  // every wave has stored its rows from the staging area
-        {
-            int f = min(kUnitRows * u + (kQB / 2) * wu, nflat - 1);
-            const int t0 = fdiv(f, fG);
-            int g = f - t0 * G;
-            uint64_t sb = (uint64_t)(uintptr_t)(a.q + ((size_t)row0 + t0) * a.q_stride + (size_t)(kvh * G + g) * D);
-            const uint64_t next = (uint64_t)((a.q_stride - (long)(G - 1) * D) * 4);
-            const uint32_t lb = scalar((int)lds_addr(stage + (kQB / 2) * wu * kRowF));
-            if (hh == 0) {
-#pragma unroll
-                for (int j = 0; j < kQB / 2; ++j) {
-                    dma16_s(sb, 16u * col, lb + j * (kRowF * 4));
-                    if (f + 1 < nflat) {
-                        ++f;
-                        ++g;
-                        sb += g == G ? next : (uint64_t)(D * 4);
-                        if (g == G) g = 0;
-                    }
-                }
-            }
-        }
-        if (n_mine > 0) load_k(0);
-        wait_vmcnt<0>();
-        lds_barrier();
-        Planes qp[8];
-        // a score on planes is off by at most 2^-134 (|q| + |k|) per element, 2^-77 with K below kPlaneMax and
-        // q below 2^50; a wave with a q element past that takes its tiles in fp32 after the key loop
-        uint64_t q_fp32;
-        {
-            const float* qs = stage + (hw * kQB + col) * kRowF + 8 * hh;
-            float most = 0.f;
-#pragma unroll
-            for (int t = 0; t < 8; ++t) {
-                float4 x = *reinterpret_cast<const float4*>(qs + 16 * t);
-                float4 y = *reinterpret_cast<const float4*>(qs + 16 * t + 4);
-                x.x *= sl2, x.y *= sl2, x.z *= sl2, x.w *= sl2, y.x *= sl2, y.y *= sl2, y.z *= sl2, y.w *= sl2;
-#pragma unroll
-                for (const float f : {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w}) most = fmaxf(most, __builtin_fabsf(f));
-                uint32_t h[4], m[4], l[4];
-                split_pair(x.x, x.y, h[0], m[0], l[0]);
-                split_pair(x.z, x.w, h[1], m[1], l[1]);
-                split_pair(y.x, y.y, h[2], m[2], l[2]);
-                split_pair(y.z, y.w, h[3], m[3], l[3]);
-                qp[t] = {u32x4{h[0], h[1], h[2], h[3]}, u32x4{m[0], m[1], m[2], m[3]}, u32x4{l[0], l[1], l[2], l[3]}};
-            }
-            q_fp32 = __builtin_amdgcn_ballot_w64(!(most < 0x1p50f));
-        }
-        if (n_mine > 0) {
-#pragma unroll
-            for (int x = 0; x < 2; ++x) conv_k(x);
-            load_v(0);
-        }
-        floatx16 o[4];
-        float m, lsum;
-        auto clear = [&]() {
-#pragma unroll
-            for (int db = 0; db < 4; ++db)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) o[db][i] = 0.f;
-            m = -INFINITY;
-            lsum = 0.f;
-        };
-        // scores s of tile kt -> P (in place), the running maximum and sum, O rescaled if it rose
-        auto softmax = [&](int kt, floatx16& s) {
-            if (kt >= nfull) {  // tile crosses the diagonal (wave-uniform)
-                const int k0 = unhoisted(kt * kKT + 4 * hh);
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if (k0 + 8 * (r >> 2) + (r & 3) > qpos) s[r] = -INFINITY;
-            }
-            float mx = s[0];
-#pragma unroll
-            for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-            const float ms = half_max(mx);
-            if (__builtin_amdgcn_ballot_w64(ms > m + kLazy)) {  // rare after the first tile
-                const float mn = fmaxf(m, ms);
-                const float corr = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-                lsum *= corr;
-#pragma unroll
-                for (int db = 0; db < 4; ++db)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) o[db][r] *= corr;
-                m = mn;
-            }
-            const float nb_ = m == -INFINITY ? 0.f : -m;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[r] = __builtin_amdgcn_exp2f(s[r] + nb_);
-                lsum += s[r];
-            }
-        };
-        // The two products in fp32 from the cache, for a wave that planes do not serve: see after the key
-        // loop.  q comes from its row again; values 16t + 8hh .. + 7 take the registers of planes h and m.
-        auto q_whole = [&]() {
-            const int ln = unhoisted(lane), f = min(f0 + (ln & 31), nflat - 1), t0 = fdiv(f, fG);
-            const float* row =
-                a.q + ((size_t)row0 + t0) * a.q_stride + (size_t)(kvh * G + f - t0 * G) * D + 8 * (ln >> 5);
-#pragma unroll
-            for (int t = 0; t < 8; ++t) {
-                qp[t].h = *reinterpret_cast<const u32x4*>(row + 16 * t);
-                qp[t].m = *reinterpret_cast<const u32x4*>(row + 16 * t + 4);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    qp[t].h[j] = __float_as_uint(__uint_as_float(qp[t].h[j]) * sl2);
-                    qp[t].m[j] = __float_as_uint(__uint_as_float(qp[t].m[j]) * sl2);
-                }
-            }
-        };
-        auto qk_fp32 = [&](int i, floatx16& s) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = 0.f;
-            const Rsrc rs = tile_rsrc(kbase, (kt_lo + kGroups * i + grp) * kKT);
-            const int ln = unhoisted(lane);
-            const uint32_t off = (ln & 31) * row_bytes + 32u * (ln >> 5);
-#pragma unroll
-            for (int t = 0; t < 8; ++t) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {  // d = 16t + 8hh + 2j and the next
-                    const u32x2 v = __builtin_amdgcn_raw_buffer_load_b64(rs, off + 64 * t + 8 * j, 0, 0);
-                    const u32x4 qv = j < 2 ? qp[t].h : qp[t].m;
-                    const float q0 = __uint_as_float(qv[2 * (j & 1)]), q1 = __uint_as_float(qv[2 * (j & 1) + 1]);
-                    s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(v.x), q0, s, 0, 0, 0);
-                    s = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(v.y), q1, s, 0, 0, 0);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        };
-        auto pv_fp32 = [&](int i, const floatx16& p) {
-            const Rsrc rs = tile_rsrc(vbase, (kt_lo + kGroups * i + grp) * kKT);
-            const uint32_t off = unhoisted(4 * hh) * row_bytes + 4u * col;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {  // lane half hh: key 8(r/4) + 4hh + r%4
-#pragma unroll
-                for (int db = 0; db < 4; ++db) {
-                    const float v = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
-                        rs, off + (8 * (r >> 2) + (r & 3)) * row_bytes + 128 * db, 0, 0));
-                    o[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, p[r], o[db], 0, 0, 0);
-                }
-                __builtin_amdgcn_sched_barrier(0);
-            }
-        };
-        // The same for a tile that crosses the diagonal, key after key: a value that a row does not see
-        // must not be multiplied at all (0 times infinity), and the matrix instruction takes every row
-        // with every key.  P passes through the wave's own part of the exchange area, [key][row].
-        auto pv_seen = [&](int i, const floatx16& p) {
-            const int t0 = (kt_lo + kGroups * i + grp) * kKT;
-            const Rsrc rs = tile_rsrc(vbase, t0);
-            const int ln = unhoisted(lane);
-            float* pw = smem + w * (kXchF * 64) + (ln & 31);
-#pragma unroll
-            for (int r = 0; r < 16; ++r) pw[32 * (8 * (r >> 2) + 4 * (ln >> 5) + (r & 3))] = p[r];
-            __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-            for (int key = 0; key < kKT; ++key) {
-                const float pk = pw[32 * key];
-                const uint32_t off = key * row_bytes + 16u * (ln >> 5);
-                if (t0 + key <= qpos) {
-#pragma unroll
-                    for (int db = 0; db < 4; ++db) {
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {  // d = 32 db + 8x + 4hh + 0 .. 3
-                            const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(rs, off + 128 * db + 32 * x, 0, 0);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e)
-                                o[db][4 * x + e] = __builtin_fmaf(pk, __uint_as_float(v[e]), o[db][4 * x + e]);
-                        }
-                        __builtin_amdgcn_sched_barrier(0);
-                    }
-                }
-            }
-            __builtin_amdgcn_wave_barrier();
-        };
-
-        clear();
-        lds_barrier();  // every wave has its q (the staging area is free for the V planes); K planes stored
-        if (grp == 1) lds_barrier();
-        for (int i = 0; i < n_it; ++i) {
-            floatx16 s;
-            if (i < n_mine) {
-                // S^T = K . Q^T, while V(i) goes to its planes; then K(i+1) is fetched
-                if (live) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) s[r] = 0.f;
-                    Planes kf;
-                    kf.l = k_frag(0, 2), kf.m = k_frag(0, 1), kf.h = k_frag(0, 0);
-#pragma unroll
-                    for (int t = 0; t < 8; ++t) {
-                        if (t == 4 || t == 6) conv_v(t == 6);
-                        mfma_split(kf, qp[t], s, [&](int p) { return t < 7 ? k_frag(t + 1, p) : u32x4{}; });
-                    }
-                } else {
-                    conv_v(0);
-                    conv_v(1);
-                }
-                if (i + 1 < n_mine) load_k(i + 1);
-            }
-            lds_barrier();
-            if (i < n_mine) {
-                const bool more = i + 1 < n_mine;
-                if (live) {
-                    __builtin_amdgcn_s_setprio(1);
-                    softmax(kt_lo + kGroups * i + grp, s);
-                    // O^T += V^T . P^T, while K(i+1) goes to its planes; then V(i+1) is fetched
-                    Planes vf, pp;
-                    vf.l = v_frag(0, 2), vf.m = v_frag(0, 1), vf.h = v_frag(0, 0);
-#pragma unroll
-                    for (int x = 0; x < 8; ++x) {
-                        if ((x & 3) == 0) {
-                            uint32_t ph[4], pm[4], pl[4];
-#pragma unroll
-                            for (int j = 0; j < 4; ++j)
-                                split_pair(s[2 * x + 2 * j], s[2 * x + 2 * j + 1], ph[j], pm[j], pl[j]);
-                            pp = {u32x4{ph[0], ph[1], ph[2], ph[3]}, u32x4{pm[0], pm[1], pm[2], pm[3]},
-                                  u32x4{pl[0], pl[1], pl[2], pl[3]}};
-                        }
-                        if (x == 4 || x == 6) conv_k(x == 6);
-                        mfma_split(vf, pp, o[x & 3], [&](int p) { return x < 7 ? v_frag(x + 1, p) : u32x4{}; });
-                    }
-                } else {
-                    conv_k(0);
-                    conv_k(1);
-                }
-                if (more) load_v(i + 1);
-                __builtin_amdgcn_s_setprio(0);
-            }
-            lds_barrier();
-        }
-        if (grp == 0) lds_barrier();
-
-        // Which sums planes do not serve (prefill.hip has the same rule): an infinite value, or one past
-        // kPlaneMax, in K or V shows as a sum that is not finite.  A V value or a weight below kPlaneMin
-        // may have lost bits of its third plane, 2^-134, which shows in no sum from kSmallSum up; a smaller
-        // one has the wave look through its V tiles, in the blocks of 32 columns with such a sum: it stands
-        // if no V value there is below kPlaneMin and the largest one is too small for the weights' 2^-134
-        // to show in it.  Otherwise, and for a q past its limit, the wave takes its tiles again in fp32.
-        if (live) {
-            float z = lsum * 0.f, least[4];  // per block of 32 columns
-#pragma unroll
-            for (int db = 0; db < 4; ++db) {
-                least[db] = INFINITY;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    z = __builtin_fmaf(o[db][r], 0.f, z);
-                    least[db] = fminf(least[db], __builtin_fabsf(o[db][r]));
-                }
-            }
-            const float least_all = fminf(fminf(least[0], least[1]), fminf(least[2], least[3]));
-            uint64_t redo = q_fp32 | __builtin_amdgcn_ballot_w64(z != 0.f);
-            // (a lane without a visible key has no sum: m stays -inf)
-            if (!redo && __builtin_amdgcn_ballot_w64(least_all < kSmallSum && m != -INFINITY)) {
-                uint32_t small = 0xFFFFFFFFu, tiny = 0xFFFFFFFFu;  // the smallest nonzero sum and V value
-                if (m != -INFINITY) {
-#pragma unroll
-                    for (int db = 0; db < 4; ++db)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r) small = min(small, magnitude(__float_as_uint(o[db][r])));
-                }
-                float most = 0.f;
-#pragma unroll
-                for (int db = 0; db < 4; ++db) {
-                    if (!__builtin_amdgcn_ballot_w64(least[db] < kSmallSum && m != -INFINITY)) continue;
-                    for (int i = 0; i < n_mine; ++i) {
-                        const Rsrc rs = tile_rsrc(vbase, (kt_lo + kGroups * i + grp) * kKT);
-                        const int ln = unhoisted(lane);
-                        const uint32_t off = (ln >> 3) * row_bytes + 16u * (ln & 7) + 128u * db;
-#pragma unroll
-                        for (int j = 0; j < kKT / 8; ++j) {
-                            const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(rs, off + 8 * j * row_bytes, 0, 0);
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                tiny = min(tiny, magnitude(v[e]));
-                                most = fmaxf(most, __builtin_fabsf(__uint_as_float(v[e])));
-                            }
-                        }
-                    }
-                }
-                // the sums are off by up to 2^20 2^-134 most; a lane without a nonzero one has nothing to lose
-                const float limit = wave_max(most) * 0x1p-84f;
-                redo = __builtin_amdgcn_ballot_w64(tiny < kTinyMagnitude || limit > of_magnitude(small));
-            }
-            if (redo) {
-                clear();
-                q_whole();
-                for (int i = 0; i < n_mine; ++i) {
-                    floatx16 s;
-                    const int kt = kt_lo + kGroups * i + grp;
-                    qk_fp32(i, s);
-                    softmax(kt, s);
-                    if (kt >= nfull) pv_seen(i, s);
-                    else pv_fp32(i, s);
-                }
-            }
-        }
-
-        // ---- the key groups meet through LDS (tile buffers are free after the barrier): group g finishes
-        // output blocks db = 2g, 2g+1 and hands the other two to its partner
-        float* xw = smem + w * (kXchF * 64) + lane;
-        xw[0] = m;
-        xw[64] = lsum;
-        // (grp is wave-uniform: selects, not a dynamic register index)
-        const floatx16 give0 = grp ? o[0] : o[2], give1 = grp ? o[1] : o[3];
-        const floatx16 keep0 = grp ? o[2] : o[0], keep1 = grp ? o[3] : o[1];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            xw[(2 + i) * 64] = give0[i];
-            xw[(18 + i) * 64] = give1[i];
-        }
-        lds_barrier();
-        const float* xp = smem + ((1 - grp) * kSlots + hw) * (kXchF * 64) + lane;
-        const float mp = xp[0], lp = xp[64];
-        const float mt = fmaxf(m, mp);  // -inf only when the pass holds no visible key for the row
-        const float c0 = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mt);
-        const float cp = mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mp - mt);
-        const float l = half_sum(lsum * c0 + lp * cp);
-        float* dst_part = parts + (size_t)(2 * blockIdx.x + (kt_lo > 0 ? 0 : 1)) * kPartFloats;
-        {
-            // finished rows (normalised; a row that sees no key: zeros), or the part's, to the staging area
-            const float inv = part ? 1.f : qpos < 0 ? 0.f : 1.f / l;
-            float* ost = stage + (hw * kQB + col) * kRowF + 64 * grp + 4 * hh;
-#pragma unroll
-            for (int r = 0; r < 16; r += 4) {
-                // O^T registers r .. r+3 of block db are d = 32 db + 8(r/4) + 4hh + 0 .. 3
-                float v0[4], v1[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    v0[j] = (keep0[r + j] * c0 + xp[(2 + r + j) * 64] * cp) * inv;
-                    v1[j] = (keep1[r + j] * c0 + xp[(18 + r + j) * 64] * cp) * inv;
-                }
-                *reinterpret_cast<float4*>(ost + 2 * r) = make_float4(v0[0], v0[1], v0[2], v0[3]);
-                *reinterpret_cast<float4*>(ost + 32 + 2 * r) = make_float4(v1[0], v1[1], v1[2], v1[3]);
-            }
-            if (part && hh == 0 && grp == 0)
-                *reinterpret_cast<float2*>(dst_part + kUnitRows * D + 2 * (hw * kQB + col)) = make_float2(mt, l);
-        }
-        lds_barrier();
-        {
-            const int ln = unhoisted(lane), c4 = 4 * (ln & 31);
-#pragma unroll
-            for (int j = 0; j < kQB / 4; ++j) {  // wave wu: rows 16*wu .. of the unit, two per instruction
-                const int jj = (kQB / 2) * wu + 2 * j + (ln >> 5), f = kUnitRows * u + jj;
-                const float4 v = *reinterpret_cast<const float4*>(stage + jj * kRowF + c4);
-                const int t0 = fdiv(f, fG);
-                float* dst = part ? dst_part + jj * D
-                                  : a.out + (((size_t)row0 + t0) * H + kvh * G + f - t0 * G) * D;
-                if (f < nflat) *reinterpret_cast<float4*>(dst + c4) = v;
-            }
-        }
+        const Unit x = list.units[at];
+        const int n = scalar(x.n), len = scalar(x.len);
+        p.seq = scalar(x.seq), p.u = scalar(x.u), p.row0 = scalar(x.row0);
+        p.pos0 = len - n;
+        p.nflat = n * (int)fG.d;
+        p.T = min(max(p.pos0 + fdiv(min(kUnitRows * p.u + kUnitRows, p.nflat) - 1, fG) + 1, 0), len);
+        p.nrange = (cut >= 0 ? cut : scalar(x.tiles)) - p.kt_lo;
+        p.part = p.kt_lo > 0 || cut >= 0 ? parts + part_at(kFew, blockIdx.x, p.kt_lo > 0 ? 0 : 1) : nullptr;
+        if (pass > 0) lds_barrier();  // the last pass's rows have been read
+        if constexpr (kFew) few_pass<kPaged>(a, p, kvh, fG, sl2, smem);
+        else wide_pass<kPaged>(a, p, kvh, fG, sl2, smem);
     }
 }
+template <bool kPaged>
+__global__ __launch_bounds__(64 * kWaves) void k_packed_wide(PackedArgs a, int shares, float* __restrict__ parts) {
+    extern __shared__ __align__(16) float smem[];
+    walk_list<kPaged, false>(a, shares, parts, smem);
+}
+template <bool kPaged>
+__global__ __launch_bounds__(64 * kWaves) void k_packed_few(PackedArgs a, int shares, float* __restrict__ parts) {
+    extern __shared__ __align__(16) float smem[];
+    walk_list<kPaged, true>(a, shares, parts, smem);
+}
 
-// The units that the plan's cuts divide: workgroup (share, KV head; 8 rows) merges the unit that starts in
+// The units that the cuts divide: workgroup (share, KV head; 8 rows) merges the unit that starts in
 // this share and goes on in the next ones.  Part p of it is the share's own (its slot 1), then slot 0 of
 // each share that it reaches.  o = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p over the parts that saw a
 // key (m = -inf and l = 0 otherwise; m = -inf with a NaN l counts).
+constexpr int kCombineRows = 8;
+constexpr int kCombineWide = kUnitRows / kCombineRows, kCombineFew = kFewRows / kCombineRows;
 __global__ __launch_bounds__(256) void k_packed_combine(PackedArgs a, bool prompts, int shares,
-                                                        const float* __restrict__ parts) {
-    if (!plan_fits(a.plan, a.n_seq, a.rows, a.H, a.HKV, prompts)) return;
+                                                        const float* __restrict__ wide_parts,
+                                                        const float* __restrict__ few_parts) {
     const int kvh = blockIdx.x % a.HKV, share = blockIdx.x / a.HKV, G = a.H / a.HKV;
-    const PlanView pv = plan_view(const_cast<char*>(a.plan), a.n_seq, a.rows, G);
-    const int dealt = reinterpret_cast<const int*>(a.plan)[7];
-    const int2 from = pv.cuts[share], to = pv.cuts[share + 1];
+    const bool few = blockIdx.y >= kCombineWide;
+    const PlanView pv = plan_view(const_cast<char*>(a.plan), a.n_seq, a.rows, G, shares);
+    const List list = few ? pv.few : pv.wide;
+    const int dealt = few ? 0 : reinterpret_cast<const int*>(a.plan)[kHeadDealt];
+    const int2 from = list.cuts[share], to = list.cuts[share + 1];
+    if (!plan_fits(a.plan, a.n_seq, a.rows, a.H, a.HKV, prompts)) return;
     if (to.y == 0 || (from.x == to.x && from.y > 0)) return;  // ends between units, or goes on with a unit
-    const int4 x = pv.units[dealt + to.x], e = pv.seq[x.x];
-    const int row = blockIdx.y * 8 + (threadIdx.x >> 5), f = kUnitRows * x.y + row, d = 4 * (threadIdx.x & 31);
-    if (f >= e.y * G) return;
+    const Unit x = list.units[dealt + to.x];
+    const int row = (few ? blockIdx.y - kCombineWide : blockIdx.y) * kCombineRows + (threadIdx.x >> 5);
+    const int f = kUnitRows * x.u + row, d = 4 * (threadIdx.x & 31);
+    if (f >= x.n * G) return;
     const int t0 = f / G;
     int end = share + 1;  // the last share with a part
-    while (pv.cuts[end + 1].x == to.x && pv.cuts[end + 1].y > 0) ++end;
-    auto slot = [&](int p) {
-        return parts + (size_t)(2 * (p * a.HKV + kvh) + (p == share ? 1 : 0)) * kPartFloats;
-    };
+    while (list.cuts[end + 1].x == to.x && list.cuts[end + 1].y > 0) ++end;
     float M = -INFINITY, L = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     constexpr int kAtOnce = 8;  // parts whose loads are in flight together
@@ -776,8 +1049,9 @@ __global__ __launch_bounds__(256) void k_packed_combine(PackedArgs a, bool promp
         float4 v[kAtOnce];
 #pragma unroll
         for (int i = 0; i < kAtOnce; ++i) {
-            const float* b = slot(min(p + i, end));
-            ml[i] = *reinterpret_cast<const float2*>(b + kUnitRows * kHeadDim + 2 * row);
+            const int q = min(p + i, end);
+            const float* b = (few ? few_parts : wide_parts) + part_at(few, q * a.HKV + kvh, q == share ? 1 : 0);
+            ml[i] = *reinterpret_cast<const float2*>(b + (few ? kFewRows : kUnitRows) * kHeadDim + 2 * row);
             v[i] = *reinterpret_cast<const float4*>(b + row * kHeadDim + d);
         }
         float mn = M;
@@ -796,8 +1070,8 @@ __global__ __launch_bounds__(256) void k_packed_combine(PackedArgs a, bool promp
             o.z = __builtin_fmaf(wv, v[i].z, o.z), o.w = __builtin_fmaf(wv, v[i].w, o.w);
         }
     }
-    const float inv = e.z - e.y + t0 < 0 ? 0.f : 1.f / L;  // a row that sees no key: zeros
-    *reinterpret_cast<float4*>(a.out + (((size_t)e.x + t0) * a.H + kvh * G + f - t0 * G) * kHeadDim + d) =
+    const float inv = x.len - x.n + t0 < 0 ? 0.f : 1.f / L;  // a row that sees no key: zeros
+    *reinterpret_cast<float4*>(a.out + (((size_t)x.row0 + t0) * a.H + kvh * G + f - t0 * G) * kHeadDim + d) =
         make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
 }
 
@@ -818,7 +1092,7 @@ __global__ __launch_bounds__(256) void k_packed_prepare(const float* __restrict_
     const int H = a.H, HKV = a.HKV, NH = H + HKV;
     const int h0 = (blockIdx.y * 4 + w) * kPrepHeads;
     if (h0 >= NH || !plan_fits(a.plan, a.n_seq, a.rows, H, HKV, false)) return;  // wave-uniform, no barrier here
-    const int4* seq = reinterpret_cast<const int4*>(a.plan + plan_seq_at());
+    const int4* seq = reinterpret_cast<const int4*>(a.plan + kPlanSeqAt);
     const int s = row_owner(seq, a.n_seq, b, lane);
     if (s < 0) return;
     const int4 e = seq[s];
@@ -878,25 +1152,32 @@ hipError_t launch_packed_plan(hipStream_t st, const int* cu, const int* kv_len, 
 static size_t q_bytes(int rows, int H) { return ((size_t)rows * H * kHeadDim * 4 + 255) & ~(size_t)255; }
 
 size_t packed_ws_bytes(int rows, int H, int HKV) {
-    return q_bytes(rows, H) + (size_t)packed_shares(HKV) * HKV * 2 * kPartFloats * 4;
+    return q_bytes(rows, H) + (size_t)packed_shares(HKV) * HKV * 2 * (kWidePart + kFewPart) * sizeof(float);
 }
 
 template <bool kPaged>
-static hipError_t launch_packed_attn(hipStream_t st, const PackedArgs& a, int shares, float* parts) {
-    static std::atomic<bool> opted;
-    constexpr size_t lds = (size_t)kLdsF * sizeof(float);
-    if (const hipError_t e = opt_in_lds(opted, (const void*)k_packed_attn<kPaged>, lds); e != hipSuccess) return e;
-    k_packed_attn<kPaged><<<(unsigned)(shares * a.HKV), 64 * kSlots * kGroups, lds, st>>>(a, shares, parts);
+static hipError_t launch_packed_attn(hipStream_t st, const PackedArgs& a, int shares, float* wide, float* few) {
+    static std::atomic<bool> opted_wide, opted_few;
+    constexpr size_t lds_wide = (size_t)kWideF * sizeof(float), lds_few = (size_t)kFewF * sizeof(float);
+    if (const hipError_t e = opt_in_lds(opted_wide, (const void*)k_packed_wide<kPaged>, lds_wide); e != hipSuccess)
+        return e;
+    if (const hipError_t e = opt_in_lds(opted_few, (const void*)k_packed_few<kPaged>, lds_few); e != hipSuccess)
+        return e;
+    const unsigned grid = (unsigned)(shares * a.HKV);
+    k_packed_wide<kPaged><<<grid, 64 * kWaves, lds_wide, st>>>(a, shares, wide);
+    k_packed_few<kPaged><<<grid, 64 * kWaves, lds_few, st>>>(a, shares, few);
     return hipGetLastError();
 }
 
 hipError_t launch_packed(hipStream_t st, const PackedArgs& a, void* ws) {
-    float* parts = reinterpret_cast<float*>(static_cast<char*>(ws) + q_bytes(a.rows, a.H));
     const int shares = packed_shares(a.HKV);
-    const hipError_t e = a.btab ? launch_packed_attn<true>(st, a, shares, parts)
-                                : launch_packed_attn<false>(st, a, shares, parts);
+    float* wide = reinterpret_cast<float*>(static_cast<char*>(ws) + q_bytes(a.rows, a.H));
+    float* few = wide + (size_t)shares * a.HKV * 2 * kWidePart;
+    const hipError_t e = a.btab ? launch_packed_attn<true>(st, a, shares, wide, few)
+                                : launch_packed_attn<false>(st, a, shares, wide, few);
     if (e != hipSuccess) return e;
-    k_packed_combine<<<dim3(shares * a.HKV, kUnitRows / 8), 256, 0, st>>>(a, a.btab == nullptr, shares, parts);
+    k_packed_combine<<<dim3(shares * a.HKV, kCombineWide + kCombineFew), 256, 0, st>>>(a, a.btab == nullptr, shares,
+                                                                                        wide, few);
     return hipGetLastError();
 }
 

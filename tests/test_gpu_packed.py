@@ -45,15 +45,20 @@ def _shares(HKV):
 
 
 def _read_plan(batch, lens, rows, H, HKV):
-    """The plan's units and cuts, from its buffer (header, sequences, units, cuts)."""
+    """The plan's two lists, wide and few-row units with their cuts, from its buffer (header, sequences, units of
+    both, cuts of both)."""
     raw = batch.buf.cpu().numpy()
     head = raw[:256].view(np.int32)
-    G, n_seq = H // HKV, len(lens)
-    at = 256 + 16 * n_seq
-    cap = rows * G // 128 + n_seq
-    units = raw[at:at + 16 * cap].view(np.int32).reshape(-1, 4)
-    cuts = raw[at + 16 * cap:at + 16 * cap + 8 * (_shares(HKV) + 1)].view(np.int32).reshape(-1, 2)
-    return head, units[:head[7] + head[8]], cuts
+    G, n_seq, cuts = H // HKV, len(lens), 8 * (_shares(HKV) + 1)
+    wide = 256 + 16 * n_seq
+    few = wide + 32 * (rows * G // 128 + n_seq)
+    at = few + 32 * n_seq
+
+    def units(start, n):
+        return raw[start:start + 32 * n].view(np.int32).reshape(-1, 8)
+
+    return (head, units(wide, head[7] + head[8]), raw[at:at + cuts].view(np.int32).reshape(-1, 2),
+            units(few, head[9]), raw[at + cuts:at + 2 * cuts].view(np.int32).reshape(-1, 2))
 
 
 BATCHES = [  # H, HKV, lens, kv_len (None: whole prompts)
@@ -72,36 +77,43 @@ def test_plan_covers_every_unit_once(gpu, H, HKV, lens, kv):
     rows, G = sum(lens), H // HKV
     b = gpu.PackedBatch(len(lens), rows, H, HKV)
     b.plan(_i32(_cu(lens)), rows, max(kv or lens), kv_len=None if kv is None else _i32(kv))
-    head, units, cuts = _read_plan(b, lens, rows, H, HKV)
+    head, wide, wide_cuts, few, few_cuts = _read_plan(b, lens, rows, H, HKV)
     N = _shares(HKV)
-    want = {}
+    want = {True: {}, False: {}}
     for s, n in enumerate(lens):
         total = n if kv is None else kv[s]
         for u in range((n * G + 127) // 128):
             last = min(n - 1, (128 * u + 127) // G)
-            want[s, u] = (max(0, min(total, total - n + last + 1)) + 31) // 32
-    assert {(int(s), int(u)): int(t) for s, u, t, _ in units} == want and len(units) == len(want)
+            want[n * G - 128 * u <= 32][s, u] = (max(0, min(total, total - n + last + 1)) + 31) // 32
     rounds, dealt, line = int(head[6]), int(head[7]), int(head[8])
-    assert dealt == rounds * N and dealt + line == len(units)
-    tiles = units[:, 2].astype(int)
-    if rounds:
-        assert np.all(np.diff(tiles) <= 0)  # descending
-    load = np.zeros(N, int)
-    for i in range(dealt):
-        r, j = divmod(i, N)
-        load[N - 1 - j if r % 2 else j] += tiles[i] + 5
-    assert tuple(cuts[0]) == (0, 0) and tuple(cuts[N]) == (line, 0)
-    for j in range(N):
-        (a, ta), (e, te) = cuts[j], cuts[j + 1]
-        assert (a, ta) <= (e, te)
-        for i, t in ((a, ta), (e, te)):
-            assert t == 0 or (i < line and 2 <= t < tiles[dealt + i] and t % 2 == 0)
-        for i in range(a, min(e + 1, line)):
-            lo, hi = (ta if i == a else 0), (te if i == e else tiles[dealt + i])
-            if i < e or te > 0:
-                load[j] += hi - lo + 5
-    fair = max(sum(t + 5 for t in want.values()) / N, 8)
-    assert load.max() <= fair + 2 * 5 + 4 + (max(tiles, default=0) if dealt else 0), (load, fair)
+    assert dealt == rounds * N and dealt + line == len(wide)
+    for is_few, units, cuts, first, (once, least, turn) in ((False, wide, wide_cuts, dealt, (5, 8, 2)),
+                                                            (True, few, few_cuts, 0, (8, 16, 8))):
+        cost = want[is_few]
+        assert {(int(x[4]), int(x[3])): int(x[5]) for x in units} == cost and len(units) == len(cost)
+        for x in units:
+            s = int(x[4])
+            assert (int(x[0]), int(x[1]), int(x[2])) == (int(_cu(lens)[s]), lens[s], lens[s] if kv is None else kv[s])
+        tiles = units[:, 5].astype(int)
+        if first:
+            assert np.all(np.diff(tiles) <= 0)  # descending
+        load = np.zeros(N, int)
+        for i in range(first):
+            r, j = divmod(i, N)
+            load[N - 1 - j if r % 2 else j] += tiles[i] + once
+        n = len(units) - first
+        assert tuple(cuts[0]) == (0, 0) and tuple(cuts[N]) == (n, 0)
+        for j in range(N):
+            (a, ta), (e, te) = cuts[j], cuts[j + 1]
+            assert (a, ta) <= (e, te)
+            for i, t in ((a, ta), (e, te)):
+                assert t == 0 or (i < n and turn <= t <= tiles[first + i] - turn and t % turn == 0)
+            for i in range(a, min(e + 1, n)):
+                lo, hi = (ta if i == a else 0), (te if i == e else tiles[first + i])
+                if i < e or te > 0:
+                    load[j] += hi - lo + once
+        fair = max(sum(t + once for t in cost.values()) / N, least)
+        assert load.max() <= fair + 2 * once + 2 * turn + (max(tiles, default=0) if first else 0), (load, fair)
 
 
 def _prompts(H, HKV, lens, seed, extra=0):
