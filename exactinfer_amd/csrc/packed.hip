@@ -15,7 +15,7 @@ constexpr int kFewRows = 32;    // units of up to so many rows go to k_packed_fe
 // The query rows of a sequence and KV head are taken flat, row f = token * G + head of the group, and
 // cut into units of kUnitRows: a unit shares its K and V tiles, whatever G is and however few tokens
 // there are.  A sequence's last unit, if it has at most kFewRows rows (single tokens, drafts, tails of
-// prompts), goes to the list of few-row units and its own kernel, the others to the wide list.
+// prompts), goes to the list of few-row units, the others to the wide list.
 //
 // `shares` workgroups serve each KV head, all heads alike, and take the same cost each: a unit's causal key
 // tiles, and something for what is done once per unit.  Few-row units are laid end to end on a line
@@ -32,9 +32,17 @@ struct Unit {
     int seq, tiles, pad[2];
 };
 static_assert(sizeof(Unit) == 32, "two 16-byte pieces");
-struct List {      // one kernel's work
-    Unit* units;   // dealt units in the order of the deal, then the line
-    int2* cuts;    // [shares + 1]: on the line, unit and first tile
+struct Share {
+    int first, first_tile, last, last_tile;  // on the line: from tile first_tile of unit `first` to last_tile of `last`
+    int merge_end;  // the last share with a part of the unit that begins here and is cut; 0: none does
+    int pad[3];
+    Unit start;     // what this share begins with
+    Unit merge;     // the unit that merge_end speaks of
+};
+static_assert(sizeof(Share) == 96, "six 16-byte pieces");
+struct List {
+    Unit* units;    // dealt units in the order of the deal, then the line
+    Share* shares;  // one per workgroup of a KV head
 };
 struct PlanView {
     int4* seq;     // first row, rows, keys, wide units before this sequence's
@@ -48,18 +56,18 @@ __host__ __device__ inline size_t plan_wide_at(int n_seq) { return kPlanSeqAt + 
 __host__ __device__ inline size_t plan_few_at(int n_seq, int rows, int G) {
     return plan_wide_at(n_seq) + (size_t)plan_max_wide(n_seq, rows, G) * sizeof(Unit);
 }
-__host__ __device__ inline size_t plan_cuts_at(int n_seq, int rows, int G) {
+__host__ __device__ inline size_t plan_shares_at(int n_seq, int rows, int G) {
     return plan_few_at(n_seq, rows, G) + (size_t)n_seq * sizeof(Unit);
 }
 __device__ __forceinline__ PlanView plan_view(char* plan, int n_seq, int rows, int G, int shares) {
-    int2* cuts = reinterpret_cast<int2*>(plan + plan_cuts_at(n_seq, rows, G));
+    Share* at = reinterpret_cast<Share*>(plan + plan_shares_at(n_seq, rows, G));
     return {reinterpret_cast<int4*>(plan + kPlanSeqAt),
-            {reinterpret_cast<Unit*>(plan + plan_wide_at(n_seq)), cuts},
-            {reinterpret_cast<Unit*>(plan + plan_few_at(n_seq, rows, G)), cuts + shares + 1}};
+            {reinterpret_cast<Unit*>(plan + plan_wide_at(n_seq)), at},
+            {reinterpret_cast<Unit*>(plan + plan_few_at(n_seq, rows, G)), at + shares}};
 }
 int packed_shares(int HKV) { return kPackedCus / HKV > 1 ? kPackedCus / HKV : 1; }
 size_t packed_plan_bytes(int n_seq, int rows, int H, int HKV) {
-    const size_t b = plan_cuts_at(n_seq, rows, H / HKV) + 2 * (size_t)(packed_shares(HKV) + 1) * sizeof(int2);
+    const size_t b = plan_shares_at(n_seq, rows, H / HKV) + 2 * (size_t)packed_shares(HKV) * sizeof(Share);
     return (b + 255) & ~(size_t)255;
 }
 
@@ -68,22 +76,29 @@ constexpr int kPlanSeqLds = 1024;       // sequences held in LDS (more are read 
 constexpr int kPlanLineLds = 1024;      // units of the line held in LDS (likewise)
 constexpr long kMaxRankWork = 1 << 20;  // wide units x sequences up to which units are sorted
 
-// What the two kernels' work costs, in tiles: `pass` for everything done once per unit; a workgroup is worth
-// `least`; a cut leaves whole turns (the tiles that a workgroup's waves take at a time) on both sides.
+// What a list's work costs, in tiles: `pass` for everything done once per unit or part of one; a cut leaves
+// whole turns (the tiles that a workgroup's waves take at a time) on both sides, and keeps off a unit's
+// ends by what a pass costs, so that a share does not run one for a few tiles.
 struct ListCost {
-    int pass, least, turn;
+    int pass, turn;
 };
-constexpr ListCost kWideCost = {5, 8, 2}, kFewCost = {8, 16, 8};
+constexpr ListCost kWideCost = {5, 2}, kFewCost = {8, 8};
 
-// Sum over the lanes up to this one.
+// Sum over the lanes up to this one, by DPP: within rows of 16, then the last lane of each row (15), of
+// the two upper rows (31) onwards.
+template <int kCtrl, int kRows>
+__device__ __forceinline__ long long dpp_add(long long v) {
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)v, kCtrl, kRows, 0xF, false);
+    const int hi = __builtin_amdgcn_update_dpp(0, (int)(v >> 32), kCtrl, kRows, 0xF, false);
+    return v + (long long)(((unsigned long long)(unsigned)hi << 32) | (unsigned)lo);
+}
 __device__ __forceinline__ long long wave_scan(long long v) {
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const long long t = __shfl_up(v, d);
-        if (lane >= d) v += t;
-    }
-    return v;
+    v = dpp_add<0x111, 0xF>(v);  // row_shr:1, 2, 4, 8
+    v = dpp_add<0x112, 0xF>(v);
+    v = dpp_add<0x114, 0xF>(v);
+    v = dpp_add<0x118, 0xF>(v);
+    v = dpp_add<0x142, 0xA>(v);  // row_bcast:15
+    return dpp_add<0x143, 0xC>(v);  // row_bcast:31
 }
 // Exclusive sum over the workgroup; total in every thread.
 __device__ __forceinline__ long long block_scan(long long v, long long* total) {
@@ -110,23 +125,21 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
                                                               char* __restrict__ plan) {
     __shared__ int4 seq_lds[kPlanSeqLds];
     __shared__ int line_lds[kPlanLineLds];
-    __shared__ unsigned long long load[kPackedCus];
+    __shared__ unsigned long long load[kPackedCus], few_cost, wide_cost;
     __shared__ long long cut_at[kPackedCus + 1];
+    __shared__ int2 cuts[kPackedCus + 1];
     const int tid = threadIdx.x, G = H / HKV;
     const PlanView pv = plan_view(plan, n_seq, rows, G, shares);
     // keys that rows up to `row` of a sequence of n rows and len keys see, in tiles
     auto tiles_of = [](int n, int len, int row) { return (max(min(len - n + row + 1, len), 0) + kKT - 1) / kKT; };
     auto wide_of = [&](int n) { return (int)(((long long)n * G + kUnitRows - 1 - kFewRows) / kUnitRows); };
 
-    // The cuts of a line of `line` units: share j's end where `before` (its and the earlier shares' wants)
-    // falls on the running cost.
-    auto cut_line = [&](const List& list, int dealt, int line, ListCost c, const int* lds, long long want) {
-        long long all;
-        const long long before = block_scan(want, &all);
-        if (tid <= shares) {
-            cut_at[tid] = tid == 0 ? 0 : before;  // (thread `shares` wants nothing: the sum of all)
-            list.cuts[tid] = make_int2(tid == 0 ? 0 : line, 0);
-        }
+    // The shares of a list whose line has `line` units: share j's end where cut_at[j + 1] falls on the
+    // line's running cost (cut_at is set, the units are written).
+    auto cut_line = [&](const List& list, int rounds, int line, ListCost c, const int* lds, long long share) {
+        const int dealt = rounds * shares;
+        const int keep = max(c.turn, min(c.pass, (int)min(share / 2, (long long)c.pass)));
+        if (tid <= shares) cuts[tid] = make_int2(tid == 0 ? 0 : line, 0);
         __syncthreads();
         long long at = 0;
         for (int base = 0; base < line; base += kPlanThreads) {
@@ -142,18 +155,34 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
                     if (cut_at[mid] >= a) hi = mid;
                     else lo = mid + 1;
                 }
-                for (; lo <= shares && cut_at[lo] < a + cost; ++lo) {
+                for (; lo < shares && cut_at[lo] < a + cost; ++lo) {
                     const long long t = (cut_at[lo] - a) / c.turn * c.turn;
-                    if (lo == shares || t + c.turn > tiles) list.cuts[lo] = make_int2(lo == shares ? line : i + 1, 0);
-                    else list.cuts[lo] = make_int2(i, (int)t);
+                    cuts[lo] = t + keep > tiles ? make_int2(i + 1, 0) : make_int2(i, t < keep ? 0 : (int)t);
                 }
             }
             at += sum;
         }
+        __syncthreads();
+        if (tid < shares) {
+            const int2 from = cuts[tid], to = cuts[tid + 1];
+            Share& x = list.shares[tid];
+            x.first = from.x, x.first_tile = from.y, x.last = to.x, x.last_tile = to.y;
+            if (rounds > 0 || from.x < line) x.start = list.units[rounds > 0 ? tid : from.x];
+            int end = 0;
+            if (to.y > 0 && !(from.x == to.x && from.y > 0)) {  // a unit begins here and goes on
+                end = tid + 1;
+                while (cuts[end + 1].x == to.x && cuts[end + 1].y > 0) ++end;
+                x.merge = list.units[dealt + to.x];
+            }
+            x.merge_end = end;
+        }
+        __syncthreads();
     };
 
+    if (tid == 0) few_cost = wide_cost = 0;
+    for (int j = tid; j < shares; j += kPlanThreads) load[j] = 0;
     // sequences: rows, keys, first wide unit; the few-row units
-    long long units = 0, few = 0, few_cost = 0;
+    long long units = 0, few = 0;
     int bad = 0;
     for (int base = 0; base < n_seq; base += kPlanThreads) {
         const int s = base + tid;
@@ -181,19 +210,19 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
             pv.few.units[i] = Unit{lo, n, len, nw, s, tiles, {0, 0}};
             if (i < kPlanLineLds) line_lds[i] = tiles;
         }
+        const long long cost = wave_scan(is_few ? tiles + kFewCost.pass : 0);
+        if ((tid & 63) == 63 && cost > 0) atomicAdd(&few_cost, (unsigned long long)cost);
         units += all >> 32;
         few += all & 0xFFFFFFFF;
-        block_scan(is_few ? tiles + kFewCost.pass : 0, &all);
-        few_cost += all;
     }
     if (bad) units = few = 0;
     const int U = (int)units;
     __syncthreads();
-    if (few > 0) {  // uniform
-        const long long share = max((few_cost + shares - 1) / shares, (long long)kFewCost.least);
-        cut_line(pv.few, 0, (int)few, kFewCost, few <= kPlanLineLds ? line_lds : nullptr, tid < shares ? share : 0);
-        __syncthreads();
-    } else if (tid <= shares) pv.few.cuts[tid] = make_int2(0, 0);
+    {
+        const long long share = few > 0 ? ((long long)few_cost + shares - 1) / shares : 0;
+        if (tid <= shares) cut_at[tid] = tid * share;
+        cut_line(pv.few, 0, (int)few, kFewCost, few <= kPlanLineLds ? line_lds : nullptr, share);
+    }
 
     const bool in_lds = n_seq <= kPlanSeqLds;
     auto seq_at = [&](int s) { return in_lds ? seq_lds[s] : pv.seq[s]; };
@@ -217,57 +246,44 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
         if (m <= 0) return nw;
         return m >= e.y ? 0 : nw - min(nw, (int)(m * G / kUnitRows));
     };
-    if (U > 0) {  // uniform
-        Unit own{};  // this thread's first unit
-        long long mine = 0, total;
-        for (int i = tid; i < U; i += kPlanThreads) {
-            const Unit x = unit(i);
-            if (i == tid) own = x;
-            mine += x.tiles + kWideCost.pass;
-        }
-        for (int j = tid; j < shares; j += kPlanThreads) load[j] = 0;
-        block_scan(mine, &total);
-        const long long share = max((total + shares - 1) / shares, (long long)kWideCost.least);
-        // (sorting costs units x sequences: where that is much, there is enough work for the order not to matter)
-        const int rounds = (long long)U * n_seq <= kMaxRankWork && U / shares > 1 ? U / shares - 1 : 0;
-        const int dealt = rounds * shares, line = U - dealt;
-        for (int i = tid; i < U; i += kPlanThreads) {
-            const Unit x = i == tid ? own : unit(i);
-            int at = i;
-            if (rounds > 0) {
-                // units before this one: more tiles, or as many in an earlier sequence, or later in its own
-                at = 0;
-                for (int s = 0; s < n_seq; ++s) {
-                    const int4 e = seq_at(s);
-                    at += s < x.seq ? above(e, x.tiles - 1) : s > x.seq ? above(e, x.tiles) : wide_of(e.y) - 1 - x.u;
-                }
+    // (sorting costs units x sequences: where that is much, there is enough work for the order not to matter)
+    const int rounds = (long long)U * n_seq <= kMaxRankWork && U / shares > 1 ? U / shares - 1 : 0;
+    const int dealt = rounds * shares, line = U - dealt;
+    long long mine = 0;
+    for (int i = tid; i < U; i += kPlanThreads) {
+        const Unit x = unit(i);
+        mine += x.tiles + kWideCost.pass;
+        int at = i;
+        if (rounds > 0) {
+            // units before this one: more tiles, or as many in an earlier sequence, or later in its own
+            at = 0;
+            for (int s = 0; s < n_seq; ++s) {
+                const int4 e = seq_at(s);
+                at += s < x.seq ? above(e, x.tiles - 1) : s > x.seq ? above(e, x.tiles) : wide_of(e.y) - 1 - x.u;
             }
-            pv.wide.units[at] = x;
-            if (at < dealt) {
-                const int r = at / shares, j = at - r * shares;
-                atomicAdd(&load[(r & 1) ? shares - 1 - j : j], (unsigned long long)(x.tiles + kWideCost.pass));
-            } else if (at - dealt < kPlanLineLds) line_lds[at - dealt] = x.tiles;
         }
-        __syncthreads();
-        const long long want = tid < shares ? max(share - (long long)load[tid], 0LL) : 0;
-        cut_line(pv.wide, dealt, line, kWideCost, line <= kPlanLineLds ? line_lds : nullptr, want);
-        if (tid == 0) {
-            int* h = reinterpret_cast<int*>(plan);
-            h[kHeadRounds] = rounds, h[kHeadDealt] = dealt, h[kHeadLine] = line;
-        }
-    } else {
-        if (tid <= shares) pv.wide.cuts[tid] = make_int2(0, 0);
-        if (tid == 0) {
-            int* h = reinterpret_cast<int*>(plan);
-            h[kHeadRounds] = h[kHeadDealt] = h[kHeadLine] = 0;
-        }
+        pv.wide.units[at] = x;
+        if (at < dealt) {
+            const int r = at / shares, j = at - r * shares;
+            atomicAdd(&load[(r & 1) ? shares - 1 - j : j], (unsigned long long)(x.tiles + kWideCost.pass));
+        } else if (at - dealt < kPlanLineLds) line_lds[at - dealt] = x.tiles;
+    }
+    mine = wave_scan(mine);
+    if ((tid & 63) == 63 && mine > 0) atomicAdd(&wide_cost, (unsigned long long)mine);
+    __syncthreads();
+    {
+        const long long share = U > 0 ? ((long long)wide_cost + shares - 1) / shares : 0;
+        long long before = tid * share, all;
+        if (rounds > 0) before = block_scan(tid < shares ? max(share - (long long)load[tid], 0LL) : 0, &all);
+        if (tid <= shares) cut_at[tid] = before;
+        cut_line(pv.wide, rounds, line, kWideCost, line <= kPlanLineLds ? line_lds : nullptr, share);
     }
     if (tid == 0) {
         int* h = reinterpret_cast<int*>(plan);
         h[0] = bad ? 0 : kPlanMagic;
         h[1] = n_seq, h[2] = rows, h[3] = H, h[4] = HKV;
         h[5] = kv_len == nullptr;
-        h[kHeadFew] = (int)few;
+        h[kHeadRounds] = rounds, h[kHeadDealt] = dealt, h[kHeadLine] = line, h[kHeadFew] = (int)few;
     }
 }
 
@@ -312,7 +328,7 @@ __device__ __forceinline__ int row_owner(const int4* seq, int n_seq, int b, int 
 //
 // Few-row units (few_pass): every wave holds the same rows and a tile of its own, loaded straight into the
 // operands' registers (more loads in flight, no barrier in the loop); q's planes are in LDS.  (Both kinds
-// in one kernel leave the compiler short of registers in both loops.)
+// of pass in one loop leave the compiler short of registers in both: they are a workgroup's role.)
 typedef __amdgpu_buffer_rsrc_t Rsrc;
 constexpr int kQB = 32;                         // flat rows per wave
 constexpr int kSlots = kUnitRows / kQB;         // waves per key group
@@ -977,9 +993,9 @@ __device__ __forceinline__ void walk_list(const PackedArgs& a, int shares, float
     const List list = kFew ? pv.few : pv.wide;
     const int* head = reinterpret_cast<const int*>(a.plan);
     const int rounds = kFew ? 0 : scalar(head[kHeadRounds]), dealt = kFew ? 0 : scalar(head[kHeadDealt]);
-    const int2 from = list.cuts[share], to = list.cuts[share + 1];
+    const int4 sh = *reinterpret_cast<const int4*>(list.shares + share);
     if (!plan_fits(a.plan, a.n_seq, a.rows, a.H, a.HKV, !kPaged)) return;
-    const int first = scalar(from.x), first_tile = scalar(from.y), last = scalar(to.x), last_tile = scalar(to.y);
+    const int first = scalar(sh.x), first_tile = scalar(sh.y), last = scalar(sh.z), last_tile = scalar(sh.w);
     for (int pass = 0;; ++pass) {
         int at, cut = -1;
         Pass p;
@@ -993,7 +1009,8 @@ __device__ __forceinline__ void walk_list(const PackedArgs& a, int shares, float
             cut = i == last ? last_tile : -1;
             p.kt_lo = i == first ? first_tile : 0;
         }
-        const Unit x = list.units[at];
+        // (the share's own copy comes with the line just read: no wait for a list entry)
+        const Unit x = *(pass == 0 ? &list.shares[share].start : list.units + at);
         const int n = scalar(x.n), len = scalar(x.len);
         p.seq = scalar(x.seq), p.u = scalar(x.u), p.row0 = scalar(x.row0);
         p.pos0 = len - n;
@@ -1006,15 +1023,15 @@ __device__ __forceinline__ void walk_list(const PackedArgs& a, int shares, float
         else wide_pass<kPaged>(a, p, kvh, fG, sl2, smem);
     }
 }
+
+// grid (shares x KV heads, 2): the wide list's workgroups, then the few-row list's, which start as the others
+// finish (a workgroup's LDS takes a CU) or at once where there is no wide work.
 template <bool kPaged>
-__global__ __launch_bounds__(64 * kWaves) void k_packed_wide(PackedArgs a, int shares, float* __restrict__ parts) {
+__global__ __launch_bounds__(64 * kWaves) void k_packed_attn(PackedArgs a, int shares, float* __restrict__ wide,
+                                                             float* __restrict__ few) {
     extern __shared__ __align__(16) float smem[];
-    walk_list<kPaged, false>(a, shares, parts, smem);
-}
-template <bool kPaged>
-__global__ __launch_bounds__(64 * kWaves) void k_packed_few(PackedArgs a, int shares, float* __restrict__ parts) {
-    extern __shared__ __align__(16) float smem[];
-    walk_list<kPaged, true>(a, shares, parts, smem);
+    if (blockIdx.y == 0) walk_list<kPaged, false>(a, shares, wide, smem);
+    else walk_list<kPaged, true>(a, shares, few, smem);
 }
 
 // The units that the cuts divide: workgroup (share, KV head; 8 rows) merges the unit that starts in
@@ -1030,17 +1047,13 @@ __global__ __launch_bounds__(256) void k_packed_combine(PackedArgs a, bool promp
     const bool few = blockIdx.y >= kCombineWide;
     const PlanView pv = plan_view(const_cast<char*>(a.plan), a.n_seq, a.rows, G, shares);
     const List list = few ? pv.few : pv.wide;
-    const int dealt = few ? 0 : reinterpret_cast<const int*>(a.plan)[kHeadDealt];
-    const int2 from = list.cuts[share], to = list.cuts[share + 1];
-    if (!plan_fits(a.plan, a.n_seq, a.rows, a.H, a.HKV, prompts)) return;
-    if (to.y == 0 || (from.x == to.x && from.y > 0)) return;  // ends between units, or goes on with a unit
-    const Unit x = list.units[dealt + to.x];
+    const int end = list.shares[share].merge_end;
+    const Unit x = list.shares[share].merge;
+    if (!plan_fits(a.plan, a.n_seq, a.rows, a.H, a.HKV, prompts) || end == 0) return;
     const int row = (few ? blockIdx.y - kCombineWide : blockIdx.y) * kCombineRows + (threadIdx.x >> 5);
     const int f = kUnitRows * x.u + row, d = 4 * (threadIdx.x & 31);
     if (f >= x.n * G) return;
     const int t0 = f / G;
-    int end = share + 1;  // the last share with a part
-    while (list.cuts[end + 1].x == to.x && list.cuts[end + 1].y > 0) ++end;
     float M = -INFINITY, L = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     constexpr int kAtOnce = 8;  // parts whose loads are in flight together
@@ -1157,15 +1170,10 @@ size_t packed_ws_bytes(int rows, int H, int HKV) {
 
 template <bool kPaged>
 static hipError_t launch_packed_attn(hipStream_t st, const PackedArgs& a, int shares, float* wide, float* few) {
-    static std::atomic<bool> opted_wide, opted_few;
-    constexpr size_t lds_wide = (size_t)kWideF * sizeof(float), lds_few = (size_t)kFewF * sizeof(float);
-    if (const hipError_t e = opt_in_lds(opted_wide, (const void*)k_packed_wide<kPaged>, lds_wide); e != hipSuccess)
-        return e;
-    if (const hipError_t e = opt_in_lds(opted_few, (const void*)k_packed_few<kPaged>, lds_few); e != hipSuccess)
-        return e;
-    const unsigned grid = (unsigned)(shares * a.HKV);
-    k_packed_wide<kPaged><<<grid, 64 * kWaves, lds_wide, st>>>(a, shares, wide);
-    k_packed_few<kPaged><<<grid, 64 * kWaves, lds_few, st>>>(a, shares, few);
+    static std::atomic<bool> opted;
+    constexpr size_t lds = (size_t)(kWideF > kFewF ? kWideF : kFewF) * sizeof(float);
+    if (const hipError_t e = opt_in_lds(opted, (const void*)k_packed_attn<kPaged>, lds); e != hipSuccess) return e;
+    k_packed_attn<kPaged><<<dim3(shares * a.HKV, 2), 64 * kWaves, lds, st>>>(a, shares, wide, few);
     return hipGetLastError();
 }
 

@@ -45,11 +45,11 @@ def _shares(HKV):
 
 
 def _read_plan(batch, lens, rows, H, HKV):
-    """The plan's two lists, wide and few-row units with their cuts, from its buffer (header, sequences, units of
-    both, cuts of both)."""
+    """The plan's header and two lists, wide and few-row: their units and shares (first, first tile, last, last tile,
+    last share of a merge, 3 words, the unit it starts with, the unit to merge)."""
     raw = batch.buf.cpu().numpy()
     head = raw[:256].view(np.int32)
-    G, n_seq, cuts = H // HKV, len(lens), 8 * (_shares(HKV) + 1)
+    G, n_seq, shares = H // HKV, len(lens), 96 * _shares(HKV)
     wide = 256 + 16 * n_seq
     few = wide + 32 * (rows * G // 128 + n_seq)
     at = few + 32 * n_seq
@@ -57,8 +57,8 @@ def _read_plan(batch, lens, rows, H, HKV):
     def units(start, n):
         return raw[start:start + 32 * n].view(np.int32).reshape(-1, 8)
 
-    return (head, units(wide, head[7] + head[8]), raw[at:at + cuts].view(np.int32).reshape(-1, 2),
-            units(few, head[9]), raw[at + cuts:at + 2 * cuts].view(np.int32).reshape(-1, 2))
+    return (head, units(wide, head[7] + head[8]), raw[at:at + shares].view(np.int32).reshape(-1, 24),
+            units(few, head[9]), raw[at + shares:at + 2 * shares].view(np.int32).reshape(-1, 24))
 
 
 BATCHES = [  # H, HKV, lens, kv_len (None: whole prompts)
@@ -77,7 +77,7 @@ def test_plan_covers_every_unit_once(gpu, H, HKV, lens, kv):
     rows, G = sum(lens), H // HKV
     b = gpu.PackedBatch(len(lens), rows, H, HKV)
     b.plan(_i32(_cu(lens)), rows, max(kv or lens), kv_len=None if kv is None else _i32(kv))
-    head, wide, wide_cuts, few, few_cuts = _read_plan(b, lens, rows, H, HKV)
+    head, wide, wide_shares, few, few_shares = _read_plan(b, lens, rows, H, HKV)
     N = _shares(HKV)
     want = {True: {}, False: {}}
     for s, n in enumerate(lens):
@@ -87,8 +87,8 @@ def test_plan_covers_every_unit_once(gpu, H, HKV, lens, kv):
             want[n * G - 128 * u <= 32][s, u] = (max(0, min(total, total - n + last + 1)) + 31) // 32
     rounds, dealt, line = int(head[6]), int(head[7]), int(head[8])
     assert dealt == rounds * N and dealt + line == len(wide)
-    for is_few, units, cuts, first, (once, least, turn) in ((False, wide, wide_cuts, dealt, (5, 8, 2)),
-                                                            (True, few, few_cuts, 0, (8, 16, 8))):
+    for is_few, units, shares, first, (once, turn) in ((False, wide, wide_shares, dealt, (5, 2)),
+                                                       (True, few, few_shares, 0, (8, 8))):
         cost = want[is_few]
         assert {(int(x[4]), int(x[3])): int(x[5]) for x in units} == cost and len(units) == len(cost)
         for x in units:
@@ -101,19 +101,30 @@ def test_plan_covers_every_unit_once(gpu, H, HKV, lens, kv):
         for i in range(first):
             r, j = divmod(i, N)
             load[N - 1 - j if r % 2 else j] += tiles[i] + once
-        n = len(units) - first
-        assert tuple(cuts[0]) == (0, 0) and tuple(cuts[N]) == (n, 0)
+        n, at = len(units) - first, (0, 0)
+        begins, ends = {}, {}  # shares in which a cut unit begins; the last share with a part of a unit
         for j in range(N):
-            (a, ta), (e, te) = cuts[j], cuts[j + 1]
-            assert (a, ta) <= (e, te)
-            for i, t in ((a, ta), (e, te)):
-                assert t == 0 or (i < n and turn <= t <= tiles[first + i] - turn and t % turn == 0)
+            (a, ta), (e, te) = shares[j, 0:2], shares[j, 2:4]
+            assert (a, ta) == at and (a, ta) <= (e, te)
+            at = (e, te)
+            assert te == 0 or (e < n and turn <= te <= tiles[first + e] - turn and te % turn == 0)
             for i in range(a, min(e + 1, n)):
                 lo, hi = (ta if i == a else 0), (te if i == e else tiles[first + i])
                 if i < e or te > 0:
                     load[j] += hi - lo + once
-        fair = max(sum(t + once for t in cost.values()) / N, least)
-        assert load.max() <= fair + 2 * once + 2 * turn + (max(tiles, default=0) if first else 0), (load, fair)
+                    if lo == 0 and hi < tiles[first + i]:
+                        begins[j] = i
+                    if lo > 0:
+                        ends[i] = j
+            if first or a < n:
+                assert np.array_equal(shares[j, 8:16], units[j if first else a])
+        assert at == (n, 0)
+        for j in range(N):
+            assert shares[j, 4] == (ends[begins[j]] if j in begins else 0)
+            if j in begins:
+                assert np.array_equal(shares[j, 16:24], units[first + begins[j]])
+        fair = sum(t + once for t in cost.values()) / N
+        assert load.max() <= fair + 4 * once + 2 * turn + (max(tiles, default=0) if first else 0), (load, fair)
 
 
 def _prompts(H, HKV, lens, seed, extra=0):
@@ -344,8 +355,8 @@ def _norm_rope64(x, gamma, pos, rd, theta=1e6, eps=1e-6):
 
 
 @pytest.mark.parametrize("H,HKV,bs,lens,kv,rd", [
-    (16, 8, 64, [1, 100, 1, 60, 1], [301, 612, 34, 60, 901], 128), (32, 8, 32, [5] * 6, [29, 64, 101, 256, 300, 5], 128),
-    (40, 8, 128, [130, 1], [131, 1], 64), (8, 1, 32, [0, 7, 33], [40, 39, 33], 126), (64, 8, 64, [3, 3], [3, 400], 128),
+    (16, 8, 64, [1, 100, 1, 60, 1], [301, 612, 34, 60, 901], 128),
+    (32, 8, 32, [5] * 6, [29, 64, 101, 256, 300, 5], 128), (40, 8, 128, [130, 1], [131, 1], 64), (8, 1, 32, [0, 7, 33], [40, 39, 33], 126), (64, 8, 64, [3, 3], [3, 400], 128),
 ])
 def test_step(gpu, H, HKV, bs, lens, kv, rd):
     kc, vc, table, rows_of = _pool(lens, kv, HKV, bs, 41)

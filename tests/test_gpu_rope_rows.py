@@ -175,7 +175,8 @@ def test_python_refusals(gpu):
     cs, pos = gpu.rope_table_scaled(16), torch.zeros(4, dtype=torch.int32, device="cuda")
     ok = dict(x=x, n_heads=2, cs=cs, pos=pos)
     for match, kw in (("layout", dict(layout="pairs")), ("int32", dict(pos=pos.long())), ("float32", dict(x=x.half())),
-                      ("rows of", dict(n_heads=3)), ("rows of", dict(pos=torch.zeros(5, dtype=torch.int32, device="cuda"))),
+                      ("rows of", dict(n_heads=3)),
+                      ("rows of", dict(pos=torch.zeros(5, dtype=torch.int32, device="cuda"))),
                      
                       ("cs must be", dict(rope_dim=64)), ("contiguous", dict(x=x.t())), ("GPU tensor", dict(x=x.cpu())),
                       ("128 values", dict(gamma=x[0])), ("rows of", dict(out=x[:3])),
