@@ -1,6 +1,6 @@
 // packed.hip — attention of the new rows of several sequences on gfx950: the plan that lays a batch
 // out over the GPU, the attention kernel over packed prompts or a paged pool, and the step's prologue.
-#include <cstdlib>
+#include <type_traits>
 
 #include "common.h"
 #include "launch.h"
@@ -326,9 +326,10 @@ __device__ __forceinline__ int row_owner(const int4* seq, int n_seq, int b, int 
 // without rows repeat the sequence's last one and write nothing (a branch round their products costs the
 // other waves registers).
 //
-// Few-row units (few_pass): every wave holds the same rows and a tile of its own, loaded straight into the
-// operands' registers (more loads in flight, no barrier in the loop); q's planes are in LDS.  (Both kinds
-// of pass in one loop leave the compiler short of registers in both: they are a workgroup's role.)
+// Few-row units (few_pass), single tokens and short drafts, read much and multiply little: every wave holds
+// the same rows and a tile of its own, loaded straight into the operands' registers, and multiplies in
+// fp32, which needs no planes.  (Both kinds of pass in one loop leave the compiler short of registers in
+// both: they are a workgroup's role.)
 typedef __amdgpu_buffer_rsrc_t Rsrc;
 constexpr int kQB = 32;                         // flat rows per wave
 constexpr int kSlots = kUnitRows / kQB;         // waves per key group
@@ -343,16 +344,26 @@ constexpr int kKRowB = 2 * kHeadDim + 16, kKPlane = kKT * kKRowB;  // K plane: [
 constexpr int kVRowB = 2 * kKT + 16, kVPlane = kHeadDim * kVRowB;  // V plane, transposed: [128 d][32 keys]
 // LDS of a wide pass: the K planes of both groups, and the merge's exchange area, from 0; the V planes
 // after it, and over them the staging area of the unit's rows (queries, later outputs).  Of a few-rows
-// pass: q's planes from 0; then, over them, every wave's rows, and their (m, l).
+// pass: every wave's rows, and their (m, l).
 constexpr int kStageF = kWaves * kXchF * 64;
 constexpr int kWideF = kStageF + kUnitRows * kRowF;
-constexpr int kFewML = kWaves * kQB * kRowF;
-constexpr int kFewF = kFewML + kWaves * kQB * 2;
+constexpr int kFewBlock = 16;                   // rows of one matrix instruction of few_pass
+constexpr int kFewML = kWaves * kFewRows * kRowF;
+constexpr int kFewF = kFewML + kWaves * kFewRows * 2;
+static_assert(kWaves * 64 == kFewRows * 16, "sixteen threads stage a row");
 static_assert(kGroups * 3 * kKPlane <= kStageF * 4, "K planes below the staging area");
 static_assert(kStageF * 4 + kGroups * 3 * kVPlane <= kWideF * 4, "V planes within the LDS span");
 static_assert(kWideF * 4 <= 160 * 1024 && kFewF * 4 <= 160 * 1024, "LDS budget");
 
 __device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// The lane's number, made where it is used (two instructions; kept, it would be spilled and come back by a
+// load that waits for every load before it).
+__device__ __forceinline__ uint32_t lane_now() {
+    uint32_t zero = 0;
+    asm volatile("" : "+v"(zero));
+    return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, zero));
+}
 
 // A pass, all of it wave-uniform.
 struct Pass {
@@ -364,11 +375,13 @@ struct Pass {
     float* part;           // where its unnormalised rows go, or null: a whole unit
 };
 
-// The visible rows of a tile as a buffer: reads past the last one, and of a missing page, give zeros.
+// The visible rows of a tile as a buffer: reads past the last one, and of a missing page, give zeros (all
+// reads, if the tile is not `wanted`).
 template <bool kPaged>
-__device__ __forceinline__ Rsrc tile_rsrc(const PackedArgs& a, const Pass& p, const float* cache, int t0) {
+__device__ __forceinline__ Rsrc tile_rsrc(const PackedArgs& a, const Pass& p, const float* cache, int t0,
+                                          bool wanted = true) {
     size_t row = (size_t)p.row0 + t0;
-    int there = min(kKT, p.T - t0);
+    int there = wanted ? min(kKT, p.T - t0) : 0;
     if constexpr (kPaged) {
         const int blk = t0 >> a.bshift;
         const int phys = blk < a.max_blocks ? a.btab[(size_t)p.seq * a.max_blocks + blk] : -1;
@@ -445,9 +458,8 @@ __device__ __forceinline__ Planes split_p(const floatx16& s, int x) {
 // may have lost bits of its third plane, 2^-134, which shows in no sum from kSmallSum up; with a
 // smaller one the wave looks through its V tiles, in the quarters of the columns with such a sum: it
 // stands if no V value there is below kPlaneMin and the largest one is too small for the weights' 2^-134
-// to show in it.  tile(i) is the wave's i-th tile, at(db, row, quarter piece) the byte offset of four
-// values of column quarter db.
-template <bool kFew, typename Tile>
+// to show in it.  v_tile(i) is the wave's i-th tile.
+template <typename Tile>
 __device__ __forceinline__ bool planes_failed(const Sums& x, int n_mine, Tile v_tile, uint32_t row_bytes, int lane) {
     float z = x.l * 0.f, least[4];
 #pragma unroll
@@ -477,16 +489,14 @@ __device__ __forceinline__ bool planes_failed(const Sums& x, int n_mine, Tile v_
         for (int i = 0; i < n_mine; ++i) {
             const Rsrc rs = v_tile(i);
             const int ln = unhoisted(lane);
-            // lane: rows ln / 8 + 8j, four of the quarter's 32 values
-            const uint32_t off = (ln >> 3) * row_bytes + (kFew ? 64u * (ln & 7) + 4u * db : 16u * (ln & 7) + 128u * db);
+            const uint32_t off = (ln >> 3) * row_bytes + 16u * (ln & 7) + 128u * db;
 #pragma unroll
             for (int j = 0; j < kKT / 8; ++j) {
+                const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(rs, off + 8 * j * row_bytes, 0, 0);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const uint32_t v = __builtin_amdgcn_raw_buffer_load_b32(
-                        rs, off + 8 * j * row_bytes + (kFew ? 16 : 4) * e, 0, 0);
-                    tiny = min(tiny, magnitude(v));
-                    most = fmaxf(most, __builtin_fabsf(__uint_as_float(v)));
+                    tiny = min(tiny, magnitude(v[e]));
+                    most = fmaxf(most, __builtin_fabsf(__uint_as_float(v[e])));
                 }
             }
         }
@@ -499,8 +509,8 @@ __device__ __forceinline__ bool planes_failed(const Sums& x, int n_mine, Tile v_
 // A wave's tiles again, both products in fp32 from the cache.  In a tile that crosses the diagonal a
 // value that a row does not see must not be multiplied at all (0 times infinity), and the matrix
 // instruction takes every row with every key: P . V goes key by key there, P through p_lds, 32 x 32
-// floats of the wave's own.  Column of sum (db, i): 32 db + i, with kFew 4 i + db.
-template <bool kFew, typename KTile, typename VTile, typename Index>
+// floats of the wave's own.
+template <typename KTile, typename VTile, typename Index>
 __device__ __forceinline__ void redo_fp32(Sums& x, const PackedArgs& a, const Pass& p, const float* q_row, float sl2,
                                           int n_mine, KTile k_tile, VTile v_tile, Index index, int nfull, int qpos,
                                           uint32_t row_bytes, float* p_lds, int lane) {
@@ -534,15 +544,14 @@ __device__ __forceinline__ void redo_fp32(Sums& x, const PackedArgs& a, const Pa
         }
         softmax_tile(x, s, kt, nfull, qpos, hh);
         const Rsrc rs = v_tile(i);
-        constexpr uint32_t kI = kFew ? 16 : 4, kDb = kFew ? 4 : 128;
         if (kt < nfull) {
-            const uint32_t off = unhoisted(4 * hh) * row_bytes + kI * col;
+            const uint32_t off = unhoisted(4 * hh) * row_bytes + 4u * col;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {  // lane half hh: key 8(r/4) + 4hh + r%4
 #pragma unroll
                 for (int db = 0; db < 4; ++db) {
                     const float v = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
-                        rs, off + (8 * (r >> 2) + (r & 3)) * row_bytes + kDb * db, 0, 0));
+                        rs, off + (8 * (r >> 2) + (r & 3)) * row_bytes + 128 * db, 0, 0));
                     x.o[db] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[r], x.o[db], 0, 0, 0);
                 }
                 __builtin_amdgcn_sched_barrier(0);
@@ -557,15 +566,16 @@ __device__ __forceinline__ void redo_fp32(Sums& x, const PackedArgs& a, const Pa
 #pragma unroll 1
         for (int key = 0; key < kKT; ++key) {
             const float pk = pw[32 * key];
-            const uint32_t off = key * row_bytes + 4 * kI * (ln >> 5);
+            const uint32_t off = key * row_bytes + 16u * (ln >> 5);
             if (kt * kKT + key <= qpos) {
 #pragma unroll
                 for (int db = 0; db < 4; ++db) {
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) {  // i = 8(r/4) + 4hh + r%4
-                        const float v = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(
-                            rs, off + kDb * db + kI * (8 * (r >> 2) + (r & 3)), 0, 0));
-                        x.o[db][r] = __builtin_fmaf(pk, v, x.o[db][r]);
+                    for (int y = 0; y < 4; ++y) {  // d = 32 db + 8y + 4hh + 0 .. 3
+                        const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(rs, off + 128 * db + 32 * y, 0, 0);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            x.o[db][4 * y + e] = __builtin_fmaf(pk, __uint_as_float(v[e]), x.o[db][4 * y + e]);
                     }
                     __builtin_amdgcn_sched_barrier(0);
                 }
@@ -755,10 +765,10 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
     }
     if (grp == 0) lds_barrier();
 
-    if (live && (q_fp32 || planes_failed<false>(x, n_mine, v_tile, row_bytes, lane))) {
+    if (live && (q_fp32 || planes_failed(x, n_mine, v_tile, row_bytes, lane))) {
         const int f = min(f0 + col, p.nflat - 1), t0 = fdiv(f, fG);
         const float* q_row = a.q + ((size_t)p.row0 + t0) * a.q_stride + (size_t)(kvh * G + f - t0 * G) * D;
-        redo_fp32<false>(x, a, p, q_row, sl2, n_mine, k_tile, v_tile, index, nfull, qpos, row_bytes,
+        redo_fp32(x, a, p, q_row, sl2, n_mine, k_tile, v_tile, index, nfull, qpos, row_bytes,
                          smem + w * (kXchF * 64), lane);
     }
 
@@ -816,170 +826,259 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
 }
 
 // ---- a unit of few rows
-template <bool kPaged>
+// On v_mfma_f32_16x16x4_f32: S^T[key][row] = K . Q^T and O^T[d][row] = V^T . P^T for kBlocks sixteens of
+// rows; lane = row l % 16 of each, quarter l / 16.  Of a tile's half kb a lane holds the scores of the keys
+// 16 kb + 4 quarter + r (r = 0 .. 3), which are the operand of P . V for the steps (kb, r): step by step a
+// quarter of the lanes takes each of four keys.  K: step (x, e) takes d = 16x + 4 quarter + e, so that a
+// lane's row comes in 16-byte pieces; V: a lane's pieces hold d = 64y + 4 (l % 16) + e, sum 4y + e takes
+// element e.  Pieces of the next tile are fetched as this one's are used up.
+template <bool kPaged, int kBlocks>
 __device__ __forceinline__ void few_pass(const PackedArgs& a, const Pass& p, int kvh, FastDiv fG, float sl2,
                                          float* smem) {
-    constexpr int D = kHeadDim;
-    const int tid = unhoisted(threadIdx.x), lane = tid & 63, w = tid >> 6, wu = scalar(w);
-    const int col = lane & 31, hh = lane >> 5;
+    constexpr int D = kHeadDim, kRows = kFewBlock * kBlocks;
+    const int tid = unhoisted(threadIdx.x), lane = tid & 63, wu = scalar(tid >> 6);
+    const int j = lane & 15, quarter = lane >> 4;
     const int G = (int)fG.d;
     const uint32_t row_bytes = (uint32_t)(a.kv_stride * 4);
-    char* const qpl = reinterpret_cast<char*>(smem);
-    const int f0 = kUnitRows * p.u, last = p.nflat - 1;
-    const int qpos = p.pos0 + fdiv(min(f0 + col, last), fG);
+    const int f0 = kUnitRows * p.u, last = p.nflat - 1, rows = p.nflat - f0;
     const int nfull = max(p.pos0 + fdiv(f0, fG) + 1, 0) / kKT;
     const int n_mine = (p.nrange - wu + kWaves - 1) / kWaves;
     auto index = [&](int i) { return p.kt_lo + kWaves * i + wu; };
-    auto k_tile = [&](int i) { return tile_rsrc<kPaged>(a, p, a.k + (size_t)kvh * D, index(i) * kKT); };
-    auto v_tile = [&](int i) { return tile_rsrc<kPaged>(a, p, a.v + (size_t)kvh * D, index(i) * kKT); };
-    // K: lane's key col, d = 16t + 8hh .. + 7 (t of the four of half y), as the operand wants it
-    u32x4 kr[2][8];
-    const uint32_t voff_k = (uint32_t)col * row_bytes + 32u * hh;
-    auto load_k = [&](const Rsrc& rs, int y) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-            kr[y][j] = __builtin_amdgcn_raw_buffer_load_b128(rs, voff_k + 256 * y + 64 * (j >> 1) + 16 * (j & 1), 0, 0);
+    auto k_tile = [&](int i, bool wanted = true) {
+        return tile_rsrc<kPaged>(a, p, a.k + (size_t)kvh * D, index(i) * kKT, wanted);
     };
-    // V: d = 4 col .. + 3, one in each column quarter; step y holds the keys 16y + 4hh + {0..3, 8..11}
-    u32x4 vr[2][8];
-    const uint32_t voff_v = (uint32_t)(4 * hh) * row_bytes + 16u * col;
-    auto load_v = [&](const Rsrc& rs, int y) {
-        const uint32_t off = unhoisted(voff_v);
+    auto v_tile = [&](int i, bool wanted = true) {
+        return tile_rsrc<kPaged>(a, p, a.v + (size_t)kvh * D, index(i) * kKT, wanted);
+    };
+    u32x4 kr[2][8], vr[8][2];
+    auto load_k = [&](const Rsrc& rs, int x, uint32_t off) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            vr[y][j] = __builtin_amdgcn_raw_buffer_load_b128(
-                rs, off + (uint32_t)(16 * y + 8 * (j >> 2) + (j & 3)) * row_bytes, 0, 0);
+        for (int kb = 0; kb < 2; ++kb)
+            kr[kb][x] = __builtin_amdgcn_raw_buffer_load_b128(rs, off + 16 * kb * row_bytes + 64 * x, 0, 0);
+    };
+    auto k_offset = [&]() {
+        const uint32_t ln = lane_now();
+        return (ln & 15) * row_bytes + (ln & 48);
+    };
+    auto load_v = [&](const Rsrc& rs, int t, uint32_t off) {
+        const uint32_t at = off + (uint32_t)(16 * (t >> 2) + (t & 3)) * row_bytes;
+        vr[t][0] = __builtin_amdgcn_raw_buffer_load_b128(rs, at, 0, 0);
+        vr[t][1] = __builtin_amdgcn_raw_buffer_load_b128(rs, at + 256, 0, 0);
+    };
+    auto v_offset = [&]() {
+        const uint32_t ln = lane_now();
+        return (ln >> 4) * 4 * row_bytes + 16 * (ln & 15);
     };
     if (n_mine > 0) {
         const Rsrc rk = k_tile(0), rv = v_tile(0);
-        load_k(rk, 0);
-        load_k(rk, 1);
-        load_v(rv, 0);
-        load_v(rv, 1);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) load_k(rk, x, k_offset());
+#pragma unroll
+        for (int t = 0; t < 8; ++t) load_v(rv, t, v_offset());
     }
-    // q's planes, 8 values per thread: rows past the last repeat it
-    int q_fp32;
-    {
-        const int row = tid >> 4, d = 8 * (tid & 15), f = min(f0 + row, last), t0 = fdiv(f, fG);
-        const float* src = a.q + ((size_t)p.row0 + t0) * a.q_stride + (size_t)(kvh * G + f - t0 * G) * D + d;
-        float v[8];
-        *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
-        *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(src + 4);
-        float most = 0.f;
-        uint32_t h[4], m[4], l[4];
+    // q by the first rows' lanes; more than sixteen rows' through LDS (registers), [row][d]
+    int qpos[kBlocks];  // (rows past the last repeat it)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            v[j] *= sl2;
-            most = fmaxf(most, __builtin_fabsf(v[j]));
-        }
+    for (int rb = 0; rb < kBlocks; ++rb) qpos[rb] = p.pos0 + fdiv(min(f0 + kFewBlock * rb + j, last), fG);
+    auto q_row = [&](int f) {
+        const int tok = fdiv(f, fG);
+        return a.q + ((size_t)p.row0 + tok) * a.q_stride + (size_t)(kvh * G + f - tok * G) * D;
+    };
+    auto scaled = [&](const float4& v) { return f32x4{v.x * sl2, v.y * sl2, v.z * sl2, v.w * sl2}; };
+    f32x4 q[kBlocks == 1 ? 8 : 1];
+    if constexpr (kBlocks == 1) {
+        const float* src = q_row(min(f0 + j, last)) + 4 * quarter;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) split_pair(v[2 * j], v[2 * j + 1], h[j], m[j], l[j]);
-        char* dst = qpl + row * kKRowB + 2 * d;
-        *reinterpret_cast<u32x4*>(dst) = u32x4{h[0], h[1], h[2], h[3]};
-        *reinterpret_cast<u32x4*>(dst + kKPlane) = u32x4{m[0], m[1], m[2], m[3]};
-        *reinterpret_cast<u32x4*>(dst + 2 * kKPlane) = u32x4{l[0], l[1], l[2], l[3]};
-        q_fp32 = __syncthreads_or(!(most < 0x1p50f));  // (see wide_pass)
+        for (int x = 0; x < 8; ++x) q[x] = scaled(*reinterpret_cast<const float4*>(src + 16 * x));
+    } else {
+        const float* src = q_row(min(f0 + (tid >> 4), last)) + 8 * (tid & 15);
+        float* dst = smem + (tid >> 4) * kRowF + 8 * (tid & 15);
+        *reinterpret_cast<f32x4*>(dst) = scaled(*reinterpret_cast<const float4*>(src));
+        *reinterpret_cast<f32x4*>(dst + 4) = scaled(*reinterpret_cast<const float4*>(src + 4));
+        lds_barrier();
     }
-    auto q_frag = [&](int t) {
-        const char* q = qpl + col * kKRowB + 16 * hh + 32 * t;
-        return Planes{*reinterpret_cast<const u32x4*>(q), *reinterpret_cast<const u32x4*>(q + kKPlane),
-                      *reinterpret_cast<const u32x4*>(q + 2 * kKPlane)};
+    auto q_at = [&](int rb, int x) -> f32x4 {
+        if constexpr (kBlocks == 1) return q[x];
+        else return *reinterpret_cast<const f32x4*>(smem + (kFewBlock * rb + j) * kRowF + 16 * x + 4 * quarter);
     };
-    auto mul = [&](const Planes& x, const Planes& y, floatx16& c) {
-        c = mfma_bf16(x.l, y.h, c);
-        c = mfma_bf16(x.m, y.m, c);
-        c = mfma_bf16(x.m, y.h, c);
-        c = mfma_bf16(x.h, y.l, c);
-        c = mfma_bf16(x.h, y.m, c);
-        c = mfma_bf16(x.h, y.h, c);
-    };
-    // eight values' planes; one past kPlaneMax turns into NaN, which reaches a sum
-    auto planes_of = [&](const float (&v)[8]) {
-        uint32_t h[4], m[4], l[4];
-        float most = 0.f;
+    f32x4 o[kBlocks][8];
+    float m[kBlocks], l[kBlocks];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) most = fmaxf(most, __builtin_fabsf(v[j]));
-        const float v0 = most < kPlaneMax ? v[0] : __uint_as_float(0xFFFFFFFFu);
+    for (int rb = 0; rb < kBlocks; ++rb) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) split_pair(j ? v[2 * j] : v0, v[2 * j + 1], h[j], m[j], l[j]);
-        return Planes{u32x4{h[0], h[1], h[2], h[3]}, u32x4{m[0], m[1], m[2], m[3]}, u32x4{l[0], l[1], l[2], l[3]}};
-    };
-    Sums x;
-    x.clear();
+        for (int y = 0; y < 8; ++y) o[rb][y] = f32x4{0.f, 0.f, 0.f, 0.f};
+        m[rb] = -INFINITY;
+        l[rb] = 0.f;
+    }
     for (int i = 0; i < n_mine; ++i) {
         const bool more = i + 1 < n_mine;
-        const Rsrc rk = k_tile(more ? i + 1 : i), rv = v_tile(more ? i + 1 : i);
-        floatx16 s;
+        const int kt = index(i);
+        const Rsrc rk = k_tile(more ? i + 1 : i, more), rv = v_tile(more ? i + 1 : i, more);
+        f32x4 s[kBlocks][2];
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = 0.f;
+        for (int rb = 0; rb < kBlocks; ++rb) s[rb][0] = s[rb][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        const uint32_t off_k = k_offset();
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            f32x4 qx[kBlocks];
+#pragma unroll
+            for (int rb = 0; rb < kBlocks; ++rb) qx[rb] = q_at(rb, x);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int rb = 0; rb < kBlocks; ++rb)
+#pragma unroll
+                    for (int kb = 0; kb < 2; ++kb)
+                        s[rb][kb] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[kb][x][e]), qx[rb][e],
+                                                                         s[rb][kb], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            load_k(rk, x, off_k);
+        }
+#pragma unroll
+        for (int rb = 0; rb < kBlocks; ++rb) {
+            if (kt >= nfull) {
+                const int k0 = unhoisted(kt * kKT + 4 * quarter);
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (k0 + 16 * (r >> 2) + (r & 3) > qpos[rb]) s[rb][r >> 2][r & 3] = -INFINITY;
+            }
+            float mx = s[rb][0][0];
+#pragma unroll
+            for (int r = 1; r < 8; ++r) mx = fmaxf(mx, s[rb][r >> 2][r & 3]);
+            mx = half_max(fmaxf(mx, lane_xor16(mx)));
+            if (__builtin_amdgcn_ballot_w64(mx > m[rb] + kLazy)) {  // rare after the first tile
+                const float mn = fmaxf(m[rb], mx);
+                const float corr = m[rb] == mn ? 1.f : __builtin_amdgcn_exp2f(m[rb] - mn);
+                l[rb] *= corr;
+#pragma unroll
+                for (int y = 0; y < 8; ++y)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) o[rb][y][r] *= corr;
+                m[rb] = mn;
+            }
+            const float nb = m[rb] == -INFINITY ? 0.f : -m[rb];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                s[rb][r >> 2][r & 3] = __builtin_amdgcn_exp2f(s[rb][r >> 2][r & 3] + nb);
+                l[rb] += s[rb][r >> 2][r & 3];
+            }
+        }
+        const uint32_t off_v = v_offset();
 #pragma unroll
         for (int t = 0; t < 8; ++t) {
-            float v[8];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(kr[t >> 2][2 * (t & 3) + (j >> 2)][j & 3]);
-            mul(planes_of(v), q_frag(t), s);
-            if (more && (t == 3 || t == 7)) load_k(rk, t >> 2);
+            for (int rb = 0; rb < kBlocks; ++rb)
+#pragma unroll
+                for (int y = 0; y < 8; ++y)
+                    o[rb][y] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[t][y >> 2][y & 3]),
+                                                                    s[rb][t >> 2][t & 3], o[rb][y], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            load_v(rv, t, off_v);
         }
-        softmax_tile(x, s, index(i), nfull, qpos, hh);
+    }
+    // A sum that is not finite: an infinite value or NaN among the keys, seen by the row or not (the matrix
+    // instruction multiplies every row with every key, and 0 times infinity is NaN).  The wave then takes
+    // its tiles again, key by key: a lane has 32 products of its row's score and 32 columns of its sums.
+    {
+        float z = 0.f;
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-            const Planes pp = split_p(s, y);
+        for (int rb = 0; rb < kBlocks; ++rb) {
+            z = __builtin_fmaf(l[rb], 0.f, z);
 #pragma unroll
-            for (int db = 0; db < 4; ++db) {
-                float v[8];
+            for (int y = 0; y < 8; ++y)
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = __uint_as_float(vr[y][j][db]);
-                mul(planes_of(v), pp, x.o[db]);
+                for (int r = 0; r < 4; ++r) z = __builtin_fmaf(o[rb][y][r], 0.f, z);
+        }
+        if (__builtin_amdgcn_ballot_w64(z != 0.f)) {
+#pragma unroll
+            for (int rb = 0; rb < kBlocks; ++rb) {
+#pragma unroll
+                for (int y = 0; y < 8; ++y) o[rb][y] = f32x4{0.f, 0.f, 0.f, 0.f};
+                m[rb] = -INFINITY;
+                l[rb] = 0.f;
+#pragma unroll 1
+                for (int c = 0; c < n_mine * kKT; ++c) {
+                    const Rsrc rk = k_tile(c / kKT), rv = v_tile(c / kKT);
+                    const uint32_t row = (uint32_t)(c % kKT) * row_bytes;
+                    if (index(c / kKT) * kKT + c % kKT > qpos[rb]) continue;
+                    float dot = 0.f;
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) {
+                        const u32x4 k = __builtin_amdgcn_raw_buffer_load_b128(rk, row + 16 * quarter + 64 * x, 0, 0);
+                        const f32x4 qx = q_at(rb, x);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) dot = __builtin_fmaf(__uint_as_float(k[e]), qx[e], dot);
+                    }
+                    // (the four lanes of a row see the same keys: the exchange stays among active lanes)
+                    dot += lane_xor16(dot);
+                    dot += lane_xor32(dot);
+                    const float mn = fmaxf(m[rb], dot);
+                    const float corr = m[rb] == mn ? 1.f : __builtin_amdgcn_exp2f(m[rb] - mn);
+                    const float w = __builtin_amdgcn_exp2f(dot - (mn == -INFINITY ? 0.f : mn));
+                    m[rb] = mn;
+                    l[rb] = quarter == 0 ? l[rb] * corr + w : 0.f;  // (summed over the quarters below)
+#pragma unroll
+                    for (int x = 0; x < 8; ++x) {  // d = 64 (x/4) + 16 quarter + 4 (x%4) + e
+                        const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(
+                            rv, row + 64 * quarter + 256 * (x >> 2) + 16 * (x & 3), 0, 0);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            f32x4& sum = o[rb][4 * (x >> 2) + e];
+                            sum[x & 3] = __builtin_fmaf(w, __uint_as_float(v[e]), sum[x & 3] * corr);
+                        }
+                    }
+                }
             }
-            if (more) load_v(rv, y);
         }
     }
-    lds_barrier();  // q's planes have been read
-    float* const mine = smem + wu * (kQB * kRowF);
-    if (q_fp32 || planes_failed<true>(x, n_mine, v_tile, row_bytes, lane)) {
-        const int f = min(f0 + col, last), t0 = fdiv(f, fG);
-        const float* q_row = a.q + ((size_t)p.row0 + t0) * a.q_stride + (size_t)(kvh * G + f - t0 * G) * D;
-        redo_fp32<true>(x, a, p, q_row, sl2, n_mine, k_tile, v_tile, index, nfull, qpos, row_bytes, mine, lane);
-    }
-    // every wave's rows meet: O^T register r of quarter db is d = 4 (8(r/4) + 4hh + r%4) + db
+    // every wave's rows meet: register r of sum 4y + e is d = 64y + 16 quarter + 4r + e
+    if constexpr (kBlocks > 1) lds_barrier();  // q has been read
+    float* const mine = smem + wu * (kRows * kRowF);
+    float* const ml_at = smem + kFewML;
 #pragma unroll
-    for (int r = 0; r < 16; ++r)
-        *reinterpret_cast<float4*>(mine + col * kRowF + 4 * (8 * (r >> 2) + 4 * hh + (r & 3))) =
-            make_float4(x.o[0][r], x.o[1][r], x.o[2][r], x.o[3][r]);
-    const float l_row = half_sum(x.l);
-    if (hh == 0) *reinterpret_cast<float2*>(smem + kFewML + 2 * (wu * kQB + col)) = make_float2(x.m, l_row);
+    for (int rb = 0; rb < kBlocks; ++rb) {
+#pragma unroll
+        for (int x = 0; x < 8; ++x)
+            *reinterpret_cast<float4*>(mine + (kFewBlock * rb + j) * kRowF + 64 * (x >> 2) + 16 * quarter +
+                                       4 * (x & 3)) =
+                make_float4(o[rb][4 * (x >> 2)][x & 3], o[rb][4 * (x >> 2) + 1][x & 3], o[rb][4 * (x >> 2) + 2][x & 3],
+                            o[rb][4 * (x >> 2) + 3][x & 3]);
+        const float sum = half_sum(l[rb] + lane_xor16(l[rb]));
+        if (quarter == 0)
+            *reinterpret_cast<float2*>(ml_at + 2 * (wu * kRows + kFewBlock * rb + j)) = make_float2(m[rb], sum);
+    }
     lds_barrier();
     // two rows per wave and round, a lane four columns
-    const int rows = min(kQB, p.nflat - f0), d = 4 * col;
-    for (int row = 2 * wu + hh; row < rows; row += 2 * kWaves) {
-        float M = -INFINITY, L = 0.f, c[kWaves];
+    const int d = 4 * (lane & 31);
+    for (int row = 2 * wu + (lane >> 5); row < rows; row += 2 * kWaves) {
+        float M = -INFINITY, L = 0.f;
         float2 ml[kWaves];
 #pragma unroll
         for (int i = 0; i < kWaves; ++i) {
-            ml[i] = *reinterpret_cast<const float2*>(smem + kFewML + 2 * (i * kQB + row));
+            ml[i] = *reinterpret_cast<const float2*>(ml_at + 2 * (i * kRows + row));
             M = fmaxf(M, ml[i].x);
         }
-        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int i = 0; i < kWaves; ++i) {
-            c[i] = ml[i].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[i].x - M);
+            const float c = ml[i].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ml[i].x - M);
             // (a wave whose every score is NaN keeps m at -inf, and its NaN sum counts)
-            L += ml[i].x == -INFINITY ? ml[i].y : ml[i].y * c[i];
-            const float4 v = *reinterpret_cast<const float4*>(smem + (i * kQB + row) * kRowF + d);
-            o.x = __builtin_fmaf(c[i], v.x, o.x), o.y = __builtin_fmaf(c[i], v.y, o.y);
-            o.z = __builtin_fmaf(c[i], v.z, o.z), o.w = __builtin_fmaf(c[i], v.w, o.w);
+            L += ml[i].x == -INFINITY ? ml[i].y : ml[i].y * c;
+            const float4 v = *reinterpret_cast<const float4*>(smem + (i * kRows + row) * kRowF + d);
+            x.x = __builtin_fmaf(c, v.x, x.x), x.y = __builtin_fmaf(c, v.y, x.y);
+            x.z = __builtin_fmaf(c, v.z, x.z), x.w = __builtin_fmaf(c, v.w, x.w);
         }
-        const int f = f0 + row, t0 = fdiv(f, fG);
+        const int g = f0 + row, t0 = fdiv(g, fG);
         float* dst;
         if (p.part) {
             dst = p.part + row * D;
-            if (col == 0) *reinterpret_cast<float2*>(p.part + kFewRows * D + 2 * row) = make_float2(M, L);
+            if (d == 0) *reinterpret_cast<float2*>(p.part + kFewRows * D + 2 * row) = make_float2(M, L);
         } else {
-            dst = a.out + (((size_t)p.row0 + t0) * a.H + kvh * G + f - t0 * G) * D;
+            dst = a.out + (((size_t)p.row0 + t0) * a.H + kvh * G + g - t0 * G) * D;
             const float inv = p.pos0 + t0 < 0 ? 0.f : 1.f / L;  // a row that sees no key: zeros
-            o.x *= inv, o.y *= inv, o.z *= inv, o.w *= inv;
+            x.x *= inv, x.y *= inv, x.z *= inv, x.w *= inv;
         }
-        *reinterpret_cast<float4*>(dst + d) = o;
+        *reinterpret_cast<float4*>(dst + d) = x;
     }
 }
 
@@ -1019,8 +1118,10 @@ __device__ __forceinline__ void walk_list(const PackedArgs& a, int shares, float
         p.nrange = (cut >= 0 ? cut : scalar(x.tiles)) - p.kt_lo;
         p.part = p.kt_lo > 0 || cut >= 0 ? parts + part_at(kFew, blockIdx.x, p.kt_lo > 0 ? 0 : 1) : nullptr;
         if (pass > 0) lds_barrier();  // the last pass's rows have been read
-        if constexpr (kFew) few_pass<kPaged>(a, p, kvh, fG, sl2, smem);
-        else wide_pass<kPaged>(a, p, kvh, fG, sl2, smem);
+        if constexpr (kFew) {
+            if (p.nflat - kUnitRows * p.u <= kFewBlock) few_pass<kPaged, 1>(a, p, kvh, fG, sl2, smem);
+            else few_pass<kPaged, kFewRows / kFewBlock>(a, p, kvh, fG, sl2, smem);
+        } else wide_pass<kPaged>(a, p, kvh, fG, sl2, smem);
     }
 }
 

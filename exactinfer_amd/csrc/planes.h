@@ -40,6 +40,7 @@ __device__ __forceinline__ float uniform(float x) {  // a wave-uniform value, in
 // as none of them leaves bf16's range: from kPlaneMin up, where x's last bit is a normal bf16, to
 // bf16's largest value.  What lies outside is noticed and multiplied in fp32.
 typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
