@@ -310,10 +310,22 @@ __device__ __forceinline__ int row_owner(const int4* seq, int n_seq, int b, int 
 }
 
 // ------------------------------------------------------------------ attention
-// Both products on v_mfma_f32_32x32x16_bf16 with fp32 operands as three bf16 planes (planes.h), six
-// plane products each, as in prefill.hip, and with its wave layout: a wave holds 32 flat query rows,
-// computes S^T[key][row] = K . Q^T, so that each lane owns one row and 16 of a tile's 32 keys, and
-// O^T[d][row] = V^T . P^T from the same registers.  The softmax scale is multiplied into q.
+// Wide units multiply on v_mfma_f32_32x32x16_f16 with every fp32 operand in two binary16 planes, x = h + l:
+// h = f16(x) and l = f16(x - h), after a scaling by a power of two that brings the largest of its fellows
+// to 2^13 .. 2^15: the residual is exact, and l keeps it to 2^-22 of x (2^-24.6 in the root mean square)
+// or to 2^-25, 2^-39 of the largest, whichever is more.  Three of the four plane products are taken; l.l
+// is at most 2^-22 of |a||b|, 2^-23.6 in the root mean square.  Together that is about what fp32 loses in
+// adding 128 products, for half the matrix instructions of three bf16 planes (prefill.hip), which keep
+// every bit.  The scalings:
+//   q, with the softmax scale in it: per row, taken back in the exponent's FMA
+//   K: per key, taken back in the scores (16 products per tile and lane)
+//   V: per 32 columns, the running largest value of the tiles so far; sums are rescaled when it grows
+//   P: 2^14, so that weights of up to 2^kLazy fit (of one below 2^-39 nothing is left, at most that times
+//     the number of keys in all); the weights' sum has it too
+// What the scaling of V cannot hold is noticed at the end of a pass (planes_failed) and multiplied in fp32.
+//
+// A wave holds 32 flat query rows and computes S^T[key][row] = K . Q^T, so that each lane owns one row and
+// 16 of a tile's 32 keys, and O^T[d][row] = V^T . P^T from the same registers.
 //
 // A workgroup of eight waves walks its share of a list pass by pass: a pass is a unit, or the part of it
 // between two cuts of the list's line.  A part goes unnormalised to the workspace.
@@ -335,24 +347,29 @@ constexpr int kQB = 32;                         // flat rows per wave
 constexpr int kSlots = kUnitRows / kQB;         // waves per key group
 constexpr int kGroups = 2;                      // key groups per workgroup
 constexpr int kWaves = kSlots * kGroups;
-constexpr float kLazy = 8.f;                    // lazy-rescale threshold (log2 units)
+// lazy-rescale thresholds (log2 units): sums are rescaled when the running maximum has risen by more (for
+// wide units, what a weight may pass 1 by comes off the range of its planes)
+constexpr float kLazy = 1.f, kFewLazy = 8.f;
+constexpr float kPBits = 14.f;                  // wide units' weights and sums are times 2^kPBits
 constexpr int kXchF = 34;                       // floats per lane exchanged by the merge
 constexpr int kRowF = kHeadDim + 4;             // padded fp32 row of the staging area
 // plane rows padded to an odd number of 16-byte pieces: the rows that an operand read takes, one per
 // lane, spread over all LDS banks
-constexpr int kKRowB = 2 * kHeadDim + 16, kKPlane = kKT * kKRowB;  // K plane: [32 keys][128 d] bf16
+constexpr int kKRowB = 2 * kHeadDim + 16, kKPlane = kKT * kKRowB;  // K plane: [32 keys][128 d] binary16
 constexpr int kVRowB = 2 * kKT + 16, kVPlane = kHeadDim * kVRowB;  // V plane, transposed: [128 d][32 keys]
 // LDS of a wide pass: the K planes of both groups, and the merge's exchange area, from 0; the V planes
-// after it, and over them the staging area of the unit's rows (queries, later outputs).  Of a few-rows
-// pass: every wave's rows, and their (m, l).
+// after it, and over them the staging area of the unit's rows (queries, later outputs); then the scalings,
+// of K [group][tile parity][key] and of V [group][32 columns].  Of a few-rows pass: every wave's rows, and
+// their (m, l).
 constexpr int kStageF = kWaves * kXchF * 64;
-constexpr int kWideF = kStageF + kUnitRows * kRowF;
+constexpr int kScaleK = kStageF + kUnitRows * kRowF, kScaleV = kScaleK + kGroups * 2 * kKT;
+constexpr int kWideF = kScaleV + kGroups * 4;
 constexpr int kFewBlock = 16;                   // rows of one matrix instruction of few_pass
 constexpr int kFewML = kWaves * kFewRows * kRowF;
 constexpr int kFewF = kFewML + kWaves * kFewRows * 2;
 static_assert(kWaves * 64 == kFewRows * 16, "sixteen threads stage a row");
-static_assert(kGroups * 3 * kKPlane <= kStageF * 4, "K planes below the staging area");
-static_assert(kStageF * 4 + kGroups * 3 * kVPlane <= kWideF * 4, "V planes within the LDS span");
+static_assert(kGroups * 2 * kKPlane <= kStageF * 4, "K planes below the staging area");
+static_assert(kStageF * 4 + kGroups * 2 * kVPlane <= kScaleK * 4, "V planes within the LDS span");
 static_assert(kWideF * 4 <= 160 * 1024 && kFewF * 4 <= 160 * 1024, "LDS budget");
 
 __device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
@@ -414,9 +431,9 @@ struct Sums {  // of 32 rows, one per lane and its lane ^ 32: O^T, running maxim
     }
 };
 
-// Scores s of tile kt -> P (in place), the running maximum and sum, O rescaled if the maximum rose by
-// more than kLazy.  Tiles from nfull on cross the diagonal of the wave's rows.
-__device__ __forceinline__ void softmax_tile(Sums& x, floatx16& s, int kt, int nfull, int qpos, int hh) {
+// Scores s of tile kt (times sq: log2 units) -> 2^kPBits P (in place), the running maximum and sum, O rescaled
+// if the maximum rose by more than kLazy.  Tiles from nfull on cross the diagonal of the wave's rows.
+__device__ __forceinline__ void softmax_tile(Sums& x, floatx16& s, float sq, int kt, int nfull, int qpos, int hh) {
     if (kt >= nfull) {
         const int k0 = unhoisted(kt * kKT + 4 * hh);
 #pragma unroll
@@ -426,7 +443,7 @@ __device__ __forceinline__ void softmax_tile(Sums& x, floatx16& s, int kt, int n
     float mx = s[0];
 #pragma unroll
     for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-    const float ms = half_max(mx);
+    const float ms = half_max(mx) * sq;
     if (__builtin_amdgcn_ballot_w64(ms > x.m + kLazy)) {  // rare after the first tile
         const float mn = fmaxf(x.m, ms);
         const float corr = x.m == mn ? 1.f : __builtin_amdgcn_exp2f(x.m - mn);
@@ -437,73 +454,73 @@ __device__ __forceinline__ void softmax_tile(Sums& x, floatx16& s, int kt, int n
             for (int r = 0; r < 16; ++r) x.o[db][r] *= corr;
         x.m = mn;
     }
-    const float nb = x.m == -INFINITY ? 0.f : -x.m;
+    const float nb = x.m == -INFINITY ? 0.f : kPBits - x.m;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
-        s[r] = __builtin_amdgcn_exp2f(s[r] + nb);
+        s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sq, nb));
         x.l += s[r];
     }
 }
 
+// ---- two binary16 planes
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+struct Halves {  // eight values: one MFMA operand per plane
+    u32x4 h, l;
+};
+__device__ __forceinline__ void split_f16(float a, float b, uint32_t& h, uint32_t& l) {
+    h = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
+    float ra, rb;  // a - h's low half, b - its high half, in one instruction each
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(ra) : "v"(h), "v"(a));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(rb) : "v"(h), "v"(b));
+    l = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{ra, rb}, f16x2));
+}
+__device__ __forceinline__ floatx16 mfma_f16(u32x4 a, u32x4 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                  0);
+}
+__device__ __forceinline__ void mfma_halves(const Halves& a, const Halves& b, floatx16& c) {
+    c = mfma_f16(a.l, b.h, c);
+    c = mfma_f16(a.h, b.l, c);
+    c = mfma_f16(a.h, b.h, c);
+}
+// The power of two that brings `most` to 2^kTop .. 2^(kTop+1), and its inverse: `most`'s exponent is kept
+// where both are normal numbers.
+template <int kTop>
+__device__ __forceinline__ uint32_t scale_to(float most) {
+    const uint32_t e = min(max(__float_as_uint(most) >> 23, kTop + 2u), 254u);
+    return (254u + kTop - e) << 23;
+}
+__device__ __forceinline__ float inverse(uint32_t scale) { return __uint_as_float(0x7F000000u - scale); }
+constexpr uint32_t kNoScale = 253u << 23;  // of columns that have been zero so far
+
 // The planes of P's half x (registers 8x .. 8x + 7): the B operand of two steps' worth of keys.
-__device__ __forceinline__ Planes split_p(const floatx16& s, int x) {
-    uint32_t h[4], m[4], l[4];
+__device__ __forceinline__ Halves split_p(const floatx16& s, int x) {
+    uint32_t h[4], l[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) split_pair(s[8 * x + 2 * j], s[8 * x + 2 * j + 1], h[j], m[j], l[j]);
-    return {u32x4{h[0], h[1], h[2], h[3]}, u32x4{m[0], m[1], m[2], m[3]}, u32x4{l[0], l[1], l[2], l[3]}};
+    for (int j = 0; j < 4; ++j) split_f16(s[8 * x + 2 * j], s[8 * x + 2 * j + 1], h[j], l[j]);
+    return {u32x4{h[0], h[1], h[2], h[3]}, u32x4{l[0], l[1], l[2], l[3]}};
 }
 
-// Whether planes did not serve a wave's sums (prefill.hip has the same rule): an infinite value, or one
-// past kPlaneMax, in K or V shows as a sum that is not finite.  A V value or a weight below kPlaneMin
-// may have lost bits of its third plane, 2^-134, which shows in no sum from kSmallSum up; with a
-// smaller one the wave looks through its V tiles, in the quarters of the columns with such a sum: it
-// stands if no V value there is below kPlaneMin and the largest one is too small for the weights' 2^-134
-// to show in it.  v_tile(i) is the wave's i-th tile.
-template <typename Tile>
-__device__ __forceinline__ bool planes_failed(const Sums& x, int n_mine, Tile v_tile, uint32_t row_bytes, int lane) {
-    float z = x.l * 0.f, least[4];
+// Takes V's scalings out of the sums, and says whether the planes did not serve them: a sum is not finite (an
+// infinite value or NaN in K or V, seen by the row or not), or a row's sums are so small, against V's
+// largest values on the way and the sum of weights, that the 2^-25 which planes keep of scaled values may
+// show (2^-22 of the row's largest sum).
+__device__ __forceinline__ bool planes_failed(Sums& x, const uint32_t (&scale)[4]) {
+    float z = x.l * 0.f, most = 0.f, step = 0.f;
 #pragma unroll
     for (int db = 0; db < 4; ++db) {
-        least[db] = INFINITY;
+        const float inv = scale[db] == kNoScale ? 0.f : inverse(scale[db]);
+        step = fmaxf(step, inv);
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             z = __builtin_fmaf(x.o[db][r], 0.f, z);
-            least[db] = fminf(least[db], __builtin_fabsf(x.o[db][r]));
+            x.o[db][r] *= inv;
+            most = fmaxf(most, __builtin_fabsf(x.o[db][r]));
         }
     }
-    if (__builtin_amdgcn_ballot_w64(z != 0.f)) return true;
-    const float least_all = fminf(fminf(least[0], least[1]), fminf(least[2], least[3]));
-    // (a lane without a visible key has no sum: m stays -inf)
-    if (!__builtin_amdgcn_ballot_w64(least_all < kSmallSum && x.m != -INFINITY)) return false;
-    uint32_t small = 0xFFFFFFFFu, tiny = 0xFFFFFFFFu;  // the smallest nonzero sum and V value
-    if (x.m != -INFINITY) {
-#pragma unroll
-        for (int db = 0; db < 4; ++db)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) small = min(small, magnitude(__float_as_uint(x.o[db][r])));
-    }
-    float most = 0.f;
-#pragma unroll
-    for (int db = 0; db < 4; ++db) {
-        if (!__builtin_amdgcn_ballot_w64(least[db] < kSmallSum && x.m != -INFINITY)) continue;
-        for (int i = 0; i < n_mine; ++i) {
-            const Rsrc rs = v_tile(i);
-            const int ln = unhoisted(lane);
-            const uint32_t off = (ln >> 3) * row_bytes + 16u * (ln & 7) + 128u * db;
-#pragma unroll
-            for (int j = 0; j < kKT / 8; ++j) {
-                const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(rs, off + 8 * j * row_bytes, 0, 0);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    tiny = min(tiny, magnitude(v[e]));
-                    most = fmaxf(most, __builtin_fabsf(__uint_as_float(v[e])));
-                }
-            }
-        }
-    }
-    // the sums are off by up to 2^20 2^-134 most; a lane without a nonzero one has nothing to lose
-    const float limit = wave_max(most) * 0x1p-84f;
-    return __builtin_amdgcn_ballot_w64(tiny < kTinyMagnitude || limit > of_magnitude(small)) != 0;
+    const float l = half_sum(x.l);
+    return __builtin_amdgcn_ballot_w64(z != 0.f || l * step * 0x1p-25f > half_max(most) * 0x1p-22f) != 0;
 }
 
 // A wave's tiles again, both products in fp32 from the cache.  In a tile that crosses the diagonal a
@@ -542,7 +559,7 @@ __device__ __forceinline__ void redo_fp32(Sums& x, const PackedArgs& a, const Pa
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        softmax_tile(x, s, kt, nfull, qpos, hh);
+        softmax_tile(x, s, 1.f, kt, nfull, qpos, hh);
         const Rsrc rs = v_tile(i);
         if (kt < nfull) {
             const uint32_t off = unhoisted(4 * hh) * row_bytes + 4u * col;
@@ -597,9 +614,11 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
     const int G = (int)fG.d;
     const uint32_t row_bytes = (uint32_t)(a.kv_stride * 4);
     char* const lds = reinterpret_cast<char*>(smem);
-    char* const kpl = lds + grp * 3 * kKPlane;
-    char* const vpl = lds + kStageF * 4 + grp * 3 * kVPlane;
+    char* const kpl = lds + grp * 2 * kKPlane;
+    char* const vpl = lds + kStageF * 4 + grp * 2 * kVPlane;
     float* const stage = smem + kStageF;
+    float* const k_scale = smem + kScaleK + grp * 2 * kKT;
+    uint32_t* const v_scale = reinterpret_cast<uint32_t*>(smem + kScaleV) + grp * 4;
     const uint32_t voff_k = (uint32_t)(8 * hw + (lane >> 3)) * row_bytes + 32u * (lane & 7);
     const uint32_t voff_v =
         (uint32_t)(16 * (lane >> 5) + 4 * ((lane >> 4) & 1)) * row_bytes + 4u * (32 * hw + 2 * (lane & 15));
@@ -635,41 +654,59 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
             rg[2 * j] = __uint_as_float(v.x), rg[2 * j + 1] = __uint_as_float(v.y);
         }
     };
-    // a value of rg past kPlaneMax turns one of them into NaN, which reaches a sum of every wave that
-    // multiplies it
-    auto check_planes = [&]() {
+    auto largest = [&]() {
         float most = 0.f;
 #pragma unroll
         for (int j = 0; j < 16; ++j) most = fmaxf(most, __builtin_fabsf(rg[j]));
-        rg[0] = most < kPlaneMax ? rg[0] : __uint_as_float(0xFFFFFFFFu);
+        return most;
     };
-    // half x of the conversion of rg: eight values, one 16-byte piece of each plane
-    auto conv_k = [&](int x) {
-        uint32_t ch[4], cm[4], cl[4];
-        if (x == 0) check_planes();
+    // half x of the conversion of rg, eight values, one 16-byte piece of each plane; the first half finds the
+    // scaling: of K the row's, of V the running one of the wave's 32 columns (four times its largest value
+    // fits, so it changes rarely)
+    float fk;
+    auto conv_k = [&](int x, int parity) {
+        uint32_t ch[4], cl[4];
+        if (x == 0) {
+            float most = largest();
+            most = fmaxf(most, lane_xor1(most));
+            most = fmaxf(most, lane_xor2(most));
+            most = fmaxf(most, lane_xor4(most));
+            const uint32_t f = scale_to<14>(most);
+            fk = __uint_as_float(f);
+            if ((lane & 7) == 0) k_scale[kKT * parity + 8 * hw + (lane >> 3)] = inverse(f);
+        }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) split_pair(rg[8 * x + 2 * j], rg[8 * x + 2 * j + 1], ch[j], cm[j], cl[j]);
+        for (int j = 0; j < 4; ++j) split_f16(rg[8 * x + 2 * j] * fk, rg[8 * x + 2 * j + 1] * fk, ch[j], cl[j]);
         char* d = kpl + (8 * hw + (lane >> 3)) * kKRowB + 16 * (lane & 7) + 128 * x;
         *reinterpret_cast<u32x4*>(d) = u32x4{ch[0], ch[1], ch[2], ch[3]};
-        *reinterpret_cast<u32x4*>(d + kKPlane) = u32x4{cm[0], cm[1], cm[2], cm[3]};
-        *reinterpret_cast<u32x4*>(d + 2 * kKPlane) = u32x4{cl[0], cl[1], cl[2], cl[3]};
+        *reinterpret_cast<u32x4*>(d + kKPlane) = u32x4{cl[0], cl[1], cl[2], cl[3]};
     };
+    uint32_t fv = kNoScale;
+    float limit = 0.f;
     auto conv_v = [&](int x) {  // d + x
-        uint32_t ch[4], cm[4], cl[4];
-        if (x == 0) check_planes();
+        uint32_t ch[4], cl[4];
+        if (x == 0) {
+            const float most = largest();
+            if (__builtin_amdgcn_ballot_w64(most > limit)) {
+                fv = scalar(scale_to<13>(wave_max(most)));
+                limit = uniform(65000.f * inverse(fv));
+            }
+            if (lane == 0) v_scale[hw] = fv;
+        }
+        const float f = __uint_as_float(fv);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) split_pair(rg[4 * j + x], rg[4 * j + 2 + x], ch[j], cm[j], cl[j]);
+        for (int j = 0; j < 4; ++j) split_f16(rg[4 * j + x] * f, rg[4 * j + 2 + x] * f, ch[j], cl[j]);
         char* d = vpl + (32 * hw + 2 * (lane & 15) + x) * kVRowB + 16 * (lane >> 4);
         *reinterpret_cast<u32x4*>(d) = u32x4{ch[0], ch[1], ch[2], ch[3]};
-        *reinterpret_cast<u32x4*>(d + kVPlane) = u32x4{cm[0], cm[1], cm[2], cm[3]};
-        *reinterpret_cast<u32x4*>(d + 2 * kVPlane) = u32x4{cl[0], cl[1], cl[2], cl[3]};
+        *reinterpret_cast<u32x4*>(d + kVPlane) = u32x4{cl[0], cl[1], cl[2], cl[3]};
     };
-    auto k_frag = [&](int t, int plane) {  // K[key col][16t + 8hh ..]
-        return *reinterpret_cast<const u32x4*>(kpl + col * kKRowB + 16 * hh + 32 * t + plane * kKPlane);
+    auto k_frag = [&](int t) {  // K[key col][16t + 8hh ..]
+        const char* k = kpl + col * kKRowB + 16 * hh + 32 * t;
+        return Halves{*reinterpret_cast<const u32x4*>(k), *reinterpret_cast<const u32x4*>(k + kKPlane)};
     };
-    auto v_frag = [&](int x, int plane) {  // step s = x/4, d = 32 (x%4) + col
-        return *reinterpret_cast<const u32x4*>(vpl + (32 * (x & 3) + col) * kVRowB + 32 * (x >> 2) + 16 * hh +
-                                               plane * kVPlane);
+    auto v_frag = [&](int x) {  // step s = x/4, d = 32 (x%4) + col
+        const char* v = vpl + (32 * (x & 3) + col) * kVRowB + 32 * (x >> 2) + 16 * hh;
+        return Halves{*reinterpret_cast<const u32x4*>(v), *reinterpret_cast<const u32x4*>(v + kVPlane)};
     };
 
     // the unit's query rows by LDS DMA, once for both groups: wave wu rows 16*wu .. of the unit
@@ -697,36 +734,40 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
     if (n_mine > 0) load_k(0);
     wait_vmcnt<0>();
     lds_barrier();
-    Planes qp[8];
-    // a score on planes is off by at most 2^-134 (|q| + |k|) per element, 2^-77 with K below kPlaneMax and
-    // q below 2^50; a wave with a q element past that takes its tiles in fp32 after the key loop
-    uint64_t q_fp32;
+    Halves qp[8];
+    float sq;  // takes the row's scaling out of its scores
     {
         const float* qs = stage + (hw * kQB + col) * kRowF + 8 * hh;
         float most = 0.f;
 #pragma unroll
-        for (int t = 0; t < 8; ++t) {
-            float4 x = *reinterpret_cast<const float4*>(qs + 16 * t);
-            float4 y = *reinterpret_cast<const float4*>(qs + 16 * t + 4);
-            x.x *= sl2, x.y *= sl2, x.z *= sl2, x.w *= sl2, y.x *= sl2, y.y *= sl2, y.z *= sl2, y.w *= sl2;
-#pragma unroll
-            for (const float f : {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w}) most = fmaxf(most, __builtin_fabsf(f));
-            uint32_t h[4], m[4], l[4];
-            split_pair(x.x, x.y, h[0], m[0], l[0]);
-            split_pair(x.z, x.w, h[1], m[1], l[1]);
-            split_pair(y.x, y.y, h[2], m[2], l[2]);
-            split_pair(y.z, y.w, h[3], m[3], l[3]);
-            qp[t] = {u32x4{h[0], h[1], h[2], h[3]}, u32x4{m[0], m[1], m[2], m[3]}, u32x4{l[0], l[1], l[2], l[3]}};
+        for (int t = 0; t < 16; ++t) {
+            const float4 v = *reinterpret_cast<const float4*>(qs + 16 * (t >> 1) + 4 * (t & 1));
+            most = fmaxf(fmaxf(most, __builtin_fabsf(v.x * sl2)), __builtin_fabsf(v.y * sl2));
+            most = fmaxf(fmaxf(most, __builtin_fabsf(v.z * sl2)), __builtin_fabsf(v.w * sl2));
         }
-        q_fp32 = __builtin_amdgcn_ballot_w64(!(most < 0x1p50f));
+        const uint32_t f = scale_to<14>(half_max(most));
+        const float fq = __uint_as_float(f);
+        sq = inverse(f);
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+            const float4 u = *reinterpret_cast<const float4*>(qs + 16 * t);
+            const float4 v = *reinterpret_cast<const float4*>(qs + 16 * t + 4);
+            uint32_t h[4], l[4];
+            split_f16(u.x * sl2 * fq, u.y * sl2 * fq, h[0], l[0]);
+            split_f16(u.z * sl2 * fq, u.w * sl2 * fq, h[1], l[1]);
+            split_f16(v.x * sl2 * fq, v.y * sl2 * fq, h[2], l[2]);
+            split_f16(v.z * sl2 * fq, v.w * sl2 * fq, h[3], l[3]);
+            qp[t] = {u32x4{h[0], h[1], h[2], h[3]}, u32x4{l[0], l[1], l[2], l[3]}};
+        }
     }
     if (n_mine > 0) {
 #pragma unroll
-        for (int x = 0; x < 2; ++x) conv_k(x);
+        for (int x = 0; x < 2; ++x) conv_k(x, 0);
         load_v(0);
     }
     Sums x;
     x.clear();
+    uint32_t scale[4] = {kNoScale, kNoScale, kNoScale, kNoScale};  // V's, as the sums have it
     lds_barrier();  // every wave has its q (the staging area is free for the V planes); K planes stored
     if (grp == 1) lds_barrier();
     for (int i = 0; i < n_it; ++i) {
@@ -735,28 +776,47 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
             // S^T = K . Q^T, while V(i) goes to its planes; then K(i+1) is fetched
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = 0.f;
-            Planes kf;
-            kf.l = k_frag(0, 2), kf.m = k_frag(0, 1), kf.h = k_frag(0, 0);
+            Halves kf[2];
+            kf[0] = k_frag(0);
 #pragma unroll
             for (int t = 0; t < 8; ++t) {
-                if (t == 4 || t == 6) conv_v(t == 6);
-                mfma_split(kf, qp[t], s, [&](int pl) { return t < 7 ? k_frag(t + 1, pl) : u32x4{}; });
+                if (t < 7) kf[(t + 1) & 1] = k_frag(t + 1);
+                if (t == 2 || t == 4) conv_v(t == 4);
+                mfma_halves(kf[t & 1], qp[t], s);
             }
             if (i + 1 < n_mine) load_k(i + 1);
+            const float* ks = k_scale + kKT * (i & 1) + 4 * hh;
+#pragma unroll
+            for (int r = 0; r < 16; r += 4) {
+                const float4 f = *reinterpret_cast<const float4*>(ks + 2 * r);
+                s[r] *= f.x, s[r + 1] *= f.y, s[r + 2] *= f.z, s[r + 3] *= f.w;
+            }
         }
         lds_barrier();
         if (i < n_mine) {
             __builtin_amdgcn_s_setprio(1);
-            softmax_tile(x, s, index(i), nfull, qpos, hh);
+            const u32x4 f = *reinterpret_cast<const u32x4*>(v_scale);
+#pragma unroll
+            for (int db = 0; db < 4; ++db) {
+                const uint32_t now = scalar(f[db]);
+                if (now != scale[db]) {  // rare after the first tile
+                    const float by = __uint_as_float(now) * inverse(scale[db]);
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) x.o[db][r] *= by;
+                    scale[db] = now;
+                }
+            }
+            softmax_tile(x, s, sq, index(i), nfull, qpos, hh);
             // O^T += V^T . P^T, while K(i+1) goes to its planes; then V(i+1) is fetched
             const bool more = i + 1 < n_mine;
-            Planes vf, pp;
-            vf.l = v_frag(0, 2), vf.m = v_frag(0, 1), vf.h = v_frag(0, 0);
+            Halves vf[2], pp;
+            vf[0] = v_frag(0);
 #pragma unroll
             for (int y = 0; y < 8; ++y) {
                 if ((y & 3) == 0) pp = split_p(s, y >> 2);
-                if (y == 4 || y == 6) conv_k(y == 6);
-                mfma_split(vf, pp, x.o[y & 3], [&](int pl) { return y < 7 ? v_frag(y + 1, pl) : u32x4{}; });
+                if (y < 7) vf[(y + 1) & 1] = v_frag(y + 1);
+                if (y == 4 || y == 6) conv_k(y == 6, (i + 1) & 1);
+                mfma_halves(vf[y & 1], pp, x.o[y & 3]);
             }
             if (more) load_v(i + 1);
             __builtin_amdgcn_s_setprio(0);
@@ -765,11 +825,11 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
     }
     if (grp == 0) lds_barrier();
 
-    if (live && (q_fp32 || planes_failed(x, n_mine, v_tile, row_bytes, lane))) {
+    if (planes_failed(x, scale) && live) {
         const int f = min(f0 + col, p.nflat - 1), t0 = fdiv(f, fG);
         const float* q_row = a.q + ((size_t)p.row0 + t0) * a.q_stride + (size_t)(kvh * G + f - t0 * G) * D;
         redo_fp32(x, a, p, q_row, sl2, n_mine, k_tile, v_tile, index, nfull, qpos, row_bytes,
-                         smem + w * (kXchF * 64), lane);
+                  smem + w * (kXchF * 64), lane);
     }
 
     // ---- the key groups meet through LDS (tile buffers are free after the barrier): group g finishes
@@ -946,7 +1006,7 @@ __device__ __forceinline__ void few_pass(const PackedArgs& a, const Pass& p, int
 #pragma unroll
             for (int r = 1; r < 8; ++r) mx = fmaxf(mx, s[rb][r >> 2][r & 3]);
             mx = half_max(fmaxf(mx, lane_xor16(mx)));
-            if (__builtin_amdgcn_ballot_w64(mx > m[rb] + kLazy)) {  // rare after the first tile
+            if (__builtin_amdgcn_ballot_w64(mx > m[rb] + kFewLazy)) {  // rare after the first tile
                 const float mn = fmaxf(m[rb], mx);
                 const float corr = m[rb] == mn ? 1.f : __builtin_amdgcn_exp2f(m[rb] - mn);
                 l[rb] *= corr;
