@@ -18,12 +18,13 @@ constexpr int kFewRows = 32;    // units of up to so many rows go to k_packed_fe
 // prompts), goes to the list of few-row units, the others to the wide list.
 //
 // `shares` workgroups serve each KV head, all heads alike, and take the same cost each: a unit's causal key
-// tiles, and something for what is done once per unit.  Few-row units are laid end to end on a line
-// and the line cut evenly.  Of the wide list each workgroup first takes whole units, dealt out in
-// descending order of tiles and back and forth, round by round, so that the workgroups walk units of
-// about the same keys at the same time (their tiles meet in the XCD's L2); the last units (the
-// smallest: one to two rounds of them, or all if there are fewer) form a line, of which each gets what
-// is missing to an equal share.  A cut may fall inside a unit: its parts are merged by k_packed_combine.
+// tiles, and something for what is done once per unit.  Of the wide list each workgroup first takes whole
+// units, dealt out in descending order of tiles and back and forth, round by round, so that the
+// workgroups walk units of about the same keys at the same time (their tiles meet in the XCD's L2); the
+// last units (the smallest: one to two rounds of them, or all if there are fewer) are laid end to end on
+// a line, of which each gets what is missing to an equal share.  The few-row units lie on a line of their
+// own, of which each workgroup gets what its wide work leaves of an equal share of everything.  A cut may
+// fall inside a unit: its parts are merged by k_packed_combine.
 //
 // Order and cuts follow from the lengths alone (no atomics decide them), so a batch planned twice
 // gives the same bits twice.
@@ -124,10 +125,11 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
                                                               int max_kv, int H, int HKV, int shares,
                                                               char* __restrict__ plan) {
     __shared__ int4 seq_lds[kPlanSeqLds];
-    __shared__ int line_lds[kPlanLineLds];
+    __shared__ int wide_lds[kPlanLineLds], few_lds[kPlanLineLds];  // tiles of the lines' units
     __shared__ unsigned long long load[kPackedCus], few_cost, wide_cost;
     __shared__ long long cut_at[kPackedCus + 1];
     __shared__ int2 cuts[kPackedCus + 1];
+    __shared__ long long cut_cost[kPackedCus + 1];  // the line's cost before each cut
     const int tid = threadIdx.x, G = H / HKV;
     const PlanView pv = plan_view(plan, n_seq, rows, G, shares);
     // keys that rows up to `row` of a sequence of n rows and len keys see, in tiles
@@ -139,7 +141,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
     auto cut_line = [&](const List& list, int rounds, int line, ListCost c, const int* lds, long long share) {
         const int dealt = rounds * shares;
         const int keep = max(c.turn, min(c.pass, (int)min(share / 2, (long long)c.pass)));
-        if (tid <= shares) cuts[tid] = make_int2(tid == 0 ? 0 : line, 0);
+        if (tid <= shares) cuts[tid] = make_int2(tid == 0 ? 0 : line, 0), cut_cost[tid] = tid == 0 ? 0 : -1;
         __syncthreads();
         long long at = 0;
         for (int base = 0; base < line; base += kPlanThreads) {
@@ -158,11 +160,13 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
                 for (; lo < shares && cut_at[lo] < a + cost; ++lo) {
                     const long long t = (cut_at[lo] - a) / c.turn * c.turn;
                     cuts[lo] = t + keep > tiles ? make_int2(i + 1, 0) : make_int2(i, t < keep ? 0 : (int)t);
+                    cut_cost[lo] = a + (t + keep > tiles ? cost : t < keep ? 0 : t);
                 }
             }
             at += sum;
         }
         __syncthreads();
+        if (tid <= shares && cut_cost[tid] < 0) cut_cost[tid] = at;  // past the line's end
         if (tid < shares) {
             const int2 from = cuts[tid], to = cuts[tid + 1];
             Share& x = list.shares[tid];
@@ -208,7 +212,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
         if (is_few) {
             const int i = (int)(few + (at & 0xFFFFFFFF));
             pv.few.units[i] = Unit{lo, n, len, nw, s, tiles, {0, 0}};
-            if (i < kPlanLineLds) line_lds[i] = tiles;
+            if (i < kPlanLineLds) few_lds[i] = tiles;
         }
         const long long cost = wave_scan(is_few ? tiles + kFewCost.pass : 0);
         if ((tid & 63) == 63 && cost > 0) atomicAdd(&few_cost, (unsigned long long)cost);
@@ -218,12 +222,6 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
     if (bad) units = few = 0;
     const int U = (int)units;
     __syncthreads();
-    {
-        const long long share = few > 0 ? ((long long)few_cost + shares - 1) / shares : 0;
-        if (tid <= shares) cut_at[tid] = tid * share;
-        cut_line(pv.few, 0, (int)few, kFewCost, few <= kPlanLineLds ? line_lds : nullptr, share);
-    }
-
     const bool in_lds = n_seq <= kPlanSeqLds;
     auto seq_at = [&](int s) { return in_lds ? seq_lds[s] : pv.seq[s]; };
     auto unit = [&](int i) {
@@ -266,17 +264,26 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
         if (at < dealt) {
             const int r = at / shares, j = at - r * shares;
             atomicAdd(&load[(r & 1) ? shares - 1 - j : j], (unsigned long long)(x.tiles + kWideCost.pass));
-        } else if (at - dealt < kPlanLineLds) line_lds[at - dealt] = x.tiles;
+        } else if (at - dealt < kPlanLineLds) wide_lds[at - dealt] = x.tiles;
     }
     mine = wave_scan(mine);
     if ((tid & 63) == 63 && mine > 0) atomicAdd(&wide_cost, (unsigned long long)mine);
     __syncthreads();
     {
-        const long long share = U > 0 ? ((long long)wide_cost + shares - 1) / shares : 0;
+        const long long share = ((long long)wide_cost + shares - 1) / shares;
         long long before = tid * share, all;
         if (rounds > 0) before = block_scan(tid < shares ? max(share - (long long)load[tid], 0LL) : 0, &all);
         if (tid <= shares) cut_at[tid] = before;
-        cut_line(pv.wide, rounds, line, kWideCost, line <= kPlanLineLds ? line_lds : nullptr, share);
+        cut_line(pv.wide, rounds, line, kWideCost, line <= kPlanLineLds ? wide_lds : nullptr, share);
+    }
+    {
+        const long long share = ((long long)few_cost + shares - 1) / shares;
+        const long long both = ((long long)(wide_cost + few_cost) + shares - 1) / shares;
+        const long long wide = tid < shares ? (long long)load[tid] + cut_cost[tid + 1] - cut_cost[tid] : 0;
+        long long all;
+        const long long before = block_scan(tid < shares ? max(both - wide, 0LL) : 0, &all);
+        if (tid <= shares) cut_at[tid] = before;
+        cut_line(pv.few, 0, (int)few, kFewCost, few <= kPlanLineLds ? few_lds : nullptr, share);
     }
     if (tid == 0) {
         int* h = reinterpret_cast<int*>(plan);
@@ -1142,18 +1149,14 @@ __device__ __forceinline__ void few_pass(const PackedArgs& a, const Pass& p, int
     }
 }
 
-// Workgroup (share, KV head) walks its part of the wide list, or of the few-row one.
+// A workgroup's part of a list: `sh` its share of the line (first unit, first tile, last unit, last tile), before
+// it `rounds` whole units.
 template <bool kPaged, bool kFew>
-__device__ __forceinline__ void walk_list(const PackedArgs& a, int shares, float* parts, float* smem) {
-    const int kvh = blockIdx.x % a.HKV, share = blockIdx.x / a.HKV;  // a KV head's workgroups share an XCD's L2
+__device__ __forceinline__ void walk_list(const PackedArgs& a, const List& list, int4 sh, int rounds, int shares,
+                                          int share, int kvh, float* parts, float* smem) {
     const FastDiv fG = fast_div((uint32_t)(a.H / a.HKV));
     const float sl2 = a.scale * 1.44269504088896340736f;  // scores come out in log2 units
-    const PlanView pv = plan_view(const_cast<char*>(a.plan), a.n_seq, a.rows, (int)fG.d, shares);
-    const List list = kFew ? pv.few : pv.wide;
-    const int* head = reinterpret_cast<const int*>(a.plan);
-    const int rounds = kFew ? 0 : scalar(head[kHeadRounds]), dealt = kFew ? 0 : scalar(head[kHeadDealt]);
-    const int4 sh = *reinterpret_cast<const int4*>(list.shares + share);
-    if (!plan_fits(a.plan, a.n_seq, a.rows, a.H, a.HKV, !kPaged)) return;
+    const int dealt = rounds * shares;
     const int first = scalar(sh.x), first_tile = scalar(sh.y), last = scalar(sh.z), last_tile = scalar(sh.w);
     for (int pass = 0;; ++pass) {
         int at, cut = -1;
@@ -1176,7 +1179,7 @@ __device__ __forceinline__ void walk_list(const PackedArgs& a, int shares, float
         p.nflat = n * (int)fG.d;
         p.T = min(max(p.pos0 + fdiv(min(kUnitRows * p.u + kUnitRows, p.nflat) - 1, fG) + 1, 0), len);
         p.nrange = (cut >= 0 ? cut : scalar(x.tiles)) - p.kt_lo;
-        p.part = p.kt_lo > 0 || cut >= 0 ? parts + part_at(kFew, blockIdx.x, p.kt_lo > 0 ? 0 : 1) : nullptr;
+        p.part = p.kt_lo > 0 || cut >= 0 ? parts + part_at(kFew, share * a.HKV + kvh, p.kt_lo > 0 ? 0 : 1) : nullptr;
         if (pass > 0) lds_barrier();  // the last pass's rows have been read
         if constexpr (kFew) {
             if (p.nflat - kUnitRows * p.u <= kFewBlock) few_pass<kPaged, 1>(a, p, kvh, fG, sl2, smem);
@@ -1185,14 +1188,21 @@ __device__ __forceinline__ void walk_list(const PackedArgs& a, int shares, float
     }
 }
 
-// grid (shares x KV heads, 2): the wide list's workgroups, then the few-row list's, which start as the others
-// finish (a workgroup's LDS takes a CU) or at once where there is no wide work.
+// grid shares x KV heads (a KV head's workgroups share an XCD's L2): each workgroup's part of the wide list, then of
+// the few-row list.  The plan's header and both shares are read before anything waits for them.
 template <bool kPaged>
-__global__ __launch_bounds__(64 * kWaves) void k_packed_attn(PackedArgs a, int shares, float* __restrict__ wide,
-                                                             float* __restrict__ few) {
+__global__ __launch_bounds__(64 * kWaves) void k_packed_attn(PackedArgs a, int shares, float* __restrict__ wide_parts,
+                                                             float* __restrict__ few_parts) {
     extern __shared__ __align__(16) float smem[];
-    if (blockIdx.y == 0) walk_list<kPaged, false>(a, shares, wide, smem);
-    else walk_list<kPaged, true>(a, shares, few, smem);
+    const int kvh = blockIdx.x % a.HKV, share = blockIdx.x / a.HKV;
+    const PlanView pv = plan_view(const_cast<char*>(a.plan), a.n_seq, a.rows, a.H / a.HKV, shares);
+    const int rounds = scalar(reinterpret_cast<const int*>(a.plan)[kHeadRounds]);
+    const int4 wide = *reinterpret_cast<const int4*>(pv.wide.shares + share);
+    const int4 few = *reinterpret_cast<const int4*>(pv.few.shares + share);
+    if (!plan_fits(a.plan, a.n_seq, a.rows, a.H, a.HKV, !kPaged)) return;
+    walk_list<kPaged, false>(a, pv.wide, wide, rounds, shares, share, kvh, wide_parts, smem);
+    lds_barrier();  // the last wide pass's rows have been read
+    walk_list<kPaged, true>(a, pv.few, few, 0, shares, share, kvh, few_parts, smem);
 }
 
 // The units that the cuts divide: workgroup (share, KV head; 8 rows) merges the unit that starts in
@@ -1334,7 +1344,7 @@ static hipError_t launch_packed_attn(hipStream_t st, const PackedArgs& a, int sh
     static std::atomic<bool> opted;
     constexpr size_t lds = (size_t)(kWideF > kFewF ? kWideF : kFewF) * sizeof(float);
     if (const hipError_t e = opt_in_lds(opted, (const void*)k_packed_attn<kPaged>, lds); e != hipSuccess) return e;
-    k_packed_attn<kPaged><<<dim3(shares * a.HKV, 2), 64 * kWaves, lds, st>>>(a, shares, wide, few);
+    k_packed_attn<kPaged><<<shares * a.HKV, 64 * kWaves, lds, st>>>(a, shares, wide, few);
     return hipGetLastError();
 }
 

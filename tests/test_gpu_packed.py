@@ -87,6 +87,7 @@ def test_plan_covers_every_unit_once(gpu, H, HKV, lens, kv):
             want[n * G - 128 * u <= 32][s, u] = (max(0, min(total, total - n + last + 1)) + 31) // 32
     rounds, dealt, line = int(head[6]), int(head[7]), int(head[8])
     assert dealt == rounds * N and dealt + line == len(wide)
+    load = np.zeros(N, int)
     for is_few, units, shares, first, (once, turn) in ((False, wide, wide_shares, dealt, (5, 2)),
                                                        (True, few, few_shares, 0, (8, 8))):
         cost = want[is_few]
@@ -97,7 +98,6 @@ def test_plan_covers_every_unit_once(gpu, H, HKV, lens, kv):
         tiles = units[:, 5].astype(int)
         if first:
             assert np.all(np.diff(tiles) <= 0)  # descending
-        load = np.zeros(N, int)
         for i in range(first):
             r, j = divmod(i, N)
             load[N - 1 - j if r % 2 else j] += tiles[i] + once
@@ -123,8 +123,8 @@ def test_plan_covers_every_unit_once(gpu, H, HKV, lens, kv):
             assert shares[j, 4] == (ends[begins[j]] if j in begins else 0)
             if j in begins:
                 assert np.array_equal(shares[j, 16:24], units[first + begins[j]])
-        fair = sum(t + once for t in cost.values()) / N
-        assert load.max() <= fair + 4 * once + 2 * turn + (max(tiles, default=0) if first else 0), (load, fair)
+        fair = sum(sum(t + c for t in want[f].values()) for f, c in ((False, 5), (True, 8))[:1 + is_few]) / N
+        assert load.max() <= fair + 4 * once + 2 * turn + (max(tiles, default=0) if first else 0) + 24 * is_few
 
 
 def _prompts(H, HKV, lens, seed, extra=0):
