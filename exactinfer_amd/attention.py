@@ -291,21 +291,24 @@ class RopeScaling:
     attn_factor: float = 0.0  # yarn: factor on cos and sin, 0: 0.1 ln(factor) + 1
 
 
-def _need_here(name: str, t: torch.Tensor, dtype: torch.dtype, inner: bool = True) -> None:
-    """A tensor of this dtype on the current device, whose stream the call is launched on."""
+def _device() -> int:
+    """The current device, on whose current stream a call is launched."""
+    return torch._C._cuda_getDevice()  # (torch.cuda.current_device() checks for a context first: 0.1 us)
+
+
+def _refuse(name: str, t: torch.Tensor, dtype: torch.dtype) -> None:
+    """Says why a tensor that failed a check is not one of this dtype on the current device."""
     if not t.is_cuda:
         raise ValueError(f"{name} must be a GPU tensor")
     if t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
     if t.device.index != torch.cuda.current_device():
         raise ValueError(f"{name} is on {t.device}, the current device is cuda:{torch.cuda.current_device()}")
-    if inner and t.numel() and t.stride(-1) != 1:
-        raise ValueError(f"{name} must be contiguous in its last dimension")
 
 
 def _need_contiguous(name: str, t: torch.Tensor, dtype: torch.dtype) -> None:
-    _need_here(name, t, dtype, inner=False)
-    if not t.is_contiguous():
+    if t.dtype is not dtype or t.get_device() != _device() or not t.is_contiguous():
+        _refuse(name, t, dtype)
         raise ValueError(f"{name} must be contiguous")
 
 
@@ -318,17 +321,21 @@ def _need_gamma(name: str, t: torch.Tensor | None) -> None:
 
 def _rows_of(name: str, t: torch.Tensor, rows: int, width: int) -> int:
     """Row stride of a [>= rows, >= width] matrix (or [>= rows, heads, 128]), after checking it."""
-    _need_here(name, t, torch.float32)
-    if t.dim() == 3 and (t.stride(1) == t.shape[2] or t.shape[1] == 1):
-        have = t.shape[1] * t.shape[2]
-    elif t.dim() == 2:
-        have = t.shape[1]
+    shape, stride = t.shape, t.stride()
+    if t.dtype is not torch.float32 or t.get_device() != _device():
+        _refuse(name, t, torch.float32)
+    if len(shape) == 2:
+        have = shape[1]
+    elif len(shape) == 3 and (stride[1] == shape[2] or shape[1] == 1):
+        have = shape[1] * shape[2]
     else:
         raise ValueError(f"{name} must be [rows, values] or [rows, heads, {HEAD_DIM}] with whole rows")
-    if t.shape[0] < rows or have < width:
-        raise ValueError(f"{name} must hold {rows} rows of {width} values, got {tuple(t.shape)}")
+    if stride[-1] != 1 and t.numel():
+        raise ValueError(f"{name} must be contiguous in its last dimension")
+    if shape[0] < rows or have < width:
+        raise ValueError(f"{name} must hold {rows} rows of {width} values, got {tuple(shape)}")
     # (the stride of a single row is whatever the view says, and is not used)
-    return t.stride(0) if t.shape[0] > 1 else max(t.stride(0), (have + 3) // 4 * 4)
+    return stride[0] if shape[0] > 1 else max(stride[0], (have + 3) // 4 * 4)
 
 
 def rope_table_scaled(n_pos: int, rope_dim: int = HEAD_DIM, theta: float = 1e6, scaling: RopeScaling | None = None,
@@ -351,9 +358,10 @@ def rope_table_scaled(n_pos: int, rope_dim: int = HEAD_DIM, theta: float = 1e6, 
 
 def _table_positions(cs: torch.Tensor, rope_dim: int) -> int:
     _need_contiguous("cs", cs, torch.float32)
-    if cs.dim() != 3 or cs.shape[1] != rope_dim // 2 or cs.shape[2] != 2:
-        raise ValueError(f"cs must be [positions, {rope_dim // 2}, 2], got {tuple(cs.shape)}")
-    return cs.shape[0]
+    shape = cs.shape
+    if len(shape) != 3 or shape[1] != rope_dim // 2 or shape[2] != 2:
+        raise ValueError(f"cs must be [positions, {rope_dim // 2}, 2], got {tuple(shape)}")
+    return shape[0]
 
 
 def rope_rows(x: torch.Tensor, n_heads: int, cs: torch.Tensor, pos: torch.Tensor, rope_dim: int = HEAD_DIM,

@@ -74,11 +74,11 @@ size_t packed_plan_bytes(int n_seq, int rows, int H, int HKV) {
 
 constexpr int kPlanThreads = 512;
 constexpr int kPlanSeqLds = 1024;       // sequences held in LDS (more are read from the plan)
-constexpr int kPlanLineLds = 1024;      // units of the line held in LDS (likewise)
+constexpr int kPlanLineLds = 512;       // units of a line held in LDS (likewise)
 constexpr long kMaxRankWork = 1 << 20;  // wide units x sequences up to which units are sorted
 
 // What a list's work costs, in tiles: `pass` for everything done once per unit or part of one; a cut leaves
-// whole turns (the tiles that a workgroup's waves take at a time) on both sides, and keeps off a unit's
+// whole turns (the tiles that a workgroup's waves take at a time, a power of two) on both sides, and keeps off a unit's
 // ends by what a pass costs, so that a share does not run one for a few tiles.
 struct ListCost {
     int pass, turn;
@@ -125,58 +125,65 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
                                                               int max_kv, int H, int HKV, int shares,
                                                               char* __restrict__ plan) {
     __shared__ int4 seq_lds[kPlanSeqLds];
-    __shared__ int wide_lds[kPlanLineLds], few_lds[kPlanLineLds];  // tiles of the lines' units
+    __shared__ Unit wide_lds[kPlanLineLds], few_lds[kPlanLineLds];  // the lines' units
     __shared__ unsigned long long load[kPackedCus], few_cost, wide_cost;
-    __shared__ long long cut_at[kPackedCus + 1];
     __shared__ int2 cuts[kPackedCus + 1];
     __shared__ long long cut_cost[kPackedCus + 1];  // the line's cost before each cut
+    __shared__ long long line_at[kPlanThreads];     // units of the line: cost before, tiles
+    __shared__ int line_tiles[kPlanThreads];
     const int tid = threadIdx.x, G = H / HKV;
     const PlanView pv = plan_view(plan, n_seq, rows, G, shares);
     // keys that rows up to `row` of a sequence of n rows and len keys see, in tiles
     auto tiles_of = [](int n, int len, int row) { return (max(min(len - n + row + 1, len), 0) + kKT - 1) / kKT; };
     auto wide_of = [&](int n) { return (int)(((long long)n * G + kUnitRows - 1 - kFewRows) / kUnitRows); };
 
-    // The shares of a list whose line has `line` units: share j's end where cut_at[j + 1] falls on the
-    // line's running cost (cut_at is set, the units are written).
-    auto cut_line = [&](const List& list, int rounds, int line, ListCost c, const int* lds, long long share) {
+    // The shares of a list whose line has `line` units: share j's end where `mine` of thread j + 1 falls on
+    // the line's running cost.
+    auto cut_line = [&](const List& list, int rounds, int line, ListCost c, const Unit* lds, long long share,
+                        long long mine) {
         const int dealt = rounds * shares;
-        const int keep = max(c.turn, min(c.pass, (int)min(share / 2, (long long)c.pass)));
-        if (tid <= shares) cuts[tid] = make_int2(tid == 0 ? 0 : line, 0), cut_cost[tid] = tid == 0 ? 0 : -1;
-        __syncthreads();
+        const int keep = max(c.turn, (int)min(share / 2, (long long)c.pass));
+        int2 cut = make_int2(tid == 0 ? 0 : line, 0);  // thread j: the end of share j - 1
+        long long cost_at = tid == 0 ? 0 : -1;
+        if (tid == 0 || tid >= shares) mine = -1;
         long long at = 0;
         for (int base = 0; base < line; base += kPlanThreads) {
             const int i = base + tid;
-            const int tiles = i >= line ? 0 : lds ? lds[i] : list.units[dealt + i].tiles;
-            const long long cost = i < line ? tiles + c.pass : 0;
+            const int tiles = i >= line ? 0 : lds ? lds[i].tiles : list.units[dealt + i].tiles;
             long long sum;
-            const long long a = at + block_scan(cost, &sum);
-            if (i < line) {
-                int lo = 1, hi = shares + 1;  // the first cut not before a
-                while (lo < hi) {
-                    const int mid = (lo + hi) >> 1;
-                    if (cut_at[mid] >= a) hi = mid;
-                    else lo = mid + 1;
+            const long long a = at + block_scan(i < line ? tiles + c.pass : 0, &sum);
+            line_at[tid] = a, line_tiles[tid] = tiles;
+            __syncthreads();
+            if (mine >= at && mine < at + sum) {
+                int lo = 0, hi = min(line - base, kPlanThreads) - 1;
+                while (lo < hi) {  // the last unit that begins at or before the cut
+                    const int mid = (lo + hi + 1) >> 1;
+                    if (line_at[mid] <= mine) lo = mid;
+                    else hi = mid - 1;
                 }
-                for (; lo < shares && cut_at[lo] < a + cost; ++lo) {
-                    const long long t = (cut_at[lo] - a) / c.turn * c.turn;
-                    cuts[lo] = t + keep > tiles ? make_int2(i + 1, 0) : make_int2(i, t < keep ? 0 : (int)t);
-                    cut_cost[lo] = a + (t + keep > tiles ? cost : t < keep ? 0 : t);
-                }
+                const int t = (int)(mine - line_at[lo]) & ~(c.turn - 1), n = line_tiles[lo];
+                cut = t + keep > n ? make_int2(base + lo + 1, 0) : make_int2(base + lo, t < keep ? 0 : t);
+                cost_at = line_at[lo] + (t + keep > n ? n + c.pass : t < keep ? 0 : t);
             }
             at += sum;
         }
+        if (tid <= shares) cuts[tid] = cut, cut_cost[tid] = cost_at < 0 ? at : cost_at;  // (past the end: all of it)
         __syncthreads();
-        if (tid <= shares && cut_cost[tid] < 0) cut_cost[tid] = at;  // past the line's end
         if (tid < shares) {
             const int2 from = cuts[tid], to = cuts[tid + 1];
             Share& x = list.shares[tid];
             x.first = from.x, x.first_tile = from.y, x.last = to.x, x.last_tile = to.y;
-            if (rounds > 0 || from.x < line) x.start = list.units[rounds > 0 ? tid : from.x];
+            if (rounds > 0) x.start = list.units[tid];
+            else if (from.x < line) x.start = lds ? lds[from.x] : list.units[from.x];
             int end = 0;
             if (to.y > 0 && !(from.x == to.x && from.y > 0)) {  // a unit begins here and goes on
                 end = tid + 1;
-                while (cuts[end + 1].x == to.x && cuts[end + 1].y > 0) ++end;
-                x.merge = list.units[dealt + to.x];
+                for (int hi = shares - 1; end < hi;) {  // to the last cut that is not past it
+                    const int mid = (end + hi + 1) >> 1;
+                    if (cuts[mid].x == to.x) end = mid;
+                    else hi = mid - 1;
+                }
+                x.merge = lds ? lds[to.x] : list.units[dealt + to.x];
             }
             x.merge_end = end;
         }
@@ -211,8 +218,9 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
         }
         if (is_few) {
             const int i = (int)(few + (at & 0xFFFFFFFF));
-            pv.few.units[i] = Unit{lo, n, len, nw, s, tiles, {0, 0}};
-            if (i < kPlanLineLds) few_lds[i] = tiles;
+            const Unit x{lo, n, len, nw, s, tiles, {0, 0}};
+            pv.few.units[i] = x;
+            if (i < kPlanLineLds) few_lds[i] = x;
         }
         const long long cost = wave_scan(is_few ? tiles + kFewCost.pass : 0);
         if ((tid & 63) == 63 && cost > 0) atomicAdd(&few_cost, (unsigned long long)cost);
@@ -255,6 +263,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
         if (rounds > 0) {
             // units before this one: more tiles, or as many in an earlier sequence, or later in its own
             at = 0;
+#pragma unroll 4
             for (int s = 0; s < n_seq; ++s) {
                 const int4 e = seq_at(s);
                 at += s < x.seq ? above(e, x.tiles - 1) : s > x.seq ? above(e, x.tiles) : wide_of(e.y) - 1 - x.u;
@@ -264,26 +273,24 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
         if (at < dealt) {
             const int r = at / shares, j = at - r * shares;
             atomicAdd(&load[(r & 1) ? shares - 1 - j : j], (unsigned long long)(x.tiles + kWideCost.pass));
-        } else if (at - dealt < kPlanLineLds) wide_lds[at - dealt] = x.tiles;
+        } else if (at - dealt < kPlanLineLds) wide_lds[at - dealt] = x;
     }
     mine = wave_scan(mine);
     if ((tid & 63) == 63 && mine > 0) atomicAdd(&wide_cost, (unsigned long long)mine);
     __syncthreads();
     {
-        const long long share = ((long long)wide_cost + shares - 1) / shares;
+        const long long share = (long long)((double)wide_cost / shares) + 1;
         long long before = tid * share, all;
         if (rounds > 0) before = block_scan(tid < shares ? max(share - (long long)load[tid], 0LL) : 0, &all);
-        if (tid <= shares) cut_at[tid] = before;
-        cut_line(pv.wide, rounds, line, kWideCost, line <= kPlanLineLds ? wide_lds : nullptr, share);
+        cut_line(pv.wide, rounds, line, kWideCost, line <= kPlanLineLds ? wide_lds : nullptr, share, before);
     }
     {
-        const long long share = ((long long)few_cost + shares - 1) / shares;
-        const long long both = ((long long)(wide_cost + few_cost) + shares - 1) / shares;
+        const long long share = (long long)((double)few_cost / shares) + 1;
+        const long long both = (long long)((double)(wide_cost + few_cost) / shares) + 1;
         const long long wide = tid < shares ? (long long)load[tid] + cut_cost[tid + 1] - cut_cost[tid] : 0;
         long long all;
         const long long before = block_scan(tid < shares ? max(both - wide, 0LL) : 0, &all);
-        if (tid <= shares) cut_at[tid] = before;
-        cut_line(pv.few, 0, (int)few, kFewCost, few <= kPlanLineLds ? few_lds : nullptr, share);
+        cut_line(pv.few, 0, (int)few, kFewCost, few <= kPlanLineLds ? few_lds : nullptr, share, before);
     }
     if (tid == 0) {
         int* h = reinterpret_cast<int*>(plan);
@@ -1211,7 +1218,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_packed_attn(PackedArgs a, int s
 // key (m = -inf and l = 0 otherwise; m = -inf with a NaN l counts).
 constexpr int kCombineRows = 8;
 constexpr int kCombineWide = kUnitRows / kCombineRows, kCombineFew = kFewRows / kCombineRows;
-__global__ __launch_bounds__(256) void k_packed_combine(PackedArgs a, bool prompts, int shares,
+__global__ __launch_bounds__(32 * kCombineRows) void k_packed_combine(PackedArgs a, bool prompts, int shares,
                                                         const float* __restrict__ wide_parts,
                                                         const float* __restrict__ few_parts) {
     const int kvh = blockIdx.x % a.HKV, share = blockIdx.x / a.HKV, G = a.H / a.HKV;
@@ -1275,7 +1282,24 @@ __global__ __launch_bounds__(256) void k_packed_prepare(const float* __restrict_
     const int b = blockIdx.x, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int H = a.H, HKV = a.HKV, NH = H + HKV;
     const int h0 = (blockIdx.y * 4 + w) * kPrepHeads;
-    if (h0 >= NH || !plan_fits(a.plan, a.n_seq, a.rows, H, HKV, false)) return;  // wave-uniform, no barrier here
+    if (h0 >= NH) return;  // wave-uniform, no barrier here
+    // (the row's values are on their way while its place is looked up; of a row that nobody owns they are not used)
+    const float* row = qkv + (size_t)b * row_stride;
+    float x0[kPrepHeads], x1[kPrepHeads], v0[kPrepHeads], v1[kPrepHeads], inv[kPrepHeads];
+#pragma unroll
+    for (int j = 0; j < kPrepHeads; ++j) {
+        const int hh = min(h0 + j, NH - 1);  // clamped: heads past NH are loaded, not used
+        const float* v = row + (size_t)hh * kHeadDim;
+        x0[j] = v[lane];
+        x1[j] = v[lane + 64];
+        v0[j] = v1[j] = 0.f;
+        if (hh >= H) {
+            const float* vs = row + (size_t)(NH + hh - H) * kHeadDim;  // V of a key head
+            v0[j] = vs[lane];
+            v1[j] = vs[lane + 64];
+        }
+    }
+    if (!plan_fits(a.plan, a.n_seq, a.rows, H, HKV, false)) return;
     const int4* seq = reinterpret_cast<const int4*>(a.plan + kPlanSeqAt);
     const int s = row_owner(seq, a.n_seq, b, lane);
     if (s < 0) return;
@@ -1286,19 +1310,7 @@ __global__ __launch_bounds__(256) void k_packed_prepare(const float* __restrict_
     const int phys = in && blk < a.max_blocks ? a.btab[(size_t)s * a.max_blocks + blk] : -1;
     const bool there = phys >= 0 && phys < a.n_blocks;
     const size_t crow = ((size_t)(there ? phys : 0) << a.bshift) | (size_t)(pos & ((1 << a.bshift) - 1));
-    const float* row = qkv + (size_t)b * row_stride;
     const float2* cs_row = cs + (size_t)(in ? pos : 0) * (rope_dim >> 1);
-    float x0[kPrepHeads], x1[kPrepHeads], v0[kPrepHeads], v1[kPrepHeads], inv[kPrepHeads];
-#pragma unroll
-    for (int j = 0; j < kPrepHeads; ++j) {
-        const int hh = min(h0 + j, NH - 1);  // clamped: heads past NH are loaded, not used
-        const float* v = row + (size_t)hh * kHeadDim;
-        x0[j] = v[lane];
-        x1[j] = v[lane + 64];
-        const float* vs = row + (size_t)(NH + max(hh - H, 0)) * kHeadDim;  // V of a key head
-        v0[j] = vs[lane];
-        v1[j] = vs[lane + 64];
-    }
     const float qg0 = q_gamma[lane], qg1 = q_gamma[lane + 64];
     const float kg0 = k_gamma[lane], kg1 = k_gamma[lane + 64];
     head_inv<kPrepHeads>(x0, x1, eps, inv, lane);
@@ -1355,8 +1367,8 @@ hipError_t launch_packed(hipStream_t st, const PackedArgs& a, void* ws) {
     const hipError_t e = a.btab ? launch_packed_attn<true>(st, a, shares, wide, few)
                                 : launch_packed_attn<false>(st, a, shares, wide, few);
     if (e != hipSuccess) return e;
-    k_packed_combine<<<dim3(shares * a.HKV, kCombineWide + kCombineFew), 256, 0, st>>>(a, a.btab == nullptr, shares,
-                                                                                        wide, few);
+    k_packed_combine<<<dim3(shares * a.HKV, kCombineWide + kCombineFew), 32 * kCombineRows, 0, st>>>(
+        a, a.btab == nullptr, shares, wide, few);
     return hipGetLastError();
 }
 
