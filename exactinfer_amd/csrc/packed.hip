@@ -161,9 +161,14 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
                     if (line_at[mid] <= mine) lo = mid;
                     else hi = mid - 1;
                 }
-                const int t = (int)(mine - line_at[lo]) & ~(c.turn - 1), n = line_tiles[lo];
-                cut = t + keep > n ? make_int2(base + lo + 1, 0) : make_int2(base + lo, t < keep ? 0 : t);
-                cost_at = line_at[lo] + (t + keep > n ? n + c.pass : t < keep ? 0 : t);
+                const long long in = mine - line_at[lo];
+                const int n = line_tiles[lo], t = (int)min(in, (long long)n) & ~(c.turn - 1);
+                // inside the unit, or at the end of it whose `keep` tiles it falls in (the nearer one, if it is
+                // too short to be cut at all): later cuts never come before earlier ones
+                const bool inside = t >= keep && t + keep <= n;
+                const bool after = !inside && (n >= 2 * keep ? t >= keep : 2 * in >= n + c.pass);
+                cut = make_int2(base + lo + after, inside ? t : 0);
+                cost_at = line_at[lo] + (inside ? t : after ? n + c.pass : 0);
             }
             at += sum;
         }
@@ -279,14 +284,14 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
     if ((tid & 63) == 63 && mine > 0) atomicAdd(&wide_cost, (unsigned long long)mine);
     __syncthreads();
     {
-        const long long share = (long long)((double)wide_cost / shares) + 1;
+        const long long share = (long long)ceil((double)wide_cost / shares);
         long long before = tid * share, all;
         if (rounds > 0) before = block_scan(tid < shares ? max(share - (long long)load[tid], 0LL) : 0, &all);
         cut_line(pv.wide, rounds, line, kWideCost, line <= kPlanLineLds ? wide_lds : nullptr, share, before);
     }
     {
-        const long long share = (long long)((double)few_cost / shares) + 1;
-        const long long both = (long long)((double)(wide_cost + few_cost) / shares) + 1;
+        const long long share = (long long)ceil((double)few_cost / shares);
+        const long long both = (long long)ceil((double)(wide_cost + few_cost) / shares);
         const long long wide = tid < shares ? (long long)load[tid] + cut_cost[tid + 1] - cut_cost[tid] : 0;
         long long all;
         const long long before = block_scan(tid < shares ? max(both - wide, 0LL) : 0, &all);
