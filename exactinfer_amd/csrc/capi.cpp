@@ -659,8 +659,9 @@ int check_packed(int n_seq, int rows, int n_head, int n_head_kv, int head_dim, c
     return EI_OK;
 }
 
+// The pools, and that what the call writes does not lie in them.
 int check_pool(const float* kc, const float* vc, int n_blocks, const int* block_table, int max_blocks, int block_size,
-               int* shift) {
+               int n_head_kv, const float* out, size_t out_bytes, const void* ws, size_t ws_bytes, int* shift) {
     REQUIRE(kc && vc && block_table, "null pointer argument");
     REQUIRE(aligned16(kc) && aligned16(vc), "pointers must be 16-byte aligned");
     REQUIRE(block_size >= 32 && (block_size & (block_size - 1)) == 0,
@@ -668,6 +669,11 @@ int check_pool(const float* kc, const float* vc, int n_blocks, const int* block_
     REQUIRE(max_blocks > 0 && (long)max_blocks * block_size <= 0x7FFFFFFFL,
             "max_blocks %d x block_size %d must lie in [1, 2^31 - 1] keys", max_blocks, block_size);
     REQUIRE(n_blocks > 0, "n_blocks %d must be positive", n_blocks);
+    const size_t pool = (size_t)n_blocks * block_size * n_head_kv * 128 * sizeof(float);
+    REQUIRE(!overlap(kc, pool, vc, pool), "the K and V pools overlap");
+    for (const float* c : {kc, vc})
+        REQUIRE(!overlap(c, pool, out, out_bytes) && !overlap(c, pool, ws, ws_bytes),
+                "out or workspace lies in a pool of %zu bytes", pool);
     int s = 0;
     while ((1 << s) < block_size) ++s;
     *shift = s;
@@ -773,7 +779,7 @@ EI_API int ei_attn_packed(ei_stream_t stream, const float* q, long q_stride, con
     REQUIRE(aligned16(q) && aligned16(k) && aligned16(v), "pointers must be 16-byte aligned");
     const long qw = (long)n_head * head_dim, kw = (long)n_head_kv * head_dim;
     REQUIRE(q_stride >= qw && q_stride % 4 == 0, "q_stride %ld", q_stride);
-    REQUIRE(kv_stride >= kw && kv_stride % 4 == 0 && kv_stride <= (1L << 24), "kv_stride %ld", kv_stride);
+    REQUIRE(kv_stride >= kw && kv_stride % 4 == 0 && kv_stride <= (1L << 22), "kv_stride %ld", kv_stride);
     const size_t ob = span_bytes(rows, qw, qw);
     REQUIRE(!overlap(out, ob, q, span_bytes(rows, q_stride, qw)) &&
                 !overlap(out, ob, k, span_bytes(rows, kv_stride, kw)) &&
@@ -796,9 +802,11 @@ EI_API int ei_attn_packed_paged(ei_stream_t stream, const float* q, long q_strid
                                 const void* plan, size_t plan_bytes, void* ws, size_t ws_bytes) {
     if (int e = check_packed(n_seq, rows, n_head, n_head_kv, head_dim, plan, plan_bytes, ws, ws_bytes, out)) return e;
     int shift = 0;
-    if (int e = check_pool(kc, vc, n_blocks, block_table, max_blocks, block_size, &shift)) return e;
-    REQUIRE(q && aligned16(q), "q missing or not 16-byte aligned");
     const long qw = (long)n_head * head_dim;
+    if (int e = check_pool(kc, vc, n_blocks, block_table, max_blocks, block_size, n_head_kv, out,
+                           span_bytes(rows, qw, qw), ws, ei::packed_ws_bytes(rows, n_head, n_head_kv), &shift))
+        return e;
+    REQUIRE(q && aligned16(q), "q missing or not 16-byte aligned");
     REQUIRE(q_stride >= qw && q_stride % 4 == 0, "q_stride %ld", q_stride);
     REQUIRE(!overlap(out, span_bytes(rows, qw, qw), q, span_bytes(rows, q_stride, qw)), "out overlaps q");
     if (rows == 0) return ok();
@@ -822,16 +830,20 @@ EI_API int ei_packed_step_paged(ei_stream_t stream, const float* qkv, long row_s
     if (int e = check_packed(n_seq, rows, n_head, n_head_kv, head_dim, plan, plan_bytes, ws, ws_bytes, out)) return e;
     if (int e = check_rope(rope_dim, head_dim)) return e;
     int shift = 0;
-    if (int e = check_pool(kc, vc, n_blocks, block_table, max_blocks, block_size, &shift)) return e;
+    const long w = (long)(n_head + 2 * n_head_kv) * head_dim, qw = (long)n_head * head_dim;
+    if (int e = check_pool(kc, vc, n_blocks, block_table, max_blocks, block_size, n_head_kv, out,
+                           span_bytes(rows, qw, qw), ws, ei::packed_ws_bytes(rows, n_head, n_head_kv), &shift))
+        return e;
     REQUIRE(qkv && q_gamma && k_gamma && cs, "null pointer argument");
     REQUIRE(n_pos > 0, "n_pos %d must be positive", n_pos);
-    const long w = (long)(n_head + 2 * n_head_kv) * head_dim, qw = (long)n_head * head_dim;
     REQUIRE(row_stride >= w && row_stride % 4 == 0 && aligned16(qkv),
             "qkv must be 16-byte aligned, row_stride %ld a multiple of 4 and >= (H+2*HKV)*head_dim", row_stride);
     const size_t in = span_bytes(rows, row_stride, w);
     REQUIRE(!overlap(out, span_bytes(rows, qw, qw), qkv, in) &&
                 !overlap(ws, ei::packed_ws_bytes(rows, n_head, n_head_kv), qkv, in),
             "out or workspace overlaps qkv");
+    const size_t pool = (size_t)n_blocks * block_size * n_head_kv * head_dim * sizeof(float);
+    REQUIRE(!overlap(kc, pool, qkv, in) && !overlap(vc, pool, qkv, in), "qkv lies in a pool");
     if (rows == 0) return ok();
     ei::PackedArgs a{};
     a.k = kc, a.v = vc, a.kv_stride = (long)n_head_kv * head_dim;

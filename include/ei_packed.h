@@ -84,8 +84,16 @@ size_t ei_packed_ws_bytes(int rows, int n_head, int n_head_kv);
 /* ------------------------------------------------------------------ attention over packed prompts
  * Causal attention of every sequence over its own rows: q row b at q + b*q_stride ([n_head][128],
  * normed and turned), k and v rows at k + b*kv_stride ([n_head_kv][128]); views of one [Q | K | V]
- * buffer are fine.  out [rows][n_head][128], which must not overlap the inputs.  The plan must be one
- * of whole prompts (kv_len NULL).  Arithmetic as in ei_attn_prefill. */
+ * buffer are fine; kv_stride at most 2^22.  out [rows][n_head][128], which must not overlap the inputs.
+ * The plan must be one of whole prompts (kv_len NULL).
+ *
+ * Arithmetic of this call and the two below: fp32 sums of products whose operands keep 22 bits of 24
+ * (two binary16 planes), or of fp32 products for the last few rows of a sequence (single tokens, drafts);
+ * softmax in fp32.  Outputs differ from ei_attn_prefill's and ei_attn_decode's in the last bits, and with
+ * the batch a sequence is in; a batch called twice gives the same bits.  Key and value rows that a
+ * row does not see never reach it, whatever they hold.  Infinite or NaN values in K or V, or a V whose
+ * largest values are 2^15 times a row's sums, make the waves that meet them take their keys again in
+ * fp32, some ten times slower. */
 int ei_attn_packed(ei_stream_t stream, const float* q, long q_stride, const float* k, const float* v,
                    long kv_stride, float* out, int n_seq, int rows, int n_head, int n_head_kv, int head_dim,
                    float scale, const void* plan, size_t plan_bytes, void* ws, size_t ws_bytes);

@@ -265,6 +265,146 @@ def test_visible_infinities_and_nan(gpu):
     assert torch.isnan(out[10:, 0]).all() and torch.isfinite(out[:10]).all() and torch.isfinite(out[:, 1:]).all()
 
 
+def _run_prompts(gpu, q, k, v, lens, H, HKV, scale=None):
+    b = gpu.PackedBatch(len(lens), sum(lens), H, HKV)
+    b.plan(_i32(_cu(lens)), sum(lens), max(lens))
+    return gpu.attn_packed(q, k, v, b, gpu.AttnShape(H, HKV), scale=scale)
+
+
+@pytest.mark.parametrize("H,HKV,lens", [(16, 8, [100, 7, 300]), (32, 8, [4, 8, 1]), (8, 1, [60])])
+@pytest.mark.parametrize("e_qk,e_v", [(60, 0), (-60, 0), (0, 100), (0, -90), (100, 30), (-30, 60)])
+def test_powers_of_two_come_out_exactly(gpu, H, HKV, lens, e_qk, e_v):
+    """q by 2^e and k by 2^-e change nothing, v by 2^e the output by 2^e: every scaling in the kernels is a
+    power of two that follows the values."""
+    _, q, k, v = _prompts(H, HKV, lens, 101)
+    ref = _run_prompts(gpu, q, k, v, lens, H, HKV)
+    out = _run_prompts(gpu, (q * 2.0 ** e_qk).contiguous(), (k * 2.0 ** -e_qk).contiguous(),
+                       (v * 2.0 ** e_v).contiguous(), lens, H, HKV)
+    assert torch.equal(out, ref * 2.0 ** e_v)
+
+
+@pytest.mark.parametrize("H,HKV,lens", [(16, 8, [150, 40]), (32, 8, [8, 5])])
+@pytest.mark.parametrize("what", ["k_row", "k_channel", "v_row", "v_column", "v_zero", "v_heads", "q_row"])
+def test_uneven_magnitudes(gpu, H, HKV, lens, what):
+    """Rows and columns far larger or smaller than the others, against 64 bits."""
+    _, q, k, v = (t.contiguous() for t in _prompts(H, HKV, lens, 102))
+    if what == "k_row":  # every seventh key large: its row's own scaling must not cost the others
+        k[::7] *= 1000.0
+        q *= 1e-3
+    elif what == "k_channel":
+        k[:, 5::128] *= 300.0
+        q[:, 5::128] *= 1e-3
+    elif what == "v_row":  # a value row 2^30 times the others, at a key whose weight is e^-40 or so
+        k[3] = 0.0
+        q[:, ::128] = 40.0
+        k[:, ::128] = 12.0
+        k[3, ::128] = 0.0
+        v[3] *= 2.0 ** 30
+    elif what == "v_column":
+        v[:, 9::128] *= 1e-6
+    elif what == "v_zero":
+        v[:] = 0.0
+    elif what == "v_heads":
+        v[:, :D] *= 1e20
+        v[:, D:2 * D] *= 1e-30
+    else:
+        q[11] *= 50.0
+    out = _run_prompts(gpu, q, k, v, lens, H, HKV)
+    if what == "v_row":
+        # Scores of 40 * 12 / sqrt(128) lie near 61 in log2 units, where an fp32 sum is rounded by up to 2^-18:
+        # 127 additions move a score by at most 127 * 2^-18, a weight by that times ln 2 of itself, and an
+        # output by twice as much of the largest ordinary value.  (Unnoticed, the planes of V would be off by
+        # 2^-25 of their range, 2^-6 here, five times that.)
+        tol = 2 * 127 * 2.0 ** -18 * np.log(2) * v[np.r_[0:3, 4:v.shape[0]]].abs().max().item()
+        for a, n in zip(_cu(lens), lens):
+            r = slice(int(a), int(a) + n)
+            ref = _attend64(q[r].double().view(n, H, D), k[r].double().view(n, HKV, D), v[r].double().view(n, HKV, D), n)
+            assert (out[r] - ref).abs().max().item() <= tol
+        return
+    if what == "q_row":
+        # A row 50 times the others has scores of hundreds of log2 units.  An fp32 sum of 128 products is off by at
+        # most 127 * 2^-24 of the sum of their magnitudes, a weight by that times ln 2 of itself, and the row's output
+        # by twice as much of the largest value.  The other rows keep the tolerance below.
+        most = v.abs().max().item()
+        for a, n in zip(_cu(lens), lens):
+            a = int(a)
+            if not a <= 11 < a + n:
+                continue
+            r = slice(a, a + n)
+            ref = _attend64(q[r].double().view(n, H, D), k[r].double().view(n, HKV, D), v[r].double().view(n, HKV, D), n)
+            mags = q[11].double().view(HKV, -1, D).abs() @ k[a:12].double().view(-1, HKV, D).abs().permute(1, 2, 0).contiguous()
+            off = 127 * 2.0 ** -24 * mags.max().item() * SCALE * np.log2(np.e)
+            assert (out[11] - ref[11 - a]).abs().max().item() <= 2 * off * np.log(2) * most
+            out[11] = ref[11 - a]
+    _check_prompts(out, q, k, v, lens, H, HKV)
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_a_bad_query_row_stays_its_own(gpu, bad):
+    H, HKV, lens = 16, 8, [70, 6]
+    _, q, k, v = (t.contiguous() for t in _prompts(H, HKV, lens, 103))
+    clean = _run_prompts(gpu, q, k, v, lens, H, HKV)
+    q[33, 4] = bad   # head 0 of a row of the wide unit
+    q[72, 130] = bad  # head 1 of a row of the few-row unit
+    out = _run_prompts(gpu, q, k, v, lens, H, HKV)
+    keep = torch.ones_like(out, dtype=torch.bool)
+    keep[33, 0] = keep[72, 1] = False
+    assert torch.isnan(out[33, 0]).all() and torch.isnan(out[72, 1]).all()
+    assert rel_err(torch.where(keep, out, clean).cpu().numpy(), clean.cpu().numpy()) <= ATTN_RTOL
+
+
+@pytest.mark.parametrize("H,HKV,n_seq,most", [(8, 8, 1500, 80), (2, 1, 1200, 30), (40, 8, 700, 40)])
+def test_many_sequences(gpu, H, HKV, n_seq, most):
+    """More sequences than the plan holds in shared memory, more units on a line than it does, and too many
+    of both to be sorted."""
+    rng = np.random.default_rng(n_seq)
+    lens = [int(x) for x in rng.integers(0, most + 1, n_seq)]
+    _, q, k, v = _prompts(H, HKV, lens, 104)
+    out = _run_prompts(gpu, q, k, v, lens, H, HKV)
+    # one causal block-diagonal softmax per head in 64 bits, a few hundred rows at a time
+    cu = _cu(lens)
+    pick = sorted(set(rng.integers(0, n_seq, 60).tolist()) | {0, n_seq - 1})
+    for s in pick:
+        if lens[s]:
+            r = slice(int(cu[s]), int(cu[s + 1]))
+            _check_prompts(out[r], q[r], k[r], v[r], [lens[s]], H, HKV)
+    assert torch.isfinite(out).all()
+
+
+def test_other_batches_on_one_plan_buffer(gpu):
+    """A buffer made for a large batch serves smaller ones after it, and the large one again."""
+    H, HKV = 16, 8
+    b = gpu.PackedBatch(20, 900, H, HKV)
+    for lens in ([400, 500], [1] * 20, [33], [0, 0, 12], [400, 500]):
+        _, q, k, v = _prompts(H, HKV, lens, 105)
+        b.plan(_i32(_cu(lens)), sum(lens), max(lens))
+        _check_prompts(gpu.attn_packed(q, k, v, b, gpu.AttnShape(H, HKV)), q, k, v, lens, H, HKV)
+
+
+def test_one_plan_on_two_streams(gpu):
+    """A plan is only read by the calls: two workspaces, two streams, one plan."""
+    from exactinfer_amd import _capi
+    H, HKV, lens = 16, 8, [300, 20, 1, 700]
+    rows = sum(lens)
+    _, q, k, v = _prompts(H, HKV, lens, 106)
+    b = gpu.PackedBatch(4, rows, H, HKV)
+    b.plan(_i32(_cu(lens)), rows, 700)
+    ref = gpu.attn_packed(q, k, v, b, gpu.AttnShape(H, HKV))
+    torch.cuda.synchronize()
+    streams, outs, spaces = [torch.cuda.Stream() for _ in range(2)], [], []
+    for s in streams:
+        outs.append(torch.zeros_like(ref))
+        spaces.append(torch.empty_like(b.ws))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for s, o, w in zip(streams, outs, spaces):
+            _capi.call("ei_attn_packed", s.cuda_stream, q.data_ptr(), q.stride(0), k.data_ptr(), v.data_ptr(),
+                       k.stride(0), o.data_ptr(), 4, rows, H, HKV, D, float(gpu.default_scale()), b.buf.data_ptr(),
+                       b.nbytes, w.data_ptr(), b.ws_nbytes)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, ref) for o in outs)
+
+
 def _pool(lens, kv, HKV, bs, seed, shared=0, spare=3, slack=1):
     """A pool of shuffled blocks, block table and every sequence's pool rows."""
     rng = np.random.default_rng(seed)
@@ -356,7 +496,8 @@ def _norm_rope64(x, gamma, pos, rd, theta=1e6, eps=1e-6):
 
 @pytest.mark.parametrize("H,HKV,bs,lens,kv,rd", [
     (16, 8, 64, [1, 100, 1, 60, 1], [301, 612, 34, 60, 901], 128),
-    (32, 8, 32, [5] * 6, [29, 64, 101, 256, 300, 5], 128), (40, 8, 128, [130, 1], [131, 1], 64), (8, 1, 32, [0, 7, 33], [40, 39, 33], 126), (64, 8, 64, [3, 3], [3, 400], 128),
+    (32, 8, 32, [5] * 6, [29, 64, 101, 256, 300, 5], 128), (40, 8, 128, [130, 1], [131, 1], 64),
+    (8, 1, 32, [0, 7, 33], [40, 39, 33], 126), (64, 8, 64, [3, 3], [3, 400], 128),
 ])
 def test_step(gpu, H, HKV, bs, lens, kv, rd):
     kc, vc, table, rows_of = _pool(lens, kv, HKV, bs, 41)

@@ -127,6 +127,7 @@ def test_sizes():
     ("rows -1", (P, None, 4, -1, 100, 32, 8, P, BIG)),
     ("2\\^20 rows", (P, None, 4, (1 << 20) + 1, 100, 32, 8, P, BIG)),
     ("max_kv -1", (P, None, 4, 100, -1, 32, 8, P, BIG)),
+    ("max_kv", (P, None, 4, 100, (1 << 30) + 1, 32, 8, P, BIG)),
     ("cu_rows", (None, None, 4, 100, 100, 32, 8, P, BIG)),
     ("plan missing", (P, None, 4, 100, 100, 32, 8, None, BIG)),
     ("ei_packed_plan_bytes", (P, None, 4, 100, 100, 32, 8, P, 64)),
@@ -190,6 +191,9 @@ POOL = [
     ("null", dict(vc=None)),
     ("null", dict(table=None)),
     ("aligned", dict(kc=_off(FAR[4], 1))),
+    ("pools overlap", dict(vc=_off(FAR[4], 1024))),
+    ("lies in a pool", dict(kc=_off(FAR[1], 4096))),
+    ("lies in a pool", dict(vc=_off(FAR[3], 4096))),
 ]
 
 
@@ -201,7 +205,7 @@ POOL = [
     ("q_stride", dict(qs=6145)),
     ("kv_stride", dict(kvs=1020)),
     ("kv_stride", dict(kvs=6146)),
-    ("kv_stride", dict(kvs=1 << 25)),
+    ("kv_stride", dict(kvs=1 << 23)),
     ("overlaps q", dict(out=_off(FAR[0], 6144))),
     ("overlaps q", dict(out=FAR[5], k=FAR[5])),
     ("overlaps q", dict(out=FAR[5], v=_off(FAR[5], 4096))),
@@ -230,6 +234,7 @@ def test_paged_arguments(match, kw):
     ("row_stride", dict(rs=6146)),
     ("overlaps qkv", dict(out=FAR[0])),
     ("overlaps qkv", dict(ws=_off(FAR[0], 6144))),
+    ("qkv lies in a pool", dict(vc=_off(FAR[0], 4096))),
 ])
 def test_step_arguments(match, kw):
     _refused(match, "ei_packed_step_paged", *_step(**kw))
