@@ -334,8 +334,7 @@ def _rows_of(name: str, t: torch.Tensor, rows: int, width: int) -> int:
         raise ValueError(f"{name} must be contiguous in its last dimension")
     if shape[0] < rows or have < width:
         raise ValueError(f"{name} must hold {rows} rows of {width} values, got {tuple(shape)}")
-    # (the stride of a single row is whatever the view says, and is not used)
-    return stride[0] if shape[0] > 1 else max(stride[0], (have + 3) // 4 * 4)
+    return stride[0] if shape[0] > 1 else width  # (a single row's stride is whatever the view says)
 
 
 def rope_table_scaled(n_pos: int, rope_dim: int = HEAD_DIM, theta: float = 1e6, scaling: RopeScaling | None = None,
@@ -407,6 +406,7 @@ class PackedBatch:
         """cu_rows int32 [n_seq + 1]: sequence s owns rows cu_rows[s] .. cu_rows[s+1] - 1, of `rows` in
         all (later ones belong to nobody).  kv_len int32 [n_seq], each at most max_kv: keys after the
         new rows are appended; None: whole prompts."""
+        self._check_device()
         _need_contiguous("cu_rows", cu_rows, torch.int32)
         n_seq = cu_rows.numel() - 1
         if not 1 <= n_seq <= self.max_seq or not 0 <= rows <= self.max_rows:
@@ -420,9 +420,14 @@ class PackedBatch:
                    self.n_head_kv, self.buf.data_ptr(), self.nbytes)
         self.n_seq, self.rows, self.prompts = n_seq, rows, kv_len is None
 
+    def _check_device(self) -> None:
+        if self.buf.get_device() != _device():
+            _refuse("the batch's plan", self.buf, torch.uint8)
+
     def _check(self, shape: AttnShape) -> None:
         if self.n_seq == 0:
             raise ValueError("the batch has no plan yet: call plan() first")
+        self._check_device()
         if (shape.n_head, shape.n_head_kv) != (self.n_head, self.n_head_kv):
             raise ValueError(f"the batch was made for {self.n_head}/{self.n_head_kv} heads, the call has "
                              f"{shape.n_head}/{shape.n_head_kv}")

@@ -711,6 +711,7 @@ EI_API int ei_rope_table_scaled(ei_stream_t stream, float* cs, int n_pos, int ro
         lo = std::fmax(std::floor(pair(scaling->beta_fast)), 0.0);
         const double hi = std::fmin(std::ceil(pair(scaling->beta_slow)), rope_dim - 1.0);
         width = std::fmax(hi - lo, 1e-3);
+        REQUIRE(std::isfinite(scaling->attn_factor), "attn_factor must be finite");
         fr.m = scaling->attn_factor > 0.0 ? scaling->attn_factor : 0.1 * std::log(s) + 1.0;
     }
     for (int i = 0; i < rope_dim / 2; ++i) {
@@ -780,11 +781,11 @@ EI_API int ei_attn_packed(ei_stream_t stream, const float* q, long q_stride, con
     const long qw = (long)n_head * head_dim, kw = (long)n_head_kv * head_dim;
     REQUIRE(q_stride >= qw && q_stride % 4 == 0, "q_stride %ld", q_stride);
     REQUIRE(kv_stride >= kw && kv_stride % 4 == 0 && kv_stride <= (1L << 22), "kv_stride %ld", kv_stride);
-    const size_t ob = span_bytes(rows, qw, qw);
-    REQUIRE(!overlap(out, ob, q, span_bytes(rows, q_stride, qw)) &&
-                !overlap(out, ob, k, span_bytes(rows, kv_stride, kw)) &&
-                !overlap(out, ob, v, span_bytes(rows, kv_stride, kw)),
-            "out overlaps q, k or v");
+    const size_t ob = span_bytes(rows, qw, qw), wb = ei::packed_ws_bytes(rows, n_head, n_head_kv);
+    const size_t qb = span_bytes(rows, q_stride, qw), kb = span_bytes(rows, kv_stride, kw);
+    REQUIRE(!overlap(out, ob, q, qb) && !overlap(out, ob, k, kb) && !overlap(out, ob, v, kb), "out overlaps q, k or v");
+    REQUIRE(!overlap(ws, wb, q, qb) && !overlap(ws, wb, k, kb) && !overlap(ws, wb, v, kb),
+            "workspace overlaps q, k or v");
     if (rows == 0) return ok();
     ei::PackedArgs a{};
     a.q = q, a.q_stride = q_stride;
@@ -808,7 +809,10 @@ EI_API int ei_attn_packed_paged(ei_stream_t stream, const float* q, long q_strid
         return e;
     REQUIRE(q && aligned16(q), "q missing or not 16-byte aligned");
     REQUIRE(q_stride >= qw && q_stride % 4 == 0, "q_stride %ld", q_stride);
-    REQUIRE(!overlap(out, span_bytes(rows, qw, qw), q, span_bytes(rows, q_stride, qw)), "out overlaps q");
+    const size_t qb = span_bytes(rows, q_stride, qw);
+    REQUIRE(!overlap(out, span_bytes(rows, qw, qw), q, qb) &&
+                !overlap(ws, ei::packed_ws_bytes(rows, n_head, n_head_kv), q, qb),
+            "out or workspace overlaps q");
     if (rows == 0) return ok();
     ei::PackedArgs a{};
     a.q = q, a.q_stride = q_stride;

@@ -9,7 +9,7 @@
 namespace ei {
 
 constexpr int kKT = 32;         // keys per tile
-constexpr int kFewRows = 32;    // units of up to so many rows go to k_packed_few
+constexpr int kFewRows = 32;    // a sequence's last unit of up to so many rows: few_pass
 
 // ------------------------------------------------------------------ the plan
 // The query rows of a sequence and KV head are taken flat, row f = token * G + head of the group, and
@@ -360,7 +360,7 @@ __device__ __forceinline__ int row_owner(const int4* seq, int n_seq, int b, int 
 // Few-row units (few_pass), single tokens and short drafts, read much and multiply little: every wave holds
 // the same rows and a tile of its own, loaded straight into the operands' registers, and multiplies in
 // fp32, which needs no planes.  (Both kinds of pass in one loop leave the compiler short of registers in
-// both: they are a workgroup's role.)
+// both: a workgroup walks its wide units first, then its few-row ones.)
 typedef __amdgpu_buffer_rsrc_t Rsrc;
 constexpr int kQB = 32;                         // flat rows per wave
 constexpr int kSlots = kUnitRows / kQB;         // waves per key group

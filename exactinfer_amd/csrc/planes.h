@@ -1,5 +1,6 @@
-// planes.h — fp32 operands on bf16 matrix cores: the three-plane split and its product, shared by the
-// attention kernels of prefill.hip and packed.hip.
+// planes.h — what the attention kernels of prefill.hip and packed.hip share (vector types, index
+// arithmetic, values kept from being hoisted), and prefill.hip's fp32 operands on bf16 matrix cores:
+// the three-plane split and its product.
 #pragma once
 
 #include "common.h"

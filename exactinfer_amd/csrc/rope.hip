@@ -28,19 +28,18 @@ __global__ __launch_bounds__(256) void k_rope_table(float2* __restrict__ cs, lon
 //                other; the other lanes two pieces each of the rest of the head
 //   interleaved  lane l holds the pieces at 4l and 64 + 4l, two pairs each
 // Otherwise lane l holds elements l + 16j and reads the partners from the row itself, all before the
-// head is written.  A group of sixteen lanes takes `heads_per` heads of one row, 16 / its row's share
-// of the workgroup apart, so that its table entries are read once.
-template <bool kHalf, bool kVec, bool kNorm, int kHeads>
+// head is written.
+template <bool kHalf, bool kVec, bool kNorm>
 __global__ __launch_bounds__(256) void k_rope_rows(const float* x, long x_stride, float* y, long y_stride,
                                                    int rows, int n_heads, const float* __restrict__ gamma, float eps,
                                                    const float2* __restrict__ cs, int n_pos,
-                                                   const int* __restrict__ pos, int rope_dim, int groups) {
+                                                   const int* __restrict__ pos, int rope_dim) {
 #pragma clang fp contract(off)
     const int lane = threadIdx.x & 15;
-    const long unit = (long)blockIdx.x * 16 + (threadIdx.x >> 4);
-    const long b = unit / groups;
-    if (b >= rows) return;  // a whole group of sixteen; no barrier here
-    const int h0 = (int)(unit - b * groups) * kHeads;
+    const uint32_t unit = blockIdx.x * 16 + (threadIdx.x >> 4);  // (below 2^31 + 15)
+    const uint32_t b = unit / (uint32_t)n_heads;
+    if (b >= (uint32_t)rows) return;  // a whole group of sixteen; no barrier here
+    const int h = (int)(unit - b * (uint32_t)n_heads);
     const int p = pos[b], half = rope_dim >> 1;
     const bool in = p >= 0 && p < n_pos;
     const float2* row = cs + (size_t)(in ? p : 0) * half;
@@ -56,20 +55,17 @@ __global__ __launch_bounds__(256) void k_rope_rows(const float* x, long x_stride
 #pragma unroll
         for (int j = 0; j < 8; ++j) g[j] = gamma[at(j)];
     }
-    float v[kHeads][8];
+    float v[8];
+    const float* src = x + (size_t)b * x_stride + (size_t)h * kHeadDim;
+    if constexpr (kVec) {
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-        const float* src = x + (size_t)b * x_stride + (size_t)min(h0 + i, n_heads - 1) * kHeadDim;
-        if constexpr (kVec) {
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                const float4 t = *reinterpret_cast<const float4*>(src + at(4 * k));
-                v[i][4 * k] = t.x, v[i][4 * k + 1] = t.y, v[i][4 * k + 2] = t.z, v[i][4 * k + 3] = t.w;
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = src[at(j)];
+        for (int k = 0; k < 2; ++k) {
+            const float4 t = *reinterpret_cast<const float4*>(src + at(4 * k));
+            v[4 * k] = t.x, v[4 * k + 1] = t.y, v[4 * k + 2] = t.z, v[4 * k + 3] = t.w;
         }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = src[at(j)];
     }
     // the pairs' (cos, sin): kVec half 4 of one pair per piece, interleaved 2 per piece; else one per value
     float2 t[kVec ? 4 : 8];
@@ -89,74 +85,67 @@ __global__ __launch_bounds__(256) void k_rope_rows(const float* x, long x_stride
             if (e < rope_dim) t[j] = row[kHalf ? (e < half ? e : e - half) : e >> 1];
         }
     }
+    float inv = 1.f;
+    if constexpr (kNorm) {
+        double ss = 0.0;
 #pragma unroll
-    for (int i = 0; i < kHeads; ++i) {
-        if (h0 + i >= n_heads) break;
-        float inv = 1.f;
-        if constexpr (kNorm) {
-            double ss = 0.0;
+        for (int j = 0; j < 8; ++j) ss = __builtin_fma((double)v[j], (double)v[j], ss);
+        ss += lane_xor_f64<1>(ss);
+        ss += lane_xor_f64<2>(ss);
+        ss += lane_xor_f64<4>(ss);
+        ss += lane_xor_f64<8>(ss);
+        inv = (float)(1.0 / sqrt(ss / (double)kHeadDim + (double)eps));
+    }
+    auto scaled = [&](float f, int j) { return kNorm ? (f * inv) * g[j] : f; };
+    float w[8];
+    if (!in) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) ss = __builtin_fma((double)v[i][j], (double)v[i][j], ss);
-            ss += lane_xor_f64<1>(ss);
-            ss += lane_xor_f64<2>(ss);
-            ss += lane_xor_f64<4>(ss);
-            ss += lane_xor_f64<8>(ss);
-            inv = (float)(1.0 / sqrt(ss / (double)kHeadDim + (double)eps));
-        }
-        float w[8];
-        if (in) {
-            auto scaled = [&](float f, int j) { return kNorm ? (f * inv) * g[j] : f; };
-            if constexpr (kVec) {
+        for (int j = 0; j < 8; ++j) w[j] = v[j];
+    } else if constexpr (kVec) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) w[j] = scaled(v[i][j], j);
-                if constexpr (kHalf) {
-                    if (lane < (rope_dim >> 3)) {
+        for (int j = 0; j < 8; ++j) w[j] = scaled(v[j], j);
+        if constexpr (kHalf) {
+            if (lane < (rope_dim >> 3)) {
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const float a = w[j], c = w[4 + j];
-                            const float ac = a * t[j].x, cn = c * t[j].y, an = a * t[j].y, cc = c * t[j].x;
-                            w[j] = ac - cn, w[4 + j] = an + cc;
-                        }
-                    }
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; j += 2)
-                        if (at(j) < rope_dim) {
-                            const float a = w[j], c = w[j + 1];
-                            const float2 q = t[j >> 1];
-                            const float ac = a * q.x, cn = c * q.y, an = a * q.y, cc = c * q.x;
-                            w[j] = ac - cn, w[j + 1] = an + cc;
-                        }
-                }
-            } else {
-                const float* src = x + (size_t)b * x_stride + (size_t)(h0 + i) * kHeadDim;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int e = at(j);
-                    w[j] = scaled(v[i][j], j);
-                    if (e < rope_dim) {
-                        const bool first = kHalf ? e < half : (e & 1) == 0;
-                        const int o = kHalf ? (first ? e + half : e - half) : e ^ 1;
-                        const float other = kNorm ? (src[o] * inv) * gamma[o] : src[o];
-                        const float own_c = w[j] * t[j].x, other_s = other * t[j].y;
-                        w[j] = first ? own_c - other_s : other_s + own_c;
-                    }
+                for (int j = 0; j < 4; ++j) {
+                    const float a = w[j], c = w[4 + j];
+                    const float ac = a * t[j].x, cn = c * t[j].y, an = a * t[j].y, cc = c * t[j].x;
+                    w[j] = ac - cn, w[4 + j] = an + cc;
                 }
             }
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) w[j] = v[i][j];
+            for (int j = 0; j < 8; j += 2)
+                if (at(j) < rope_dim) {
+                    const float a = w[j], c = w[j + 1];
+                    const float2 q = t[j >> 1];
+                    const float ac = a * q.x, cn = c * q.y, an = a * q.y, cc = c * q.x;
+                    w[j] = ac - cn, w[j + 1] = an + cc;
+                }
         }
-        float* dst = y + (size_t)b * y_stride + (size_t)(h0 + i) * kHeadDim;
-        if constexpr (kVec) {
+    } else {
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
-                *reinterpret_cast<float4*>(dst + at(4 * k)) =
-                    make_float4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) dst[at(j)] = w[j];
+        for (int j = 0; j < 8; ++j) {
+            const int e = at(j);
+            w[j] = scaled(v[j], j);
+            if (e < rope_dim) {
+                const bool first = kHalf ? e < half : (e & 1) == 0;
+                const int o = kHalf ? (first ? e + half : e - half) : e ^ 1;
+                const float other = kNorm ? (src[o] * inv) * gamma[o] : src[o];
+                const float own_c = w[j] * t[j].x, other_s = other * t[j].y;
+                w[j] = first ? own_c - other_s : other_s + own_c;
+            }
         }
+    }
+    float* dst = y + (size_t)b * y_stride + (size_t)h * kHeadDim;
+    if constexpr (kVec) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+            *reinterpret_cast<float4*>(dst + at(4 * k)) =
+                make_float4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) dst[at(j)] = w[j];
     }
 }
 
@@ -172,10 +161,9 @@ template <bool kHalf, bool kVec, bool kNorm>
 static hipError_t launch_rope_rows_as(hipStream_t st, const float* x, long x_stride, float* y, long y_stride, int rows,
                                       int n_heads, const float* gamma, float eps, const float2* cs, int n_pos,
                                       const int* pos, int rope_dim) {
-    const int groups = n_heads;
-    const long blocks = ((long)rows * groups + 15) / 16;
-    k_rope_rows<kHalf, kVec, kNorm, 1><<<(unsigned)blocks, 256, 0, st>>>(x, x_stride, y, y_stride, rows, n_heads, gamma,
-                                                                       eps, cs, n_pos, pos, rope_dim, groups);
+    const long blocks = ((long)rows * n_heads + 15) / 16;
+    k_rope_rows<kHalf, kVec, kNorm><<<(unsigned)blocks, 256, 0, st>>>(x, x_stride, y, y_stride, rows, n_heads, gamma,
+                                                                    eps, cs, n_pos, pos, rope_dim);
     return hipGetLastError();
 }
 

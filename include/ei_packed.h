@@ -8,8 +8,8 @@
  *
  * A batch holds n_seq sequences whose new rows follow one another: rows cu_rows[s] ..
  * cu_rows[s+1] - 1 (device int32 [n_seq + 1], from 0 up, never falling, cu_rows[n_seq] <= rows) belong
- * to sequence s, which may have none.  Rows from cu_rows[n_seq] on belong to nobody: they are neither
- * read nor written.
+ * to sequence s, which may have none.  Rows from cu_rows[n_seq] on belong to nobody: nothing is
+ * written there, and it does not matter what they hold.
  */
 #ifndef EI_PACKED_H
 #define EI_PACKED_H
@@ -92,7 +92,7 @@ size_t ei_packed_ws_bytes(int rows, int n_head, int n_head_kv);
  * softmax in fp32.  Outputs differ from ei_attn_prefill's and ei_attn_decode's in the last bits, and with
  * the batch a sequence is in; a batch called twice gives the same bits.  Key and value rows that a
  * row does not see never reach it, whatever they hold.  Infinite or NaN values in K or V, or a V whose
- * largest values are 2^15 times a row's sums, make the waves that meet them take their keys again in
+ * largest values are 2^16 times a row's outputs, make the waves that meet them take their keys again in
  * fp32, some ten times slower. */
 int ei_attn_packed(ei_stream_t stream, const float* q, long q_stride, const float* k, const float* v,
                    long kv_stride, float* out, int n_seq, int rows, int n_head, int n_head_kv, int head_dim,

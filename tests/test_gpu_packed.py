@@ -694,3 +694,22 @@ def test_python_refusals(gpu):
         gpu.attn_packed(q, k, v, b, shape)
     b.plan(_i32([0, 0]), 0, 8)
     assert gpu.attn_packed(q, k, v, b, shape).shape == (0, H, D)
+    with pytest.raises(ValueError, match="GPU tensor"):
+        gpu.PackedBatch(2, 8, H, HKV, device="cpu").plan(_i32([0, 8]), 8, 8)
+
+
+def test_single_rows_of_any_stride(gpu):
+    """The stride of a one-row view is not used: rows of buffers whose width is no multiple of four serve, and
+    keys and values of buffers of different widths."""
+    H, HKV = 16, 8
+    _, q, k, v = _prompts(H, HKV, [1], 92)
+    q1, k1 = torch.zeros((3, H * D + 1), device="cuda")[:1, :H * D], torch.zeros((2, HKV * D + 64), device="cuda")[:1]
+    q1.copy_(q)
+    k1[:, :HKV * D].copy_(k)
+    b = gpu.PackedBatch(1, 1, H, HKV)
+    b.plan(_i32([0, 1]), 1, 1)
+    out = gpu.attn_packed(q1, k1[:, :HKV * D], v.contiguous(), b, gpu.AttnShape(H, HKV))
+    assert torch.equal(out, gpu.attn_packed(q, k, v, b, gpu.AttnShape(H, HKV)))
+    cs = gpu.rope_table_scaled(16, D, 1e6)
+    pos = _i32([9])
+    assert torch.equal(gpu.rope_rows(q1, H, cs, pos), gpu.rope_rows(q, H, cs, pos))

@@ -55,6 +55,7 @@ def test_table_arguments(match, args):
     ("beta_fast", dict(kind=3, factor=2.0, beta_fast=0.5), 128),
     ("beta_fast", dict(kind=3, factor=2.0, beta_slow=0.0), 128),
     ("beta_fast", dict(kind=3, factor=2.0, beta_fast=float("nan")), 128),
+    ("attn_factor", dict(kind=3, factor=2.0, attn_factor=float("inf")), 128),
 ])
 def test_scaling_arguments(match, kw, rope_dim):
     _refused(match, "ei_rope_table_scaled", None, P, 16, rope_dim, 1e6, _scaling(**kw))
@@ -209,6 +210,9 @@ POOL = [
     ("overlaps q", dict(out=_off(FAR[0], 6144))),
     ("overlaps q", dict(out=FAR[5], k=FAR[5])),
     ("overlaps q", dict(out=FAR[5], v=_off(FAR[5], 4096))),
+    ("workspace overlaps", dict(ws=_off(FAR[0], 4096))),
+    ("workspace overlaps", dict(ws=FAR[5], k=FAR[5])),
+    ("workspace overlaps", dict(ws=FAR[5], v=FAR[5])),
 ])
 def test_packed_arguments(match, kw):
     _refused(match, "ei_attn_packed", *_packed(**kw))
@@ -218,6 +222,7 @@ def test_packed_arguments(match, kw):
     ("q missing", dict(q=None)),
     ("q_stride", dict(qs=4092)),
     ("overlaps q", dict(out=_off(FAR[0], 4096))),
+    ("workspace overlaps", dict(ws=_off(FAR[0], 4096))),
 ])
 def test_paged_arguments(match, kw):
     _refused(match, "ei_attn_packed_paged", *_paged(**kw))
