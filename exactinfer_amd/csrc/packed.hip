@@ -21,10 +21,14 @@ constexpr int kFewRows = 32;    // a sequence's last unit of up to so many rows:
 // tiles, and something for what is done once per unit.  Of the wide list each workgroup first takes whole
 // units, dealt out in descending order of tiles and back and forth, round by round, so that the
 // workgroups walk units of about the same keys at the same time (their tiles meet in the XCD's L2); the
-// last units (the smallest: one to two rounds of them, or all if there are fewer) are laid end to end on
-// a line, of which each gets what is missing to an equal share.  The few-row units lie on a line of their
-// own, of which each workgroup gets what its wide work leaves of an equal share of everything.  A cut may
-// fall inside a unit: its parts are merged by k_packed_combine.
+// rest (less than a round, or the last full one too, if some workgroup would have more than an equal share with
+// it) is laid end to end on a line, of which each gets what is missing to an equal share.  The few-row units
+// lie on a line of their own, of which each workgroup gets what its wide work leaves of an equal share of
+// everything.  A cut may fall inside a unit: its parts are merged by k_packed_combine.
+//
+// Dealing the last full round, against leaving it on the line in any case (H 32, HKV 8): 8 prompts of 250
+// rows 42 us against 52, one of 2048 132 against 145, 1500 rows after 8000 keys 729 against 770, 1024 after
+// 30000 with a prompt of 400 1747 against 1810; at worst (H 40, prompts of 900 and 700) 97 against 89.
 //
 // Order and cuts follow from the lengths alone (no atomics decide them), so a batch planned twice
 // gives the same bits twice.
@@ -76,6 +80,9 @@ constexpr int kPlanThreads = 512;
 constexpr int kPlanSeqLds = 1024;       // sequences held in LDS (more are read from the plan)
 constexpr int kPlanLineLds = 512;       // units of a line held in LDS (likewise)
 constexpr long kMaxRankWork = 1 << 20;  // wide units x sequences up to which units are sorted
+constexpr int kDealSlack = 32;          // whole units may pass an equal share by 1/32 (by 1/128: 1024 rows after
+                                        // 30000 keys take 1770 us instead of 1715; by all of it: H 64, prompts of
+                                        // 600 rows after 9000 keys, 300 and 200, 928 instead of 644)
 
 // What a list's work costs, in tiles: `pass` for everything done once per unit or part of one; a cut leaves
 // whole turns (the tiles that a workgroup's waves take at a time, a power of two) on both sides, and keeps off a unit's
@@ -127,6 +134,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
     __shared__ int4 seq_lds[kPlanSeqLds];
     __shared__ Unit wide_lds[kPlanLineLds], few_lds[kPlanLineLds];  // the lines' units
     __shared__ unsigned long long load[kPackedCus], few_cost, wide_cost;
+    __shared__ int last_round[kPackedCus];  // the cost of the units of the last full round, share by share
     __shared__ int2 cuts[kPackedCus + 1];
     __shared__ long long cut_cost[kPackedCus + 1];  // the line's cost before each cut
     __shared__ long long line_at[kPlanThreads];     // units of the line: cost before, tiles
@@ -258,14 +266,14 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
         return m >= e.y ? 0 : nw - min(nw, (int)(m * G / kUnitRows));
     };
     // (sorting costs units x sequences: where that is much, there is enough work for the order not to matter)
-    const int rounds = (long long)U * n_seq <= kMaxRankWork && U / shares > 1 ? U / shares - 1 : 0;
-    const int dealt = rounds * shares, line = U - dealt;
+    const int full = (long long)U * n_seq <= kMaxRankWork ? U / shares : 0, sure = max(full - 1, 0) * shares;
     long long mine = 0;
     for (int i = tid; i < U; i += kPlanThreads) {
         const Unit x = unit(i);
-        mine += x.tiles + kWideCost.pass;
+        const int cost = x.tiles + kWideCost.pass;
+        mine += cost;
         int at = i;
-        if (rounds > 0) {
+        if (full > 0) {
             // units before this one: more tiles, or as many in an earlier sequence, or later in its own
             at = 0;
 #pragma unroll 4
@@ -275,23 +283,29 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
             }
         }
         pv.wide.units[at] = x;
-        if (at < dealt) {
-            const int r = at / shares, j = at - r * shares;
-            atomicAdd(&load[(r & 1) ? shares - 1 - j : j], (unsigned long long)(x.tiles + kWideCost.pass));
-        } else if (at - dealt < kPlanLineLds) wide_lds[at - dealt] = x;
+        const int r = at / shares, j = at - r * shares;
+        if (at < sure) atomicAdd(&load[(r & 1) ? shares - 1 - j : j], (unsigned long long)cost);
+        else if (r < full) last_round[(r & 1) ? shares - 1 - j : j] = cost;
+        if (at >= sure && at - sure < kPlanLineLds) wide_lds[at - sure] = x;
     }
     mine = wave_scan(mine);
     if ((tid & 63) == 63 && mine > 0) atomicAdd(&wide_cost, (unsigned long long)mine);
     __syncthreads();
+    // all rounds, or all but one
+    const long long both = (long long)ceil((double)(wide_cost + few_cost) / shares);
+    const bool over = full > 0 && tid < shares && (long long)load[tid] + last_round[tid] > both + both / kDealSlack;
+    const int rounds = __syncthreads_or(over) ? full - 1 : full;
+    const int dealt = rounds * shares, line = U - dealt;
+    if (rounds > 0 && rounds == full && tid < shares) load[tid] += last_round[tid];
     {
         const long long share = (long long)ceil((double)wide_cost / shares);
         long long before = tid * share, all;
         if (rounds > 0) before = block_scan(tid < shares ? max(share - (long long)load[tid], 0LL) : 0, &all);
-        cut_line(pv.wide, rounds, line, kWideCost, line <= kPlanLineLds ? wide_lds : nullptr, share, before);
+        cut_line(pv.wide, rounds, line, kWideCost, U - sure <= kPlanLineLds ? wide_lds + (dealt - sure) : nullptr, share,
+                 before);
     }
     {
         const long long share = (long long)ceil((double)few_cost / shares);
-        const long long both = (long long)ceil((double)(wide_cost + few_cost) / shares);
         const long long wide = tid < shares ? (long long)load[tid] + cut_cost[tid + 1] - cut_cost[tid] : 0;
         long long all;
         const long long before = block_scan(tid < shares ? max(both - wide, 0LL) : 0, &all);
