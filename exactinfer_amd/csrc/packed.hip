@@ -425,18 +425,32 @@ struct Pass {
     float* part;           // where its unnormalised rows go, or null: a whole unit
 };
 
+// What earlier launches wrote and this one only reads, at a wave-uniform address, by a scalar load: after the
+// kernel's own stores the compiler would take a vector load, whose wait is for every load before it too.
+template <typename T>
+__device__ __forceinline__ T scalar_load(const T* at) {
+    return *reinterpret_cast<const __attribute__((address_space(4))) T*>(reinterpret_cast<uintptr_t>(at));
+}
+
+// The pool block of the page that holds key t0 of the pass's sequence, -1 past the table's end.
+template <bool kPaged>
+__device__ __forceinline__ int page_of(const PackedArgs& a, const Pass& p, int t0) {
+    if constexpr (!kPaged) return 0;
+    const int blk = t0 >> a.bshift;
+    const int e = scalar_load(a.btab + (size_t)p.seq * a.max_blocks + min(blk, a.max_blocks - 1));
+    return blk < a.max_blocks ? e : -1;
+}
+
 // The visible rows of a tile as a buffer: reads past the last one, and of a missing page, give zeros (all
 // reads, if the tile is not `wanted`).
 template <bool kPaged>
-__device__ __forceinline__ Rsrc tile_rsrc(const PackedArgs& a, const Pass& p, const float* cache, int t0,
+__device__ __forceinline__ Rsrc tile_rsrc(const PackedArgs& a, const Pass& p, const float* cache, int t0, int page,
                                           bool wanted = true) {
     size_t row = (size_t)p.row0 + t0;
     int there = wanted ? min(kKT, p.T - t0) : 0;
     if constexpr (kPaged) {
-        const int blk = t0 >> a.bshift;
-        const int phys = blk < a.max_blocks ? a.btab[(size_t)p.seq * a.max_blocks + blk] : -1;
-        const bool ok = phys >= 0 && phys < a.n_blocks;
-        row = ok ? ((size_t)phys << a.bshift) | (size_t)(t0 & ((1 << a.bshift) - 1)) : 0;
+        const bool ok = page >= 0 && page < a.n_blocks;
+        row = ok ? ((size_t)page << a.bshift) | (size_t)(t0 & ((1 << a.bshift) - 1)) : 0;
         if (!ok) there = 0;
     }
     return __builtin_amdgcn_make_buffer_rsrc(
@@ -661,16 +675,17 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
     const int nfull = max(p.pos0 + fdiv(min(f0, p.nflat - 1), fG) + 1, 0) / kKT;  // tiles below the wave's diagonal
     const int n_it = (p.nrange + kGroups - 1) / kGroups, n_mine = (p.nrange - grp + kGroups - 1) / kGroups;
     auto index = [&](int i) { return p.kt_lo + kGroups * i + grp; };
-    auto k_tile = [&](int i) { return tile_rsrc<kPaged>(a, p, a.k + (size_t)kvh * D, index(i) * kKT); };
-    auto v_tile = [&](int i) { return tile_rsrc<kPaged>(a, p, a.v + (size_t)kvh * D, index(i) * kKT); };
+    auto page = [&](int i) { return page_of<kPaged>(a, p, index(i) * kKT); };
+    auto k_tile = [&](int i, int pg) { return tile_rsrc<kPaged>(a, p, a.k + (size_t)kvh * D, index(i) * kKT, pg); };
+    auto v_tile = [&](int i, int pg) { return tile_rsrc<kPaged>(a, p, a.v + (size_t)kvh * D, index(i) * kKT, pg); };
 
     // K and V of this group's i-th tile, a quarter per wave:
     //   K: row 8*hw + lane/8, d = 8c .. 8c+7 and 64 + 8c .. (c = lane%8)
     //   V: d = 32*hw + 2*(lane%16) and the next, the eight keys of chunk lane/16 (step s = chunk/2,
     //     half hh = chunk%2 of the P.V operand: keys 16s + 4hh + {0..3, 8..11})
     float rg[16];
-    auto load_k = [&](int i) {
-        const Rsrc rs = k_tile(i);
+    auto load_k = [&](int i, int pg) {
+        const Rsrc rs = k_tile(i, pg);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(rs, voff_k + 256 * (j >> 1) + 16 * (j & 1), 0, 0);
@@ -678,8 +693,8 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
             rg[4 * j + 2] = __uint_as_float(v.z), rg[4 * j + 3] = __uint_as_float(v.w);
         }
     };
-    auto load_v = [&](int i) {
-        const Rsrc rs = v_tile(i);
+    auto load_v = [&](int i, int pg) {
+        const Rsrc rs = v_tile(i, pg);
         const uint32_t off = unhoisted(voff_v);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -764,7 +779,8 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
             }
         }
     }
-    if (n_mine > 0) load_k(0);
+    int pg = page(0);  // of the tile that is loaded next
+    if (n_mine > 0) load_k(0, pg);
     wait_vmcnt<0>();
     lds_barrier();
     Halves qp[8];
@@ -796,7 +812,8 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
     if (n_mine > 0) {
 #pragma unroll
         for (int x = 0; x < 2; ++x) conv_k(x, 0);
-        load_v(0);
+        load_v(0, pg);
+        pg = page(1);
     }
     Sums x;
     x.clear();
@@ -817,7 +834,7 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
                 if (t == 2 || t == 4) conv_v(t == 4);
                 mfma_halves(kf[t & 1], qp[t], s);
             }
-            if (i + 1 < n_mine) load_k(i + 1);
+            if (i + 1 < n_mine) load_k(i + 1, pg);
             const float* ks = k_scale + kKT * (i & 1) + 4 * hh;
 #pragma unroll
             for (int r = 0; r < 16; r += 4) {
@@ -851,7 +868,8 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
                 if (y == 4 || y == 6) conv_k(y == 6, (i + 1) & 1);
                 mfma_halves(vf[y & 1], pp, x.o[y & 3]);
             }
-            if (more) load_v(i + 1);
+            if (more) load_v(i + 1, pg);
+            pg = page(i + 2);  // (looked up here, its wait is the barrier's)
             __builtin_amdgcn_s_setprio(0);
         }
         lds_barrier();
@@ -861,7 +879,9 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
     if (planes_failed(x, scale) && live) {
         const int f = min(f0 + col, p.nflat - 1), t0 = fdiv(f, fG);
         const float* q_row = a.q + ((size_t)p.row0 + t0) * a.q_stride + (size_t)(kvh * G + f - t0 * G) * D;
-        redo_fp32(x, a, p, q_row, sl2, n_mine, k_tile, v_tile, index, nfull, qpos, row_bytes,
+        redo_fp32(
+            x, a, p, q_row, sl2, n_mine, [&](int i) { return k_tile(i, page(i)); },
+            [&](int i) { return v_tile(i, page(i)); }, index, nfull, qpos, row_bytes,
                   smem + w * (kXchF * 64), lane);
     }
 
@@ -937,11 +957,12 @@ __device__ __forceinline__ void few_pass(const PackedArgs& a, const Pass& p, int
     const int nfull = max(p.pos0 + fdiv(f0, fG) + 1, 0) / kKT;
     const int n_mine = (p.nrange - wu + kWaves - 1) / kWaves;
     auto index = [&](int i) { return p.kt_lo + kWaves * i + wu; };
-    auto k_tile = [&](int i, bool wanted = true) {
-        return tile_rsrc<kPaged>(a, p, a.k + (size_t)kvh * D, index(i) * kKT, wanted);
+    auto page = [&](int i) { return page_of<kPaged>(a, p, index(i) * kKT); };
+    auto k_tile = [&](int i, int pg, bool wanted = true) {
+        return tile_rsrc<kPaged>(a, p, a.k + (size_t)kvh * D, index(i) * kKT, pg, wanted);
     };
-    auto v_tile = [&](int i, bool wanted = true) {
-        return tile_rsrc<kPaged>(a, p, a.v + (size_t)kvh * D, index(i) * kKT, wanted);
+    auto v_tile = [&](int i, int pg, bool wanted = true) {
+        return tile_rsrc<kPaged>(a, p, a.v + (size_t)kvh * D, index(i) * kKT, pg, wanted);
     };
     u32x4 kr[2][8], vr[8][2];
     auto load_k = [&](const Rsrc& rs, int x, uint32_t off) {
@@ -962,14 +983,9 @@ __device__ __forceinline__ void few_pass(const PackedArgs& a, const Pass& p, int
         const uint32_t ln = lane_now();
         return (ln >> 4) * 4 * row_bytes + 16 * (ln & 15);
     };
-    if (n_mine > 0) {
-        const Rsrc rk = k_tile(0), rv = v_tile(0);
-#pragma unroll
-        for (int x = 0; x < 8; ++x) load_k(rk, x, k_offset());
-#pragma unroll
-        for (int t = 0; t < 8; ++t) load_v(rv, t, v_offset());
-    }
-    // q by the first rows' lanes; more than sixteen rows' through LDS (registers), [row][d]
+    int pg = page(0);  // of the tile that is loaded next
+    // q first (a wait for it is not one for the tiles), by the first rows' lanes; more than sixteen rows' goes
+    // through LDS (registers), [row][d]
     int qpos[kBlocks];  // (rows past the last repeat it)
 #pragma unroll
     for (int rb = 0; rb < kBlocks; ++rb) qpos[rb] = p.pos0 + fdiv(min(f0 + kFewBlock * rb + j, last), fG);
@@ -977,17 +993,34 @@ __device__ __forceinline__ void few_pass(const PackedArgs& a, const Pass& p, int
         const int tok = fdiv(f, fG);
         return a.q + ((size_t)p.row0 + tok) * a.q_stride + (size_t)(kvh * G + f - tok * G) * D;
     };
-    auto scaled = [&](const float4& v) { return f32x4{v.x * sl2, v.y * sl2, v.z * sl2, v.w * sl2}; };
-    f32x4 q[kBlocks == 1 ? 8 : 1];
+    float4 q_raw[kBlocks == 1 ? 8 : 2];
     if constexpr (kBlocks == 1) {
         const float* src = q_row(min(f0 + j, last)) + 4 * quarter;
 #pragma unroll
-        for (int x = 0; x < 8; ++x) q[x] = scaled(*reinterpret_cast<const float4*>(src + 16 * x));
+        for (int x = 0; x < 8; ++x) q_raw[x] = *reinterpret_cast<const float4*>(src + 16 * x);
     } else {
         const float* src = q_row(min(f0 + (tid >> 4), last)) + 8 * (tid & 15);
+        q_raw[0] = *reinterpret_cast<const float4*>(src);
+        q_raw[1] = *reinterpret_cast<const float4*>(src + 4);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    if (n_mine > 0) {
+        const Rsrc rk = k_tile(0, pg), rv = v_tile(0, pg);
+#pragma unroll
+        for (int x = 0; x < 8; ++x) load_k(rk, x, k_offset());
+#pragma unroll
+        for (int t = 0; t < 8; ++t) load_v(rv, t, v_offset());
+        pg = page(1);
+    }
+    auto scaled = [&](const float4& v) { return f32x4{v.x * sl2, v.y * sl2, v.z * sl2, v.w * sl2}; };
+    f32x4 q[kBlocks == 1 ? 8 : 1];
+    if constexpr (kBlocks == 1) {
+#pragma unroll
+        for (int x = 0; x < 8; ++x) q[x] = scaled(q_raw[x]);
+    } else {
         float* dst = smem + (tid >> 4) * kRowF + 8 * (tid & 15);
-        *reinterpret_cast<f32x4*>(dst) = scaled(*reinterpret_cast<const float4*>(src));
-        *reinterpret_cast<f32x4*>(dst + 4) = scaled(*reinterpret_cast<const float4*>(src + 4));
+        *reinterpret_cast<f32x4*>(dst) = scaled(q_raw[0]);
+        *reinterpret_cast<f32x4*>(dst + 4) = scaled(q_raw[1]);
         lds_barrier();
     }
     auto q_at = [&](int rb, int x) -> f32x4 {
@@ -1006,7 +1039,7 @@ __device__ __forceinline__ void few_pass(const PackedArgs& a, const Pass& p, int
     for (int i = 0; i < n_mine; ++i) {
         const bool more = i + 1 < n_mine;
         const int kt = index(i);
-        const Rsrc rk = k_tile(more ? i + 1 : i, more), rv = v_tile(more ? i + 1 : i, more);
+        const Rsrc rk = k_tile(more ? i + 1 : i, pg, more), rv = v_tile(more ? i + 1 : i, pg, more);
         f32x4 s[kBlocks][2];
 #pragma unroll
         for (int rb = 0; rb < kBlocks; ++rb) s[rb][0] = s[rb][1] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -1057,6 +1090,7 @@ __device__ __forceinline__ void few_pass(const PackedArgs& a, const Pass& p, int
             }
         }
         const uint32_t off_v = v_offset();
+        pg = page(i + 2);
 #pragma unroll
         for (int t = 0; t < 8; ++t) {
 #pragma unroll
@@ -1091,7 +1125,8 @@ __device__ __forceinline__ void few_pass(const PackedArgs& a, const Pass& p, int
                 l[rb] = 0.f;
 #pragma unroll 1
                 for (int c = 0; c < n_mine * kKT; ++c) {
-                    const Rsrc rk = k_tile(c / kKT), rv = v_tile(c / kKT);
+                    const int at = page(c / kKT);
+                    const Rsrc rk = k_tile(c / kKT, at), rv = v_tile(c / kKT, at);
                     const uint32_t row = (uint32_t)(c % kKT) * row_bytes;
                     if (index(c / kKT) * kKT + c % kKT > qpos[rb]) continue;
                     float dot = 0.f;
@@ -1198,13 +1233,14 @@ __device__ __forceinline__ void walk_list(const PackedArgs& a, const List& list,
             p.kt_lo = i == first ? first_tile : 0;
         }
         // (the share's own copy comes with the line just read: no wait for a list entry)
-        const Unit x = *(pass == 0 ? &list.shares[share].start : list.units + at);
-        const int n = scalar(x.n), len = scalar(x.len);
-        p.seq = scalar(x.seq), p.u = scalar(x.u), p.row0 = scalar(x.row0);
+        const u32x4* unit = reinterpret_cast<const u32x4*>(pass == 0 ? &list.shares[share].start : list.units + at);
+        const u32x4 x = scalar_load(unit), y = scalar_load(unit + 1);  // a Unit's fields, in order
+        const int n = (int)x.y, len = (int)x.z;
+        p.row0 = (int)x.x, p.u = (int)x.w, p.seq = (int)y.x;
         p.pos0 = len - n;
         p.nflat = n * (int)fG.d;
         p.T = min(max(p.pos0 + fdiv(min(kUnitRows * p.u + kUnitRows, p.nflat) - 1, fG) + 1, 0), len);
-        p.nrange = (cut >= 0 ? cut : scalar(x.tiles)) - p.kt_lo;
+        p.nrange = (cut >= 0 ? cut : (int)y.y) - p.kt_lo;
         p.part = p.kt_lo > 0 || cut >= 0 ? parts + part_at(kFew, share * a.HKV + kvh, p.kt_lo > 0 ? 0 : 1) : nullptr;
         if (pass > 0) lds_barrier();  // the last pass's rows have been read
         if constexpr (kFew) {
