@@ -1267,15 +1267,69 @@ __global__ __launch_bounds__(64 * kWaves) void k_packed_attn(PackedArgs a, int s
     walk_list<kPaged, true>(a, pv.few, few, 0, shares, share, kvh, few_parts, smem);
 }
 
-// The units that the cuts divide: workgroup (share, KV head; 8 rows) merges the unit that starts in
+// The units that the cuts divide: workgroup (share, KV head; 32 rows) merges the unit that starts in
 // this share and goes on in the next ones.  Part p of it is the share's own (its slot 1), then slot 0 of
 // each share that it reaches.  o = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p over the parts that saw a
-// key (m = -inf and l = 0 otherwise; m = -inf with a NaN l counts).
-constexpr int kCombineRows = 8;
-constexpr int kCombineWide = kUnitRows / kCombineRows, kCombineFew = kFewRows / kCombineRows;
+// key (m = -inf and l = 0 otherwise; m = -inf with a NaN l counts).  A thread has four columns of one row, or
+// of four rows at a time (eight rows apart) where the unit has more than eight; the loads of 16 or 8 parts' rows
+// are in flight together, for what this takes is their latency.  Workgroups that find nothing to merge cost
+// too: with 8 rows each, four times as many, 32 single tokens at 475 keys take 28.5 us in all instead of 26.5.
+constexpr int kCombineRows = 8, kCombineSpan = 32;
+constexpr int kCombineWide = kUnitRows / kCombineSpan;
+static_assert(kFewRows == kCombineSpan, "one workgroup per few-row unit");
+template <int kRows, int kAtOnce>
+__device__ __forceinline__ void merge_rows(const PackedArgs& a, const Unit& x, int kvh, int G, const float* parts,
+                                           bool few, int share, int end, int row0) {
+    const int d = 4 * (threadIdx.x & 31);
+    float M[kRows], L[kRows];
+    float4 o[kRows];
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) M[r] = -INFINITY, L[r] = 0.f, o[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p = share; p <= end; p += kAtOnce) {
+        float2 ml[kAtOnce][kRows];
+        float4 v[kAtOnce][kRows];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int q = min(p + i, end);
+            const float* b = parts + part_at(few, q * a.HKV + kvh, q == share ? 1 : 0);
+#pragma unroll
+            for (int r = 0; r < kRows; ++r) {  // (rows past the unit's last: what the part has there, not written)
+                const int row = row0 + kCombineRows * r;
+                ml[i][r] = *reinterpret_cast<const float2*>(b + (few ? kFewRows : kUnitRows) * kHeadDim + 2 * row);
+                v[i][r] = *reinterpret_cast<const float4*>(b + row * kHeadDim + d);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+            float mn = M[r];
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i)
+                if (p + i <= end) mn = fmaxf(mn, ml[i][r].x);
+            const float c = M[r] == mn ? 1.f : __builtin_amdgcn_exp2f(M[r] - mn);
+            M[r] = mn;
+            L[r] *= c, o[r].x *= c, o[r].y *= c, o[r].z *= c, o[r].w *= c;
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) {
+                if (p + i > end || (ml[i][r].x == -INFINITY && ml[i][r].y == 0.f)) continue;
+                const float wv = __builtin_amdgcn_exp2f(ml[i][r].x - mn);
+                L[r] = __builtin_fmaf(wv, ml[i][r].y, L[r]);
+                o[r].x = __builtin_fmaf(wv, v[i][r].x, o[r].x), o[r].y = __builtin_fmaf(wv, v[i][r].y, o[r].y);
+                o[r].z = __builtin_fmaf(wv, v[i][r].z, o[r].z), o[r].w = __builtin_fmaf(wv, v[i][r].w, o[r].w);
+            }
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < kRows; ++r) {
+        const int f = kUnitRows * x.u + row0 + kCombineRows * r, t0 = f / G;
+        if (f >= x.n * G) break;
+        const float inv = x.len - x.n + t0 < 0 ? 0.f : 1.f / L[r];  // a row that sees no key: zeros
+        *reinterpret_cast<float4*>(a.out + (((size_t)x.row0 + t0) * a.H + kvh * G + f - t0 * G) * kHeadDim + d) =
+            make_float4(o[r].x * inv, o[r].y * inv, o[r].z * inv, o[r].w * inv);
+    }
+}
 __global__ __launch_bounds__(32 * kCombineRows) void k_packed_combine(PackedArgs a, bool prompts, int shares,
-                                                        const float* __restrict__ wide_parts,
-                                                        const float* __restrict__ few_parts) {
+                                                                      const float* __restrict__ wide_parts,
+                                                                      const float* __restrict__ few_parts) {
     const int kvh = blockIdx.x % a.HKV, share = blockIdx.x / a.HKV, G = a.H / a.HKV;
     const bool few = blockIdx.y >= kCombineWide;
     const PlanView pv = plan_view(const_cast<char*>(a.plan), a.n_seq, a.rows, G, shares);
@@ -1283,42 +1337,12 @@ __global__ __launch_bounds__(32 * kCombineRows) void k_packed_combine(PackedArgs
     const int end = list.shares[share].merge_end;
     const Unit x = list.shares[share].merge;
     if (!plan_fits(a.plan, a.n_seq, a.rows, a.H, a.HKV, prompts) || end == 0) return;
-    const int row = (few ? blockIdx.y - kCombineWide : blockIdx.y) * kCombineRows + (threadIdx.x >> 5);
-    const int f = kUnitRows * x.u + row, d = 4 * (threadIdx.x & 31);
-    if (f >= x.n * G) return;
-    const int t0 = f / G;
-    float M = -INFINITY, L = 0.f;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    constexpr int kAtOnce = 8;  // parts whose loads are in flight together
-    for (int p = share; p <= end; p += kAtOnce) {
-        float2 ml[kAtOnce];
-        float4 v[kAtOnce];
-#pragma unroll
-        for (int i = 0; i < kAtOnce; ++i) {
-            const int q = min(p + i, end);
-            const float* b = (few ? few_parts : wide_parts) + part_at(few, q * a.HKV + kvh, q == share ? 1 : 0);
-            ml[i] = *reinterpret_cast<const float2*>(b + (few ? kFewRows : kUnitRows) * kHeadDim + 2 * row);
-            v[i] = *reinterpret_cast<const float4*>(b + row * kHeadDim + d);
-        }
-        float mn = M;
-#pragma unroll
-        for (int i = 0; i < kAtOnce; ++i)
-            if (p + i <= end) mn = fmaxf(mn, ml[i].x);
-        const float c = M == mn ? 1.f : __builtin_amdgcn_exp2f(M - mn);
-        M = mn;
-        L *= c, o.x *= c, o.y *= c, o.z *= c, o.w *= c;
-#pragma unroll
-        for (int i = 0; i < kAtOnce; ++i) {
-            if (p + i > end || (ml[i].x == -INFINITY && ml[i].y == 0.f)) continue;
-            const float wv = __builtin_amdgcn_exp2f(ml[i].x - M);
-            L = __builtin_fmaf(wv, ml[i].y, L);
-            o.x = __builtin_fmaf(wv, v[i].x, o.x), o.y = __builtin_fmaf(wv, v[i].y, o.y);
-            o.z = __builtin_fmaf(wv, v[i].z, o.z), o.w = __builtin_fmaf(wv, v[i].w, o.w);
-        }
-    }
-    const float inv = x.len - x.n + t0 < 0 ? 0.f : 1.f / L;  // a row that sees no key: zeros
-    *reinterpret_cast<float4*>(a.out + (((size_t)x.row0 + t0) * a.H + kvh * G + f - t0 * G) * kHeadDim + d) =
-        make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    const int first = few ? 0 : (int)blockIdx.y * kCombineSpan, row0 = first + (int)(threadIdx.x >> 5);
+    const int rows = x.n * G - kUnitRows * x.u - first;  // (of the unit, from this workgroup's first on)
+    if (row0 - first >= rows) return;
+    const float* parts = few ? few_parts : wide_parts;
+    if (rows <= kCombineRows) merge_rows<1, 8>(a, x, kvh, G, parts, few, share, end, row0);
+    else merge_rows<kCombineSpan / kCombineRows, 4>(a, x, kvh, G, parts, few, share, end, row0);
 }
 
 // ------------------------------------------------------------------ the step's prologue
@@ -1422,7 +1446,7 @@ hipError_t launch_packed(hipStream_t st, const PackedArgs& a, void* ws) {
     const hipError_t e = a.btab ? launch_packed_attn<true>(st, a, shares, wide, few)
                                 : launch_packed_attn<false>(st, a, shares, wide, few);
     if (e != hipSuccess) return e;
-    k_packed_combine<<<dim3(shares * a.HKV, kCombineWide + kCombineFew), 32 * kCombineRows, 0, st>>>(
+    k_packed_combine<<<dim3(shares * a.HKV, kCombineWide + 1), 32 * kCombineRows, 0, st>>>(
         a, a.btab == nullptr, shares, wide, few);
     return hipGetLastError();
 }
