@@ -89,7 +89,7 @@ def test_plan_covers_every_unit_once(gpu, H, HKV, lens, kv):
     assert dealt == rounds * N and dealt + line == len(wide)
     load = np.zeros(N, int)
     for is_few, units, shares, first, (once, turn) in ((False, wide, wide_shares, dealt, (5, 2)),
-                                                       (True, few, few_shares, 0, (8, 8))):
+                                                       (True, few, few_shares, 0, (5, 8))):
         cost = want[is_few]
         assert {(int(x[4]), int(x[3])): int(x[5]) for x in units} == cost and len(units) == len(cost)
         for x in units:
@@ -123,7 +123,7 @@ def test_plan_covers_every_unit_once(gpu, H, HKV, lens, kv):
             assert shares[j, 4] == (ends[begins[j]] if j in begins else 0)
             if j in begins:
                 assert np.array_equal(shares[j, 16:24], units[first + begins[j]])
-        fair = sum(sum(t + c for t in want[f].values()) for f, c in ((False, 5), (True, 8))[:1 + is_few]) / N
+        fair = sum(sum(t + c for t in want[f].values()) for f, c in ((False, 5), (True, 5))[:1 + is_few]) / N
         assert load.max() <= fair + 4 * once + 2 * turn + (max(tiles, default=0) if first else 0) + 24 * is_few
 
 
