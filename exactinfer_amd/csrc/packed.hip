@@ -948,10 +948,21 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
 // quarter of the lanes takes each of four keys.  K: step (x, e) takes d = 16x + 4 quarter + e, so that a
 // lane's row comes in 16-byte pieces; V: a lane's pieces hold d = 64y + 4 (l % 16) + e, sum 4y + e takes
 // element e.  Pieces of the next tile are fetched as this one's are used up.
-template <bool kPaged, int kBlocks>
+//
+// kQuad: four more rows, row l % 4 of them, on v_mfma_f32_4x4x1_16b_f32 from the same K and V registers, at a
+// quarter of the time: its block l / 4 holds keys 4 (l/4 % 4) .. + 3 of the half for the scores, the same of d for
+// O, and the quarters' products (of d, of keys) are summed afterwards.
+//
+// Single tokens are bound by reading K and V: 24 sequences of 57000 keys in all (H 16 / HKV 8, pages of 64),
+// 494 MB in 90 us, 5.5 TB/s.  Where sequences share their keys and have more rows it is the matrix instructions
+// (busy a third of the time) and what a pass does once: 16 drafts of 5 tokens after 1024 shared keys and up to
+// 555 more (H 32 / HKV 8) 42 us.  By rows (H 32 / HKV 8, 32 sequences of 480 keys, with the merge): up to
+// sixteen 27 us (with kBlocks 2 37), up to twenty 33 (35), 32 rows 35 (44 as a wide unit; 4067 keys 193 against
+// 297; single tokens as wide units 44 and 290 against 27 and 181).
+template <bool kPaged, int kBlocks, bool kQuad>
 __device__ __forceinline__ void few_pass(const PackedArgs& a, const Pass& p, int kvh, FastDiv fG, float sl2,
                                          float* smem) {
-    constexpr int D = kHeadDim, kRows = kFewBlock * kBlocks;
+    constexpr int D = kHeadDim, kSets = kBlocks + kQuad, kRows = kFewBlock * kBlocks + 4 * kQuad;
     const int tid = unhoisted(threadIdx.x), lane = tid & 63, wu = scalar(tid >> 6);
     const int j = lane & 15, quarter = lane >> 4;
     const int G = (int)fG.d;
@@ -989,15 +1000,17 @@ __device__ __forceinline__ void few_pass(const PackedArgs& a, const Pass& p, int
     int pg = page(0);  // of the tile that is loaded next
     // q first (a wait for it is not one for the tiles), by the first rows' lanes; more than sixteen rows' goes
     // through LDS (registers), [row][d]
-    int qpos[kBlocks];  // (rows past the last repeat it)
+    auto quad = [](int rb) { return rb == kBlocks; };  // the set of four
+    auto row_of = [&](int rb) { return kFewBlock * rb + (quad(rb) ? j & 3 : j); };
+    int qpos[kSets];  // (rows past the last repeat it)
 #pragma unroll
-    for (int rb = 0; rb < kBlocks; ++rb) qpos[rb] = p.pos0 + fdiv(min(f0 + kFewBlock * rb + j, last), fG);
+    for (int rb = 0; rb < kSets; ++rb) qpos[rb] = p.pos0 + fdiv(min(f0 + row_of(rb), last), fG);
     auto q_row = [&](int f) {
         const int tok = fdiv(f, fG);
         return a.q + ((size_t)p.row0 + tok) * a.q_stride + (size_t)(kvh * G + f - tok * G) * D;
     };
-    float4 q_raw[kBlocks == 1 ? 8 : 2];
-    if constexpr (kBlocks == 1) {
+    float4 q_raw[kSets == 1 ? 8 : 2];
+    if constexpr (kSets == 1) {
         const float* src = q_row(min(f0 + j, last)) + 4 * quarter;
 #pragma unroll
         for (int x = 0; x < 8; ++x) q_raw[x] = *reinterpret_cast<const float4*>(src + 16 * x);
@@ -1016,8 +1029,8 @@ __device__ __forceinline__ void few_pass(const PackedArgs& a, const Pass& p, int
         pg = page(1);
     }
     auto scaled = [&](const float4& v) { return f32x4{v.x * sl2, v.y * sl2, v.z * sl2, v.w * sl2}; };
-    f32x4 q[kBlocks == 1 ? 8 : 1];
-    if constexpr (kBlocks == 1) {
+    f32x4 q[kSets == 1 ? 8 : 1];
+    if constexpr (kSets == 1) {
 #pragma unroll
         for (int x = 0; x < 8; ++x) q[x] = scaled(q_raw[x]);
     } else {
@@ -1027,44 +1040,58 @@ __device__ __forceinline__ void few_pass(const PackedArgs& a, const Pass& p, int
         lds_barrier();
     }
     auto q_at = [&](int rb, int x) -> f32x4 {
-        if constexpr (kBlocks == 1) return q[x];
-        else return *reinterpret_cast<const f32x4*>(smem + (kFewBlock * rb + j) * kRowF + 16 * x + 4 * quarter);
+        if constexpr (kSets == 1) return q[x];
+        else return *reinterpret_cast<const f32x4*>(smem + row_of(rb) * kRowF + 16 * x + 4 * quarter);
     };
-    f32x4 o[kBlocks][8];
-    float m[kBlocks], l[kBlocks];
+    f32x4 o[kSets][8];
+    float m[kSets], l[kSets];
 #pragma unroll
-    for (int rb = 0; rb < kBlocks; ++rb) {
+    for (int rb = 0; rb < kSets; ++rb) {
 #pragma unroll
         for (int y = 0; y < 8; ++y) o[rb][y] = f32x4{0.f, 0.f, 0.f, 0.f};
         m[rb] = -INFINITY;
         l[rb] = 0.f;
     }
+    auto mma = [&](int rb, uint32_t x, float y, f32x4 c) {
+        return quad(rb) ? __builtin_amdgcn_mfma_f32_4x4x1f32(__uint_as_float(x), y, c, 0, 0, 0)
+                        : __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(x), y, c, 0, 0, 0);
+    };
     for (int i = 0; i < n_mine; ++i) {
         const bool more = i + 1 < n_mine;
         const int kt = index(i);
         const Rsrc rk = k_tile(more ? i + 1 : i, pg, more), rv = v_tile(more ? i + 1 : i, pg, more);
-        f32x4 s[kBlocks][2];
+        f32x4 s[kSets][2];
 #pragma unroll
-        for (int rb = 0; rb < kBlocks; ++rb) s[rb][0] = s[rb][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int rb = 0; rb < kSets; ++rb) s[rb][0] = s[rb][1] = f32x4{0.f, 0.f, 0.f, 0.f};
         const uint32_t off_k = k_offset();
 #pragma unroll
         for (int x = 0; x < 8; ++x) {
-            f32x4 qx[kBlocks];
+            f32x4 qx[kSets];
 #pragma unroll
-            for (int rb = 0; rb < kBlocks; ++rb) qx[rb] = q_at(rb, x);
+            for (int rb = 0; rb < kSets; ++rb) qx[rb] = q_at(rb, x);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
 #pragma unroll
-                for (int rb = 0; rb < kBlocks; ++rb)
+                for (int rb = 0; rb < kSets; ++rb)
 #pragma unroll
                     for (int kb = 0; kb < 2; ++kb)
-                        s[rb][kb] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(kr[kb][x][e]), qx[rb][e],
-                                                                         s[rb][kb], 0, 0, 0);
+                        s[rb][kb] = mma(rb, kr[kb][x][e], qx[rb][e], s[rb][kb]);
             __builtin_amdgcn_sched_barrier(0);
             load_k(rk, x, off_k);
         }
 #pragma unroll
-        for (int rb = 0; rb < kBlocks; ++rb) {
+        for (int rb = 0; rb < kSets; ++rb) {
+            if (quad(rb)) {  // the quarters' sums, then each quarter its four keys of every sixteen
+                const int from = 4 * (20 * quarter + (lane & 3));
+#pragma unroll
+                for (int r = 0; r < 8; ++r) {
+                    float v = s[rb][r >> 2][r & 3];
+                    v += lane_xor16(v);
+                    v += lane_xor32(v);
+                    s[rb][r >> 2][r & 3] =
+                        __uint_as_float(__builtin_amdgcn_ds_bpermute(from, __float_as_uint(v)));
+                }
+            }
             if (kt >= nfull) {
                 const int k0 = unhoisted(kt * kKT + 4 * quarter);
 #pragma unroll
@@ -1097,11 +1124,10 @@ __device__ __forceinline__ void few_pass(const PackedArgs& a, const Pass& p, int
 #pragma unroll
         for (int t = 0; t < 8; ++t) {
 #pragma unroll
-            for (int rb = 0; rb < kBlocks; ++rb)
+            for (int rb = 0; rb < kSets; ++rb)
 #pragma unroll
                 for (int y = 0; y < 8; ++y)
-                    o[rb][y] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(vr[t][y >> 2][y & 3]),
-                                                                    s[rb][t >> 2][t & 3], o[rb][y], 0, 0, 0);
+                    o[rb][y] = mma(rb, vr[t][y >> 2][y & 3], s[rb][t >> 2][t & 3], o[rb][y]);
             __builtin_amdgcn_sched_barrier(0);
             load_v(rv, t, off_v);
         }
@@ -1112,7 +1138,7 @@ __device__ __forceinline__ void few_pass(const PackedArgs& a, const Pass& p, int
     {
         float z = 0.f;
 #pragma unroll
-        for (int rb = 0; rb < kBlocks; ++rb) {
+        for (int rb = 0; rb < kSets; ++rb) {
             z = __builtin_fmaf(l[rb], 0.f, z);
 #pragma unroll
             for (int y = 0; y < 8; ++y)
@@ -1121,7 +1147,7 @@ __device__ __forceinline__ void few_pass(const PackedArgs& a, const Pass& p, int
         }
         if (__builtin_amdgcn_ballot_w64(z != 0.f)) {
 #pragma unroll
-            for (int rb = 0; rb < kBlocks; ++rb) {
+            for (int rb = 0; rb < kSets; ++rb) {
 #pragma unroll
                 for (int y = 0; y < 8; ++y) o[rb][y] = f32x4{0.f, 0.f, 0.f, 0.f};
                 m[rb] = -INFINITY;
@@ -1148,10 +1174,12 @@ __device__ __forceinline__ void few_pass(const PackedArgs& a, const Pass& p, int
                     const float w = __builtin_amdgcn_exp2f(dot - (mn == -INFINITY ? 0.f : mn));
                     m[rb] = mn;
                     l[rb] = quarter == 0 ? l[rb] * corr + w : 0.f;  // (summed over the quarters below)
+                    if (quad(rb) && quarter > 0) continue;          // (the sums too)
+                    const int part = quad(rb) ? j >> 2 : quarter;
 #pragma unroll
-                    for (int x = 0; x < 8; ++x) {  // d = 64 (x/4) + 16 quarter + 4 (x%4) + e
+                    for (int x = 0; x < 8; ++x) {  // d = 64 (x/4) + 16 part + 4 (x%4) + e
                         const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(
-                            rv, row + 64 * quarter + 256 * (x >> 2) + 16 * (x & 3), 0, 0);
+                            rv, row + 64 * part + 256 * (x >> 2) + 16 * (x & 3), 0, 0);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
                             f32x4& sum = o[rb][4 * (x >> 2) + e];
@@ -1163,20 +1191,31 @@ __device__ __forceinline__ void few_pass(const PackedArgs& a, const Pass& p, int
         }
     }
     // every wave's rows meet: register r of sum 4y + e is d = 64y + 16 quarter + 4r + e
-    if constexpr (kBlocks > 1) lds_barrier();  // q has been read
+    if constexpr (kSets > 1) lds_barrier();  // q has been read
     float* const mine = smem + wu * (kRows * kRowF);
     float* const ml_at = smem + kFewML;
 #pragma unroll
-    for (int rb = 0; rb < kBlocks; ++rb) {
+    for (int rb = 0; rb < kSets; ++rb) {
+        if (quad(rb)) {
 #pragma unroll
-        for (int x = 0; x < 8; ++x)
-            *reinterpret_cast<float4*>(mine + (kFewBlock * rb + j) * kRowF + 64 * (x >> 2) + 16 * quarter +
-                                       4 * (x & 3)) =
-                make_float4(o[rb][4 * (x >> 2)][x & 3], o[rb][4 * (x >> 2) + 1][x & 3], o[rb][4 * (x >> 2) + 2][x & 3],
-                            o[rb][4 * (x >> 2) + 3][x & 3]);
+            for (int y = 0; y < 8; ++y)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    o[rb][y][r] += lane_xor16(o[rb][y][r]);
+                    o[rb][y][r] += lane_xor32(o[rb][y][r]);
+                }
+        }
         const float sum = half_sum(l[rb] + lane_xor16(l[rb]));
-        if (quarter == 0)
-            *reinterpret_cast<float2*>(ml_at + 2 * (wu * kRows + kFewBlock * rb + j)) = make_float2(m[rb], sum);
+        const int row = row_of(rb), part = quad(rb) ? j >> 2 : quarter;
+        if (!quad(rb) || quarter == 0) {
+#pragma unroll
+            for (int x = 0; x < 8; ++x)
+                *reinterpret_cast<float4*>(mine + row * kRowF + 64 * (x >> 2) + 16 * part + 4 * (x & 3)) =
+                    make_float4(o[rb][4 * (x >> 2)][x & 3], o[rb][4 * (x >> 2) + 1][x & 3],
+                                o[rb][4 * (x >> 2) + 2][x & 3], o[rb][4 * (x >> 2) + 3][x & 3]);
+        }
+        if (quarter == 0 && (!quad(rb) || j < 4))
+            *reinterpret_cast<float2*>(ml_at + 2 * (wu * kRows + row)) = make_float2(m[rb], sum);
     }
     lds_barrier();
     // two rows per wave and round, a lane four columns
@@ -1247,8 +1286,10 @@ __device__ __forceinline__ void walk_list(const PackedArgs& a, const List& list,
         p.part = p.kt_lo > 0 || cut >= 0 ? parts + part_at(kFew, share * a.HKV + kvh, p.kt_lo > 0 ? 0 : 1) : nullptr;
         if (pass > 0) lds_barrier();  // the last pass's rows have been read
         if constexpr (kFew) {
-            if (p.nflat - kUnitRows * p.u <= kFewBlock) few_pass<kPaged, 1>(a, p, kvh, fG, sl2, smem);
-            else few_pass<kPaged, kFewRows / kFewBlock>(a, p, kvh, fG, sl2, smem);
+            const int rows = p.nflat - kUnitRows * p.u;
+            if (rows <= kFewBlock) few_pass<kPaged, 1, false>(a, p, kvh, fG, sl2, smem);
+            else if (rows <= kFewBlock + 4) few_pass<kPaged, 1, true>(a, p, kvh, fG, sl2, smem);
+            else few_pass<kPaged, kFewRows / kFewBlock, false>(a, p, kvh, fG, sl2, smem);
         } else wide_pass<kPaged>(a, p, kvh, fG, sl2, smem);
     }
 }

@@ -464,6 +464,42 @@ def test_paged_chunks(gpu, H, HKV, bs, lens, kv):
         assert rel_err(got, ref) <= ATTN_RTOL, s
 
 
+@pytest.mark.parametrize("H,HKV,lens", [(8, 2, [4, 5, 6, 8, 1]), (5, 1, [3, 4, 5, 6]), (8, 1, [2, 3, 4]),
+                                        (4, 2, [8, 9, 10, 11])])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_bad_values_beside_few_rows(gpu, H, HKV, lens, bad):
+    """16 to 32 rows of a KV head, with a bad key row or value that only the last two rows of each sequence
+    see: the others keep their outputs, and a value's column alone is bad."""
+    kv = [300 + 13 * i for i in range(len(lens))]
+    kc, vc, table, rows_of = _pool(lens, kv, HKV, 32, 23)
+    rows, cu = sum(lens), _cu(lens)
+    q = torch.randn((rows, H * D), generator=torch.Generator(device="cuda").manual_seed(24), device="cuda")
+    shape = gpu.AttnShape(H, HKV)
+    b = gpu.PackedBatch(len(lens), rows, H, HKV)
+    b.plan(_i32(cu), rows, max(kv), kv_len=_i32(kv))
+    clean = gpu.attn_packed_paged(q, kc, vc, table, 32, b, shape)
+    for s, n in enumerate(lens):
+        r = slice(int(cu[s]), int(cu[s + 1]))
+        ref = _attend64(q[r].double().view(n, H, D), kc[rows_of[s]].double(), vc[rows_of[s]].double(), kv[s])
+        assert rel_err(clean[r].cpu().numpy(), ref.cpu().numpy()) <= ATTN_RTOL, s
+    at = torch.stack([rows_of[s][kv[s] - 2] for s in range(len(lens))])
+    sees = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    for s, n in enumerate(lens):
+        sees[max(int(cu[s]), int(cu[s + 1]) - 2):int(cu[s + 1])] = True
+    k2, v2 = kc.clone(), vc.clone()
+    k2[at] = float("nan")
+    out = gpu.attn_packed_paged(q, k2, vc, table, 32, b, shape)
+    assert torch.isnan(out[sees]).all()
+    if not sees.all():
+        assert rel_err(out[~sees].cpu().numpy(), clean[~sees].cpu().numpy()) <= ATTN_RTOL
+    v2[at, 0, 37] = bad
+    out = gpu.attn_packed_paged(q, kc, v2, table, 32, b, shape)
+    hit = torch.zeros_like(clean, dtype=torch.bool)
+    hit[:, :H // HKV, 37] = sees[:, None]
+    assert torch.equal(~torch.isfinite(out), hit)
+    assert rel_err(torch.where(hit, clean, out).cpu().numpy(), clean.cpu().numpy()) <= ATTN_RTOL
+
+
 def test_missing_pages_count_as_zeros(gpu):
     """Entries outside the pool and keys past the table: zeros, and nothing is read there."""
     H, HKV, bs = 16, 8, 32
