@@ -949,16 +949,16 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
 // lane's row comes in 16-byte pieces; V: a lane's pieces hold d = 64y + 4 (l % 16) + e, sum 4y + e takes
 // element e.  Pieces of the next tile are fetched as this one's are used up.
 //
-// kQuad: four more rows, row l % 4 of them, on v_mfma_f32_4x4x1_16b_f32 from the same K and V registers, at a
-// quarter of the time: its block l / 4 holds keys 4 (l/4 % 4) .. + 3 of the half for the scores, the same of d for
-// O, and the quarters' products (of d, of keys) are summed afterwards.
+// kQuad: four more rows (or the only ones), row l % 4 of them, on v_mfma_f32_4x4x1_16b_f32 from the same K and V
+// registers, at a quarter of the time: its block l / 4 holds keys 4 (l/4 % 4) .. + 3 of the half for the scores,
+// the same of d for O, and the quarters' products (of d, of keys) are summed afterwards.
 //
 // Single tokens are bound by reading K and V: 24 sequences of 57000 keys in all (H 16 / HKV 8, pages of 64),
-// 494 MB in 90 us, 5.5 TB/s.  Where sequences share their keys and have more rows it is the matrix instructions
-// (busy a third of the time) and what a pass does once: 16 drafts of 5 tokens after 1024 shared keys and up to
-// 555 more (H 32 / HKV 8) 42 us.  By rows (H 32 / HKV 8, 32 sequences of 480 keys, with the merge): up to
-// sixteen 27 us (with kBlocks 2 37), up to twenty 33 (35), 32 rows 35 (44 as a wide unit; 4067 keys 193 against
-// 297; single tokens as wide units 44 and 290 against 27 and 181).
+// 494 MB in 88 us, 5.6 TB/s.  Where sequences share their keys and have more rows it is the matrix instructions
+// and what a pass does once: 16 drafts of 5 tokens after 1024 shared keys and up to 555 more (H 32 / HKV 8) 41 us.
+// By rows (H 32 / HKV 8, 32 sequences of 480 keys, with the merge): four 26.2 us (27.1 as sixteen), sixteen 27
+// (37 as 32), twenty 32.3 (35.5 as 32), 32 rows 36 (44 as a wide unit; of 4067 keys 192 against 297; single
+// tokens as wide units 44, and of 4059 keys 290 against 179).
 template <bool kPaged, int kBlocks, bool kQuad>
 __device__ __forceinline__ void few_pass(const PackedArgs& a, const Pass& p, int kvh, FastDiv fG, float sl2,
                                          float* smem) {
@@ -1011,7 +1011,7 @@ __device__ __forceinline__ void few_pass(const PackedArgs& a, const Pass& p, int
     };
     float4 q_raw[kSets == 1 ? 8 : 2];
     if constexpr (kSets == 1) {
-        const float* src = q_row(min(f0 + j, last)) + 4 * quarter;
+        const float* src = q_row(min(f0 + row_of(0), last)) + 4 * quarter;
 #pragma unroll
         for (int x = 0; x < 8; ++x) q_raw[x] = *reinterpret_cast<const float4*>(src + 16 * x);
     } else {
@@ -1196,21 +1196,30 @@ __device__ __forceinline__ void few_pass(const PackedArgs& a, const Pass& p, int
     float* const ml_at = smem + kFewML;
 #pragma unroll
     for (int rb = 0; rb < kSets; ++rb) {
-        if (quad(rb)) {
-#pragma unroll
-            for (int y = 0; y < 8; ++y)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    o[rb][y][r] += lane_xor16(o[rb][y][r]);
-                    o[rb][y][r] += lane_xor32(o[rb][y][r]);
-                }
-        }
         const float sum = half_sum(l[rb] + lane_xor16(l[rb]));
-        const int row = row_of(rb), part = quad(rb) ? j >> 2 : quarter;
-        if (!quad(rb) || quarter == 0) {
+        const int row = row_of(rb);
+        if (quad(rb)) {
+            // register r of sum 4y + e is d = 64y + 16 (j / 4) + 4r + e there, over a quarter's keys: quarter r of
+            // the lanes sums and writes it, handing on the others
+            float sums[8];
+#pragma unroll
+            for (int y = 0; y < 8; ++y) {
+                float half[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float lo = o[rb][y][2 * i], hi = o[rb][y][2 * i + 1];
+                    half[i] = (quarter & 1 ? hi : lo) + lane_xor16(quarter & 1 ? lo : hi);
+                }
+                sums[y] = (quarter & 2 ? half[1] : half[0]) + lane_xor32(quarter & 2 ? half[0] : half[1]);
+            }
+#pragma unroll
+            for (int y = 0; y < 2; ++y)
+                *reinterpret_cast<float4*>(mine + row * kRowF + 64 * y + 16 * (j >> 2) + 4 * quarter) =
+                    make_float4(sums[4 * y], sums[4 * y + 1], sums[4 * y + 2], sums[4 * y + 3]);
+        } else {
 #pragma unroll
             for (int x = 0; x < 8; ++x)
-                *reinterpret_cast<float4*>(mine + row * kRowF + 64 * (x >> 2) + 16 * part + 4 * (x & 3)) =
+                *reinterpret_cast<float4*>(mine + row * kRowF + 64 * (x >> 2) + 16 * quarter + 4 * (x & 3)) =
                     make_float4(o[rb][4 * (x >> 2)][x & 3], o[rb][4 * (x >> 2) + 1][x & 3],
                                 o[rb][4 * (x >> 2) + 2][x & 3], o[rb][4 * (x >> 2) + 3][x & 3]);
         }
@@ -1287,7 +1296,9 @@ __device__ __forceinline__ void walk_list(const PackedArgs& a, const List& list,
         if (pass > 0) lds_barrier();  // the last pass's rows have been read
         if constexpr (kFew) {
             const int rows = p.nflat - kUnitRows * p.u;
-            if (rows <= kFewBlock) few_pass<kPaged, 1, false>(a, p, kvh, fG, sl2, smem);
+            // (up to so many rows: the fewest matrix instructions that hold them)
+            if (rows <= 4) few_pass<kPaged, 0, true>(a, p, kvh, fG, sl2, smem);
+            else if (rows <= kFewBlock) few_pass<kPaged, 1, false>(a, p, kvh, fG, sl2, smem);
             else if (rows <= kFewBlock + 4) few_pass<kPaged, 1, true>(a, p, kvh, fG, sl2, smem);
             else few_pass<kPaged, kFewRows / kFewBlock, false>(a, p, kvh, fG, sl2, smem);
         } else wide_pass<kPaged>(a, p, kvh, fG, sl2, smem);

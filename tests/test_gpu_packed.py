@@ -465,10 +465,11 @@ def test_paged_chunks(gpu, H, HKV, bs, lens, kv):
 
 
 @pytest.mark.parametrize("H,HKV,lens", [(8, 2, [4, 5, 6, 8, 1]), (5, 1, [3, 4, 5, 6]), (8, 1, [2, 3, 4]),
-                                        (4, 2, [8, 9, 10, 11])])
+                                        (4, 2, [8, 9, 10, 11]), (8, 2, [1, 1, 1]), (2, 1, [2, 1, 2]),
+                                        (1, 1, [4, 5, 3])])
 @pytest.mark.parametrize("bad", [float("nan"), float("inf")])
 def test_bad_values_beside_few_rows(gpu, H, HKV, lens, bad):
-    """16 to 32 rows of a KV head, with a bad key row or value that only the last two rows of each sequence
+    """1 to 32 rows of a KV head, with a bad key row or value that only the last two rows of each sequence
     see: the others keep their outputs, and a value's column alone is bad."""
     kv = [300 + 13 * i for i in range(len(lens))]
     kc, vc, table, rows_of = _pool(lens, kv, HKV, 32, 23)
