@@ -32,6 +32,10 @@ constexpr int kFewRows = 32;    // a sequence's last unit of up to so many rows:
 //
 // Order and cuts follow from the lengths alone (no atomics decide them), so a batch planned twice
 // gives the same bits twice.
+//
+// One workgroup, a thread per sequence, unit or cut, everything in LDS as long as it fits: its time is the
+// latency of a dozen steps that need each other, 7 us for 5 sequences, 10 for 6 of up to 8192 rows (490 wide
+// units), 5.5 and 8 in a graph; once per forward pass, not per layer.
 struct Unit {
     int row0, n, len, u;    // the sequence's first row, rows and keys; the unit's number in it
     int seq, tiles, pad[2];
@@ -359,6 +363,11 @@ __device__ __forceinline__ int row_owner(const int4* seq, int n_seq, int b, int 
 //   P: 2^14, so that weights of up to 2^kLazy fit (of one below 2^-39 nothing is left, at most that times
 //     the number of keys in all); the weights' sum has it too
 // What the scaling of V cannot hold is noticed at the end of a pass (planes_failed) and multiplied in fp32.
+//
+// What bounds it is the power of the matrix instructions: 8192, 4096, 2048, 1024, 300 and 17 rows (H 32 / HKV 8)
+// take 2235 us, 327 TFLOP/s, with the matrix unit busy 46% of the time at 1.9 GHz.  With two products of three
+// taken out 1530 us, with the loop's loads out 11% less, with the LDS reads out 3%; more fragments in flight,
+// other interleavings of the splits and no priorities all came within 3%.  Three bf16 planes: 3370 us.
 //
 // A wave holds 32 flat query rows and computes S^T[key][row] = K . Q^T, so that each lane owns one row and
 // 16 of a tile's 32 keys, and O^T[d][row] = V^T . P^T from the same registers.
@@ -1401,6 +1410,8 @@ __global__ __launch_bounds__(32 * kCombineRows) void k_packed_combine(PackedArgs
 }
 
 // ------------------------------------------------------------------ the step's prologue
+// Bound by memory, after the latency of two lookups (the row's owner, its page): 824 rows of H 16 / HKV 8 9.2 us
+// (27 MB), 1424 of H 32 / HKV 8 18.6 us (70 MB, 3.8 TB/s).
 // grid (rows, ceil((H + HKV) / 16)), block 256: each wave four consecutive heads of the row, loads of
 // all of them first.  Query heads go, normed and turned, to q_out; key heads with the V rows of the same
 // KV heads to the pool.

