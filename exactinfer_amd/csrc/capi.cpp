@@ -670,7 +670,6 @@ int check_pool(const float* kc, const float* vc, int n_blocks, const int* block_
             "max_blocks %d x block_size %d must lie in [1, 2^31 - 1] keys", max_blocks, block_size);
     REQUIRE(n_blocks > 0, "n_blocks %d must be positive", n_blocks);
     const size_t pool = (size_t)n_blocks * block_size * n_head_kv * 128 * sizeof(float);
-    REQUIRE(!overlap(kc, pool, vc, pool), "the K and V pools overlap");
     for (const float* c : {kc, vc})
         REQUIRE(!overlap(c, pool, out, out_bytes) && !overlap(c, pool, ws, ws_bytes),
                 "out or workspace lies in a pool of %zu bytes", pool);
@@ -848,6 +847,7 @@ EI_API int ei_packed_step_paged(ei_stream_t stream, const float* qkv, long row_s
             "out or workspace overlaps qkv");
     const size_t pool = (size_t)n_blocks * block_size * n_head_kv * head_dim * sizeof(float);
     REQUIRE(!overlap(kc, pool, qkv, in) && !overlap(vc, pool, qkv, in), "qkv lies in a pool");
+    REQUIRE(!overlap(kc, pool, vc, pool), "the K and V pools overlap");  // (both are written)
     if (rows == 0) return ok();
     ei::PackedArgs a{};
     a.k = kc, a.v = vc, a.kv_stride = (long)n_head_kv * head_dim;

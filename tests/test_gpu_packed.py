@@ -750,3 +750,99 @@ def test_single_rows_of_any_stride(gpu):
     cs = gpu.rope_table_scaled(16, D, 1e6)
     pos = _i32([9])
     assert torch.equal(gpu.rope_rows(q1, H, cs, pos), gpu.rope_rows(q, H, cs, pos))
+
+
+@pytest.mark.parametrize("H,HKV", [(7, 1), (18, 3), (30, 5), (14, 7), (300, 300), (264, 33), (6, 6)])
+def test_any_number_of_heads(gpu, H, HKV):
+    """KV heads that do not divide the GPU's units, more of them than it has, and every group's size."""
+    lens = [3, 45, 1, 20] if H < 100 else [3, 33, 1]
+    _, q, k, v = _prompts(H, HKV, lens, 111)
+    _check_prompts(_run_prompts(gpu, q, k, v, lens, H, HKV), q, k, v, lens, H, HKV)
+    kv = [n + 90 for n in lens]
+    kc, vc, table, rows_of = _pool(lens, kv, HKV, 32, 112)
+    b = gpu.PackedBatch(len(lens), sum(lens), H, HKV)
+    b.plan(_i32(_cu(lens)), sum(lens), max(kv), kv_len=_i32(kv))
+    out = gpu.attn_packed_paged(q, kc, vc, table, 32, b, gpu.AttnShape(H, HKV))
+    for s, (a, n) in enumerate(zip(_cu(lens), lens)):
+        r = slice(int(a), int(a) + n)
+        ref = _attend64(q[r].double().view(n, H, D), kc[rows_of[s]].double(), vc[rows_of[s]].double(), kv[s])
+        assert rel_err(out[r].cpu().numpy(), ref.cpu().numpy()) <= ATTN_RTOL, s
+
+
+def test_batches_without_rows_or_keys(gpu):
+    """Rows that belong to nobody stay; rows of sequences without keys are zeros, lengths below 0 count as 0 and
+    lengths above max_kv as max_kv."""
+    H, HKV = 16, 8
+    shape = gpu.AttnShape(H, HKV)
+    _, q, k, v = _prompts(H, HKV, [6], 113)
+    b = gpu.PackedBatch(3, 6, H, HKV)
+    mark = torch.full((6, H, D), 7.5, device="cuda")
+    b.plan(_i32([0, 0, 0, 0]), 6, 10)
+    out = gpu.attn_packed(q, k, v, b, shape, out=mark.clone())
+    assert torch.equal(out, mark)
+    b.plan(_i32([0, 2, 2, 5]), 6, 0)
+    out = gpu.attn_packed(q, k, v, b, shape, out=mark.clone())
+    assert (out[:5] == 0).all() and torch.equal(out[5:], mark[5:])
+    kc, vc, table, rows_of = _pool([2, 1, 3], [40, 1, 50], HKV, 32, 114)
+    b.plan(_i32([0, 2, 3, 6]), 6, 50, kv_len=_i32([40, -5, 2 ** 31 - 1]))
+    out = gpu.attn_packed_paged(q, kc, vc, table, 32, b, shape)
+    assert (out[2] == 0).all()
+    b.plan(_i32([0, 2, 3, 6]), 6, 50, kv_len=_i32([40, 0, 50]))
+    assert torch.equal(out, gpu.attn_packed_paged(q, kc, vc, table, 32, b, shape))
+    qg = torch.ones(D, device="cuda")
+    qkv = torch.randn((6, shape.qkv), device="cuda")
+    cs = gpu.rope_table_scaled(64)
+    b.plan(_i32([0, 0, 0, 0]), 6, 50, kv_len=_i32([40, 1, 50]))
+    k0, v0 = kc.clone(), vc.clone()
+    out = gpu.packed_step_paged(qkv, kc, vc, table, 32, b, shape, qg, qg, cs, out=mark.clone())
+    assert torch.equal(out, mark) and torch.equal(kc, k0) and torch.equal(vc, v0)
+
+
+def test_blocks_past_32_bits(gpu):
+    """Pool rows beyond 2^31 values and 2^32 bytes, appended and read."""
+    H, HKV, bs = 16, 8, 256
+    n_blocks = 2 ** 31 // (HKV * D * bs) + 6
+    kc = torch.empty((n_blocks * bs, HKV, D), device="cuda")
+    vc = torch.empty_like(kc)
+    lens, kv = [1, 40], [300, 200]
+    table = _i32([[n_blocks - 1, n_blocks - 4], [n_blocks // 2 + 3, 0]])
+    rows_of = [torch.cat([torch.arange(bs) + int(e) * bs for e in row])[:kv[s]].cuda()
+               for s, row in enumerate(table.tolist())]
+    g = torch.Generator(device="cuda").manual_seed(115)
+    for r in rows_of:
+        kc[r] = torch.randn((len(r), HKV, D), generator=g, device="cuda")
+        vc[r] = torch.randn((len(r), HKV, D), generator=g, device="cuda")
+    shape = gpu.AttnShape(H, HKV)
+    qkv = torch.randn((41, shape.qkv), generator=g, device="cuda")
+    one = torch.ones(D, device="cuda")
+    b = gpu.PackedBatch(2, 41, H, HKV)
+    b.plan(_i32(_cu(lens)), 41, 300, kv_len=_i32(kv))
+    out = gpu.packed_step_paged(qkv, kc, vc, table, bs, b, shape, one, one, gpu.rope_table_scaled(512))
+    x = qkv.double().view(41, H + 2 * HKV, D)
+    for s, (a, n) in enumerate(zip(_cu(lens), lens)):
+        r = slice(int(a), int(a) + n)
+        new = rows_of[s][kv[s] - n:]
+        assert torch.equal(vc[new], qkv[r].view(n, -1, D)[:, H + HKV:])
+        pos = torch.arange(kv[s] - n, kv[s], device="cuda")
+        q64 = _norm_rope64(x[r, :H], one, pos, D)
+        ref = _attend64(q64, kc[rows_of[s]].double(), vc[rows_of[s]].double(), kv[s])
+        assert rel_err(out[r].cpu().numpy(), ref.cpu().numpy()) <= ATTN_RTOL, s
+
+
+def test_keys_and_values_in_one_pool(gpu):
+    """A pool may serve as keys and values where it is only read, and sequences may list the same block twice."""
+    H, HKV, bs = 16, 8, 32
+    lens, kv = [5, 1], [90, 70]
+    kc, _, table, _ = _pool(lens, kv, HKV, bs, 116)
+    table[0, 1] = table[0, 0]
+    table[1] = table[0]
+    b = gpu.PackedBatch(2, 6, H, HKV)
+    b.plan(_i32(_cu(lens)), 6, 90, kv_len=_i32(kv))
+    q = torch.randn((6, H * D), generator=torch.Generator(device="cuda").manual_seed(117), device="cuda")
+    out = gpu.attn_packed_paged(q, kc, kc, table, bs, b, gpu.AttnShape(H, HKV))
+    for s, (a, n) in enumerate(zip(_cu(lens), lens)):
+        t = np.arange(kv[s])
+        rows = torch.from_numpy(table[s].cpu().numpy().astype(np.int64)[t // bs] * bs + t % bs).cuda()
+        x = kc[rows].double()
+        ref = _attend64(q[int(a):int(a) + n].double().view(n, H, D), x, x, kv[s])
+        assert rel_err(out[int(a):int(a) + n].cpu().numpy(), ref.cpu().numpy()) <= ATTN_RTOL, s

@@ -192,7 +192,6 @@ POOL = [
     ("null", dict(vc=None)),
     ("null", dict(table=None)),
     ("aligned", dict(kc=_off(FAR[4], 1))),
-    ("pools overlap", dict(vc=_off(FAR[4], 1024))),
     ("lies in a pool", dict(kc=_off(FAR[1], 4096))),
     ("lies in a pool", dict(vc=_off(FAR[3], 4096))),
 ]
@@ -240,6 +239,7 @@ def test_paged_arguments(match, kw):
     ("overlaps qkv", dict(out=FAR[0])),
     ("overlaps qkv", dict(ws=_off(FAR[0], 6144))),
     ("qkv lies in a pool", dict(vc=_off(FAR[0], 4096))),
+    ("pools overlap", dict(vc=_off(FAR[4], 1024))),
 ])
 def test_step_arguments(match, kw):
     _refused(match, "ei_packed_step_paged", *_step(**kw))
