@@ -1331,82 +1331,94 @@ __global__ __launch_bounds__(64 * kWaves) void k_packed_attn(PackedArgs a, int s
     walk_list<kPaged, true>(a, pv.few, few, 0, shares, share, kvh, few_parts, smem);
 }
 
-// The units that the cuts divide: workgroup (share, KV head; 32 rows) merges the unit that starts in
-// this share and goes on in the next ones.  Part p of it is the share's own (its slot 1), then slot 0 of
-// each share that it reaches.  o = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p over the parts that saw a
-// key (m = -inf and l = 0 otherwise; m = -inf with a NaN l counts).  A thread has four columns of one row, or
-// of four rows at a time (eight rows apart) where the unit has more than eight; the loads of 16 or 8 parts' rows
-// are in flight together, for what this takes is their latency.  Workgroups that find nothing to merge cost
-// too: with 8 rows each, four times as many, 32 single tokens at 475 keys take 28.5 us in all instead of 26.5.
-constexpr int kCombineRows = 8, kCombineSpan = 32;
-constexpr int kCombineWide = kUnitRows / kCombineSpan;
-static_assert(kFewRows == kCombineSpan, "one workgroup per few-row unit");
-template <int kRows, int kAtOnce>
-__device__ __forceinline__ void merge_rows(const PackedArgs& a, const Unit& x, int kvh, int G, const float* parts,
-                                           bool few, int share, int end, int row0) {
-    const int d = 4 * (threadIdx.x & 31);
-    float M[kRows], L[kRows];
-    float4 o[kRows];
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) M[r] = -INFINITY, L[r] = 0.f, o[r] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int p = share; p <= end; p += kAtOnce) {
-        float2 ml[kAtOnce][kRows];
-        float4 v[kAtOnce][kRows];
-#pragma unroll
-        for (int i = 0; i < kAtOnce; ++i) {
-            const int q = min(p + i, end);
-            const float* b = parts + part_at(few, q * a.HKV + kvh, q == share ? 1 : 0);
-#pragma unroll
-            for (int r = 0; r < kRows; ++r) {  // (rows past the unit's last: what the part has there, not written)
-                const int row = row0 + kCombineRows * r;
-                ml[i][r] = *reinterpret_cast<const float2*>(b + (few ? kFewRows : kUnitRows) * kHeadDim + 2 * row);
-                v[i][r] = *reinterpret_cast<const float4*>(b + row * kHeadDim + d);
-            }
-        }
-#pragma unroll
-        for (int r = 0; r < kRows; ++r) {
-            float mn = M[r];
-#pragma unroll
-            for (int i = 0; i < kAtOnce; ++i)
-                if (p + i <= end) mn = fmaxf(mn, ml[i][r].x);
-            const float c = M[r] == mn ? 1.f : __builtin_amdgcn_exp2f(M[r] - mn);
-            M[r] = mn;
-            L[r] *= c, o[r].x *= c, o[r].y *= c, o[r].z *= c, o[r].w *= c;
-#pragma unroll
-            for (int i = 0; i < kAtOnce; ++i) {
-                if (p + i > end || (ml[i][r].x == -INFINITY && ml[i][r].y == 0.f)) continue;
-                const float wv = __builtin_amdgcn_exp2f(ml[i][r].x - mn);
-                L[r] = __builtin_fmaf(wv, ml[i][r].y, L[r]);
-                o[r].x = __builtin_fmaf(wv, v[i][r].x, o[r].x), o[r].y = __builtin_fmaf(wv, v[i][r].y, o[r].y);
-                o[r].z = __builtin_fmaf(wv, v[i][r].z, o[r].z), o[r].w = __builtin_fmaf(wv, v[i][r].w, o[r].w);
-            }
-        }
-    }
-#pragma unroll
-    for (int r = 0; r < kRows; ++r) {
-        const int f = kUnitRows * x.u + row0 + kCombineRows * r, t0 = f / G;
-        if (f >= x.n * G) break;
-        const float inv = x.len - x.n + t0 < 0 ? 0.f : 1.f / L[r];  // a row that sees no key: zeros
-        *reinterpret_cast<float4*>(a.out + (((size_t)x.row0 + t0) * a.H + kvh * G + f - t0 * G) * kHeadDim + d) =
-            make_float4(o[r].x * inv, o[r].y * inv, o[r].z * inv, o[r].w * inv);
-    }
-}
-__global__ __launch_bounds__(32 * kCombineRows) void k_packed_combine(PackedArgs a, bool prompts, int shares,
+// The units that the cuts divide.  Part p of a unit is slot 1 of the share that it begins in, then slot 0 of each share
+// that it reaches: o = sum_p 2^(m_p - M) O_p / sum_p 2^(m_p - M) l_p over the parts that saw a key (m = -inf and
+// l = 0 otherwise; m = -inf with a NaN l counts).
+//
+// Every workgroup of a KV head collects the head's cut units from the shares, and they take eight rows at a time in
+// turn, a thread four columns of one.  A round trip to memory for the shares, one for the parts: those of one
+// unit on many CUs, since one CU draws some 20 KB/us.
+constexpr int kCombineRows = 8, kCombineWgs = 512;
+struct Merge {
+    Unit x;
+    int share, end;
+};
+__global__ __launch_bounds__(32 * kCombineRows) void k_packed_combine(PackedArgs a, bool prompts, int shares, int wgs,
                                                                       const float* __restrict__ wide_parts,
                                                                       const float* __restrict__ few_parts) {
-    const int kvh = blockIdx.x % a.HKV, share = blockIdx.x / a.HKV, G = a.H / a.HKV;
-    const bool few = blockIdx.y >= kCombineWide;
+    __shared__ Merge merges[2 * kPackedCus];  // by share, few-row ones after the wide ones
+    __shared__ uint64_t cut[2 * kPackedCus / 64];
+    __shared__ int order[2 * kPackedCus];     // the shares with one, in order
+    const int tid = threadIdx.x, kvh = blockIdx.x % a.HKV, G = a.H / a.HKV;
     const PlanView pv = plan_view(const_cast<char*>(a.plan), a.n_seq, a.rows, G, shares);
-    const List list = few ? pv.few : pv.wide;
-    const int end = list.shares[share].merge_end;
-    const Unit x = list.shares[share].merge;
-    if (!plan_fits(a.plan, a.n_seq, a.rows, a.H, a.HKV, prompts) || end == 0) return;
-    const int first = few ? 0 : (int)blockIdx.y * kCombineSpan, row0 = first + (int)(threadIdx.x >> 5);
-    const int rows = x.n * G - kUnitRows * x.u - first;  // (of the unit, from this workgroup's first on)
-    if (row0 - first >= rows) return;
-    const float* parts = few ? few_parts : wide_parts;
-    if (rows <= kCombineRows) merge_rows<1, 8>(a, x, kvh, G, parts, few, share, end, row0);
-    else merge_rows<kCombineSpan / kCombineRows, 4>(a, x, kvh, G, parts, few, share, end, row0);
+    if (!plan_fits(a.plan, a.n_seq, a.rows, a.H, a.HKV, prompts)) return;
+    for (int t = tid; t < 2 * kPackedCus; t += 32 * kCombineRows) {
+        int end = 0;
+        if (t < 2 * shares) {
+            const Share* at = pv.wide.shares + t;  // (the few-row list's follow)
+            end = at->merge_end;
+            merges[t] = {at->merge, t < shares ? t : t - shares, end};
+        }
+        const uint64_t cuts = __builtin_amdgcn_ballot_w64(end > 0);
+        if ((t & 63) == 0) cut[t >> 6] = cuts;
+    }
+    __syncthreads();
+    auto before = [&](int t) {  // shares below t with a cut unit
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < 2 * kPackedCus / 64; ++i) {
+            const int in = min(max(t - 64 * i, 0), 64);
+            n += __builtin_popcountll(in == 64 ? cut[i] : cut[i] & ((1ull << in) - 1));
+        }
+        return n;
+    };
+    for (int t = tid; t < 2 * shares; t += 32 * kCombineRows)
+        if (cut[t >> 6] >> (t & 63) & 1) order[before(t)] = t;
+    const int wide = before(shares), few_rows = before(2 * shares) - wide;
+    __syncthreads();
+    const int n_wide = wide * (kUnitRows / kCombineRows), n_few = few_rows * (kFewRows / kCombineRows);
+    const int d = 4 * (tid & 31);
+    for (int i = blockIdx.x / a.HKV; i < n_wide + n_few; i += wgs) {
+        const bool few = i >= n_wide;
+        const int j = few ? i - n_wide : i, n = few ? few_rows : wide;
+        const Merge& m = merges[order[few ? wide + j % n : j % n]];
+        const int row = j / n * kCombineRows + (tid >> 5), f = kUnitRows * m.x.u + row;
+        if (f >= m.x.n * G) continue;
+        const float* parts = few ? few_parts : wide_parts;
+        float M = -INFINITY, L = 0.f;
+        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+        constexpr int kAtOnce = 8;  // parts whose loads are in flight together
+        for (int p = m.share; p <= m.end; p += kAtOnce) {
+            float2 ml[kAtOnce];
+            float4 v[kAtOnce];
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+                const int q = min(p + k, m.end);
+                const float* b = parts + part_at(few, q * a.HKV + kvh, q == m.share ? 1 : 0);
+                ml[k] = *reinterpret_cast<const float2*>(b + (few ? kFewRows : kUnitRows) * kHeadDim + 2 * row);
+                v[k] = *reinterpret_cast<const float4*>(b + row * kHeadDim + d);
+            }
+            float mn = M;
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) mn = fmaxf(mn, ml[k].x);
+            const float c = M == mn ? 1.f : __builtin_amdgcn_exp2f(M - mn);
+            M = mn;
+            L *= c, o.x *= c, o.y *= c, o.z *= c, o.w *= c;
+#pragma unroll
+            for (int k = 0; k < kAtOnce; ++k) {
+                // (past the end: the last part again, with no weight)
+                const bool none = (p + k > m.end) | ((ml[k].x == -INFINITY) & (ml[k].y == 0.f));
+                const float wv = none ? 0.f : __builtin_amdgcn_exp2f(ml[k].x - M);
+                L = __builtin_fmaf(wv, ml[k].y, L);
+                o.x = __builtin_fmaf(wv, v[k].x, o.x), o.y = __builtin_fmaf(wv, v[k].y, o.y);
+                o.z = __builtin_fmaf(wv, v[k].z, o.z), o.w = __builtin_fmaf(wv, v[k].w, o.w);
+            }
+        }
+        const int t0 = f / G;
+        const float inv = m.x.len - m.x.n + t0 < 0 ? 0.f : 1.f / L;  // a row that sees no key: zeros
+        *reinterpret_cast<float4*>(a.out + (((size_t)m.x.row0 + t0) * a.H + kvh * G + f - t0 * G) * kHeadDim + d) =
+            make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+    }
 }
 
 // ------------------------------------------------------------------ the step's prologue
@@ -1512,8 +1524,8 @@ hipError_t launch_packed(hipStream_t st, const PackedArgs& a, void* ws) {
     const hipError_t e = a.btab ? launch_packed_attn<true>(st, a, shares, wide, few)
                                 : launch_packed_attn<false>(st, a, shares, wide, few);
     if (e != hipSuccess) return e;
-    k_packed_combine<<<dim3(shares * a.HKV, kCombineWide + 1), 32 * kCombineRows, 0, st>>>(
-        a, a.btab == nullptr, shares, wide, few);
+    const int wgs = kCombineWgs / a.HKV > 1 ? kCombineWgs / a.HKV : 1;
+    k_packed_combine<<<wgs * a.HKV, 32 * kCombineRows, 0, st>>>(a, a.btab == nullptr, shares, wgs, wide, few);
     return hipGetLastError();
 }
 
