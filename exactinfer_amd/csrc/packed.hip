@@ -34,7 +34,7 @@ constexpr int kFewRows = 32;    // a sequence's last unit of up to so many rows:
 // gives the same bits twice.
 //
 // One workgroup, a thread per sequence, unit or cut, everything in LDS as long as it fits: its time is the
-// latency of a dozen steps that need each other, 7 us for 5 sequences, 10 for 6 of up to 8192 rows (490 wide
+// latency of a dozen steps that need each other, 8 us for 5 sequences, 10 for 6 of up to 8192 rows (490 wide
 // units), 5.5 and 8 in a graph; once per forward pass, not per layer.
 struct Unit {
     int row0, n, len, u;    // the sequence's first row, rows and keys; the unit's number in it
@@ -369,7 +369,7 @@ __device__ __forceinline__ int row_owner(const int4* seq, int n_seq, int b, int 
 // What the scaling of V cannot hold is noticed at the end of a pass (planes_failed) and multiplied in fp32.
 //
 // What bounds it is the power of the matrix instructions: 8192, 4096, 2048, 1024, 300 and 17 rows (H 32 / HKV 8)
-// take 2235 us, 327 TFLOP/s, with the matrix unit busy 46% of the time at 1.9 GHz.  With two products of three
+// take 2236 to 2315 us, 316 to 327 TFLOP/s, with the matrix unit busy 46% of the time at 1.9 GHz.  With two products of three
 // taken out 1530 us, with the loop's loads out 11% less, with the LDS reads out 3%; more fragments in flight,
 // other interleavings of the splits and no priorities all came within 3%.  Three bf16 planes: 3370 us.
 //
@@ -1342,6 +1342,8 @@ __global__ __launch_bounds__(64 * kWaves) void k_packed_attn(PackedArgs a, int s
 // Every workgroup of a KV head collects the head's cut units from the shares, and they take eight rows at a time in
 // turn, a thread four columns of one.  A round trip to memory for the shares, one for the parts: those of one
 // unit on many CUs, since one CU draws some 20 KB/us.
+// 64 rows after 448 keys (8 parts each) 5 us, against 17 with four workgroups per unit.  1024 workgroups instead of 512
+// cost 0.5 us where there is nothing to merge.
 constexpr int kCombineRows = 8, kCombineWgs = 512;
 struct Merge {
     Unit x;
