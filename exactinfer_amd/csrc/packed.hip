@@ -138,7 +138,8 @@ __device__ __forceinline__ long long block_scan(long long v, long long* total) {
 
 __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restrict__ cu,
                                                               const int* __restrict__ kv_len, int n_seq, int rows,
-                                                              int max_kv, int H, int HKV, int shares,
+                                                              int max_kv, int H, int HKV, int shares, FastDiv by_g,
+                                                              FastDiv by_shares, double one_share,
                                                               char* __restrict__ plan) {
     __shared__ int4 seq_lds[kPlanSeqLds];
     __shared__ Unit wide_lds[kPlanLineLds], few_lds[kPlanLineLds];  // the lines' units
@@ -152,67 +153,9 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
     const PlanView pv = plan_view(plan, n_seq, rows, G, shares);
     // keys that rows up to `row` of a sequence of n rows and len keys see, in tiles
     auto tiles_of = [](int n, int len, int row) { return (max(min(len - n + row + 1, len), 0) + kKT - 1) / kKT; };
-    auto wide_of = [&](int n) { return (int)(((long long)n * G + kUnitRows - 1 - kFewRows) / kUnitRows); };
-
-    // The shares of a list whose line has `line` units: share j's end where `mine` of thread j + 1 falls on
-    // the line's running cost.
-    auto cut_line = [&](const List& list, int rounds, int line, ListCost c, const Unit* lds, long long share,
-                        long long mine) {
-        const int dealt = rounds * shares;
-        int turn = c.turn;
-        while (turn > 1 && turn > share) turn >>= 1;  // (less than a turn each: idle waves cost nothing then)
-        const int keep = max(turn, (int)min(share / 2, (long long)c.pass));
-        int2 cut = make_int2(tid == 0 ? 0 : line, 0);  // thread j: the end of share j - 1
-        long long cost_at = tid == 0 ? 0 : -1;
-        if (tid == 0 || tid >= shares) mine = -1;
-        long long at = 0;
-        for (int base = 0; base < line; base += kPlanThreads) {
-            const int i = base + tid;
-            const int tiles = i >= line ? 0 : lds ? lds[i].tiles : list.units[dealt + i].tiles;
-            long long sum;
-            const long long a = at + block_scan(i < line ? tiles + c.pass : 0, &sum);
-            line_at[tid] = a, line_tiles[tid] = tiles;
-            __syncthreads();
-            if (mine >= at && mine < at + sum) {
-                int lo = 0, hi = min(line - base, kPlanThreads) - 1;
-                while (lo < hi) {  // the last unit that begins at or before the cut
-                    const int mid = (lo + hi + 1) >> 1;
-                    if (line_at[mid] <= mine) lo = mid;
-                    else hi = mid - 1;
-                }
-                const long long in = mine - line_at[lo];
-                const int n = line_tiles[lo], t = (int)min(in, (long long)n) & ~(turn - 1);
-                // inside the unit, or at the end of it whose `keep` tiles it falls in (the nearer one, if it is
-                // too short to be cut at all): later cuts never come before earlier ones
-                const bool inside = t >= keep && t + keep <= n;
-                const bool after = !inside && (n >= 2 * keep ? t >= keep : 2 * in >= n + c.pass);
-                cut = make_int2(base + lo + after, inside ? t : 0);
-                cost_at = line_at[lo] + (inside ? t : after ? n + c.pass : 0);
-            }
-            at += sum;
-        }
-        if (tid <= shares) cuts[tid] = cut, cut_cost[tid] = cost_at < 0 ? at : cost_at;  // (past the end: all of it)
-        __syncthreads();
-        if (tid < shares) {
-            const int2 from = cuts[tid], to = cuts[tid + 1];
-            Share& x = list.shares[tid];
-            x.first = from.x, x.first_tile = from.y, x.last = to.x, x.last_tile = to.y;
-            if (rounds > 0) x.start = list.units[tid];
-            else if (from.x < line) x.start = lds ? lds[from.x] : list.units[from.x];
-            int end = 0;
-            if (to.y > 0 && !(from.x == to.x && from.y > 0)) {  // a unit begins here and goes on
-                end = tid + 1;
-                for (int hi = shares - 1; end < hi;) {  // to the last cut that is not past it
-                    const int mid = (end + hi + 1) >> 1;
-                    if (cuts[mid].x == to.x) end = mid;
-                    else hi = mid - 1;
-                }
-                x.merge = lds ? lds[to.x] : list.units[dealt + to.x];
-            }
-            x.merge_end = end;
-        }
-        __syncthreads();
-    };
+    auto wide_of = [&](int n) { return (int)((unsigned)(n * G + kUnitRows - 1 - kFewRows) / kUnitRows); };
+    // a share of a cost, rounded up (one_share = 1 / shares; what its rounding adds is below the 2^-20)
+    auto share_of = [&](unsigned long long cost) { return (long long)ceil((double)(long long)cost * one_share - 0x1p-20); };
 
     if (tid == 0) few_cost = wide_cost = 0;
     for (int j = tid; j < shares; j += kPlanThreads) load[j] = 0;
@@ -231,7 +174,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
         }
         bad = __syncthreads_or(bad);
         if (bad) n = 0;  // rows outside the batch: no call on this plan does anything
-        const int nw = wide_of(n), is_few = (long long)n * G > (long long)nw * kUnitRows;
+        const int nw = wide_of(n), is_few = n * G > nw * kUnitRows;
         const int tiles = is_few ? tiles_of(n, len, n - 1) : 0;
         long long all;
         const long long at = block_scan((long long)nw << 32 | is_few, &all);  // (both sums stay below 2^31)
@@ -265,7 +208,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
         }
         const int4 e = seq_at(lo);
         const int u = i - e.w;
-        const int row = min(e.y - 1, (kUnitRows * u + kUnitRows - 1) / G);
+        const int row = min(e.y - 1, fdiv(kUnitRows * u + kUnitRows - 1, by_g));
         return Unit{e.x, e.y, e.z, u, lo, tiles_of(e.y, e.z, row), {0, 0}};
     };
     // wide units of sequence e with more than t tiles (they are its last ones)
@@ -274,10 +217,10 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
         if (t < 0) return nw;
         const long long m = 32LL * t - (e.z - e.y);  // rows that see at most t tiles
         if (m <= 0) return nw;
-        return m >= e.y ? 0 : nw - min(nw, (int)(m * G / kUnitRows));
+        return m >= e.y ? 0 : nw - min(nw, (int)((unsigned)((int)m * G) / kUnitRows));
     };
     // (sorting costs units x sequences: where that is much, there is enough work for the order not to matter)
-    const int full = (long long)U * n_seq <= kMaxRankWork ? U / shares : 0, sure = max(full - 1, 0) * shares;
+    const int full = (long long)U * n_seq <= kMaxRankWork ? fdiv(U, by_shares) : 0, sure = max(full - 1, 0) * shares;
     long long mine = 0;
     for (int i = tid; i < U; i += kPlanThreads) {
         const Unit x = unit(i);
@@ -294,7 +237,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
             }
         }
         pv.wide.units[at] = x;
-        const int r = at / shares, j = at - r * shares;
+        const int r = fdiv(at, by_shares), j = at - r * shares;
         if (at < sure) atomicAdd(&load[(r & 1) ? shares - 1 - j : j], (unsigned long long)cost);
         else if (r < full) last_round[(r & 1) ? shares - 1 - j : j] = cost;
         if (at >= sure && at - sure < kPlanLineLds) wide_lds[at - sure] = x;
@@ -303,31 +246,86 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
     if ((tid & 63) == 63 && mine > 0) atomicAdd(&wide_cost, (unsigned long long)mine);
     __syncthreads();
     // all rounds, or all but one
-    const long long both = (long long)ceil((double)(wide_cost + few_cost) / shares);
+    const long long both = share_of(wide_cost + few_cost);
     const bool over = full > 0 && tid < shares && (long long)load[tid] + last_round[tid] > both + both / kDealSlack;
     const int rounds = __syncthreads_or(over) ? full - 1 : full;
-    const int dealt = rounds * shares, line = U - dealt;
+    const int dealt = rounds * shares;
     if (rounds > 0 && rounds == full && tid < shares) load[tid] += last_round[tid];
-    {
-        const long long share = (long long)ceil((double)wide_cost / shares);
-        long long before = tid * share, all;
-        if (rounds > 0) before = block_scan(tid < shares ? max(share - (long long)load[tid], 0LL) : 0, &all);
-        cut_line(pv.wide, rounds, line, kWideCost, U - sure <= kPlanLineLds ? wide_lds + (dealt - sure) : nullptr, share,
-                 before);
-    }
-    {
-        const long long share = (long long)ceil((double)few_cost / shares);
-        const long long wide = tid < shares ? (long long)load[tid] + cut_cost[tid + 1] - cut_cost[tid] : 0;
-        long long all;
-        const long long before = block_scan(tid < shares ? max(both - wide, 0LL) : 0, &all);
-        cut_line(pv.few, 0, (int)few, kFewCost, few <= kPlanLineLds ? few_lds : nullptr, share, before);
+    // The wide line's shares, then the few-row line's.  Share j's end lies where the sum of what shares 0 .. j want
+    // falls on the line's running cost.  (One code for both: a single workgroup waits for each instruction once.)
+    long long taken = tid < shares ? (long long)load[tid] : 0;  // the share's work so far
+#pragma unroll 1
+    for (int which = 0; which < 2; ++which) {
+        const List& list = which ? pv.few : pv.wide;
+        const int line = which ? (int)few : U - dealt, first = which ? 0 : dealt;
+        const int pass = which ? kFewCost.pass : kWideCost.pass;
+        const long long share = share_of(which ? few_cost : wide_cost);
+        // the line's units in LDS, where it fits
+        const bool fits = (which ? line : U - sure) <= kPlanLineLds;
+        const Unit* lds = which ? few_lds : wide_lds + (dealt - sure);
+        auto unit_at = [&](int i) { return fits ? lds[i] : list.units[first + i]; };
+        int turn = which ? kFewCost.turn : kWideCost.turn;
+        while (turn > 1 && turn > share) turn >>= 1;  // (less than a turn each: idle waves cost nothing then)
+        const int keep = max(turn, (int)min(share / 2, (long long)pass));
+        long long total;
+        long long mine = block_scan(tid < shares ? max((which ? both : share) - taken, 0LL) : 0, &total);
+        int2 cut = make_int2(tid == 0 ? 0 : line, 0);  // thread j: the end of share j - 1
+        long long cost_at = tid == 0 ? 0 : -1;
+        if (tid == 0 || tid >= shares) mine = -1;
+        long long at = 0;
+        for (int base = 0; base < line; base += kPlanThreads) {
+            const int i = base + tid;
+            const int tiles = i >= line ? 0 : fits ? lds[i].tiles : list.units[first + i].tiles;
+            long long sum;
+            const long long a = at + block_scan(i < line ? tiles + pass : 0, &sum);
+            line_at[tid] = a, line_tiles[tid] = tiles;
+            __syncthreads();
+            if (mine >= at && mine < at + sum) {
+                int lo = 0, hi = min(line - base, kPlanThreads) - 1;
+                while (lo < hi) {  // the last unit that begins at or before the cut
+                    const int mid = (lo + hi + 1) >> 1;
+                    if (line_at[mid] <= mine) lo = mid;
+                    else hi = mid - 1;
+                }
+                const long long in = mine - line_at[lo];
+                const int n = line_tiles[lo], t = (int)min(in, (long long)n) & ~(turn - 1);
+                // inside the unit, or at the end of it whose `keep` tiles it falls in (the nearer one, if it is
+                // too short to be cut at all): later cuts never come before earlier ones
+                const bool inside = t >= keep && t + keep <= n;
+                const bool after = !inside && (n >= 2 * keep ? t >= keep : 2 * in >= n + pass);
+                cut = make_int2(base + lo + after, inside ? t : 0);
+                cost_at = line_at[lo] + (inside ? t : after ? n + pass : 0);
+            }
+            at += sum;
+        }
+        if (tid <= shares) cuts[tid] = cut, cut_cost[tid] = cost_at < 0 ? at : cost_at;  // (past the end: all of it)
+        __syncthreads();
+        if (tid < shares) {
+            const int2 from = cuts[tid], to = cuts[tid + 1];
+            taken += cut_cost[tid + 1] - cut_cost[tid];
+            Share& x = list.shares[tid];
+            x.first = from.x, x.first_tile = from.y, x.last = to.x, x.last_tile = to.y;
+            if (first > 0) x.start = list.units[tid];
+            else if (from.x < line) x.start = unit_at(from.x);
+            int end = 0;
+            if (to.y > 0 && !(from.x == to.x && from.y > 0)) {  // a unit begins here and goes on
+                end = tid + 1;
+                for (int hi = shares - 1; end < hi;) {  // to the last cut that is not past it
+                    const int mid = (end + hi + 1) >> 1;
+                    if (cuts[mid].x == to.x) end = mid;
+                    else hi = mid - 1;
+                }
+                x.merge = unit_at(to.x);
+            }
+            x.merge_end = end;
+        }
     }
     if (tid == 0) {
         int* h = reinterpret_cast<int*>(plan);
         h[0] = bad ? 0 : kPlanMagic;
         h[1] = n_seq, h[2] = rows, h[3] = H, h[4] = HKV;
         h[5] = kv_len == nullptr;
-        h[kHeadRounds] = rounds, h[kHeadDealt] = dealt, h[kHeadLine] = line, h[kHeadFew] = (int)few;
+        h[kHeadRounds] = rounds, h[kHeadDealt] = dealt, h[kHeadLine] = U - dealt, h[kHeadFew] = (int)few;
     }
 }
 
@@ -1503,8 +1501,10 @@ __global__ __launch_bounds__(256) void k_packed_prepare(const float* __restrict_
 // ------------------------------------------------------------------ launchers
 hipError_t launch_packed_plan(hipStream_t st, const int* cu, const int* kv_len, int n_seq, int rows, int max_kv, int H,
                               int HKV, void* plan) {
-    k_packed_plan<<<1, kPlanThreads, 0, st>>>(cu, kv_len, n_seq, rows, max_kv, H, HKV, packed_shares(HKV),
-                                              static_cast<char*>(plan));
+    const int shares = packed_shares(HKV);
+    auto by = [](uint32_t d) { return FastDiv{d == 1 ? 0u : 0xFFFFFFFFu / d + 1u, d}; };
+    k_packed_plan<<<1, kPlanThreads, 0, st>>>(cu, kv_len, n_seq, rows, max_kv, H, HKV, shares, by((uint32_t)(H / HKV)),
+                                              by((uint32_t)shares), 1.0 / shares, static_cast<char*>(plan));
     return hipGetLastError();
 }
 
