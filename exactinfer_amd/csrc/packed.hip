@@ -35,7 +35,7 @@ constexpr int kFewRows = 32;    // a sequence's last unit of up to so many rows:
 //
 // One workgroup, a thread per sequence, unit or cut, everything in LDS as long as it fits: its time is the
 // latency of a dozen steps that need each other, 8 us for 5 sequences, 10 for 6 of up to 8192 rows (490 wide
-// units), 5.5 and 8 in a graph; once per forward pass, not per layer.
+// units), 6 to 8 in a graph; once per forward pass, not per layer.
 struct Unit {
     int row0, n, len, u;    // the sequence's first row, rows and keys; the unit's number in it
     int seq, tiles, pad[2];
@@ -98,7 +98,8 @@ struct ListCost {
 };
 // Measured (H / HKV, single tokens): a few-row pass at 5 instead of 8, 24 sequences of 2001 keys 77 us against 85
 // (16/8), 50 of up to 4000 117 against 122 (16/8), 6 of 4 tokens after 3000 keys 38 against 41 (32/8); 16 of 5
-// tokens after 1024 to 1579 keys 57 against 55.  A wide pass at 7 instead of 5: one prompt of 1024 rows 66 us against 61.
+// tokens after 1024 to 1579 keys 57 against 55.  A wide pass at 7 instead of 5: one prompt of 1024 rows 66 us
+// against 61.
 constexpr ListCost kWideCost = {5, 2}, kFewCost = {5, 8};
 
 // Sum over the lanes up to this one, by DPP: within rows of 16, then the last lane of each row (15), of
@@ -155,7 +156,9 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
     auto tiles_of = [](int n, int len, int row) { return (max(min(len - n + row + 1, len), 0) + kKT - 1) / kKT; };
     auto wide_of = [&](int n) { return (int)((unsigned)(n * G + kUnitRows - 1 - kFewRows) / kUnitRows); };
     // a share of a cost, rounded up (one_share = 1 / shares; what its rounding adds is below the 2^-20)
-    auto share_of = [&](unsigned long long cost) { return (long long)ceil((double)(long long)cost * one_share - 0x1p-20); };
+    auto share_of = [&](unsigned long long cost) {
+        return (long long)ceil((double)(long long)cost * one_share - 0x1p-20);
+    };
 
     if (tid == 0) few_cost = wide_cost = 0;
     for (int j = tid; j < shares; j += kPlanThreads) load[j] = 0;
@@ -367,8 +370,8 @@ __device__ __forceinline__ int row_owner(const int4* seq, int n_seq, int b, int 
 // What the scaling of V cannot hold is noticed at the end of a pass (planes_failed) and multiplied in fp32.
 //
 // What bounds it is the power of the matrix instructions: 8192, 4096, 2048, 1024, 300 and 17 rows (H 32 / HKV 8)
-// take 2236 to 2315 us, 316 to 327 TFLOP/s, with the matrix unit busy 46% of the time at 1.9 GHz.  With two products of three
-// taken out 1530 us, with the loop's loads out 11% less, with the LDS reads out 3%; more fragments in flight,
+// take 2236 to 2315 us, 316 to 327 TFLOP/s, with the matrix unit busy 46% of the time at 1.9 GHz.  With two products
+// of three taken out 1530 us, with the loop's loads out 11% less, with the LDS reads out 3%; more fragments in flight,
 // other interleavings of the splits and no priorities all came within 3%.  Three bf16 planes: 3370 us.
 //
 // A wave holds 32 flat query rows and computes S^T[key][row] = K . Q^T, so that each lane owns one row and

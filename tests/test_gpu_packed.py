@@ -151,7 +151,7 @@ def _check_prompts(out, q, k, v, lens, H, HKV, scale=SCALE):
 
 @pytest.mark.parametrize("H,HKV,lens", [
     (8, 8, [1]), (16, 8, [2, 1]), (16, 8, [37, 1, 96, 5, 64]), (32, 8, [0, 40, 0, 0, 300, 3, 0]),
-    (40, 8, [31, 32, 33, 64, 65, 127, 128, 129]), (24, 8, [77, 200]), (8, 1, [257, 13]), (48, 8, [50, 51]),
+    (40, 8, [31, 32, 33, 64, 65, 127, 128, 129]), (18, 6, [77, 200]), (8, 1, [257, 13]), (48, 8, [50, 51]),
     (56, 8, [19, 90]), (6, 3, [100, 45]), (32, 8, [1100, 900, 17]), (8, 8, [600] * 3),
 ])
 def test_packed_prompts(gpu, H, HKV, lens):
@@ -434,7 +434,7 @@ CHUNKS = [  # H, HKV, block, lens, kv_len
     (8, 8, 32, [1], [1]), (16, 8, 64, [1] * 7, [1, 31, 32, 33, 64, 65, 700]),
     (16, 8, 64, [1, 100, 1, 60, 1], [301, 612, 34, 60, 901]), (40, 8, 32, [5] * 6, [29, 64, 101, 256, 300, 5]),
     (32, 8, 128, [130, 40], [1300, 40]), (8, 1, 256, [17, 0, 3], [500, 77, 1000]), (64, 8, 32, [3, 33], [400, 33]),
-    (16, 8, 32, [6, 9, 3, 1], [2, 0, 3, 0]), (24, 8, 64, [2, 70], [4000, 333]), (8, 2, 64, [1, 1], [9000, 12]),
+    (16, 8, 32, [6, 9, 3, 1], [2, 0, 3, 0]), (18, 6, 64, [2, 70], [4000, 333]), (8, 2, 64, [1, 1], [9000, 12]),
 ]
 
 
