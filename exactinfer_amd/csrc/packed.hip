@@ -89,8 +89,8 @@ constexpr int kDealSlack = 32;          // whole units may pass an equal share b
                                         // 600 rows after 9000 keys, 300 and 200, 928 instead of 644)
 
 // What a list's work costs, in tiles: `pass` for everything done once per unit or part of one; a cut leaves
-// whole turns (the tiles that a workgroup's waves take at a time, a power of two; less where there is less than a turn
-// for each) on both sides, and keeps off a unit's ends by what a pass costs, so that a share does not run one for a
+// whole turns (the tiles that a workgroup's waves take at a time, a power of two; less where all the work there is
+// would not give each one) on both sides, and keeps off a unit's ends by what a pass costs, so that a share does not run one for a
 // few tiles.  Without the smaller turns one token at 2000 keys takes 20.3 us instead of 13.7, at 255 14.3 instead of
 // 11.0, a draft of 5 of H 32 after 1000 keys 21.4 instead of 15.5.
 struct ListCost {
@@ -268,7 +268,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
         const Unit* lds = which ? few_lds : wide_lds + (dealt - sure);
         auto unit_at = [&](int i) { return fits ? lds[i] : list.units[first + i]; };
         int turn = which ? kFewCost.turn : kWideCost.turn;
-        while (turn > 1 && turn > share) turn >>= 1;  // (less than a turn each: idle waves cost nothing then)
+        while (both < kFewCost.turn && turn > 1 && turn > share) turn >>= 1;  // (idle waves cost nothing then)
         const int keep = max(turn, (int)min(share / 2, (long long)pass));
         long long total;
         long long mine = block_scan(tid < shares ? max((which ? both : share) - taken, 0LL) : 0, &total);

@@ -102,7 +102,7 @@ def test_plan_covers_every_unit_once(gpu, H, HKV, lens, kv):
             r, j = divmod(i, N)
             load[N - 1 - j if r % 2 else j] += tiles[i] + once
         share = -(-sum(t + once for t in cost.values()) // N)
-        while turn > max(share, 1):
+        while turn > max(share, 1) and sum(t + 5 for c in want.values() for t in c.values()) <= 7 * N:
             turn //= 2
         n, at = len(units) - first, (0, 0)
         begins, ends = {}, {}  # shares in which a cut unit begins; the last share with a part of a unit
