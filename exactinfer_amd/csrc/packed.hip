@@ -1413,12 +1413,13 @@ __global__ __launch_bounds__(32 * kCombineRows) void k_packed_combine(PackedArgs
             L *= c, o.x *= c, o.y *= c, o.z *= c, o.w *= c;
 #pragma unroll
             for (int k = 0; k < kAtOnce; ++k) {
-                // (past the end: the last part again, with no weight)
+                // (past the end the last part was read again: no row then, since zero times an infinite one is NaN)
                 const bool none = (p + k > m.end) | ((ml[k].x == -INFINITY) & (ml[k].y == 0.f));
                 const float wv = none ? 0.f : __builtin_amdgcn_exp2f(ml[k].x - M);
+                const float4 x = none ? make_float4(0.f, 0.f, 0.f, 0.f) : v[k];
                 L = __builtin_fmaf(wv, ml[k].y, L);
-                o.x = __builtin_fmaf(wv, v[k].x, o.x), o.y = __builtin_fmaf(wv, v[k].y, o.y);
-                o.z = __builtin_fmaf(wv, v[k].z, o.z), o.w = __builtin_fmaf(wv, v[k].w, o.w);
+                o.x = __builtin_fmaf(wv, x.x, o.x), o.y = __builtin_fmaf(wv, x.y, o.y);
+                o.z = __builtin_fmaf(wv, x.z, o.z), o.w = __builtin_fmaf(wv, x.w, o.w);
             }
         }
         const int t0 = f / G;

@@ -1,0 +1,43 @@
+"""GPU tests of the packed batch (include/ei_packed.h) at the edges of its arithmetic and of its lengths, against
+softmax attention in 64 bits; the bar is that of tests/test_gpu_packed.py unless a test derives its own."""
+import pytest
+import torch
+
+from tests.parity import ATTN_RTOL, rel_err
+from tests.test_gpu_packed import D, SCALE, _attend64, _cu, _i32, _pool, _read_plan
+
+pytestmark = pytest.mark.gpu
+
+
+def _paged(gpu, q, kc, vc, table, bs, lens, kv, H, HKV, scale=None):
+    b = gpu.PackedBatch(len(lens), sum(lens), H, HKV)
+    b.plan(_i32(_cu(lens)), sum(lens), max(kv), kv_len=_i32(kv))
+    return b, gpu.attn_packed_paged(q, kc, vc, table, bs, b, gpu.AttnShape(H, HKV), scale=scale)
+
+
+def _check_paged(out, q, kc, vc, rows_of, lens, kv, H, scale=SCALE):
+    for s, (a, n) in enumerate(zip(_cu(lens), lens)):
+        r = slice(int(a), int(a) + n)
+        ref = _attend64(q[r].double().view(n, H, D), kc[rows_of[s]].double(), vc[rows_of[s]].double(), kv[s], scale)
+        e = rel_err(out[r].cpu().numpy(), ref.cpu().numpy())
+        assert e <= ATTN_RTOL, (s, e)
+
+
+@pytest.mark.parametrize("H,HKV,n", [(8, 1, 16), (32, 8, 64), (8, 1, 1), (16, 8, 1), (32, 8, 5)])
+@pytest.mark.parametrize("T", [3000, 5000, 9000])
+def test_infinite_value_in_the_last_part(gpu, H, HKV, n, T):
+    """Wide and few-row units cut into parts whose number is whatever it is: an infinity that every row sees in the
+    last part reaches the output as it is."""
+    kc, vc, table, rows_of = _pool([n], [T], HKV, 64, 201)
+    q = torch.randn((n, H * D), generator=torch.Generator(device="cuda").manual_seed(202), device="cuda")
+    at = rows_of[0][T - n]
+    vc[at, 0, 5], vc[at, 0, 70] = float("inf"), float("-inf")
+    b, out = _paged(gpu, q, kc, vc, table, 64, [n], [T], H, HKV)
+    _, _, wide, _, few = _read_plan(b, [n], n, H, HKV)
+    assert (wide[:, 4] > 0).any() or (few[:, 4] > 0).any()  # (a unit is cut)
+    G = H // HKV
+    assert (out[:, :G, 5] == float("inf")).all() and (out[:, :G, 70] == float("-inf")).all()
+    vc[at, 0, 5] = vc[at, 0, 70] = 0.0
+    ref = _attend64(q.double().view(n, H, D), kc[rows_of[0]].double(), vc[rows_of[0]].double(), T)
+    out[:, :G, 5], out[:, :G, 70] = ref[:, :G, 5].float(), ref[:, :G, 70].float()
+    assert rel_err(out.cpu().numpy(), ref.cpu().numpy()) <= ATTN_RTOL
