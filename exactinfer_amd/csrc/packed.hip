@@ -363,7 +363,8 @@ __device__ __forceinline__ int row_owner(const int4* seq, int n_seq, int b, int 
 // adding 128 products, for half the matrix instructions of three bf16 planes (prefill.hip), which keep
 // every bit.  The scalings:
 //   q, with the softmax scale in it: per row, taken back in the exponent's FMA
-//   K: per key, taken back in the scores (16 products per tile and lane)
+//   K: per key, taken back in the scores (16 products per tile and lane), before q's: up to kMostK, where the sum of
+//     128 products of up to 2^16 each stays finite; one that overflowed to -infinity would leave no trace
 //   V: per 32 columns, the running largest value of the tiles so far; sums are rescaled when it grows
 //   P: 2^14, so that weights of up to 2^kLazy fit (of one below 2^-39 nothing is left, at most that times
 //     the number of keys in all); the weights' sum has it too
@@ -400,6 +401,7 @@ constexpr int kWaves = kSlots * kGroups;
 // lazy-rescale thresholds (log2 units): sums are rescaled when the running maximum has risen by more (for
 // wide units, what a weight may pass 1 by comes off the range of its planes)
 constexpr float kLazy = 1.f, kFewLazy = 8.f;
+constexpr uint32_t kMostK = 127 + 100;          // the largest (biased) exponent of a key's planes
 constexpr float kPBits = 14.f;                  // wide units' weights and sums are times 2^kPBits
 constexpr int kXchF = 34;                       // floats per lane exchanged by the merge
 constexpr int kRowF = kHeadDim + 4;             // padded fp32 row of the staging area
@@ -548,11 +550,12 @@ __device__ __forceinline__ void mfma_halves(const Halves& a, const Halves& b, fl
     c = mfma_f16(a.h, b.l, c);
     c = mfma_f16(a.h, b.h, c);
 }
-// The power of two that brings `most` to 2^kTop .. 2^(kTop+1), and its inverse: `most`'s exponent is kept
-// where both are normal numbers.
-template <int kTop>
+// The power of two that brings `most` to 2^kTop .. 2^(kTop+1), and its inverse: `most`'s exponent (biased) is kept
+// where both are normal numbers, and below kMost: planes of what passes that overflow to infinities, their products
+// to NaN, and the wave takes its keys again in fp32.
+template <int kTop, uint32_t kMost = 254>
 __device__ __forceinline__ uint32_t scale_to(float most) {
-    const uint32_t e = min(max(__float_as_uint(most) >> 23, kTop + 2u), 254u);
+    const uint32_t e = min(max(__float_as_uint(most) >> 23, kTop + 2u), kMost);
     return (254u + kTop - e) << 23;
 }
 __device__ __forceinline__ float inverse(uint32_t scale) { return __uint_as_float(0x7F000000u - scale); }
@@ -736,7 +739,7 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
             most = fmaxf(most, lane_xor1(most));
             most = fmaxf(most, lane_xor2(most));
             most = fmaxf(most, lane_xor4(most));
-            const uint32_t f = scale_to<14>(most);
+            const uint32_t f = scale_to<14, kMostK>(most);
             fk = __uint_as_float(f);
             if ((lane & 7) == 0) k_scale[kKT * parity + 8 * hw + (lane >> 3)] = inverse(f);
         }

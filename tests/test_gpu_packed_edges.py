@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from tests.parity import ATTN_RTOL, rel_err
-from tests.test_gpu_packed import D, SCALE, _attend64, _cu, _i32, _pool, _read_plan
+from tests.test_gpu_packed import D, SCALE, _attend64, _check_prompts, _cu, _i32, _pool, _prompts, _read_plan, _run_prompts
 
 pytestmark = pytest.mark.gpu
 
@@ -41,3 +41,18 @@ def test_infinite_value_in_the_last_part(gpu, H, HKV, n, T):
     ref = _attend64(q.double().view(n, H, D), kc[rows_of[0]].double(), vc[rows_of[0]].double(), T)
     out[:, :G, 5], out[:, :G, 70] = ref[:, :G, 5].float(), ref[:, :G, 70].float()
     assert rel_err(out.cpu().numpy(), ref.cpu().numpy()) <= ATTN_RTOL
+
+
+@pytest.mark.parametrize("H,HKV,lens", [(16, 8, [100, 7, 300]), (8, 1, [60]), (32, 8, [4, 8, 1])])
+@pytest.mark.parametrize("e", [-104, -108, -112])
+@pytest.mark.parametrize("signs", ["any", "against", "one key"])
+def test_tiny_queries_of_huge_keys(gpu, H, HKV, lens, e, signs):
+    """q of about 2^e against keys of about 2^-e: the scores are ordinary, whatever lies between, also where all of a
+    row are negative, or a single key is huge."""
+    _, q, k, v = _prompts(H, HKV, lens, 203)
+    if signs != "any":
+        q, k = -q.abs(), k.abs()
+    if signs == "one key":
+        k[1:], k[0] = 0.0, k[0] * 0.25
+    q, k, v = (q * 2.0 ** e).contiguous(), (k * 2.0 ** -e).contiguous(), v.contiguous()
+    _check_prompts(_run_prompts(gpu, q, k, v, lens, H, HKV), q, k, v, lens, H, HKV)
