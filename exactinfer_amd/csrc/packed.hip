@@ -363,8 +363,13 @@ __device__ __forceinline__ int row_owner(const int4* seq, int n_seq, int b, int 
 // adding 128 products, for half the matrix instructions of three bf16 planes (prefill.hip), which keep
 // every bit.  The scalings:
 //   q, with the softmax scale in it: per row, taken back in the exponent's FMA
-//   K: per key, taken back in the scores (16 products per tile and lane), before q's: up to kMostK, where the sum of
-//     128 products of up to 2^16 each stays finite; one that overflowed to -infinity would leave no trace
+//   K: per key, taken back in the scores (16 products per tile and lane), before q's
+// What q's planes and K's lose at their lower end, 2^-39 of the row's largest, is at most 2^-31 of the product of the two
+// largest in a score, which shows where that product is large and the score is not (a channel of q far above the
+// others that meets zeros, and one of K).  So a key's planes go up to the exponent at which its largest value times the
+// unit's largest q is 2^13, and beyond that they overflow, which is noticed (2^-18 of a log2 unit is left; products of
+// trained models are some 2^10 at most); and up to kMostK, where the sum of 128 products of up to 2^32 is finite
+// with K's scaling taken out: one that went to -infinity on the way would leave no trace.
 //   V: per 32 columns, the running largest value of the tiles so far; sums are rescaled when it grows
 //   P: 2^14, so that weights of up to 2^kLazy fit (of one below 2^-39 nothing is left, at most that times
 //     the number of keys in all); the weights' sum has it too
@@ -401,7 +406,8 @@ constexpr int kWaves = kSlots * kGroups;
 // lazy-rescale thresholds (log2 units): sums are rescaled when the running maximum has risen by more (for
 // wide units, what a weight may pass 1 by comes off the range of its planes)
 constexpr float kLazy = 1.f, kFewLazy = 8.f;
-constexpr uint32_t kMostK = 127 + 100;          // the largest (biased) exponent of a key's planes
+// the largest (biased) exponents of a query's planes, of a key's, and of both together
+constexpr uint32_t kMostQ = 127 + 121, kMostK = 127 + 100, kMostQK = 2 * 127 + 10;
 constexpr float kPBits = 14.f;                  // wide units' weights and sums are times 2^kPBits
 constexpr int kXchF = 34;                       // floats per lane exchanged by the merge
 constexpr int kRowF = kHeadDim + 4;             // padded fp32 row of the staging area
@@ -411,15 +417,16 @@ constexpr int kKRowB = 2 * kHeadDim + 16, kKPlane = kKT * kKRowB;  // K plane: [
 constexpr int kVRowB = 2 * kKT + 16, kVPlane = kHeadDim * kVRowB;  // V plane, transposed: [128 d][32 keys]
 // LDS of a wide pass: the K planes of both groups, and the merge's exchange area, from 0; the V planes
 // after it, and over them the staging area of the unit's rows (queries, later outputs); then the scalings,
-// of K [group][tile parity][key] and of V [group][32 columns].  Of a few-rows pass: every wave's rows, and
+// of K [group][tile parity][key] and of V [group][32 columns], and each wave's largest q.  Of a few-rows pass: every wave's rows, and
 // their (m, l).
 constexpr int kStageF = kWaves * kXchF * 64;
 constexpr int kScaleK = kStageF + kUnitRows * kRowF, kScaleV = kScaleK + kGroups * 2 * kKT;
-constexpr int kWideF = kScaleV + kGroups * 4;
+constexpr int kMaxQ = kScaleV + kGroups * 4, kWideF = kMaxQ + kWaves;
 constexpr int kFewBlock = 16;                   // rows of one matrix instruction of few_pass
 constexpr int kFewML = kWaves * kFewRows * kRowF;
 constexpr int kFewF = kFewML + kWaves * kFewRows * 2;
 static_assert(kWaves * 64 == kFewRows * 16, "sixteen threads stage a row");
+static_assert(kSlots == 4, "a float4 of the largest q");
 static_assert(kGroups * 2 * kKPlane <= kStageF * 4, "K planes below the staging area");
 static_assert(kStageF * 4 + kGroups * 2 * kVPlane <= kScaleK * 4, "V planes within the LDS span");
 static_assert(kWideF * 4 <= 160 * 1024 && kFewF * 4 <= 160 * 1024, "LDS budget");
@@ -551,11 +558,11 @@ __device__ __forceinline__ void mfma_halves(const Halves& a, const Halves& b, fl
     c = mfma_f16(a.h, b.h, c);
 }
 // The power of two that brings `most` to 2^kTop .. 2^(kTop+1), and its inverse: `most`'s exponent (biased) is kept
-// where both are normal numbers, and below kMost: planes of what passes that overflow to infinities, their products
-// to NaN, and the wave takes its keys again in fp32.
-template <int kTop, uint32_t kMost = 254>
-__device__ __forceinline__ uint32_t scale_to(float most) {
-    const uint32_t e = min(max(__float_as_uint(most) >> 23, kTop + 2u), kMost);
+// where both are normal numbers, and up to `limit`: planes of what passes that by two overflow to infinities, their
+// products to NaN, and the waves that meet them take their keys again in fp32.
+template <int kTop>
+__device__ __forceinline__ uint32_t scale_to(float most, uint32_t limit = 254) {
+    const uint32_t e = min(max(__float_as_uint(most) >> 23, kTop + 2u), limit);
     return (254u + kTop - e) << 23;
 }
 __device__ __forceinline__ float inverse(uint32_t scale) { return __uint_as_float(0x7F000000u - scale); }
@@ -732,6 +739,7 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
     // scaling: of K the row's, of V the running one of the wave's 32 columns (four times its largest value
     // fits, so it changes rarely)
     float fk;
+    uint32_t k_limit;
     auto conv_k = [&](int x, int parity) {
         uint32_t ch[4], cl[4];
         if (x == 0) {
@@ -739,7 +747,7 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
             most = fmaxf(most, lane_xor1(most));
             most = fmaxf(most, lane_xor2(most));
             most = fmaxf(most, lane_xor4(most));
-            const uint32_t f = scale_to<14, kMostK>(most);
+            const uint32_t f = scale_to<14>(most, k_limit);
             fk = __uint_as_float(f);
             if ((lane & 7) == 0) k_scale[kKT * parity + 8 * hw + (lane >> 3)] = inverse(f);
         }
@@ -814,7 +822,8 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
             most = fmaxf(fmaxf(most, __builtin_fabsf(v.x * sl2)), __builtin_fabsf(v.y * sl2));
             most = fmaxf(fmaxf(most, __builtin_fabsf(v.z * sl2)), __builtin_fabsf(v.w * sl2));
         }
-        const uint32_t f = scale_to<14>(half_max(most));
+        most = half_max(most);
+        const uint32_t f = scale_to<14>(most, kMostQ);
         const float fq = __uint_as_float(f);
         sq = inverse(f);
 #pragma unroll
@@ -828,6 +837,13 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
             split_f16(v.z * sl2 * fq, v.w * sl2 * fq, h[3], l[3]);
             qp[t] = {u32x4{h[0], h[1], h[2], h[3]}, u32x4{l[0], l[1], l[2], l[3]}};
         }
+        // the unit's largest q, from the group's four waves, sets how large a key's planes may be
+        most = wave_max(most);
+        if (lane == 0) smem[kMaxQ + wu] = most;
+        lds_barrier();
+        const float4 m = *reinterpret_cast<const float4*>(smem + kMaxQ + kSlots * grp);
+        const float unit = fmaxf(fmaxf(m.x, m.y), fmaxf(m.z, m.w));
+        k_limit = scalar(min(kMostQK - min(max(__float_as_uint(unit) >> 23, 16u), kMostQ), kMostK));
     }
     if (n_mine > 0) {
 #pragma unroll

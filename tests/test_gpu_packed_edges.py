@@ -56,3 +56,15 @@ def test_tiny_queries_of_huge_keys(gpu, H, HKV, lens, e, signs):
         k[1:], k[0] = 0.0, k[0] * 0.25
     q, k, v = (q * 2.0 ** e).contiguous(), (k * 2.0 ** -e).contiguous(), v.contiguous()
     _check_prompts(_run_prompts(gpu, q, k, v, lens, H, HKV), q, k, v, lens, H, HKV)
+
+
+@pytest.mark.parametrize("H,HKV,lens", [(8, 1, [200]), (16, 8, [90, 300])])
+@pytest.mark.parametrize("e", [10, 22, 30, 60])
+def test_channels_that_meet_zeros(gpu, H, HKV, lens, e):
+    """A channel of q and one of K 2^e times the others, each against zeros: the scores are those of the others."""
+    _, q, k, v = (t.contiguous() for t in _prompts(H, HKV, lens, 208))
+    q[:, 3::D] *= 2.0 ** e
+    k[:, 3::D] = 0.0
+    k[:, 77::D] *= 2.0 ** e
+    q[:, 77::D] = 0.0
+    _check_prompts(_run_prompts(gpu, q, k, v, lens, H, HKV), q, k, v, lens, H, HKV)
