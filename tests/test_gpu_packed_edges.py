@@ -1,5 +1,6 @@
 """GPU tests of the packed batch (include/ei_packed.h) at the edges of its arithmetic and of its lengths, against
 softmax attention in 64 bits; the bar is that of tests/test_gpu_packed.py unless a test derives its own."""
+import numpy as np
 import pytest
 import torch
 
@@ -68,3 +69,63 @@ def test_channels_that_meet_zeros(gpu, H, HKV, lens, e):
     k[:, 77::D] *= 2.0 ** e
     q[:, 77::D] = 0.0
     _check_prompts(_run_prompts(gpu, q, k, v, lens, H, HKV), q, k, v, lens, H, HKV)
+
+
+PAGED_WIDE = [  # H, HKV, lens, kv_len, whole units, cut ones
+    (8, 2, [40, 70, 33], [300, 70, 700], False, True), (8, 1, [20], [4000], False, True),
+    (16, 8, [60] * 64, [200 + i % 20 for i in range(64)], True, False),
+]
+
+
+@pytest.mark.parametrize("H,HKV,lens,kv,whole,cut", PAGED_WIDE)
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_bad_values_beside_many_rows(gpu, H, HKV, lens, kv, whole, cut, bad):
+    """More than 32 rows of a KV head over shuffled pages, with a bad key row or value that only the last two rows of
+    each sequence see: the others keep their outputs, and a value's column alone is bad."""
+    kc, vc, table, rows_of = _pool(lens, kv, HKV, 32, 209)
+    rows, cu, G = sum(lens), _cu(lens), H // HKV
+    q = torch.randn((rows, H * D), generator=torch.Generator(device="cuda").manual_seed(210), device="cuda")
+    b, clean = _paged(gpu, q, kc, vc, table, 32, lens, kv, H, HKV)
+    head, _, wide, _, _ = _read_plan(b, lens, rows, H, HKV)
+    assert not whole or head[6] > 0
+    assert not cut or (wide[:, 4] > 0).any()
+    _check_paged(clean, q, kc, vc, rows_of, lens, kv, H)
+    at = torch.stack([rows_of[s][kv[s] - 2] for s in range(len(lens))])
+    sees = torch.zeros(rows, dtype=torch.bool, device="cuda")
+    for s in range(len(lens)):
+        sees[int(cu[s + 1]) - 2:int(cu[s + 1])] = True
+    k2, v2 = kc.clone(), vc.clone()
+    k2[at] = float("nan")
+    _, out = _paged(gpu, q, k2, vc, table, 32, lens, kv, H, HKV)
+    assert torch.isnan(out[sees]).all()
+    assert rel_err(out[~sees].cpu().numpy(), clean[~sees].cpu().numpy()) <= ATTN_RTOL
+    v2[at, 0, 37] = bad
+    _, out = _paged(gpu, q, kc, v2, table, 32, lens, kv, H, HKV)
+    hit = torch.zeros_like(clean, dtype=torch.bool)
+    hit[:, :G, 37] = sees[:, None]
+    assert torch.equal(torch.isnan(out) if bad != bad else out == bad, hit)
+    assert rel_err(torch.where(hit, clean, out).cpu().numpy(), clean.cpu().numpy()) <= ATTN_RTOL
+
+
+@pytest.mark.parametrize("H,HKV,lens,kv,whole,cut", PAGED_WIDE)
+def test_large_value_of_a_light_key_over_pages(gpu, H, HKV, lens, kv, whole, cut):
+    """A value row 2^30 times the others at a key of weight e^-22.6: its part of the outputs and theirs.
+
+    Scores of up to 33 + 6 in log2 units are rounded by up to 2^-19 in each of 127 additions, a weight by that times
+    ln 2 of itself, an output by twice as much of the largest ordinary value, and of the light key's part.  (Planes of
+    V scaled to the large row would be off by 2^-25 of 2^-13 of it, 2^-6.)"""
+    kc, vc, table, rows_of = _pool(lens, kv, HKV, 32, 211)
+    q = torch.randn((sum(lens), H * D), generator=torch.Generator(device="cuda").manual_seed(212), device="cuda")
+    q[:, ::D] = 32.0
+    kc[:, :, 0] = 8.0
+    for s in range(len(lens)):
+        kc[rows_of[s][7], :, 0] = 0.0
+        vc[rows_of[s][7]] *= 2.0 ** 30
+    _, out = _paged(gpu, q, kc, vc, table, 32, lens, kv, H, HKV)
+    for s, (a, n) in enumerate(zip(_cu(lens), lens)):
+        r = slice(int(a), int(a) + n)
+        k64, v64 = kc[rows_of[s]].double(), vc[rows_of[s]].double()
+        ref = _attend64(q[r].double().view(n, H, D), k64, v64, kv[s])
+        v64[7] = 0.0
+        most = v64.abs().max() + (ref - _attend64(q[r].double().view(n, H, D), k64, v64, kv[s])).abs().max()
+        assert (out[r] - ref).abs().max() <= 2 * 127 * 2.0 ** -19 * np.log(2) * most, s
