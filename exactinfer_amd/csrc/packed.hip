@@ -357,23 +357,25 @@ __device__ __forceinline__ int row_owner(const int4* seq, int n_seq, int b, int 
 // ------------------------------------------------------------------ attention
 // Wide units multiply on v_mfma_f32_32x32x16_f16 with every fp32 operand in two binary16 planes, x = h + l:
 // h = f16(x) and l = f16(x - h), after a scaling by a power of two that brings the largest of its fellows
-// to 2^13 .. 2^15: the residual is exact, and l keeps it to 2^-22 of x (2^-24.6 in the root mean square)
+// to 2^14 .. 2^16: the residual is exact, and l keeps it to 2^-22 of x (2^-24.6 in the root mean square)
 // or to 2^-25, 2^-39 of the largest, whichever is more.  Three of the four plane products are taken; l.l
 // is at most 2^-22 of |a||b|, 2^-23.6 in the root mean square.  Together that is about what fp32 loses in
 // adding 128 products, for half the matrix instructions of three bf16 planes (prefill.hip), which keep
 // every bit.  The scalings:
 //   q, with the softmax scale in it: per row, taken back in the exponent's FMA
 //   K: per key, taken back in the scores (16 products per tile and lane), before q's
-// What q's planes and K's lose at their lower end, 2^-39 of the row's largest, is at most 2^-31 of the product of the two
-// largest in a score, which shows where that product is large and the score is not (a channel of q far above the
-// others that meets zeros, and one of K).  So a key's planes go up to the exponent at which its largest value times the
-// unit's largest q is 2^13, and beyond that they overflow, which is noticed (2^-18 of a log2 unit is left; products of
-// trained models are some 2^10 at most); and up to kMostK, where the sum of 128 products of up to 2^32 is finite
-// with K's scaling taken out: one that went to -infinity on the way would leave no trace.
 //   V: per 32 columns, the running largest value of the tiles so far; sums are rescaled when it grows
-//   P: 2^14, so that weights of up to 2^kLazy fit (of one below 2^-39 nothing is left, at most that times
-//     the number of keys in all); the weights' sum has it too
-// What the scaling of V cannot hold is noticed at the end of a pass (planes_failed) and multiplied in fp32.
+//   P: 2^14 against the row's reference, so that weights of up to 2^kLazy fit; the weights' sum has it too.  The
+//     reference is the running maximum until a tile's largest score lies more than kWindow below it; then it
+//     goes down after the tile.  (Behind a key that takes nearly all of the weight, 2^-39 of it, the planes' end, would
+//     be 2^-13 of an ordinary weight.)  What its planes may still be off by is counted, 32 times 2^-25 a tile.
+// What the planes of q and K lose at their lower end, 2^-39 of a row's largest value, is at most 2^-31 of the product of
+// the two largest in a score, which shows where that product is large and the score is not (a channel of q far
+// above the others that meets zeros, and one of K).  So a key's planes go up to the exponent at which its largest
+// value times the unit's largest q is 2^13 (2^-18 of a log2 unit is left), and what is larger overflows, which is
+// noticed; and up to kMostK, where the sum of 128 products of up to 2^32 is finite with K's scaling taken out: one that
+// went to -infinity on the way would leave no trace.
+// What the scalings of V and P cannot hold is noticed at the end of a pass (planes_failed) and multiplied in fp32.
 //
 // What bounds it is the power of the matrix instructions: 8192, 4096, 2048, 1024, 300 and 17 rows (H 32 / HKV 8)
 // take 2236 to 2315 us, 316 to 327 TFLOP/s, with the matrix unit busy 46% of the time at 1.9 GHz.  With two products
@@ -406,6 +408,12 @@ constexpr int kWaves = kSlots * kGroups;
 // lazy-rescale thresholds (log2 units): sums are rescaled when the running maximum has risen by more (for
 // wide units, what a weight may pass 1 by comes off the range of its planes)
 constexpr float kLazy = 1.f, kFewLazy = 8.f;
+// Wide units' reference goes down where a tile's scores are all more than kWindow below it, to kWindow / 2 above them,
+// as long as the sums stay below 2^kTopSum.  So a tile's largest weight is 2^2 or more, with its 2^14, and what its
+// weights may be off by, 2^-20, shows only where their values are small too.  8192 rows (H 32 / HKV 8), scores of
+// standard deviation 4: 1793 us (at 8 1843, never going down 1686); of 1: 1703 (1702, 1690).
+constexpr float kWindow = 12.f;
+constexpr int kTopSum = 64;
 // the largest (biased) exponents of a query's planes, of a key's, and of both together
 constexpr uint32_t kMostQ = 127 + 121, kMostK = 127 + 100, kMostQK = 2 * 127 + 10;
 constexpr float kPBits = 14.f;                  // wide units' weights and sums are times 2^kPBits
@@ -417,11 +425,11 @@ constexpr int kKRowB = 2 * kHeadDim + 16, kKPlane = kKT * kKRowB;  // K plane: [
 constexpr int kVRowB = 2 * kKT + 16, kVPlane = kHeadDim * kVRowB;  // V plane, transposed: [128 d][32 keys]
 // LDS of a wide pass: the K planes of both groups, and the merge's exchange area, from 0; the V planes
 // after it, and over them the staging area of the unit's rows (queries, later outputs); then the scalings,
-// of K [group][tile parity][key] and of V [group][32 columns], and each wave's largest q.  Of a few-rows pass: every wave's rows, and
-// their (m, l).
+// of K [group][tile parity][key] and of V [group][32 columns], each wave's largest q, each lane's Before.  Of a
+// few-rows pass: every wave's rows, and their (m, l).
 constexpr int kStageF = kWaves * kXchF * 64;
 constexpr int kScaleK = kStageF + kUnitRows * kRowF, kScaleV = kScaleK + kGroups * 2 * kKT;
-constexpr int kMaxQ = kScaleV + kGroups * 4, kWideF = kMaxQ + kWaves;
+constexpr int kMaxQ = kScaleV + kGroups * 4, kBefore = kMaxQ + kWaves, kWideF = kBefore + 3 * kWaves * 64;
 constexpr int kFewBlock = 16;                   // rows of one matrix instruction of few_pass
 constexpr int kFewML = kWaves * kFewRows * kRowF;
 constexpr int kFewF = kFewML + kWaves * kFewRows * 2;
@@ -491,7 +499,7 @@ __device__ __forceinline__ size_t part_at(bool few, int block, int slot) {
     return (size_t)(2 * block + slot) * (few ? kFewPart : kWidePart);
 }
 
-struct Sums {  // of 32 rows, one per lane and its lane ^ 32: O^T, running maximum (log2 units), sum of weights
+struct Sums {  // of 32 rows, one per lane and its lane ^ 32: O^T, their reference (log2 units), sum of weights
     floatx16 o[4];
     float m, l;
     __device__ __forceinline__ void clear() {
@@ -504,9 +512,25 @@ struct Sums {  // of 32 rows, one per lane and its lane ^ 32: O^T, running maxim
     }
 };
 
-// Scores s of tile kt (times sq: log2 units) -> 2^kPBits P (in place), the running maximum and sum, O rescaled
-// if the maximum rose by more than kLazy.  Tiles from nfull on cross the diagonal of the wave's rows.
-__device__ __forceinline__ void softmax_tile(Sums& x, floatx16& s, float sq, int kt, int nfull, int qpos, int hh) {
+// What a row's sums leave behind where its reference goes down, kept in LDS, a float per lane of each: the weights' sum
+// (small weights added to a sum that one key has nearly all of would be lost), the tiles summed so far, each counted as
+// one of the reference it was summed against (or of a higher one), and the reference that both are in.
+struct Before {
+    float* at;
+    int from;    // the tile at which a reference of the wave went down last
+    float rest;  // of sums in fp32 alone, whose reference never does: what rounding has kept from the weights' sum
+};
+constexpr int kTiles = kWaves * 64, kRef = 2 * kWaves * 64;
+__device__ __forceinline__ float moved(float from, float to) {  // a sum's factor for another reference
+    return from == to ? 1.f : __builtin_amdgcn_exp2f(from - to);
+}
+
+// Scores s of tile kt (times sq: log2 units) -> 2^kPBits P (in place) and its sum; O rescaled if the reference moves:
+// to the tile's maximum, if that is higher by more than kLazy, and with planes down towards it (kWindow).  Tiles from
+// nfull on cross the diagonal of the wave's rows.  The wave's i-th tile.
+template <bool kPlanes>
+__device__ __forceinline__ void softmax_tile(Sums& x, floatx16& s, float sq, int kt, int nfull, int qpos, int hh,
+                                             Before& before, int i) {
     if (kt >= nfull) {
         const int k0 = unhoisted(kt * kKT + 4 * hh);
 #pragma unroll
@@ -517,21 +541,46 @@ __device__ __forceinline__ void softmax_tile(Sums& x, floatx16& s, float sq, int
 #pragma unroll
     for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
     const float ms = half_max(mx) * sq;
-    if (__builtin_amdgcn_ballot_w64(ms > x.m + kLazy)) {  // rare after the first tile
-        const float mn = fmaxf(x.m, ms);
-        const float corr = x.m == mn ? 1.f : __builtin_amdgcn_exp2f(x.m - mn);
-        x.l *= corr;
+    const bool out = kPlanes ? __builtin_fabsf(ms - x.m + 0.5f * (kWindow - kLazy)) > 0.5f * (kWindow + kLazy)
+                             : ms > x.m + kLazy;
+    if (__builtin_amdgcn_ballot_w64(out)) {  // rare after the first tile
+        float mn = fmaxf(x.m, ms);
+        const bool down = kPlanes && ms < x.m - kWindow && ms > -INFINITY;
+        if (kPlanes && __builtin_amdgcn_ballot_w64(down)) {
+            const float by = moved(before.at[kRef], x.m);
+            const float sum = __builtin_fmaf(before.at[0], by, x.l);
+            const float tiles = __builtin_fmaf(before.at[kTiles], by, (float)(i - before.from));
+            const int room = max(127 + kTopSum - (int)(__float_as_uint(half_max(sum)) >> 23), 0);
+            if (down) mn = fmaxf(ms + 0.5f * kWindow, x.m - (float)room);
+            const float now = moved(x.m, mn);
+            before.at[0] = sum * now, before.at[kTiles] = tiles * now, before.at[kRef] = mn;
+            before.from = i;
+            x.l = 0.f;
+        }
+        if (!kPlanes || __builtin_amdgcn_ballot_w64(x.m != mn)) {  // (not for rows that see nothing of the tile)
+            const float corr = moved(x.m, mn);
+            x.l *= corr;
+            if constexpr (!kPlanes) before.rest *= corr;
 #pragma unroll
-        for (int db = 0; db < 4; ++db)
+            for (int db = 0; db < 4; ++db)
 #pragma unroll
-            for (int r = 0; r < 16; ++r) x.o[db][r] *= corr;
-        x.m = mn;
+                for (int r = 0; r < 16; ++r) x.o[db][r] *= corr;
+            x.m = mn;
+        }
     }
     const float nb = x.m == -INFINITY ? 0.f : kPBits - x.m;
+    float sum = 0.f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
         s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sq, nb));
-        x.l += s[r];
+        sum += s[r];
+    }
+    if constexpr (kPlanes) {
+        x.l += sum;
+    } else {
+        const float l = x.l + sum;
+        before.rest += sum > x.l ? x.l - (l - sum) : sum - (l - x.l);
+        x.l = l;
     }
 }
 
@@ -576,11 +625,24 @@ __device__ __forceinline__ Halves split_p(const floatx16& s, int x) {
     return {u32x4{h[0], h[1], h[2], h[3]}, u32x4{l[0], l[1], l[2], l[3]}};
 }
 
-// Takes V's scalings out of the sums, and says whether the planes did not serve them: a sum is not finite (an
-// infinite value or NaN in K or V, seen by the row or not), or a row's sums are so small, against V's
-// largest values on the way and the sum of weights, that the 2^-25 which planes keep of scaled values may
-// show (2^-22 of the row's largest sum).
-__device__ __forceinline__ bool planes_failed(Sums& x, const uint32_t (&scale)[4]) {
+// Takes V's scalings out of the sums, and says whether the planes did not serve them:
+//   - a sum is not finite (an infinite value or NaN in K or V, seen by the row or not, or q and K out of range);
+//   - a row's sums are so small, against V's largest values on the way and the sum of weights, that the 2^-25 which
+//     planes keep of scaled values of V may show (2^-22 of the row's largest sum);
+//   - or so small that the 2^-25 which they keep of scaled weights may: 32 weights a tile, times values of up to 2^16
+//     as scaled, together 2^-17 of the row's largest sum (`tiles`: see Before).
+__device__ __forceinline__ bool planes_failed(Sums& x, const uint32_t (&scale)[4], float tiles) {
+    float l = half_sum(x.l);
+    if (__builtin_amdgcn_ballot_w64(l > 0x1p40f)) {  // the reference went far down: up again, by a power of two
+        const uint32_t e = l > 0x1p40f ? min(__float_as_uint(l) >> 23, 254u) : 127u + 14u;
+        const float by = __uint_as_float((127u + 127u + 14u - e) << 23);
+        l *= by, x.l *= by, tiles *= by;
+        x.m += (float)((int)e - (127 + 14));
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) x.o[db][r] *= by;
+    }
     float z = x.l * 0.f, most = 0.f, step = 0.f;
 #pragma unroll
     for (int db = 0; db < 4; ++db) {
@@ -593,8 +655,9 @@ __device__ __forceinline__ bool planes_failed(Sums& x, const uint32_t (&scale)[4
             most = fmaxf(most, __builtin_fabsf(x.o[db][r]));
         }
     }
-    const float l = half_sum(x.l);
-    return __builtin_amdgcn_ballot_w64(z != 0.f || l * step * 0x1p-25f > half_max(most) * 0x1p-22f) != 0;
+    most = half_max(most);
+    const bool small = l * step * 0x1p-25f > most * 0x1p-22f || (l > 0.f && tiles * step * 0x1p-4f > most * 0x1p-17f);
+    return __builtin_amdgcn_ballot_w64(z != 0.f || small) != 0;
 }
 
 // A wave's tiles again, both products in fp32 from the cache.  In a tile that crosses the diagonal a
@@ -614,6 +677,7 @@ __device__ __forceinline__ void redo_fp32(Sums& x, const PackedArgs& a, const Pa
         q[4 * t] = v.x * sl2, q[4 * t + 1] = v.y * sl2, q[4 * t + 2] = v.z * sl2, q[4 * t + 3] = v.w * sl2;
     }
     x.clear();
+    Before before{};
     for (int i = 0; i < n_mine; ++i) {
         const int kt = index(i);
         floatx16 s;
@@ -633,7 +697,7 @@ __device__ __forceinline__ void redo_fp32(Sums& x, const PackedArgs& a, const Pa
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        softmax_tile(x, s, 1.f, kt, nfull, qpos, hh);
+        softmax_tile<false>(x, s, 1.f, kt, nfull, qpos, hh, before, i);
         const Rsrc rs = v_tile(i);
         if (kt < nfull) {
             const uint32_t off = unhoisted(4 * hh) * row_bytes + 4u * col;
@@ -674,6 +738,7 @@ __device__ __forceinline__ void redo_fp32(Sums& x, const PackedArgs& a, const Pa
         }
         __builtin_amdgcn_wave_barrier();
     }
+    x.l += before.rest;
 }
 
 // ---- a wide unit
@@ -736,7 +801,7 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
         return most;
     };
     // half x of the conversion of rg, eight values, one 16-byte piece of each plane; the first half finds the
-    // scaling: of K the row's, of V the running one of the wave's 32 columns (four times its largest value
+    // scaling: of K the row's, of V the running one of the wave's 32 columns (twice its largest value
     // fits, so it changes rarely)
     float fk;
     uint32_t k_limit;
@@ -764,7 +829,7 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
         if (x == 0) {
             const float most = largest();
             if (__builtin_amdgcn_ballot_w64(most > limit)) {
-                fv = scalar(scale_to<13>(wave_max(most)));
+                fv = scalar(scale_to<14>(wave_max(most)));
                 limit = uniform(65000.f * inverse(fv));
             }
             if (lane == 0) v_scale[hw] = fv;
@@ -854,6 +919,9 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
     Sums x;
     x.clear();
     uint32_t scale[4] = {kNoScale, kNoScale, kNoScale, kNoScale};  // V's, as the sums have it
+    Before before{smem + kBefore + tid, 0, 0.f};
+    before.at[0] = before.at[kTiles] = 0.f;
+    before.at[kRef] = -INFINITY;
     lds_barrier();  // every wave has its q (the staging area is free for the V planes); K planes stored
     if (grp == 1) lds_barrier();
     for (int i = 0; i < n_it; ++i) {
@@ -892,7 +960,7 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
                     scale[db] = now;
                 }
             }
-            softmax_tile(x, s, sq, index(i), nfull, qpos, hh);
+            softmax_tile<true>(x, s, sq, index(i), nfull, qpos, hh, before, i);
             // O^T += V^T . P^T, while K(i+1) goes to its planes; then V(i+1) is fetched
             const bool more = i + 1 < n_mine;
             Halves vf[2], pp;
@@ -912,7 +980,9 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
     }
     if (grp == 0) lds_barrier();
 
-    if (planes_failed(x, scale) && live) {
+    const float by = moved(before.at[kRef], x.m);
+    x.l = __builtin_fmaf(before.at[0], by, x.l);
+    if (planes_failed(x, scale, __builtin_fmaf(before.at[kTiles], by, (float)(n_mine - before.from))) && live) {
         const int f = min(f0 + col, p.nflat - 1), t0 = fdiv(f, fG);
         const float* q_row = a.q + ((size_t)p.row0 + t0) * a.q_stride + (size_t)(kvh * G + f - t0 * G) * D;
         redo_fp32(
@@ -937,7 +1007,7 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
     lds_barrier();
     const float* xp = smem + ((1 - grp) * kSlots + hw) * (kXchF * 64) + lane;
     const float mp = xp[0], lp = xp[64];
-    const float mt = fmaxf(x.m, mp);  // -inf only when the pass holds no visible key for the row
+    const float mt = fmaxf(x.m, mp);  // (references) -inf only when the pass holds no visible key for the row
     const float c0 = x.m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(x.m - mt);
     const float cp = mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mp - mt);
     const float l = half_sum(x.l * c0 + lp * cp);
@@ -1146,11 +1216,13 @@ __device__ __forceinline__ void few_pass(const PackedArgs& a, const Pass& p, int
                 m[rb] = mn;
             }
             const float nb = m[rb] == -INFINITY ? 0.f : -m[rb];
+            float sum = 0.f;  // (the tile's first: small weights would be lost one by one beside a large one)
 #pragma unroll
             for (int r = 0; r < 8; ++r) {
                 s[rb][r >> 2][r & 3] = __builtin_amdgcn_exp2f(s[rb][r >> 2][r & 3] + nb);
-                l[rb] += s[rb][r >> 2][r & 3];
+                sum += s[rb][r >> 2][r & 3];
             }
+            l[rb] += sum;
         }
         const uint32_t off_v = v_offset();
         pg = page(i + 2);
@@ -1429,17 +1501,22 @@ __global__ __launch_bounds__(32 * kCombineRows) void k_packed_combine(PackedArgs
             for (int k = 0; k < kAtOnce; ++k) mn = fmaxf(mn, ml[k].x);
             const float c = M == mn ? 1.f : __builtin_amdgcn_exp2f(M - mn);
             M = mn;
-            L *= c, o.x *= c, o.y *= c, o.z *= c, o.w *= c;
+            // (these parts' sum first: fewer roundings of a long unit's)
+            float l = 0.f;
+            float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int k = 0; k < kAtOnce; ++k) {
                 // (past the end the last part was read again: no row then, since zero times an infinite one is NaN)
                 const bool none = (p + k > m.end) | ((ml[k].x == -INFINITY) & (ml[k].y == 0.f));
                 const float wv = none ? 0.f : __builtin_amdgcn_exp2f(ml[k].x - M);
                 const float4 x = none ? make_float4(0.f, 0.f, 0.f, 0.f) : v[k];
-                L = __builtin_fmaf(wv, ml[k].y, L);
-                o.x = __builtin_fmaf(wv, x.x, o.x), o.y = __builtin_fmaf(wv, x.y, o.y);
-                o.z = __builtin_fmaf(wv, x.z, o.z), o.w = __builtin_fmaf(wv, x.w, o.w);
+                l = __builtin_fmaf(wv, ml[k].y, l);
+                sum.x = __builtin_fmaf(wv, x.x, sum.x), sum.y = __builtin_fmaf(wv, x.y, sum.y);
+                sum.z = __builtin_fmaf(wv, x.z, sum.z), sum.w = __builtin_fmaf(wv, x.w, sum.w);
             }
+            L = __builtin_fmaf(L, c, l);
+            o.x = __builtin_fmaf(o.x, c, sum.x), o.y = __builtin_fmaf(o.y, c, sum.y);
+            o.z = __builtin_fmaf(o.z, c, sum.z), o.w = __builtin_fmaf(o.w, c, sum.w);
         }
         const int t0 = f / G;
         const float inv = m.x.len - m.x.n + t0 < 0 ? 0.f : 1.f / L;  // a row that sees no key: zeros

@@ -87,13 +87,19 @@ size_t ei_packed_ws_bytes(int rows, int n_head, int n_head_kv);
  * buffer are fine; kv_stride at most 2^22.  out [rows][n_head][128], which must not overlap the inputs.
  * The plan must be one of whole prompts (kv_len NULL).
  *
- * Arithmetic of this call and the two below: fp32 sums of products whose operands keep 22 bits of 24
- * (two binary16 planes), or of fp32 products for the last few rows of a sequence (single tokens, drafts);
- * softmax in fp32.  Outputs differ from ei_attn_prefill's and ei_attn_decode's in the last bits, and with
- * the batch a sequence is in; a batch called twice gives the same bits.  Key and value rows that a
- * row does not see never reach it, whatever they hold.  Infinite or NaN values in K or V, or a V whose
- * largest values are 2^16 times a row's outputs, make the waves that meet them take their keys again in
- * fp32, some ten times slower. */
+ * Arithmetic of this call and the two below: sums and softmax in fp32, and for the last few rows of a
+ * sequence (single tokens, drafts) the products too.  Other rows' are made of two binary16 planes per
+ * operand, which keep 22 bits of 24 (the product of two low planes is left out, another 2^-22 at most), and
+ *   V        to 2^-39 of the largest value in its 32 columns (0 .. 31, ...) at the keys before and beside it: a
+ *            column far below those keeps fewer bits, at 2^-20 of them 17 to 19;
+ *   q and K  so that a score is off by 2^-18 of a log2 unit at most;
+ *   weights  so that an output is off by 2^-17 of the row's largest at most.
+ * Where more is lost, the waves that notice it take their keys again in fp32, three to ten times slower:
+ * V's largest values 2^17 times a row's outputs; weights that are nearly all at keys without a value; the
+ * largest q of some neighbouring rows times the largest K of a key, times scale, above 2^12; infinite or NaN
+ * values in K or V.  Outputs differ from ei_attn_prefill's, which keeps all 24 bits, and ei_attn_decode's in
+ * the last bits, and with the batch a sequence is in; a batch called twice gives the same bits.  Key and
+ * value rows that a row does not see never reach it, whatever they hold. */
 int ei_attn_packed(ei_stream_t stream, const float* q, long q_stride, const float* k, const float* v,
                    long kv_stride, float* out, int n_seq, int rows, int n_head, int n_head_kv, int head_dim,
                    float scale, const void* plan, size_t plan_bytes, void* ws, size_t ws_bytes);

@@ -5,7 +5,8 @@ import pytest
 import torch
 
 from tests.parity import ATTN_RTOL, rel_err
-from tests.test_gpu_packed import D, SCALE, _attend64, _check_prompts, _cu, _i32, _pool, _prompts, _read_plan, _run_prompts
+from tests.test_gpu_packed import (D, SCALE, _attend64, _check_prompts, _cu, _i32, _pool, _prompts, _read_plan,
+                                   _run_prompts)
 
 pytestmark = pytest.mark.gpu
 
@@ -16,12 +17,12 @@ def _paged(gpu, q, kc, vc, table, bs, lens, kv, H, HKV, scale=None):
     return b, gpu.attn_packed_paged(q, kc, vc, table, bs, b, gpu.AttnShape(H, HKV), scale=scale)
 
 
-def _check_paged(out, q, kc, vc, rows_of, lens, kv, H, scale=SCALE):
+def _check_paged(out, q, kc, vc, rows_of, lens, kv, H, scale=SCALE, tol=ATTN_RTOL):
     for s, (a, n) in enumerate(zip(_cu(lens), lens)):
         r = slice(int(a), int(a) + n)
         ref = _attend64(q[r].double().view(n, H, D), kc[rows_of[s]].double(), vc[rows_of[s]].double(), kv[s], scale)
         e = rel_err(out[r].cpu().numpy(), ref.cpu().numpy())
-        assert e <= ATTN_RTOL, (s, e)
+        assert e <= tol, (s, e)
 
 
 @pytest.mark.parametrize("H,HKV,n", [(8, 1, 16), (32, 8, 64), (8, 1, 1), (16, 8, 1), (32, 8, 5)])
@@ -57,6 +58,86 @@ def test_tiny_queries_of_huge_keys(gpu, H, HKV, lens, e, signs):
         k[1:], k[0] = 0.0, k[0] * 0.25
     q, k, v = (q * 2.0 ** e).contiguous(), (k * 2.0 ** -e).contiguous(), v.contiguous()
     _check_prompts(_run_prompts(gpu, q, k, v, lens, H, HKV), q, k, v, lens, H, HKV)
+
+
+def _sink_batch(gpu, T, n_seq, seed):
+    """n_seq sequences of 16 new rows over the same T keys, zero but for channel 0, with values about 1: one sequence of
+    a single KV head, cut into parts, or 32 of eight heads, in whole units.
+
+    In a whole unit each of two accumulators is rounded twice in each of six matrix instructions per 64 keys, by at
+    most 2^-24 of the sum so far, half of the last one on the average.  Equal weights round alike: 12 T / 64 * 2^-25
+    on top of the bar (whose signs are random)."""
+    H, HKV, n = (8, 1, 16) if n_seq == 1 else (64, 8, 16)
+    tol = ATTN_RTOL + (0 if n_seq == 1 else 12 * T / 64 * 2.0 ** -25)
+    kc, vc, table, rows_of = _pool([n], [T], HKV, 64, seed)
+    r = rows_of[0]
+    kc[r] = 0.0
+    vc[r] = vc[r] * 0.25 + 1.0
+    q = torch.randn((n * n_seq, H * D), generator=torch.Generator(device="cuda").manual_seed(seed + 1), device="cuda")
+    q[:, ::D] = 8.0
+
+    def run():
+        b, out = _paged(gpu, q, kc, vc, table.repeat(n_seq, 1), 64, [n] * n_seq, [T] * n_seq, H, HKV, scale=0.125)
+        head, _, wide, _, _ = _read_plan(b, [n] * n_seq, n * n_seq, H, HKV)
+        assert head[6] == 1 if n_seq > 1 else T < 200 or (wide[:, 4] > 0).any()
+        for s in (0, n_seq - 1):
+            _check_paged(out[n * s:n * s + n], q[n * s:n * s + n], kc, vc, rows_of, [n], [T], H, 0.125, tol)
+
+    return kc, vc, r, n, run
+
+
+@pytest.mark.parametrize("T", [64, 200, 2000, 8000, 30000])
+@pytest.mark.parametrize("nats", [8.0, 12.0, 15.0, 16.3, 17.0, 17.7, 18.0, 20.0])
+@pytest.mark.parametrize("sinks", ["first", "every tile"])
+@pytest.mark.parametrize("n_seq", [1, 32])
+def test_dominant_keys_with_no_value(gpu, T, nats, sinks, n_seq):
+    """Keys that take nearly all of the weight and have a value of zero: the output is what the many equal small
+    weights of the others give, so an error that they share does not average out.
+
+    The scores are 8 * nats / 8 at the sinks and 0 elsewhere, each off by some 4 * 2^-24 of itself at most, up to 29
+    in log2 units: weights by 29 * 2^-22 * ln 2 = 4.8e-6, all by the same."""
+    kc, vc, r, n, run = _sink_batch(gpu, T, n_seq, 204)
+    at = r[:1] if sinks == "first" else r[torch.arange(0, T - n + 1, 32, device="cuda")]
+    kc[at, :, 0] = nats
+    vc[at] = 0.0
+    run()
+
+
+@pytest.mark.parametrize("H,HKV,n", [(8, 8, 1), (32, 8, 1), (32, 8, 5), (32, 8, 8)])
+@pytest.mark.parametrize("T", [3000, 30000])
+@pytest.mark.parametrize("nats", [8.0, 12.0, 15.0, 18.0])
+def test_dominant_key_before_few_rows(gpu, H, HKV, n, T, nats):
+    """The same for single tokens and drafts of 64 sequences over one sequence's keys.
+
+    A wave's accumulators are rounded in each of eight matrix instructions per 256 keys, by at most 2^-24 of the sum so
+    far, half of the last one on the average, and equal weights round alike: T / 32 * 2^-25 on top of the bar."""
+    kc, vc, table, rows_of = _pool([n], [T], HKV, 64, 215)
+    r = rows_of[0]
+    kc[r] = 0.0
+    vc[r] = vc[r] * 0.25 + 1.0
+    kc[r[0], :, 0] = nats
+    vc[r[0]] = 0.0
+    q = torch.randn((n * 64, H * D), generator=torch.Generator(device="cuda").manual_seed(216), device="cuda")
+    q[:, ::D] = 8.0
+    _, out = _paged(gpu, q, kc, vc, table.repeat(64, 1), 64, [n] * 64, [T] * 64, H, HKV, scale=0.125)
+    for s in (0, 31, 63):
+        rows = slice(n * s, n * s + n)
+        _check_paged(out[rows], q[rows], kc, vc, rows_of, [n], [T], H, 0.125, ATTN_RTOL + T / 32 * 2.0 ** -25)
+
+
+@pytest.mark.parametrize("up", [False, True])
+@pytest.mark.parametrize("step", [1.0, 3.0])
+@pytest.mark.parametrize("n_seq", [1, 32])
+def test_scores_that_fall_or_rise_over_the_tiles(gpu, up, step, n_seq):
+    """Scores that fall or rise by `step` a tile, most of the weight without a value: the sums follow in both
+    directions.  (Scores of at most 24: as above.)"""
+    T = int(24 / step) * 32
+    kc, vc, r, n, run = _sink_batch(gpu, T, n_seq, 206)
+    level = torch.arange(T, device="cuda") // 32
+    level = level if up else T // 32 - 1 - level
+    kc[r, :, 0] = level[:, None].float() * step
+    vc[r[level >= T // 64]] = 0.0
+    run()
 
 
 @pytest.mark.parametrize("H,HKV,lens", [(8, 1, [200]), (16, 8, [90, 300])])
