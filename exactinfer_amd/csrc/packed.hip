@@ -525,7 +525,7 @@ __device__ __forceinline__ float moved(float from, float to) {  // a sum's facto
     return from == to ? 1.f : __builtin_amdgcn_exp2f(from - to);
 }
 
-// Scores s of tile kt (times sq: log2 units) -> 2^kPBits P (in place) and its sum; O rescaled if the reference moves:
+// Scores s of tile kt (times sq: log2 units) -> P (in place; with planes times 2^kPBits) and its sum; O rescaled if the reference moves:
 // to the tile's maximum, if that is higher by more than kLazy, and with planes down towards it (kWindow).  Tiles from
 // nfull on cross the diagonal of the wave's rows.  The wave's i-th tile.
 template <bool kPlanes>
@@ -568,7 +568,7 @@ __device__ __forceinline__ void softmax_tile(Sums& x, floatx16& s, float sq, int
             x.m = mn;
         }
     }
-    const float nb = x.m == -INFINITY ? 0.f : kPBits - x.m;
+    const float nb = x.m == -INFINITY ? 0.f : (kPlanes ? kPBits : 0.f) - x.m;
     float sum = 0.f;
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
@@ -625,19 +625,22 @@ __device__ __forceinline__ Halves split_p(const floatx16& s, int x) {
     return {u32x4{h[0], h[1], h[2], h[3]}, u32x4{l[0], l[1], l[2], l[3]}};
 }
 
-// Takes V's scalings out of the sums, and says whether the planes did not serve them:
+// Takes V's scalings and P's 2^kPBits out of the sums, and says whether the planes did not serve them:
 //   - a sum is not finite (an infinite value or NaN in K or V, seen by the row or not, or q and K out of range);
 //   - a row's sums are so small, against V's largest values on the way and the sum of weights, that the 2^-25 which
 //     planes keep of scaled values of V may show (2^-22 of the row's largest sum);
 //   - or so small that the 2^-25 which they keep of scaled weights may: 32 weights a tile, times values of up to 2^16
 //     as scaled, together 2^-17 of the row's largest sum (`tiles`: see Before).
 __device__ __forceinline__ bool planes_failed(Sums& x, const uint32_t (&scale)[4], float tiles) {
+    constexpr float kOne = 0x1p-14f;
+    static_assert(kPBits == 14.f, "kOne is its inverse");
+    x.l *= kOne, tiles *= kOne;
     float l = half_sum(x.l);
-    if (__builtin_amdgcn_ballot_w64(l > 0x1p40f)) {  // the reference went far down: up again, by a power of two
-        const uint32_t e = l > 0x1p40f ? min(__float_as_uint(l) >> 23, 254u) : 127u + 14u;
-        const float by = __uint_as_float((127u + 127u + 14u - e) << 23);
+    if (__builtin_amdgcn_ballot_w64(l > 0x1p26f)) {  // the reference went far down: up again, by a power of two
+        const uint32_t e = l > 0x1p26f ? min(__float_as_uint(l) >> 23, 253u) : 127u;
+        const float by = __uint_as_float((127u + 127u - e) << 23);
         l *= by, x.l *= by, tiles *= by;
-        x.m += (float)((int)e - (127 + 14));
+        x.m += (float)((int)e - 127);
 #pragma unroll
         for (int db = 0; db < 4; ++db)
 #pragma unroll
@@ -651,7 +654,7 @@ __device__ __forceinline__ bool planes_failed(Sums& x, const uint32_t (&scale)[4
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             z = __builtin_fmaf(x.o[db][r], 0.f, z);
-            x.o[db][r] *= inv;
+            x.o[db][r] *= inv * kOne;
             most = fmaxf(most, __builtin_fabsf(x.o[db][r]));
         }
     }

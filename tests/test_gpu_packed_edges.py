@@ -210,3 +210,14 @@ def test_large_value_of_a_light_key_over_pages(gpu, H, HKV, lens, kv, whole, cut
         v64[7] = 0.0
         most = v64.abs().max() + (ref - _attend64(q[r].double().view(n, H, D), k64, v64, kv[s])).abs().max()
         assert (out[r] - ref).abs().max() <= 2 * 127 * 2.0 ** -19 * np.log(2) * most, s
+
+
+@pytest.mark.parametrize("H,HKV,lens", [(16, 8, [100, 7, 300]), (8, 1, [60, 700]), (32, 8, [4, 8, 1])])
+@pytest.mark.parametrize("e", [104, 110, 118])
+def test_values_near_the_end_of_fp32(gpu, H, HKV, lens, e):
+    """Values of up to 2^(e + 2): so are the outputs, and the sums on the way to them at most some tens of times that."""
+    _, q, k, v = (t.contiguous() for t in _prompts(H, HKV, lens, 217))
+    v *= 2.0 ** e
+    _check_prompts(_run_prompts(gpu, q, k, v, lens, H, HKV), q, k, v, lens, H, HKV)
+    v[::5] *= 2.0 ** -60  # (rows that see such values alone have the fp32 products)
+    _check_prompts(_run_prompts(gpu, q, k, v, lens, H, HKV), q, k, v, lens, H, HKV)
