@@ -405,7 +405,7 @@ class PackedBatch:
     def plan(self, cu_rows: torch.Tensor, rows: int, max_kv: int, kv_len: torch.Tensor | None = None) -> None:
         """cu_rows int32 [n_seq + 1]: sequence s owns rows cu_rows[s] .. cu_rows[s+1] - 1, of `rows` in
         all (later ones belong to nobody).  kv_len int32 [n_seq], each at most max_kv: keys after the
-        new rows are appended; None: whole prompts."""
+        new rows are appended; None: whole prompts, of at most max_kv rows each."""
         self._check_device()
         _need_contiguous("cu_rows", cu_rows, torch.int32)
         n_seq = cu_rows.numel() - 1

@@ -54,11 +54,11 @@ struct List {
     Share* shares;  // one per workgroup of a KV head
 };
 struct PlanView {
-    int4* seq;     // first row, rows, keys, wide units before this sequence's
+    int4* seq;     // first row, rows, keys (kv_len itself, also past max_kv), wide units before this sequence's
     List wide, few;
 };
-// header words past the shape: rounds of the deal, units dealt, on the wide line, few-row units
-enum { kHeadRounds = 6, kHeadDealt = 7, kHeadLine = 8, kHeadFew = 9 };
+// header words past the shape: rounds of the deal, units dealt, on the wide line, few-row units, max_kv
+enum { kHeadRounds = 6, kHeadDealt = 7, kHeadLine = 8, kHeadFew = 9, kHeadMaxKv = 10 };
 constexpr size_t kPlanSeqAt = 256;
 __host__ __device__ inline long plan_max_wide(int n_seq, int rows, int G) { return (long)rows * G / kUnitRows + n_seq; }
 __host__ __device__ inline size_t plan_wide_at(int n_seq) { return kPlanSeqAt + (size_t)n_seq * sizeof(int4); }
@@ -167,13 +167,14 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
     int bad = 0;
     for (int base = 0; base < n_seq; base += kPlanThreads) {
         const int s = base + tid;
-        int lo = 0, n = 0, len = 0;
+        int lo = 0, n = 0, len = 0, all_keys = 0;
         if (s < n_seq) {
             lo = cu[s];
             const int hi = cu[s + 1];
             bad |= lo < 0 || hi < lo || hi > rows;
             n = hi - lo;
-            len = kv_len ? min(max(kv_len[s], 0), max_kv) : min(n, max_kv);
+            all_keys = kv_len ? max(kv_len[s], 0) : n;
+            len = min(all_keys, max_kv);
         }
         bad = __syncthreads_or(bad);
         if (bad) n = 0;  // rows outside the batch: no call on this plan does anything
@@ -182,9 +183,9 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
         long long all;
         const long long at = block_scan((long long)nw << 32 | is_few, &all);  // (both sums stay below 2^31)
         if (s < n_seq) {
-            const int4 e = make_int4(lo, n, len, (int)(units + (at >> 32)));
-            pv.seq[s] = e;
-            if (s < kPlanSeqLds) seq_lds[s] = e;
+            const int first = (int)(units + (at >> 32));
+            pv.seq[s] = make_int4(lo, n, all_keys, first);
+            if (s < kPlanSeqLds) seq_lds[s] = make_int4(lo, n, len, first);
         }
         if (is_few) {
             const int i = (int)(few + (at & 0xFFFFFFFF));
@@ -201,7 +202,12 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
     const int U = (int)units;
     __syncthreads();
     const bool in_lds = n_seq <= kPlanSeqLds;
-    auto seq_at = [&](int s) { return in_lds ? seq_lds[s] : pv.seq[s]; };
+    auto seq_at = [&](int s) {
+        if (in_lds) return seq_lds[s];
+        int4 e = pv.seq[s];
+        e.z = min(e.z, max_kv);
+        return e;
+    };
     auto unit = [&](int i) {
         int lo = 0, hi = n_seq - 1;
         while (lo < hi) {  // the last sequence whose first unit is not past i
@@ -329,6 +335,7 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
         h[1] = n_seq, h[2] = rows, h[3] = H, h[4] = HKV;
         h[5] = kv_len == nullptr;
         h[kHeadRounds] = rounds, h[kHeadDealt] = dealt, h[kHeadLine] = U - dealt, h[kHeadFew] = (int)few;
+        h[kHeadMaxKv] = max_kv;
     }
 }
 
@@ -1569,7 +1576,7 @@ __global__ __launch_bounds__(256) void k_packed_prepare(const float* __restrict_
     if (s < 0) return;
     const int4 e = seq[s];
     const int pos = e.z - e.y + (b - e.x);
-    const bool in = pos >= 0 && pos < n_pos;
+    const bool in = pos >= 0 && pos < min(n_pos, reinterpret_cast<const int*>(a.plan)[kHeadMaxKv]);
     const int blk = pos >> a.bshift;
     const int phys = in && blk < a.max_blocks ? a.btab[(size_t)s * a.max_blocks + blk] : -1;
     const bool there = phys >= 0 && phys < a.n_blocks;

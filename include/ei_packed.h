@@ -68,7 +68,10 @@ int ei_rope_rows(ei_stream_t stream, const float* x, long x_stride, float* y, lo
  * made once for a batch, it serves every layer, on any stream that the plan's launch comes before.
  * kv_len (device int32 [n_seq]): keys of sequence s after its new rows are appended, so that its
  * row i of n sees keys 0 .. kv_len[s] - n + i; a row that sees none (kv_len[s] < n) gets zeros.
- * kv_len NULL: whole prompts, kv_len[s] = n.  Lengths are taken as lying in [0, max_kv], max_kv <= 2^30.
+ * kv_len NULL: whole prompts, kv_len[s] = n.  max_kv (<= 2^30) must be at least the longest length, prompts'
+ * own lengths too: attention takes a longer sequence as one of max_kv keys, whose rows see as many keys fewer
+ * as it is longer (and the first rows of a prompt none), and the step appends nothing at positions from
+ * max_kv on.  Lengths below 0 count as 0.
  * A call of the entry points below whose n_seq, rows, heads differ from the plan's writes nothing, and so
  * does one on a plan whose cu_rows count more rows than `rows`.
  * The plan of n_seq sequences and `rows` rows takes ei_packed_plan_bytes(n_seq, rows, ...) bytes (0
@@ -119,8 +122,8 @@ int ei_attn_packed_paged(ei_stream_t stream, const float* q, long q_stride, floa
  * Row i of n of sequence s stands at position kv_len[s] - n + i: its Q and K heads are normed and
  * turned there (half layout, full or partial rope_dim, table cs of n_pos positions; as
  * ei_qkv_prepare), K and V appended to the sequence's pool row, then attention as
- * ei_attn_packed_paged.  A row at a position < 0, >= n_pos or past its sequence's pages appends
- * nothing, and its query is neither normed nor turned.  Blocks that are written must belong to one
+ * ei_attn_packed_paged.  A row at a position < 0, >= n_pos, >= the plan's max_kv or past its sequence's pages
+ * appends nothing; at a position < 0, >= n_pos or >= max_kv its query is neither normed nor turned.  Blocks that are written must belong to one
  * sequence alone. */
 int ei_packed_step_paged(ei_stream_t stream, const float* qkv, long row_stride, float* out, float* kc, float* vc,
                          int n_blocks, const int* block_table, int max_blocks, int block_size, int n_seq, int rows,

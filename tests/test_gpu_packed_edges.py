@@ -5,8 +5,8 @@ import pytest
 import torch
 
 from tests.parity import ATTN_RTOL, rel_err
-from tests.test_gpu_packed import (D, SCALE, _attend64, _check_prompts, _cu, _i32, _pool, _prompts, _read_plan,
-                                   _run_prompts)
+from tests.test_gpu_packed import (D, SCALE, _attend64, _check_prompts, _cu, _i32, _norm_rope64, _pool, _prompts,
+                                   _read_plan, _run_prompts)
 
 pytestmark = pytest.mark.gpu
 
@@ -221,3 +221,45 @@ def test_values_near_the_end_of_fp32(gpu, H, HKV, lens, e):
     _check_prompts(_run_prompts(gpu, q, k, v, lens, H, HKV), q, k, v, lens, H, HKV)
     v[::5] *= 2.0 ** -60  # (rows that see such values alone have the fp32 products)
     _check_prompts(_run_prompts(gpu, q, k, v, lens, H, HKV), q, k, v, lens, H, HKV)
+
+
+@pytest.mark.parametrize("H,HKV,bs,lens,kv,max_kv", [
+    (16, 8, 32, [1, 3, 40, 2], [51, 52, 90, 40], 50), (8, 1, 64, [30], [140], 128),
+    (32, 8, 32, [2, 2], [2 ** 31 - 1, 64], 64), (8, 8, 32, [1] * 1100, [33 + i % 40 for i in range(1100)], 64),
+])
+def test_step_past_max_kv_leaves_the_pool(gpu, H, HKV, bs, lens, kv, max_kv):
+    """Sequences longer than the plan's max_kv: rows at positions from max_kv on append nothing, rows below it stand
+    where kv_len puts them, other sequences are as ever."""
+    real = [min(t, 200) for t in kv]  # (pages for all of a sequence's rows: nothing else keeps them from the pool)
+    kc, vc, table, rows_of = _pool(lens, real, HKV, bs, 213)
+    shape = gpu.AttnShape(H, HKV)
+    rows, cu = sum(lens), _cu(lens)
+    g = torch.Generator(device="cuda").manual_seed(214)
+    qkv = torch.randn((rows, shape.qkv), generator=g, device="cuda")
+    one = torch.ones(D, device="cuda")
+    cs = gpu.rope_table_scaled(256)
+    b = gpu.PackedBatch(len(lens), rows, H, HKV)
+    b.plan(_i32(cu), rows, max_kv, kv_len=_i32(kv))
+    k0, v0 = kc.clone(), vc.clone()
+    out = gpu.packed_step_paged(qkv, kc, vc, table, bs, b, shape, one, one, cs)
+    x = qkv.double().view(rows, H + 2 * HKV, D)
+    written = torch.zeros(kc.shape[0], dtype=torch.bool, device="cuda")
+    for s, n in enumerate(lens):
+        pos = torch.arange(kv[s] - n, kv[s])
+        keep = pos[pos < max_kv].cuda()
+        if len(keep) == 0:
+            continue
+        new = rows_of[s][keep]
+        written[new] = True
+        r = slice(int(cu[s]), int(cu[s]) + len(keep))
+        assert torch.equal(vc[new], qkv[r].view(len(keep), -1, D)[:, H + HKV:]), s
+        want = _norm_rope64(x[r, H:H + HKV], one, keep, D)
+        assert (kc[new].double() - want).abs().max() <= 8.2 * 2 ** -24 * 16, s
+    assert torch.equal(kc[~written], k0[~written]) and torch.equal(vc[~written], v0[~written])
+    for s, n in enumerate(lens):
+        if kv[s] <= max_kv and s < 40:
+            r = slice(int(cu[s]), int(cu[s + 1]))
+            q64 = _norm_rope64(x[r, :H], one, torch.arange(kv[s] - n, kv[s], device="cuda"), D)
+            ref = _attend64(q64, kc[rows_of[s]].double(), vc[rows_of[s]].double(), kv[s])
+            assert rel_err(out[r].cpu().numpy(), ref.cpu().numpy()) <= ATTN_RTOL, s
+    assert torch.isfinite(out).all()
