@@ -412,6 +412,8 @@ class PackedBatch:
         if not 1 <= n_seq <= self.max_seq or not 0 <= rows <= self.max_rows:
             raise ValueError(f"batch of {n_seq} sequences and {rows} rows: made for 1 to {self.max_seq} sequences and "
                              f"up to {self.max_rows} rows")
+        if not 0 <= max_kv <= 1 << 30:  # (ctypes would cut it to 32 bits)
+            raise ValueError(f"max_kv {max_kv} out of range [0, 2^30]")
         if kv_len is not None:
             _need_contiguous("kv_len", kv_len, torch.int32)
             if kv_len.numel() != n_seq:

@@ -263,3 +263,11 @@ def test_step_past_max_kv_leaves_the_pool(gpu, H, HKV, bs, lens, kv, max_kv):
             ref = _attend64(q64, kc[rows_of[s]].double(), vc[rows_of[s]].double(), kv[s])
             assert rel_err(out[r].cpu().numpy(), ref.cpu().numpy()) <= ATTN_RTOL, s
     assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("max_kv", [-1, 2 ** 30 + 1, 2 ** 32 + 8, -2 ** 32 + 8])
+def test_max_kv_out_of_range_is_refused(gpu, max_kv):
+    """Also where its lowest 32 bits are a length."""
+    b = gpu.PackedBatch(1, 8, 16, 8)
+    with pytest.raises(ValueError, match="max_kv"):
+        b.plan(_i32([0, 8]), 8, max_kv, kv_len=_i32([8]))
