@@ -630,6 +630,15 @@ bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
 size_t span_bytes(int rows, long stride, long width) {
     return rows > 0 ? ((size_t)(rows - 1) * (size_t)stride + (size_t)width) * sizeof(float) : 0;
 }
+// whether the rows of two matrices share a byte; rows of one stride may lie between each other's
+bool rows_overlap(const float* a, long a_stride, const float* b, long b_stride, int rows, long width) {
+    if (!overlap(a, span_bytes(rows, a_stride, width), b, span_bytes(rows, b_stride, width))) return false;
+    if (a_stride != b_stride) return true;
+    const uintptr_t stride = (uintptr_t)a_stride * sizeof(float), w = (uintptr_t)width * sizeof(float);
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    const uintptr_t behind = x < y ? (y - x) % stride : (stride - (x - y) % stride) % stride;
+    return behind < w || behind > stride - w;
+}
 
 constexpr int kMaxPackedSeqs = 65535;
 
@@ -738,8 +747,7 @@ EI_API int ei_rope_rows(ei_stream_t stream, const float* x, long x_stride, float
     REQUIRE(x_stride >= width && y_stride >= width && x_stride % 4 == 0 && y_stride % 4 == 0,
             "strides %ld / %ld must be multiples of 4 and >= n_heads*head_dim", x_stride, y_stride);
     REQUIRE(aligned16(x) && aligned16(y) && aligned16(cs) && aligned16(gamma), "pointers must be 16-byte aligned");
-    REQUIRE((x == y && x_stride == y_stride) ||
-                !overlap(x, span_bytes(rows, x_stride, width), y, span_bytes(rows, y_stride, width)),
+    REQUIRE((x == y && x_stride == y_stride) || !rows_overlap(x, x_stride, y, y_stride, rows, width),
             "y overlaps x without being x");
     if (rows == 0) return ok();
     return hip_status(ei::launch_rope_rows(static_cast<hipStream_t>(stream), x, x_stride, y, y_stride, rows, n_heads,
