@@ -705,7 +705,7 @@ EI_API int ei_rope_table_scaled(ei_stream_t stream, float* cs, int n_pos, int ro
     if (kind == EI_ROPE_NTK) theta *= std::pow(s, double(rope_dim) / (rope_dim - 2));
     ei::RopeFrequencies fr{};
     fr.m = 1.0;
-    double lo = 0.0, width = 1.0;
+    double lo = 0.0, width = 1.0, slow = 1.0;
     if (kind == EI_ROPE_YARN) {
         REQUIRE(scaling->n_trained > 0, "n_trained %d must be positive", scaling->n_trained);
         REQUIRE(scaling->beta_slow > 0.0 && scaling->beta_fast >= scaling->beta_slow &&
@@ -717,7 +717,8 @@ EI_API int ei_rope_table_scaled(ei_stream_t stream, float* cs, int n_pos, int ro
             return rope_dim * std::log(scaling->n_trained / (turns * 6.283185307179586)) / (2.0 * std::log(theta));
         };
         lo = std::fmax(std::floor(pair(scaling->beta_fast)), 0.0);
-        const double hi = std::fmin(std::ceil(pair(scaling->beta_slow)), rope_dim - 1.0);
+        slow = pair(scaling->beta_slow);
+        const double hi = std::fmin(std::ceil(slow), rope_dim - 1.0);
         width = std::fmax(hi - lo, 1e-3);
         REQUIRE(std::isfinite(scaling->attn_factor), "attn_factor must be finite");
         fr.m = scaling->attn_factor > 0.0 ? scaling->attn_factor : 0.1 * std::log(s) + 1.0;
@@ -726,7 +727,8 @@ EI_API int ei_rope_table_scaled(ei_stream_t stream, float* cs, int n_pos, int ro
         const double f = std::pow(theta, -2.0 * i / rope_dim);
         if (kind == EI_ROPE_LINEAR) fr.f[i] = f / s;
         else if (kind == EI_ROPE_YARN) {
-            const double ramp = std::fmin(std::fmax((i - lo) / width, 0.0), 1.0);
+            // (slow <= 0: the fastest pair makes beta_slow turns at most, where the ramp would begin with it at 0)
+            const double ramp = slow <= 0.0 ? 1.0 : std::fmin(std::fmax((i - lo) / width, 0.0), 1.0);
             fr.f[i] = f / s * ramp + f * (1.0 - ramp);
         } else fr.f[i] = f;
     }

@@ -1,4 +1,5 @@
 """GPU tests of rotary positions (include/ei_packed.h) at the edges of their arguments."""
+import numpy as np
 import pytest
 import torch
 
@@ -26,3 +27,12 @@ def test_rows_side_by_side_in_one_buffer(gpu):
         a, b = (buf.as_strided((rows - 1, H * D), buf.stride(), at) for at in (x, y))
         with pytest.raises(RuntimeError, match="overlaps"):
             gpu.rope_rows(a, H, cs, pos[1:], out=b)
+
+
+@pytest.mark.parametrize("n_trained,beta_slow", [(4, 1.0), (6, 1.0), (100, 16.0)])
+def test_yarn_where_no_pair_is_fast(gpu, n_trained, beta_slow):
+    """Every pair makes at most beta_slow turns over the trained positions: all of them are slowed by factor."""
+    yarn = gpu.RopeScaling("yarn", 4.0, n_trained, 32.0, beta_slow, 1.0)
+    assert n_trained / (2 * np.pi) <= beta_slow
+    assert torch.equal(gpu.rope_table_scaled(300, scaling=yarn),
+                       gpu.rope_table_scaled(300, scaling=gpu.RopeScaling("linear", 4.0)))
