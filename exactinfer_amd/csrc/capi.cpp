@@ -751,6 +751,11 @@ EI_API int ei_rope_rows(ei_stream_t stream, const float* x, long x_stride, float
     REQUIRE(aligned16(x) && aligned16(y) && aligned16(cs) && aligned16(gamma), "pointers must be 16-byte aligned");
     REQUIRE((x == y && x_stride == y_stride) || !rows_overlap(x, x_stride, y, y_stride, rows, width),
             "y overlaps x without being x");
+    const size_t yb = span_bytes(rows, y_stride, width);
+    REQUIRE(!overlap(y, yb, cs, (size_t)n_pos * rope_dim * sizeof(float)) &&
+                !overlap(y, yb, pos, (size_t)rows * sizeof(int)) &&
+                !(gamma && overlap(y, yb, gamma, (size_t)head_dim * sizeof(float))),
+            "y overlaps cs, pos or gamma");
     if (rows == 0) return ok();
     return hip_status(ei::launch_rope_rows(static_cast<hipStream_t>(stream), x, x_stride, y, y_stride, rows, n_heads,
                                            gamma, eps, cs, n_pos, pos, rope_dim, layout == EI_ROPE_HALF),

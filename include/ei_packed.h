@@ -51,8 +51,9 @@ int ei_rope_table_scaled(ei_stream_t stream, float* cs, int n_pos, int rope_dim,
 
 /* Turns n_heads heads of `rows` rows, each row at its own position pos[b] (device int32 [rows]):
  * head h of row b at x + b*x_stride + h*128, written to y + b*y_stride + h*128.  y may be x with the
- * same stride (in place), or other columns of one buffer; any overlap of their rows is refused.  gamma (128 values, or NULL): each head is
- * RMS-normed first, as in ei_headnorm_rope.  Pairs of the first rope_dim elements:
+ * same stride (in place), or other columns of one buffer; any overlap of their rows is refused, and y over
+ * cs, pos or gamma.  gamma (128 values, or NULL): each head is RMS-normed first, as in ei_headnorm_rope.
+ * Pairs of the first rope_dim elements:
  *   EI_ROPE_HALF         (i, i + rope_dim/2)
  *   EI_ROPE_INTERLEAVED  (2i, 2i + 1)
  * elements from rope_dim on are only normed.  y columns past the heads are not written.  A row whose

@@ -243,3 +243,13 @@ def test_paged_arguments(match, kw):
 ])
 def test_step_arguments(match, kw):
     _refused(match, "ei_packed_step_paged", *_step(**kw))
+
+
+@pytest.mark.parametrize("kw", [
+    dict(cs=_off(FAR[1], 8 * 4096 - 4)), dict(cs=ctypes.c_void_p(FAR[1].value - 64 * 128 * 4 + 16)),
+    dict(pos=_off(FAR[1], 4096)), dict(pos=ctypes.c_void_p(FAR[1].value - 8 * 4 + 4)),
+    dict(gamma=_off(FAR[1], 512)), dict(y=FAR[0], gamma=_off(FAR[0], 128)), dict(y=FAR[0], cs=FAR[0]),
+])
+def test_rope_rows_over_its_own_tables(kw):
+    """Rows that would be written over the table, the positions or gamma, which other rows still read."""
+    _refused("overlaps cs, pos or gamma", "ei_rope_rows", *_rope(**kw))
