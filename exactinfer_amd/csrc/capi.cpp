@@ -668,9 +668,10 @@ int check_packed(int n_seq, int rows, int n_head, int n_head_kv, int head_dim, c
     return EI_OK;
 }
 
-// The pools, and that what the call writes does not lie in them.
+// The pools and the block table, and that what the call writes does not lie in them.
 int check_pool(const float* kc, const float* vc, int n_blocks, const int* block_table, int max_blocks, int block_size,
-               int n_head_kv, const float* out, size_t out_bytes, const void* ws, size_t ws_bytes, int* shift) {
+               int n_seq, int n_head_kv, const float* out, size_t out_bytes, const void* ws, size_t ws_bytes,
+               int* shift) {
     REQUIRE(kc && vc && block_table, "null pointer argument");
     REQUIRE(aligned16(kc) && aligned16(vc), "pointers must be 16-byte aligned");
     REQUIRE(block_size >= 32 && (block_size & (block_size - 1)) == 0,
@@ -682,6 +683,9 @@ int check_pool(const float* kc, const float* vc, int n_blocks, const int* block_
     for (const float* c : {kc, vc})
         REQUIRE(!overlap(c, pool, out, out_bytes) && !overlap(c, pool, ws, ws_bytes),
                 "out or workspace lies in a pool of %zu bytes", pool);
+    const size_t table = (size_t)n_seq * max_blocks * sizeof(int);
+    REQUIRE(!overlap(out, out_bytes, block_table, table) && !overlap(ws, ws_bytes, block_table, table),
+            "out or workspace overlaps the block table");
     int s = 0;
     while ((1 << s) < block_size) ++s;
     *shift = s;
@@ -781,6 +785,9 @@ EI_API int ei_packed_plan(ei_stream_t stream, const int* cu_rows, const int* kv_
     const size_t need = ei::packed_plan_bytes(n_seq, rows, n_head, n_head_kv);
     REQUIRE(plan && aligned16(plan) && plan_bytes >= need,
             "plan missing, not 16-byte aligned or %zu B < %zu B (ei_packed_plan_bytes)", plan_bytes, need);
+    REQUIRE(!overlap(plan, need, cu_rows, (size_t)(n_seq + 1) * sizeof(int)) &&
+                !(kv_len && overlap(plan, need, kv_len, (size_t)n_seq * sizeof(int))),
+            "plan overlaps cu_rows or kv_len");
     return hip_status(ei::launch_packed_plan(static_cast<hipStream_t>(stream), cu_rows, kv_len, n_seq, rows, max_kv,
                                              n_head, n_head_kv, plan),
                       "packed plan launch");
@@ -818,7 +825,7 @@ EI_API int ei_attn_packed_paged(ei_stream_t stream, const float* q, long q_strid
     if (int e = check_packed(n_seq, rows, n_head, n_head_kv, head_dim, plan, plan_bytes, ws, ws_bytes, out)) return e;
     int shift = 0;
     const long qw = (long)n_head * head_dim;
-    if (int e = check_pool(kc, vc, n_blocks, block_table, max_blocks, block_size, n_head_kv, out,
+    if (int e = check_pool(kc, vc, n_blocks, block_table, max_blocks, block_size, n_seq, n_head_kv, out,
                            span_bytes(rows, qw, qw), ws, ei::packed_ws_bytes(rows, n_head, n_head_kv), &shift))
         return e;
     REQUIRE(q && aligned16(q), "q missing or not 16-byte aligned");
@@ -849,7 +856,7 @@ EI_API int ei_packed_step_paged(ei_stream_t stream, const float* qkv, long row_s
     if (int e = check_rope(rope_dim, head_dim)) return e;
     int shift = 0;
     const long w = (long)(n_head + 2 * n_head_kv) * head_dim, qw = (long)n_head * head_dim;
-    if (int e = check_pool(kc, vc, n_blocks, block_table, max_blocks, block_size, n_head_kv, out,
+    if (int e = check_pool(kc, vc, n_blocks, block_table, max_blocks, block_size, n_seq, n_head_kv, out,
                            span_bytes(rows, qw, qw), ws, ei::packed_ws_bytes(rows, n_head, n_head_kv), &shift))
         return e;
     REQUIRE(qkv && q_gamma && k_gamma && cs, "null pointer argument");
@@ -863,6 +870,20 @@ EI_API int ei_packed_step_paged(ei_stream_t stream, const float* qkv, long row_s
     const size_t pool = (size_t)n_blocks * block_size * n_head_kv * head_dim * sizeof(float);
     REQUIRE(!overlap(kc, pool, qkv, in) && !overlap(vc, pool, qkv, in), "qkv lies in a pool");
     REQUIRE(!overlap(kc, pool, vc, pool), "the K and V pools overlap");  // (both are written)
+    const size_t gamma = (size_t)head_dim * sizeof(float), wb = ei::packed_ws_bytes(rows, n_head, n_head_kv);
+    const struct {
+        const void* at;
+        size_t bytes;
+        const char* name;
+    } read[] = {{plan, ei::packed_plan_bytes(n_seq, rows, n_head, n_head_kv), "the plan"},
+                {block_table, (size_t)n_seq * max_blocks * sizeof(int), "the block table"},
+                {q_gamma, gamma, "q_gamma"},
+                {k_gamma, gamma, "k_gamma"},
+                {cs, (size_t)n_pos * rope_dim * sizeof(float), "cs"}};
+    for (const auto& r : read)
+        REQUIRE(!overlap(kc, pool, r.at, r.bytes) && !overlap(vc, pool, r.at, r.bytes) &&
+                    !overlap(out, span_bytes(rows, qw, qw), r.at, r.bytes) && !overlap(ws, wb, r.at, r.bytes),
+                "a pool, out or workspace overlaps %s", r.name);
     if (rows == 0) return ok();
     ei::PackedArgs a{};
     a.k = kc, a.v = vc, a.kv_stride = (long)n_head_kv * head_dim;

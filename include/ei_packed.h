@@ -10,6 +10,8 @@
  * cu_rows[s+1] - 1 (device int32 [n_seq + 1], from 0 up, never falling, cu_rows[n_seq] <= rows) belong
  * to sequence s, which may have none.  Rows from cu_rows[n_seq] on belong to nobody: nothing is
  * written there, and it does not matter what they hold.
+ *
+ * A call whose outputs, workspace, plan or (in the step) pools overlap anything that it reads is refused.
  */
 #ifndef EI_PACKED_H
 #define EI_PACKED_H

@@ -253,3 +253,26 @@ def test_step_arguments(match, kw):
 def test_rope_rows_over_its_own_tables(kw):
     """Rows that would be written over the table, the positions or gamma, which other rows still read."""
     _refused("overlaps cs, pos or gamma", "ei_rope_rows", *_rope(**kw))
+
+
+@pytest.mark.parametrize("cu,kv", [(_at(0), None), (_at(-16), None), (FAR[0], _at(256)), (FAR[0], _at(-12))])
+def test_plan_over_its_lengths(cu, kv):
+    """The plan is written while its workgroup reads them."""
+    _refused("plan overlaps", "ei_packed_plan", None, cu, kv, 4, 100, 100, 32, 8, P, BIG)
+
+
+@pytest.mark.parametrize("at", ["out", "ws"])
+def test_paged_table_that_the_call_writes(at):
+    for call, args in (("ei_attn_packed_paged", _paged), ("ei_packed_step_paged", _step)):
+        to = {"out": FAR[1], "ws": FAR[3]}[at]
+        _refused("overlaps the block table", call, *args(table=_off(to, 1024)))
+        _refused("overlaps the block table", call, *args(table=ctypes.c_void_p(to.value - 4 * 4 * 4 + 4)))
+
+
+@pytest.mark.parametrize("what", ["plan", "table", "qg", "kg", "cs"])
+@pytest.mark.parametrize("into", ["kc", "vc", "out", "ws"])
+def test_step_inputs_that_it_writes(what, into):
+    """What the step reads must not lie in the pools, the outputs or the workspace."""
+    to = dict(kc=FAR[4], vc=FAR[5], out=FAR[1], ws=FAR[3])[into]
+    _refused("overlap", "ei_packed_step_paged", *_step(**{what: _off(to, 4096)}))
+    _refused("overlap", "ei_packed_step_paged", *_step(**{what: ctypes.c_void_p(to.value - 16)}))
