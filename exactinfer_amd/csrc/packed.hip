@@ -17,14 +17,19 @@ constexpr int kFewRows = 32;    // a sequence's last unit of up to so many rows:
 // there are.  A sequence's last unit, if it has at most kFewRows rows (single tokens, drafts, tails of
 // prompts), goes to the list of few-row units, the others to the wide list.
 //
-// `shares` workgroups serve each KV head, all heads alike, and take the same cost each: a unit's causal key
-// tiles, and something for what is done once per unit.  Of the wide list each workgroup first takes whole
-// units, dealt out in descending order of tiles and back and forth, round by round, so that the
-// workgroups walk units of about the same keys at the same time (their tiles meet in the XCD's L2); the
-// rest (less than a round, or the last full one too, if some workgroup would have more than an equal share with
-// it) is laid end to end on a line, of which each gets what is missing to an equal share.  The few-row units
-// lie on a line of their own, of which each workgroup gets what its wide work leaves of an equal share of
-// everything.  A cut may fall inside a unit: its parts are merged by k_packed_combine.
+// `shares` workgroups serve each KV head, all heads alike.  A unit costs its causal key tiles, and something for what
+// is done once per unit.  Of the wide list each workgroup first takes whole units, dealt out in descending order of
+// tiles and back and forth, round by round, so that the workgroups walk units of about the same keys at the same
+// time (their tiles meet in the XCD's L2); the rest (less than a round, or the last full one too, if some workgroup
+// would have more than an equal share of everything and 1/32 with it) is laid end to end on a line, of which each gets
+// what is missing to an equal share.  The few-row units lie on a line of their own, of which each workgroup gets
+// what its wide work leaves of an equal share of everything.  A cut may fall inside a unit: its parts are merged by
+// k_packed_combine.
+//
+// So the workgroups' shares are equal where the units are, and where there is less than a round of them (to within
+// what cuts are moved by); a unit of an earlier round is dealt whole, whatever it costs.  One chunk of 64 rows after 30000 keys among
+// 64 prompts of 32 rows (H 32 / HKV 8, 66 units for 32 workgroups) is 945 tiles for one workgroup of each head, against
+// an equal share of 72, and 1333 us; in a batch of its own, where it is cut, it takes 130, the prompts 34.
 //
 // Dealing the last full round, against leaving it on the line in any case (H 32, HKV 8): 8 prompts of 250
 // rows 42 us against 52, one of 2048 132 against 145, 1500 rows after 8000 keys 729 against 770, 1024 after
@@ -35,7 +40,9 @@ constexpr int kFewRows = 32;    // a sequence's last unit of up to so many rows:
 //
 // One workgroup, a thread per sequence, unit or cut, everything in LDS as long as it fits: its time is the
 // latency of a dozen steps that need each other, 8 us for 5 sequences, 10 for 6 of up to 8192 rows (490 wide
-// units), 6 to 8 in a graph; once per forward pass, not per layer.
+// units), 6 to 8 in a graph; once per forward pass, not per layer.  With many sequences it is the sorting, which looks
+// at every sequence for every unit (in a graph): 256 single tokens 6.5 us, 64 prompts of 32 rows 18, 256 of 64 rows
+// 48, 512 of 64 rows 169, the most there is (kMaxRankWork); beyond, unsorted, 1000 of 64 rows 17, 16000 tokens 85.
 struct Unit {
     int row0, n, len, u;    // the sequence's first row, rows and keys; the unit's number in it
     int seq, tiles, pad[2];
@@ -90,9 +97,9 @@ constexpr int kDealSlack = 32;          // whole units may pass an equal share b
 
 // What a list's work costs, in tiles: `pass` for everything done once per unit or part of one; a cut leaves
 // whole turns (the tiles that a workgroup's waves take at a time, a power of two; less where all the work there is
-// would not give each one) on both sides, and keeps off a unit's ends by what a pass costs, so that a share does not run one for a
-// few tiles.  Without the smaller turns one token at 2000 keys takes 20.3 us instead of 13.7, at 255 14.3 instead of
-// 11.0, a draft of 5 of H 32 after 1000 keys 21.4 instead of 15.5.
+// would not give each one) on both sides, and keeps off a unit's ends by what a pass costs, so that a share does not
+// run one for a few tiles.  Without the smaller turns one token at 2000 keys takes 20.3 us instead of 13.7, at 255
+// 14.3 instead of 11.0, a draft of 5 of H 32 after 1000 keys 21.4 instead of 15.5.
 struct ListCost {
     int pass, turn;
 };
@@ -376,18 +383,20 @@ __device__ __forceinline__ int row_owner(const int4* seq, int n_seq, int b, int 
 //     reference is the running maximum until a tile's largest score lies more than kWindow below it; then it
 //     goes down after the tile.  (Behind a key that takes nearly all of the weight, 2^-39 of it, the planes' end, would
 //     be 2^-13 of an ordinary weight.)  What its planes may still be off by is counted, 32 times 2^-25 a tile.
-// What the planes of q and K lose at their lower end, 2^-39 of a row's largest value, is at most 2^-31 of the product of
-// the two largest in a score, which shows where that product is large and the score is not (a channel of q far
+// What the planes of q and K lose at their lower end, 2^-39 of a row's largest value, is at most 2^-31 of the product
+// of the two largest in a score, which shows where that product is large and the score is not (a channel of q far
 // above the others that meets zeros, and one of K).  So a key's planes go up to the exponent at which its largest
 // value times the unit's largest q is 2^13 (2^-18 of a log2 unit is left), and what is larger overflows, which is
 // noticed; and up to kMostK, where the sum of 128 products of up to 2^32 is finite with K's scaling taken out: one that
 // went to -infinity on the way would leave no trace.
 // What the scalings of V and P cannot hold is noticed at the end of a pass (planes_failed) and multiplied in fp32.
 //
-// What bounds it is the power of the matrix instructions: 8192, 4096, 2048, 1024, 300 and 17 rows (H 32 / HKV 8)
-// take 2236 to 2315 us, 316 to 327 TFLOP/s, with the matrix unit busy 46% of the time at 1.9 GHz.  With two products
-// of three taken out 1530 us, with the loop's loads out 11% less, with the LDS reads out 3%; more fragments in flight,
-// other interleavings of the splits and no priorities all came within 3%.  Three bf16 planes: 3370 us.
+// What bounds it: matrix and vector instructions follow one another.  8192, 4096, 2048, 1024, 300 and 17 rows (H 32 /
+// HKV 8) take 2271 to 2334 us by box, 313 to 322 TFLOP/s, with the matrix unit busy 45% of the cycles and the other
+// vector instructions (splits, softmax, scalings; four cycles each) another 37%, at 1.87 GHz of 2.4 under this load.
+// With two products of three taken out 1530 us, with the loop's loads out 11% less, with the LDS reads out 3%; more
+// fragments in flight, other interleavings of the splits and no priorities all came within 3%.  Three bf16 planes:
+// 3370 us.
 //
 // A wave holds 32 flat query rows and computes S^T[key][row] = K . Q^T, so that each lane owns one row and
 // 16 of a tile's 32 keys, and O^T[d][row] = V^T . P^T from the same registers.
@@ -532,9 +541,9 @@ __device__ __forceinline__ float moved(float from, float to) {  // a sum's facto
     return from == to ? 1.f : __builtin_amdgcn_exp2f(from - to);
 }
 
-// Scores s of tile kt (times sq: log2 units) -> P (in place; with planes times 2^kPBits) and its sum; O rescaled if the reference moves:
-// to the tile's maximum, if that is higher by more than kLazy, and with planes down towards it (kWindow).  Tiles from
-// nfull on cross the diagonal of the wave's rows.  The wave's i-th tile.
+// Scores s of tile kt (times sq: log2 units) -> P (in place; with planes times 2^kPBits) and its sum; O rescaled if the
+// reference moves: to the tile's maximum, if that is higher by more than kLazy, and with planes down towards it
+// (kWindow).  Tiles from nfull on cross the diagonal of the wave's rows.  The wave's i-th tile.
 template <bool kPlanes>
 __device__ __forceinline__ void softmax_tile(Sums& x, floatx16& s, float sq, int kt, int nfull, int qpos, int hh,
                                              Before& before, int i) {
@@ -1067,7 +1076,7 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
 // the same of d for O, and the quarters' products (of d, of keys) are summed afterwards.
 //
 // Single tokens are bound by reading K and V: 24 sequences of 57000 keys in all (H 16 / HKV 8, pages of 64),
-// 494 MB in 88 us, 5.6 TB/s.  Where sequences share their keys and have more rows it is the matrix instructions
+// 494 MB in 87 to 91 us, 5.4 to 5.7 TB/s.  Where sequences share their keys and have more rows it is the matrix instructions
 // and what a pass does once: 16 drafts of 5 tokens after 1024 shared keys and up to 555 more (H 32 / HKV 8) 41 us.
 // By rows (H 32 / HKV 8, 32 sequences of 480 keys, with the merge): four 26.2 us (27.1 as sixteen), sixteen 27
 // (37 as 32), twenty 32.3 (35.5 as 32), 32 rows 36 (44 as a wide unit; of 4067 keys 192 against 297; single

@@ -100,7 +100,8 @@ size_t ei_packed_ws_bytes(int rows, int n_head, int n_head_kv);
  *            column far below those keeps fewer bits, at 2^-20 of them 17 to 19;
  *   q and K  so that a score is off by 2^-18 of a log2 unit at most;
  *   weights  so that an output is off by 2^-17 of the row's largest at most.
- * Where more is lost, the waves that notice it take their keys again in fp32, three to ten times slower:
+ * Where more is lost, the waves that notice it take their keys again in fp32, three to five times slower
+ * (bad values beside 17 to 32 flat rows of a KV head: up to fourteen times):
  * V's largest values 2^17 times a row's outputs; weights that are nearly all at keys without a value; the
  * largest q of some neighbouring rows times the largest K of a key, times scale, above 2^12; infinite or NaN
  * values in K or V.  Outputs differ from ei_attn_prefill's, which keeps all 24 bits, and ei_attn_decode's in
