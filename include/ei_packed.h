@@ -126,9 +126,9 @@ int ei_attn_packed_paged(ei_stream_t stream, const float* q, long q_stride, floa
  * Row i of n of sequence s stands at position kv_len[s] - n + i: its Q and K heads are normed and
  * turned there (half layout, full or partial rope_dim, table cs of n_pos positions; as
  * ei_qkv_prepare), K and V appended to the sequence's pool row, then attention as
- * ei_attn_packed_paged.  A row at a position < 0, >= n_pos, >= the plan's max_kv or past its sequence's pages
- * appends nothing; at a position < 0, >= n_pos or >= max_kv its query is neither normed nor turned.  Blocks that are written must belong to one
- * sequence alone. */
+ * ei_attn_packed_paged.  A row at a position < 0, >= n_pos, >= the plan's max_kv or past its sequence's
+ * pages appends nothing; at a position < 0, >= n_pos or >= max_kv its query is neither normed nor turned.
+ * Blocks that are written must belong to one sequence alone. */
 int ei_packed_step_paged(ei_stream_t stream, const float* qkv, long row_stride, float* out, float* kc, float* vc,
                          int n_blocks, const int* block_table, int max_blocks, int block_size, int n_seq, int rows,
                          int n_head, int n_head_kv, int head_dim, const float* q_gamma, const float* k_gamma,
