@@ -27,9 +27,10 @@ constexpr int kFewRows = 32;    // a sequence's last unit of up to so many rows:
 // k_packed_combine.
 //
 // So the workgroups' shares are equal where the units are, and where there is less than a round of them (to within
-// what cuts are moved by); a unit of an earlier round is dealt whole, whatever it costs.  One chunk of 64 rows after 30000 keys among
-// 64 prompts of 32 rows (H 32 / HKV 8, 66 units for 32 workgroups) is 945 tiles for one workgroup of each head, against
-// an equal share of 72, and 1333 us; in a batch of its own, where it is cut, it takes 130, the prompts 34.
+// what cuts are moved by); a unit of an earlier round is dealt whole, whatever it costs.  One chunk of 64 rows after
+// 30000 keys among 64 prompts of 32 rows (H 32 / HKV 8, 66 units for 32 workgroups) is 945 tiles for one workgroup of
+// each head, against an equal share of 72, and 1333 us; in a batch of its own, where it is cut, it takes 130, the
+// prompts 34.
 //
 // Dealing the last full round, against leaving it on the line in any case (H 32, HKV 8): 8 prompts of 250
 // rows 42 us against 52, one of 2048 132 against 145, 1500 rows after 8000 keys 729 against 770, 1024 after
@@ -1076,8 +1077,9 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
 // the same of d for O, and the quarters' products (of d, of keys) are summed afterwards.
 //
 // Single tokens are bound by reading K and V: 24 sequences of 57000 keys in all (H 16 / HKV 8, pages of 64),
-// 494 MB in 87 to 91 us, 5.4 to 5.7 TB/s.  Where sequences share their keys and have more rows it is the matrix instructions
-// and what a pass does once: 16 drafts of 5 tokens after 1024 shared keys and up to 555 more (H 32 / HKV 8) 41 us.
+// 494 MB in 87 to 91 us, 5.4 to 5.7 TB/s.  Where sequences share their keys and have more rows it is the matrix
+// instructions and what a pass does once: 16 drafts of 5 tokens after 1024 shared keys and up to 555 more (H 32 / HKV 8)
+// 41 us.
 // By rows (H 32 / HKV 8, 32 sequences of 480 keys, with the merge): four 26.2 us (27.1 as sixteen), sixteen 27
 // (37 as 32), twenty 32.3 (35.5 as 32), 32 rows 36 (44 as a wide unit; of 4067 keys 192 against 297; single
 // tokens as wide units 44, and of 4059 keys 290 against 179).
