@@ -26,6 +26,9 @@ EXPORTS = (
     # include/ei_packed.h
     "ei_rope_table_scaled", "ei_rope_rows", "ei_packed_plan_bytes", "ei_packed_plan", "ei_packed_ws_bytes",
     "ei_attn_packed", "ei_attn_packed_paged", "ei_packed_step_paged",
+    # include/ei_cache8.h
+    "ei_cache8_store", "ei_cache8_load", "ei_attn_packed_cache8", "ei_packed_step_cache8", "ei_attn_tree_paged",
+    "ei_tree_step_paged", "ei_cache_keep", "ei_cache8_keep",
     # include/ei_gguf.h
     "ei_gguf_open", "ei_gguf_close", "ei_gguf_version", "ei_gguf_n_tensors", "ei_gguf_tensor", "ei_gguf_find_tensor",
     "ei_gguf_get_int", "ei_gguf_get_float", "ei_gguf_get_str", "ei_gguf_qwen3_config",
@@ -73,6 +76,19 @@ _SIGS = {
                              _i),
     "ei_packed_step_paged": ([_vp, _vp, _l, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _i, _i,
                               _f, _f, _vp, _sz, _vp, _sz], _i),
+    "ei_cache8_store": ([_vp, _vp, _l, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _i, _vp, _i, _f, _vp, _sz],
+                        _i),
+    "ei_cache8_load": ([_vp, _vp, _vp, _i, _vp, _vp, _l, _i, _i, _i, _i, _i, _vp, _sz], _i),
+    "ei_attn_packed_cache8": ([_vp, _vp, _l, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _i, _f, _vp, _sz, _vp, _sz],
+                              _i),
+    "ei_packed_step_cache8": ([_vp, _vp, _l, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _i, _vp, _i, _f, _vp,
+                               _i, _f, _vp, _sz, _vp, _sz], _i),
+    "ei_attn_tree_paged": ([_vp, _vp, _l, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _i, _f, _vp, _sz,
+                            _vp, _sz], _i),
+    "ei_tree_step_paged": ([_vp, _vp, _l, _vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _vp, _vp, _i, _vp,
+                            _i, _f, _vp, _i, _f, _vp, _sz, _vp, _sz], _i),
+    "ei_cache_keep": ([_vp, _vp, _vp, _i, _vp, _i, _i, _i, _i, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _sz], _i),
+    "ei_cache8_keep": ([_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _vp, _i, _vp, _vp, _vp, _sz], _i),
     "ei_gguf_open": ([ctypes.c_char_p], _vp),
     "ei_gguf_close": ([_vp], None),
     "ei_gguf_version": ([_vp], _i),
@@ -93,6 +109,13 @@ class RopeScalingC(ctypes.Structure):
 
     _fields_ = [("kind", _i), ("factor", _d), ("n_trained", _i), ("beta_fast", _d), ("beta_slow", _d),
                 ("attn_factor", _d)]
+
+
+class Cache8C(ctypes.Structure):
+    """ei_cache8 of include/ei_cache8.h."""
+
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("kind", _i), ("n_blocks", _i),
+                ("block_size", _i)]
 
 
 _lib = None

@@ -524,6 +524,246 @@ def packed_step_paged(qkv: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor, blo
     return out
 
 
+# ---------------------------------------------------------------- 8-bit cache, trees of drafted tokens
+_CACHE_KINDS = {"e4m3": (1, torch.float8_e4m3fn), "int8": (2, torch.int8)}
+
+
+class Cache8:
+    """A paged pool of 8-bit keys and values (include/ei_cache8.h): codes k, v [n_blocks, HKV, block_size, 128]
+    (float8_e4m3fn or int8) and scales k_scale, v_scale [n_blocks, HKV, block_size]; a code stands for
+    code * scale.  Made empty (zeros), or of tensors that a program has already."""
+
+    def __init__(self, n_blocks: int, block_size: int, n_head_kv: int, kind: str = "e4m3", device="cuda"):
+        if kind not in _CACHE_KINDS:
+            raise ValueError(f"cache kind {kind!r}: one of {', '.join(_CACHE_KINDS)}")
+        shape = (n_blocks, n_head_kv, block_size)
+        codes = [torch.zeros((*shape, HEAD_DIM), dtype=torch.int8, device=device).view(_CACHE_KINDS[kind][1])
+                 for _ in range(2)]
+        self._take(*codes, *(torch.zeros(shape, dtype=torch.float32, device=device) for _ in range(2)))
+
+    @classmethod
+    def of(cls, k: torch.Tensor, v: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor) -> "Cache8":
+        cache = cls.__new__(cls)
+        cache._take(k, v, k_scale, v_scale)
+        return cache
+
+    def _take(self, k, v, k_scale, v_scale) -> None:
+        kinds = {dtype: (name, number) for name, (number, dtype) in _CACHE_KINDS.items()}
+        if k.dtype not in kinds:
+            raise ValueError(f"codes must be torch.float8_e4m3fn or torch.int8, got {k.dtype}")
+        if k.dim() != 4 or k.shape[-1] != HEAD_DIM:
+            raise ValueError(f"codes must be [blocks, KV heads, block size, {HEAD_DIM}], got {tuple(k.shape)}")
+        for name, t, shape, dtype in (("k", k, k.shape, k.dtype), ("v", v, k.shape, k.dtype),
+                                      ("k_scale", k_scale, k.shape[:3], torch.float32),
+                                      ("v_scale", v_scale, k.shape[:3], torch.float32)):
+            if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or t.device != k.device:
+                raise ValueError(f"{name} must be a contiguous {dtype} tensor {tuple(shape)} on {k.device}, got "
+                                 f"{t.dtype} {tuple(t.shape)} on {t.device}")
+        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self.kind, number = kinds[k.dtype]
+        self.n_blocks, self.n_head_kv, self.block_size = k.shape[:3]
+        import ctypes
+        self._c = _capi.Cache8C(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), number,
+                                self.n_blocks, self.block_size)
+        self._at = ctypes.addressof(self._c)
+
+
+def _cache8_args(cache: Cache8, block_table: torch.Tensor, batch: PackedBatch, n_head_kv: int) -> tuple:
+    if cache.n_head_kv != n_head_kv:
+        raise ValueError(f"the cache holds {cache.n_head_kv} KV heads, the call has {n_head_kv}")
+    if cache.k.get_device() != _device():
+        _refuse("the cache", cache.k, cache.k.dtype)
+    return cache._at, *_table_args(block_table, batch)
+
+
+def _table_args(block_table: torch.Tensor, batch: PackedBatch) -> tuple:
+    _need_contiguous("block_table", block_table, torch.int32)
+    if block_table.dim() != 2 or block_table.shape[0] < batch.n_seq:
+        raise ValueError(f"block_table must be [{batch.n_seq}, blocks], got {tuple(block_table.shape)}")
+    return block_table.data_ptr(), block_table.shape[1]
+
+
+def _need_cached(batch: PackedBatch) -> None:
+    """A batch that is not planned yet is refused, and one on another device."""
+    if batch.n_seq == 0:
+        raise ValueError("the batch has no plan yet: call plan() first")
+    batch._check_device()
+
+
+def _mask_args(mask: torch.Tensor | None, rows: int) -> tuple:
+    if mask is None:
+        return None, 0
+    _need_contiguous("mask", mask, torch.int64)
+    if mask.dim() != 2 or mask.shape[0] < rows or mask.shape[1] < 1:
+        raise ValueError(f"mask must be [{rows}, words], got {tuple(mask.shape)}")
+    return mask.data_ptr(), mask.shape[1]
+
+
+def _turn_args(cs: torch.Tensor, pos: torch.Tensor | None, shape: AttnShape, rows: int, q_gamma: torch.Tensor,
+               k_gamma: torch.Tensor) -> tuple:
+    """q_gamma, k_gamma, cs, n_pos, turn_at, rope_dim, eps."""
+    for name, t in (("q_gamma", q_gamma), ("k_gamma", k_gamma)):
+        if t is None:
+            raise ValueError(f"{name} is missing")
+        _need_gamma(name, t)
+    n_pos = _table_positions(cs, shape.rope_dim)
+    if pos is not None:
+        _need_contiguous("pos", pos, torch.int32)
+        if pos.numel() < rows:
+            raise ValueError(f"pos must hold {rows} positions, got {pos.numel()}")
+    return (q_gamma.data_ptr(), k_gamma.data_ptr(), cs.data_ptr(), n_pos, _ptr(pos), shape.rope_dim, float(shape.eps))
+
+
+def cache8_store(qkv: torch.Tensor, cache: Cache8, block_table: torch.Tensor, batch: PackedBatch, shape: AttnShape,
+                 q_gamma: torch.Tensor, k_gamma: torch.Tensor, cs: torch.Tensor, pos: torch.Tensor | None = None,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
+    """Norms, turns and quantises the batch's new rows from raw projections qkv [rows, >= (H+2HKV)*128] into their
+    sequences' pages, and returns the normed and turned queries [rows, H, 128] (ei_cache8_store).  pos
+    int32 [rows]: positions other than the rows' slots, as of a tree's tokens."""
+    batch._check(shape)
+    rs = _rows_of("qkv", qkv, batch.rows, shape.qkv)
+    where = _cache8_args(cache, block_table, batch, shape.n_head_kv)
+    turn = _turn_args(cs, pos, shape, batch.rows, q_gamma, k_gamma)
+    out = batch._out(out, qkv.device)
+    if batch.rows:
+        _capi.call("ei_cache8_store", _stream(), qkv.data_ptr(), rs, out.data_ptr(), *where, batch.n_seq, batch.rows,
+                   shape.n_head, shape.n_head_kv, shape.head_dim, *turn, batch.buf.data_ptr(), batch.nbytes)
+    return out
+
+
+def cache8_load(cache: Cache8, block_table: torch.Tensor, batch: PackedBatch,
+                out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The cached keys and values of the batch's new rows in 32 bits, [rows, HKV, 128] each (ei_cache8_load); a batch
+    planned with longer runs of rows reads more of the sequences.  out: two tensors of one row stride."""
+    _need_cached(batch)
+    where = _cache8_args(cache, block_table, batch, batch.n_head_kv)
+    width = cache.n_head_kv * HEAD_DIM
+    if out is None:
+        out = tuple(torch.empty((batch.rows, cache.n_head_kv, HEAD_DIM), dtype=torch.float32, device=cache.k.device)
+                    for _ in range(2))
+    k, v = out
+    ks, vs = _rows_of("out[0]", k, batch.rows, width), _rows_of("out[1]", v, batch.rows, width)
+    if ks != vs:
+        raise ValueError(f"the two outputs must share a row stride, got {ks} and {vs}")
+    if batch.rows:
+        _capi.call("ei_cache8_load", _stream(), *where, k.data_ptr(), v.data_ptr(), ks, batch.n_seq, batch.rows,
+                   batch.n_head, batch.n_head_kv, HEAD_DIM, batch.buf.data_ptr(), batch.nbytes)
+    return k, v
+
+
+def attn_packed_cache8(q: torch.Tensor, cache: Cache8, block_table: torch.Tensor, batch: PackedBatch, shape: AttnShape,
+                       mask: torch.Tensor | None = None, scale: float | None = None,
+                       out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of the batch's new rows, q [rows, >= H*128] normed and turned, over their sequences' pages of the
+    8-bit cache (ei_attn_packed_cache8): causal, or with mask (int64 [rows, words]) a row sees of the new rows
+    those whose bit is set in its words, up to itself.  Returns [rows, H, 128]."""
+    batch._check(shape)
+    qs = _rows_of("q", q, batch.rows, shape.n_head * HEAD_DIM)
+    where = _cache8_args(cache, block_table, batch, shape.n_head_kv)
+    bits = _mask_args(mask, batch.rows)
+    out = batch._out(out, q.device)
+    scale = default_scale() if scale is None else scale
+    if batch.rows:
+        _capi.call("ei_attn_packed_cache8", _stream(), q.data_ptr(), qs, out.data_ptr(), *where, batch.n_seq,
+                   batch.rows, shape.n_head, shape.n_head_kv, shape.head_dim, *bits, float(scale), *batch._tail())
+    return out
+
+
+def packed_step_cache8(qkv: torch.Tensor, cache: Cache8, block_table: torch.Tensor, batch: PackedBatch,
+                       shape: AttnShape, q_gamma: torch.Tensor, k_gamma: torch.Tensor, cs: torch.Tensor,
+                       pos: torch.Tensor | None = None, mask: torch.Tensor | None = None, scale: float | None = None,
+                       out: torch.Tensor | None = None) -> torch.Tensor:
+    """The whole step of a batch over the 8-bit cache: cache8_store, then attn_packed_cache8 on its queries
+    (ei_packed_step_cache8).  Returns [rows, H, 128]."""
+    batch._check(shape)
+    rs = _rows_of("qkv", qkv, batch.rows, shape.qkv)
+    where = _cache8_args(cache, block_table, batch, shape.n_head_kv)
+    turn = _turn_args(cs, pos, shape, batch.rows, q_gamma, k_gamma)
+    bits = _mask_args(mask, batch.rows)
+    out = batch._out(out, qkv.device)
+    scale = default_scale() if scale is None else scale
+    if batch.rows:
+        _capi.call("ei_packed_step_cache8", _stream(), qkv.data_ptr(), rs, out.data_ptr(), *where, batch.n_seq,
+                   batch.rows, shape.n_head, shape.n_head_kv, shape.head_dim, *turn, *bits, float(scale),
+                   *batch._tail())
+    return out
+
+
+def attn_tree_paged(q: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor, block_table: torch.Tensor, block_size: int,
+                    batch: PackedBatch, shape: AttnShape, mask: torch.Tensor, scale: float | None = None,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+    """attn_packed_paged for trees of drafted tokens (ei_attn_tree_paged): a row sees the keys before its sequence's
+    new rows, and of those the ones whose bit is set in its row of mask (int64 [rows, words]), up to itself."""
+    batch._check(shape)
+    qs = _rows_of("q", q, batch.rows, shape.n_head * HEAD_DIM)
+    pool = _pool_args(kc, vc, block_table, block_size, batch, shape)
+    bits = _mask_args(mask, batch.rows)
+    out = batch._out(out, q.device)
+    scale = default_scale() if scale is None else scale
+    if batch.rows:
+        _capi.call("ei_attn_tree_paged", _stream(), q.data_ptr(), qs, out.data_ptr(), *pool, batch.n_seq, batch.rows,
+                   shape.n_head, shape.n_head_kv, shape.head_dim, *bits, float(scale), *batch._tail())
+    return out
+
+
+def tree_step_paged(qkv: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor, block_table: torch.Tensor, block_size: int,
+                    batch: PackedBatch, shape: AttnShape, q_gamma: torch.Tensor, k_gamma: torch.Tensor,
+                    cs: torch.Tensor, pos: torch.Tensor | None = None, mask: torch.Tensor | None = None,
+                    scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """packed_step_paged for trees of drafted tokens, at positions pos (int32 [rows], None: the rows' slots) and with
+    a mask (ei_tree_step_paged).  Returns [rows, H, 128]."""
+    batch._check(shape)
+    rs = _rows_of("qkv", qkv, batch.rows, shape.qkv)
+    pool = _pool_args(kc, vc, block_table, block_size, batch, shape)
+    turn = _turn_args(cs, pos, shape, batch.rows, q_gamma, k_gamma)
+    bits = _mask_args(mask, batch.rows)
+    out = batch._out(out, qkv.device)
+    scale = default_scale() if scale is None else scale
+    if batch.rows:
+        _capi.call("ei_tree_step_paged", _stream(), qkv.data_ptr(), rs, out.data_ptr(), *pool, batch.n_seq, batch.rows,
+                   shape.n_head, shape.n_head_kv, shape.head_dim, *turn, *bits, float(scale), *batch._tail())
+    return out
+
+
+def _kept_args(batch: PackedBatch, kept: torch.Tensor, n_kept: torch.Tensor, out: torch.Tensor | None) -> tuple:
+    _need_contiguous("kept", kept, torch.int32)
+    _need_contiguous("n_kept", n_kept, torch.int32)
+    if kept.dim() != 2 or kept.shape[0] < batch.n_seq or kept.shape[1] < 1:
+        raise ValueError(f"kept must be [{batch.n_seq}, most], got {tuple(kept.shape)}")
+    if out is None:
+        out = torch.empty(batch.n_seq, dtype=torch.int32, device=kept.device)
+    _need_contiguous("out", out, torch.int32)
+    for name, t in (("n_kept", n_kept), ("out", out)):
+        if t.numel() < batch.n_seq:
+            raise ValueError(f"{name} must hold {batch.n_seq} numbers, got {t.numel()}")
+    return (kept.data_ptr(), kept.shape[1], n_kept.data_ptr(), out.data_ptr(), batch.buf.data_ptr(), batch.nbytes), out
+
+
+def cache_keep(kc: torch.Tensor, vc: torch.Tensor, block_table: torch.Tensor, block_size: int, batch: PackedBatch,
+               shape: AttnShape, kept: torch.Tensor, n_kept: torch.Tensor,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """After a batch of drafts was checked: moves the accepted rows of each sequence's new rows, kept int32
+    [n_seq, most] (rising; n_kept int32 [n_seq] of them count), together behind its earlier keys in the fp32 pool
+    (ei_cache_keep).  Returns the sequences' lengths with them, int32 [n_seq]; `out` may be the batch's kv_len."""
+    batch._check(shape)
+    pool = _pool_args(kc, vc, block_table, block_size, batch, shape)
+    args, out = _kept_args(batch, kept, n_kept, out)
+    _capi.call("ei_cache_keep", _stream(), *pool, batch.n_seq, batch.rows, shape.n_head, shape.n_head_kv,
+               shape.head_dim, *args)
+    return out
+
+
+def cache8_keep(cache: Cache8, block_table: torch.Tensor, batch: PackedBatch, kept: torch.Tensor, n_kept: torch.Tensor,
+                out: torch.Tensor | None = None) -> torch.Tensor:
+    """cache_keep in the 8-bit cache (ei_cache8_keep)."""
+    _need_cached(batch)
+    where = _cache8_args(cache, block_table, batch, batch.n_head_kv)
+    args, out = _kept_args(batch, kept, n_kept, out)
+    _capi.call("ei_cache8_keep", _stream(), *where, batch.n_seq, batch.rows, batch.n_head, batch.n_head_kv, HEAD_DIM,
+               *args)
+    return out
+
+
 # ---------------------------------------------------------------- synthetic inputs
 def synth_fill(t: torch.Tensor, seed: int, offset: int = 0, row_len: int = 1, spike_every: int = 0,
                spike_mult: float = 1.0) -> torch.Tensor:
@@ -551,5 +791,6 @@ __all__ = [
     "AttnShape", "DecodeWorkspace", "attn_decode", "attn_decode_batched", "attn_prefill", "decode_step",
     "default_scale", "headnorm_rope", "kv_append", "qkv_prepare", "rope_table", "synth_fill", "flops_causal",
     "decode_bytes", "RopeScaling", "rope_table_scaled", "rope_rows", "PackedBatch", "attn_packed",
-    "attn_packed_paged", "packed_step_paged",
+    "attn_packed_paged", "packed_step_paged", "Cache8", "cache8_store", "cache8_load", "attn_packed_cache8",
+    "packed_step_cache8", "attn_tree_paged", "tree_step_paged", "cache_keep", "cache8_keep",
 ]

@@ -1,0 +1,668 @@
+// cache8.hip — a paged cache of 8-bit keys and values on gfx950: quantising a batch's new rows into it, reading rows
+// back, attention over it (causal or over trees of drafts), and moving an accepted path's rows together.
+#include <type_traits>
+
+#include "packed.h"
+
+namespace ei {
+
+// ------------------------------------------------------------------ codes and their scales
+// y of largest magnitude a: int8 scale a / 127, code rint(y (127 / a)); e4m3 scale a / 448, code e4m3(y (448 / a)).
+// Below kNothing 127 / a and 448 / a would pass fp32's range on the way to it: such a head row is all zeros.
+constexpr float kNothing = 0x1p-110f;
+struct Coding {
+    float scale, by;  // what a code stands for, and what a value is multiplied by
+    bool bad;         // a value that is not finite: scale NaN, codes 0
+};
+template <bool kInt8>
+__device__ __forceinline__ Coding coding(float most) {
+    constexpr float kTop = kInt8 ? 127.f : 448.f;
+    const bool bad = !(most < INFINITY);  // (infinite or NaN)
+    if (bad) return {__builtin_nanf(""), 0.f, true};
+    if (most < kNothing) return {0.f, 0.f, false};
+    return {most / kTop, kTop / most, false};
+}
+// the code of y, in the low byte
+template <bool kInt8>
+__device__ __forceinline__ uint32_t code_of(float y, const Coding& c) {
+#pragma clang fp contract(off)
+    const float x = c.bad ? 0.f : y * c.by;
+    if constexpr (kInt8) return (uint32_t)(int)rintf(x) & 0xFFu;
+    else return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false) & 0xFFu;
+}
+// the largest magnitude over the wave; NaN where a value is (fmaxf would drop it)
+__device__ __forceinline__ float wave_most(float a, float b) {
+    const float m = wave_max(fmaxf(__builtin_fabsf(a), __builtin_fabsf(b)));
+    const bool nan = __builtin_amdgcn_ballot_w64(!(a == a) || !(b == b)) != 0;
+    return nan ? __builtin_nanf("") : m;
+}
+// two values of a code pair
+template <bool kInt8, int kByte>
+__device__ __forceinline__ float value_of(uint32_t codes) {
+    if constexpr (kInt8) return (float)(int)(int8_t)(codes >> (8 * kByte));
+    else return __builtin_amdgcn_cvt_f32_fp8((int)codes, kByte);
+}
+// the head row of key t in page `page`: rows of 128 codes, and scales
+__device__ __forceinline__ size_t head_row(int page, int HKV, int kvh, int shift, int t) {
+    return (((size_t)page * HKV + kvh) << shift) | (size_t)(t & ((1 << shift) - 1));
+}
+
+// ------------------------------------------------------------------ storing
+// grid (rows, ceil((H + HKV) / 16)), block 256: each wave four consecutive heads of the row, a key head with the value
+// head beside it, loads first (as k_packed_prepare).  Lane l holds elements l and l + 64; four lanes' codes are put
+// together for one store.
+constexpr int kStoreHeads = 4;
+template <bool kInt8>
+__global__ __launch_bounds__(256) void k_cache8_store(const float* __restrict__ qkv, long row_stride,
+                                                      float* __restrict__ q_out, Cache8Args a,
+                                                      const float* __restrict__ q_gamma,
+                                                      const float* __restrict__ k_gamma,
+                                                      const float2* __restrict__ cs, int n_pos,
+                                                      const int* __restrict__ turn_at, int rope_dim, float eps) {
+    __shared__ float scratch[4][kHeadDim];
+    const int b = blockIdx.x, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int H = a.H, HKV = a.HKV, NH = H + HKV;
+    const int h0 = (blockIdx.y * 4 + w) * kStoreHeads;
+    if (h0 >= NH) return;  // wave-uniform, no barrier here
+    const float* row = qkv + (size_t)b * row_stride;
+    float x0[kStoreHeads], x1[kStoreHeads], v0[kStoreHeads], v1[kStoreHeads], inv[kStoreHeads];
+#pragma unroll
+    for (int j = 0; j < kStoreHeads; ++j) {
+        const int hh = min(h0 + j, NH - 1);  // clamped: heads past NH are loaded, not used
+        const float* v = row + (size_t)hh * kHeadDim;
+        x0[j] = v[lane];
+        x1[j] = v[lane + 64];
+        v0[j] = v1[j] = 0.f;
+        if (hh >= H) {
+            const float* vs = row + (size_t)(NH + hh - H) * kHeadDim;  // V of a key head
+            v0[j] = vs[lane];
+            v1[j] = vs[lane + 64];
+        }
+    }
+    if (!plan_fits(a.plan, a.n_seq, a.rows, H, HKV, false)) return;
+    const int4* seq = reinterpret_cast<const int4*>(a.plan + kPlanSeqAt);
+    const int s = row_owner(seq, a.n_seq, b, lane);
+    if (s < 0) return;
+    const int4 e = seq[s];
+    const int slot = e.z - e.y + (b - e.x);
+    const int turn = turn_at ? turn_at[b] : slot;
+    const bool in = slot >= 0 && slot < reinterpret_cast<const int*>(a.plan)[kHeadMaxKv] && turn >= 0 && turn < n_pos;
+    const int blk = slot >> a.bshift;
+    const int page = in && blk < a.max_blocks ? a.btab[(size_t)s * a.max_blocks + blk] : -1;
+    const bool there = page >= 0 && page < a.n_blocks;
+    const float2* cs_row = cs + (size_t)(in ? turn : 0) * (rope_dim >> 1);
+    const float qg0 = q_gamma[lane], qg1 = q_gamma[lane + 64];
+    const float kg0 = k_gamma[lane], kg1 = k_gamma[lane + 64];
+    head_inv<kStoreHeads>(x0, x1, eps, inv, lane);
+    auto store = [&](uint8_t* codes, float* scales, size_t at, float y0, float y1) {
+        const Coding c = coding<kInt8>(wave_most(y0, y1));
+        uint32_t w0 = code_of<kInt8>(y0, c) << (8 * (lane & 3)), w1 = code_of<kInt8>(y1, c) << (8 * (lane & 3));
+        auto joined = [](uint32_t x) {
+            x |= __float_as_uint(lane_xor1(__uint_as_float(x)));
+            return x | __float_as_uint(lane_xor2(__uint_as_float(x)));
+        };
+        w0 = joined(w0), w1 = joined(w1);
+        uint32_t* dst = reinterpret_cast<uint32_t*>(codes + at * kHeadDim) + (lane >> 2);
+        if ((lane & 3) == 0) dst[0] = w0, dst[16] = w1;
+        if (lane == 0) scales[at] = c.scale;
+    };
+#pragma unroll
+    for (int j = 0; j < kStoreHeads; ++j) {
+        const int hh = h0 + j;
+        if (hh >= NH) break;
+        const bool is_k = hh >= H;
+        if (!is_k && !q_out) continue;
+        float o0 = x0[j], o1 = x1[j];
+        if (in)
+            scale_rope_vals(x0[j], x1[j], inv[j], is_k ? kg0 : qg0, is_k ? kg1 : qg1, cs_row, rope_dim, scratch[w],
+                            lane, &o0, &o1);
+        if (!is_k) {
+            float* dst = q_out + ((size_t)b * H + hh) * kHeadDim;
+            dst[lane] = o0;
+            dst[lane + 64] = o1;
+        } else if (there) {
+            const size_t at = head_row(page, HKV, hh - H, a.bshift, slot);
+            store(a.k8, a.ks, at, o0, o1);
+            store(a.v8, a.vs, at, v0[j], v1[j]);
+        }
+    }
+}
+
+// ------------------------------------------------------------------ reading back
+// A wave per row and turn, a lane four codes: 32 lanes a head row, two head rows of K and V at a time.
+template <bool kInt8>
+__global__ __launch_bounds__(256) void k_cache8_load(Cache8Args a, float* __restrict__ k_out,
+                                                     float* __restrict__ v_out, long out_stride) {
+    const int lane = threadIdx.x & 63, HKV = a.HKV;
+    if (!plan_fits(a.plan, a.n_seq, a.rows, a.H, HKV, false)) return;
+    const int b = blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (b >= a.rows) return;
+    const int4* seq = reinterpret_cast<const int4*>(a.plan + kPlanSeqAt);
+    const int s = row_owner(seq, a.n_seq, b, lane);
+    if (s < 0) return;
+    const int4 e = seq[s];
+    const int slot = e.z - e.y + (b - e.x), blk = slot >> a.bshift;
+    const int page = slot >= 0 && blk < a.max_blocks ? a.btab[(size_t)s * a.max_blocks + blk] : -1;
+    const bool there = page >= 0 && page < a.n_blocks;
+    const int c = lane & 31;
+    for (int h = lane >> 5; h < HKV; h += 2) {
+        const size_t at = head_row(there ? page : 0, HKV, h, a.bshift, there ? slot : 0);
+        auto read = [&](const uint8_t* codes, const float* scales, float* out) {
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (there) {
+                const uint32_t x = reinterpret_cast<const uint32_t*>(codes + at * kHeadDim)[c];
+                const float f = scales[at];
+                y = make_float4(value_of<kInt8, 0>(x) * f, value_of<kInt8, 1>(x) * f, value_of<kInt8, 2>(x) * f,
+                                value_of<kInt8, 3>(x) * f);
+            }
+            reinterpret_cast<float4*>(out + (size_t)b * out_stride + (size_t)h * kHeadDim)[c] = y;
+        };
+        read(a.k8, a.ks, k_out);
+        read(a.v8, a.vs, v_out);
+    }
+}
+
+// ------------------------------------------------------------------ the accepted path
+// Moves rows of `a row's pieces` of 16 bytes (or scales of 4): a thread takes one piece of a sequence's rows and walks
+// the list, kAtOnce loads in flight.  Entries rise, so kept[j] >= j: a row that is read has not been written before.
+constexpr int kKeepAtOnce = 8;
+template <typename T, typename At>
+__device__ __forceinline__ void move_rows(T* pool, const int* kept, int n, At at) {
+    for (int j0 = 0; j0 < n; j0 += kKeepAtOnce) {
+        T x[kKeepAtOnce];
+        long to[kKeepAtOnce];
+#pragma unroll
+        for (int j = 0; j < kKeepAtOnce; ++j) {
+            const int i = min(j0 + j, n - 1);
+            const long from = at(kept[i]);
+            to[j] = from < 0 || j0 + j >= n ? -1 : at(i);
+            if (to[j] >= 0) x[j] = pool[from];
+        }
+#pragma unroll
+        for (int j = 0; j < kKeepAtOnce; ++j)
+            if (to[j] >= 0) pool[to[j]] = x[j];
+    }
+}
+// grid (n_seq, pieces / 256): pieces of 16 bytes of K, then of V, then (8-bit) the scales
+template <bool kF32>
+__global__ __launch_bounds__(256) void k_cache_keep(Cache8Args a, float* __restrict__ kc, float* __restrict__ vc,
+                                                    const int* __restrict__ kept, int max_kept,
+                                                    const int* __restrict__ n_kept, int* __restrict__ new_len) {
+    if (!plan_fits(a.plan, a.n_seq, a.rows, a.H, a.HKV, false)) return;
+    const int s = blockIdx.x, lane = threadIdx.x & 63;
+    const int4 e = reinterpret_cast<const int4*>(a.plan + kPlanSeqAt)[s];
+    const int first = e.z - e.y;
+    const int* list = kept + (size_t)s * max_kept;
+    // the entries that rise and are rows of the sequence, 64 at a time
+    int n = min(max(n_kept[s], 0), min(max_kept, e.y));
+    for (int j0 = 0; j0 < n; j0 += 64) {
+        const int j = j0 + lane;
+        bool good = true;
+        if (j < n) {
+            const int x = list[j], before = j > 0 ? list[j - 1] : -1;
+            good = x > before && x < e.y;
+        }
+        const uint64_t bad = __builtin_amdgcn_ballot_w64(!good);
+        if (bad) n = j0 + __builtin_ctzll(bad);
+    }
+    if (blockIdx.y == 0 && threadIdx.x == 0) new_len[s] = max(first + n, 0);
+    const int per_row = a.HKV * (kF32 ? 32 : 8);  // pieces of a row of K
+    int i = blockIdx.y * 256 + threadIdx.x;
+    // the place of a new row: its page and row in it; -1: none
+    auto place = [&](int row, int& page) {
+        const int slot = first + row, blk = slot >> a.bshift;
+        page = slot >= 0 && blk < a.max_blocks ? a.btab[(size_t)s * a.max_blocks + blk] : -1;
+        if (page >= a.n_blocks) page = -1;
+        return slot & ((1 << a.bshift) - 1);
+    };
+    if (i < 2 * per_row) {
+        const bool is_v = i >= per_row;
+        if (is_v) i -= per_row;
+        auto at = [&](int row) -> long {
+            int page;
+            const int t = place(row, page);
+            if (page < 0) return -1;
+            if constexpr (kF32) return (long)((((size_t)page << a.bshift) | (size_t)t) * per_row + i);
+            else return (long)(((((size_t)page * a.HKV + (i >> 3)) << a.bshift) | (size_t)t) * 8 + (i & 7));
+        };
+        void* pool = kF32 ? (is_v ? (void*)vc : (void*)kc) : is_v ? (void*)a.v8 : (void*)a.k8;
+        move_rows(reinterpret_cast<u32x4*>(pool), list, n, at);
+        return;
+    }
+    if constexpr (!kF32) {
+        i -= 2 * per_row;
+        if (i >= 2 * a.HKV) return;
+        const int h = i % a.HKV;
+        auto at = [&](int row) -> long {
+            int page;
+            const int t = place(row, page);
+            return page < 0 ? -1 : (long)((((size_t)page * a.HKV + h) << a.bshift) | (size_t)t);
+        };
+        move_rows(i >= a.HKV ? a.vs : a.ks, list, n, at);
+    }
+}
+
+// ------------------------------------------------------------------ attention
+// Codes are exact in binary16, so a product with an fp32 operand takes two planes of it, x = h + l (22 bits of
+// 24): two matrix instructions where two fp32 operands take three (packed.hip) or six (prefill.hip).
+//
+//   scores   q, scaled per row to a largest value of 2^14, against the codes of K; times the key's scale in fp32
+//   output   weights p = 2^(s - m) times the value's scale times F, a power of two of the row's own: the largest
+//            p s_v F so far lies below 2^15 and F only goes down where a larger one comes (the sums go with it),
+//            up where the reference m rises (the sums stay).  So what the planes lose, 2^-39 of the row's largest weight
+//            times scale, never shows, however uneven the values' scales are.  m is a whole number: every factor
+//            of the sums is a power of two, exact.
+struct Tile8 {
+    u32x4 k[2][2];  // [sixteen keys][half of the lane's 32 codes]
+    u32x2 v[8];
+    f32x4 ks[2], vs[2];
+};
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                  0);
+}
+// Codes 2x and 2x + 1 of four as binary16: e4m3 by its conversion; int8 as 1024 + 128 + code, the code's sign bit
+// flipped in the low bits of 1024, less 1152.  (`flipped`: the four codes with their sign bits flipped, for int8.)
+template <bool kInt8, int x>
+__device__ __forceinline__ uint32_t pair_f16(uint32_t codes) {
+    if constexpr (kInt8) {
+        const uint32_t biased = __builtin_amdgcn_perm(0x64646464u, codes, x ? 0x04030402u : 0x04010400u);
+        const f16x2 y = __builtin_bit_cast(f16x2, biased) + f16x2{(_Float16)-1152.f, (_Float16)-1152.f};
+        return __builtin_bit_cast(uint32_t, y);
+    } else {
+        return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 1.f, x));
+    }
+}
+template <bool kInt8>
+__device__ __forceinline__ uint32_t flipped(uint32_t codes) { return kInt8 ? codes ^ 0x80808080u : codes; }
+
+constexpr int kRow8 = 16;                              // rows of one matrix instruction
+constexpr int kFew8ML = kWaves * kRow8 * kRowF;        // LDS: every wave's rows, then their (m, l)
+constexpr int kFew8F = kFew8ML + kWaves * kRow8 * 2;
+constexpr int kTopF = 100;                             // log2 F at most, and of a row without weights
+constexpr float kTopW = 0x1p15f;                       // p s_v F at most
+constexpr float kLazy8 = 8.f;                          // the reference moves when a score passes it by more (log2 units)
+__device__ __forceinline__ float pow2(int e) { return __builtin_amdgcn_ldexpf(1.f, e); }
+
+// The unit's rows in blocks of sixteen, one per wave; waves of a block take its tiles in turn, each lane
+// its row l % 16 and quarter l / 16:
+//   S^T[key][row] = K . Q^T: the lane has of key 16 kb + l % 16 codes 32 quarter .. + 31, and gets the scores of the
+//     keys 16 kb + 4 quarter + r (kb = 0, 1; r = 0 .. 3) for its row;
+//   O^T[d][row] = V^T . P^T over the tile's 32 keys in the order of those scores: the lane has codes
+//     8 (l % 16) .. + 7 of its eight keys, put together pair of keys by pair; sum y, register r is
+//     d = 32 quarter + 8 r + y.
+template <bool kInt8, bool kTree>
+__device__ __forceinline__ void rows_pass(const Cache8Args& a, const Pass& p, int kvh, FastDiv fG, float sl2,
+                                          int ml_at, float* smem) {
+    constexpr int D = kHeadDim;
+    const int tid = unhoisted(threadIdx.x), lane = tid & 63, wu = scalar(tid >> 6);
+    const int j = lane & 15, quarter = lane >> 4;
+    const int G = (int)fG.d;
+    const int f0 = kUnitRows * p.u, last = p.nflat - 1, rows = min(p.nflat - f0, kUnitRows);
+    const int nb = rows <= kRow8 ? 1 : rows <= 2 * kRow8 ? 2 : rows <= 4 * kRow8 ? 4 : 8;
+    const int rb = wu & (nb - 1), off = wu / nb, step = kWaves / nb;
+    const int row = min(f0 + kRow8 * rb + j, last);  // (rows past the last repeat it)
+    const int tok = fdiv(row, fG), qpos = p.pos0 + tok;
+    const int nfull = max(kTree ? p.pos0 : p.pos0 + fdiv(min(f0 + kRow8 * rb, last), fG) + 1, 0) / kKT;
+    const int n_mine = (p.nrange - off + step - 1) / step;
+    auto index = [&](int i) { return p.kt_lo + step * i + off; };
+    auto page = [&](int i) { return page_of<true>(a, p, index(i) * kKT); };
+    auto codes_at = [&](const uint8_t* codes, int i, int pg, bool wanted) {
+        const int t0 = index(i) * kKT;
+        const bool ok = wanted && pg >= 0 && pg < a.n_blocks;
+        return __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint8_t*>(codes) + (ok ? head_row(pg, a.HKV, kvh, a.bshift, t0) * D : 0), 0,
+            ok ? min(kKT, p.T - t0) * D : 0, kBufferDword3);
+    };
+    auto scales_at = [&](const float* scales, int i, int pg, bool wanted) {  // (whole tiles: pages hold them)
+        const bool ok = wanted && pg >= 0 && pg < a.n_blocks;
+        return __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<float*>(scales) + (ok ? head_row(pg, a.HKV, kvh, a.bshift, index(i) * kKT) : 0), 0,
+            ok ? kKT * 4 : 0, kBufferDword3);
+    };
+    auto as_f32x4 = [](u32x4 x) { return __builtin_bit_cast(f32x4, x); };
+    auto load = [&](Tile8& t, int i, int pg, bool wanted) {
+        const uint32_t ln = lane_now();
+        const Rsrc rk = codes_at(a.k8, i, pg, wanted), rv = codes_at(a.v8, i, pg, wanted);
+        const Rsrc sk = scales_at(a.ks, i, pg, wanted), sv = scales_at(a.vs, i, pg, wanted);
+        const uint32_t ok = (ln & 15) * D + (ln >> 4) * 32, ov = (ln >> 4) * (4 * D) + (ln & 15) * 8;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+            for (int x = 0; x < 2; ++x)
+                t.k[kb][x] = __builtin_amdgcn_raw_buffer_load_b128(rk, ok + 16 * kb * D + 16 * x, 0, 0);
+            t.ks[kb] = as_f32x4(__builtin_amdgcn_raw_buffer_load_b128(sk, (ln >> 4) * 16 + 64 * kb, 0, 0));
+            t.vs[kb] = as_f32x4(__builtin_amdgcn_raw_buffer_load_b128(sv, (ln >> 4) * 16 + 64 * kb, 0, 0));
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            t.v[e] = __builtin_amdgcn_raw_buffer_load_b64(rv, ov + (16 * (e >> 2) + (e & 3)) * D, 0, 0);
+    };
+
+    // q: planes of d = 32 quarter + 8 x + 0 .. 7
+    u32x4 qh[4], ql[4];
+    float sq;  // takes the row's scaling out of its scores
+    {
+        const float* src = a.q + ((size_t)p.row0 + tok) * a.q_stride + (size_t)(kvh * G + row - tok * G) * D + 32 * quarter;
+        float4 q[8];
+        float most = 0.f;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            const float4 v = *reinterpret_cast<const float4*>(src + 4 * x);
+            q[x] = make_float4(v.x * sl2, v.y * sl2, v.z * sl2, v.w * sl2);
+            most = fmaxf(fmaxf(most, __builtin_fabsf(q[x].x)), __builtin_fabsf(q[x].y));
+            most = fmaxf(fmaxf(most, __builtin_fabsf(q[x].z)), __builtin_fabsf(q[x].w));
+        }
+        most = half_max(fmaxf(most, lane_xor16(most)));
+        const uint32_t f = scale_to<14>(most);
+        const float fq = __uint_as_float(f);
+        sq = inverse(f);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            uint32_t h[4], l[4];
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const float4 v = q[2 * x + y];
+                split_f16(v.x * fq, v.y * fq, h[2 * y], l[2 * y]);
+                split_f16(v.z * fq, v.w * fq, h[2 * y + 1], l[2 * y + 1]);
+            }
+            qh[x] = u32x4{h[0], h[1], h[2], h[3]};
+            ql[x] = u32x4{l[0], l[1], l[2], l[3]};
+        }
+    }
+    f32x4 o[8];
+    float m = -INFINITY, l = 0.f;
+    int fe = kTopF;  // log2 F
+#pragma unroll
+    for (int y = 0; y < 8; ++y) o[y] = f32x4{0.f, 0.f, 0.f, 0.f};
+    auto scale_o = [&](float by) {
+#pragma unroll
+        for (int y = 0; y < 8; ++y)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[y][r] *= by;
+    };
+    auto row_max = [&](float x) { return half_max(fmaxf(x, lane_xor16(x))); };
+
+    auto tile = [&](const Tile8& t, int i, int pg) {
+        const int kt = index(i);
+        f32x4 s[2];
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb) {
+            s[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+                const uint32_t lo = flipped<kInt8>(t.k[kb][x >> 1][2 * (x & 1)]);
+                const uint32_t hi = flipped<kInt8>(t.k[kb][x >> 1][2 * (x & 1) + 1]);
+                const u32x4 kf = {pair_f16<kInt8, 0>(lo), pair_f16<kInt8, 1>(lo), pair_f16<kInt8, 0>(hi),
+                                  pair_f16<kInt8, 1>(hi)};
+                s[kb] = mfma16(kf, ql[x], s[kb]);
+                s[kb] = mfma16(kf, qh[x], s[kb]);
+            }
+        }
+        uint32_t bits = ~0u;
+        if (kt >= nfull) {
+            if constexpr (kTree) bits = tree_bits(a, p, qpos, kt * kKT);
+            else {
+                const int n = qpos - kt * kKT + 1;
+                bits = n >= kKT ? ~0u : n <= 0 ? 0u : (1u << n) - 1u;
+            }
+        }
+        const uint32_t mine = bits >> (4 * quarter);
+        auto seen = [&](int r) { return (mine >> (16 * (r >> 2) + (r & 3)) & 1) != 0; };
+        float mx = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) s[r >> 2][r & 3] = s[r >> 2][r & 3] * sq * t.ks[r >> 2][r & 3];
+        if (kt >= nfull) {
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+                if (!seen(r)) s[r >> 2][r & 3] = -INFINITY;
+        }
+#pragma unroll
+        for (int r = 0; r < 8; ++r) mx = fmaxf(mx, s[r >> 2][r & 3]);
+        mx = row_max(mx);
+        if (__builtin_amdgcn_ballot_w64(mx > m + kLazy8)) {  // rare after the first tile
+            const float mn = fmaxf(m, ceilf(mx));
+            const int up = m == mn ? 0 : (int)fminf(mn - m, 1000.f);
+            l *= pow2(-up);
+            const int fn = min(fe + up, kTopF);  // the sums stay where F can go up by as much
+            if (__builtin_amdgcn_ballot_w64(fn - fe != up)) scale_o(pow2(fn - fe - up));
+            fe = fn;
+            m = mn;
+        }
+        const float nb = m == -INFINITY ? 0.f : -m;
+        float sum = 0.f, wm = 0.f;
+        float wt[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const float pr = __builtin_amdgcn_exp2f(s[r >> 2][r & 3] + nb);
+            sum += pr;
+            wt[r] = pr * t.vs[r >> 2][r & 3];
+        }
+        l += sum;
+        if (kt >= nfull) {  // (a scale that the row does not see may be anything)
+#pragma unroll
+            for (int r = 0; r < 8; ++r)
+                if (!seen(r)) wt[r] = 0.f;
+        }
+#pragma unroll
+        for (int r = 0; r < 8; ++r) wm = fmaxf(wm, __builtin_fabsf(wt[r]));
+        wm = row_max(wm);
+        float F = pow2(fe);
+        if (__builtin_amdgcn_ballot_w64(wm * F > kTopW)) {  // rare after the first tile
+            // wm F: 2^14 .. 2^15
+            const int fn = wm * F > kTopW ? 127 + 14 - (int)min(__float_as_uint(wm) >> 23, 254u) : fe;
+            scale_o(pow2(fn - fe));
+            fe = fn;
+            F = pow2(fe);
+        }
+        uint32_t wh[4], wl[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) split_f16(wt[2 * r] * F, wt[2 * r + 1] * F, wh[r], wl[r]);
+        const u32x4 ph = {wh[0], wh[1], wh[2], wh[3]}, pl = {wl[0], wl[1], wl[2], wl[3]};
+        if constexpr (!kInt8) {
+            // a NaN among codes that not every row sees must not meet them: key by key then
+            uint32_t nan = 0;
+            if (kt >= nfull) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) nan |= ((t.v[e][x] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+            }
+            if (__builtin_amdgcn_ballot_w64(nan != 0)) {
+                const Rsrc rv = codes_at(a.v8, i, pg, true);
+#pragma unroll 1
+                for (int c = 0; c < kKT; ++c) {
+                    float wc = 0.f;
+#pragma unroll
+                    for (int r = 0; r < 8; ++r)  // key 16 (r / 4) + 4 quarter + r % 4
+                        if (c == 16 * (r >> 2) + 4 * quarter + (r & 3)) wc = wt[r] * F;
+                    wc += lane_xor16(wc);
+                    wc += lane_xor32(wc);
+#pragma unroll
+                    for (int x = 0; x < 2; ++x) {
+                        const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(rv, c * D + 32 * quarter + 16 * x, 0, 0);
+                        if (bits >> c & 1) {
+#pragma unroll
+                            for (int y = 0; y < 4; ++y) {  // d = 32 quarter + 16x + 4y + 0 .. 3
+                                const int r = 2 * x + (y >> 1), at = 4 * (y & 1);
+                                o[at][r] = __builtin_fmaf(wc, value_of<false, 0>(v[y]), o[at][r]);
+                                o[at + 1][r] = __builtin_fmaf(wc, value_of<false, 1>(v[y]), o[at + 1][r]);
+                                o[at + 2][r] = __builtin_fmaf(wc, value_of<false, 2>(v[y]), o[at + 2][r]);
+                                o[at + 3][r] = __builtin_fmaf(wc, value_of<false, 3>(v[y]), o[at + 3][r]);
+                            }
+                        }
+                    }
+                }
+                return;
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            uint32_t vf[4][4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {  // keys 2e, 2e + 1 of the lane's eight
+                const uint32_t u = t.v[2 * e][x], w = t.v[2 * e + 1][x];
+                const uint32_t lo = flipped<kInt8>(__builtin_amdgcn_perm(w, u, 0x05010400u));
+                const uint32_t hi = flipped<kInt8>(__builtin_amdgcn_perm(w, u, 0x07030602u));
+                vf[0][e] = pair_f16<kInt8, 0>(lo), vf[1][e] = pair_f16<kInt8, 1>(lo);
+                vf[2][e] = pair_f16<kInt8, 0>(hi), vf[3][e] = pair_f16<kInt8, 1>(hi);
+            }
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                const u32x4 v = {vf[y][0], vf[y][1], vf[y][2], vf[y][3]};
+                o[4 * x + y] = mfma16(v, pl, o[4 * x + y]);
+                o[4 * x + y] = mfma16(v, ph, o[4 * x + y]);
+            }
+        }
+    };
+    Tile8 t0, t1;
+    if (n_mine > 0) {
+        int p0 = page(0), p1 = page(1);
+        load(t0, 0, p0, true);
+        for (int i = 0; i < n_mine; i += 2) {
+            load(t1, i + 1, p1, i + 1 < n_mine);
+            const int p2 = page(i + 2);
+            __builtin_amdgcn_sched_barrier(0);
+            tile(t0, i, p0);
+            __builtin_amdgcn_sched_barrier(0);
+            if (i + 1 >= n_mine) break;
+            load(t0, i + 2, p2, i + 2 < n_mine);
+            const int p3 = page(i + 3);
+            __builtin_amdgcn_sched_barrier(0);
+            tile(t1, i + 1, p1);
+            __builtin_amdgcn_sched_barrier(0);
+            p0 = p2, p1 = p3;
+        }
+    }
+    // every wave's rows meet
+    float* const own = smem + wu * (kRow8 * kRowF);
+    float* const ml = smem + kFew8ML;
+    {
+        const float f = pow2(-fe);
+        if (m == -INFINITY) {  // (scores of -infinity beside infinite values: parts without weights are passed over)
+            float z = 0.f;
+#pragma unroll
+            for (int y = 0; y < 8; ++y)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) z = __builtin_fmaf(o[y][r], 0.f, z);
+            l += z;
+        }
+        const float sum = half_sum(l + lane_xor16(l));
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int y = 0; y < 8; y += 4)
+                *reinterpret_cast<float4*>(own + j * kRowF + 32 * quarter + 8 * r + y) =
+                    make_float4(o[y][r] * f, o[y + 1][r] * f, o[y + 2][r] * f, o[y + 3][r] * f);
+        if (quarter == 0) *reinterpret_cast<float2*>(ml + 2 * (wu * kRow8 + j)) = make_float2(m, sum);
+    }
+    lds_barrier();
+    const int d = 4 * (lane & 31);
+    for (int i = 2 * wu + (lane >> 5); i < rows; i += 2 * kWaves) {
+        const int b = i >> 4, at = i & 15;
+        float M = -INFINITY, L = 0.f;
+        for (int w = b; w < kWaves; w += nb) M = fmaxf(M, ml[2 * (w * kRow8 + at)]);
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int w = b; w < kWaves; w += nb) {
+            const float2 e = *reinterpret_cast<const float2*>(ml + 2 * (w * kRow8 + at));
+            // (a wave whose every score is NaN keeps m at -inf, and its NaN sum counts)
+            const float c = e.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(e.x - M);
+            L += e.x == -INFINITY ? e.y : e.y * c;
+            const float4 v = *reinterpret_cast<const float4*>(smem + (w * kRow8 + at) * kRowF + d);
+            x.x = __builtin_fmaf(c, v.x, x.x), x.y = __builtin_fmaf(c, v.y, x.y);
+            x.z = __builtin_fmaf(c, v.z, x.z), x.w = __builtin_fmaf(c, v.w, x.w);
+        }
+        const int g = f0 + i, t = fdiv(g, fG);
+        float* dst;
+        if (p.part) {
+            dst = p.part + i * D;
+            if (d == 0) *reinterpret_cast<float2*>(p.part + ml_at + 2 * i) = make_float2(M, L);
+        } else {
+            dst = a.out + (((size_t)p.row0 + t) * a.H + kvh * G + g - t * G) * D;
+            bool none = p.pos0 + t < 0;  // a row that sees no key: zeros
+            if constexpr (kTree) none = L == 0.f && tree_sees_none(a, p.row0, p.pos0, t);
+            const float inv = none ? 0.f : 1.f / L;
+            x.x *= inv, x.y *= inv, x.z *= inv, x.w *= inv;
+        }
+        *reinterpret_cast<float4*>(dst + d) = x;
+    }
+}
+
+// grid shares x KV heads, as k_packed_attn
+template <bool kInt8, bool kTree>
+__global__ __launch_bounds__(64 * kWaves) void k_cache8_attn(Cache8Args a, int shares, float* __restrict__ wide_parts,
+                                                             float* __restrict__ few_parts) {
+    extern __shared__ __align__(16) float smem[];
+    const int kvh = blockIdx.x % a.HKV, share = blockIdx.x / a.HKV;
+    const PlanView pv = plan_view(const_cast<char*>(a.plan), a.n_seq, a.rows, a.H / a.HKV, shares);
+    const int rounds = scalar(reinterpret_cast<const int*>(a.plan)[kHeadRounds]);
+    const int4 wide = *reinterpret_cast<const int4*>(pv.wide.shares + share);
+    const int4 few = *reinterpret_cast<const int4*>(pv.few.shares + share);
+    if (!plan_fits(a.plan, a.n_seq, a.rows, a.H, a.HKV, false)) return;
+    const FastDiv fG = fast_div((uint32_t)(a.H / a.HKV));
+    const float sl2 = a.scale * 1.44269504088896340736f;  // scores come out in log2 units
+    walk_share<false>(a, pv.wide, wide, rounds, shares, share, kvh, fG, wide_parts, [&](const Pass& p) {
+        rows_pass<kInt8, kTree>(a, p, kvh, fG, sl2, kUnitRows * kHeadDim, smem);
+    });
+    lds_barrier();  // the last wide pass's rows have been read
+    walk_share<true>(a, pv.few, few, 0, shares, share, kvh, fG, few_parts, [&](const Pass& p) {
+        rows_pass<kInt8, kTree>(a, p, kvh, fG, sl2, kFewRows * kHeadDim, smem);
+    });
+}
+
+// ------------------------------------------------------------------ launchers
+template <typename F>
+static hipError_t by_kind(const Cache8Args& a, F f) {
+    return a.int8 ? f(std::true_type{}) : f(std::false_type{});
+}
+
+hipError_t launch_cache8_store(hipStream_t st, const Cache8Args& a, const float* qkv, long row_stride, float* q_out,
+                               const float* q_gamma, const float* k_gamma, const float* cs, int n_pos,
+                               const int* turn_at, int rope_dim, float eps) {
+    return by_kind(a, [&](auto kind) {
+        k_cache8_store<decltype(kind)::value><<<dim3(a.rows, (a.H + a.HKV + 15) / 16), 256, 0, st>>>(
+            qkv, row_stride, q_out, a, q_gamma, k_gamma, reinterpret_cast<const float2*>(cs), n_pos, turn_at, rope_dim,
+            eps);
+        return hipGetLastError();
+    });
+}
+
+hipError_t launch_cache8_load(hipStream_t st, const Cache8Args& a, float* k_out, float* v_out, long out_stride) {
+    return by_kind(a, [&](auto kind) {
+        k_cache8_load<decltype(kind)::value><<<(a.rows + 3) / 4, 256, 0, st>>>(a, k_out, v_out, out_stride);
+        return hipGetLastError();
+    });
+}
+
+hipError_t launch_cache_keep(hipStream_t st, const Cache8Args& a, float* kc, float* vc, const int* kept, int max_kept,
+                             const int* n_kept, int* new_len) {
+    const int pieces = kc ? 64 * a.HKV : 16 * a.HKV + 2 * a.HKV;
+    const dim3 grid(a.n_seq, (pieces + 255) / 256);
+    if (kc) k_cache_keep<true><<<grid, 256, 0, st>>>(a, kc, vc, kept, max_kept, n_kept, new_len);
+    else k_cache_keep<false><<<grid, 256, 0, st>>>(a, nullptr, nullptr, kept, max_kept, n_kept, new_len);
+    return hipGetLastError();
+}
+
+template <bool kInt8, bool kTree>
+static hipError_t launch_cache8_attn_as(hipStream_t st, const Cache8Args& a, int shares, const PackedParts& parts) {
+    static std::atomic<bool> opted;
+    constexpr size_t lds = (size_t)kFew8F * sizeof(float);
+    if (const hipError_t e = opt_in_lds(opted, (const void*)k_cache8_attn<kInt8, kTree>, lds); e != hipSuccess) return e;
+    k_cache8_attn<kInt8, kTree><<<shares * a.HKV, 64 * kWaves, lds, st>>>(a, shares, parts.wide, parts.few);
+    return hipGetLastError();
+}
+
+hipError_t launch_cache8_attn(hipStream_t st, const Cache8Args& a, void* ws) {
+    const int shares = packed_shares(a.HKV);
+    const PackedParts parts = packed_parts(ws, a.rows, a.H, a.HKV);
+    const hipError_t e = by_kind(a, [&](auto kind) {
+        constexpr bool kInt8 = decltype(kind)::value;
+        return a.mask ? launch_cache8_attn_as<kInt8, true>(st, a, shares, parts)
+                      : launch_cache8_attn_as<kInt8, false>(st, a, shares, parts);
+    });
+    if (e != hipSuccess) return e;
+    return launch_packed_combine(st, a, false, parts);
+}
+
+}  // namespace ei

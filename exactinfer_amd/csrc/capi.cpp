@@ -8,9 +8,11 @@
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
+#include <initializer_list>
 #include <string>
 
 #include "../../include/ei_attn.h"
+#include "../../include/ei_cache8.h"
 #include "../../include/ei_gguf.h"
 #include "../../include/ei_packed.h"
 #include "../host/gguf_index.h"
@@ -896,6 +898,353 @@ EI_API int ei_packed_step_paged(ei_stream_t stream, const float* qkv, long row_s
     return hip_status(ei::launch_packed_step(static_cast<hipStream_t>(stream), a, qkv, row_stride, kc, vc, q_gamma,
                                              k_gamma, cs, n_pos, rope_dim, eps, ws),
                       "packed step launch");
+}
+
+// ------------------------------------------------------------------ 8-bit cache, trees (include/ei_cache8.h)
+namespace {
+
+struct Span {  // what a call reads or writes
+    const void* at;
+    size_t bytes;
+    const char* name;
+};
+
+// Whether any of `written` shares a byte with another of them, or with one of `read` (null pointers: not there).
+int check_apart(std::initializer_list<Span> written, std::initializer_list<Span> read) {
+    for (const Span* w = written.begin(); w != written.end(); ++w) {
+        if (!w->at) continue;
+        for (const Span* x = w + 1; x != written.end(); ++x)
+            REQUIRE(!(x->at && overlap(w->at, w->bytes, x->at, x->bytes)), "%s overlaps %s", w->name, x->name);
+        for (const Span& r : read)
+            REQUIRE(!(r.at && overlap(w->at, w->bytes, r.at, r.bytes)), "%s overlaps %s", w->name, r.name);
+    }
+    return EI_OK;
+}
+
+int check_pages(const int* block_table, int max_blocks, int block_size, int n_blocks, int* shift) {
+    REQUIRE(block_table != nullptr, "null pointer argument");
+    REQUIRE(block_size >= 32 && (block_size & (block_size - 1)) == 0,
+            "block_size %d must be a power of two >= 32 (whole 32-key tiles per block)", block_size);
+    REQUIRE(max_blocks > 0 && (long)max_blocks * block_size <= 0x7FFFFFFFL,
+            "max_blocks %d x block_size %d must lie in [1, 2^31 - 1] keys", max_blocks, block_size);
+    REQUIRE(n_blocks > 0, "n_blocks %d must be positive", n_blocks);
+    int s = 0;
+    while ((1 << s) < block_size) ++s;
+    *shift = s;
+    return EI_OK;
+}
+
+int check_batch(int n_seq, int rows, int n_head, int n_head_kv, int head_dim, const void* plan, size_t plan_bytes) {
+    if (int e = check_heads(n_head, n_head_kv, head_dim)) return e;
+    REQUIRE(n_seq > 0 && n_seq <= kMaxPackedSeqs, "n_seq %d out of range [1, 65535]", n_seq);
+    REQUIRE(rows >= 0 && prefill_rows_ok(rows, n_head),
+            "rows %d x n_head %d: at most 2^20 rows and 2^28 query rows per launch", rows, n_head);
+    const size_t need = ei::packed_plan_bytes(n_seq, rows, n_head, n_head_kv);
+    REQUIRE(plan && aligned16(plan) && plan_bytes >= need,
+            "plan missing, not 16-byte aligned or %zu B < %zu B (ei_packed_plan_bytes)", plan_bytes, need);
+    return EI_OK;
+}
+
+int check_ws(const void* ws, size_t ws_bytes, int rows, int n_head, int n_head_kv) {
+    const size_t need = ei::packed_ws_bytes(rows, n_head, n_head_kv);
+    REQUIRE(ws && aligned16(ws) && ws_bytes >= need,
+            "workspace missing, not 16-byte aligned or %zu B < %zu B (ei_packed_ws_bytes)", ws_bytes, need);
+    return EI_OK;
+}
+
+int check_mask(const uint64_t* mask, int mask_words) {
+    REQUIRE(!mask || (mask_words > 0 && mask_words <= (1 << 20)), "mask_words %d out of range [1, 2^20]", mask_words);
+    REQUIRE((reinterpret_cast<uintptr_t>(mask) & 7u) == 0, "mask must be 8-byte aligned");
+    return EI_OK;
+}
+
+// The batch and the 8-bit pool into `a`, after checking both.
+int check_cache8(const ei_cache8* c, const int* block_table, int max_blocks, int n_seq, int rows, int n_head,
+                 int n_head_kv, int head_dim, const void* plan, size_t plan_bytes, ei::Cache8Args* a) {
+    if (int e = check_batch(n_seq, rows, n_head, n_head_kv, head_dim, plan, plan_bytes)) return e;
+    REQUIRE(c && c->k && c->v && c->k_scale && c->v_scale, "null pointer argument");
+    REQUIRE(c->kind == EI_CACHE_E4M3 || c->kind == EI_CACHE_INT8, "cache kind %d", c->kind);
+    REQUIRE(aligned16(c->k) && aligned16(c->v) && aligned16(c->k_scale) && aligned16(c->v_scale),
+            "codes and scales must be 16-byte aligned");
+    if (int e = check_pages(block_table, max_blocks, c->block_size, c->n_blocks, &a->bshift)) return e;
+    a->k8 = static_cast<uint8_t*>(c->k), a->v8 = static_cast<uint8_t*>(c->v);
+    a->ks = c->k_scale, a->vs = c->v_scale;
+    a->int8 = c->kind == EI_CACHE_INT8;
+    a->btab = block_table;
+    a->max_blocks = max_blocks, a->n_blocks = c->n_blocks;
+    a->n_seq = n_seq, a->rows = rows, a->H = n_head, a->HKV = n_head_kv;
+    a->plan = static_cast<const char*>(plan);
+    return EI_OK;
+}
+
+size_t head_rows(const ei::Cache8Args& a) { return ((size_t)a.n_blocks << a.bshift) * (size_t)a.HKV; }
+Span codes_k(const ei::Cache8Args& a) { return {a.k8, head_rows(a) * 128, "the K codes"}; }
+Span codes_v(const ei::Cache8Args& a) { return {a.v8, head_rows(a) * 128, "the V codes"}; }
+Span scales_k(const ei::Cache8Args& a) { return {a.ks, head_rows(a) * 4, "the K scales"}; }
+Span scales_v(const ei::Cache8Args& a) { return {a.vs, head_rows(a) * 4, "the V scales"}; }
+Span the_table(const ei::PackedArgs& a) {
+    return {a.btab, (size_t)a.n_seq * a.max_blocks * sizeof(int), "the block table"};
+}
+Span the_plan(const ei::PackedArgs& a) {
+    return {a.plan, ei::packed_plan_bytes(a.n_seq, a.rows, a.H, a.HKV), "the plan"};
+}
+Span the_ws(const ei::PackedArgs& a, const void* ws) {
+    return {ws, ei::packed_ws_bytes(a.rows, a.H, a.HKV), "the workspace"};
+}
+Span the_mask(const ei::PackedArgs& a) {
+    return {a.mask, (size_t)a.rows * a.mask_words * sizeof(uint32_t), "the mask"};
+}
+Span the_rows(const ei::PackedArgs& a, const void* out, const char* name) {
+    return {out, (size_t)a.rows * a.H * 128 * sizeof(float), name};
+}
+Span the_turns(const ei::PackedArgs& a, const int* turn_at) {
+    return {turn_at, (size_t)a.rows * sizeof(int), "turn_at"};
+}
+
+// The raw rows and what they are normed and turned with.
+int check_raw(const float* qkv, long row_stride, int n_head, int n_head_kv, const float* q_gamma, const float* k_gamma,
+              const float* cs, int n_pos, int rope_dim) {
+    if (int e = check_rope(rope_dim, 128)) return e;
+    REQUIRE(qkv && q_gamma && k_gamma && cs, "null pointer argument");
+    REQUIRE(n_pos > 0, "n_pos %d must be positive", n_pos);
+    REQUIRE(row_stride >= (long)(n_head + 2 * n_head_kv) * 128 && row_stride % 4 == 0 && aligned16(qkv),
+            "qkv must be 16-byte aligned, row_stride %ld a multiple of 4 and >= (H+2*HKV)*head_dim", row_stride);
+    return EI_OK;
+}
+
+constexpr size_t kGammaBytes = 128 * sizeof(float);
+
+}  // namespace
+
+EI_API int ei_cache8_store(ei_stream_t stream, const float* qkv, long row_stride, float* q_out, const ei_cache8* cache,
+                           const int* block_table, int max_blocks, int n_seq, int rows, int n_head, int n_head_kv,
+                           int head_dim, const float* q_gamma, const float* k_gamma, const float* cs, int n_pos,
+                           const int* turn_at, int rope_dim, float eps, const void* plan, size_t plan_bytes) {
+    ei::Cache8Args a{};
+    if (int e = check_cache8(cache, block_table, max_blocks, n_seq, rows, n_head, n_head_kv, head_dim, plan, plan_bytes,
+                             &a))
+        return e;
+    if (int e = check_raw(qkv, row_stride, n_head, n_head_kv, q_gamma, k_gamma, cs, n_pos, rope_dim)) return e;
+    REQUIRE(aligned16(q_out), "q_out must be 16-byte aligned");
+    if (int e = check_apart({the_rows(a, q_out, "q_out"), codes_k(a), codes_v(a), scales_k(a), scales_v(a)},
+                            {{qkv, span_bytes(rows, row_stride, (n_head + 2L * n_head_kv) * 128), "qkv"},
+                             the_table(a), the_plan(a), the_turns(a, turn_at),
+                             {q_gamma, kGammaBytes, "q_gamma"}, {k_gamma, kGammaBytes, "k_gamma"},
+                             {cs, (size_t)n_pos * rope_dim * sizeof(float), "cs"}}))
+        return e;
+    if (rows == 0) return ok();
+    return hip_status(ei::launch_cache8_store(static_cast<hipStream_t>(stream), a, qkv, row_stride, q_out, q_gamma,
+                                              k_gamma, cs, n_pos, turn_at, rope_dim, eps),
+                      "cache8 store launch");
+}
+
+EI_API int ei_cache8_load(ei_stream_t stream, const ei_cache8* cache, const int* block_table, int max_blocks,
+                          float* k_out, float* v_out, long out_stride, int n_seq, int rows, int n_head, int n_head_kv,
+                          int head_dim, const void* plan, size_t plan_bytes) {
+    ei::Cache8Args a{};
+    if (int e = check_cache8(cache, block_table, max_blocks, n_seq, rows, n_head, n_head_kv, head_dim, plan, plan_bytes,
+                             &a))
+        return e;
+    REQUIRE(k_out && v_out && aligned16(k_out) && aligned16(v_out), "k_out or v_out missing or not 16-byte aligned");
+    const long width = (long)n_head_kv * 128;
+    REQUIRE(out_stride >= width && out_stride % 4 == 0, "out_stride %ld must be a multiple of 4 and >= n_head_kv*128",
+            out_stride);
+    // (k_out and v_out may be columns of one buffer)
+    REQUIRE(!rows_overlap(k_out, out_stride, v_out, out_stride, rows, width), "k_out overlaps v_out");
+    const size_t bytes = span_bytes(rows, out_stride, width);
+    for (const Span& w : {Span{k_out, bytes, "k_out"}, Span{v_out, bytes, "v_out"}})
+        if (int e = check_apart({w}, {codes_k(a), codes_v(a), scales_k(a), scales_v(a), the_table(a), the_plan(a)}))
+            return e;
+    if (rows == 0) return ok();
+    return hip_status(ei::launch_cache8_load(static_cast<hipStream_t>(stream), a, k_out, v_out, out_stride),
+                      "cache8 load launch");
+}
+
+EI_API int ei_attn_packed_cache8(ei_stream_t stream, const float* q, long q_stride, float* out, const ei_cache8* cache,
+                                 const int* block_table, int max_blocks, int n_seq, int rows, int n_head,
+                                 int n_head_kv, int head_dim, const uint64_t* mask, int mask_words, float scale,
+                                 const void* plan, size_t plan_bytes, void* ws, size_t ws_bytes) {
+    ei::Cache8Args a{};
+    if (int e = check_cache8(cache, block_table, max_blocks, n_seq, rows, n_head, n_head_kv, head_dim, plan, plan_bytes,
+                             &a))
+        return e;
+    if (int e = check_ws(ws, ws_bytes, rows, n_head, n_head_kv)) return e;
+    if (int e = check_mask(mask, mask_words)) return e;
+    REQUIRE(q && aligned16(q), "q missing or not 16-byte aligned");
+    REQUIRE(q_stride >= (long)n_head * head_dim && q_stride % 4 == 0, "q_stride %ld", q_stride);
+    REQUIRE(out && aligned16(out), "out missing or not 16-byte aligned");
+    a.q = q, a.q_stride = q_stride;
+    a.out = out;
+    a.scale = scale;
+    a.mask = reinterpret_cast<const uint32_t*>(mask), a.mask_words = mask ? 2 * mask_words : 0;
+    if (int e = check_apart({the_rows(a, out, "out"), the_ws(a, ws)},
+                            {{q, span_bytes(rows, q_stride, (long)n_head * head_dim), "q"}, codes_k(a), codes_v(a),
+                             scales_k(a), scales_v(a), the_table(a), the_plan(a), the_mask(a)}))
+        return e;
+    if (rows == 0) return ok();
+    return hip_status(ei::launch_cache8_attn(static_cast<hipStream_t>(stream), a, ws), "cache8 attention launch");
+}
+
+EI_API int ei_packed_step_cache8(ei_stream_t stream, const float* qkv, long row_stride, float* out,
+                                 const ei_cache8* cache, const int* block_table, int max_blocks, int n_seq, int rows,
+                                 int n_head, int n_head_kv, int head_dim, const float* q_gamma, const float* k_gamma,
+                                 const float* cs, int n_pos, const int* turn_at, int rope_dim, float eps,
+                                 const uint64_t* mask, int mask_words, float scale, const void* plan,
+                                 size_t plan_bytes, void* ws, size_t ws_bytes) {
+    ei::Cache8Args a{};
+    if (int e = check_cache8(cache, block_table, max_blocks, n_seq, rows, n_head, n_head_kv, head_dim, plan, plan_bytes,
+                             &a))
+        return e;
+    if (int e = check_raw(qkv, row_stride, n_head, n_head_kv, q_gamma, k_gamma, cs, n_pos, rope_dim)) return e;
+    if (int e = check_ws(ws, ws_bytes, rows, n_head, n_head_kv)) return e;
+    if (int e = check_mask(mask, mask_words)) return e;
+    REQUIRE(out && aligned16(out), "out missing or not 16-byte aligned");
+    a.out = out;
+    a.scale = scale;
+    a.mask = reinterpret_cast<const uint32_t*>(mask), a.mask_words = mask ? 2 * mask_words : 0;
+    if (int e = check_apart({the_rows(a, out, "out"), the_ws(a, ws), codes_k(a), codes_v(a), scales_k(a), scales_v(a)},
+                            {{qkv, span_bytes(rows, row_stride, (n_head + 2L * n_head_kv) * 128), "qkv"},
+                             the_table(a), the_plan(a), the_mask(a), the_turns(a, turn_at),
+                             {q_gamma, kGammaBytes, "q_gamma"}, {k_gamma, kGammaBytes, "k_gamma"},
+                             {cs, (size_t)n_pos * rope_dim * sizeof(float), "cs"}}))
+        return e;
+    if (rows == 0) return ok();
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    float* normed = ei::packed_parts(ws, rows, n_head, n_head_kv).q;
+    if (int e = hip_status(ei::launch_cache8_store(st, a, qkv, row_stride, normed, q_gamma, k_gamma, cs, n_pos, turn_at,
+                                                   rope_dim, eps),
+                           "cache8 store launch"))
+        return e;
+    a.q = normed, a.q_stride = (long)n_head * head_dim;
+    return hip_status(ei::launch_cache8_attn(st, a, ws), "cache8 attention launch");
+}
+
+namespace {
+
+// The fp32 pool and the batch into `a`, after checking both.
+int check_pool_f32(const float* kc, const float* vc, int n_blocks, const int* block_table, int max_blocks,
+                   int block_size, int n_seq, int rows, int n_head, int n_head_kv, int head_dim, const void* plan,
+                   size_t plan_bytes, ei::PackedArgs* a) {
+    if (int e = check_batch(n_seq, rows, n_head, n_head_kv, head_dim, plan, plan_bytes)) return e;
+    REQUIRE(kc && vc, "null pointer argument");
+    REQUIRE(aligned16(kc) && aligned16(vc), "pointers must be 16-byte aligned");
+    if (int e = check_pages(block_table, max_blocks, block_size, n_blocks, &a->bshift)) return e;
+    a->k = kc, a->v = vc, a->kv_stride = (long)n_head_kv * head_dim;
+    a->btab = block_table;
+    a->max_blocks = max_blocks, a->n_blocks = n_blocks;
+    a->n_seq = n_seq, a->rows = rows, a->H = n_head, a->HKV = n_head_kv;
+    a->plan = static_cast<const char*>(plan);
+    return EI_OK;
+}
+
+Span pool_f32(const ei::PackedArgs& a, const float* at, const char* name) {
+    return {at, ((size_t)a.n_blocks << a.bshift) * (size_t)a.HKV * 128 * sizeof(float), name};
+}
+
+}  // namespace
+
+EI_API int ei_attn_tree_paged(ei_stream_t stream, const float* q, long q_stride, float* out, const float* kc,
+                              const float* vc, int n_blocks, const int* block_table, int max_blocks, int block_size,
+                              int n_seq, int rows, int n_head, int n_head_kv, int head_dim, const uint64_t* mask,
+                              int mask_words, float scale, const void* plan, size_t plan_bytes, void* ws,
+                              size_t ws_bytes) {
+    ei::PackedArgs a{};
+    if (int e = check_pool_f32(kc, vc, n_blocks, block_table, max_blocks, block_size, n_seq, rows, n_head, n_head_kv,
+                               head_dim, plan, plan_bytes, &a))
+        return e;
+    if (int e = check_ws(ws, ws_bytes, rows, n_head, n_head_kv)) return e;
+    if (int e = check_mask(mask, mask_words)) return e;
+    REQUIRE(q && aligned16(q), "q missing or not 16-byte aligned");
+    REQUIRE(q_stride >= (long)n_head * head_dim && q_stride % 4 == 0, "q_stride %ld", q_stride);
+    REQUIRE(out && aligned16(out), "out missing or not 16-byte aligned");
+    a.q = q, a.q_stride = q_stride;
+    a.out = out;
+    a.scale = scale;
+    a.mask = reinterpret_cast<const uint32_t*>(mask), a.mask_words = mask ? 2 * mask_words : 0;
+    if (int e = check_apart({the_rows(a, out, "out"), the_ws(a, ws)},
+                            {{q, span_bytes(rows, q_stride, (long)n_head * head_dim), "q"},
+                             pool_f32(a, kc, "the K pool"), pool_f32(a, vc, "the V pool"), the_table(a), the_plan(a),
+                             the_mask(a)}))
+        return e;
+    if (rows == 0) return ok();
+    return hip_status(ei::launch_packed(static_cast<hipStream_t>(stream), a, ws), "tree attention launch");
+}
+
+EI_API int ei_tree_step_paged(ei_stream_t stream, const float* qkv, long row_stride, float* out, float* kc, float* vc,
+                              int n_blocks, const int* block_table, int max_blocks, int block_size, int n_seq,
+                              int rows, int n_head, int n_head_kv, int head_dim, const float* q_gamma,
+                              const float* k_gamma, const float* cs, int n_pos, const int* turn_at, int rope_dim,
+                              float eps, const uint64_t* mask, int mask_words, float scale, const void* plan,
+                              size_t plan_bytes, void* ws, size_t ws_bytes) {
+    ei::PackedArgs a{};
+    if (int e = check_pool_f32(kc, vc, n_blocks, block_table, max_blocks, block_size, n_seq, rows, n_head, n_head_kv,
+                               head_dim, plan, plan_bytes, &a))
+        return e;
+    if (int e = check_raw(qkv, row_stride, n_head, n_head_kv, q_gamma, k_gamma, cs, n_pos, rope_dim)) return e;
+    if (int e = check_ws(ws, ws_bytes, rows, n_head, n_head_kv)) return e;
+    if (int e = check_mask(mask, mask_words)) return e;
+    REQUIRE(out && aligned16(out), "out missing or not 16-byte aligned");
+    a.out = out;
+    a.scale = scale;
+    a.mask = reinterpret_cast<const uint32_t*>(mask), a.mask_words = mask ? 2 * mask_words : 0;
+    if (int e = check_apart({the_rows(a, out, "out"), the_ws(a, ws), pool_f32(a, kc, "the K pool"),
+                             pool_f32(a, vc, "the V pool")},
+                            {{qkv, span_bytes(rows, row_stride, (n_head + 2L * n_head_kv) * 128), "qkv"},
+                             the_table(a), the_plan(a), the_mask(a), the_turns(a, turn_at),
+                             {q_gamma, kGammaBytes, "q_gamma"}, {k_gamma, kGammaBytes, "k_gamma"},
+                             {cs, (size_t)n_pos * rope_dim * sizeof(float), "cs"}}))
+        return e;
+    if (rows == 0) return ok();
+    return hip_status(ei::launch_packed_step(static_cast<hipStream_t>(stream), a, qkv, row_stride, kc, vc, q_gamma,
+                                             k_gamma, cs, n_pos, rope_dim, eps, ws, turn_at),
+                      "tree step launch");
+}
+
+namespace {
+
+int check_kept(const int* kept, int max_kept, const int* n_kept, const int* new_len) {
+    REQUIRE(kept && n_kept && new_len, "null pointer argument");
+    REQUIRE(max_kept > 0 && max_kept <= (1 << 20), "max_kept %d out of range [1, 2^20]", max_kept);
+    return EI_OK;
+}
+
+}  // namespace
+
+EI_API int ei_cache_keep(ei_stream_t stream, float* kc, float* vc, int n_blocks, const int* block_table, int max_blocks,
+                         int block_size, int n_seq, int rows, int n_head, int n_head_kv, int head_dim,
+                         const int* kept, int max_kept, const int* n_kept, int* new_len, const void* plan,
+                         size_t plan_bytes) {
+    ei::Cache8Args a{};
+    if (int e = check_pool_f32(kc, vc, n_blocks, block_table, max_blocks, block_size, n_seq, rows, n_head, n_head_kv,
+                               head_dim, plan, plan_bytes, &a))
+        return e;
+    if (int e = check_kept(kept, max_kept, n_kept, new_len)) return e;
+    if (int e = check_apart({pool_f32(a, kc, "the K pool"), pool_f32(a, vc, "the V pool"),
+                             {new_len, n_seq * sizeof(int), "new_len"}},
+                            {{kept, (size_t)n_seq * max_kept * sizeof(int), "kept"},
+                             {n_kept, n_seq * sizeof(int), "n_kept"}, the_table(a), the_plan(a)}))
+        return e;
+    return hip_status(ei::launch_cache_keep(static_cast<hipStream_t>(stream), a, kc, vc, kept, max_kept, n_kept,
+                                            new_len),
+                      "cache keep launch");
+}
+
+EI_API int ei_cache8_keep(ei_stream_t stream, const ei_cache8* cache, const int* block_table, int max_blocks,
+                          int n_seq, int rows, int n_head, int n_head_kv, int head_dim, const int* kept, int max_kept,
+                          const int* n_kept, int* new_len, const void* plan, size_t plan_bytes) {
+    ei::Cache8Args a{};
+    if (int e = check_cache8(cache, block_table, max_blocks, n_seq, rows, n_head, n_head_kv, head_dim, plan, plan_bytes,
+                             &a))
+        return e;
+    if (int e = check_kept(kept, max_kept, n_kept, new_len)) return e;
+    if (int e = check_apart({codes_k(a), codes_v(a), scales_k(a), scales_v(a),
+                             {new_len, n_seq * sizeof(int), "new_len"}},
+                            {{kept, (size_t)n_seq * max_kept * sizeof(int), "kept"},
+                             {n_kept, n_seq * sizeof(int), "n_kept"}, the_table(a), the_plan(a)}))
+        return e;
+    return hip_status(ei::launch_cache_keep(static_cast<hipStream_t>(stream), a, nullptr, nullptr, kept, max_kept,
+                                            n_kept, new_len),
+                      "cache keep launch");
 }
 
 // ------------------------------------------------------------------ GGUF reader (include/ei_gguf.h)

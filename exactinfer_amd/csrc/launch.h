@@ -178,10 +178,34 @@ struct PackedArgs {
     int n_seq, rows, H, HKV;
     float scale;
     const char* plan;
+    const uint32_t* mask;  // [rows][mask_words] of the new rows' trees (paged), or null: causal
+    int mask_words;
 };
 hipError_t launch_packed(hipStream_t st, const PackedArgs& a, void* ws);
 hipError_t launch_packed_step(hipStream_t st, PackedArgs a, const float* qkv, long row_stride, float* kc, float* vc,
                               const float* q_gamma, const float* k_gamma, const float* cs, int n_pos, int rope_dim,
-                              float eps, void* ws);
+                              float eps, void* ws, const int* turn_at = nullptr);
+// where the parts of cut units go in the workspace, behind the step's queries (wide ones, then few-row ones)
+struct PackedParts {
+    float *q, *wide, *few;
+};
+PackedParts packed_parts(void* ws, int rows, int H, int HKV);
+// the merge of cut units
+hipError_t launch_packed_combine(hipStream_t st, const PackedArgs& a, bool prompts, const PackedParts& parts);
+
+// ------------------------------------------------------------------ cache8.hip
+struct Cache8Args : PackedArgs {  // (k, v and kv_stride are not used: the pool's codes and scales instead)
+    uint8_t *k8, *v8;             // [n_blocks][HKV][block size][128]
+    float *ks, *vs;               // [n_blocks][HKV][block size]
+    bool int8;                    // else e4m3
+};
+hipError_t launch_cache8_store(hipStream_t st, const Cache8Args& a, const float* qkv, long row_stride, float* q_out,
+                               const float* q_gamma, const float* k_gamma, const float* cs, int n_pos,
+                               const int* turn_at, int rope_dim, float eps);
+hipError_t launch_cache8_load(hipStream_t st, const Cache8Args& a, float* k_out, float* v_out, long out_stride);
+hipError_t launch_cache8_attn(hipStream_t st, const Cache8Args& a, void* ws);
+// kc, vc: the fp32 pool, or null: the 8-bit one
+hipError_t launch_cache_keep(hipStream_t st, const Cache8Args& a, float* kc, float* vc, const int* kept, int max_kept,
+                             const int* n_kept, int* new_len);
 
 }  // namespace ei

@@ -2,14 +2,9 @@
 // out over the GPU, the attention kernel over packed prompts or a paged pool, and the step's prologue.
 #include <type_traits>
 
-#include "common.h"
-#include "launch.h"
-#include "planes.h"
+#include "packed.h"
 
 namespace ei {
-
-constexpr int kKT = 32;         // keys per tile
-constexpr int kFewRows = 32;    // a sequence's last unit of up to so many rows: few_pass
 
 // ------------------------------------------------------------------ the plan
 // The query rows of a sequence and KV head are taken flat, row f = token * G + head of the group, and
@@ -44,44 +39,6 @@ constexpr int kFewRows = 32;    // a sequence's last unit of up to so many rows:
 // units), 6 to 8 in a graph; once per forward pass, not per layer.  With many sequences it is the sorting, which looks
 // at every sequence for every unit (in a graph): 256 single tokens 6.5 us, 64 prompts of 32 rows 18, 256 of 64 rows
 // 48, 512 of 64 rows 169, the most there is (kMaxRankWork); beyond, unsorted, 1000 of 64 rows 17, 16000 tokens 85.
-struct Unit {
-    int row0, n, len, u;    // the sequence's first row, rows and keys; the unit's number in it
-    int seq, tiles, pad[2];
-};
-static_assert(sizeof(Unit) == 32, "two 16-byte pieces");
-struct Share {
-    int first, first_tile, last, last_tile;  // on the line: from tile first_tile of unit `first` to last_tile of `last`
-    int merge_end;  // the last share with a part of the unit that begins here and is cut; 0: none does
-    int pad[3];
-    Unit start;     // what this share begins with
-    Unit merge;     // the unit that merge_end speaks of
-};
-static_assert(sizeof(Share) == 96, "six 16-byte pieces");
-struct List {
-    Unit* units;    // dealt units in the order of the deal, then the line
-    Share* shares;  // one per workgroup of a KV head
-};
-struct PlanView {
-    int4* seq;     // first row, rows, keys (kv_len itself, also past max_kv), wide units before this sequence's
-    List wide, few;
-};
-// header words past the shape: rounds of the deal, units dealt, on the wide line, few-row units, max_kv
-enum { kHeadRounds = 6, kHeadDealt = 7, kHeadLine = 8, kHeadFew = 9, kHeadMaxKv = 10 };
-constexpr size_t kPlanSeqAt = 256;
-__host__ __device__ inline long plan_max_wide(int n_seq, int rows, int G) { return (long)rows * G / kUnitRows + n_seq; }
-__host__ __device__ inline size_t plan_wide_at(int n_seq) { return kPlanSeqAt + (size_t)n_seq * sizeof(int4); }
-__host__ __device__ inline size_t plan_few_at(int n_seq, int rows, int G) {
-    return plan_wide_at(n_seq) + (size_t)plan_max_wide(n_seq, rows, G) * sizeof(Unit);
-}
-__host__ __device__ inline size_t plan_shares_at(int n_seq, int rows, int G) {
-    return plan_few_at(n_seq, rows, G) + (size_t)n_seq * sizeof(Unit);
-}
-__device__ __forceinline__ PlanView plan_view(char* plan, int n_seq, int rows, int G, int shares) {
-    Share* at = reinterpret_cast<Share*>(plan + plan_shares_at(n_seq, rows, G));
-    return {reinterpret_cast<int4*>(plan + kPlanSeqAt),
-            {reinterpret_cast<Unit*>(plan + plan_wide_at(n_seq)), at},
-            {reinterpret_cast<Unit*>(plan + plan_few_at(n_seq, rows, G)), at + shares}};
-}
 int packed_shares(int HKV) { return kPackedCus / HKV > 1 ? kPackedCus / HKV : 1; }
 size_t packed_plan_bytes(int n_seq, int rows, int H, int HKV) {
     const size_t b = plan_shares_at(n_seq, rows, H / HKV) + 2 * (size_t)packed_shares(HKV) * sizeof(Share);
@@ -347,28 +304,6 @@ __global__ __launch_bounds__(kPlanThreads) void k_packed_plan(const int* __restr
     }
 }
 
-// Whether the plan is one of this call's batch (and of whole prompts, where the keys are the rows).
-__device__ __forceinline__ bool plan_fits(const char* plan, int n_seq, int rows, int H, int HKV, bool prompts) {
-    const int* h = reinterpret_cast<const int*>(plan);
-    return (h[0] == kPlanMagic) & (h[1] == n_seq) & (h[2] == rows) & (h[3] == H) & (h[4] == HKV) &
-           (!prompts | (h[5] != 0));
-}
-
-// The sequence that owns row b: the last whose first row is not past it, if it has that row; else -1.
-// 64 probes at a time, one per lane.
-__device__ __forceinline__ int row_owner(const int4* seq, int n_seq, int b, int lane) {
-    int lo = 0, n = n_seq;
-    while (n > 1) {
-        const int step = (n + 63) >> 6, s = lo + lane * step;
-        const uint64_t le = __builtin_amdgcn_ballot_w64(lane * step < n && seq[min(s, n_seq - 1)].x <= b);
-        const int k = le ? 63 - __builtin_clzll(le) : 0;
-        lo += k * step;
-        n = min(step, n - k * step);
-    }
-    const int4 e = seq[lo];
-    return b >= e.x && b < e.x + e.y ? lo : -1;
-}
-
 // ------------------------------------------------------------------ attention
 // Wide units multiply on v_mfma_f32_32x32x16_f16 with every fp32 operand in two binary16 planes, x = h + l:
 // h = f16(x) and l = f16(x - h), after a scaling by a power of two that brings the largest of its fellows
@@ -417,11 +352,6 @@ __device__ __forceinline__ int row_owner(const int4* seq, int n_seq, int b, int 
 // the same rows and a tile of its own, loaded straight into the operands' registers, and multiplies in
 // fp32, which needs no planes.  (Both kinds of pass in one loop leave the compiler short of registers in
 // both: a workgroup walks its wide units first, then its few-row ones.)
-typedef __amdgpu_buffer_rsrc_t Rsrc;
-constexpr int kQB = 32;                         // flat rows per wave
-constexpr int kSlots = kUnitRows / kQB;         // waves per key group
-constexpr int kGroups = 2;                      // key groups per workgroup
-constexpr int kWaves = kSlots * kGroups;
 // lazy-rescale thresholds (log2 units): sums are rescaled when the running maximum has risen by more (for
 // wide units, what a weight may pass 1 by comes off the range of its planes)
 constexpr float kLazy = 1.f, kFewLazy = 8.f;
@@ -435,7 +365,6 @@ constexpr int kTopSum = 64;
 constexpr uint32_t kMostQ = 127 + 121, kMostK = 127 + 100, kMostQK = 2 * 127 + 10;
 constexpr float kPBits = 14.f;                  // wide units' weights and sums are times 2^kPBits
 constexpr int kXchF = 34;                       // floats per lane exchanged by the merge
-constexpr int kRowF = kHeadDim + 4;             // padded fp32 row of the staging area
 // plane rows padded to an odd number of 16-byte pieces: the rows that an operand read takes, one per
 // lane, spread over all LDS banks
 constexpr int kKRowB = 2 * kHeadDim + 16, kKPlane = kKT * kKRowB;  // K plane: [32 keys][128 d] binary16
@@ -456,42 +385,6 @@ static_assert(kGroups * 2 * kKPlane <= kStageF * 4, "K planes below the staging 
 static_assert(kStageF * 4 + kGroups * 2 * kVPlane <= kScaleK * 4, "V planes within the LDS span");
 static_assert(kWideF * 4 <= 160 * 1024 && kFewF * 4 <= 160 * 1024, "LDS budget");
 
-__device__ __forceinline__ int scalar(int x) { return __builtin_amdgcn_readfirstlane(x); }
-
-// The lane's number, made where it is used (two instructions; kept, it would be spilled and come back by a
-// load that waits for every load before it).
-__device__ __forceinline__ uint32_t lane_now() {
-    uint32_t zero = 0;
-    asm volatile("" : "+v"(zero));
-    return __builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, zero));
-}
-
-// A pass, all of it wave-uniform.
-struct Pass {
-    int seq, u;            // sequence, unit of the sequence
-    int row0, pos0;        // first row of the sequence and its position (may be negative)
-    int nflat;             // the sequence's flat rows of this KV head
-    int T;                 // keys that the unit's last row sees
-    int kt_lo, nrange;     // tiles [kt_lo, kt_lo + nrange)
-    float* part;           // where its unnormalised rows go, or null: a whole unit
-};
-
-// What earlier launches wrote and this one only reads, at a wave-uniform address, by a scalar load: after the
-// kernel's own stores the compiler would take a vector load, whose wait is for every load before it too.
-template <typename T>
-__device__ __forceinline__ T scalar_load(const T* at) {
-    return *reinterpret_cast<const __attribute__((address_space(4))) T*>(reinterpret_cast<uintptr_t>(at));
-}
-
-// The pool block of the page that holds key t0 of the pass's sequence, -1 past the table's end.
-template <bool kPaged>
-__device__ __forceinline__ int page_of(const PackedArgs& a, const Pass& p, int t0) {
-    if constexpr (!kPaged) return 0;
-    const int blk = t0 >> a.bshift;
-    const int e = scalar_load(a.btab + (size_t)p.seq * a.max_blocks + min(blk, a.max_blocks - 1));
-    return blk < a.max_blocks ? e : -1;
-}
-
 // The visible rows of a tile as a buffer: reads past the last one, and of a missing page, give zeros (all
 // reads, if the tile is not `wanted`).
 template <bool kPaged>
@@ -507,13 +400,6 @@ __device__ __forceinline__ Rsrc tile_rsrc(const PackedArgs& a, const Pass& p, co
     return __builtin_amdgcn_make_buffer_rsrc(
         const_cast<float*>(cache) + row * a.kv_stride, 0,
         there ? (int)((uint32_t)(there - 1) * (uint32_t)(a.kv_stride * 4) + kHeadDim * 4) : 0, kBufferDword3);
-}
-
-// A workgroup's parts in its kernel's share of the workspace: slot 0 of the unit that it goes on with, slot 1
-// of the one that it begins; O rows, then (m, l) of each.
-constexpr size_t kWidePart = kUnitRows * (kHeadDim + 2), kFewPart = kFewRows * (kHeadDim + 2);
-__device__ __forceinline__ size_t part_at(bool few, int block, int slot) {
-    return (size_t)(2 * block + slot) * (few ? kFewPart : kWidePart);
 }
 
 struct Sums {  // of 32 rows, one per lane and its lane ^ 32: O^T, their reference (log2 units), sum of weights
@@ -545,14 +431,21 @@ __device__ __forceinline__ float moved(float from, float to) {  // a sum's facto
 // Scores s of tile kt (times sq: log2 units) -> P (in place; with planes times 2^kPBits) and its sum; O rescaled if the
 // reference moves: to the tile's maximum, if that is higher by more than kLazy, and with planes down towards it
 // (kWindow).  Tiles from nfull on cross the diagonal of the wave's rows.  The wave's i-th tile.
-template <bool kPlanes>
-__device__ __forceinline__ void softmax_tile(Sums& x, floatx16& s, float sq, int kt, int nfull, int qpos, int hh,
-                                             Before& before, int i) {
+template <bool kPlanes, bool kTree>
+__device__ __forceinline__ void softmax_tile(const PackedArgs& a, const Pass& p, Sums& x, floatx16& s, float sq, int kt,
+                                             int nfull, int qpos, int hh, Before& before, int i) {
     if (kt >= nfull) {
-        const int k0 = unhoisted(kt * kKT + 4 * hh);
+        if constexpr (kTree) {
+            const uint32_t bits = tree_bits(a, p, qpos, kt * kKT) >> (4 * hh);
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-            if (k0 + 8 * (r >> 2) + (r & 3) > qpos) s[r] = -INFINITY;
+            for (int r = 0; r < 16; ++r)
+                if (!(bits >> (8 * (r >> 2) + (r & 3)) & 1)) s[r] = -INFINITY;
+        } else {
+            const int k0 = unhoisted(kt * kKT + 4 * hh);
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (k0 + 8 * (r >> 2) + (r & 3) > qpos) s[r] = -INFINITY;
+        }
     }
     float mx = s[0];
 #pragma unroll
@@ -602,18 +495,9 @@ __device__ __forceinline__ void softmax_tile(Sums& x, floatx16& s, float sq, int
 }
 
 // ---- two binary16 planes
-typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 struct Halves {  // eight values: one MFMA operand per plane
     u32x4 h, l;
 };
-__device__ __forceinline__ void split_f16(float a, float b, uint32_t& h, uint32_t& l) {
-    h = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
-    float ra, rb;  // a - h's low half, b - its high half, in one instruction each
-    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(ra) : "v"(h), "v"(a));
-    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(rb) : "v"(h), "v"(b));
-    l = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{ra, rb}, f16x2));
-}
 __device__ __forceinline__ floatx16 mfma_f16(u32x4 a, u32x4 b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
                                                   0);
@@ -623,15 +507,6 @@ __device__ __forceinline__ void mfma_halves(const Halves& a, const Halves& b, fl
     c = mfma_f16(a.h, b.l, c);
     c = mfma_f16(a.h, b.h, c);
 }
-// The power of two that brings `most` to 2^kTop .. 2^(kTop+1), and its inverse: `most`'s exponent (biased) is kept
-// where both are normal numbers, and up to `limit`: planes of what passes that by two overflow to infinities, their
-// products to NaN, and the waves that meet them take their keys again in fp32.
-template <int kTop>
-__device__ __forceinline__ uint32_t scale_to(float most, uint32_t limit = 254) {
-    const uint32_t e = min(max(__float_as_uint(most) >> 23, kTop + 2u), limit);
-    return (254u + kTop - e) << 23;
-}
-__device__ __forceinline__ float inverse(uint32_t scale) { return __uint_as_float(0x7F000000u - scale); }
 constexpr uint32_t kNoScale = 253u << 23;  // of columns that have been zero so far
 
 // The planes of P's half x (registers 8x .. 8x + 7): the B operand of two steps' worth of keys.
@@ -684,7 +559,7 @@ __device__ __forceinline__ bool planes_failed(Sums& x, const uint32_t (&scale)[4
 // value that a row does not see must not be multiplied at all (0 times infinity), and the matrix
 // instruction takes every row with every key: P . V goes key by key there, P through p_lds, 32 x 32
 // floats of the wave's own.
-template <typename KTile, typename VTile, typename Index>
+template <bool kTree, typename KTile, typename VTile, typename Index>
 __device__ __forceinline__ void redo_fp32(Sums& x, const PackedArgs& a, const Pass& p, const float* q_row, float sl2,
                                           int n_mine, KTile k_tile, VTile v_tile, Index index, int nfull, int qpos,
                                           uint32_t row_bytes, float* p_lds, int lane) {
@@ -717,7 +592,7 @@ __device__ __forceinline__ void redo_fp32(Sums& x, const PackedArgs& a, const Pa
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
-        softmax_tile<false>(x, s, 1.f, kt, nfull, qpos, hh, before, i);
+        softmax_tile<false, kTree>(a, p, x, s, 1.f, kt, nfull, qpos, hh, before, i);
         const Rsrc rs = v_tile(i);
         if (kt < nfull) {
             const uint32_t off = unhoisted(4 * hh) * row_bytes + 4u * col;
@@ -738,11 +613,13 @@ __device__ __forceinline__ void redo_fp32(Sums& x, const PackedArgs& a, const Pa
 #pragma unroll
         for (int r = 0; r < 16; ++r) pw[32 * (8 * (r >> 2) + 4 * (ln >> 5) + (r & 3))] = s[r];
         __builtin_amdgcn_wave_barrier();
+        uint32_t bits = 0;
+        if constexpr (kTree) bits = tree_bits(a, p, qpos, kt * kKT);
 #pragma unroll 1
         for (int key = 0; key < kKT; ++key) {
             const float pk = pw[32 * key];
             const uint32_t off = key * row_bytes + 16u * (ln >> 5);
-            if (kt * kKT + key <= qpos) {
+            if (kTree ? (bits >> key & 1) != 0 : kt * kKT + key <= qpos) {
 #pragma unroll
                 for (int db = 0; db < 4; ++db) {
 #pragma unroll
@@ -762,7 +639,7 @@ __device__ __forceinline__ void redo_fp32(Sums& x, const PackedArgs& a, const Pa
 }
 
 // ---- a wide unit
-template <bool kPaged>
+template <bool kPaged, bool kTree>
 __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, int kvh, FastDiv fG, float sl2,
                                           float* smem) {
     constexpr int D = kHeadDim;
@@ -784,7 +661,8 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
     const int f0 = kUnitRows * p.u + kQB * hw;  // this wave's first row
     const bool live = f0 < p.nflat;
     const int qpos = p.pos0 + fdiv(min(f0 + col, p.nflat - 1), fG);  // this lane's query
-    const int nfull = max(p.pos0 + fdiv(min(f0, p.nflat - 1), fG) + 1, 0) / kKT;  // tiles below the wave's diagonal
+    // tiles below the wave's diagonal (before a tree)
+    const int nfull = max(kTree ? p.pos0 : p.pos0 + fdiv(min(f0, p.nflat - 1), fG) + 1, 0) / kKT;
     const int n_it = (p.nrange + kGroups - 1) / kGroups, n_mine = (p.nrange - grp + kGroups - 1) / kGroups;
     auto index = [&](int i) { return p.kt_lo + kGroups * i + grp; };
     auto page = [&](int i) { return page_of<kPaged>(a, p, index(i) * kKT); };
@@ -980,7 +858,7 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
                     scale[db] = now;
                 }
             }
-            softmax_tile<true>(x, s, sq, index(i), nfull, qpos, hh, before, i);
+            softmax_tile<true, kTree>(a, p, x, s, sq, index(i), nfull, qpos, hh, before, i);
             // O^T += V^T . P^T, while K(i+1) goes to its planes; then V(i+1) is fetched
             const bool more = i + 1 < n_mine;
             Halves vf[2], pp;
@@ -1005,7 +883,7 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
     if (planes_failed(x, scale, __builtin_fmaf(before.at[kTiles], by, (float)(n_mine - before.from))) && live) {
         const int f = min(f0 + col, p.nflat - 1), t0 = fdiv(f, fG);
         const float* q_row = a.q + ((size_t)p.row0 + t0) * a.q_stride + (size_t)(kvh * G + f - t0 * G) * D;
-        redo_fp32(
+        redo_fp32<kTree>(
             x, a, p, q_row, sl2, n_mine, [&](int i) { return k_tile(i, page(i)); },
             [&](int i) { return v_tile(i, page(i)); }, index, nfull, qpos, row_bytes,
                   smem + w * (kXchF * 64), lane);
@@ -1033,7 +911,9 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
     const float l = half_sum(x.l * c0 + lp * cp);
     {
         // finished rows (normalised; a row that sees no key: zeros), or the part's, to the staging area
-        const float inv = p.part ? 1.f : qpos < 0 ? 0.f : 1.f / l;
+        bool none = qpos < 0;
+        if constexpr (kTree) none = l == 0.f && tree_sees_none(a, p.row0, p.pos0, qpos - p.pos0);
+        const float inv = p.part ? 1.f : none ? 0.f : 1.f / l;
         float* ost = stage + (hw * kQB + col) * kRowF + 64 * grp + 4 * hh;
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
@@ -1083,7 +963,7 @@ __device__ __forceinline__ void wide_pass(const PackedArgs& a, const Pass& p, in
 // By rows (H 32 / HKV 8, 32 sequences of 480 keys, with the merge): four 26.2 us (27.1 as sixteen), sixteen 27
 // (37 as 32), twenty 32.3 (35.5 as 32), 32 rows 36 (44 as a wide unit; of 4067 keys 192 against 297; single
 // tokens as wide units 44, and of 4059 keys 290 against 179).
-template <bool kPaged, int kBlocks, bool kQuad>
+template <bool kPaged, bool kTree, int kBlocks, bool kQuad>
 __device__ __forceinline__ void few_pass(const PackedArgs& a, const Pass& p, int kvh, FastDiv fG, float sl2,
                                          float* smem) {
     constexpr int D = kHeadDim, kSets = kBlocks + kQuad, kRows = kFewBlock * kBlocks + 4 * kQuad;
@@ -1092,7 +972,7 @@ __device__ __forceinline__ void few_pass(const PackedArgs& a, const Pass& p, int
     const int G = (int)fG.d;
     const uint32_t row_bytes = (uint32_t)(a.kv_stride * 4);
     const int f0 = kUnitRows * p.u, last = p.nflat - 1, rows = p.nflat - f0;
-    const int nfull = max(p.pos0 + fdiv(f0, fG) + 1, 0) / kKT;
+    const int nfull = max(kTree ? p.pos0 : p.pos0 + fdiv(f0, fG) + 1, 0) / kKT;
     const int n_mine = (p.nrange - wu + kWaves - 1) / kWaves;
     auto index = [&](int i) { return p.kt_lo + kWaves * i + wu; };
     auto page = [&](int i) { return page_of<kPaged>(a, p, index(i) * kKT); };
@@ -1217,10 +1097,17 @@ __device__ __forceinline__ void few_pass(const PackedArgs& a, const Pass& p, int
                 }
             }
             if (kt >= nfull) {
-                const int k0 = unhoisted(kt * kKT + 4 * quarter);
+                if constexpr (kTree) {
+                    const uint32_t bits = tree_bits(a, p, qpos[rb], kt * kKT) >> (4 * quarter);
 #pragma unroll
-                for (int r = 0; r < 8; ++r)
-                    if (k0 + 16 * (r >> 2) + (r & 3) > qpos[rb]) s[rb][r >> 2][r & 3] = -INFINITY;
+                    for (int r = 0; r < 8; ++r)
+                        if (!(bits >> (16 * (r >> 2) + (r & 3)) & 1)) s[rb][r >> 2][r & 3] = -INFINITY;
+                } else {
+                    const int k0 = unhoisted(kt * kKT + 4 * quarter);
+#pragma unroll
+                    for (int r = 0; r < 8; ++r)
+                        if (k0 + 16 * (r >> 2) + (r & 3) > qpos[rb]) s[rb][r >> 2][r & 3] = -INFINITY;
+                }
             }
             float mx = s[rb][0][0];
 #pragma unroll
@@ -1283,7 +1170,9 @@ __device__ __forceinline__ void few_pass(const PackedArgs& a, const Pass& p, int
                     const int at = page(c / kKT);
                     const Rsrc rk = k_tile(c / kKT, at), rv = v_tile(c / kKT, at);
                     const uint32_t row = (uint32_t)(c % kKT) * row_bytes;
-                    if (index(c / kKT) * kKT + c % kKT > qpos[rb]) continue;
+                    if constexpr (kTree) {
+                        if (!(tree_bits(a, p, qpos[rb], index(c / kKT) * kKT) >> (c % kKT) & 1)) continue;
+                    } else if (index(c / kKT) * kKT + c % kKT > qpos[rb]) continue;
                     float dot = 0.f;
 #pragma unroll
                     for (int x = 0; x < 8; ++x) {
@@ -1380,60 +1269,36 @@ __device__ __forceinline__ void few_pass(const PackedArgs& a, const Pass& p, int
             if (d == 0) *reinterpret_cast<float2*>(p.part + kFewRows * D + 2 * row) = make_float2(M, L);
         } else {
             dst = a.out + (((size_t)p.row0 + t0) * a.H + kvh * G + g - t0 * G) * D;
-            const float inv = p.pos0 + t0 < 0 ? 0.f : 1.f / L;  // a row that sees no key: zeros
+            bool none = p.pos0 + t0 < 0;  // a row that sees no key: zeros
+            if constexpr (kTree) none = L == 0.f && tree_sees_none(a, p.row0, p.pos0, t0);
+            const float inv = none ? 0.f : 1.f / L;
             x.x *= inv, x.y *= inv, x.z *= inv, x.w *= inv;
         }
         *reinterpret_cast<float4*>(dst + d) = x;
     }
 }
 
-// A workgroup's part of a list: `sh` its share of the line (first unit, first tile, last unit, last tile), before
-// it `rounds` whole units.
-template <bool kPaged, bool kFew>
+// A workgroup's part of a list.
+template <bool kPaged, bool kTree, bool kFew>
 __device__ __forceinline__ void walk_list(const PackedArgs& a, const List& list, int4 sh, int rounds, int shares,
                                           int share, int kvh, float* parts, float* smem) {
     const FastDiv fG = fast_div((uint32_t)(a.H / a.HKV));
     const float sl2 = a.scale * 1.44269504088896340736f;  // scores come out in log2 units
-    const int dealt = rounds * shares;
-    const int first = scalar(sh.x), first_tile = scalar(sh.y), last = scalar(sh.z), last_tile = scalar(sh.w);
-    for (int pass = 0;; ++pass) {
-        int at, cut = -1;
-        Pass p;
-        p.kt_lo = 0;
-        if (pass < rounds) {
-            at = pass * shares + ((pass & 1) ? shares - 1 - share : share);
-        } else {
-            const int i = first + pass - rounds;
-            if (i > last || (i == last && last_tile == 0)) break;
-            at = dealt + i;
-            cut = i == last ? last_tile : -1;
-            p.kt_lo = i == first ? first_tile : 0;
-        }
-        // (the share's own copy comes with the line just read: no wait for a list entry)
-        const u32x4* unit = reinterpret_cast<const u32x4*>(pass == 0 ? &list.shares[share].start : list.units + at);
-        const u32x4 x = scalar_load(unit), y = scalar_load(unit + 1);  // a Unit's fields, in order
-        const int n = (int)x.y, len = (int)x.z;
-        p.row0 = (int)x.x, p.u = (int)x.w, p.seq = (int)y.x;
-        p.pos0 = len - n;
-        p.nflat = n * (int)fG.d;
-        p.T = min(max(p.pos0 + fdiv(min(kUnitRows * p.u + kUnitRows, p.nflat) - 1, fG) + 1, 0), len);
-        p.nrange = (cut >= 0 ? cut : (int)y.y) - p.kt_lo;
-        p.part = p.kt_lo > 0 || cut >= 0 ? parts + part_at(kFew, share * a.HKV + kvh, p.kt_lo > 0 ? 0 : 1) : nullptr;
-        if (pass > 0) lds_barrier();  // the last pass's rows have been read
+    walk_share<kFew>(a, list, sh, rounds, shares, share, kvh, fG, parts, [&](const Pass& p) {
         if constexpr (kFew) {
             const int rows = p.nflat - kUnitRows * p.u;
             // (up to so many rows: the fewest matrix instructions that hold them)
-            if (rows <= 4) few_pass<kPaged, 0, true>(a, p, kvh, fG, sl2, smem);
-            else if (rows <= kFewBlock) few_pass<kPaged, 1, false>(a, p, kvh, fG, sl2, smem);
-            else if (rows <= kFewBlock + 4) few_pass<kPaged, 1, true>(a, p, kvh, fG, sl2, smem);
-            else few_pass<kPaged, kFewRows / kFewBlock, false>(a, p, kvh, fG, sl2, smem);
-        } else wide_pass<kPaged>(a, p, kvh, fG, sl2, smem);
-    }
+            if (rows <= 4) few_pass<kPaged, kTree, 0, true>(a, p, kvh, fG, sl2, smem);
+            else if (rows <= kFewBlock) few_pass<kPaged, kTree, 1, false>(a, p, kvh, fG, sl2, smem);
+            else if (rows <= kFewBlock + 4) few_pass<kPaged, kTree, 1, true>(a, p, kvh, fG, sl2, smem);
+            else few_pass<kPaged, kTree, kFewRows / kFewBlock, false>(a, p, kvh, fG, sl2, smem);
+        } else wide_pass<kPaged, kTree>(a, p, kvh, fG, sl2, smem);
+    });
 }
 
 // grid shares x KV heads (a KV head's workgroups share an XCD's L2): each workgroup's part of the wide list, then of
 // the few-row list.  The plan's header and both shares are read before anything waits for them.
-template <bool kPaged>
+template <bool kPaged, bool kTree>
 __global__ __launch_bounds__(64 * kWaves) void k_packed_attn(PackedArgs a, int shares, float* __restrict__ wide_parts,
                                                              float* __restrict__ few_parts) {
     extern __shared__ __align__(16) float smem[];
@@ -1443,9 +1308,9 @@ __global__ __launch_bounds__(64 * kWaves) void k_packed_attn(PackedArgs a, int s
     const int4 wide = *reinterpret_cast<const int4*>(pv.wide.shares + share);
     const int4 few = *reinterpret_cast<const int4*>(pv.few.shares + share);
     if (!plan_fits(a.plan, a.n_seq, a.rows, a.H, a.HKV, !kPaged)) return;
-    walk_list<kPaged, false>(a, pv.wide, wide, rounds, shares, share, kvh, wide_parts, smem);
+    walk_list<kPaged, kTree, false>(a, pv.wide, wide, rounds, shares, share, kvh, wide_parts, smem);
     lds_barrier();  // the last wide pass's rows have been read
-    walk_list<kPaged, true>(a, pv.few, few, 0, shares, share, kvh, few_parts, smem);
+    walk_list<kPaged, kTree, true>(a, pv.few, few, 0, shares, share, kvh, few_parts, smem);
 }
 
 // The units that the cuts divide.  Part p of a unit is slot 1 of the share that it begins in, then slot 0 of each share
@@ -1540,7 +1405,9 @@ __global__ __launch_bounds__(32 * kCombineRows) void k_packed_combine(PackedArgs
             o.z = __builtin_fmaf(o.z, c, sum.z), o.w = __builtin_fmaf(o.w, c, sum.w);
         }
         const int t0 = f / G;
-        const float inv = m.x.len - m.x.n + t0 < 0 ? 0.f : 1.f / L;  // a row that sees no key: zeros
+        const int pos0 = m.x.len - m.x.n;  // a row that sees no key: zeros
+        const bool none = a.mask ? L == 0.f && tree_sees_none(a, m.x.row0, pos0, t0) : pos0 + t0 < 0;
+        const float inv = none ? 0.f : 1.f / L;
         *reinterpret_cast<float4*>(a.out + (((size_t)m.x.row0 + t0) * a.H + kvh * G + f - t0 * G) * kHeadDim + d) =
             make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
     }
@@ -1559,7 +1426,7 @@ __global__ __launch_bounds__(256) void k_packed_prepare(const float* __restrict_
                                                         const float* __restrict__ q_gamma,
                                                         const float* __restrict__ k_gamma,
                                                         const float2* __restrict__ cs, int n_pos, int rope_dim,
-                                                        float eps) {
+                                                        float eps, const int* __restrict__ turn_at) {
     __shared__ float scratch[4][kHeadDim];
     const int b = blockIdx.x, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int H = a.H, HKV = a.HKV, NH = H + HKV;
@@ -1587,12 +1454,13 @@ __global__ __launch_bounds__(256) void k_packed_prepare(const float* __restrict_
     if (s < 0) return;
     const int4 e = seq[s];
     const int pos = e.z - e.y + (b - e.x);
-    const bool in = pos >= 0 && pos < min(n_pos, reinterpret_cast<const int*>(a.plan)[kHeadMaxKv]);
+    const int turn = turn_at ? turn_at[b] : pos;
+    const bool in = pos >= 0 && pos < reinterpret_cast<const int*>(a.plan)[kHeadMaxKv] && turn >= 0 && turn < n_pos;
     const int blk = pos >> a.bshift;
     const int phys = in && blk < a.max_blocks ? a.btab[(size_t)s * a.max_blocks + blk] : -1;
     const bool there = phys >= 0 && phys < a.n_blocks;
     const size_t crow = ((size_t)(there ? phys : 0) << a.bshift) | (size_t)(pos & ((1 << a.bshift) - 1));
-    const float2* cs_row = cs + (size_t)(in ? pos : 0) * (rope_dim >> 1);
+    const float2* cs_row = cs + (size_t)(in ? turn : 0) * (rope_dim >> 1);
     const float qg0 = q_gamma[lane], qg1 = q_gamma[lane + 64];
     const float kg0 = k_gamma[lane], kg1 = k_gamma[lane + 64];
     head_inv<kPrepHeads>(x0, x1, eps, inv, lane);
@@ -1635,33 +1503,45 @@ size_t packed_ws_bytes(int rows, int H, int HKV) {
     return q_bytes(rows, H) + (size_t)packed_shares(HKV) * HKV * 2 * (kWidePart + kFewPart) * sizeof(float);
 }
 
-template <bool kPaged>
-static hipError_t launch_packed_attn(hipStream_t st, const PackedArgs& a, int shares, float* wide, float* few) {
+PackedParts packed_parts(void* ws, int rows, int H, int HKV) {
+    float* wide = reinterpret_cast<float*>(static_cast<char*>(ws) + q_bytes(rows, H));
+    return {static_cast<float*>(ws), wide, wide + (size_t)packed_shares(HKV) * HKV * 2 * kWidePart};
+}
+
+template <bool kPaged, bool kTree>
+static hipError_t launch_packed_attn(hipStream_t st, const PackedArgs& a, int shares, const PackedParts& parts) {
     static std::atomic<bool> opted;
     constexpr size_t lds = (size_t)(kWideF > kFewF ? kWideF : kFewF) * sizeof(float);
-    if (const hipError_t e = opt_in_lds(opted, (const void*)k_packed_attn<kPaged>, lds); e != hipSuccess) return e;
-    k_packed_attn<kPaged><<<shares * a.HKV, 64 * kWaves, lds, st>>>(a, shares, wide, few);
+    if (const hipError_t e = opt_in_lds(opted, (const void*)k_packed_attn<kPaged, kTree>, lds); e != hipSuccess)
+        return e;
+    k_packed_attn<kPaged, kTree><<<shares * a.HKV, 64 * kWaves, lds, st>>>(a, shares, parts.wide, parts.few);
+    return hipGetLastError();
+}
+
+hipError_t launch_packed_combine(hipStream_t st, const PackedArgs& a, bool prompts, const PackedParts& parts) {
+    const int wgs = kCombineWgs / a.HKV > 1 ? kCombineWgs / a.HKV : 1;
+    k_packed_combine<<<wgs * a.HKV, 32 * kCombineRows, 0, st>>>(a, prompts, packed_shares(a.HKV), wgs, parts.wide,
+                                                               parts.few);
     return hipGetLastError();
 }
 
 hipError_t launch_packed(hipStream_t st, const PackedArgs& a, void* ws) {
     const int shares = packed_shares(a.HKV);
-    float* wide = reinterpret_cast<float*>(static_cast<char*>(ws) + q_bytes(a.rows, a.H));
-    float* few = wide + (size_t)shares * a.HKV * 2 * kWidePart;
-    const hipError_t e = a.btab ? launch_packed_attn<true>(st, a, shares, wide, few)
-                                : launch_packed_attn<false>(st, a, shares, wide, few);
+    const PackedParts parts = packed_parts(ws, a.rows, a.H, a.HKV);
+    const hipError_t e = !a.btab ? launch_packed_attn<false, false>(st, a, shares, parts)
+                         : a.mask ? launch_packed_attn<true, true>(st, a, shares, parts)
+                                  : launch_packed_attn<true, false>(st, a, shares, parts);
     if (e != hipSuccess) return e;
-    const int wgs = kCombineWgs / a.HKV > 1 ? kCombineWgs / a.HKV : 1;
-    k_packed_combine<<<wgs * a.HKV, 32 * kCombineRows, 0, st>>>(a, a.btab == nullptr, shares, wgs, wide, few);
-    return hipGetLastError();
+    return launch_packed_combine(st, a, a.btab == nullptr, parts);
 }
 
 hipError_t launch_packed_step(hipStream_t st, PackedArgs a, const float* qkv, long row_stride, float* kc, float* vc,
                               const float* q_gamma, const float* k_gamma, const float* cs, int n_pos, int rope_dim,
-                              float eps, void* ws) {
+                              float eps, void* ws, const int* turn_at) {
     float* q = static_cast<float*>(ws);
     k_packed_prepare<<<dim3(a.rows, (a.H + a.HKV + 15) / 16), 256, 0, st>>>(
-        qkv, row_stride, q, a, kc, vc, q_gamma, k_gamma, reinterpret_cast<const float2*>(cs), n_pos, rope_dim, eps);
+        qkv, row_stride, q, a, kc, vc, q_gamma, k_gamma, reinterpret_cast<const float2*>(cs), n_pos, rope_dim, eps,
+        turn_at);
     if (const hipError_t e = hipGetLastError(); e != hipSuccess) return e;
     a.q = q;
     a.q_stride = (long)a.H * kHeadDim;
