@@ -589,6 +589,401 @@ __device__ __forceinline__ void rows_pass(const Cache8Args& a, const Pass& p, in
     }
 }
 
+// ---- a wide unit: up to 128 rows
+// Two key groups of four waves; a group's waves hold 32 rows each and share its tiles (tile kt to group
+// (kt - first) % 2), whose codes each wave turns a quarter of into binary16 in LDS, V transposed, two tiles of a
+// group at a time there, one barrier a tile.  On v_mfma_f32_32x32x16_f16 S^T[key][row] = K . Q^T gives a lane 16 of a
+// tile's 32 keys for one row, which are the operand of O^T[d][row] = V^T . P^T.  The two waves of a SIMD
+// are of different groups, and the second group's iteration begins with the softmax: one has matrix work while the
+// other has not.
+constexpr int kK8RowB = 2 * kHeadDim + 16, kK8Tile = kKT * kK8RowB;  // [32 keys][128 d] binary16, rows spread over banks
+constexpr int kV8RowB = 2 * kKT + 16, kV8Tile = kHeadDim * kV8RowB;  // [128 d][32 keys]
+constexpr int kScales8 = 2 * kKT * 4 + 16;                          // of K, of V; a word per wave: NaN among its codes
+constexpr int kBuf8 = kK8Tile + kV8Tile + kScales8;                 // one tile of a group
+static_assert(kBuf8 % 16 == 0, "16-byte pieces");
+constexpr int kXch8 = 34;                                           // floats per lane exchanged by the merge
+constexpr int kStage8 = kWaves * kXch8 * 64;                        // then the unit's rows
+constexpr int kWide8F = kStage8 + kUnitRows * kRowF;
+static_assert(4 * kBuf8 <= kWide8F * 4, "the tiles lie below the merge's areas");
+static_assert(kWide8F * 4 <= 160 * 1024 && kFew8F <= kWide8F, "LDS budget");
+__device__ __forceinline__ floatx16 mfma32(u32x4 a, u32x4 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
+                                                  0);
+}
+
+template <bool kInt8, bool kTree>
+__device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, int kvh, FastDiv fG, float sl2,
+                                           float* smem) {
+    constexpr int D = kHeadDim;
+    const int tid = unhoisted(threadIdx.x), lane = tid & 63, w = tid >> 6;
+    const int wu = scalar(w), hw = wu % kSlots, grp = wu / kSlots;
+    const int col = lane & 31, hh = lane >> 5;
+    const int G = (int)fG.d;
+    char* const lds = reinterpret_cast<char*>(smem) + grp * (2 * kBuf8);
+    const int f0 = kUnitRows * p.u + kQB * hw;  // this wave's first row
+    const int row = min(f0 + col, p.nflat - 1), tok = fdiv(row, fG);  // (rows past the last repeat it)
+    const int qpos = p.pos0 + tok;
+    const int nfull = max(kTree ? p.pos0 : p.pos0 + fdiv(min(f0, p.nflat - 1), fG) + 1, 0) / kKT;
+    const int n_it = (p.nrange + kGroups - 1) / kGroups, n_mine = (p.nrange - grp + kGroups - 1) / kGroups;
+    auto index = [&](int i) { return p.kt_lo + kGroups * i + grp; };
+    auto page = [&](int i) { return page_of<true>(a, p, index(i) * kKT); };
+    auto codes_at = [&](const uint8_t* codes, int i, int pg) {
+        const int t0 = index(i) * kKT;
+        const bool ok = i < n_mine && pg >= 0 && pg < a.n_blocks;
+        return __builtin_amdgcn_make_buffer_rsrc(
+            const_cast<uint8_t*>(codes) + (ok ? head_row(pg, a.HKV, kvh, a.bshift, t0) * D : 0), 0,
+            ok ? min(kKT, p.T - t0) * D : 0, kBufferDword3);
+    };
+    // this wave's quarter of the group's i-th tile:
+    //   K: codes 16 (lane % 8) .. + 15 of row 8 hw + lane / 8
+    //   V: codes 32 hw + 4 (lane % 8) .. + 3 of the four rows from 4 (lane / 8) on
+    // and, by the first wave, the scales: of K by its lower half, of V by its upper
+    struct Quarter {
+        u32x4 k;
+        uint32_t v[4];
+        float scale;
+    };
+    auto load_k = [&](Quarter& t, int i, int pg) {
+        const Rsrc rs = codes_at(a.k8, i, pg);
+        const uint32_t ln = lane_now();
+        t.k = __builtin_amdgcn_raw_buffer_load_b128(rs, (8 * hw + (ln >> 3)) * D + 16 * (ln & 7), 0, 0);
+    };
+    auto load_v = [&](Quarter& t, int i, int pg) {
+        const Rsrc rs = codes_at(a.v8, i, pg);
+        const uint32_t ln = lane_now(), at = 4 * (ln >> 3) * D + 32 * hw + 4 * (ln & 7);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) t.v[x] = __builtin_amdgcn_raw_buffer_load_b32(rs, at + x * D, 0, 0);
+    };
+    auto load_scales = [&](Quarter& t, int i, int pg) {
+        if (hw != 0) return;
+        const bool ok = i < n_mine && pg >= 0 && pg < a.n_blocks;
+        const size_t at = ok ? head_row(pg, a.HKV, kvh, a.bshift, index(i) * kKT) : 0;
+        const uint32_t ln = lane_now();
+        t.scale = ok ? (ln & 32 ? a.vs : a.ks)[at + (ln & 31)] : 0.f;
+    };
+    auto store_k = [&](const Quarter& t, int i) {
+        const uint32_t ln = lane_now();
+        char* d = lds + (i & 1) * kBuf8 + (8 * hw + (ln >> 3)) * kK8RowB + 32 * (ln & 7);
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const uint32_t lo = flipped<kInt8>(t.k[2 * x]), hi = flipped<kInt8>(t.k[2 * x + 1]);
+            *reinterpret_cast<u32x4*>(d + 16 * x) = u32x4{pair_f16<kInt8, 0>(lo), pair_f16<kInt8, 1>(lo),
+                                                          pair_f16<kInt8, 0>(hi), pair_f16<kInt8, 1>(hi)};
+        }
+    };
+    // V transposed: the keys of P . V's operand, half hh of step x, are 16x + 4hh + {0 .. 3, 8 .. 11}
+    auto store_v = [&](const Quarter& t, int i) {
+        const uint32_t ln = lane_now(), c = ln >> 3;
+        char* d = lds + (i & 1) * kBuf8 + kK8Tile + (32 * hw + 4 * (ln & 7)) * kV8RowB + 32 * (c >> 2) + 16 * (c & 1) +
+                  8 * ((c >> 1) & 1);
+        uint32_t x[2][2];  // [codes 0, 1 or 2, 3][keys 0, 1 or 2, 3]
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            x[0][y] = flipped<kInt8>(__builtin_amdgcn_perm(t.v[2 * y + 1], t.v[2 * y], 0x05010400u));
+            x[1][y] = flipped<kInt8>(__builtin_amdgcn_perm(t.v[2 * y + 1], t.v[2 * y], 0x07030602u));
+        }
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+            *reinterpret_cast<u32x2*>(d + (2 * y) * kV8RowB) = u32x2{pair_f16<kInt8, 0>(x[y][0]), pair_f16<kInt8, 0>(x[y][1])};
+            *reinterpret_cast<u32x2*>(d + (2 * y + 1) * kV8RowB) =
+                u32x2{pair_f16<kInt8, 1>(x[y][0]), pair_f16<kInt8, 1>(x[y][1])};
+        }
+        if constexpr (!kInt8) {
+            uint32_t nan = 0;
+#pragma unroll
+            for (int y = 0; y < 4; ++y) nan |= ((t.v[y] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+            const bool any = __builtin_amdgcn_ballot_w64(nan != 0) != 0;
+            if (ln == 0)
+                *reinterpret_cast<uint32_t*>(lds + (i & 1) * kBuf8 + kK8Tile + kV8Tile + 2 * kKT * 4 + 4 * hw) = any;
+        }
+    };
+    auto store_scales = [&](const Quarter& t, int i) {
+        if (hw == 0)
+            *reinterpret_cast<float*>(lds + (i & 1) * kBuf8 + kK8Tile + kV8Tile + 4 * lane_now()) = t.scale;
+    };
+    const int p0 = page(0), p1 = page(1);
+    Quarter t0, t1;  // (t1: the tile after it)
+    t0.scale = t1.scale = 0.f;
+    load_k(t0, 0, p0);
+    load_v(t0, 0, p0);
+    load_scales(t0, 0, p0);
+    load_k(t1, 1, p1);
+    load_v(t1, 1, p1);
+    load_scales(t1, 1, p1);
+
+    // q: planes of d = 16 t + 8 hh + 0 .. 7
+    u32x4 qh[8], ql[8];
+    float sq;  // takes the row's scaling out of its scores
+    {
+        const float* src = a.q + ((size_t)p.row0 + tok) * a.q_stride + (size_t)(kvh * G + row - tok * G) * D + 8 * hh;
+        float most = 0.f;
+        float4 q[16];
+#pragma unroll
+        for (int t = 0; t < 16; ++t) {
+            const float4 v = *reinterpret_cast<const float4*>(src + 16 * (t >> 1) + 4 * (t & 1));
+            q[t] = make_float4(v.x * sl2, v.y * sl2, v.z * sl2, v.w * sl2);
+            most = fmaxf(fmaxf(most, __builtin_fabsf(q[t].x)), __builtin_fabsf(q[t].y));
+            most = fmaxf(fmaxf(most, __builtin_fabsf(q[t].z)), __builtin_fabsf(q[t].w));
+        }
+        most = half_max(most);
+        const uint32_t f = scale_to<14>(most);
+        const float fq = __uint_as_float(f);
+        sq = inverse(f);
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+            uint32_t h[4], l[4];
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const float4 v = q[2 * t + y];
+                split_f16(v.x * fq, v.y * fq, h[2 * y], l[2 * y]);
+                split_f16(v.z * fq, v.w * fq, h[2 * y + 1], l[2 * y + 1]);
+            }
+            qh[t] = u32x4{h[0], h[1], h[2], h[3]};
+            ql[t] = u32x4{l[0], l[1], l[2], l[3]};
+        }
+    }
+    floatx16 o[4], s;
+    float m = -INFINITY, l = 0.f;
+    int fe = kTopF;  // log2 F
+#pragma unroll
+    for (int db = 0; db < 4; ++db)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
+    auto scale_o = [&](float by) {
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) o[db][r] *= by;
+    };
+    auto scores = [&](int i) {
+        const char* k = lds + (i & 1) * kBuf8 + col * kK8RowB + 16 * hh;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = 0.f;
+        u32x4 kf[2];
+        kf[0] = *reinterpret_cast<const u32x4*>(k);
+#pragma unroll
+        for (int t = 0; t < 8; ++t) {
+            if (t < 7) kf[(t + 1) & 1] = *reinterpret_cast<const u32x4*>(k + 32 * (t + 1));
+            s = mfma32(kf[t & 1], ql[t], s);
+            s = mfma32(kf[t & 1], qh[t], s);
+        }
+    };
+    // weights times scales times F in place of the scores; the bits of the keys that the row sees
+    auto weights = [&](int i, uint32_t& bits) {
+        const int kt = index(i);
+        const float* sc = reinterpret_cast<const float*>(lds + (i & 1) * kBuf8 + kK8Tile + kV8Tile) + 4 * hh;
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(sc + 2 * r);
+            s[r] = s[r] * sq * f.x, s[r + 1] = s[r + 1] * sq * f.y;
+            s[r + 2] = s[r + 2] * sq * f.z, s[r + 3] = s[r + 3] * sq * f.w;
+        }
+        bits = ~0u;
+        if (kt >= nfull) {
+            if constexpr (kTree) bits = tree_bits(a, p, qpos, kt * kKT);
+            else {
+                const int n = qpos - kt * kKT + 1;
+                bits = n >= kKT ? ~0u : n <= 0 ? 0u : (1u << n) - 1u;
+            }
+            const uint32_t mine = bits >> (4 * hh);
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (!(mine >> (8 * (r >> 2) + (r & 3)) & 1)) s[r] = -INFINITY;
+        }
+        float mx = s[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+        mx = half_max(mx);
+        if (__builtin_amdgcn_ballot_w64(mx > m + kLazy8)) {  // rare after the first tile
+            const float mn = fmaxf(m, ceilf(mx));
+            const int up = m == mn ? 0 : (int)fminf(mn - m, 1000.f);
+            l *= pow2(-up);
+            const int fn = min(fe + up, kTopF);  // the sums stay where F can go up by as much
+            if (__builtin_amdgcn_ballot_w64(fn - fe != up)) scale_o(pow2(fn - fe - up));
+            fe = fn;
+            m = mn;
+        }
+        const float nb = m == -INFINITY ? 0.f : -m;
+        float sum = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[r] = __builtin_amdgcn_exp2f(s[r] + nb);
+            sum += s[r];
+        }
+        l += sum;
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(sc + kKT + 2 * r);
+            s[r] *= f.x, s[r + 1] *= f.y, s[r + 2] *= f.z, s[r + 3] *= f.w;
+        }
+        if (kt >= nfull) {  // (a scale that the row does not see may be anything)
+            const uint32_t mine = bits >> (4 * hh);
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (!(mine >> (8 * (r >> 2) + (r & 3)) & 1)) s[r] = 0.f;
+        }
+        float wm = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) wm = fmaxf(wm, __builtin_fabsf(s[r]));
+        wm = half_max(wm);
+        float F = pow2(fe);
+        if (__builtin_amdgcn_ballot_w64(wm * F > kTopW)) {  // rare after the first tile
+            const int fn = wm * F > kTopW ? 127 + 14 - (int)min(__float_as_uint(wm) >> 23, 254u) : fe;
+            scale_o(pow2(fn - fe));
+            fe = fn;
+            F = pow2(fe);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] *= F;
+    };
+    // a tile whose codes of V hold a NaN that not every row sees, key by key
+    auto key_by_key = [&](int i, uint32_t bits) {
+        const Rsrc rv = codes_at(a.v8, i, page(i));
+#pragma unroll 1
+        for (int c = 0; c < kKT; ++c) {
+            float wc = 0.f;
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if (c == 8 * (r >> 2) + 4 * hh + (r & 3)) wc = s[r];
+            wc += lane_xor32(wc);
+#pragma unroll
+            for (int db = 0; db < 4; ++db)
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {  // d = 32 db + 8y + 4hh + 0 .. 3
+                    const uint32_t v = __builtin_amdgcn_raw_buffer_load_b32(rv, c * D + 32 * db + 8 * y + 4 * hh, 0, 0);
+                    if (bits >> c & 1) {
+                        o[db][4 * y] = __builtin_fmaf(wc, value_of<false, 0>(v), o[db][4 * y]);
+                        o[db][4 * y + 1] = __builtin_fmaf(wc, value_of<false, 1>(v), o[db][4 * y + 1]);
+                        o[db][4 * y + 2] = __builtin_fmaf(wc, value_of<false, 2>(v), o[db][4 * y + 2]);
+                        o[db][4 * y + 3] = __builtin_fmaf(wc, value_of<false, 3>(v), o[db][4 * y + 3]);
+                    }
+                }
+        }
+    };
+    auto values = [&](int i, uint32_t bits) {
+        const char* v = lds + (i & 1) * kBuf8 + kK8Tile + col * kV8RowB + 16 * hh;
+        if constexpr (!kInt8) {
+            if (index(i) >= nfull) {
+                const u32x4 nan = *reinterpret_cast<const u32x4*>(lds + (i & 1) * kBuf8 + kK8Tile + kV8Tile + 2 * kKT * 4);
+                if (scalar(nan.x | nan.y | nan.z | nan.w)) return key_by_key(i, bits);
+            }
+        }
+        u32x4 vf[2], ph, pl;
+        vf[0] = *reinterpret_cast<const u32x4*>(v);
+#pragma unroll
+        for (int y = 0; y < 8; ++y) {
+            if ((y & 3) == 0) {
+                uint32_t h[4], lo[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) split_f16(s[2 * y + 2 * j], s[2 * y + 2 * j + 1], h[j], lo[j]);
+                ph = u32x4{h[0], h[1], h[2], h[3]}, pl = u32x4{lo[0], lo[1], lo[2], lo[3]};
+            }
+            if (y < 7)
+                vf[(y + 1) & 1] = *reinterpret_cast<const u32x4*>(v + 32 * ((y + 1) & 3) * kV8RowB + 32 * ((y + 1) >> 2));
+            o[y & 3] = mfma32(vf[y & 1], pl, o[y & 3]);
+            o[y & 3] = mfma32(vf[y & 1], ph, o[y & 3]);
+        }
+    };
+    // Tile i + 1 goes to LDS while tile i is worked on, into the places of tile i - 1.  The second group takes the next
+    // tile's scores at the end of an iteration, so its K is a tile further: K of i + 2 goes where K of i was, whose
+    // scores every wave took before the last barrier.
+    store_k(t0, 0);
+    store_v(t0, 0);
+    store_scales(t0, 0);
+    int pg = page(2);
+    if (grp == 1) {
+        store_k(t1, 1);
+        load_k(t1, 2, pg);
+    }
+    lds_barrier();
+    if (grp == 1 && n_mine > 0) scores(0);
+    lds_barrier();  // (K of tile 0 has been read)
+    for (int i = 0; i < n_it; ++i) {
+        // t1: V and scales of tile i + 1, K of tile i + 1 (second group: i + 2)
+        const int next = page(i + 3);
+        uint32_t bits = ~0u;
+        if (grp == 0 && i < n_mine) scores(i);
+        if (i + 1 + grp < n_mine) store_k(t1, i + 1 + grp);
+        load_k(t1, i + 2 + grp, grp ? next : pg);
+        if (i < n_mine) weights(i, bits);
+        if (i + 1 < n_mine) {
+            store_v(t1, i + 1);
+            store_scales(t1, i + 1);
+        }
+        load_v(t1, i + 2, pg);
+        load_scales(t1, i + 2, pg);
+        if (i < n_mine) values(i, bits);
+        if (grp == 1 && i + 1 < n_mine) scores(i + 1);
+        pg = next;
+        lds_barrier();
+    }
+
+    // ---- the key groups meet through LDS, as in k_packed_attn: group g finishes blocks db = 2g, 2g + 1
+    {
+        const float f = pow2(-fe);
+        if (m == -INFINITY) {  // (scores of -infinity beside infinite values: parts without weights are passed over)
+            float z = 0.f;
+#pragma unroll
+            for (int db = 0; db < 4; ++db)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) z = __builtin_fmaf(o[db][r], 0.f, z);
+            l += z;
+        }
+        scale_o(f);
+    }
+    lds_barrier();  // the tiles have been read
+    float* xw = smem + w * (kXch8 * 64) + lane;
+    xw[0] = m;
+    xw[64] = l;
+    const floatx16 give0 = grp ? o[0] : o[2], give1 = grp ? o[1] : o[3];
+    const floatx16 keep0 = grp ? o[2] : o[0], keep1 = grp ? o[3] : o[1];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        xw[(2 + i) * 64] = give0[i];
+        xw[(18 + i) * 64] = give1[i];
+    }
+    lds_barrier();
+    float* const stage = smem + kStage8;
+    const float* xp = smem + ((1 - grp) * kSlots + hw) * (kXch8 * 64) + lane;
+    const float mp = xp[0], lp = xp[64];
+    const float mt = fmaxf(m, mp);
+    const float c0 = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mt);
+    const float cp = mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mp - mt);
+    // (a group whose every score is NaN keeps m at -inf, and its NaN sum counts)
+    const float ls = half_sum((m == -INFINITY ? l : l * c0) + (mp == -INFINITY ? lp : lp * cp));
+    {
+        bool none = qpos < 0;  // a row that sees no key: zeros
+        if constexpr (kTree) none = ls == 0.f && tree_sees_none(a, p.row0, p.pos0, tok);
+        const float inv = p.part ? 1.f : none ? 0.f : 1.f / ls;
+        float* ost = stage + (hw * kQB + col) * kRowF + 64 * grp + 4 * hh;
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+            float v0[4], v1[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                v0[j] = (keep0[r + j] * c0 + xp[(2 + r + j) * 64] * cp) * inv;
+                v1[j] = (keep1[r + j] * c0 + xp[(18 + r + j) * 64] * cp) * inv;
+            }
+            *reinterpret_cast<float4*>(ost + 2 * r) = make_float4(v0[0], v0[1], v0[2], v0[3]);
+            *reinterpret_cast<float4*>(ost + 32 + 2 * r) = make_float4(v1[0], v1[1], v1[2], v1[3]);
+        }
+        if (p.part && hh == 0 && grp == 0)
+            *reinterpret_cast<float2*>(p.part + kUnitRows * D + 2 * (hw * kQB + col)) = make_float2(mt, ls);
+    }
+    lds_barrier();
+    {
+        const int ln = unhoisted(lane), c4 = 4 * (ln & 31);
+#pragma unroll
+        for (int j = 0; j < kQB / 4; ++j) {  // wave wu: rows 16 wu .. of the unit, two per instruction
+            const int jj = (kQB / 2) * wu + 2 * j + (ln >> 5), f = kUnitRows * p.u + jj;
+            const float4 v = *reinterpret_cast<const float4*>(stage + jj * kRowF + c4);
+            const int t = fdiv(f, fG);
+            float* dst = p.part ? p.part + jj * D : a.out + (((size_t)p.row0 + t) * a.H + kvh * G + f - t * G) * D;
+            if (f < p.nflat) *reinterpret_cast<float4*>(dst + c4) = v;
+        }
+    }
+}
+
 // grid shares x KV heads, as k_packed_attn
 template <bool kInt8, bool kTree>
 __global__ __launch_bounds__(64 * kWaves) void k_cache8_attn(Cache8Args a, int shares, float* __restrict__ wide_parts,
@@ -603,7 +998,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_cache8_attn(Cache8Args a, int s
     const FastDiv fG = fast_div((uint32_t)(a.H / a.HKV));
     const float sl2 = a.scale * 1.44269504088896340736f;  // scores come out in log2 units
     walk_share<false>(a, pv.wide, wide, rounds, shares, share, kvh, fG, wide_parts, [&](const Pass& p) {
-        rows_pass<kInt8, kTree>(a, p, kvh, fG, sl2, kUnitRows * kHeadDim, smem);
+        wide8_pass<kInt8, kTree>(a, p, kvh, fG, sl2, smem);
     });
     lds_barrier();  // the last wide pass's rows have been read
     walk_share<true>(a, pv.few, few, 0, shares, share, kvh, fG, few_parts, [&](const Pass& p) {
@@ -647,7 +1042,7 @@ hipError_t launch_cache_keep(hipStream_t st, const Cache8Args& a, float* kc, flo
 template <bool kInt8, bool kTree>
 static hipError_t launch_cache8_attn_as(hipStream_t st, const Cache8Args& a, int shares, const PackedParts& parts) {
     static std::atomic<bool> opted;
-    constexpr size_t lds = (size_t)kFew8F * sizeof(float);
+    constexpr size_t lds = (size_t)kWide8F * sizeof(float);
     if (const hipError_t e = opt_in_lds(opted, (const void*)k_cache8_attn<kInt8, kTree>, lds); e != hipSuccess) return e;
     k_cache8_attn<kInt8, kTree><<<shares * a.HKV, 64 * kWaves, lds, st>>>(a, shares, parts.wide, parts.few);
     return hipGetLastError();
