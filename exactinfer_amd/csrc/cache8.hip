@@ -247,11 +247,11 @@ __global__ __launch_bounds__(256) void k_cache_keep(Cache8Args a, float* __restr
 // 24): two matrix instructions where two fp32 operands take three (packed.hip) or six (prefill.hip).
 //
 //   scores   q, scaled per row to a largest value of 2^14, against the codes of K; times the key's scale in fp32
-//   output   weights p = 2^(s - m) times the value's scale times F, a power of two of the row's own: the largest
-//            p s_v F so far lies below 2^15 and F only goes down where a larger one comes (the sums go with it),
-//            up where the reference m rises (the sums stay).  So what the planes lose, 2^-39 of the row's largest weight
-//            times scale, never shows, however uneven the values' scales are.  m is a whole number: every factor
-//            of the sums is a power of two, exact.
+//   output   weights p = 2^(s - m) F, F a power of two of the row's own, times the value's scale: the largest
+//            p s_v lies between 2^14 and 2^15 at first, and F goes down where one passes that (the sums go with it), up
+//            where the reference m rises (the sums stay).  So what the planes lose, 2^-39 of the row's largest
+//            weight times scale, never shows, however uneven the values' scales are.  m is a whole number: every
+//            factor of the sums is a power of two, exact.
 struct Tile8 {
     u32x4 k[2][2];  // [sixteen keys][half of the lane's 32 codes]
     u32x2 v[8];
@@ -280,7 +280,7 @@ __device__ __forceinline__ uint32_t flipped(uint32_t codes) { return kInt8 ? cod
 constexpr int kRow8 = 16;                              // rows of one matrix instruction
 constexpr int kFew8ML = kWaves * kRow8 * kRowF;        // LDS: every wave's rows, then their (m, l)
 constexpr int kFew8F = kFew8ML + kWaves * kRow8 * 2;
-constexpr int kTopF = 100;                             // log2 F at most, and of a row without weights
+constexpr int kTopF = 96;                              // log2 F at most
 constexpr float kTopW = 0x1p15f;                       // p s_v F at most
 constexpr float kLazy8 = 8.f;                          // the reference moves when a score passes it by more (log2 units)
 __device__ __forceinline__ float pow2(int e) { return __builtin_amdgcn_ldexpf(1.f, e); }
@@ -372,11 +372,12 @@ __device__ __forceinline__ void rows_pass(const Cache8Args& a, const Pass& p, in
         }
     }
     f32x4 o[8];
-    float m = -INFINITY, l = 0.f;
-    int fe = kTopF;  // log2 F
+    float m = -INFINITY, l = 0.f, limit = 0.f;  // (limit of a row without weights so far)
+    int fe = 0;                                 // log2 F
 #pragma unroll
     for (int y = 0; y < 8; ++y) o[y] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto scale_o = [&](float by) {
+    auto scale_sums = [&](float by) {
+        l *= by;
 #pragma unroll
         for (int y = 0; y < 8; ++y)
 #pragma unroll
@@ -412,7 +413,7 @@ __device__ __forceinline__ void rows_pass(const Cache8Args& a, const Pass& p, in
         auto seen = [&](int r) { return (mine >> (16 * (r >> 2) + (r & 3)) & 1) != 0; };
         float mx = -INFINITY;
 #pragma unroll
-        for (int r = 0; r < 8; ++r) s[r >> 2][r & 3] = s[r >> 2][r & 3] * sq * t.ks[r >> 2][r & 3];
+        for (int r = 0; r < 8; ++r) s[r >> 2][r & 3] *= t.ks[r >> 2][r & 3];
         if (kt >= nfull) {
 #pragma unroll
             for (int r = 0; r < 8; ++r)
@@ -420,22 +421,21 @@ __device__ __forceinline__ void rows_pass(const Cache8Args& a, const Pass& p, in
         }
 #pragma unroll
         for (int r = 0; r < 8; ++r) mx = fmaxf(mx, s[r >> 2][r & 3]);
-        mx = row_max(mx);
+        mx = row_max(mx) * sq;
         if (__builtin_amdgcn_ballot_w64(mx > m + kLazy8)) {  // rare after the first tile
             const float mn = fmaxf(m, ceilf(mx));
-            const int up = m == mn ? 0 : (int)fminf(mn - m, 1000.f);
-            l *= pow2(-up);
+            const int up = m == -INFINITY || m == mn ? 0 : (int)fminf(mn - m, 1000.f);
             const int fn = min(fe + up, kTopF);  // the sums stay where F can go up by as much
-            if (__builtin_amdgcn_ballot_w64(fn - fe != up)) scale_o(pow2(fn - fe - up));
+            if (__builtin_amdgcn_ballot_w64(fn - fe != up)) scale_sums(pow2(fn - fe - up));
             fe = fn;
             m = mn;
         }
-        const float nb = m == -INFINITY ? 0.f : -m;
+        const float nb = m == -INFINITY ? 0.f : (float)fe - m;
         float sum = 0.f, wm = 0.f;
         float wt[8];
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
-            const float pr = __builtin_amdgcn_exp2f(s[r >> 2][r & 3] + nb);
+            const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r >> 2][r & 3], sq, nb));
             sum += pr;
             wt[r] = pr * t.vs[r >> 2][r & 3];
         }
@@ -448,17 +448,20 @@ __device__ __forceinline__ void rows_pass(const Cache8Args& a, const Pass& p, in
 #pragma unroll
         for (int r = 0; r < 8; ++r) wm = fmaxf(wm, __builtin_fabsf(wt[r]));
         wm = row_max(wm);
-        float F = pow2(fe);
-        if (__builtin_amdgcn_ballot_w64(wm * F > kTopW)) {  // rare after the first tile
-            // wm F: 2^14 .. 2^15
-            const int fn = wm * F > kTopW ? 127 + 14 - (int)min(__float_as_uint(wm) >> 23, 254u) : fe;
-            scale_o(pow2(fn - fe));
+        if (__builtin_amdgcn_ballot_w64(wm > limit)) {  // rare after the first tile
+            // the largest: 2^14 .. 2^15
+            const bool over = wm > limit;
+            const int fn = over ? min(fe + 127 + 14 - (int)min(__float_as_uint(wm) >> 23, 254u), kTopF) : fe;
+            const float by = pow2(fn - fe);
+            scale_sums(by);
+#pragma unroll
+            for (int r = 0; r < 8; ++r) wt[r] *= by;
             fe = fn;
-            F = pow2(fe);
+            if (over) limit = kTopW;
         }
         uint32_t wh[4], wl[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) split_f16(wt[2 * r] * F, wt[2 * r + 1] * F, wh[r], wl[r]);
+        for (int r = 0; r < 4; ++r) split_f16(wt[2 * r], wt[2 * r + 1], wh[r], wl[r]);
         const u32x4 ph = {wh[0], wh[1], wh[2], wh[3]}, pl = {wl[0], wl[1], wl[2], wl[3]};
         if constexpr (!kInt8) {
             // a NaN among codes that not every row sees must not meet them: key by key then
@@ -476,7 +479,7 @@ __device__ __forceinline__ void rows_pass(const Cache8Args& a, const Pass& p, in
                     float wc = 0.f;
 #pragma unroll
                     for (int r = 0; r < 8; ++r)  // key 16 (r / 4) + 4 quarter + r % 4
-                        if (c == 16 * (r >> 2) + 4 * quarter + (r & 3)) wc = wt[r] * F;
+                        if (c == 16 * (r >> 2) + 4 * quarter + (r & 3)) wc = wt[r];
                     wc += lane_xor16(wc);
                     wc += lane_xor32(wc);
 #pragma unroll
@@ -540,6 +543,7 @@ __device__ __forceinline__ void rows_pass(const Cache8Args& a, const Pass& p, in
     float* const ml = smem + kFew8ML;
     {
         const float f = pow2(-fe);
+        l *= f;
         if (m == -INFINITY) {  // (scores of -infinity beside infinite values: parts without weights are passed over)
             float z = 0.f;
 #pragma unroll
@@ -627,12 +631,18 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
     const int n_it = (p.nrange + kGroups - 1) / kGroups, n_mine = (p.nrange - grp + kGroups - 1) / kGroups;
     auto index = [&](int i) { return p.kt_lo + kGroups * i + grp; };
     auto page = [&](int i) { return page_of<true>(a, p, index(i) * kKT); };
-    auto codes_at = [&](const uint8_t* codes, int i, int pg) {
+    struct Place {   // of a tile
+        size_t row;  // its first head row
+        int there;   // keys of it
+    };
+    auto place = [&](int i, int pg) {
         const int t0 = index(i) * kKT;
         const bool ok = i < n_mine && pg >= 0 && pg < a.n_blocks;
-        return __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<uint8_t*>(codes) + (ok ? head_row(pg, a.HKV, kvh, a.bshift, t0) * D : 0), 0,
-            ok ? min(kKT, p.T - t0) * D : 0, kBufferDword3);
+        return Place{ok ? head_row(pg, a.HKV, kvh, a.bshift, t0) : 0, ok ? min(kKT, p.T - t0) : 0};
+    };
+    auto codes_at = [&](const uint8_t* codes, const Place& at) {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(codes) + at.row * D, 0, at.there * D,
+                                                 kBufferDword3);
     };
     // this wave's quarter of the group's i-th tile:
     //   K: codes 16 (lane % 8) .. + 15 of row 8 hw + lane / 8
@@ -643,23 +653,22 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
         uint32_t v[4];
         float scale;
     };
-    auto load_k = [&](Quarter& t, int i, int pg) {
-        const Rsrc rs = codes_at(a.k8, i, pg);
+    auto load_k = [&](Quarter& t, const Place& at) {
+        const Rsrc rs = codes_at(a.k8, at);
         const uint32_t ln = lane_now();
         t.k = __builtin_amdgcn_raw_buffer_load_b128(rs, (8 * hw + (ln >> 3)) * D + 16 * (ln & 7), 0, 0);
     };
-    auto load_v = [&](Quarter& t, int i, int pg) {
-        const Rsrc rs = codes_at(a.v8, i, pg);
-        const uint32_t ln = lane_now(), at = 4 * (ln >> 3) * D + 32 * hw + 4 * (ln & 7);
+    auto load_v = [&](Quarter& t, const Place& at) {
+        const Rsrc rs = codes_at(a.v8, at);
+        const uint32_t ln = lane_now(), off = 4 * (ln >> 3) * D + 32 * hw + 4 * (ln & 7);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) t.v[x] = __builtin_amdgcn_raw_buffer_load_b32(rs, at + x * D, 0, 0);
+        for (int x = 0; x < 4; ++x) t.v[x] = __builtin_amdgcn_raw_buffer_load_b32(rs, off + x * D, 0, 0);
     };
-    auto load_scales = [&](Quarter& t, int i, int pg) {
+    auto load_scales = [&](Quarter& t, const Place& at) {  // (whole tiles: pages hold them)
         if (hw != 0) return;
-        const bool ok = i < n_mine && pg >= 0 && pg < a.n_blocks;
-        const size_t at = ok ? head_row(pg, a.HKV, kvh, a.bshift, index(i) * kKT) : 0;
         const uint32_t ln = lane_now();
-        t.scale = ok ? (ln & 32 ? a.vs : a.ks)[at + (ln & 31)] : 0.f;
+        t.scale = 0.f;
+        if (at.there > 0) t.scale = (ln & 32 ? a.vs : a.ks)[at.row + (ln & 31)];
     };
     auto store_k = [&](const Quarter& t, int i) {
         const uint32_t ln = lane_now();
@@ -701,15 +710,16 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
         if (hw == 0)
             *reinterpret_cast<float*>(lds + (i & 1) * kBuf8 + kK8Tile + kV8Tile + 4 * lane_now()) = t.scale;
     };
-    const int p0 = page(0), p1 = page(1);
     Quarter t0, t1;  // (t1: the tile after it)
-    t0.scale = t1.scale = 0.f;
-    load_k(t0, 0, p0);
-    load_v(t0, 0, p0);
-    load_scales(t0, 0, p0);
-    load_k(t1, 1, p1);
-    load_v(t1, 1, p1);
-    load_scales(t1, 1, p1);
+    {
+        const Place first = place(0, page(0)), second = place(1, page(1));
+        load_k(t0, first);
+        load_v(t0, first);
+        load_scales(t0, first);
+        load_k(t1, second);
+        load_v(t1, second);
+        load_scales(t1, second);
+    }
 
     // q: planes of d = 16 t + 8 hh + 0 .. 7
     u32x4 qh[8], ql[8];
@@ -743,29 +753,37 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
         }
     }
     floatx16 o[4], s;
-    float m = -INFINITY, l = 0.f;
-    int fe = kTopF;  // log2 F
+    float m = -INFINITY, l = 0.f, limit = 0.f;  // (limit of a row without weights so far)
+    int fe = 0;                                 // log2 F
 #pragma unroll
     for (int db = 0; db < 4; ++db)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[db][r] = 0.f;
-    auto scale_o = [&](float by) {
+    auto scale_sums = [&](float by) {
+        l *= by;
 #pragma unroll
         for (int db = 0; db < 4; ++db)
 #pragma unroll
             for (int r = 0; r < 16; ++r) o[db][r] *= by;
     };
+    // (operands three steps ahead of their use: the compiler would read each right before it)
+    constexpr int kAhead = 3;
     auto scores = [&](int i) {
         const char* k = lds + (i & 1) * kBuf8 + col * kK8RowB + 16 * hh;
+        auto frag = [&](int t) { return *reinterpret_cast<const u32x4*>(k + 32 * t); };
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = 0.f;
-        u32x4 kf[2];
-        kf[0] = *reinterpret_cast<const u32x4*>(k);
+        u32x4 kf[kAhead + 1];
+#pragma unroll
+        for (int t = 0; t < kAhead; ++t) kf[t] = frag(t);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int t = 0; t < 8; ++t) {
-            if (t < 7) kf[(t + 1) & 1] = *reinterpret_cast<const u32x4*>(k + 32 * (t + 1));
-            s = mfma32(kf[t & 1], ql[t], s);
-            s = mfma32(kf[t & 1], qh[t], s);
+            if (t + kAhead < 8) kf[(t + kAhead) % (kAhead + 1)] = frag(t + kAhead);
+            __builtin_amdgcn_sched_barrier(0);
+            s = mfma32(kf[t % (kAhead + 1)], ql[t], s);
+            s = mfma32(kf[t % (kAhead + 1)], qh[t], s);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
     // weights times scales times F in place of the scores; the bits of the keys that the row sees
@@ -775,8 +793,7 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
             const float4 f = *reinterpret_cast<const float4*>(sc + 2 * r);
-            s[r] = s[r] * sq * f.x, s[r + 1] = s[r + 1] * sq * f.y;
-            s[r + 2] = s[r + 2] * sq * f.z, s[r + 3] = s[r + 3] * sq * f.w;
+            s[r] *= f.x, s[r + 1] *= f.y, s[r + 2] *= f.z, s[r + 3] *= f.w;
         }
         bits = ~0u;
         if (kt >= nfull) {
@@ -793,21 +810,20 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
         float mx = s[0];
 #pragma unroll
         for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
-        mx = half_max(mx);
+        mx = half_max(mx) * sq;
         if (__builtin_amdgcn_ballot_w64(mx > m + kLazy8)) {  // rare after the first tile
             const float mn = fmaxf(m, ceilf(mx));
-            const int up = m == mn ? 0 : (int)fminf(mn - m, 1000.f);
-            l *= pow2(-up);
+            const int up = m == -INFINITY || m == mn ? 0 : (int)fminf(mn - m, 1000.f);
             const int fn = min(fe + up, kTopF);  // the sums stay where F can go up by as much
-            if (__builtin_amdgcn_ballot_w64(fn - fe != up)) scale_o(pow2(fn - fe - up));
+            if (__builtin_amdgcn_ballot_w64(fn - fe != up)) scale_sums(pow2(fn - fe - up));
             fe = fn;
             m = mn;
         }
-        const float nb = m == -INFINITY ? 0.f : -m;
+        const float nb = m == -INFINITY ? 0.f : (float)fe - m;
         float sum = 0.f;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            s[r] = __builtin_amdgcn_exp2f(s[r] + nb);
+            s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sq, nb));
             sum += s[r];
         }
         l += sum;
@@ -826,19 +842,22 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
 #pragma unroll
         for (int r = 0; r < 16; ++r) wm = fmaxf(wm, __builtin_fabsf(s[r]));
         wm = half_max(wm);
-        float F = pow2(fe);
-        if (__builtin_amdgcn_ballot_w64(wm * F > kTopW)) {  // rare after the first tile
-            const int fn = wm * F > kTopW ? 127 + 14 - (int)min(__float_as_uint(wm) >> 23, 254u) : fe;
-            scale_o(pow2(fn - fe));
-            fe = fn;
-            F = pow2(fe);
-        }
+        if (__builtin_amdgcn_ballot_w64(wm > limit)) {  // rare after the first tile
+            // the largest: 2^14 .. 2^15
+            const bool over = wm > limit;
+            const int fn = over ? min(fe + 127 + 14 - (int)min(__float_as_uint(wm) >> 23, 254u), kTopF) : fe;
+            const float by = pow2(fn - fe);
+            scale_sums(by);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] *= F;
+            for (int r = 0; r < 16; ++r) s[r] *= by;
+            fe = fn;
+            if (over) limit = kTopW;
+        }
     };
     // a tile whose codes of V hold a NaN that not every row sees, key by key
     auto key_by_key = [&](int i, uint32_t bits) {
-        const Rsrc rv = codes_at(a.v8, i, page(i));
+        const Place at = place(i, page(i));
+        const Rsrc rv = codes_at(a.v8, at);
 #pragma unroll 1
         for (int c = 0; c < kKT; ++c) {
             float wc = 0.f;
@@ -861,15 +880,18 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
         }
     };
     auto values = [&](int i, uint32_t bits) {
-        const char* v = lds + (i & 1) * kBuf8 + kK8Tile + col * kV8RowB + 16 * hh;
         if constexpr (!kInt8) {
             if (index(i) >= nfull) {
                 const u32x4 nan = *reinterpret_cast<const u32x4*>(lds + (i & 1) * kBuf8 + kK8Tile + kV8Tile + 2 * kKT * 4);
                 if (scalar(nan.x | nan.y | nan.z | nan.w)) return key_by_key(i, bits);
             }
         }
-        u32x4 vf[2], ph, pl;
-        vf[0] = *reinterpret_cast<const u32x4*>(v);
+        const char* v = lds + (i & 1) * kBuf8 + kK8Tile + col * kV8RowB + 16 * hh;
+        auto frag = [&](int y) { return *reinterpret_cast<const u32x4*>(v + 32 * (y & 3) * kV8RowB + 32 * (y >> 2)); };
+        u32x4 vf[kAhead + 1], ph, pl;
+#pragma unroll
+        for (int y = 0; y < kAhead; ++y) vf[y] = frag(y);
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
         for (int y = 0; y < 8; ++y) {
             if ((y & 3) == 0) {
@@ -878,10 +900,11 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
                 for (int j = 0; j < 4; ++j) split_f16(s[2 * y + 2 * j], s[2 * y + 2 * j + 1], h[j], lo[j]);
                 ph = u32x4{h[0], h[1], h[2], h[3]}, pl = u32x4{lo[0], lo[1], lo[2], lo[3]};
             }
-            if (y < 7)
-                vf[(y + 1) & 1] = *reinterpret_cast<const u32x4*>(v + 32 * ((y + 1) & 3) * kV8RowB + 32 * ((y + 1) >> 2));
-            o[y & 3] = mfma32(vf[y & 1], pl, o[y & 3]);
-            o[y & 3] = mfma32(vf[y & 1], ph, o[y & 3]);
+            if (y + kAhead < 8) vf[(y + kAhead) % (kAhead + 1)] = frag(y + kAhead);
+            __builtin_amdgcn_sched_barrier(0);
+            o[y & 3] = mfma32(vf[y % (kAhead + 1)], pl, o[y & 3]);
+            o[y & 3] = mfma32(vf[y % (kAhead + 1)], ph, o[y & 3]);
+            __builtin_amdgcn_sched_barrier(0);
         }
     };
     // Tile i + 1 goes to LDS while tile i is worked on, into the places of tile i - 1.  The second group takes the next
@@ -890,37 +913,45 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
     store_k(t0, 0);
     store_v(t0, 0);
     store_scales(t0, 0);
-    int pg = page(2);
+    Place at = place(2, page(2));
+    int pg = page(2 + grp);  // of the K tile that is loaded next
     if (grp == 1) {
         store_k(t1, 1);
-        load_k(t1, 2, pg);
+        load_k(t1, at);
+        pg = page(3);
     }
     lds_barrier();
     if (grp == 1 && n_mine > 0) scores(0);
     lds_barrier();  // (K of tile 0 has been read)
     for (int i = 0; i < n_it; ++i) {
         // t1: V and scales of tile i + 1, K of tile i + 1 (second group: i + 2)
-        const int next = page(i + 3);
+        const Place ahead = place(i + 2 + grp, pg);
+        pg = page(i + 3 + grp);
         uint32_t bits = ~0u;
-        if (grp == 0 && i < n_mine) scores(i);
+        if (grp == 0) {
+            at = ahead;
+            if (i < n_mine) scores(i);
+        }
         if (i + 1 + grp < n_mine) store_k(t1, i + 1 + grp);
-        load_k(t1, i + 2 + grp, grp ? next : pg);
+        load_k(t1, ahead);
         if (i < n_mine) weights(i, bits);
         if (i + 1 < n_mine) {
             store_v(t1, i + 1);
             store_scales(t1, i + 1);
         }
-        load_v(t1, i + 2, pg);
-        load_scales(t1, i + 2, pg);
+        load_v(t1, at);
+        load_scales(t1, at);
         if (i < n_mine) values(i, bits);
-        if (grp == 1 && i + 1 < n_mine) scores(i + 1);
-        pg = next;
+        if (grp == 1) {
+            at = ahead;
+            if (i + 1 < n_mine) scores(i + 1);
+        }
         lds_barrier();
     }
 
     // ---- the key groups meet through LDS, as in k_packed_attn: group g finishes blocks db = 2g, 2g + 1
     {
-        const float f = pow2(-fe);
+        scale_sums(pow2(-fe));
         if (m == -INFINITY) {  // (scores of -infinity beside infinite values: parts without weights are passed over)
             float z = 0.f;
 #pragma unroll
@@ -929,7 +960,6 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
                 for (int r = 0; r < 16; ++r) z = __builtin_fmaf(o[db][r], 0.f, z);
             l += z;
         }
-        scale_o(f);
     }
     lds_barrier();  // the tiles have been read
     float* xw = smem + w * (kXch8 * 64) + lane;
