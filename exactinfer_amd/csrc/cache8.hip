@@ -274,8 +274,22 @@ __device__ __forceinline__ uint32_t pair_f16(uint32_t codes) {
         return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(codes, 1.f, x));
     }
 }
+// e4m3 codes that are NaN: 0x80 in the byte of each; and the codes with zeros in their place.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t codes) {
+    return ((codes & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+}
+__device__ __forceinline__ uint32_t without_nan(uint32_t codes) {
+    const uint32_t m = nan_bytes(codes);
+    return codes & ~(m | (m - (m >> 7)));
+}
 template <bool kInt8>
 __device__ __forceinline__ uint32_t flipped(uint32_t codes) { return kInt8 ? codes ^ 0x80808080u : codes; }
+
+// Keys of the tile at t0 that a row at position qpos sees, a bit each.
+__device__ __forceinline__ uint32_t causal_bits(int qpos, int t0) {
+    const int n = qpos - t0 + 1;
+    return n >= kKT ? ~0u : n <= 0 ? 0u : (1u << n) - 1u;
+}
 
 constexpr int kRow8 = 16;                              // rows of one matrix instruction
 constexpr int kFew8ML = kWaves * kRow8 * kRowF;        // LDS: every wave's rows, then their (m, l)
@@ -385,7 +399,8 @@ __device__ __forceinline__ void rows_pass(const Cache8Args& a, const Pass& p, in
     };
     auto row_max = [&](float x) { return half_max(fmaxf(x, lane_xor16(x))); };
 
-    auto tile = [&](const Tile8& t, int i, int pg) {
+    int nan_tile = n_mine;  // the first with a NaN code that not every row sees
+    auto tile = [&](Tile8& t, int i) {
         const int kt = index(i);
         f32x4 s[2];
 #pragma unroll
@@ -403,11 +418,7 @@ __device__ __forceinline__ void rows_pass(const Cache8Args& a, const Pass& p, in
         }
         uint32_t bits = ~0u;
         if (kt >= nfull) {
-            if constexpr (kTree) bits = tree_bits(a, p, qpos, kt * kKT);
-            else {
-                const int n = qpos - kt * kKT + 1;
-                bits = n >= kKT ? ~0u : n <= 0 ? 0u : (1u << n) - 1u;
-            }
+            bits = kTree ? tree_bits(a, p, qpos, kt * kKT) : causal_bits(qpos, kt * kKT);
         }
         const uint32_t mine = bits >> (4 * quarter);
         auto seen = [&](int r) { return (mine >> (16 * (r >> 2) + (r & 3)) & 1) != 0; };
@@ -464,40 +475,16 @@ __device__ __forceinline__ void rows_pass(const Cache8Args& a, const Pass& p, in
         for (int r = 0; r < 4; ++r) split_f16(wt[2 * r], wt[2 * r + 1], wh[r], wl[r]);
         const u32x4 ph = {wh[0], wh[1], wh[2], wh[3]}, pl = {wl[0], wl[1], wl[2], wl[3]};
         if constexpr (!kInt8) {
-            // a NaN among codes that not every row sees must not meet them: key by key then
-            uint32_t nan = 0;
-            if (kt >= nfull) {
+            if (kt >= nfull) {  // a NaN that not every row sees must not meet them: put in at the end
+                uint32_t nan = 0;
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
 #pragma unroll
-                    for (int x = 0; x < 2; ++x) nan |= ((t.v[e][x] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
-            }
-            if (__builtin_amdgcn_ballot_w64(nan != 0)) {
-                const Rsrc rv = codes_at(a.v8, i, pg, true);
-#pragma unroll 1
-                for (int c = 0; c < kKT; ++c) {
-                    float wc = 0.f;
-#pragma unroll
-                    for (int r = 0; r < 8; ++r)  // key 16 (r / 4) + 4 quarter + r % 4
-                        if (c == 16 * (r >> 2) + 4 * quarter + (r & 3)) wc = wt[r];
-                    wc += lane_xor16(wc);
-                    wc += lane_xor32(wc);
-#pragma unroll
                     for (int x = 0; x < 2; ++x) {
-                        const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(rv, c * D + 32 * quarter + 16 * x, 0, 0);
-                        if (bits >> c & 1) {
-#pragma unroll
-                            for (int y = 0; y < 4; ++y) {  // d = 32 quarter + 16x + 4y + 0 .. 3
-                                const int r = 2 * x + (y >> 1), at = 4 * (y & 1);
-                                o[at][r] = __builtin_fmaf(wc, value_of<false, 0>(v[y]), o[at][r]);
-                                o[at + 1][r] = __builtin_fmaf(wc, value_of<false, 1>(v[y]), o[at + 1][r]);
-                                o[at + 2][r] = __builtin_fmaf(wc, value_of<false, 2>(v[y]), o[at + 2][r]);
-                                o[at + 3][r] = __builtin_fmaf(wc, value_of<false, 3>(v[y]), o[at + 3][r]);
-                            }
-                        }
+                        nan |= nan_bytes(t.v[e][x]);
+                        t.v[e][x] = without_nan(t.v[e][x]);
                     }
-                }
-                return;
+                if (__builtin_amdgcn_ballot_w64(nan != 0)) nan_tile = min(nan_tile, i);
             }
         }
 #pragma unroll
@@ -527,15 +514,37 @@ __device__ __forceinline__ void rows_pass(const Cache8Args& a, const Pass& p, in
             load(t1, i + 1, p1, i + 1 < n_mine);
             const int p2 = page(i + 2);
             __builtin_amdgcn_sched_barrier(0);
-            tile(t0, i, p0);
+            tile(t0, i);
             __builtin_amdgcn_sched_barrier(0);
             if (i + 1 >= n_mine) break;
             load(t0, i + 2, p2, i + 2 < n_mine);
             const int p3 = page(i + 3);
             __builtin_amdgcn_sched_barrier(0);
-            tile(t1, i + 1, p1);
+            tile(t1, i + 1);
             __builtin_amdgcn_sched_barrier(0);
             p0 = p2, p1 = p3;
+        }
+    }
+    if constexpr (!kInt8) {
+#pragma unroll 1
+        for (int i = nan_tile; i < n_mine; ++i) {
+            const int t0 = index(i) * kKT;
+            const uint32_t bits = kTree ? tree_bits(a, p, qpos, t0) : causal_bits(qpos, t0);
+            const Rsrc rv = codes_at(a.v8, i, page(i), true);
+#pragma unroll 1
+            for (int c = 0; c < kKT; ++c) {
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(rv, c * D + 32 * quarter + 16 * x, 0, 0);
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {  // d = 32 quarter + 16x + 4y + 0 .. 3
+                        const uint32_t nan = bits >> c & 1 ? nan_bytes(v[y]) : 0u;
+#pragma unroll
+                        for (int z = 0; z < 4; ++z)
+                            if (nan >> (8 * z) & 0x80) o[4 * (y & 1) + z][2 * x + (y >> 1)] = __builtin_nanf("");
+                    }
+                }
+            }
         }
     }
     // every wave's rows meet
@@ -594,42 +603,55 @@ __device__ __forceinline__ void rows_pass(const Cache8Args& a, const Pass& p, in
 }
 
 // ---- a wide unit: up to 128 rows
-// Two key groups of four waves; a group's waves hold 32 rows each and share its tiles (tile kt to group
-// (kt - first) % 2), whose codes each wave turns a quarter of into binary16 in LDS, V transposed, two tiles of a
-// group at a time there, one barrier a tile.  On v_mfma_f32_32x32x16_f16 S^T[key][row] = K . Q^T gives a lane 16 of a
-// tile's 32 keys for one row, which are the operand of O^T[d][row] = V^T . P^T.  The two waves of a SIMD
-// are of different groups, and the second group's iteration begins with the softmax: one has matrix work while the
-// other has not.
+// Groups of kS waves (four of 32 rows each, or two where the unit has no more than 64 rows) share a tile, the groups take
+// the unit's tiles in turn.  Each wave turns its part of a tile's codes into binary16 in LDS, V transposed, four
+// tiles of a group at a time there (or two), one barrier for half of them.  On v_mfma_f32_32x32x16_f16 S^T[key][row] = K . Q^T gives a lane
+// 16 of a tile's 32 keys for one row, which are the operand of O^T[d][row] = V^T . P^T.
+//
+// Matrix and vector instructions of one wave overlap where neither waits for the other: the next tile's scores are
+// taken between the instructions of this one's softmax, and the next tiles' conversions and the second half of the
+// weights' planes between those of P . V, by hand, since the compiler would put each kind together (and every LDS
+// read right before its use).
 constexpr int kK8RowB = 2 * kHeadDim + 16, kK8Tile = kKT * kK8RowB;  // [32 keys][128 d] binary16, rows spread over banks
 constexpr int kV8RowB = 2 * kKT + 16, kV8Tile = kHeadDim * kV8RowB;  // [128 d][32 keys]
-constexpr int kScales8 = 2 * kKT * 4 + 16;                          // of K, of V; a word per wave: NaN among its codes
+constexpr int kScales8 = 2 * kKT * 4;                               // of K, of V
 constexpr int kBuf8 = kK8Tile + kV8Tile + kScales8;                 // one tile of a group
 static_assert(kBuf8 % 16 == 0, "16-byte pieces");
-constexpr int kXch8 = 34;                                           // floats per lane exchanged by the merge
-constexpr int kStage8 = kWaves * kXch8 * 64;                        // then the unit's rows
-constexpr int kWide8F = kStage8 + kUnitRows * kRowF;
-static_assert(4 * kBuf8 <= kWide8F * 4, "the tiles lie below the merge's areas");
-static_assert(kWide8F * 4 <= 160 * 1024 && kFew8F <= kWide8F, "LDS budget");
+template <int kS>
+struct Wide8 {
+    static constexpr int kN = kWaves / kS, kOwn = 4 / kN;  // groups, blocks of 32 d that a group finishes
+    static constexpr int kRing = kS == 4 ? 4 : 2;          // tiles of a group in LDS, a barrier every kRing / 2
+    // LDS, in floats: the tiles; after them the merge's exchange (m, l and the sums given away), and the rows
+    static constexpr int kTilesF = kN * kRing * kBuf8 / 4;
+    static constexpr int kXch = 2 + 16 * (4 - kOwn);
+    static constexpr int kStage = kWaves * kXch * 64;
+    static constexpr int kEnd = kStage + kS * kQB * kRowF;
+    static constexpr int kF = kEnd > kTilesF ? kEnd : kTilesF;
+};
+constexpr int kNanAt8 = Wide8<4>::kF > Wide8<2>::kF ? Wide8<4>::kF : Wide8<2>::kF;  // a word: NaN codes were met
+constexpr int kLds8 = 4 * (kNanAt8 + 4);
+static_assert(kLds8 <= 160 * 1024 && kFew8F <= kNanAt8, "LDS budget");
 __device__ __forceinline__ floatx16 mfma32(u32x4 a, u32x4 b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
                                                   0);
 }
 
-template <bool kInt8, bool kTree>
+template <bool kInt8, bool kTree, int kS>
 __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, int kvh, FastDiv fG, float sl2,
                                            float* smem) {
-    constexpr int D = kHeadDim;
+    constexpr int D = kHeadDim, kN = Wide8<kS>::kN, kParts = 4 / kS;  // (of a tile, each 8 rows of K and 32 d of V)
+    constexpr int kRing = Wide8<kS>::kRing, kLead = kRing / 2;
     const int tid = unhoisted(threadIdx.x), lane = tid & 63, w = tid >> 6;
-    const int wu = scalar(w), hw = wu % kSlots, grp = wu / kSlots;
+    const int wu = scalar(w), hw = wu % kS, grp = wu / kS;
     const int col = lane & 31, hh = lane >> 5;
     const int G = (int)fG.d;
-    char* const lds = reinterpret_cast<char*>(smem) + grp * (2 * kBuf8);
+    char* const lds = reinterpret_cast<char*>(smem) + grp * (kRing * kBuf8);
     const int f0 = kUnitRows * p.u + kQB * hw;  // this wave's first row
     const int row = min(f0 + col, p.nflat - 1), tok = fdiv(row, fG);  // (rows past the last repeat it)
     const int qpos = p.pos0 + tok;
     const int nfull = max(kTree ? p.pos0 : p.pos0 + fdiv(min(f0, p.nflat - 1), fG) + 1, 0) / kKT;
-    const int n_it = (p.nrange + kGroups - 1) / kGroups, n_mine = (p.nrange - grp + kGroups - 1) / kGroups;
-    auto index = [&](int i) { return p.kt_lo + kGroups * i + grp; };
+    const int n_it = (p.nrange + kN - 1) / kN, n_mine = (p.nrange - grp + kN - 1) / kN;
+    auto index = [&](int i) { return p.kt_lo + kN * i + grp; };
     auto page = [&](int i) { return page_of<true>(a, p, index(i) * kKT); };
     struct Place {   // of a tile
         size_t row;  // its first head row
@@ -644,82 +666,74 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
         return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(codes) + at.row * D, 0, at.there * D,
                                                  kBufferDword3);
     };
-    // this wave's quarter of the group's i-th tile:
-    //   K: codes 16 (lane % 8) .. + 15 of row 8 hw + lane / 8
-    //   V: codes 32 hw + 4 (lane % 8) .. + 3 of the four rows from 4 (lane / 8) on
-    // and, by the first wave, the scales: of K by its lower half, of V by its upper
-    struct Quarter {
-        u32x4 k;
-        uint32_t v[4];
-        float scale;
-    };
-    auto load_k = [&](Quarter& t, const Place& at) {
+    // this wave's parts x of a tile, y = kParts hw + x:
+    //   K: codes 16 (lane % 8) .. + 15 of row 8 y + lane / 8
+    //   V: codes 32 y + 4 (lane % 8) .. + 3 of the four rows from 4 (lane / 8) on
+    // and the scales, of K by the even waves, of V by the odd ones (whole tiles: pages hold them)
+    u32x4 tk[kParts];
+    uint32_t tv[kParts][4];
+    float ts;
+    const uint32_t from_k = (8 * kParts * hw + (lane >> 3)) * D + 16 * (lane & 7);
+    const uint32_t from_v = 4 * (lane >> 3) * D + 32 * kParts * hw + 4 * (lane & 7);
+    auto load_k = [&](const Place& at) {
         const Rsrc rs = codes_at(a.k8, at);
-        const uint32_t ln = lane_now();
-        t.k = __builtin_amdgcn_raw_buffer_load_b128(rs, (8 * hw + (ln >> 3)) * D + 16 * (ln & 7), 0, 0);
+#pragma unroll
+        for (int x = 0; x < kParts; ++x)
+            tk[x] = __builtin_amdgcn_raw_buffer_load_b128(rs, from_k + 8 * x * D, 0, 0);
     };
-    auto load_v = [&](Quarter& t, const Place& at) {
+    auto load_v = [&](const Place& at) {
         const Rsrc rs = codes_at(a.v8, at);
-        const uint32_t ln = lane_now(), off = 4 * (ln >> 3) * D + 32 * hw + 4 * (ln & 7);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) t.v[x] = __builtin_amdgcn_raw_buffer_load_b32(rs, off + x * D, 0, 0);
-    };
-    auto load_scales = [&](Quarter& t, const Place& at) {  // (whole tiles: pages hold them)
-        if (hw != 0) return;
-        const uint32_t ln = lane_now();
-        t.scale = 0.f;
-        if (at.there > 0) t.scale = (ln & 32 ? a.vs : a.ks)[at.row + (ln & 31)];
-    };
-    auto store_k = [&](const Quarter& t, int i) {
-        const uint32_t ln = lane_now();
-        char* d = lds + (i & 1) * kBuf8 + (8 * hw + (ln >> 3)) * kK8RowB + 32 * (ln & 7);
+        for (int x = 0; x < kParts; ++x)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            const uint32_t lo = flipped<kInt8>(t.k[2 * x]), hi = flipped<kInt8>(t.k[2 * x + 1]);
-            *reinterpret_cast<u32x4*>(d + 16 * x) = u32x4{pair_f16<kInt8, 0>(lo), pair_f16<kInt8, 1>(lo),
-                                                          pair_f16<kInt8, 0>(hi), pair_f16<kInt8, 1>(hi)};
-        }
+            for (int y = 0; y < 4; ++y)
+                tv[x][y] = __builtin_amdgcn_raw_buffer_load_b32(rs, from_v + 32 * x + y * D, 0, 0);
     };
-    // V transposed: the keys of P . V's operand, half hh of step x, are 16x + 4hh + {0 .. 3, 8 .. 11}
-    auto store_v = [&](const Quarter& t, int i) {
-        const uint32_t ln = lane_now(), c = ln >> 3;
-        char* d = lds + (i & 1) * kBuf8 + kK8Tile + (32 * hw + 4 * (ln & 7)) * kV8RowB + 32 * (c >> 2) + 16 * (c & 1) +
-                  8 * ((c >> 1) & 1);
-        uint32_t x[2][2];  // [codes 0, 1 or 2, 3][keys 0, 1 or 2, 3]
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-            x[0][y] = flipped<kInt8>(__builtin_amdgcn_perm(t.v[2 * y + 1], t.v[2 * y], 0x05010400u));
-            x[1][y] = flipped<kInt8>(__builtin_amdgcn_perm(t.v[2 * y + 1], t.v[2 * y], 0x07030602u));
-        }
-#pragma unroll
-        for (int y = 0; y < 2; ++y) {
-            *reinterpret_cast<u32x2*>(d + (2 * y) * kV8RowB) = u32x2{pair_f16<kInt8, 0>(x[y][0]), pair_f16<kInt8, 0>(x[y][1])};
-            *reinterpret_cast<u32x2*>(d + (2 * y + 1) * kV8RowB) =
-                u32x2{pair_f16<kInt8, 1>(x[y][0]), pair_f16<kInt8, 1>(x[y][1])};
-        }
-        if constexpr (!kInt8) {
-            uint32_t nan = 0;
-#pragma unroll
-            for (int y = 0; y < 4; ++y) nan |= ((t.v[y] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
-            const bool any = __builtin_amdgcn_ballot_w64(nan != 0) != 0;
-            if (ln == 0)
-                *reinterpret_cast<uint32_t*>(lds + (i & 1) * kBuf8 + kK8Tile + kV8Tile + 2 * kKT * 4 + 4 * hw) = any;
-        }
+    auto load_scales = [&](const Place& at) {
+        const Rsrc rs = __builtin_amdgcn_make_buffer_rsrc((hw & 1 ? a.vs : a.ks) + at.row, 0, at.there ? kKT * 4 : 0,
+                                                          kBufferDword3);
+        ts = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, 4 * (lane & 31), 0, 0));
     };
-    auto store_scales = [&](const Quarter& t, int i) {
-        if (hw == 0)
-            *reinterpret_cast<float*>(lds + (i & 1) * kBuf8 + kK8Tile + kV8Tile + 4 * lane_now()) = t.scale;
+    auto buf = [&](int i) { return lds + (i & (kRing - 1)) * kBuf8; };
+    // halves of 16 bytes of K's part x
+    const uint32_t to_k = (8 * kParts * hw + (lane >> 3)) * kK8RowB + 32 * (lane & 7);
+    auto store_k = [&](int i, int x, int half) {
+        const uint32_t lo = flipped<kInt8>(tk[x][2 * half]), hi = flipped<kInt8>(tk[x][2 * half + 1]);
+        *reinterpret_cast<u32x4*>(buf(i) + to_k + 8 * x * kK8RowB + 16 * half) =
+            u32x4{pair_f16<kInt8, 0>(lo), pair_f16<kInt8, 1>(lo), pair_f16<kInt8, 0>(hi), pair_f16<kInt8, 1>(hi)};
     };
-    Quarter t0, t1;  // (t1: the tile after it)
+    // V transposed, codes 2y and 2y + 1 of part x: the keys of P . V's operand, half hh of step z, are
+    // 16z + 4hh + {0 .. 3, 8 .. 11}
+    const uint32_t to_v = kK8Tile + (32 * kParts * hw + 4 * (lane & 7)) * kV8RowB + 32 * (lane >> 5) +
+                          16 * ((lane >> 3) & 1) + 8 * ((lane >> 4) & 1);
+    auto store_v = [&](int i, int x, int y) {
+        char* d = buf(i) + to_v + (32 * x + 2 * y) * kV8RowB;
+        const uint32_t pick = y ? 0x07030602u : 0x05010400u;
+        const uint32_t lo = flipped<kInt8>(__builtin_amdgcn_perm(tv[x][1], tv[x][0], pick));
+        const uint32_t hi = flipped<kInt8>(__builtin_amdgcn_perm(tv[x][3], tv[x][2], pick));
+        *reinterpret_cast<u32x2*>(d) = u32x2{pair_f16<kInt8, 0>(lo), pair_f16<kInt8, 0>(hi)};
+        *reinterpret_cast<u32x2*>(d + kV8RowB) = u32x2{pair_f16<kInt8, 1>(lo), pair_f16<kInt8, 1>(hi)};
+    };
+    const uint32_t to_scales = kK8Tile + kV8Tile + 4 * kKT * (hw & 1) + 4 * (lane & 31);
+    auto store_scales = [&](int i) { *reinterpret_cast<float*>(buf(i) + to_scales) = ts; };
+    auto store_all_k = [&](int i) {
+#pragma unroll
+        for (int x = 0; x < kParts; ++x) store_k(i, x, 0), store_k(i, x, 1);
+    };
+    auto store_all_v = [&](int i) {
+#pragma unroll
+        for (int x = 0; x < kParts; ++x) store_v(i, x, 0), store_v(i, x, 1);
+        store_scales(i);
+    };
     {
-        const Place first = place(0, page(0)), second = place(1, page(1));
-        load_k(t0, first);
-        load_v(t0, first);
-        load_scales(t0, first);
-        load_k(t1, second);
-        load_v(t1, second);
-        load_scales(t1, second);
+        const Place first = place(0, page(0));
+        load_k(first);
+        load_v(first);
+        load_scales(first);
     }
+    int* const nan_met = reinterpret_cast<int*>(smem + kNanAt8);
+    if constexpr (!kInt8)
+        if (tid == 0) *nan_met = 0;
 
     // q: planes of d = 16 t + 8 hh + 0 .. 7
     u32x4 qh[8], ql[8];
@@ -752,7 +766,7 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
             ql[t] = u32x4{l[0], l[1], l[2], l[3]};
         }
     }
-    floatx16 o[4], s;
+    floatx16 o[4], even, odd;  // (scores of tiles 2i, 2i + 1)
     float m = -INFINITY, l = 0.f, limit = 0.f;  // (limit of a row without weights so far)
     int fe = 0;                                 // log2 F
 #pragma unroll
@@ -766,42 +780,74 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
 #pragma unroll
             for (int r = 0; r < 16; ++r) o[db][r] *= by;
     };
-    // (operands three steps ahead of their use: the compiler would read each right before it)
-    constexpr int kAhead = 3;
-    auto scores = [&](int i) {
-        const char* k = lds + (i & 1) * kBuf8 + col * kK8RowB + 16 * hh;
-        auto frag = [&](int t) { return *reinterpret_cast<const u32x4*>(k + 32 * t); };
+    auto fence = [] { __builtin_amdgcn_sched_barrier(0); };
+
+    // While tile i is worked on, V and scales of tile i + kLead and K of the one after it go to LDS, where tiles of kRing
+    // before were: every wave was done with those at the last barrier, and will not need these before the next.
+    store_all_k(0);
+    store_all_v(0);
+    Place at{};
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = 0.f;
-        u32x4 kf[kAhead + 1];
-#pragma unroll
-        for (int t = 0; t < kAhead; ++t) kf[t] = frag(t);
-        __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-        for (int t = 0; t < 8; ++t) {
-            if (t + kAhead < 8) kf[(t + kAhead) % (kAhead + 1)] = frag(t + kAhead);
-            __builtin_amdgcn_sched_barrier(0);
-            s = mfma32(kf[t % (kAhead + 1)], ql[t], s);
-            s = mfma32(kf[t % (kAhead + 1)], qh[t], s);
-            __builtin_amdgcn_sched_barrier(0);
+    for (int i = 1; i <= kLead; ++i) {
+        at = place(i, page(i));
+        load_k(at);
+        if (i < kLead) {
+            load_v(at);
+            load_scales(at);
+            store_all_v(i);
         }
+        store_all_k(i);
+    }
+    load_v(at);  // of kLead
+    load_scales(at);
+    at = place(kLead + 1, page(kLead + 1));
+    load_k(at);
+    int pg = page(kLead + 2);
+    lds_barrier();
+    u32x4 kf[3];
+    auto read_k = [&](int i, int t) {
+        kf[t % 3] = *reinterpret_cast<const u32x4*>(buf(i) + col * kK8RowB + 16 * hh + 32 * t);
     };
-    // weights times scales times F in place of the scores; the bits of the keys that the row sees
-    auto weights = [&](int i, uint32_t& bits) {
-        const int kt = index(i);
-        const float* sc = reinterpret_cast<const float*>(lds + (i & 1) * kBuf8 + kK8Tile + kV8Tile) + 4 * hh;
+    auto score_l = [&](floatx16& next, int t) {
+        if (t == 0) {
+            floatx16 zero;
 #pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            const float4 f = *reinterpret_cast<const float4*>(sc + 2 * r);
-            s[r] *= f.x, s[r + 1] *= f.y, s[r + 2] *= f.z, s[r + 3] *= f.w;
+            for (int r = 0; r < 16; ++r) zero[r] = 0.f;
+            next = mfma32(kf[t % 3], ql[t], zero);
+        } else next = mfma32(kf[t % 3], ql[t], next);
+    };
+    auto score_h = [&](floatx16& next, int t) { next = mfma32(kf[t % 3], qh[t], next); };
+    read_k(0, 0), read_k(0, 1);
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+        if (t + 2 < 8) read_k(0, t + 2);
+        fence();
+        score_l(even, t), score_h(even, t);
+    }
+    lds_barrier();  // (K of tile 0 has been read)
+    auto tile = [&](int i, floatx16& s, floatx16& next) {
+        const Place ahead = place(i + kLead + 2, pg);
+        pg = page(i + kLead + 3);
+        const int kt = index(i);
+        const float* sc = reinterpret_cast<const float*>(buf(i) + kK8Tile + kV8Tile) + 4 * hh;
+        // ---- scores times scales, while the next tile's are taken
+        f32x4 f[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) f[c] = *reinterpret_cast<const f32x4*>(sc + 8 * c);
+        read_k(i + 1, 0), read_k(i + 1, 1);
+        fence();
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[4 * c + r] *= f[c][r];
+            if (c == 0) read_k(i + 1, 2);
+            if (c == 1) score_l(next, 0);
+            if (c == 3) score_h(next, 0);
+            fence();
         }
-        bits = ~0u;
+        uint32_t bits = ~0u;
         if (kt >= nfull) {
-            if constexpr (kTree) bits = tree_bits(a, p, qpos, kt * kKT);
-            else {
-                const int n = qpos - kt * kKT + 1;
-                bits = n >= kKT ? ~0u : n <= 0 ? 0u : (1u << n) - 1u;
-            }
+            bits = kTree ? tree_bits(a, p, qpos, kt * kKT) : causal_bits(qpos, kt * kKT);
             const uint32_t mine = bits >> (4 * hh);
 #pragma unroll
             for (int r = 0; r < 16; ++r)
@@ -810,7 +856,12 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
         float mx = s[0];
 #pragma unroll
         for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+        read_k(i + 1, 3);
+        score_l(next, 1);
+        fence();
         mx = half_max(mx) * sq;
+        score_h(next, 1);
+        fence();
         if (__builtin_amdgcn_ballot_w64(mx > m + kLazy8)) {  // rare after the first tile
             const float mn = fmaxf(m, ceilf(mx));
             const int up = m == -INFINITY || m == mn ? 0 : (int)fminf(mn - m, 1000.f);
@@ -819,29 +870,41 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
             fe = fn;
             m = mn;
         }
+        // ---- weights times scales times F
         const float nb = m == -INFINITY ? 0.f : (float)fe - m;
-        float sum = 0.f;
+        float sum = 0.f, wm = 0.f;
+        f[0] = *reinterpret_cast<const f32x4*>(sc + kKT);
+        fence();
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            s[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r], sq, nb));
-            sum += s[r];
+        for (int c = 0; c < 4; ++c) {
+            if (c < 3) f[(c + 1) & 3] = *reinterpret_cast<const f32x4*>(sc + kKT + 8 * (c + 1));
+            read_k(i + 1, c + 4);
+            score_l(next, c + 2);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[4 * c + r] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[4 * c + r], sq, nb));
+            fence();
+            score_h(next, c + 2);
+#pragma unroll
+            for (int r = 0; r < 4; ++r) sum += s[4 * c + r];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s[4 * c + r] *= f[c][r];
+            fence();
         }
         l += sum;
-#pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            const float4 f = *reinterpret_cast<const float4*>(sc + kKT + 2 * r);
-            s[r] *= f.x, s[r + 1] *= f.y, s[r + 2] *= f.z, s[r + 3] *= f.w;
-        }
         if (kt >= nfull) {  // (a scale that the row does not see may be anything)
             const uint32_t mine = bits >> (4 * hh);
 #pragma unroll
             for (int r = 0; r < 16; ++r)
                 if (!(mine >> (8 * (r >> 2) + (r & 3)) & 1)) s[r] = 0.f;
         }
-        float wm = 0.f;
+        score_l(next, 6);
 #pragma unroll
         for (int r = 0; r < 16; ++r) wm = fmaxf(wm, __builtin_fabsf(s[r]));
+        fence();
+        score_h(next, 6);
         wm = half_max(wm);
+        fence();
+        score_l(next, 7);
         if (__builtin_amdgcn_ballot_w64(wm > limit)) {  // rare after the first tile
             // the largest: 2^14 .. 2^15
             const bool over = wm > limit;
@@ -853,150 +916,162 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
             fe = fn;
             if (over) limit = kTopW;
         }
-    };
-    // a tile whose codes of V hold a NaN that not every row sees, key by key
-    auto key_by_key = [&](int i, uint32_t bits) {
-        const Place at = place(i, page(i));
-        const Rsrc rv = codes_at(a.v8, at);
-#pragma unroll 1
-        for (int c = 0; c < kKT; ++c) {
-            float wc = 0.f;
-#pragma unroll
-            for (int r = 0; r < 16; ++r)
-                if (c == 8 * (r >> 2) + 4 * hh + (r & 3)) wc = s[r];
-            wc += lane_xor32(wc);
-#pragma unroll
-            for (int db = 0; db < 4; ++db)
-#pragma unroll
-                for (int y = 0; y < 4; ++y) {  // d = 32 db + 8y + 4hh + 0 .. 3
-                    const uint32_t v = __builtin_amdgcn_raw_buffer_load_b32(rv, c * D + 32 * db + 8 * y + 4 * hh, 0, 0);
-                    if (bits >> c & 1) {
-                        o[db][4 * y] = __builtin_fmaf(wc, value_of<false, 0>(v), o[db][4 * y]);
-                        o[db][4 * y + 1] = __builtin_fmaf(wc, value_of<false, 1>(v), o[db][4 * y + 1]);
-                        o[db][4 * y + 2] = __builtin_fmaf(wc, value_of<false, 2>(v), o[db][4 * y + 2]);
-                        o[db][4 * y + 3] = __builtin_fmaf(wc, value_of<false, 3>(v), o[db][4 * y + 3]);
-                    }
-                }
-        }
-    };
-    auto values = [&](int i, uint32_t bits) {
+        // ---- O^T += V^T . P^T
+        char* const v = buf(i) + kK8Tile + col * kV8RowB + 16 * hh;
+        auto place_of = [&](int y) { return reinterpret_cast<u32x4*>(v + 32 * (y & 3) * kV8RowB + 32 * (y >> 2)); };
         if constexpr (!kInt8) {
-            if (index(i) >= nfull) {
-                const u32x4 nan = *reinterpret_cast<const u32x4*>(lds + (i & 1) * kBuf8 + kK8Tile + kV8Tile + 2 * kKT * 4);
-                if (scalar(nan.x | nan.y | nan.z | nan.w)) return key_by_key(i, bits);
+            // A NaN that not every row sees must not meet them: zero takes its place for every wave of the group, and
+            // it is put in at the end.  (Of the codes' values only NaN has all exponent bits.)
+            if (kt >= nfull) {
+#pragma unroll
+                for (int y = 0; y < 8; ++y) {
+                    u32x4 x = *place_of(y);
+                    uint32_t nan = 0;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t n = ((x[j] & 0x7C007C00u) + 0x04000400u) & 0x80008000u;
+                        x[j] &= ~(n | (n - (n >> 15)));
+                        nan |= n;
+                    }
+                    if (__builtin_amdgcn_ballot_w64(nan != 0)) {
+                        *place_of(y) = x;
+                        *nan_met = 1;
+                    }
+                    fence();
+                }
             }
         }
-        const char* v = lds + (i & 1) * kBuf8 + kK8Tile + col * kV8RowB + 16 * hh;
-        auto frag = [&](int y) { return *reinterpret_cast<const u32x4*>(v + 32 * (y & 3) * kV8RowB + 32 * (y >> 2)); };
-        u32x4 vf[kAhead + 1], ph, pl;
+        u32x4 vf[3], ph[2], pl[2];
+        auto planes = [&](int x, int j) {  // weights 8x + 2j and the next
+            uint32_t hi, lo;
+            split_f16(s[8 * x + 2 * j], s[8 * x + 2 * j + 1], hi, lo);
+            ph[x][j] = hi, pl[x][j] = lo;
+        };
+        vf[0] = *place_of(0), vf[1] = *place_of(1);
+        score_h(next, 7);
+        fence();
 #pragma unroll
-        for (int y = 0; y < kAhead; ++y) vf[y] = frag(y);
-        __builtin_amdgcn_sched_barrier(0);
+        for (int j = 0; j < 4; ++j) planes(0, j);
+        fence();
 #pragma unroll
         for (int y = 0; y < 8; ++y) {
-            if ((y & 3) == 0) {
-                uint32_t h[4], lo[4];
+            if (y + 2 < 8) vf[(y + 2) % 3] = *place_of(y + 2);
+            o[y & 3] = mfma32(vf[y % 3], pl[y >> 2], o[y & 3]);
+            if (y < 2) planes(1, 2 * y);
+            else if (y < 4) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) split_f16(s[2 * y + 2 * j], s[2 * y + 2 * j + 1], h[j], lo[j]);
-                ph = u32x4{h[0], h[1], h[2], h[3]}, pl = u32x4{lo[0], lo[1], lo[2], lo[3]};
-            }
-            if (y + kAhead < 8) vf[(y + kAhead) % (kAhead + 1)] = frag(y + kAhead);
-            __builtin_amdgcn_sched_barrier(0);
-            o[y & 3] = mfma32(vf[y % (kAhead + 1)], pl, o[y & 3]);
-            o[y & 3] = mfma32(vf[y % (kAhead + 1)], ph, o[y & 3]);
-            __builtin_amdgcn_sched_barrier(0);
+                for (int x = 0; x < kParts; ++x) store_k(i + kLead + 1, x, y - 2);
+            } else if (y < 6) {
+#pragma unroll
+                for (int x = 0; x < kParts; ++x) store_v(i + kLead, x, y - 4);
+            } else if (y == 6) load_k(ahead);
+            fence();
+            o[y & 3] = mfma32(vf[y % 3], ph[y >> 2], o[y & 3]);
+            if (y < 2) planes(1, 2 * y + 1);
+            if (y == 5) store_scales(i + kLead);
+            if (y == 6) load_v(at);
+            if (y == 7) load_scales(at);
+            fence();
         }
+        at = ahead;
     };
-    // Tile i + 1 goes to LDS while tile i is worked on, into the places of tile i - 1.  The second group takes the next
-    // tile's scores at the end of an iteration, so its K is a tile further: K of i + 2 goes where K of i was, whose
-    // scores every wave took before the last barrier.
-    store_k(t0, 0);
-    store_v(t0, 0);
-    store_scales(t0, 0);
-    Place at = place(2, page(2));
-    int pg = page(2 + grp);  // of the K tile that is loaded next
-    if (grp == 1) {
-        store_k(t1, 1);
-        load_k(t1, at);
-        pg = page(3);
-    }
-    lds_barrier();
-    if (grp == 1 && n_mine > 0) scores(0);
-    lds_barrier();  // (K of tile 0 has been read)
-    for (int i = 0; i < n_it; ++i) {
-        // t1: V and scales of tile i + 1, K of tile i + 1 (second group: i + 2)
-        const Place ahead = place(i + 2 + grp, pg);
-        pg = page(i + 3 + grp);
-        uint32_t bits = ~0u;
-        if (grp == 0) {
-            at = ahead;
-            if (i < n_mine) scores(i);
-        }
-        if (i + 1 + grp < n_mine) store_k(t1, i + 1 + grp);
-        load_k(t1, ahead);
-        if (i < n_mine) weights(i, bits);
-        if (i + 1 < n_mine) {
-            store_v(t1, i + 1);
-            store_scales(t1, i + 1);
-        }
-        load_v(t1, at);
-        load_scales(t1, at);
-        if (i < n_mine) values(i, bits);
-        if (grp == 1) {
-            at = ahead;
-            if (i + 1 < n_mine) scores(i + 1);
-        }
+    for (int i = 0; i < n_it; i += 2) {
+        if (i < n_mine) tile(i, even, odd);
+        if constexpr (kLead == 1) lds_barrier();
+        if (i + 1 < n_mine) tile(i + 1, odd, even);
         lds_barrier();
     }
-
-    // ---- the key groups meet through LDS, as in k_packed_attn: group g finishes blocks db = 2g, 2g + 1
-    {
-        scale_sums(pow2(-fe));
-        if (m == -INFINITY) {  // (scores of -infinity beside infinite values: parts without weights are passed over)
-            float z = 0.f;
+    if constexpr (!kInt8) {
+        if (scalar(*nan_met)) {
+            // the group's tiles that not every row of the unit sees all of
+            const int low = max(kTree ? p.pos0 : p.pos0 + fdiv(min(kUnitRows * p.u, p.nflat - 1), fG) + 1, 0) / kKT;
+#pragma unroll 1
+            for (int i = 0; i < n_mine; ++i) {
+                const int t0 = index(i) * kKT;
+                if (index(i) < low) continue;
+                const uint32_t bits = kTree ? tree_bits(a, p, qpos, t0) : causal_bits(qpos, t0);
+                const Rsrc rv = codes_at(a.v8, place(i, page(i)));
+#pragma unroll 1
+                for (int c = 0; c < kKT; ++c)
 #pragma unroll
-            for (int db = 0; db < 4; ++db)
+                    for (int db = 0; db < 4; ++db)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) z = __builtin_fmaf(o[db][r], 0.f, z);
-            l += z;
+                        for (int y = 0; y < 4; ++y) {  // d = 32 db + 8y + 4hh + 0 .. 3
+                            const uint32_t x =
+                                __builtin_amdgcn_raw_buffer_load_b32(rv, c * D + 32 * db + 8 * y + 4 * hh, 0, 0);
+                            const uint32_t nan = bits >> c & 1 ? nan_bytes(x) : 0u;
+#pragma unroll
+                            for (int z = 0; z < 4; ++z)
+                                if (nan >> (8 * z) & 0x80) o[db][4 * y + z] = __builtin_nanf("");
+                        }
+            }
         }
+        lds_barrier();  // (the next pass clears the word)
     }
-    lds_barrier();  // the tiles have been read
-    float* xw = smem + w * (kXch8 * 64) + lane;
+
+    // ---- the groups meet through LDS: group g finishes the blocks of 32 d from kOwn g on
+    scale_sums(pow2(-fe));
+    if (m == -INFINITY) {  // (scores of -infinity beside infinite values: parts without weights are passed over)
+        float z = 0.f;
+#pragma unroll
+        for (int db = 0; db < 4; ++db)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) z = __builtin_fmaf(o[db][r], 0.f, z);
+        l += z;
+    }
+    constexpr int kOwn = Wide8<kS>::kOwn, kXch = Wide8<kS>::kXch;
+    float* xw = smem + w * (kXch * 64) + lane;
     xw[0] = m;
     xw[64] = l;
-    const floatx16 give0 = grp ? o[0] : o[2], give1 = grp ? o[1] : o[3];
-    const floatx16 keep0 = grp ? o[2] : o[0], keep1 = grp ? o[3] : o[1];
+    floatx16 keep[kOwn];
 #pragma unroll
-    for (int i = 0; i < 16; ++i) {
-        xw[(2 + i) * 64] = give0[i];
-        xw[(18 + i) * 64] = give1[i];
+    for (int db = 0; db < 4; ++db) {
+        if (db / kOwn != grp) {
+            float* to = xw + (2 + 16 * (db < grp * kOwn ? db : db - kOwn)) * 64;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) to[64 * i] = o[db][i];
+        } else keep[db % kOwn] = o[db];
     }
     lds_barrier();
-    float* const stage = smem + kStage8;
-    const float* xp = smem + ((1 - grp) * kSlots + hw) * (kXch8 * 64) + lane;
-    const float mp = xp[0], lp = xp[64];
-    const float mt = fmaxf(m, mp);
-    const float c0 = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - mt);
-    const float cp = mp == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mp - mt);
+    float mt = m;
+    auto of = [&](int g) { return smem + (g * kS + hw) * (kXch * 64) + lane; };
+#pragma unroll
+    for (int g = 0; g < kN; ++g) mt = fmaxf(mt, of(g)[0]);
     // (a group whose every score is NaN keeps m at -inf, and its NaN sum counts)
-    const float ls = half_sum((m == -INFINITY ? l : l * c0) + (mp == -INFINITY ? lp : lp * cp));
+    auto factor = [&](float at) { return at == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(at - mt); };
+    const float own = factor(m);
+    float ls = m == -INFINITY ? l : l * own;
+#pragma unroll
+    for (int x = 0; x < kOwn; ++x)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) keep[x][r] *= own;
+#pragma unroll
+    for (int other = 1; other < kN; ++other) {
+        const int g = (grp + other) % kN;
+        const float* xp = of(g);
+        const float mg = xp[0], lg = xp[64], c = factor(mg);
+        ls += mg == -INFINITY ? lg : lg * c;
+#pragma unroll
+        for (int x = 0; x < kOwn; ++x) {
+            const int db = grp * kOwn + x;
+            const float* from = xp + (2 + 16 * (db < g * kOwn ? db : db - kOwn)) * 64;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) keep[x][r] = __builtin_fmaf(from[64 * r], c, keep[x][r]);
+        }
+    }
+    ls = half_sum(ls);
+    float* const stage = smem + Wide8<kS>::kStage;
     {
         bool none = qpos < 0;  // a row that sees no key: zeros
         if constexpr (kTree) none = ls == 0.f && tree_sees_none(a, p.row0, p.pos0, tok);
         const float inv = p.part ? 1.f : none ? 0.f : 1.f / ls;
-        float* ost = stage + (hw * kQB + col) * kRowF + 64 * grp + 4 * hh;
+        float* ost = stage + (hw * kQB + col) * kRowF + 32 * kOwn * grp + 4 * hh;
 #pragma unroll
-        for (int r = 0; r < 16; r += 4) {
-            float v0[4], v1[4];
+        for (int x = 0; x < kOwn; ++x)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                v0[j] = (keep0[r + j] * c0 + xp[(2 + r + j) * 64] * cp) * inv;
-                v1[j] = (keep1[r + j] * c0 + xp[(18 + r + j) * 64] * cp) * inv;
-            }
-            *reinterpret_cast<float4*>(ost + 2 * r) = make_float4(v0[0], v0[1], v0[2], v0[3]);
-            *reinterpret_cast<float4*>(ost + 32 + 2 * r) = make_float4(v1[0], v1[1], v1[2], v1[3]);
-        }
+            for (int r = 0; r < 16; r += 4)  // registers r .. r + 3 of a block are d = 8 (r / 4) + 4hh + 0 .. 3 of it
+                *reinterpret_cast<float4*>(ost + 32 * x + 2 * r) =
+                    make_float4(keep[x][r] * inv, keep[x][r + 1] * inv, keep[x][r + 2] * inv, keep[x][r + 3] * inv);
         if (p.part && hh == 0 && grp == 0)
             *reinterpret_cast<float2*>(p.part + kUnitRows * D + 2 * (hw * kQB + col)) = make_float2(mt, ls);
     }
@@ -1004,12 +1079,12 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
     {
         const int ln = unhoisted(lane), c4 = 4 * (ln & 31);
 #pragma unroll
-        for (int j = 0; j < kQB / 4; ++j) {  // wave wu: rows 16 wu .. of the unit, two per instruction
-            const int jj = (kQB / 2) * wu + 2 * j + (ln >> 5), f = kUnitRows * p.u + jj;
+        for (int j = 0; j < kS * kQB / (2 * kWaves); ++j) {  // two rows per instruction
+            const int jj = 2 * (wu + kWaves * j) + (ln >> 5), g = kUnitRows * p.u + jj;
             const float4 v = *reinterpret_cast<const float4*>(stage + jj * kRowF + c4);
-            const int t = fdiv(f, fG);
-            float* dst = p.part ? p.part + jj * D : a.out + (((size_t)p.row0 + t) * a.H + kvh * G + f - t * G) * D;
-            if (f < p.nflat) *reinterpret_cast<float4*>(dst + c4) = v;
+            const int t = fdiv(g, fG);
+            float* dst = p.part ? p.part + jj * D : a.out + (((size_t)p.row0 + t) * a.H + kvh * G + g - t * G) * D;
+            if (g < p.nflat) *reinterpret_cast<float4*>(dst + c4) = v;
         }
     }
 }
@@ -1028,7 +1103,8 @@ __global__ __launch_bounds__(64 * kWaves) void k_cache8_attn(Cache8Args a, int s
     const FastDiv fG = fast_div((uint32_t)(a.H / a.HKV));
     const float sl2 = a.scale * 1.44269504088896340736f;  // scores come out in log2 units
     walk_share<false>(a, pv.wide, wide, rounds, shares, share, kvh, fG, wide_parts, [&](const Pass& p) {
-        wide8_pass<kInt8, kTree>(a, p, kvh, fG, sl2, smem);
+        if (p.nflat - kUnitRows * p.u > 2 * kQB) wide8_pass<kInt8, kTree, 4>(a, p, kvh, fG, sl2, smem);
+        else wide8_pass<kInt8, kTree, 2>(a, p, kvh, fG, sl2, smem);
     });
     lds_barrier();  // the last wide pass's rows have been read
     walk_share<true>(a, pv.few, few, 0, shares, share, kvh, fG, few_parts, [&](const Pass& p) {
@@ -1072,7 +1148,7 @@ hipError_t launch_cache_keep(hipStream_t st, const Cache8Args& a, float* kc, flo
 template <bool kInt8, bool kTree>
 static hipError_t launch_cache8_attn_as(hipStream_t st, const Cache8Args& a, int shares, const PackedParts& parts) {
     static std::atomic<bool> opted;
-    constexpr size_t lds = (size_t)kWide8F * sizeof(float);
+    constexpr size_t lds = kLds8;
     if (const hipError_t e = opt_in_lds(opted, (const void*)k_cache8_attn<kInt8, kTree>, lds); e != hipSuccess) return e;
     k_cache8_attn<kInt8, kTree><<<shares * a.HKV, 64 * kWaves, lds, st>>>(a, shares, parts.wide, parts.few);
     return hipGetLastError();
