@@ -299,306 +299,370 @@ constexpr float kTopW = 0x1p15f;                       // p s_v F at most
 constexpr float kLazy8 = 8.f;                          // the reference moves when a score passes it by more (log2 units)
 __device__ __forceinline__ float pow2(int e) { return __builtin_amdgcn_ldexpf(1.f, e); }
 
-// The unit's rows in blocks of sixteen, one per wave; waves of a block take its tiles in turn, each lane
-// its row l % 16 and quarter l / 16:
+// ---- units of up to 32 rows
+// A workgroup's share of the few-row list.  A unit's rows are one block of sixteen or two, one per wave; waves of a block
+// take its tiles in turn, each lane its row l % 16 and quarter l / 16:
 //   S^T[key][row] = K . Q^T: the lane has of key 16 kb + l % 16 codes 32 quarter .. + 31, and gets the scores of the
 //     keys 16 kb + 4 quarter + r (kb = 0, 1; r = 0 .. 3) for its row;
 //   O^T[d][row] = V^T . P^T over the tile's 32 keys in the order of those scores: the lane has codes
 //     8 (l % 16) .. + 7 of its eight keys, put together pair of keys by pair; sum y, register r is
 //     d = 32 quarter + 8 r + y.
+// Bound by reading the codes, two tiles of each wave in flight.  A pass is short where sequences are: the next unit
+// and its pages are looked up during a pass, its queries and first tiles fetched before the waves' sums meet.
 template <bool kInt8, bool kTree>
-__device__ __forceinline__ void rows_pass(const Cache8Args& a, const Pass& p, int kvh, FastDiv fG, float sl2,
-                                          int ml_at, float* smem) {
+__device__ __forceinline__ void few8_walk(const Cache8Args& a, const List& list, int4 sh, int share, int kvh, FastDiv fG,
+                                          float sl2, float* parts, float* smem) {
     constexpr int D = kHeadDim;
     const int tid = unhoisted(threadIdx.x), lane = tid & 63, wu = scalar(tid >> 6);
     const int j = lane & 15, quarter = lane >> 4;
     const int G = (int)fG.d;
-    const int f0 = kUnitRows * p.u, last = p.nflat - 1, rows = min(p.nflat - f0, kUnitRows);
-    const int nb = rows <= kRow8 ? 1 : rows <= 2 * kRow8 ? 2 : rows <= 4 * kRow8 ? 4 : 8;
-    const int rb = wu & (nb - 1), off = wu / nb, step = kWaves / nb;
-    const int row = min(f0 + kRow8 * rb + j, last);  // (rows past the last repeat it)
-    const int tok = fdiv(row, fG), qpos = p.pos0 + tok;
-    const int nfull = max(kTree ? p.pos0 : p.pos0 + fdiv(min(f0 + kRow8 * rb, last), fG) + 1, 0) / kKT;
-    const int n_mine = (p.nrange - off + step - 1) / step;
-    auto index = [&](int i) { return p.kt_lo + step * i + off; };
-    auto page = [&](int i) { return page_of<true>(a, p, index(i) * kKT); };
-    auto codes_at = [&](const uint8_t* codes, int i, int pg, bool wanted) {
-        const int t0 = index(i) * kKT;
-        const bool ok = wanted && pg >= 0 && pg < a.n_blocks;
-        return __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<uint8_t*>(codes) + (ok ? head_row(pg, a.HKV, kvh, a.bshift, t0) * D : 0), 0,
-            ok ? min(kKT, p.T - t0) * D : 0, kBufferDword3);
+    const int first = scalar(sh.x), first_tile = scalar(sh.y), last = scalar(sh.z), last_tile = scalar(sh.w);
+    auto there = [&](int at) { return at < last || (at == last && last_tile > 0); };
+    if (!there(first)) return;
+    struct Unit8 : Pass {
+        int nb, step, off, n_mine;  // blocks of rows; this wave's tiles: from `off` on every `step`-th, n_mine of them
     };
-    auto scales_at = [&](const float* scales, int i, int pg, bool wanted) {  // (whole tiles: pages hold them)
-        const bool ok = wanted && pg >= 0 && pg < a.n_blocks;
-        return __builtin_amdgcn_make_buffer_rsrc(
-            const_cast<float*>(scales) + (ok ? head_row(pg, a.HKV, kvh, a.bshift, index(i) * kKT) : 0), 0,
-            ok ? kKT * 4 : 0, kBufferDword3);
+    auto make = [&](int at, u32x4 x, u32x4 y) {
+        Unit8 p;
+        const int n = (int)x.y, len = (int)x.z, cut = at == last && last_tile > 0 ? last_tile : -1;
+        p.row0 = (int)x.x, p.u = (int)x.w, p.seq = (int)y.x;
+        p.pos0 = len - n;
+        p.nflat = n * G;
+        p.T = len;  // (a few-row unit is its sequence's last: its last row sees all)
+        p.kt_lo = at == first ? first_tile : 0;
+        p.nrange = (cut >= 0 ? cut : (int)y.y) - p.kt_lo;
+        p.part = p.kt_lo > 0 || cut >= 0 ? parts + part_at(true, share * a.HKV + kvh, p.kt_lo > 0 ? 0 : 1) : nullptr;
+        p.nb = p.nflat - kUnitRows * p.u > kRow8 ? 2 : 1;
+        p.step = kWaves / p.nb, p.off = wu / p.nb;
+        p.n_mine = (p.nrange - p.off + p.step - 1) / p.step;
+        return p;
     };
-    auto as_f32x4 = [](u32x4 x) { return __builtin_bit_cast(f32x4, x); };
-    auto load = [&](Tile8& t, int i, int pg, bool wanted) {
+    auto index = [&](const Unit8& p, int i) { return p.kt_lo + p.step * i + p.off; };
+    auto page = [&](const Unit8& p, int i) { return page_of<true>(a, p, index(p, i) * kKT); };
+    struct Place {   // of a tile
+        size_t row;  // its first head row
+        int there;   // keys of it
+    };
+    auto place = [&](const Unit8& p, int i, int pg) {
+        const int t0 = index(p, i) * kKT;
+        const bool ok = i < p.n_mine && pg >= 0 && pg < a.n_blocks;
+        return Place{ok ? head_row(pg, a.HKV, kvh, a.bshift, t0) : 0, ok ? min(kKT, p.T - t0) : 0};
+    };
+    auto codes_at = [&](const uint8_t* codes, const Place& at) {
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(codes) + at.row * D, 0, at.there * D,
+                                                 kBufferDword3);
+    };
+    auto scales_at = [&](const float* scales, const Place& at) {  // (whole tiles: pages hold them)
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(scales) + at.row, 0, at.there ? kKT * 4 : 0,
+                                                 kBufferDword3);
+    };
+    auto load = [&](Tile8& t, const Place& at) {
         const uint32_t ln = lane_now();
-        const Rsrc rk = codes_at(a.k8, i, pg, wanted), rv = codes_at(a.v8, i, pg, wanted);
-        const Rsrc sk = scales_at(a.ks, i, pg, wanted), sv = scales_at(a.vs, i, pg, wanted);
+        const Rsrc rk = codes_at(a.k8, at), rv = codes_at(a.v8, at), sk = scales_at(a.ks, at), sv = scales_at(a.vs, at);
         const uint32_t ok = (ln & 15) * D + (ln >> 4) * 32, ov = (ln >> 4) * (4 * D) + (ln & 15) * 8;
 #pragma unroll
         for (int kb = 0; kb < 2; ++kb) {
 #pragma unroll
             for (int x = 0; x < 2; ++x)
                 t.k[kb][x] = __builtin_amdgcn_raw_buffer_load_b128(rk, ok + 16 * kb * D + 16 * x, 0, 0);
-            t.ks[kb] = as_f32x4(__builtin_amdgcn_raw_buffer_load_b128(sk, (ln >> 4) * 16 + 64 * kb, 0, 0));
-            t.vs[kb] = as_f32x4(__builtin_amdgcn_raw_buffer_load_b128(sv, (ln >> 4) * 16 + 64 * kb, 0, 0));
+            t.ks[kb] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(sk, (ln >> 4) * 16 + 64 * kb, 0, 0));
+            t.vs[kb] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(sv, (ln >> 4) * 16 + 64 * kb, 0, 0));
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e)
             t.v[e] = __builtin_amdgcn_raw_buffer_load_b64(rv, ov + (16 * (e >> 2) + (e & 3)) * D, 0, 0);
     };
-
-    // q: planes of d = 32 quarter + 8 x + 0 .. 7
-    u32x4 qh[4], ql[4];
-    float sq;  // takes the row's scaling out of its scores
-    {
-        const float* src = a.q + ((size_t)p.row0 + tok) * a.q_stride + (size_t)(kvh * G + row - tok * G) * D + 32 * quarter;
-        float4 q[8];
-        float most = 0.f;
-#pragma unroll
-        for (int x = 0; x < 8; ++x) {
-            const float4 v = *reinterpret_cast<const float4*>(src + 4 * x);
-            q[x] = make_float4(v.x * sl2, v.y * sl2, v.z * sl2, v.w * sl2);
-            most = fmaxf(fmaxf(most, __builtin_fabsf(q[x].x)), __builtin_fabsf(q[x].y));
-            most = fmaxf(fmaxf(most, __builtin_fabsf(q[x].z)), __builtin_fabsf(q[x].w));
-        }
-        most = half_max(fmaxf(most, lane_xor16(most)));
-        const uint32_t f = scale_to<14>(most);
-        const float fq = __uint_as_float(f);
-        sq = inverse(f);
-#pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            uint32_t h[4], l[4];
-#pragma unroll
-            for (int y = 0; y < 2; ++y) {
-                const float4 v = q[2 * x + y];
-                split_f16(v.x * fq, v.y * fq, h[2 * y], l[2 * y]);
-                split_f16(v.z * fq, v.w * fq, h[2 * y + 1], l[2 * y + 1]);
-            }
-            qh[x] = u32x4{h[0], h[1], h[2], h[3]};
-            ql[x] = u32x4{l[0], l[1], l[2], l[3]};
-        }
-    }
-    f32x4 o[8];
-    float m = -INFINITY, l = 0.f, limit = 0.f;  // (limit of a row without weights so far)
-    int fe = 0;                                 // log2 F
-#pragma unroll
-    for (int y = 0; y < 8; ++y) o[y] = f32x4{0.f, 0.f, 0.f, 0.f};
-    auto scale_sums = [&](float by) {
-        l *= by;
-#pragma unroll
-        for (int y = 0; y < 8; ++y)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) o[y][r] *= by;
+    // this lane's row of a unit (rows past the last repeat it), and its query, d = 32 quarter .. + 31
+    auto row_of = [&](const Unit8& p) {
+        return min(kUnitRows * p.u + kRow8 * (wu & (p.nb - 1)) + j, p.nflat - 1);
     };
-    auto row_max = [&](float x) { return half_max(fmaxf(x, lane_xor16(x))); };
-
-    int nan_tile = n_mine;  // the first with a NaN code that not every row sees
-    auto tile = [&](Tile8& t, int i) {
-        const int kt = index(i);
-        f32x4 s[2];
+    float4 q[8];
+    auto load_q = [&](const Unit8& p) {
+        const int row = row_of(p), tok = fdiv(row, fG);
+        const float* src = a.q + ((size_t)p.row0 + tok) * a.q_stride + (size_t)(kvh * G + row - tok * G) * D + 32 * quarter;
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-            s[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int x = 0; x < 8; ++x) q[x] = *reinterpret_cast<const float4*>(src + 4 * x);
+    };
+
+    const u32x4* unit = reinterpret_cast<const u32x4*>(&list.shares[share].start);  // a Unit's fields, in order
+    Unit8 p = make(first, scalar_load(unit), scalar_load(unit + 1));
+    Tile8 t0, t1;
+    int pg;  // of tile 2
+    auto begin = [&](const Unit8& p, int p0, int p1) {
+        load_q(p);
+        load(t0, place(p, 0, p0));
+        load(t1, place(p, 1, p1));
+    };
+    begin(p, page(p, 0), page(p, 1));
+    pg = page(p, 2);
+    for (int at = first, turn = 0;; ++at, ++turn) {
+        const bool more = there(at + 1);
+        unit = reinterpret_cast<const u32x4*>(more ? list.units + at + 1 : &list.shares[share].start);
+        const u32x4 nx = scalar_load(unit), ny = scalar_load(unit + 1);
+        const int tok = fdiv(row_of(p), fG), qpos = p.pos0 + tok;
+        const int f0 = kUnitRows * p.u, block0 = min(f0 + kRow8 * (wu & (p.nb - 1)), p.nflat - 1);
+        const int nfull = max(kTree ? p.pos0 : p.pos0 + fdiv(block0, fG) + 1, 0) / kKT;
+        // q: planes of d = 32 quarter + 8 x + 0 .. 7
+        u32x4 qh[4], ql[4];
+        float sq;  // takes the row's scaling out of its scores
+        {
+            float most = 0.f;
+#pragma unroll
+            for (int x = 0; x < 8; ++x) {
+                q[x] = make_float4(q[x].x * sl2, q[x].y * sl2, q[x].z * sl2, q[x].w * sl2);
+                most = fmaxf(fmaxf(most, __builtin_fabsf(q[x].x)), __builtin_fabsf(q[x].y));
+                most = fmaxf(fmaxf(most, __builtin_fabsf(q[x].z)), __builtin_fabsf(q[x].w));
+            }
+            most = half_max(fmaxf(most, lane_xor16(most)));
+            const uint32_t f = scale_to<14>(most);
+            const float fq = __uint_as_float(f);
+            sq = inverse(f);
 #pragma unroll
             for (int x = 0; x < 4; ++x) {
-                const uint32_t lo = flipped<kInt8>(t.k[kb][x >> 1][2 * (x & 1)]);
-                const uint32_t hi = flipped<kInt8>(t.k[kb][x >> 1][2 * (x & 1) + 1]);
-                const u32x4 kf = {pair_f16<kInt8, 0>(lo), pair_f16<kInt8, 1>(lo), pair_f16<kInt8, 0>(hi),
-                                  pair_f16<kInt8, 1>(hi)};
-                s[kb] = mfma16(kf, ql[x], s[kb]);
-                s[kb] = mfma16(kf, qh[x], s[kb]);
+                uint32_t h[4], l[4];
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    const float4 v = q[2 * x + y];
+                    split_f16(v.x * fq, v.y * fq, h[2 * y], l[2 * y]);
+                    split_f16(v.z * fq, v.w * fq, h[2 * y + 1], l[2 * y + 1]);
+                }
+                qh[x] = u32x4{h[0], h[1], h[2], h[3]};
+                ql[x] = u32x4{l[0], l[1], l[2], l[3]};
             }
         }
-        uint32_t bits = ~0u;
-        if (kt >= nfull) {
-            bits = kTree ? tree_bits(a, p, qpos, kt * kKT) : causal_bits(qpos, kt * kKT);
-        }
-        const uint32_t mine = bits >> (4 * quarter);
-        auto seen = [&](int r) { return (mine >> (16 * (r >> 2) + (r & 3)) & 1) != 0; };
-        float mx = -INFINITY;
+        f32x4 o[8];
+        float m = -INFINITY, l = 0.f, limit = 0.f;  // (limit of a row without weights so far)
+        int fe = 0;                                 // log2 F
 #pragma unroll
-        for (int r = 0; r < 8; ++r) s[r >> 2][r & 3] *= t.ks[r >> 2][r & 3];
-        if (kt >= nfull) {
+        for (int y = 0; y < 8; ++y) o[y] = f32x4{0.f, 0.f, 0.f, 0.f};
+        auto scale_sums = [&](float by) {
+            l *= by;
 #pragma unroll
-            for (int r = 0; r < 8; ++r)
-                if (!seen(r)) s[r >> 2][r & 3] = -INFINITY;
-        }
+            for (int y = 0; y < 8; ++y)
 #pragma unroll
-        for (int r = 0; r < 8; ++r) mx = fmaxf(mx, s[r >> 2][r & 3]);
-        mx = row_max(mx) * sq;
-        if (__builtin_amdgcn_ballot_w64(mx > m + kLazy8)) {  // rare after the first tile
-            const float mn = fmaxf(m, ceilf(mx));
-            const int up = m == -INFINITY || m == mn ? 0 : (int)fminf(mn - m, 1000.f);
-            const int fn = min(fe + up, kTopF);  // the sums stay where F can go up by as much
-            if (__builtin_amdgcn_ballot_w64(fn - fe != up)) scale_sums(pow2(fn - fe - up));
-            fe = fn;
-            m = mn;
-        }
-        const float nb = m == -INFINITY ? 0.f : (float)fe - m;
-        float sum = 0.f, wm = 0.f;
-        float wt[8];
+                for (int r = 0; r < 4; ++r) o[y][r] *= by;
+        };
+        auto row_max = [&](float x) { return half_max(fmaxf(x, lane_xor16(x))); };
+
+        int nan_tile = p.n_mine;  // the first with a NaN code that not every row sees
+        auto tile = [&](Tile8& t, int i) {
+            const int kt = index(p, i);
+            f32x4 s[2];
 #pragma unroll
-        for (int r = 0; r < 8; ++r) {
-            const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r >> 2][r & 3], sq, nb));
-            sum += pr;
-            wt[r] = pr * t.vs[r >> 2][r & 3];
-        }
-        l += sum;
-        if (kt >= nfull) {  // (a scale that the row does not see may be anything)
+            for (int kb = 0; kb < 2; ++kb) {
+                s[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int r = 0; r < 8; ++r)
-                if (!seen(r)) wt[r] = 0.f;
-        }
-#pragma unroll
-        for (int r = 0; r < 8; ++r) wm = fmaxf(wm, __builtin_fabsf(wt[r]));
-        wm = row_max(wm);
-        if (__builtin_amdgcn_ballot_w64(wm > limit)) {  // rare after the first tile
-            // the largest: 2^14 .. 2^15
-            const bool over = wm > limit;
-            const int fn = over ? min(fe + 127 + 14 - (int)min(__float_as_uint(wm) >> 23, 254u), kTopF) : fe;
-            const float by = pow2(fn - fe);
-            scale_sums(by);
-#pragma unroll
-            for (int r = 0; r < 8; ++r) wt[r] *= by;
-            fe = fn;
-            if (over) limit = kTopW;
-        }
-        uint32_t wh[4], wl[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) split_f16(wt[2 * r], wt[2 * r + 1], wh[r], wl[r]);
-        const u32x4 ph = {wh[0], wh[1], wh[2], wh[3]}, pl = {wl[0], wl[1], wl[2], wl[3]};
-        if constexpr (!kInt8) {
-            if (kt >= nfull) {  // a NaN that not every row sees must not meet them: put in at the end
-                uint32_t nan = 0;
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        nan |= nan_bytes(t.v[e][x]);
-                        t.v[e][x] = without_nan(t.v[e][x]);
-                    }
-                if (__builtin_amdgcn_ballot_w64(nan != 0)) nan_tile = min(nan_tile, i);
+                for (int x = 0; x < 4; ++x) {
+                    const uint32_t lo = flipped<kInt8>(t.k[kb][x >> 1][2 * (x & 1)]);
+                    const uint32_t hi = flipped<kInt8>(t.k[kb][x >> 1][2 * (x & 1) + 1]);
+                    const u32x4 kf = {pair_f16<kInt8, 0>(lo), pair_f16<kInt8, 1>(lo), pair_f16<kInt8, 0>(hi),
+                                      pair_f16<kInt8, 1>(hi)};
+                    s[kb] = mfma16(kf, ql[x], s[kb]);
+                    s[kb] = mfma16(kf, qh[x], s[kb]);
+                }
             }
-        }
+            uint32_t bits = ~0u;
+            if (kt >= nfull) {
+                bits = kTree ? tree_bits(a, p, qpos, kt * kKT) : causal_bits(qpos, kt * kKT);
+            }
+            const uint32_t mine = bits >> (4 * quarter);
+            auto seen = [&](int r) { return (mine >> (16 * (r >> 2) + (r & 3)) & 1) != 0; };
+            float mx = -INFINITY;
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-            uint32_t vf[4][4];
+            for (int r = 0; r < 8; ++r) s[r >> 2][r & 3] *= t.ks[r >> 2][r & 3];
+            if (kt >= nfull) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {  // keys 2e, 2e + 1 of the lane's eight
-                const uint32_t u = t.v[2 * e][x], w = t.v[2 * e + 1][x];
-                const uint32_t lo = flipped<kInt8>(__builtin_amdgcn_perm(w, u, 0x05010400u));
-                const uint32_t hi = flipped<kInt8>(__builtin_amdgcn_perm(w, u, 0x07030602u));
-                vf[0][e] = pair_f16<kInt8, 0>(lo), vf[1][e] = pair_f16<kInt8, 1>(lo);
-                vf[2][e] = pair_f16<kInt8, 0>(hi), vf[3][e] = pair_f16<kInt8, 1>(hi);
+                for (int r = 0; r < 8; ++r)
+                    if (!seen(r)) s[r >> 2][r & 3] = -INFINITY;
             }
 #pragma unroll
-            for (int y = 0; y < 4; ++y) {
-                const u32x4 v = {vf[y][0], vf[y][1], vf[y][2], vf[y][3]};
-                o[4 * x + y] = mfma16(v, pl, o[4 * x + y]);
-                o[4 * x + y] = mfma16(v, ph, o[4 * x + y]);
+            for (int r = 0; r < 8; ++r) mx = fmaxf(mx, s[r >> 2][r & 3]);
+            mx = row_max(mx) * sq;
+            if (__builtin_amdgcn_ballot_w64(mx > m + kLazy8)) {  // rare after the first tile
+                const float mn = fmaxf(m, ceilf(mx));
+                const int up = m == -INFINITY || m == mn ? 0 : (int)fminf(mn - m, 1000.f);
+                const int fn = min(fe + up, kTopF);  // the sums stay where F can go up by as much
+                if (__builtin_amdgcn_ballot_w64(fn - fe != up)) scale_sums(pow2(fn - fe - up));
+                fe = fn;
+                m = mn;
             }
-        }
-    };
-    Tile8 t0, t1;
-    if (n_mine > 0) {
-        int p0 = page(0), p1 = page(1);
-        load(t0, 0, p0, true);
-        for (int i = 0; i < n_mine; i += 2) {
-            load(t1, i + 1, p1, i + 1 < n_mine);
-            const int p2 = page(i + 2);
-            __builtin_amdgcn_sched_barrier(0);
+            const float nb = m == -INFINITY ? 0.f : (float)fe - m;
+            float sum = 0.f, wm = 0.f;
+            float wt[8];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                const float pr = __builtin_amdgcn_exp2f(__builtin_fmaf(s[r >> 2][r & 3], sq, nb));
+                sum += pr;
+                wt[r] = pr * t.vs[r >> 2][r & 3];
+            }
+            l += sum;
+            if (kt >= nfull) {  // (a scale that the row does not see may be anything)
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (!seen(r)) wt[r] = 0.f;
+            }
+#pragma unroll
+            for (int r = 0; r < 8; ++r) wm = fmaxf(wm, __builtin_fabsf(wt[r]));
+            wm = row_max(wm);
+            if (__builtin_amdgcn_ballot_w64(wm > limit)) {  // rare after the first tile
+                // the largest: 2^14 .. 2^15
+                const bool over = wm > limit;
+                const int fn = over ? min(fe + 127 + 14 - (int)min(__float_as_uint(wm) >> 23, 254u), kTopF) : fe;
+                const float by = pow2(fn - fe);
+                scale_sums(by);
+#pragma unroll
+                for (int r = 0; r < 8; ++r) wt[r] *= by;
+                fe = fn;
+                if (over) limit = kTopW;
+            }
+            uint32_t wh[4], wl[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) split_f16(wt[2 * r], wt[2 * r + 1], wh[r], wl[r]);
+            const u32x4 ph = {wh[0], wh[1], wh[2], wh[3]}, pl = {wl[0], wl[1], wl[2], wl[3]};
+            if constexpr (!kInt8) {
+                if (kt >= nfull) {  // a NaN that not every row sees must not meet them: put in at the end
+                    uint32_t nan = 0;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+#pragma unroll
+                        for (int x = 0; x < 2; ++x) {
+                            nan |= nan_bytes(t.v[e][x]);
+                            t.v[e][x] = without_nan(t.v[e][x]);
+                        }
+                    if (__builtin_amdgcn_ballot_w64(nan != 0)) nan_tile = min(nan_tile, i);
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                uint32_t vf[4][4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {  // keys 2e, 2e + 1 of the lane's eight
+                    const uint32_t u = t.v[2 * e][x], w = t.v[2 * e + 1][x];
+                    const uint32_t lo = flipped<kInt8>(__builtin_amdgcn_perm(w, u, 0x05010400u));
+                    const uint32_t hi = flipped<kInt8>(__builtin_amdgcn_perm(w, u, 0x07030602u));
+                    vf[0][e] = pair_f16<kInt8, 0>(lo), vf[1][e] = pair_f16<kInt8, 1>(lo);
+                    vf[2][e] = pair_f16<kInt8, 0>(hi), vf[3][e] = pair_f16<kInt8, 1>(hi);
+                }
+#pragma unroll
+                for (int y = 0; y < 4; ++y) {
+                    const u32x4 v = {vf[y][0], vf[y][1], vf[y][2], vf[y][3]};
+                    o[4 * x + y] = mfma16(v, pl, o[4 * x + y]);
+                    o[4 * x + y] = mfma16(v, ph, o[4 * x + y]);
+                }
+            }
+        };
+        const Unit8 next = more ? make(at + 1, nx, ny) : p;
+        int n0 = -1, n1 = -1;  // the next unit's first pages
+        for (int i = 0; i < p.n_mine; i += 2) {
+            if (i == 0 && more) n0 = page(next, 0), n1 = page(next, 1);
+            const int p3 = page(p, i + 3);
             tile(t0, i);
             __builtin_amdgcn_sched_barrier(0);
-            if (i + 1 >= n_mine) break;
-            load(t0, i + 2, p2, i + 2 < n_mine);
-            const int p3 = page(i + 3);
+            if (i + 2 < p.n_mine) load(t0, place(p, i + 2, pg));
             __builtin_amdgcn_sched_barrier(0);
-            tile(t1, i + 1);
+            if (i + 1 < p.n_mine) tile(t1, i + 1);
             __builtin_amdgcn_sched_barrier(0);
-            p0 = p2, p1 = p3;
+            if (i + 3 < p.n_mine) load(t1, place(p, i + 3, p3));
+            pg = page(p, i + 4);
+            __builtin_amdgcn_sched_barrier(0);
         }
-    }
-    if constexpr (!kInt8) {
+        if constexpr (!kInt8) {
 #pragma unroll 1
-        for (int i = nan_tile; i < n_mine; ++i) {
-            const int t0 = index(i) * kKT;
-            const uint32_t bits = kTree ? tree_bits(a, p, qpos, t0) : causal_bits(qpos, t0);
-            const Rsrc rv = codes_at(a.v8, i, page(i), true);
+            for (int i = nan_tile; i < p.n_mine; ++i) {
+                const int k0 = index(p, i) * kKT;
+                const uint32_t bits = kTree ? tree_bits(a, p, qpos, k0) : causal_bits(qpos, k0);
+                const Rsrc rv = codes_at(a.v8, place(p, i, page(p, i)));
 #pragma unroll 1
-            for (int c = 0; c < kKT; ++c) {
+                for (int c = 0; c < kKT; ++c) {
 #pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(rv, c * D + 32 * quarter + 16 * x, 0, 0);
+                    for (int x = 0; x < 2; ++x) {
+                        const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(rv, c * D + 32 * quarter + 16 * x, 0, 0);
 #pragma unroll
-                    for (int y = 0; y < 4; ++y) {  // d = 32 quarter + 16x + 4y + 0 .. 3
-                        const uint32_t nan = bits >> c & 1 ? nan_bytes(v[y]) : 0u;
+                        for (int y = 0; y < 4; ++y) {  // d = 32 quarter + 16x + 4y + 0 .. 3
+                            const uint32_t nan = bits >> c & 1 ? nan_bytes(v[y]) : 0u;
 #pragma unroll
-                        for (int z = 0; z < 4; ++z)
-                            if (nan >> (8 * z) & 0x80) o[4 * (y & 1) + z][2 * x + (y >> 1)] = __builtin_nanf("");
+                            for (int z = 0; z < 4; ++z)
+                                if (nan >> (8 * z) & 0x80) o[4 * (y & 1) + z][2 * x + (y >> 1)] = __builtin_nanf("");
+                        }
                     }
                 }
             }
         }
-    }
-    // every wave's rows meet
-    float* const own = smem + wu * (kRow8 * kRowF);
-    float* const ml = smem + kFew8ML;
-    {
-        const float f = pow2(-fe);
-        l *= f;
-        if (m == -INFINITY) {  // (scores of -infinity beside infinite values: parts without weights are passed over)
-            float z = 0.f;
-#pragma unroll
-            for (int y = 0; y < 8; ++y)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) z = __builtin_fmaf(o[y][r], 0.f, z);
-            l += z;
+        if (more) {
+            if (p.n_mine <= 0) n0 = page(next, 0), n1 = page(next, 1);
+            begin(next, n0, n1);
+            pg = page(next, 2);
         }
-        const float sum = half_sum(l + lane_xor16(l));
+        __builtin_amdgcn_sched_barrier(0);
+        // every wave's rows meet, in one of two areas in turn: nobody is further than a pass ahead
+        float* const area = smem + (turn & 1) * kFew8F;
+        float* const own = area + wu * (kRow8 * kRowF);
+        float* const ml = area + kFew8ML;
+        {
+            const float f = pow2(-fe);
+            l *= f;
+            if (m == -INFINITY) {  // (scores of -infinity beside infinite values: parts without weights are passed over)
+                float z = 0.f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
+                for (int y = 0; y < 8; ++y)
 #pragma unroll
-            for (int y = 0; y < 8; y += 4)
-                *reinterpret_cast<float4*>(own + j * kRowF + 32 * quarter + 8 * r + y) =
-                    make_float4(o[y][r] * f, o[y + 1][r] * f, o[y + 2][r] * f, o[y + 3][r] * f);
-        if (quarter == 0) *reinterpret_cast<float2*>(ml + 2 * (wu * kRow8 + j)) = make_float2(m, sum);
-    }
-    lds_barrier();
-    const int d = 4 * (lane & 31);
-    for (int i = 2 * wu + (lane >> 5); i < rows; i += 2 * kWaves) {
-        const int b = i >> 4, at = i & 15;
-        float M = -INFINITY, L = 0.f;
-        for (int w = b; w < kWaves; w += nb) M = fmaxf(M, ml[2 * (w * kRow8 + at)]);
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        for (int w = b; w < kWaves; w += nb) {
-            const float2 e = *reinterpret_cast<const float2*>(ml + 2 * (w * kRow8 + at));
-            // (a wave whose every score is NaN keeps m at -inf, and its NaN sum counts)
-            const float c = e.x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(e.x - M);
-            L += e.x == -INFINITY ? e.y : e.y * c;
-            const float4 v = *reinterpret_cast<const float4*>(smem + (w * kRow8 + at) * kRowF + d);
-            x.x = __builtin_fmaf(c, v.x, x.x), x.y = __builtin_fmaf(c, v.y, x.y);
-            x.z = __builtin_fmaf(c, v.z, x.z), x.w = __builtin_fmaf(c, v.w, x.w);
+                    for (int r = 0; r < 4; ++r) z = __builtin_fmaf(o[y][r], 0.f, z);
+                l += z;
+            }
+            const float sum = half_sum(l + lane_xor16(l));
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+#pragma unroll
+                for (int y = 0; y < 8; y += 4)
+                    *reinterpret_cast<float4*>(own + j * kRowF + 32 * quarter + 8 * r + y) =
+                        make_float4(o[y][r] * f, o[y + 1][r] * f, o[y + 2][r] * f, o[y + 3][r] * f);
+            if (quarter == 0) *reinterpret_cast<float2*>(ml + 2 * (wu * kRow8 + j)) = make_float2(m, sum);
         }
-        const int g = f0 + i, t = fdiv(g, fG);
-        float* dst;
-        if (p.part) {
-            dst = p.part + i * D;
-            if (d == 0) *reinterpret_cast<float2*>(p.part + ml_at + 2 * i) = make_float2(M, L);
-        } else {
-            dst = a.out + (((size_t)p.row0 + t) * a.H + kvh * G + g - t * G) * D;
-            bool none = p.pos0 + t < 0;  // a row that sees no key: zeros
-            if constexpr (kTree) none = L == 0.f && tree_sees_none(a, p.row0, p.pos0, t);
-            const float inv = none ? 0.f : 1.f / L;
-            x.x *= inv, x.y *= inv, x.z *= inv, x.w *= inv;
-        }
-        *reinterpret_cast<float4*>(dst + d) = x;
+        lds_barrier();
+        const int rows = p.nflat - f0;
+        auto meet = [&](auto blocks) {
+            constexpr int kB = decltype(blocks)::value, kW = kWaves / kB;  // waves of a block
+            const int d = 4 * (lane & 31);
+            for (int i = 2 * wu + (lane >> 5); i < rows; i += 2 * kWaves) {
+                const int b = kB == 1 ? 0 : i >> 4, r = i & 15;
+                float2 e[kW];
+                float4 v[kW];
+                float M = -INFINITY, L = 0.f;
+#pragma unroll
+                for (int w = 0; w < kW; ++w) {
+                    e[w] = *reinterpret_cast<const float2*>(ml + 2 * ((kB * w + b) * kRow8 + r));
+                    v[w] = *reinterpret_cast<const float4*>(area + ((kB * w + b) * kRow8 + r) * kRowF + d);
+                }
+#pragma unroll
+                for (int w = 0; w < kW; ++w) M = fmaxf(M, e[w].x);
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int w = 0; w < kW; ++w) {
+                    // (a wave whose every score is NaN keeps m at -inf, and its NaN sum counts)
+                    const float c = e[w].x == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(e[w].x - M);
+                    L += e[w].x == -INFINITY ? e[w].y : e[w].y * c;
+                    x.x = __builtin_fmaf(c, v[w].x, x.x), x.y = __builtin_fmaf(c, v[w].y, x.y);
+                    x.z = __builtin_fmaf(c, v[w].z, x.z), x.w = __builtin_fmaf(c, v[w].w, x.w);
+                }
+                const int g = f0 + i, t = fdiv(g, fG);
+                float* dst;
+                if (p.part) {
+                    dst = p.part + i * D;
+                    if (d == 0) *reinterpret_cast<float2*>(p.part + kFewRows * D + 2 * i) = make_float2(M, L);
+                } else {
+                    dst = a.out + (((size_t)p.row0 + t) * a.H + kvh * G + g - t * G) * D;
+                    bool none = p.pos0 + t < 0;  // a row that sees no key: zeros
+                    if constexpr (kTree) none = L == 0.f && tree_sees_none(a, p.row0, p.pos0, t);
+                    const float inv = none ? 0.f : 1.f / L;
+                    x.x *= inv, x.y *= inv, x.z *= inv, x.w *= inv;
+                }
+                *reinterpret_cast<float4*>(dst + d) = x;
+            }
+        };
+        if (p.nb == 1) meet(std::integral_constant<int, 1>{});
+        else meet(std::integral_constant<int, 2>{});
+        if (!more) break;
+        p = next;
     }
 }
 
@@ -630,7 +694,7 @@ struct Wide8 {
 };
 constexpr int kNanAt8 = Wide8<4>::kF > Wide8<2>::kF ? Wide8<4>::kF : Wide8<2>::kF;  // a word: NaN codes were met
 constexpr int kLds8 = 4 * (kNanAt8 + 4);
-static_assert(kLds8 <= 160 * 1024 && kFew8F <= kNanAt8, "LDS budget");
+static_assert(kLds8 <= 160 * 1024 && 2 * kFew8F <= kNanAt8, "LDS budget");
 __device__ __forceinline__ floatx16 mfma32(u32x4 a, u32x4 b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
                                                   0);
@@ -1107,9 +1171,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_cache8_attn(Cache8Args a, int s
         else wide8_pass<kInt8, kTree, 2>(a, p, kvh, fG, sl2, smem);
     });
     lds_barrier();  // the last wide pass's rows have been read
-    walk_share<true>(a, pv.few, few, 0, shares, share, kvh, fG, few_parts, [&](const Pass& p) {
-        rows_pass<kInt8, kTree>(a, p, kvh, fG, sl2, kFewRows * kHeadDim, smem);
-    });
+    few8_walk<kInt8, kTree>(a, pv.few, few, share, kvh, fG, sl2, few_parts, smem);
 }
 
 // ------------------------------------------------------------------ launchers
