@@ -398,6 +398,7 @@ class PackedBatch:
             raise ValueError("invalid packed batch shape")
         self.buf = torch.empty(self.nbytes, dtype=torch.uint8, device=device)
         self.ws = torch.empty(self.ws_nbytes, dtype=torch.uint8, device=device)
+        self._device = self.buf.get_device()
         self.n_seq = 0  # no plan yet
         self.rows = 0
         self.prompts = False
@@ -566,28 +567,52 @@ class Cache8:
         self._c = _capi.Cache8C(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), number,
                                 self.n_blocks, self.block_size)
         self._at = ctypes.addressof(self._c)
+        self._device = k.get_device()
 
 
-def _cache8_args(cache: Cache8, block_table: torch.Tensor, batch: PackedBatch, n_head_kv: int) -> tuple:
-    if cache.n_head_kv != n_head_kv:
-        raise ValueError(f"the cache holds {cache.n_head_kv} KV heads, the call has {n_head_kv}")
-    if cache.k.get_device() != _device():
-        _refuse("the cache", cache.k, cache.k.dtype)
-    return cache._at, *_table_args(block_table, batch)
+# (A call's launch takes 4 us of host time; its checks, with a function and a message for each, took as much again.  So
+# each tensor's properties are asked for once, on the device `dev` that was asked for once, and what is wrong is found
+# out where something is.)
+def _check_batch(batch: PackedBatch, shape: AttnShape, dev: int) -> None:
+    if (batch.n_seq == 0 or batch._device != dev or batch.n_head != shape.n_head or
+            batch.n_head_kv != shape.n_head_kv):
+        batch._check(shape)
 
 
-def _table_args(block_table: torch.Tensor, batch: PackedBatch) -> tuple:
-    _need_contiguous("block_table", block_table, torch.int32)
-    if block_table.dim() != 2 or block_table.shape[0] < batch.n_seq:
-        raise ValueError(f"block_table must be [{batch.n_seq}, blocks], got {tuple(block_table.shape)}")
-    return block_table.data_ptr(), block_table.shape[1]
-
-
-def _need_cached(batch: PackedBatch) -> None:
-    """A batch that is not planned yet is refused, and one on another device."""
+def _check_planned(batch: PackedBatch, dev: int) -> None:
     if batch.n_seq == 0:
         raise ValueError("the batch has no plan yet: call plan() first")
-    batch._check_device()
+    if batch._device != dev:
+        batch._check_device()
+
+
+def _stride_of(name: str, t: torch.Tensor, rows: int, width: int, dev: int) -> int:
+    """_rows_of, for the usual matrix."""
+    shape, stride = t.shape, t.stride()
+    if (len(shape) == 2 and shape[0] >= rows and shape[0] > 1 and shape[1] >= width and stride[1] == 1 and
+            t.dtype is torch.float32 and t.get_device() == dev):
+        return stride[0]
+    return _rows_of(name, t, rows, width)
+
+
+def _out_of(batch: PackedBatch, out: torch.Tensor | None, dev: int) -> torch.Tensor:
+    if (out is not None and out.dtype is torch.float32 and out.get_device() == dev and
+            out.numel() >= batch.rows * batch.n_head * HEAD_DIM and out.is_contiguous()):
+        return out
+    return batch._out(out, batch.buf.device)
+
+
+def _cache8_args(cache: Cache8, block_table: torch.Tensor, batch: PackedBatch, n_head_kv: int, dev: int) -> tuple:
+    if cache.n_head_kv != n_head_kv:
+        raise ValueError(f"the cache holds {cache.n_head_kv} KV heads, the call has {n_head_kv}")
+    if cache._device != dev:
+        _refuse("the cache", cache.k, cache.k.dtype)
+    shape = block_table.shape
+    if (block_table.dtype is not torch.int32 or block_table.get_device() != dev or len(shape) != 2 or
+            shape[0] < batch.n_seq or not block_table.is_contiguous()):
+        _need_contiguous("block_table", block_table, torch.int32)
+        raise ValueError(f"block_table must be [{batch.n_seq}, blocks], got {tuple(shape)}")
+    return cache._at, block_table.data_ptr(), shape[1]
 
 
 def _mask_args(mask: torch.Tensor | None, rows: int) -> tuple:
@@ -600,18 +625,24 @@ def _mask_args(mask: torch.Tensor | None, rows: int) -> tuple:
 
 
 def _turn_args(cs: torch.Tensor, pos: torch.Tensor | None, shape: AttnShape, rows: int, q_gamma: torch.Tensor,
-               k_gamma: torch.Tensor) -> tuple:
+               k_gamma: torch.Tensor, dev: int) -> tuple:
     """q_gamma, k_gamma, cs, n_pos, turn_at, rope_dim, eps."""
+    f32 = torch.float32
     for name, t in (("q_gamma", q_gamma), ("k_gamma", k_gamma)):
         if t is None:
             raise ValueError(f"{name} is missing")
-        _need_gamma(name, t)
-    n_pos = _table_positions(cs, shape.rope_dim)
+        if t.dtype is not f32 or t.get_device() != dev or t.numel() != HEAD_DIM or not t.is_contiguous():
+            _need_gamma(name, t)
+    table = cs.shape
+    if (len(table) != 3 or table[1] != shape.rope_dim // 2 or table[2] != 2 or cs.dtype is not f32 or
+            cs.get_device() != dev or not cs.is_contiguous()):
+        _table_positions(cs, shape.rope_dim)
     if pos is not None:
         _need_contiguous("pos", pos, torch.int32)
         if pos.numel() < rows:
             raise ValueError(f"pos must hold {rows} positions, got {pos.numel()}")
-    return (q_gamma.data_ptr(), k_gamma.data_ptr(), cs.data_ptr(), n_pos, _ptr(pos), shape.rope_dim, float(shape.eps))
+        pos = pos.data_ptr()
+    return q_gamma.data_ptr(), k_gamma.data_ptr(), cs.data_ptr(), table[0], pos, shape.rope_dim, shape.eps
 
 
 def cache8_store(qkv: torch.Tensor, cache: Cache8, block_table: torch.Tensor, batch: PackedBatch, shape: AttnShape,
@@ -620,13 +651,14 @@ def cache8_store(qkv: torch.Tensor, cache: Cache8, block_table: torch.Tensor, ba
     """Norms, turns and quantises the batch's new rows from raw projections qkv [rows, >= (H+2HKV)*128] into their
     sequences' pages, and returns the normed and turned queries [rows, H, 128] (ei_cache8_store).  pos
     int32 [rows]: positions other than the rows' slots, as of a tree's tokens."""
-    batch._check(shape)
-    rs = _rows_of("qkv", qkv, batch.rows, shape.qkv)
-    where = _cache8_args(cache, block_table, batch, shape.n_head_kv)
-    turn = _turn_args(cs, pos, shape, batch.rows, q_gamma, k_gamma)
-    out = batch._out(out, qkv.device)
+    dev = _device()
+    _check_batch(batch, shape, dev)
+    rs = _stride_of("qkv", qkv, batch.rows, shape.qkv, dev)
+    where = _cache8_args(cache, block_table, batch, shape.n_head_kv, dev)
+    turn = _turn_args(cs, pos, shape, batch.rows, q_gamma, k_gamma, dev)
+    out = _out_of(batch, out, dev)
     if batch.rows:
-        _capi.call("ei_cache8_store", _stream(), qkv.data_ptr(), rs, out.data_ptr(), *where, batch.n_seq, batch.rows,
+        _capi.call("ei_cache8_store", torch._C._cuda_getCurrentRawStream(dev), qkv.data_ptr(), rs, out.data_ptr(), *where, batch.n_seq, batch.rows,
                    shape.n_head, shape.n_head_kv, shape.head_dim, *turn, batch.buf.data_ptr(), batch.nbytes)
     return out
 
@@ -635,8 +667,9 @@ def cache8_load(cache: Cache8, block_table: torch.Tensor, batch: PackedBatch,
                 out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The cached keys and values of the batch's new rows in 32 bits, [rows, HKV, 128] each (ei_cache8_load); a batch
     planned with longer runs of rows reads more of the sequences.  out: two tensors of one row stride."""
-    _need_cached(batch)
-    where = _cache8_args(cache, block_table, batch, batch.n_head_kv)
+    dev = _device()
+    _check_planned(batch, dev)
+    where = _cache8_args(cache, block_table, batch, batch.n_head_kv, dev)
     width = cache.n_head_kv * HEAD_DIM
     if out is None:
         out = tuple(torch.empty((batch.rows, cache.n_head_kv, HEAD_DIM), dtype=torch.float32, device=cache.k.device)
@@ -646,7 +679,7 @@ def cache8_load(cache: Cache8, block_table: torch.Tensor, batch: PackedBatch,
     if ks != vs:
         raise ValueError(f"the two outputs must share a row stride, got {ks} and {vs}")
     if batch.rows:
-        _capi.call("ei_cache8_load", _stream(), *where, k.data_ptr(), v.data_ptr(), ks, batch.n_seq, batch.rows,
+        _capi.call("ei_cache8_load", torch._C._cuda_getCurrentRawStream(dev), *where, k.data_ptr(), v.data_ptr(), ks, batch.n_seq, batch.rows,
                    batch.n_head, batch.n_head_kv, HEAD_DIM, batch.buf.data_ptr(), batch.nbytes)
     return k, v
 
@@ -657,15 +690,16 @@ def attn_packed_cache8(q: torch.Tensor, cache: Cache8, block_table: torch.Tensor
     """Attention of the batch's new rows, q [rows, >= H*128] normed and turned, over their sequences' pages of the
     8-bit cache (ei_attn_packed_cache8): causal, or with mask (int64 [rows, words]) a row sees of the new rows
     those whose bit is set in its words, up to itself.  Returns [rows, H, 128]."""
-    batch._check(shape)
-    qs = _rows_of("q", q, batch.rows, shape.n_head * HEAD_DIM)
-    where = _cache8_args(cache, block_table, batch, shape.n_head_kv)
+    dev = _device()
+    _check_batch(batch, shape, dev)
+    qs = _stride_of("q", q, batch.rows, shape.n_head * HEAD_DIM, dev)
+    where = _cache8_args(cache, block_table, batch, shape.n_head_kv, dev)
     bits = _mask_args(mask, batch.rows)
-    out = batch._out(out, q.device)
-    scale = default_scale() if scale is None else scale
+    out = _out_of(batch, out, dev)
+    scale = _SCALE if scale is None else float(scale)
     if batch.rows:
-        _capi.call("ei_attn_packed_cache8", _stream(), q.data_ptr(), qs, out.data_ptr(), *where, batch.n_seq,
-                   batch.rows, shape.n_head, shape.n_head_kv, shape.head_dim, *bits, float(scale), *batch._tail())
+        _capi.call("ei_attn_packed_cache8", torch._C._cuda_getCurrentRawStream(dev), q.data_ptr(), qs, out.data_ptr(), *where, batch.n_seq,
+                   batch.rows, shape.n_head, shape.n_head_kv, shape.head_dim, *bits, scale, *batch._tail())
     return out
 
 
@@ -675,16 +709,17 @@ def packed_step_cache8(qkv: torch.Tensor, cache: Cache8, block_table: torch.Tens
                        out: torch.Tensor | None = None) -> torch.Tensor:
     """The whole step of a batch over the 8-bit cache: cache8_store, then attn_packed_cache8 on its queries
     (ei_packed_step_cache8).  Returns [rows, H, 128]."""
-    batch._check(shape)
-    rs = _rows_of("qkv", qkv, batch.rows, shape.qkv)
-    where = _cache8_args(cache, block_table, batch, shape.n_head_kv)
-    turn = _turn_args(cs, pos, shape, batch.rows, q_gamma, k_gamma)
+    dev = _device()
+    _check_batch(batch, shape, dev)
+    rs = _stride_of("qkv", qkv, batch.rows, shape.qkv, dev)
+    where = _cache8_args(cache, block_table, batch, shape.n_head_kv, dev)
+    turn = _turn_args(cs, pos, shape, batch.rows, q_gamma, k_gamma, dev)
     bits = _mask_args(mask, batch.rows)
-    out = batch._out(out, qkv.device)
-    scale = default_scale() if scale is None else scale
+    out = _out_of(batch, out, dev)
+    scale = _SCALE if scale is None else float(scale)
     if batch.rows:
-        _capi.call("ei_packed_step_cache8", _stream(), qkv.data_ptr(), rs, out.data_ptr(), *where, batch.n_seq,
-                   batch.rows, shape.n_head, shape.n_head_kv, shape.head_dim, *turn, *bits, float(scale),
+        _capi.call("ei_packed_step_cache8", torch._C._cuda_getCurrentRawStream(dev), qkv.data_ptr(), rs, out.data_ptr(), *where, batch.n_seq,
+                   batch.rows, shape.n_head, shape.n_head_kv, shape.head_dim, *turn, *bits, scale,
                    *batch._tail())
     return out
 
@@ -694,15 +729,16 @@ def attn_tree_paged(q: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor, block_t
                     out: torch.Tensor | None = None) -> torch.Tensor:
     """attn_packed_paged for trees of drafted tokens (ei_attn_tree_paged): a row sees the keys before its sequence's
     new rows, and of those the ones whose bit is set in its row of mask (int64 [rows, words]), up to itself."""
-    batch._check(shape)
-    qs = _rows_of("q", q, batch.rows, shape.n_head * HEAD_DIM)
+    dev = _device()
+    _check_batch(batch, shape, dev)
+    qs = _stride_of("q", q, batch.rows, shape.n_head * HEAD_DIM, dev)
     pool = _pool_args(kc, vc, block_table, block_size, batch, shape)
     bits = _mask_args(mask, batch.rows)
-    out = batch._out(out, q.device)
-    scale = default_scale() if scale is None else scale
+    out = _out_of(batch, out, dev)
+    scale = _SCALE if scale is None else float(scale)
     if batch.rows:
-        _capi.call("ei_attn_tree_paged", _stream(), q.data_ptr(), qs, out.data_ptr(), *pool, batch.n_seq, batch.rows,
-                   shape.n_head, shape.n_head_kv, shape.head_dim, *bits, float(scale), *batch._tail())
+        _capi.call("ei_attn_tree_paged", torch._C._cuda_getCurrentRawStream(dev), q.data_ptr(), qs, out.data_ptr(), *pool, batch.n_seq, batch.rows,
+                   shape.n_head, shape.n_head_kv, shape.head_dim, *bits, scale, *batch._tail())
     return out
 
 
@@ -712,31 +748,34 @@ def tree_step_paged(qkv: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor, block
                     scale: float | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """packed_step_paged for trees of drafted tokens, at positions pos (int32 [rows], None: the rows' slots) and with
     a mask (ei_tree_step_paged).  Returns [rows, H, 128]."""
-    batch._check(shape)
-    rs = _rows_of("qkv", qkv, batch.rows, shape.qkv)
+    dev = _device()
+    _check_batch(batch, shape, dev)
+    rs = _stride_of("qkv", qkv, batch.rows, shape.qkv, dev)
     pool = _pool_args(kc, vc, block_table, block_size, batch, shape)
-    turn = _turn_args(cs, pos, shape, batch.rows, q_gamma, k_gamma)
+    turn = _turn_args(cs, pos, shape, batch.rows, q_gamma, k_gamma, dev)
     bits = _mask_args(mask, batch.rows)
-    out = batch._out(out, qkv.device)
-    scale = default_scale() if scale is None else scale
+    out = _out_of(batch, out, dev)
+    scale = _SCALE if scale is None else float(scale)
     if batch.rows:
-        _capi.call("ei_tree_step_paged", _stream(), qkv.data_ptr(), rs, out.data_ptr(), *pool, batch.n_seq, batch.rows,
-                   shape.n_head, shape.n_head_kv, shape.head_dim, *turn, *bits, float(scale), *batch._tail())
+        _capi.call("ei_tree_step_paged", torch._C._cuda_getCurrentRawStream(dev), qkv.data_ptr(), rs, out.data_ptr(), *pool, batch.n_seq, batch.rows,
+                   shape.n_head, shape.n_head_kv, shape.head_dim, *turn, *bits, scale, *batch._tail())
     return out
 
 
-def _kept_args(batch: PackedBatch, kept: torch.Tensor, n_kept: torch.Tensor, out: torch.Tensor | None) -> tuple:
-    _need_contiguous("kept", kept, torch.int32)
-    _need_contiguous("n_kept", n_kept, torch.int32)
-    if kept.dim() != 2 or kept.shape[0] < batch.n_seq or kept.shape[1] < 1:
-        raise ValueError(f"kept must be [{batch.n_seq}, most], got {tuple(kept.shape)}")
+def _kept_args(batch: PackedBatch, kept: torch.Tensor, n_kept: torch.Tensor, out: torch.Tensor | None,
+               dev: int) -> tuple:
+    shape, n_seq, i32 = kept.shape, batch.n_seq, torch.int32
+    if (len(shape) != 2 or shape[0] < n_seq or shape[1] < 1 or kept.dtype is not i32 or kept.get_device() != dev or
+            not kept.is_contiguous()):
+        _need_contiguous("kept", kept, i32)
+        raise ValueError(f"kept must be [{n_seq}, most], got {tuple(shape)}")
     if out is None:
-        out = torch.empty(batch.n_seq, dtype=torch.int32, device=kept.device)
-    _need_contiguous("out", out, torch.int32)
+        out = torch.empty(n_seq, dtype=i32, device=kept.device)
     for name, t in (("n_kept", n_kept), ("out", out)):
-        if t.numel() < batch.n_seq:
-            raise ValueError(f"{name} must hold {batch.n_seq} numbers, got {t.numel()}")
-    return (kept.data_ptr(), kept.shape[1], n_kept.data_ptr(), out.data_ptr(), batch.buf.data_ptr(), batch.nbytes), out
+        if t.dtype is not i32 or t.get_device() != dev or t.numel() < n_seq or not t.is_contiguous():
+            _need_contiguous(name, t, i32)
+            raise ValueError(f"{name} must hold {n_seq} numbers, got {t.numel()}")
+    return (kept.data_ptr(), shape[1], n_kept.data_ptr(), out.data_ptr(), batch.buf.data_ptr(), batch.nbytes), out
 
 
 def cache_keep(kc: torch.Tensor, vc: torch.Tensor, block_table: torch.Tensor, block_size: int, batch: PackedBatch,
@@ -745,10 +784,11 @@ def cache_keep(kc: torch.Tensor, vc: torch.Tensor, block_table: torch.Tensor, bl
     """After a batch of drafts was checked: moves the accepted rows of each sequence's new rows, kept int32
     [n_seq, most] (rising; n_kept int32 [n_seq] of them count), together behind its earlier keys in the fp32 pool
     (ei_cache_keep).  Returns the sequences' lengths with them, int32 [n_seq]; `out` may be the batch's kv_len."""
-    batch._check(shape)
+    dev = _device()
+    _check_batch(batch, shape, dev)
     pool = _pool_args(kc, vc, block_table, block_size, batch, shape)
-    args, out = _kept_args(batch, kept, n_kept, out)
-    _capi.call("ei_cache_keep", _stream(), *pool, batch.n_seq, batch.rows, shape.n_head, shape.n_head_kv,
+    args, out = _kept_args(batch, kept, n_kept, out, dev)
+    _capi.call("ei_cache_keep", torch._C._cuda_getCurrentRawStream(dev), *pool, batch.n_seq, batch.rows, shape.n_head, shape.n_head_kv,
                shape.head_dim, *args)
     return out
 
@@ -756,10 +796,11 @@ def cache_keep(kc: torch.Tensor, vc: torch.Tensor, block_table: torch.Tensor, bl
 def cache8_keep(cache: Cache8, block_table: torch.Tensor, batch: PackedBatch, kept: torch.Tensor, n_kept: torch.Tensor,
                 out: torch.Tensor | None = None) -> torch.Tensor:
     """cache_keep in the 8-bit cache (ei_cache8_keep)."""
-    _need_cached(batch)
-    where = _cache8_args(cache, block_table, batch, batch.n_head_kv)
-    args, out = _kept_args(batch, kept, n_kept, out)
-    _capi.call("ei_cache8_keep", _stream(), *where, batch.n_seq, batch.rows, batch.n_head, batch.n_head_kv, HEAD_DIM,
+    dev = _device()
+    _check_planned(batch, dev)
+    where = _cache8_args(cache, block_table, batch, batch.n_head_kv, dev)
+    args, out = _kept_args(batch, kept, n_kept, out, dev)
+    _capi.call("ei_cache8_keep", torch._C._cuda_getCurrentRawStream(dev), *where, batch.n_seq, batch.rows, batch.n_head, batch.n_head_kv, HEAD_DIM,
                *args)
     return out
 

@@ -299,6 +299,8 @@ constexpr float kTopW = 0x1p15f;                       // p s_v F at most
 constexpr float kLazy8 = 8.f;                          // the reference moves when a score passes it by more (log2 units)
 __device__ __forceinline__ float pow2(int e) { return __builtin_amdgcn_ldexpf(1.f, e); }
 
+constexpr int kOnce = 2;  // the streaming cache policy of a buffer load, for codes that are read once
+
 // ---- units of up to 32 rows
 // A workgroup's share of the few-row list.  A unit's rows are one block of sixteen or two, one per wave; waves of a block
 // take its tiles in turn, each lane its row l % 16 and quarter l / 16:
@@ -364,13 +366,13 @@ __device__ __forceinline__ void few8_walk(const Cache8Args& a, const List& list,
         for (int kb = 0; kb < 2; ++kb) {
 #pragma unroll
             for (int x = 0; x < 2; ++x)
-                t.k[kb][x] = __builtin_amdgcn_raw_buffer_load_b128(rk, ok + 16 * kb * D + 16 * x, 0, 0);
-            t.ks[kb] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(sk, (ln >> 4) * 16 + 64 * kb, 0, 0));
-            t.vs[kb] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(sv, (ln >> 4) * 16 + 64 * kb, 0, 0));
+                t.k[kb][x] = __builtin_amdgcn_raw_buffer_load_b128(rk, ok + 16 * kb * D + 16 * x, 0, kOnce);
+            t.ks[kb] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(sk, (ln >> 4) * 16 + 64 * kb, 0, kOnce));
+            t.vs[kb] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(sv, (ln >> 4) * 16 + 64 * kb, 0, kOnce));
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e)
-            t.v[e] = __builtin_amdgcn_raw_buffer_load_b64(rv, ov + (16 * (e >> 2) + (e & 3)) * D, 0, 0);
+            t.v[e] = __builtin_amdgcn_raw_buffer_load_b64(rv, ov + (16 * (e >> 2) + (e & 3)) * D, 0, kOnce);
     };
     // this lane's row of a unit (rows past the last repeat it), and its query, d = 32 quarter .. + 31
     auto row_of = [&](const Unit8& p) {
