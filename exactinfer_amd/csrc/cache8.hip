@@ -15,26 +15,28 @@ struct Coding {
     bool bad;         // a value that is not finite: scale NaN, codes 0
 };
 template <bool kInt8>
-__device__ __forceinline__ Coding coding(float most) {
+__device__ __forceinline__ Coding coding(float most) {  // (infinite or NaN where a value is)
     constexpr float kTop = kInt8 ? 127.f : 448.f;
-    const bool bad = !(most < INFINITY);  // (infinite or NaN)
-    if (bad) return {__builtin_nanf(""), 0.f, true};
+    if (!(most < INFINITY)) return {__builtin_nanf(""), 0.f, true};
     if (most < kNothing) return {0.f, 0.f, false};
     return {most / kTop, kTop / most, false};
 }
-// the code of y, in the low byte
+// the codes of four values
 template <bool kInt8>
-__device__ __forceinline__ uint32_t code_of(float y, const Coding& c) {
+__device__ __forceinline__ uint32_t codes_of(const float* y, const Coding& c) {
 #pragma clang fp contract(off)
-    const float x = c.bad ? 0.f : y * c.by;
-    if constexpr (kInt8) return (uint32_t)(int)rintf(x) & 0xFFu;
-    else return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false) & 0xFFu;
-}
-// the largest magnitude over the wave; NaN where a value is (fmaxf would drop it)
-__device__ __forceinline__ float wave_most(float a, float b) {
-    const float m = wave_max(fmaxf(__builtin_fabsf(a), __builtin_fabsf(b)));
-    const bool nan = __builtin_amdgcn_ballot_w64(!(a == a) || !(b == b)) != 0;
-    return nan ? __builtin_nanf("") : m;
+    float x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = c.bad ? 0.f : y[j] * c.by;
+    uint32_t u = 0;
+    if constexpr (kInt8) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u |= ((uint32_t)(int)rintf(x[j]) & 0xFFu) << (8 * j);
+    } else {
+        u = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+        u = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], (int)u, true);
+    }
+    return u;
 }
 // two values of a code pair
 template <bool kInt8, int kByte>
@@ -48,84 +50,128 @@ __device__ __forceinline__ size_t head_row(int page, int HKV, int kvh, int shift
 }
 
 // ------------------------------------------------------------------ storing
-// grid (rows, ceil((H + HKV) / 16)), block 256: each wave four consecutive heads of the row, a key head with the value
-// head beside it, loads first (as k_packed_prepare).  Lane l holds elements l and l + 64; four lanes' codes are put
-// together for one store.
-constexpr int kStoreHeads = 4;
-template <bool kInt8>
+// Sixteen lanes per head, eight values each, four heads per wave, as k_rope_rows lays them out.  kVec (rope_dim a multiple
+// of 8): a lane below rope_dim / 8 holds the pieces of four at 4l and rope_dim / 2 + 4l, partners of each other, the
+// others two pieces of the rest; otherwise elements l + 16j, whose partners are read from the row again.
+// grid (rows, ceil((H + 2 HKV) / 16)).
+template <bool kInt8, bool kVec>
 __global__ __launch_bounds__(256) void k_cache8_store(const float* __restrict__ qkv, long row_stride,
                                                       float* __restrict__ q_out, Cache8Args a,
                                                       const float* __restrict__ q_gamma,
                                                       const float* __restrict__ k_gamma,
                                                       const float2* __restrict__ cs, int n_pos,
                                                       const int* __restrict__ turn_at, int rope_dim, float eps) {
-    __shared__ float scratch[4][kHeadDim];
-    const int b = blockIdx.x, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int H = a.H, HKV = a.HKV, NH = H + HKV;
-    const int h0 = (blockIdx.y * 4 + w) * kStoreHeads;
-    if (h0 >= NH) return;  // wave-uniform, no barrier here
-    const float* row = qkv + (size_t)b * row_stride;
-    float x0[kStoreHeads], x1[kStoreHeads], v0[kStoreHeads], v1[kStoreHeads], inv[kStoreHeads];
+#pragma clang fp contract(off)
+    const int b = blockIdx.x, lane = threadIdx.x & 15, half = rope_dim >> 1;
+    const int H = a.H, HKV = a.HKV, h = blockIdx.y * 16 + (threadIdx.x >> 4);
+    const bool is_q = h < H, is_v = h >= H + HKV;
+    auto at = [&](int j) {  // the element of value j of this lane
+        if constexpr (!kVec) return lane + 16 * j;
+        else if (lane < (rope_dim >> 3)) return 4 * lane + half * (j >> 2) + (j & 3);
+        else return rope_dim + 8 * (lane - (rope_dim >> 3)) + j;
+    };
+    // (the row's values are on their way while its place is looked up; of a row that nobody owns they are not used)
+    const float* src = qkv + (size_t)b * row_stride + (size_t)min(h, H + 2 * HKV - 1) * kHeadDim;
+    const float* gamma = is_q ? q_gamma : k_gamma;
+    float v[8], g[8];
 #pragma unroll
-    for (int j = 0; j < kStoreHeads; ++j) {
-        const int hh = min(h0 + j, NH - 1);  // clamped: heads past NH are loaded, not used
-        const float* v = row + (size_t)hh * kHeadDim;
-        x0[j] = v[lane];
-        x1[j] = v[lane + 64];
-        v0[j] = v1[j] = 0.f;
-        if (hh >= H) {
-            const float* vs = row + (size_t)(NH + hh - H) * kHeadDim;  // V of a key head
-            v0[j] = vs[lane];
-            v1[j] = vs[lane + 64];
+    for (int k = 0; k < 2; ++k) {
+        if constexpr (kVec) {
+            const float4 t = *reinterpret_cast<const float4*>(src + at(4 * k));
+            v[4 * k] = t.x, v[4 * k + 1] = t.y, v[4 * k + 2] = t.z, v[4 * k + 3] = t.w;
+            const float4 u = *reinterpret_cast<const float4*>(gamma + at(4 * k));
+            g[4 * k] = u.x, g[4 * k + 1] = u.y, g[4 * k + 2] = u.z, g[4 * k + 3] = u.w;
+        } else {
+#pragma unroll
+            for (int j = 4 * k; j < 4 * k + 4; ++j) v[j] = src[at(j)], g[j] = gamma[at(j)];
         }
     }
     if (!plan_fits(a.plan, a.n_seq, a.rows, H, HKV, false)) return;
     const int4* seq = reinterpret_cast<const int4*>(a.plan + kPlanSeqAt);
-    const int s = row_owner(seq, a.n_seq, b, lane);
-    if (s < 0) return;
+    const int s = row_owner(seq, a.n_seq, b, threadIdx.x & 63);  // (with the whole wave)
+    if (s < 0 || h >= H + 2 * HKV || (is_q && !q_out)) return;   // sixteen lanes leave together
     const int4 e = seq[s];
     const int slot = e.z - e.y + (b - e.x);
     const int turn = turn_at ? turn_at[b] : slot;
     const bool in = slot >= 0 && slot < reinterpret_cast<const int*>(a.plan)[kHeadMaxKv] && turn >= 0 && turn < n_pos;
     const int blk = slot >> a.bshift;
     const int page = in && blk < a.max_blocks ? a.btab[(size_t)s * a.max_blocks + blk] : -1;
-    const bool there = page >= 0 && page < a.n_blocks;
-    const float2* cs_row = cs + (size_t)(in ? turn : 0) * (rope_dim >> 1);
-    const float qg0 = q_gamma[lane], qg1 = q_gamma[lane + 64];
-    const float kg0 = k_gamma[lane], kg1 = k_gamma[lane + 64];
-    head_inv<kStoreHeads>(x0, x1, eps, inv, lane);
-    auto store = [&](uint8_t* codes, float* scales, size_t at, float y0, float y1) {
-        const Coding c = coding<kInt8>(wave_most(y0, y1));
-        uint32_t w0 = code_of<kInt8>(y0, c) << (8 * (lane & 3)), w1 = code_of<kInt8>(y1, c) << (8 * (lane & 3));
-        auto joined = [](uint32_t x) {
-            x |= __float_as_uint(lane_xor1(__uint_as_float(x)));
-            return x | __float_as_uint(lane_xor2(__uint_as_float(x)));
-        };
-        w0 = joined(w0), w1 = joined(w1);
-        uint32_t* dst = reinterpret_cast<uint32_t*>(codes + at * kHeadDim) + (lane >> 2);
-        if ((lane & 3) == 0) dst[0] = w0, dst[16] = w1;
-        if (lane == 0) scales[at] = c.scale;
-    };
+    float w[8];
 #pragma unroll
-    for (int j = 0; j < kStoreHeads; ++j) {
-        const int hh = h0 + j;
-        if (hh >= NH) break;
-        const bool is_k = hh >= H;
-        if (!is_k && !q_out) continue;
-        float o0 = x0[j], o1 = x1[j];
-        if (in)
-            scale_rope_vals(x0[j], x1[j], inv[j], is_k ? kg0 : qg0, is_k ? kg1 : qg1, cs_row, rope_dim, scratch[w],
-                            lane, &o0, &o1);
-        if (!is_k) {
-            float* dst = q_out + ((size_t)b * H + hh) * kHeadDim;
-            dst[lane] = o0;
-            dst[lane + 64] = o1;
-        } else if (there) {
-            const size_t at = head_row(page, HKV, hh - H, a.bshift, slot);
-            store(a.k8, a.ks, at, o0, o1);
-            store(a.v8, a.vs, at, v0[j], v1[j]);
+    for (int j = 0; j < 8; ++j) w[j] = v[j];
+    if (!is_v && in) {
+        const float2* row = cs + (size_t)turn * half;
+        double ss = 0.0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss = __builtin_fma((double)v[j], (double)v[j], ss);
+        ss += lane_xor_f64<1>(ss);
+        ss += lane_xor_f64<2>(ss);
+        ss += lane_xor_f64<4>(ss);
+        ss += lane_xor_f64<8>(ss);
+        const float inv = (float)(1.0 / sqrt(ss / (double)kHeadDim + (double)eps));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = (v[j] * inv) * g[j];
+        if constexpr (kVec) {
+            if (lane < (rope_dim >> 3)) {
+                const float4 t0 = *reinterpret_cast<const float4*>(row + 4 * lane);
+                const float4 t1 = *reinterpret_cast<const float4*>(row + 4 * lane + 2);
+                const float c[4] = {t0.x, t0.z, t1.x, t1.z}, n[4] = {t0.y, t0.w, t1.y, t1.w};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float x = w[j], y = w[4 + j];
+                    const float xc = x * c[j], yn = y * n[j], xn = x * n[j], yc = y * c[j];
+                    w[j] = xc - yn, w[4 + j] = xn + yc;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int i = at(j);
+                if (i < rope_dim) {
+                    const bool first = i < half;
+                    const int o = first ? i + half : i - half;
+                    const float2 t = row[first ? i : o];
+                    const float other = (src[o] * inv) * gamma[o];
+                    const float own_c = w[j] * t.x, other_s = other * t.y;
+                    w[j] = first ? own_c - other_s : other_s + own_c;
+                }
+            }
         }
     }
+    if (is_q) {
+        float* dst = q_out + ((size_t)b * H + h) * kHeadDim;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            if constexpr (kVec)
+                *reinterpret_cast<float4*>(dst + at(4 * k)) =
+                    make_float4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+            else
+#pragma unroll
+                for (int j = 4 * k; j < 4 * k + 4; ++j) dst[at(j)] = w[j];
+        }
+        return;
+    }
+    if (page < 0 || page >= a.n_blocks) return;
+    // the largest magnitude, as bits: infinite and NaN ones are above the others
+    uint32_t most = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) most = max(most, __float_as_uint(w[j]) & 0x7FFFFFFFu);
+    most = max(most, __float_as_uint(lane_xor1(__uint_as_float(most))));
+    most = max(most, __float_as_uint(lane_xor2(__uint_as_float(most))));
+    most = max(most, __float_as_uint(lane_xor4(__uint_as_float(most))));
+    most = max(most, __float_as_uint(lane_xor8(__uint_as_float(most))));
+    const Coding c = coding<kInt8>(__uint_as_float(most));
+    const size_t place = head_row(page, HKV, is_v ? h - H - HKV : h - H, a.bshift, slot);
+    uint8_t* dst = (is_v ? a.v8 : a.k8) + place * kHeadDim;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+        const uint32_t u = codes_of<kInt8>(w + 4 * k, c);
+        if constexpr (kVec) *reinterpret_cast<uint32_t*>(dst + at(4 * k)) = u;
+        else
+#pragma unroll
+            for (int j = 0; j < 4; ++j) dst[at(4 * k + j)] = (uint8_t)(u >> (8 * j));
+    }
+    if (lane == 0) (is_v ? a.vs : a.ks)[place] = c.scale;
 }
 
 // ------------------------------------------------------------------ reading back
@@ -1185,10 +1231,18 @@ static hipError_t by_kind(const Cache8Args& a, F f) {
 hipError_t launch_cache8_store(hipStream_t st, const Cache8Args& a, const float* qkv, long row_stride, float* q_out,
                                const float* q_gamma, const float* k_gamma, const float* cs, int n_pos,
                                const int* turn_at, int rope_dim, float eps) {
+    const dim3 grid(a.rows, (a.H + 2 * a.HKV + 15) / 16);
+    const float2* t = reinterpret_cast<const float2*>(cs);
+    auto odd = [](const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) != 0; };
+    const bool vec = rope_dim % 8 == 0 && !odd(q_gamma) && !odd(k_gamma) && !odd(cs);  // (whole pieces of 16 bytes)
     return by_kind(a, [&](auto kind) {
-        k_cache8_store<decltype(kind)::value><<<dim3(a.rows, (a.H + a.HKV + 15) / 16), 256, 0, st>>>(
-            qkv, row_stride, q_out, a, q_gamma, k_gamma, reinterpret_cast<const float2*>(cs), n_pos, turn_at, rope_dim,
-            eps);
+        constexpr bool kInt8 = decltype(kind)::value;
+        if (vec)
+            k_cache8_store<kInt8, true><<<grid, 256, 0, st>>>(qkv, row_stride, q_out, a, q_gamma, k_gamma, t, n_pos,
+                                                              turn_at, rope_dim, eps);
+        else
+            k_cache8_store<kInt8, false><<<grid, 256, 0, st>>>(qkv, row_stride, q_out, a, q_gamma, k_gamma, t, n_pos,
+                                                               turn_at, rope_dim, eps);
         return hipGetLastError();
     });
 }

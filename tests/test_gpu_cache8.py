@@ -47,6 +47,10 @@ def _turned64(x, gamma, pos, rope_dim, n_pos, eps=1e-6):
     (40, 8, [100, 7], [0, 64], 64, 64, 0, True),
     (6, 2, [65, 1, 2], [63, 127, 0], 64, 128, 1, True),
     (32, 8, [300], [4000], 128, 96, 0, False),
+    (5, 1, [17, 3], [40, 0], 32, 36, 0, True),
+    (8, 4, [9], [100], 32, 2, 1, False),
+    (2, 2, [33], [31], 32, 126, 0, True),
+    (3, 3, [2], [0], 32, 8, 0, False),
 ])
 def test_store(gpu, kind, H, HKV, lens, past, bs, rope_dim, extra, turned):
     A = gpu
@@ -97,6 +101,25 @@ def test_store(gpu, kind, H, HKV, lens, past, bs, rope_dim, extra, turned):
         raw[page, :, off] = 0
         want[page, :, off] = 0
         assert torch.equal(raw, want)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_store_with_parameters_at_any_address(gpu, kind):
+    """Gammas and the table at addresses that are not a multiple of 16 bytes."""
+    A = gpu
+    b = Batch(A, 6, 2, [7, 5], [20, 64], 32, seed=9)
+    qkv, cs = _normal(10, b.rows, 10 * D), A.rope_table(80)
+    g = [1 + 0.1 * _normal(11 + i, D) for i in range(2)]
+    odd = []
+    for t in (*g, cs):
+        buf = torch.empty(t.numel() + 1, device="cuda")
+        odd.append(buf[1:].view(t.shape).copy_(t))
+    want, got = (A.Cache8(b.n_blocks, 32, 2, kind) for _ in range(2))
+    q0 = A.cache8_store(qkv, want, b.table, b.plan, b.shape, *g, cs)
+    q1 = A.cache8_store(qkv, got, b.table, b.plan, b.shape, *odd)
+    assert torch.equal(q0, q1) and bool((q0 != 0).any())
+    for x, y in ((want.k, got.k), (want.v, got.v), (want.k_scale, got.k_scale), (want.v_scale, got.v_scale)):
+        assert torch.equal(x.view(torch.int8), y.view(torch.int8))
 
 
 def _stored_values(A, kind, rows):
