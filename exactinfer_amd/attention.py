@@ -615,13 +615,27 @@ def _cache8_args(cache: Cache8, block_table: torch.Tensor, batch: PackedBatch, n
     return cache._at, block_table.data_ptr(), shape[1]
 
 
+def _pool_of(kc: torch.Tensor, vc: torch.Tensor, block_table: torch.Tensor, block_size: int, batch: PackedBatch,
+             shape: AttnShape, dev: int) -> tuple:
+    """_pool_args, for what passes its checks."""
+    f32, n, table, kd = torch.float32, kc.numel(), block_table.shape, shape.kd
+    if (kc.dtype is f32 and vc.dtype is f32 and kc.get_device() == dev and vc.get_device() == dev and
+            kc.is_contiguous() and vc.is_contiguous() and n == vc.numel() and n % kd == 0 and len(table) == 2 and
+            table[0] >= batch.n_seq and block_table.dtype is torch.int32 and block_table.get_device() == dev and
+            block_table.is_contiguous() and block_size > 0):
+        return kc.data_ptr(), vc.data_ptr(), n // kd // block_size, block_table.data_ptr(), table[1], block_size
+    return _pool_args(kc, vc, block_table, block_size, batch, shape)
+
+
 def _mask_args(mask: torch.Tensor | None, rows: int) -> tuple:
     if mask is None:
         return None, 0
-    _need_contiguous("mask", mask, torch.int64)
-    if mask.dim() != 2 or mask.shape[0] < rows or mask.shape[1] < 1:
-        raise ValueError(f"mask must be [{rows}, words], got {tuple(mask.shape)}")
-    return mask.data_ptr(), mask.shape[1]
+    shape = mask.shape
+    if mask.dtype is not torch.int64 or mask.get_device() != _device() or not mask.is_contiguous():
+        _need_contiguous("mask", mask, torch.int64)
+    if len(shape) != 2 or shape[0] < rows or shape[1] < 1:
+        raise ValueError(f"mask must be [{rows}, words], got {tuple(shape)}")
+    return mask.data_ptr(), shape[1]
 
 
 def _turn_args(cs: torch.Tensor, pos: torch.Tensor | None, shape: AttnShape, rows: int, q_gamma: torch.Tensor,
@@ -732,7 +746,7 @@ def attn_tree_paged(q: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor, block_t
     dev = _device()
     _check_batch(batch, shape, dev)
     qs = _stride_of("q", q, batch.rows, shape.n_head * HEAD_DIM, dev)
-    pool = _pool_args(kc, vc, block_table, block_size, batch, shape)
+    pool = _pool_of(kc, vc, block_table, block_size, batch, shape, dev)
     bits = _mask_args(mask, batch.rows)
     out = _out_of(batch, out, dev)
     scale = _SCALE if scale is None else float(scale)
@@ -751,7 +765,7 @@ def tree_step_paged(qkv: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor, block
     dev = _device()
     _check_batch(batch, shape, dev)
     rs = _stride_of("qkv", qkv, batch.rows, shape.qkv, dev)
-    pool = _pool_args(kc, vc, block_table, block_size, batch, shape)
+    pool = _pool_of(kc, vc, block_table, block_size, batch, shape, dev)
     turn = _turn_args(cs, pos, shape, batch.rows, q_gamma, k_gamma, dev)
     bits = _mask_args(mask, batch.rows)
     out = _out_of(batch, out, dev)
@@ -786,7 +800,7 @@ def cache_keep(kc: torch.Tensor, vc: torch.Tensor, block_table: torch.Tensor, bl
     (ei_cache_keep).  Returns the sequences' lengths with them, int32 [n_seq]; `out` may be the batch's kv_len."""
     dev = _device()
     _check_batch(batch, shape, dev)
-    pool = _pool_args(kc, vc, block_table, block_size, batch, shape)
+    pool = _pool_of(kc, vc, block_table, block_size, batch, shape, dev)
     args, out = _kept_args(batch, kept, n_kept, out, dev)
     _capi.call("ei_cache_keep", torch._C._cuda_getCurrentRawStream(dev), *pool, batch.n_seq, batch.rows, shape.n_head, shape.n_head_kv,
                shape.head_dim, *args)
