@@ -353,6 +353,13 @@ constexpr int kFew8F = kFew8ML + kWaves * kRow8 * 2;
 constexpr int kTopF = 96;                              // log2 F at most
 constexpr float kTopW = 0x1p15f;                       // p s_v F at most
 constexpr float kLazy8 = 8.f;                          // the reference moves when a score passes it by more (log2 units)
+// Scales of values in between (larger ones are not provided for) keep F so low that p s_v F stays finite.
+constexpr float kBigScale = 0x1p20f, kMostScale = 0x1p118f;
+__device__ __forceinline__ float big_scale(float s) {  // s if it is one, else 0
+    s = __builtin_fabsf(s);
+    return s > kBigScale && s <= kMostScale ? s : 0.f;
+}
+__device__ __forceinline__ int most_f(float big) { return 127 + 118 - (int)(__float_as_uint(big) >> 23); }
 __device__ __forceinline__ float pow2(int e) { return __builtin_amdgcn_ldexpf(1.f, e); }
 
 constexpr int kOnce = 2;  // the streaming cache policy of a buffer load, for codes that are read once
@@ -543,6 +550,19 @@ __device__ __forceinline__ void few8_walk(const Cache8Args& a, const List& list,
                 if (__builtin_amdgcn_ballot_w64(fn - fe != up)) scale_sums(pow2(fn - fe - up));
                 fe = fn;
                 m = mn;
+            }
+            float big = 0.f;
+#pragma unroll
+            for (int r = 0; r < 8; ++r) big = fmaxf(big, __builtin_fabsf(t.vs[r >> 2][r & 3]));
+            if (__builtin_amdgcn_ballot_w64(big > kBigScale)) {
+                big = 0.f;
+#pragma unroll
+                for (int r = 0; r < 8; ++r)
+                    if (seen(r)) big = fmaxf(big, big_scale(t.vs[r >> 2][r & 3]));
+                big = row_max(big);
+                const int fn = big > 0.f ? min(fe, most_f(big)) : fe;
+                scale_sums(pow2(fn - fe));
+                fe = fn;
             }
             const float nb = m == -INFINITY ? 0.f : (float)fe - m;
             float sum = 0.f, wm = 0.f;
@@ -736,7 +756,8 @@ __device__ __forceinline__ void few8_walk(const Cache8Args& a, const List& list,
 // read right before its use).
 constexpr int kK8RowB = 2 * kHeadDim + 16, kK8Tile = kKT * kK8RowB;  // [32 keys][128 d] binary16, rows spread over banks
 constexpr int kV8RowB = 2 * kKT + 16, kV8Tile = kHeadDim * kV8RowB;  // [128 d][32 keys]
-constexpr int kScales8 = 2 * kKT * 4;                               // of K, of V
+constexpr int kBigAt8 = 2 * kKT * 4;                                // after the scales of K and V: the largest big one (of K, of V)
+constexpr int kScales8 = kBigAt8 + 16;
 constexpr int kBuf8 = kK8Tile + kV8Tile + kScales8;                 // one tile of a group
 static_assert(kBuf8 % 16 == 0, "16-byte pieces");
 template <int kS>
@@ -791,7 +812,7 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
     // this wave's parts x of a tile, y = kParts hw + x:
     //   K: codes 16 (lane % 8) .. + 15 of row 8 y + lane / 8
     //   V: codes 32 y + 4 (lane % 8) .. + 3 of the four rows from 4 (lane / 8) on
-    // and the scales, of K by the even waves, of V by the odd ones (whole tiles: pages hold them)
+    // and the scales, of K by the even waves, of V by the odd ones
     u32x4 tk[kParts];
     uint32_t tv[kParts][4];
     float ts;
@@ -812,7 +833,7 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
                 tv[x][y] = __builtin_amdgcn_raw_buffer_load_b32(rs, from_v + 32 * x + y * D, 0, 0);
     };
     auto load_scales = [&](const Place& at) {
-        const Rsrc rs = __builtin_amdgcn_make_buffer_rsrc((hw & 1 ? a.vs : a.ks) + at.row, 0, at.there ? kKT * 4 : 0,
+        const Rsrc rs = __builtin_amdgcn_make_buffer_rsrc((hw & 1 ? a.vs : a.ks) + at.row, 0, at.there * 4,
                                                           kBufferDword3);
         ts = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rs, 4 * (lane & 31), 0, 0));
     };
@@ -836,8 +857,13 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
         *reinterpret_cast<u32x2*>(d) = u32x2{pair_f16<kInt8, 0>(lo), pair_f16<kInt8, 0>(hi)};
         *reinterpret_cast<u32x2*>(d + kV8RowB) = u32x2{pair_f16<kInt8, 1>(lo), pair_f16<kInt8, 1>(hi)};
     };
-    const uint32_t to_scales = kK8Tile + kV8Tile + 4 * kKT * (hw & 1) + 4 * (lane & 31);
-    auto store_scales = [&](int i) { *reinterpret_cast<float*>(buf(i) + to_scales) = ts; };
+    // (the upper half of the wave writes the largest big one)
+    const uint32_t to_scales = kK8Tile + kV8Tile + (hh ? kBigAt8 + 4 * (hw & 1) : 4 * kKT * (hw & 1) + 4 * col);
+    auto store_scales = [&](int i) {
+        float big = 0.f;
+        if (__builtin_amdgcn_ballot_w64(__builtin_fabsf(ts) > kBigScale)) big = wave_max(big_scale(ts));
+        *reinterpret_cast<float*>(buf(i) + to_scales) = hh ? big : ts;
+    };
     auto store_all_k = [&](int i) {
 #pragma unroll
         for (int x = 0; x < kParts; ++x) store_k(i, x, 0), store_k(i, x, 1);
@@ -956,6 +982,7 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
         f32x4 f[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) f[c] = *reinterpret_cast<const f32x4*>(sc + 8 * c);
+        const float big = *reinterpret_cast<const float*>(buf(i) + kK8Tile + kV8Tile + kBigAt8 + 4);
         read_k(i + 1, 0), read_k(i + 1, 1);
         fence();
 #pragma unroll
@@ -991,6 +1018,11 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
             if (__builtin_amdgcn_ballot_w64(fn - fe != up)) scale_sums(pow2(fn - fe - up));
             fe = fn;
             m = mn;
+        }
+        if (uniform(big) != 0.f) {
+            const int fn = min(fe, most_f(big));
+            scale_sums(pow2(fn - fe));
+            fe = fn;
         }
         // ---- weights times scales times F
         const float nb = m == -INFINITY ? 0.f : (float)fe - m;

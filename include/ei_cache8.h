@@ -89,10 +89,12 @@ int ei_tree_step_paged(ei_stream_t stream, const float* qkv, long row_stride, fl
  * of a block whose entry is not in [0, n_blocks), count as zeros: nothing is read there.
  *
  * Codes are exact in binary16; q and the weights, each times the value's scale, are two binary16 planes, which keep
- * 22 bits of 24 down to 2^-39 of a query's largest value and of a row's largest weight so far.  Sums and softmax
- * in fp32.  Outputs' sums of weight times value must stay below fp32's largest.  Key and value rows that a row
- * does not see never reach it, whatever they hold; a NaN that it does see makes its output NaN.  A batch called
- * twice gives the same bits; they differ in the last ones with the batch a sequence is in. */
+ * 22 bits of 24 down to 2^-39 of a query's largest value and of a row's largest weight times scale so far.  Sums and
+ * softmax in fp32.  Scales of keys up to 2^96 and of values up to 2^118 are provided for (larger ones give infinities
+ * and NaN; beside scales of values above 2^90 smaller ones keep fewer bits).  Key and value rows that a row does not
+ * see never reach it, whatever they hold; a NaN scale that it does see makes its output NaN, a NaN code of a key too,
+ * and one of a value that column of it.  A batch called twice gives the same bits; they differ in the last ones with
+ * the batch a sequence is in. */
 int ei_attn_packed_cache8(ei_stream_t stream, const float* q, long q_stride, float* out, const ei_cache8* cache,
                           const int* block_table, int max_blocks, int n_seq, int rows, int n_head, int n_head_kv,
                           int head_dim, const uint64_t* mask, int mask_words, float scale, const void* plan,

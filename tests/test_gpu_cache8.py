@@ -426,6 +426,31 @@ def test_uneven_scales(gpu, kind, lens, past):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("lens,past", [([1, 4], [900, 300]), ([140], [500])])
+@pytest.mark.parametrize("low,high", [(-80, 60), (-90, -90), (60, -80), (100, 100), (-90, 0)])
+def test_scales_that_jump(gpu, kind, lens, past, low, high):
+    """Values' scales of 2^low in even pages and 2^high in odd ones: small outputs keep their bits, large ones do not
+    overflow on the way.  (Keys that see only the small ones are judged by them.)"""
+    totals = [p + n for p, n in zip(past, lens)]
+    b = Batch(gpu, 4, 1, lens, totals, 32, seed=61)
+    cache = fill_cache(gpu, kind, b.n_blocks, 32, 1, 62, spread=0.3)
+    for s, total in enumerate(totals):
+        for i in range((total + 31) // 32):
+            cache.v_scale[int(b.table_np[s][i])] *= 2.0 ** (low if i % 2 == 0 else high)
+    q = _normal(63, b.rows, 4 * D)
+    out = gpu.attn_packed_cache8(q, cache, b.table, b.plan, b.shape)
+    for s, (n, total) in enumerate(zip(lens, totals)):
+        r = b.rows_of(s)
+        k, v = cached64(cache, b.table_np[s], total)
+        seen, q64 = sees(n, total), q[r].view(n, 4, D).double()
+        want, size = attend64(q64, k, v, seen), attend64(q64, k, v.abs(), seen)
+        # scores of up to 50 log2 units, and 2^-39 of a row's largest weight times scale (see test_uneven_scales)
+        most = attend64(q64, k, v.abs().amax(-1, keepdim=True).expand_as(v), seen)
+        off = (out[r] - want).abs() - total * 2.0 ** -39 * most
+        assert float((off.clamp(min=0.0) / size).max()) < 2.0 ** -20 * 50
+
+
+@pytest.mark.parametrize("kind", KINDS)
 def test_missing_pages_count_as_zeros(gpu, kind):
     lens, totals = [1, 40], [200, 150]
     b = Batch(gpu, 8, 2, lens, totals, 32, seed=30)
