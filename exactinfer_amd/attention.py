@@ -24,6 +24,10 @@ def _stream() -> int:
     return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
+def _stream_on(dev: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
 def _ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
@@ -672,8 +676,9 @@ def cache8_store(qkv: torch.Tensor, cache: Cache8, block_table: torch.Tensor, ba
     turn = _turn_args(cs, pos, shape, batch.rows, q_gamma, k_gamma, dev)
     out = _out_of(batch, out, dev)
     if batch.rows:
-        _capi.call("ei_cache8_store", torch._C._cuda_getCurrentRawStream(dev), qkv.data_ptr(), rs, out.data_ptr(), *where, batch.n_seq, batch.rows,
-                   shape.n_head, shape.n_head_kv, shape.head_dim, *turn, batch.buf.data_ptr(), batch.nbytes)
+        _capi.call("ei_cache8_store", _stream_on(dev), qkv.data_ptr(), rs, out.data_ptr(), *where, batch.n_seq,
+                   batch.rows, shape.n_head, shape.n_head_kv, shape.head_dim, *turn, batch.buf.data_ptr(),
+                   batch.nbytes)
     return out
 
 
@@ -693,7 +698,7 @@ def cache8_load(cache: Cache8, block_table: torch.Tensor, batch: PackedBatch,
     if ks != vs:
         raise ValueError(f"the two outputs must share a row stride, got {ks} and {vs}")
     if batch.rows:
-        _capi.call("ei_cache8_load", torch._C._cuda_getCurrentRawStream(dev), *where, k.data_ptr(), v.data_ptr(), ks, batch.n_seq, batch.rows,
+        _capi.call("ei_cache8_load", _stream_on(dev), *where, k.data_ptr(), v.data_ptr(), ks, batch.n_seq, batch.rows,
                    batch.n_head, batch.n_head_kv, HEAD_DIM, batch.buf.data_ptr(), batch.nbytes)
     return k, v
 
@@ -712,7 +717,7 @@ def attn_packed_cache8(q: torch.Tensor, cache: Cache8, block_table: torch.Tensor
     out = _out_of(batch, out, dev)
     scale = _SCALE if scale is None else float(scale)
     if batch.rows:
-        _capi.call("ei_attn_packed_cache8", torch._C._cuda_getCurrentRawStream(dev), q.data_ptr(), qs, out.data_ptr(), *where, batch.n_seq,
+        _capi.call("ei_attn_packed_cache8", _stream_on(dev), q.data_ptr(), qs, out.data_ptr(), *where, batch.n_seq,
                    batch.rows, shape.n_head, shape.n_head_kv, shape.head_dim, *bits, scale, *batch._tail())
     return out
 
@@ -732,9 +737,8 @@ def packed_step_cache8(qkv: torch.Tensor, cache: Cache8, block_table: torch.Tens
     out = _out_of(batch, out, dev)
     scale = _SCALE if scale is None else float(scale)
     if batch.rows:
-        _capi.call("ei_packed_step_cache8", torch._C._cuda_getCurrentRawStream(dev), qkv.data_ptr(), rs, out.data_ptr(), *where, batch.n_seq,
-                   batch.rows, shape.n_head, shape.n_head_kv, shape.head_dim, *turn, *bits, scale,
-                   *batch._tail())
+        _capi.call("ei_packed_step_cache8", _stream_on(dev), qkv.data_ptr(), rs, out.data_ptr(), *where, batch.n_seq,
+                   batch.rows, shape.n_head, shape.n_head_kv, shape.head_dim, *turn, *bits, scale, *batch._tail())
     return out
 
 
@@ -751,8 +755,8 @@ def attn_tree_paged(q: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor, block_t
     out = _out_of(batch, out, dev)
     scale = _SCALE if scale is None else float(scale)
     if batch.rows:
-        _capi.call("ei_attn_tree_paged", torch._C._cuda_getCurrentRawStream(dev), q.data_ptr(), qs, out.data_ptr(), *pool, batch.n_seq, batch.rows,
-                   shape.n_head, shape.n_head_kv, shape.head_dim, *bits, scale, *batch._tail())
+        _capi.call("ei_attn_tree_paged", _stream_on(dev), q.data_ptr(), qs, out.data_ptr(), *pool, batch.n_seq,
+                   batch.rows, shape.n_head, shape.n_head_kv, shape.head_dim, *bits, scale, *batch._tail())
     return out
 
 
@@ -771,8 +775,8 @@ def tree_step_paged(qkv: torch.Tensor, kc: torch.Tensor, vc: torch.Tensor, block
     out = _out_of(batch, out, dev)
     scale = _SCALE if scale is None else float(scale)
     if batch.rows:
-        _capi.call("ei_tree_step_paged", torch._C._cuda_getCurrentRawStream(dev), qkv.data_ptr(), rs, out.data_ptr(), *pool, batch.n_seq, batch.rows,
-                   shape.n_head, shape.n_head_kv, shape.head_dim, *turn, *bits, scale, *batch._tail())
+        _capi.call("ei_tree_step_paged", _stream_on(dev), qkv.data_ptr(), rs, out.data_ptr(), *pool, batch.n_seq,
+                   batch.rows, shape.n_head, shape.n_head_kv, shape.head_dim, *turn, *bits, scale, *batch._tail())
     return out
 
 
@@ -802,7 +806,7 @@ def cache_keep(kc: torch.Tensor, vc: torch.Tensor, block_table: torch.Tensor, bl
     _check_batch(batch, shape, dev)
     pool = _pool_of(kc, vc, block_table, block_size, batch, shape, dev)
     args, out = _kept_args(batch, kept, n_kept, out, dev)
-    _capi.call("ei_cache_keep", torch._C._cuda_getCurrentRawStream(dev), *pool, batch.n_seq, batch.rows, shape.n_head, shape.n_head_kv,
+    _capi.call("ei_cache_keep", _stream_on(dev), *pool, batch.n_seq, batch.rows, shape.n_head, shape.n_head_kv,
                shape.head_dim, *args)
     return out
 
@@ -814,8 +818,8 @@ def cache8_keep(cache: Cache8, block_table: torch.Tensor, batch: PackedBatch, ke
     _check_planned(batch, dev)
     where = _cache8_args(cache, block_table, batch, batch.n_head_kv, dev)
     args, out = _kept_args(batch, kept, n_kept, out, dev)
-    _capi.call("ei_cache8_keep", torch._C._cuda_getCurrentRawStream(dev), *where, batch.n_seq, batch.rows, batch.n_head, batch.n_head_kv, HEAD_DIM,
-               *args)
+    _capi.call("ei_cache8_keep", _stream_on(dev), *where, batch.n_seq, batch.rows, batch.n_head, batch.n_head_kv,
+               HEAD_DIM, *args)
     return out
 
 

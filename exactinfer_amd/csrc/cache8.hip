@@ -50,10 +50,13 @@ __device__ __forceinline__ size_t head_row(int page, int HKV, int kvh, int shift
 }
 
 // ------------------------------------------------------------------ storing
-// Sixteen lanes per head, eight values each, four heads per wave, as k_rope_rows lays them out.  kVec (rope_dim a multiple
-// of 8): a lane below rope_dim / 8 holds the pieces of four at 4l and rope_dim / 2 + 4l, partners of each other, the
-// others two pieces of the rest; otherwise elements l + 16j, whose partners are read from the row again.
+// Sixteen lanes per head, eight values each, four heads per wave, as k_rope_rows lays them out.  kVec (rope_dim a
+// multiple of 8): a lane below rope_dim / 8 holds the pieces of four at 4l and rope_dim / 2 + 4l, partners of each
+// other, the others two pieces of the rest; otherwise elements l + 16j, whose partners are read from the row again.
 // grid (rows, ceil((H + 2 HKV) / 16)).
+//
+// Bound by memory: 7644 rows of H 32 / HKV 8 (333 MB) 59 to 64 us, 5.2 to 5.6 TB/s, above a large copy's 4.7; with four
+// bytes a lane instead of sixteen 83 us.  48 rows of H 16 / HKV 8 take 5 us: looking up a row's owner and its page.
 template <bool kInt8, bool kVec>
 __global__ __launch_bounds__(256) void k_cache8_store(const float* __restrict__ qkv, long row_stride,
                                                       float* __restrict__ q_out, Cache8Args a,
@@ -176,7 +179,8 @@ __global__ __launch_bounds__(256) void k_cache8_store(const float* __restrict__ 
 }
 
 // ------------------------------------------------------------------ reading back
-// A wave per row and turn, a lane four codes: 32 lanes a head row, two head rows of K and V at a time.
+// A wave per row, a lane four codes: 32 lanes a head row, two head rows of K and V at a time.  Bound by the writes:
+// 61769 rows of 8 heads (636 MB) 98 us back to back, 6.5 TB/s, and 118 over changing pools.
 template <bool kInt8>
 __global__ __launch_bounds__(256) void k_cache8_load(Cache8Args a, float* __restrict__ k_out,
                                                      float* __restrict__ v_out, long out_stride) {
@@ -215,7 +219,8 @@ __global__ __launch_bounds__(256) void k_cache8_load(Cache8Args a, float* __rest
             for (int k = 0; k < 2; ++k) {
                 const f32x4 y = {value_of<kInt8, 0>(x[i][k]) * f[i][k], value_of<kInt8, 1>(x[i][k]) * f[i][k],
                                  value_of<kInt8, 2>(x[i][k]) * f[i][k], value_of<kInt8, 3>(x[i][k]) * f[i][k]};
-                f32x4* dst = reinterpret_cast<f32x4*>((k ? v_out : k_out) + (size_t)b * out_stride + (size_t)h * kHeadDim);
+                float* row = (k ? v_out : k_out) + (size_t)b * out_stride;
+                f32x4* dst = reinterpret_cast<f32x4*>(row + (size_t)h * kHeadDim);
                 __builtin_nontemporal_store(y, dst + c);  // (plain stores: 61769 rows 126 us instead of 100)
             }
         }
@@ -226,7 +231,7 @@ __global__ __launch_bounds__(256) void k_cache8_load(Cache8Args a, float* __rest
 // grid (n_seq, pieces / 256): a thread takes one piece of a sequence's rows, 16 bytes of K, then of V, then (8-bit) the
 // scales.  Latency alone: the list, the lengths and the plan are read at once, a lane per entry looks its two pages
 // up, then the rows are moved kKeepAtOnce at a time.  Entries rise, so kept[j] >= j: no row is read after another has
-// been written over it.
+// been written over it.  Up to nine rows of 48 sequences 5 us in 8-bit pools (8.2 with a thread looking up each row).
 constexpr int kKeepAtOnce = 8;
 template <bool kF32>
 __global__ __launch_bounds__(256) void k_cache_keep(Cache8Args a, float* __restrict__ kc, float* __restrict__ vc,
@@ -352,7 +357,7 @@ constexpr int kFew8ML = kWaves * kRow8 * kRowF;        // LDS: every wave's rows
 constexpr int kFew8F = kFew8ML + kWaves * kRow8 * 2;
 constexpr int kTopF = 96;                              // log2 F at most
 constexpr float kTopW = 0x1p15f;                       // p s_v F at most
-constexpr float kLazy8 = 8.f;                          // the reference moves when a score passes it by more (log2 units)
+constexpr float kLazy8 = 8.f;                          // the reference moves when a score passes it by more
 // Scales of values in between (larger ones are not provided for) keep F so low that p s_v F stays finite.
 constexpr float kBigScale = 0x1p20f, kMostScale = 0x1p118f;
 __device__ __forceinline__ float big_scale(float s) {  // s if it is one, else 0
@@ -362,11 +367,13 @@ __device__ __forceinline__ float big_scale(float s) {  // s if it is one, else 0
 __device__ __forceinline__ int most_f(float big) { return 127 + 118 - (int)(__float_as_uint(big) >> 23); }
 __device__ __forceinline__ float pow2(int e) { return __builtin_amdgcn_ldexpf(1.f, e); }
 
-constexpr int kOnce = 2;  // the streaming cache policy of a buffer load, for codes that are read once
+// The streaming cache policy of a buffer load, for codes that are read once: 60000 keys 27 us, without it 29.
+// (Where 24 sequences share all their keys it costs 2%.)
+constexpr int kOnce = 2;
 
 // ---- units of up to 32 rows
-// A workgroup's share of the few-row list.  A unit's rows are one block of sixteen or two, one per wave; waves of a block
-// take its tiles in turn, each lane its row l % 16 and quarter l / 16:
+// A workgroup's share of the few-row list.  A unit's rows are one block of sixteen or two, one per wave; waves of a
+// block take its tiles in turn, each lane its row l % 16 and quarter l / 16:
 //   S^T[key][row] = K . Q^T: the lane has of key 16 kb + l % 16 codes 32 quarter .. + 31, and gets the scores of the
 //     keys 16 kb + 4 quarter + r (kb = 0, 1; r = 0 .. 3) for its row;
 //   O^T[d][row] = V^T . P^T over the tile's 32 keys in the order of those scores: the lane has codes
@@ -374,9 +381,12 @@ constexpr int kOnce = 2;  // the streaming cache policy of a buffer load, for co
 //     d = 32 quarter + 8 r + y.
 // Bound by reading the codes, two tiles of each wave in flight.  A pass is short where sequences are: the next unit
 // and its pages are looked up during a pass, its queries and first tiles fetched before the waves' sums meet.
+// H 32 / HKV 8, pages of 64, e4m3: 60000 keys of one sequence (127 MB) 27 us, as 24 of 2500 keys 29.6, as 96 of 625
+// 32.4 (one pass after another 34.3 and 41.6); 130000 keys 49 us, 5.6 TB/s, or 6.9 past the 8 us that a call over 31
+// keys takes: launch, plan, unit, page and codes one after another.
 template <bool kInt8, bool kTree>
-__device__ __forceinline__ void few8_walk(const Cache8Args& a, const List& list, int4 sh, int share, int kvh, FastDiv fG,
-                                          float sl2, float* parts, float* smem) {
+__device__ __forceinline__ void few8_walk(const Cache8Args& a, const List& list, int4 sh, int share, int kvh,
+                                          FastDiv fG, float sl2, float* parts, float* smem) {
     constexpr int D = kHeadDim;
     const int tid = unhoisted(threadIdx.x), lane = tid & 63, wu = scalar(tid >> 6);
     const int j = lane & 15, quarter = lane >> 4;
@@ -430,8 +440,9 @@ __device__ __forceinline__ void few8_walk(const Cache8Args& a, const List& list,
 #pragma unroll
             for (int x = 0; x < 2; ++x)
                 t.k[kb][x] = __builtin_amdgcn_raw_buffer_load_b128(rk, ok + 16 * kb * D + 16 * x, 0, kOnce);
-            t.ks[kb] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(sk, (ln >> 4) * 16 + 64 * kb, 0, kOnce));
-            t.vs[kb] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(sv, (ln >> 4) * 16 + 64 * kb, 0, kOnce));
+            const uint32_t os = (ln >> 4) * 16 + 64 * kb;
+            t.ks[kb] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(sk, os, 0, kOnce));
+            t.vs[kb] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(sv, os, 0, kOnce));
         }
 #pragma unroll
         for (int e = 0; e < 8; ++e)
@@ -444,7 +455,8 @@ __device__ __forceinline__ void few8_walk(const Cache8Args& a, const List& list,
     float4 q[8];
     auto load_q = [&](const Unit8& p) {
         const int row = row_of(p), tok = fdiv(row, fG);
-        const float* src = a.q + ((size_t)p.row0 + tok) * a.q_stride + (size_t)(kvh * G + row - tok * G) * D + 32 * quarter;
+        const float* src = a.q + ((size_t)p.row0 + tok) * a.q_stride + (size_t)(kvh * G + row - tok * G) * D;
+        src += 32 * quarter;
 #pragma unroll
         for (int x = 0; x < 8; ++x) q[x] = *reinterpret_cast<const float4*>(src + 4 * x);
     };
@@ -679,7 +691,7 @@ __device__ __forceinline__ void few8_walk(const Cache8Args& a, const List& list,
         {
             const float f = pow2(-fe);
             l *= f;
-            if (m == -INFINITY) {  // (scores of -infinity beside infinite values: parts without weights are passed over)
+            if (m == -INFINITY) {  // (scores of -infinity beside infinite values; parts without weights are left out)
                 float z = 0.f;
 #pragma unroll
                 for (int y = 0; y < 8; ++y)
@@ -745,18 +757,26 @@ __device__ __forceinline__ void few8_walk(const Cache8Args& a, const List& list,
 }
 
 // ---- a wide unit: up to 128 rows
-// Groups of kS waves (four of 32 rows each, or two where the unit has no more than 64 rows) share a tile, the groups take
-// the unit's tiles in turn.  Each wave turns its part of a tile's codes into binary16 in LDS, V transposed, four
-// tiles of a group at a time there (or two), one barrier for half of them.  On v_mfma_f32_32x32x16_f16 S^T[key][row] = K . Q^T gives a lane
-// 16 of a tile's 32 keys for one row, which are the operand of O^T[d][row] = V^T . P^T.
+// Groups of kS waves (four of 32 rows each, or two where the unit has no more than 64 rows) share a tile, the groups
+// take the unit's tiles in turn.  Each wave turns its part of a tile's codes into binary16 in LDS, V transposed, four
+// tiles of a group at a time there (or two), one barrier for half of them.  On v_mfma_f32_32x32x16_f16
+// S^T[key][row] = K . Q^T gives a lane 16 of a tile's 32 keys for one row, which are the operand of
+// O^T[d][row] = V^T . P^T.
 //
 // Matrix and vector instructions of one wave overlap where neither waits for the other: the next tile's scores are
 // taken between the instructions of this one's softmax, and the next tiles' conversions and the second half of the
 // weights' planes between those of P . V, by hand, since the compiler would put each kind together (and every LDS
 // read right before its use).
-constexpr int kK8RowB = 2 * kHeadDim + 16, kK8Tile = kKT * kK8RowB;  // [32 keys][128 d] binary16, rows spread over banks
+//
+// Bound by the matrix unit and its power: 1024 rows after 12000 keys (H 32 / HKV 8, int8) 407 to 423 us, 500 to 517
+// TFLOP/s, 1.0 PFLOP/s over the two plane products, 82 to 85% of what a large fp16 product reaches; the matrix unit is
+// busy 48% of the cycles at 2.0 GHz of 2.4, vector instructions 54%, beside each other.  With the softmax between the
+// products instead of among them 464 us, a barrier for every tile and lanes' addresses made anew 456.  Units of 33 to
+// 64 rows in two groups of four waves, half of them idle: 16 trees of 48 tokens (G 4, 192 rows: units of 128 and 64,
+// e4m3) 188 us against 144.
+constexpr int kK8RowB = 2 * kHeadDim + 16, kK8Tile = kKT * kK8RowB;  // [32 keys][128 d], rows spread over banks
 constexpr int kV8RowB = 2 * kKT + 16, kV8Tile = kHeadDim * kV8RowB;  // [128 d][32 keys]
-constexpr int kBigAt8 = 2 * kKT * 4;                                // after the scales of K and V: the largest big one (of K, of V)
+constexpr int kBigAt8 = 2 * kKT * 4;  // after the scales of K and V: the largest big one (of K, of V)
 constexpr int kScales8 = kBigAt8 + 16;
 constexpr int kBuf8 = kK8Tile + kV8Tile + kScales8;                 // one tile of a group
 static_assert(kBuf8 % 16 == 0, "16-byte pieces");
@@ -930,8 +950,8 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
     };
     auto fence = [] { __builtin_amdgcn_sched_barrier(0); };
 
-    // While tile i is worked on, V and scales of tile i + kLead and K of the one after it go to LDS, where tiles of kRing
-    // before were: every wave was done with those at the last barrier, and will not need these before the next.
+    // While tile i is worked on, V and scales of tile i + kLead and K of the one after it go to LDS, where tiles of
+    // kRing before were: every wave was done with those at the last barrier, and will not need these before the next.
     store_all_k(0);
     store_all_v(0);
     Place at{};
@@ -1165,7 +1185,7 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
 
     // ---- the groups meet through LDS: group g finishes the blocks of 32 d from kOwn g on
     scale_sums(pow2(-fe));
-    if (m == -INFINITY) {  // (scores of -infinity beside infinite values: parts without weights are passed over)
+    if (m == -INFINITY) {  // (scores of -infinity beside infinite values; parts without weights are left out)
         float z = 0.f;
 #pragma unroll
         for (int db = 0; db < 4; ++db)
@@ -1309,7 +1329,8 @@ template <bool kInt8, bool kTree>
 static hipError_t launch_cache8_attn_as(hipStream_t st, const Cache8Args& a, int shares, const PackedParts& parts) {
     static std::atomic<bool> opted;
     constexpr size_t lds = kLds8;
-    if (const hipError_t e = opt_in_lds(opted, (const void*)k_cache8_attn<kInt8, kTree>, lds); e != hipSuccess) return e;
+    if (const hipError_t e = opt_in_lds(opted, (const void*)k_cache8_attn<kInt8, kTree>, lds); e != hipSuccess)
+        return e;
     k_cache8_attn<kInt8, kTree><<<shares * a.HKV, 64 * kWaves, lds, st>>>(a, shares, parts.wide, parts.few);
     return hipGetLastError();
 }

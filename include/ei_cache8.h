@@ -1,5 +1,5 @@
 /*
- * ei_cache8.h — a paged cache of 8-bit keys and values, trees of drafted tokens, and moving an accepted path together.
+ * ei_cache8.h — a paged cache of 8-bit keys and values, trees of drafted tokens, and moving what was accepted.
  *
  * Conventions as in ei_attn.h and ei_packed.h (status codes, device pointers, streams, alignment, limits):
  * queries and outputs fp32, head_dim 128, GQA groups of 1 to 8, nothing allocated, no host
