@@ -298,3 +298,58 @@ def test_drafting_gives_what_single_tokens_give(gpu, kind):
                 for x, y in ((one.k, two.k), (one.v, two.v), (one.k_scale, two.k_scale), (one.v_scale, two.v_scale)):
                     assert torch.equal(x.view(torch.int8)[pg, :, t % bs] if x.dim() == 4 else x[pg, :, t % bs],
                                        y.view(torch.int8)[pg, :, t % bs] if y.dim() == 4 else y[pg, :, t % bs])
+
+
+@pytest.mark.parametrize("kind", ["f32", "int8"])
+def test_captured_round_of_drafting(gpu, kind):
+    """Plan, tree step and keep in one graph on a side stream, replayed with other lengths, trees and accepted paths,
+    the program's own work between the replays; every replay against the same calls made eagerly on another pool."""
+    A, H, HKV, bs, n_seq, n = gpu, 8, 2, 32, 3, 12
+    b = Batch(A, H, HKV, [n] * n_seq, [200, 90, 44], bs, seed=70)
+    cs, qg, kg = A.rope_table(256), 1 + 0.1 * _normal(71, D), 1 + 0.1 * _normal(72, D)
+
+    def pool():
+        if kind == "f32":
+            return _normal(73, b.n_blocks * bs, HKV, D), _normal(74, b.n_blocks * bs, HKV, D)
+        return fill_cache(A, kind, b.n_blocks, bs, HKV, 75)
+
+    def tensors(p):
+        return p if kind == "f32" else (p.k, p.v, p.k_scale, p.v_scale)
+
+    cu_rows, new_len = i32(b.starts), torch.zeros(n_seq, dtype=torch.int32, device="cuda")
+    qkv = _normal(76, b.rows, (H + 2 * HKV) * D)
+    mask, _, pos = b.trees()
+    kept, n_kept = i32([[0] * 4] * n_seq), i32([1] * n_seq)
+
+    def calls(p, out, lengths):
+        b.plan.plan(cu_rows, b.rows, 210, kv_len=b.kv_len)
+        if kind == "f32":
+            A.tree_step_paged(qkv, *p, b.table, bs, b.plan, b.shape, qg, kg, cs, pos=pos, mask=mask, out=out)
+            return A.cache_keep(*p, b.table, bs, b.plan, b.shape, kept, n_kept, out=lengths)
+        A.packed_step_cache8(qkv, p, b.table, b.plan, b.shape, qg, kg, cs, pos=pos, mask=mask, out=out)
+        return A.cache8_keep(p, b.table, b.plan, kept, n_kept, out=lengths)
+
+    one, two = pool(), pool()
+    out, stream, graph = torch.zeros((b.rows, H, D), device="cuda"), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        calls(pool(), out, new_len)  # (the first call, outside the capture, on a pool of its own)
+        stream.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            calls(one, out, new_len)
+    torch.cuda.current_stream().wait_stream(stream)
+    for turn, (totals, keep) in enumerate([([200, 90, 44], [[0, 3, 7, 9], [1, 2, 0, 0], [5, 0, 0, 0]]),
+                                           ([130, 91, 12], [[0, 1, 2, 3], [11, 0, 0, 0], [2, 2, 2, 2]]),
+                                           ([209, 40, 100], [[4, 8, 10, 11], [0, 5, 6, 20], [0, 0, 0, 0]])]):
+        b.totals = totals
+        new_mask, _, new_pos = b.trees()
+        mask.copy_(new_mask), pos.copy_(new_pos), b.kv_len.copy_(i32(totals))
+        kept.copy_(i32(keep)), n_kept.copy_(i32([4, 2 - turn % 2, turn]))
+        qkv.copy_(_normal(80 + turn, *qkv.shape))
+        graph.replay()
+        torch.cuda.synchronize()
+        want, lengths = torch.zeros_like(out), torch.zeros_like(new_len)
+        calls(two, want, lengths)
+        assert torch.equal(out, want) and torch.equal(new_len, lengths)
+        for x, y in zip(tensors(one), tensors(two)):
+            assert torch.equal(x.view(torch.int8), y.view(torch.int8))
