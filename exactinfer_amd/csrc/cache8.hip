@@ -312,7 +312,8 @@ __global__ __launch_bounds__(256) void k_cache_keep(Cache8Args a, float* __restr
 //            p s_v lies between 2^14 and 2^15 at first, and F goes down where one passes that (the sums go with it), up
 //            where the reference m rises (the sums stay).  So what the planes lose, 2^-39 of the row's largest
 //            weight times scale, never shows, however uneven the values' scales are.  m is a whole number: every
-//            factor of the sums is a power of two, exact.
+//            factor of the sums is a power of two, exact.  The weights' sum has F too, so it stops at 2^96, and a pass
+//            that ends with it there (values' scales below 2^-82) is done again with another arithmetic (pass_again).
 struct Tile8 {
     u32x4 k[2][2];  // [sixteen keys][half of the lane's 32 codes]
     u32x2 v[8];
@@ -357,6 +358,7 @@ constexpr int kFew8ML = kWaves * kRow8 * kRowF;        // LDS: every wave's rows
 constexpr int kFew8F = kFew8ML + kWaves * kRow8 * 2;
 constexpr int kTopF = 96;                              // log2 F at most
 constexpr float kTopW = 0x1p15f;                       // p s_v F at most
+constexpr int kAgain = 64;                              // flags of passes to be done again
 constexpr float kLazy8 = 8.f;                          // the reference moves when a score passes it by more
 // Scales of values in between (larger ones are not provided for) keep F so low that p s_v F stays finite.
 constexpr float kBigScale = 0x1p20f, kMostScale = 0x1p118f;
@@ -371,14 +373,152 @@ __device__ __forceinline__ float pow2(int e) { return __builtin_amdgcn_ldexpf(1.
 // (Where 24 sequences share all their keys it costs 2%.)
 constexpr int kOnce = 2;
 
-// ---- units of up to 32 rows
-// A workgroup's share of the few-row list.  A unit's rows are one block of sixteen or two, one per wave; waves of a
-// block take its tiles in turn, each lane its row l % 16 and quarter l / 16:
+// ---- sixteen rows of a wave, a tile at a time: each lane its row l % 16 and quarter l / 16
 //   S^T[key][row] = K . Q^T: the lane has of key 16 kb + l % 16 codes 32 quarter .. + 31, and gets the scores of the
 //     keys 16 kb + 4 quarter + r (kb = 0, 1; r = 0 .. 3) for its row;
 //   O^T[d][row] = V^T . P^T over the tile's 32 keys in the order of those scores: the lane has codes
 //     8 (l % 16) .. + 7 of its eight keys, put together pair of keys by pair; sum y, register r is
 //     d = 32 quarter + 8 r + y.
+__device__ __forceinline__ Rsrc codes_rsrc(const uint8_t* codes, size_t row, int there) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(codes) + row * kHeadDim, 0, there * kHeadDim,
+                                             kBufferDword3);
+}
+// `there` keys of the tile whose first head row is `row`
+__device__ __forceinline__ void load_tile(const Cache8Args& a, size_t row, int there, Tile8& t) {
+    constexpr int D = kHeadDim;
+    auto scales_at = [&](const float* scales) {  // (whole tiles: pages hold them)
+        return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(scales) + row, 0, there ? kKT * 4 : 0,
+                                                 kBufferDword3);
+    };
+    const uint32_t ln = lane_now();
+    const Rsrc rk = codes_rsrc(a.k8, row, there), rv = codes_rsrc(a.v8, row, there), sk = scales_at(a.ks),
+               sv = scales_at(a.vs);
+    const uint32_t ok = (ln & 15) * D + (ln >> 4) * 32, ov = (ln >> 4) * (4 * D) + (ln & 15) * 8;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+            t.k[kb][x] = __builtin_amdgcn_raw_buffer_load_b128(rk, ok + 16 * kb * D + 16 * x, 0, kOnce);
+        const uint32_t os = (ln >> 4) * 16 + 64 * kb;
+        t.ks[kb] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(sk, os, 0, kOnce));
+        t.vs[kb] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(sv, os, 0, kOnce));
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+        t.v[e] = __builtin_amdgcn_raw_buffer_load_b64(rv, ov + (16 * (e >> 2) + (e & 3)) * D, 0, kOnce);
+}
+// The planes of a row's d = 32 quarter + 8 x + 0 .. 7, from its values and the softmax scale.
+struct Query8 {
+    u32x4 h[4], l[4];
+    float s;  // takes the row's scaling out of its scores
+    __device__ __forceinline__ void set(float4 (&q)[8], float sl2) {
+        float most = 0.f;
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            q[x] = make_float4(q[x].x * sl2, q[x].y * sl2, q[x].z * sl2, q[x].w * sl2);
+            most = fmaxf(fmaxf(most, __builtin_fabsf(q[x].x)), __builtin_fabsf(q[x].y));
+            most = fmaxf(fmaxf(most, __builtin_fabsf(q[x].z)), __builtin_fabsf(q[x].w));
+        }
+        most = half_max(fmaxf(most, lane_xor16(most)));
+        const uint32_t f = scale_to<14>(most);
+        const float fq = __uint_as_float(f);
+        s = inverse(f);
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            uint32_t hi[4], lo[4];
+#pragma unroll
+            for (int y = 0; y < 2; ++y) {
+                const float4 v = q[2 * x + y];
+                split_f16(v.x * fq, v.y * fq, hi[2 * y], lo[2 * y]);
+                split_f16(v.z * fq, v.w * fq, hi[2 * y + 1], lo[2 * y + 1]);
+            }
+            h[x] = u32x4{hi[0], hi[1], hi[2], hi[3]};
+            l[x] = u32x4{lo[0], lo[1], lo[2], lo[3]};
+        }
+    }
+};
+template <bool kInt8>
+__device__ __forceinline__ void scores_of(const Tile8& t, const Query8& q, f32x4 (&s)[2]) {
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+        s[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const uint32_t lo = flipped<kInt8>(t.k[kb][x >> 1][2 * (x & 1)]);
+            const uint32_t hi = flipped<kInt8>(t.k[kb][x >> 1][2 * (x & 1) + 1]);
+            const u32x4 kf = {pair_f16<kInt8, 0>(lo), pair_f16<kInt8, 1>(lo), pair_f16<kInt8, 0>(hi),
+                              pair_f16<kInt8, 1>(hi)};
+            s[kb] = mfma16(kf, q.l[x], s[kb]);
+            s[kb] = mfma16(kf, q.h[x], s[kb]);
+        }
+    }
+}
+// (whether a code of V is NaN, and zeros in place of such ones)
+__device__ __forceinline__ bool take_nans(Tile8& t) {
+    uint32_t nan = 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            nan |= nan_bytes(t.v[e][x]);
+            t.v[e][x] = without_nan(t.v[e][x]);
+        }
+    return __builtin_amdgcn_ballot_w64(nan != 0) != 0;
+}
+struct Planes8 {  // of eight weights
+    u32x4 h, l;
+    __device__ __forceinline__ explicit Planes8(const float (&w)[8]) {
+        uint32_t wh[4], wl[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) split_f16(w[2 * r], w[2 * r + 1], wh[r], wl[r]);
+        h = u32x4{wh[0], wh[1], wh[2], wh[3]}, l = u32x4{wl[0], wl[1], wl[2], wl[3]};
+    }
+};
+template <bool kInt8>
+__device__ __forceinline__ void add_values(const Tile8& t, const Planes8& p, f32x4 (&o)[8]) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+        uint32_t vf[4][4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {  // keys 2e, 2e + 1 of the lane's eight
+            const uint32_t u = t.v[2 * e][x], w = t.v[2 * e + 1][x];
+            const uint32_t lo = flipped<kInt8>(__builtin_amdgcn_perm(w, u, 0x05010400u));
+            const uint32_t hi = flipped<kInt8>(__builtin_amdgcn_perm(w, u, 0x07030602u));
+            vf[0][e] = pair_f16<kInt8, 0>(lo), vf[1][e] = pair_f16<kInt8, 1>(lo);
+            vf[2][e] = pair_f16<kInt8, 0>(hi), vf[3][e] = pair_f16<kInt8, 1>(hi);
+        }
+#pragma unroll
+        for (int y = 0; y < 4; ++y) {
+            const u32x4 v = {vf[y][0], vf[y][1], vf[y][2], vf[y][3]};
+            o[4 * x + y] = mfma16(v, p.l, o[4 * x + y]);
+            o[4 * x + y] = mfma16(v, p.h, o[4 * x + y]);
+        }
+    }
+}
+// NaN among the codes of a tile of V (rsrc rv) into the sums of rows that see them (`bits`).
+__device__ __forceinline__ void put_nans(const Rsrc& rv, uint32_t bits, int quarter, f32x4 (&o)[8]) {
+    uint32_t at = 0;  // the lane's columns d = 32 quarter + i that have one, a bit each
+#pragma unroll 1
+    for (int c = 0; c < kKT; ++c) {
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(rv, c * kHeadDim + 32 * quarter + 16 * x, 0, 0);
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+                const uint32_t nan = bits >> c & 1 ? nan_bytes(v[y]) : 0u;
+                const uint32_t four = (nan >> 7 & 1) | (nan >> 14 & 2) | (nan >> 21 & 4) | (nan >> 28 & 8);
+                at |= four << (16 * x + 4 * y);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 32; ++i)
+        if (at >> i & 1) o[i & 7][i >> 3] = __builtin_nanf("");
+}
+
+// ---- units of up to 32 rows
+// A workgroup's share of the few-row list.  A unit's rows are one block of sixteen or two, one per wave; waves of a
+// block take its tiles in turn.
 // Bound by reading the codes, two tiles of each wave in flight.  A pass is short where sequences are: the next unit
 // and its pages are looked up during a pass, its queries and first tiles fetched before the waves' sums meet.
 // H 32 / HKV 8, pages of 64, e4m3: 60000 keys of one sequence (127 MB) 27 us, as 24 of 2500 keys 29.6, as 96 of 625
@@ -386,7 +526,7 @@ constexpr int kOnce = 2;
 // keys takes: launch, plan, unit, page and codes one after another.
 template <bool kInt8, bool kTree>
 __device__ __forceinline__ void few8_walk(const Cache8Args& a, const List& list, int4 sh, int share, int kvh,
-                                          FastDiv fG, float sl2, float* parts, float* smem) {
+                                          FastDiv fG, float sl2, float* parts, float* smem, uint8_t* again) {
     constexpr int D = kHeadDim;
     const int tid = unhoisted(threadIdx.x), lane = tid & 63, wu = scalar(tid >> 6);
     const int j = lane & 15, quarter = lane >> 4;
@@ -406,7 +546,8 @@ __device__ __forceinline__ void few8_walk(const Cache8Args& a, const List& list,
         p.T = len;  // (a few-row unit is its sequence's last: its last row sees all)
         p.kt_lo = at == first ? first_tile : 0;
         p.nrange = (cut >= 0 ? cut : (int)y.y) - p.kt_lo;
-        p.part = p.kt_lo > 0 || cut >= 0 ? parts + part_at(true, share * a.HKV + kvh, p.kt_lo > 0 ? 0 : 1) : nullptr;
+        const int place = scalar((int)part_at(true, share * a.HKV + kvh, p.kt_lo > 0 ? 0 : 1));
+        p.part = p.kt_lo > 0 || cut >= 0 ? parts + place : nullptr;
         p.nb = p.nflat - kUnitRows * p.u > kRow8 ? 2 : 1;
         p.step = kWaves / p.nb, p.off = wu / p.nb;
         p.n_mine = (p.nrange - p.off + p.step - 1) / p.step;
@@ -423,31 +564,7 @@ __device__ __forceinline__ void few8_walk(const Cache8Args& a, const List& list,
         const bool ok = i < p.n_mine && pg >= 0 && pg < a.n_blocks;
         return Place{ok ? head_row(pg, a.HKV, kvh, a.bshift, t0) : 0, ok ? min(kKT, p.T - t0) : 0};
     };
-    auto codes_at = [&](const uint8_t* codes, const Place& at) {
-        return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(codes) + at.row * D, 0, at.there * D,
-                                                 kBufferDword3);
-    };
-    auto scales_at = [&](const float* scales, const Place& at) {  // (whole tiles: pages hold them)
-        return __builtin_amdgcn_make_buffer_rsrc(const_cast<float*>(scales) + at.row, 0, at.there ? kKT * 4 : 0,
-                                                 kBufferDword3);
-    };
-    auto load = [&](Tile8& t, const Place& at) {
-        const uint32_t ln = lane_now();
-        const Rsrc rk = codes_at(a.k8, at), rv = codes_at(a.v8, at), sk = scales_at(a.ks, at), sv = scales_at(a.vs, at);
-        const uint32_t ok = (ln & 15) * D + (ln >> 4) * 32, ov = (ln >> 4) * (4 * D) + (ln & 15) * 8;
-#pragma unroll
-        for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-            for (int x = 0; x < 2; ++x)
-                t.k[kb][x] = __builtin_amdgcn_raw_buffer_load_b128(rk, ok + 16 * kb * D + 16 * x, 0, kOnce);
-            const uint32_t os = (ln >> 4) * 16 + 64 * kb;
-            t.ks[kb] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(sk, os, 0, kOnce));
-            t.vs[kb] = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(sv, os, 0, kOnce));
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e)
-            t.v[e] = __builtin_amdgcn_raw_buffer_load_b64(rv, ov + (16 * (e >> 2) + (e & 3)) * D, 0, kOnce);
-    };
+    auto load = [&](Tile8& t, const Place& at) { load_tile(a, at.row, at.there, t); };
     // this lane's row of a unit (rows past the last repeat it), and its query, d = 32 quarter .. + 31
     auto row_of = [&](const Unit8& p) {
         return min(kUnitRows * p.u + kRow8 * (wu & (p.nb - 1)) + j, p.nflat - 1);
@@ -479,34 +596,9 @@ __device__ __forceinline__ void few8_walk(const Cache8Args& a, const List& list,
         const int tok = fdiv(row_of(p), fG), qpos = p.pos0 + tok;
         const int f0 = kUnitRows * p.u, block0 = min(f0 + kRow8 * (wu & (p.nb - 1)), p.nflat - 1);
         const int nfull = max(kTree ? p.pos0 : p.pos0 + fdiv(block0, fG) + 1, 0) / kKT;
-        // q: planes of d = 32 quarter + 8 x + 0 .. 7
-        u32x4 qh[4], ql[4];
-        float sq;  // takes the row's scaling out of its scores
-        {
-            float most = 0.f;
-#pragma unroll
-            for (int x = 0; x < 8; ++x) {
-                q[x] = make_float4(q[x].x * sl2, q[x].y * sl2, q[x].z * sl2, q[x].w * sl2);
-                most = fmaxf(fmaxf(most, __builtin_fabsf(q[x].x)), __builtin_fabsf(q[x].y));
-                most = fmaxf(fmaxf(most, __builtin_fabsf(q[x].z)), __builtin_fabsf(q[x].w));
-            }
-            most = half_max(fmaxf(most, lane_xor16(most)));
-            const uint32_t f = scale_to<14>(most);
-            const float fq = __uint_as_float(f);
-            sq = inverse(f);
-#pragma unroll
-            for (int x = 0; x < 4; ++x) {
-                uint32_t h[4], l[4];
-#pragma unroll
-                for (int y = 0; y < 2; ++y) {
-                    const float4 v = q[2 * x + y];
-                    split_f16(v.x * fq, v.y * fq, h[2 * y], l[2 * y]);
-                    split_f16(v.z * fq, v.w * fq, h[2 * y + 1], l[2 * y + 1]);
-                }
-                qh[x] = u32x4{h[0], h[1], h[2], h[3]};
-                ql[x] = u32x4{l[0], l[1], l[2], l[3]};
-            }
-        }
+        Query8 planes;
+        planes.set(q, sl2);
+        const float sq = planes.s;
         f32x4 o[8];
         float m = -INFINITY, l = 0.f, limit = 0.f;  // (limit of a row without weights so far)
         int fe = 0;                                 // log2 F
@@ -525,19 +617,7 @@ __device__ __forceinline__ void few8_walk(const Cache8Args& a, const List& list,
         auto tile = [&](Tile8& t, int i) {
             const int kt = index(p, i);
             f32x4 s[2];
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb) {
-                s[kb] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int x = 0; x < 4; ++x) {
-                    const uint32_t lo = flipped<kInt8>(t.k[kb][x >> 1][2 * (x & 1)]);
-                    const uint32_t hi = flipped<kInt8>(t.k[kb][x >> 1][2 * (x & 1) + 1]);
-                    const u32x4 kf = {pair_f16<kInt8, 0>(lo), pair_f16<kInt8, 1>(lo), pair_f16<kInt8, 0>(hi),
-                                      pair_f16<kInt8, 1>(hi)};
-                    s[kb] = mfma16(kf, ql[x], s[kb]);
-                    s[kb] = mfma16(kf, qh[x], s[kb]);
-                }
-            }
+            scores_of<kInt8>(t, planes, s);
             uint32_t bits = ~0u;
             if (kt >= nfull) {
                 bits = kTree ? tree_bits(a, p, qpos, kt * kKT) : causal_bits(qpos, kt * kKT);
@@ -605,41 +685,12 @@ __device__ __forceinline__ void few8_walk(const Cache8Args& a, const List& list,
                 fe = fn;
                 if (over) limit = kTopW;
             }
-            uint32_t wh[4], wl[4];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) split_f16(wt[2 * r], wt[2 * r + 1], wh[r], wl[r]);
-            const u32x4 ph = {wh[0], wh[1], wh[2], wh[3]}, pl = {wl[0], wl[1], wl[2], wl[3]};
+            const Planes8 w(wt);
             if constexpr (!kInt8) {
-                if (kt >= nfull) {  // a NaN that not every row sees must not meet them: put in at the end
-                    uint32_t nan = 0;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-#pragma unroll
-                        for (int x = 0; x < 2; ++x) {
-                            nan |= nan_bytes(t.v[e][x]);
-                            t.v[e][x] = without_nan(t.v[e][x]);
-                        }
-                    if (__builtin_amdgcn_ballot_w64(nan != 0)) nan_tile = min(nan_tile, i);
-                }
+                // a NaN that not every row sees must not meet them: put in at the end
+                if (kt >= nfull && take_nans(t)) nan_tile = min(nan_tile, i);
             }
-#pragma unroll
-            for (int x = 0; x < 2; ++x) {
-                uint32_t vf[4][4];
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {  // keys 2e, 2e + 1 of the lane's eight
-                    const uint32_t u = t.v[2 * e][x], w = t.v[2 * e + 1][x];
-                    const uint32_t lo = flipped<kInt8>(__builtin_amdgcn_perm(w, u, 0x05010400u));
-                    const uint32_t hi = flipped<kInt8>(__builtin_amdgcn_perm(w, u, 0x07030602u));
-                    vf[0][e] = pair_f16<kInt8, 0>(lo), vf[1][e] = pair_f16<kInt8, 1>(lo);
-                    vf[2][e] = pair_f16<kInt8, 0>(hi), vf[3][e] = pair_f16<kInt8, 1>(hi);
-                }
-#pragma unroll
-                for (int y = 0; y < 4; ++y) {
-                    const u32x4 v = {vf[y][0], vf[y][1], vf[y][2], vf[y][3]};
-                    o[4 * x + y] = mfma16(v, pl, o[4 * x + y]);
-                    o[4 * x + y] = mfma16(v, ph, o[4 * x + y]);
-                }
-            }
+            add_values<kInt8>(t, w, o);
         };
         const Unit8 next = more ? make(at + 1, nx, ny) : p;
         int n0 = -1, n1 = -1;  // the next unit's first pages
@@ -656,26 +707,15 @@ __device__ __forceinline__ void few8_walk(const Cache8Args& a, const List& list,
             pg = page(p, i + 4);
             __builtin_amdgcn_sched_barrier(0);
         }
+        // F stopped: scales below 2^-82 (or zeros)
+        if (__builtin_amdgcn_ballot_w64(fe == kTopF)) again[min(turn, kAgain - 1)] = 1;
         if constexpr (!kInt8) {
 #pragma unroll 1
             for (int i = nan_tile; i < p.n_mine; ++i) {
                 const int k0 = index(p, i) * kKT;
-                const uint32_t bits = kTree ? tree_bits(a, p, qpos, k0) : causal_bits(qpos, k0);
-                const Rsrc rv = codes_at(a.v8, place(p, i, page(p, i)));
-#pragma unroll 1
-                for (int c = 0; c < kKT; ++c) {
-#pragma unroll
-                    for (int x = 0; x < 2; ++x) {
-                        const u32x4 v = __builtin_amdgcn_raw_buffer_load_b128(rv, c * D + 32 * quarter + 16 * x, 0, 0);
-#pragma unroll
-                        for (int y = 0; y < 4; ++y) {  // d = 32 quarter + 16x + 4y + 0 .. 3
-                            const uint32_t nan = bits >> c & 1 ? nan_bytes(v[y]) : 0u;
-#pragma unroll
-                            for (int z = 0; z < 4; ++z)
-                                if (nan >> (8 * z) & 0x80) o[4 * (y & 1) + z][2 * x + (y >> 1)] = __builtin_nanf("");
-                        }
-                    }
-                }
+                const Place at = place(p, i, page(p, i));
+                put_nans(codes_rsrc(a.v8, at.row, at.there),
+                         kTree ? tree_bits(a, p, qpos, k0) : causal_bits(qpos, k0), quarter, o);
             }
         }
         if (more) {
@@ -792,7 +832,9 @@ struct Wide8 {
     static constexpr int kF = kEnd > kTilesF ? kEnd : kTilesF;
 };
 constexpr int kNanAt8 = Wide8<4>::kF > Wide8<2>::kF ? Wide8<4>::kF : Wide8<2>::kF;  // a word: NaN codes were met
-constexpr int kLds8 = 4 * (kNanAt8 + 4);
+// Flags of the passes to be done again, a byte each: 64 of the wide ones, 64 of the few-row ones (from the 64th on one).
+constexpr int kAgainAt8 = kNanAt8 + 4;
+constexpr int kLds8 = 4 * kAgainAt8 + 2 * kAgain;
 static_assert(kLds8 <= 160 * 1024 && 2 * kFew8F <= kNanAt8, "LDS budget");
 __device__ __forceinline__ floatx16 mfma32(u32x4 a, u32x4 b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0,
@@ -801,7 +843,7 @@ __device__ __forceinline__ floatx16 mfma32(u32x4 a, u32x4 b, floatx16 c) {
 
 template <bool kInt8, bool kTree, int kS>
 __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, int kvh, FastDiv fG, float sl2,
-                                           float* smem) {
+                                           float* smem, uint8_t* again) {
     constexpr int D = kHeadDim, kN = Wide8<kS>::kN, kParts = 4 / kS;  // (of a tile, each 8 rows of K and 32 d of V)
     constexpr int kRing = Wide8<kS>::kRing, kLead = kRing / 2;
     const int tid = unhoisted(threadIdx.x), lane = tid & 63, w = tid >> 6;
@@ -878,7 +920,9 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
         *reinterpret_cast<u32x2*>(d + kV8RowB) = u32x2{pair_f16<kInt8, 1>(lo), pair_f16<kInt8, 1>(hi)};
     };
     // (the upper half of the wave writes the largest big one)
-    const uint32_t to_scales = kK8Tile + kV8Tile + (hh ? kBigAt8 + 4 * (hw & 1) : 4 * kKT * (hw & 1) + 4 * col);
+    // (no branch: a spill among the instructions of one side would save half of the lanes)
+    const uint32_t to_scales = kK8Tile + kV8Tile + 4 * kKT * (hw & 1) + 4 * col +
+                               hh * (kBigAt8 + 4 * (hw & 1) - 4 * kKT * (hw & 1) - 4 * col);
     auto store_scales = [&](int i) {
         float big = 0.f;
         if (__builtin_amdgcn_ballot_w64(__builtin_fabsf(ts) > kBigScale)) big = wave_max(big_scale(ts));
@@ -1155,6 +1199,7 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
         if (i + 1 < n_mine) tile(i + 1, odd, even);
         lds_barrier();
     }
+    if (__builtin_amdgcn_ballot_w64(fe == kTopF)) *again = 1;  // F stopped: scales below 2^-82 (or zeros)
     if constexpr (!kInt8) {
         if (scalar(*nan_met)) {
             // the group's tiles that not every row of the unit sees all of
@@ -1263,6 +1308,140 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
     }
 }
 
+// ---- sixteen rows with two references
+// Where F could not serve, a pass is done again when the workgroup is through with the others: sixteen rows for each wave,
+// which takes all tiles, with two references, both whole numbers: m of the weights' sum, and u of the products' sums, the
+// largest log2 of a weight times its value's scale, rounded up.  The operand is (the scale's fraction)
+// 2^(s + its exponent - u + 14), so that no scale overflows or underflows, whatever stands beside it; a key that the row
+// does not see is in neither.  One tile after the other, nothing in flight.
+template <bool kInt8, bool kTree, bool kFew>
+__device__ __forceinline__ void pass_again(const Cache8Args& a, const Pass& p, int kvh, FastDiv fG, float sl2) {
+    constexpr int D = kHeadDim;
+    const int tid = unhoisted(threadIdx.x), lane = tid & 63, j = lane & 15, quarter = lane >> 4, G = (int)fG.d;
+    const int i0 = kRow8 * scalar(tid >> 6), f0 = kUnitRows * p.u + i0;
+    if (f0 >= p.nflat) return;  // wave-uniform, no barrier here
+    const int row = min(f0 + j, p.nflat - 1), tok = fdiv(row, fG), qpos = p.pos0 + tok, end = p.kt_lo + p.nrange;
+    Query8 planes;
+    {
+        const float* src = a.q + ((size_t)p.row0 + tok) * a.q_stride + (size_t)(kvh * G + row - tok * G) * D;
+        float4 q[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = *reinterpret_cast<const float4*>(src + 32 * quarter + 4 * i);
+        planes.set(q, sl2);
+    }
+    auto row_max = [&](float y) { return half_max(fmaxf(y, lane_xor16(y))); };
+    f32x4 o[8];
+    float m = -INFINITY, l = 0.f, u = -INFINITY;
+#pragma unroll
+    for (int y = 0; y < 8; ++y) o[y] = f32x4{0.f, 0.f, 0.f, 0.f};
+    struct Place {
+        size_t row;
+        int there;
+    };
+    auto place = [&](int kt) {
+        const int pg = page_of<true>(a, p, kt * kKT);
+        const bool ok = pg >= 0 && pg < a.n_blocks;
+        return Place{ok ? head_row(pg, a.HKV, kvh, a.bshift, kt * kKT) : 0, ok ? min(kKT, p.T - kt * kKT) : 0};
+    };
+    auto visible = [&](int kt) { return kTree ? tree_bits(a, p, qpos, kt * kKT) : causal_bits(qpos, kt * kKT); };
+#pragma unroll 1
+    for (int kt = p.kt_lo; kt < end; ++kt) {
+        const Place at = place(kt);
+        Tile8 t;
+        load_tile(a, at.row, at.there, t);
+        const uint32_t bits = visible(kt), mine = bits >> (4 * quarter);
+        f32x4 s[2];
+        scores_of<kInt8>(t, planes, s);
+        float score[8], scale[8], ms = -INFINITY, us = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const bool seen = (mine >> (16 * (r >> 2) + (r & 3)) & 1) != 0;
+            score[r] = seen ? s[r >> 2][r & 3] * t.ks[r >> 2][r & 3] * planes.s : -INFINITY;
+            scale[r] = seen ? t.vs[r >> 2][r & 3] : 0.f;
+            ms = fmaxf(ms, score[r]);
+            if (scale[r] != 0.f) us = fmaxf(us, score[r] + (float)__builtin_amdgcn_frexp_expf(scale[r]));
+        }
+        const float mn = fmaxf(m, ceilf(row_max(ms))), un = fmaxf(u, ceilf(row_max(us)));
+        l *= m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        const float by = u == un ? 1.f : __builtin_amdgcn_exp2f(u - un);
+#pragma unroll
+        for (int y = 0; y < 8; ++y)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[y][r] *= by;
+        m = mn, u = un;
+        float w[8], sum = 0.f;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const float e = (float)(14 + __builtin_amdgcn_frexp_expf(scale[r]));
+            sum += __builtin_amdgcn_exp2f(mn == -INFINITY ? score[r] : score[r] - mn);
+            w[r] = __builtin_amdgcn_frexp_mantf(scale[r]) *
+                   __builtin_amdgcn_exp2f(score[r] + (un == -INFINITY ? e : e - un));
+        }
+        l += sum;
+        if constexpr (kInt8) {
+            add_values<kInt8>(t, Planes8(w), o);
+        } else {
+            const bool nans = take_nans(t);
+            add_values<kInt8>(t, Planes8(w), o);
+            if (nans) put_nans(codes_rsrc(a.v8, at.row, at.there), bits, quarter, o);
+        }
+    }
+    // The weights' sum goes to 1/2 .. 1 (to 2^-17 where values may be near fp32's largest: parts are added), the sums of
+    // products with it.
+    const float sum = half_sum(l + lane_xor16(l)), up = fminf(fmaxf(u - m, -400.f), 400.f);
+    const int down = __builtin_amdgcn_frexp_expf(sum) + (up > 64.f ? 16 : 0);
+    l = __builtin_amdgcn_ldexpf(l, -down);
+    m += (float)down;
+#pragma unroll
+    for (int y = 0; y < 8; ++y)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[y][r] = __builtin_amdgcn_ldexpf(o[y][r], (int)up - 14 - down);
+    if (m == -INFINITY) {  // (scores of -infinity beside infinite values; parts without weights are left out)
+        float z = 0.f;
+#pragma unroll
+        for (int y = 0; y < 8; ++y)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) z = __builtin_fmaf(o[y][r], 0.f, z);
+        l += z;
+    }
+    const float all = half_sum(l + lane_xor16(l));
+    bool none = qpos < 0;  // a row that sees no key: zeros
+    if constexpr (kTree) none = all == 0.f && tree_sees_none(a, p.row0, p.pos0, tok);
+    const float inv = p.part ? 1.f : none ? 0.f : 1.f / all;
+    float* dst = p.part ? p.part + (i0 + j) * D : a.out + (((size_t)p.row0 + tok) * a.H + kvh * G + row - tok * G) * D;
+    if (f0 + j < p.nflat) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+#pragma unroll
+            for (int y = 0; y < 8; y += 4)
+                *reinterpret_cast<float4*>(dst + 32 * quarter + 8 * r + y) =
+                    make_float4(o[y][r] * inv, o[y + 1][r] * inv, o[y + 2][r] * inv, o[y + 3][r] * inv);
+        if (p.part && quarter == 0)
+            *reinterpret_cast<float2*>(p.part + (kFew ? kFewRows : kUnitRows) * D + 2 * (i0 + j)) = make_float2(m, all);
+    }
+}
+
+// The flagged passes of a workgroup's share.  (Not inlined: the registers of the passes before are short.)
+template <bool kInt8, bool kTree>
+__device__ __forceinline__ void share_again(Cache8Args a, int shares, int share, int kvh, uint64_t wides,
+                                                      uint64_t fews, float* wide_parts, float* few_parts) {
+    __syncthreads();  // (with the workgroup's writes done: what is written now comes after them)
+    const PlanView pv = plan_view(const_cast<char*>(a.plan), a.n_seq, a.rows, a.H / a.HKV, shares);
+    const FastDiv fG = fast_div((uint32_t)(a.H / a.HKV));
+    const float sl2 = a.scale * 1.44269504088896340736f;
+    int n = 0;
+    walk_share<false>(a, pv.wide, *reinterpret_cast<const int4*>(pv.wide.shares + share),
+                      scalar(reinterpret_cast<const int*>(a.plan)[kHeadRounds]), shares, share, kvh, fG, wide_parts,
+                      [&](const Pass& p) {
+                          if (wides >> min(n++, kAgain - 1) & 1) pass_again<kInt8, kTree, false>(a, p, kvh, fG, sl2);
+                      });
+    n = 0;
+    walk_share<true>(a, pv.few, *reinterpret_cast<const int4*>(pv.few.shares + share), 0, shares, share, kvh, fG,
+                     few_parts, [&](const Pass& p) {
+                         if (fews >> min(n++, kAgain - 1) & 1) pass_again<kInt8, kTree, true>(a, p, kvh, fG, sl2);
+                     });
+}
+
 // grid shares x KV heads, as k_packed_attn
 template <bool kInt8, bool kTree>
 __global__ __launch_bounds__(64 * kWaves) void k_cache8_attn(Cache8Args a, int shares, float* __restrict__ wide_parts,
@@ -1276,12 +1455,21 @@ __global__ __launch_bounds__(64 * kWaves) void k_cache8_attn(Cache8Args a, int s
     if (!plan_fits(a.plan, a.n_seq, a.rows, a.H, a.HKV, false)) return;
     const FastDiv fG = fast_div((uint32_t)(a.H / a.HKV));
     const float sl2 = a.scale * 1.44269504088896340736f;  // scores come out in log2 units
+    uint8_t* const again = reinterpret_cast<uint8_t*>(smem + kAgainAt8);
+    if (threadIdx.x < 2 * kAgain) again[threadIdx.x] = 0;
+    int n = 0;
     walk_share<false>(a, pv.wide, wide, rounds, shares, share, kvh, fG, wide_parts, [&](const Pass& p) {
-        if (p.nflat - kUnitRows * p.u > 2 * kQB) wide8_pass<kInt8, kTree, 4>(a, p, kvh, fG, sl2, smem);
-        else wide8_pass<kInt8, kTree, 2>(a, p, kvh, fG, sl2, smem);
+        uint8_t* const flag = again + min(n++, kAgain - 1);
+        if (p.nflat - kUnitRows * p.u > 2 * kQB) wide8_pass<kInt8, kTree, 4>(a, p, kvh, fG, sl2, smem, flag);
+        else wide8_pass<kInt8, kTree, 2>(a, p, kvh, fG, sl2, smem, flag);
     });
     lds_barrier();  // the last wide pass's rows have been read
-    few8_walk<kInt8, kTree>(a, pv.few, few, share, kvh, fG, sl2, few_parts, smem);
+    few8_walk<kInt8, kTree>(a, pv.few, few, share, kvh, fG, sl2, few_parts, smem, again + kAgain);
+    lds_barrier();
+    const int lane = threadIdx.x & 63;
+    const uint64_t wides = __builtin_amdgcn_ballot_w64(again[lane] != 0);
+    const uint64_t fews = __builtin_amdgcn_ballot_w64(again[kAgain + lane] != 0);
+    if (wides | fews) share_again<kInt8, kTree>(a, shares, share, kvh, wides, fews, wide_parts, few_parts);
 }
 
 // ------------------------------------------------------------------ launchers

@@ -154,7 +154,9 @@ __device__ __forceinline__ void walk_share(const PackedArgs& a, const List& list
         p.nflat = n * (int)fG.d;
         p.T = min(max(p.pos0 + fdiv(min(kUnitRows * p.u + kUnitRows, p.nflat) - 1, fG) + 1, 0), len);
         p.nrange = (cut >= 0 ? cut : (int)y.y) - p.kt_lo;
-        p.part = p.kt_lo > 0 || cut >= 0 ? parts + part_at(kFew, share * a.HKV + kvh, p.kt_lo > 0 ? 0 : 1) : nullptr;
+        // (its place in scalar registers: kept in vector ones it would be spilled)
+        const int place = scalar((int)part_at(kFew, share * a.HKV + kvh, p.kt_lo > 0 ? 0 : 1));
+        p.part = p.kt_lo > 0 || cut >= 0 ? parts + place : nullptr;
         if (pass > 0) lds_barrier();  // the last pass's rows have been read
         run(p);
     }

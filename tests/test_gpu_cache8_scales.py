@@ -1,0 +1,116 @@
+"""GPU tests of attention over the 8-bit pool (include/ei_cache8.h) where its scales are far from 1: everything that
+storing can write, from values of 2^-110 to the largest of fp32, against 64 bits.
+
+The bar of an element, where v_t = code * scale, w_t the row's softmax weights, N the keys and S the largest score in
+log2 units:
+
+  2^-20 (2 + S) sum_t w_t |v_t|   A score is rounded at its own size at least twice (2^-23 S together) and its weight is
+                                  off by ln 2 times that, numerator and denominator alike: below 2^-22 S.  Products of
+                                  two operands of 22 bits, and fp32 sums over tiles, waves and parts: below 2^-19.
+  2^-38 N max_t w_t scale_t max_d |code_td|
+                                  Planes of a weight times scale end at half of 2^-24 where the row's largest weight
+                                  times scale is 2^13 or more: 2^-38 of it for each key, times codes.
+  sum of w_t |v_t| over w_t < 2^-116
+                                  Such weights may count as zero.
+"""
+import math
+
+import pytest
+import torch
+
+from tests.cache8_plain import D, SCALE, Batch, cached64, fill_cache, i32, sees
+
+pytestmark = pytest.mark.gpu
+KINDS = ["e4m3", "int8"]
+# units of single tokens and drafts; of up to 64 and of up to 128 rows; more than one of them
+BATCHES = [([1, 4], [900, 300]), ([12, 15], [400, 700]), ([35], [700]), ([140], [500])]
+
+
+def _normal(seed, *shape):
+    return torch.randn(shape, generator=torch.Generator(device="cuda").manual_seed(seed), device="cuda")
+
+
+def _worst(q, k, v, seen, got):
+    """The largest error as a part of its bar (q [n, H, 128], k and v [N, 1, 128] in 64 bits)."""
+    n, H, _ = q.shape
+    k, v, N = k[:, 0], v[:, 0], v.shape[0]
+    hidden = ~seen.to(q.device)[:, None].expand(n, H, N)
+    s = (q.reshape(-1, D) @ k.t().contiguous()).view(n, H, N) * (SCALE / math.log(2.0))
+    s = s.masked_fill(hidden, -math.inf)
+    w = torch.softmax(s * math.log(2.0), -1)
+    S = s.masked_fill(hidden, 0.0).abs().amax(-1, keepdim=True)
+    def mix(w, v):
+        return (w.reshape(-1, N) @ v).view(n, H, D)
+    bar = 2.0 ** -20 * (2 + S) * mix(w, v.abs())
+    bar = bar + 2.0 ** -38 * N * (w * v.abs().amax(-1)).amax(-1, keepdim=True)
+    bar = bar + mix(torch.where(w < 2.0 ** -116, w, torch.zeros_like(w)), v.abs())
+    assert bool(torch.isfinite(got).all())
+    off = (got.double() - mix(w, v)).abs()
+    return float((off / torch.where(bar == 0, torch.ones_like(bar), bar)).max())
+
+
+def _check(b, cache, q, out, mask_bits=None):
+    for s, (n, total) in enumerate(zip(b.lens, b.totals)):
+        r = b.rows_of(s)
+        k, v = cached64(cache, b.table_np[s], total)
+        seen = sees(n, total, None if mask_bits is None else mask_bits[r])
+        e = _worst(q[r].view(n, b.H, D).double(), k, v, seen, out[r])
+        assert e < 1, (s, n, total, e)
+
+
+def _batch(gpu, lens, past, seed):
+    return Batch(gpu, 4, 1, lens, [p + n for p, n in zip(past, lens)], 32, seed=seed)
+
+
+def _keys_of_ones(gpu, kind, b, seed, log2_score):
+    """A cache whose keys give queries of ones the log2 scores log2_score(t) (a function of the keys' numbers)."""
+    cache = fill_cache(gpu, kind, b.n_blocks, 32, 1, seed, spread=0.2)
+    cache.k.copy_(torch.ones(cache.k.shape, device="cuda").to(cache.k.dtype))
+    for s, total in enumerate(b.totals):
+        t = torch.arange(total, device="cuda")
+        page = i32(b.table_np[s]).long()[t // 32]
+        cache.k_scale[page, 0, t % 32] = log2_score(t).float() * (math.log(2.0) / SCALE / D)
+    return cache
+
+
+# ------------------------------------------------------------------ tiny values
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("lens,past", BATCHES + [([1], [20000])])
+@pytest.mark.parametrize("power", [-84, -98, -104, -110])
+def test_tiny_values(gpu, kind, lens, past, power):
+    """Scales of 2^-9 to 2^-4 times 2^power: down to the smallest that are stored."""
+    b = _batch(gpu, lens, past, 1)
+    cache = fill_cache(gpu, kind, b.n_blocks, 32, 1, 2, spread=0.2)
+    cache.v_scale.clamp_(2.0 ** -9, 2.0 ** -4).mul_(2.0 ** power)
+    q = _normal(3, b.rows, 4 * D)
+    _check(b, cache, q, gpu.attn_packed_cache8(q, cache, b.table, b.plan, b.shape))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("lens,past", BATCHES)
+def test_tiny_values_behind_others(gpu, kind, lens, past):
+    """Tiny values at the keys that have all the weight, ordinary ones at earlier keys that have next to none."""
+    b = _batch(gpu, lens, past, 4)
+    cache = _keys_of_ones(gpu, kind, b, 5, lambda t: torch.where(t < 200, -150.0, 0.0))
+    for s, total in enumerate(b.totals):
+        t = torch.arange(200, total, device="cuda")
+        cache.v_scale[i32(b.table_np[s]).long()[t // 32], 0, t % 32] *= 2.0 ** -105
+    q = torch.ones((b.rows, 4 * D), device="cuda")
+    _check(b, cache, q, gpu.attn_packed_cache8(q, cache, b.table, b.plan, b.shape))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_tiny_values_as_stored(gpu, kind):
+    """A step whose values are around 2^-108 gives what the same step gives for them times 2^108, scaled."""
+    A = gpu
+    lens, past = [3, 40, 1], [0, 0, 0]
+    outs = []
+    for power in (0, -108):
+        b = Batch(A, 8, 4, lens, [p + n for p, n in zip(past, lens)], 32, seed=6)
+        qkv = _normal(7, b.rows, 16 * D)
+        qkv[:, 12 * D:] = (1 + qkv[:, 12 * D:].abs()) * 2.0 ** power
+        cache, ones = A.Cache8(b.n_blocks, 32, 4, kind), torch.ones(D, device="cuda")
+        outs.append(A.packed_step_cache8(qkv, cache, b.table, b.plan, b.shape, ones, ones, A.rope_table(64)))
+    # The same codes, in two arithmetics: positive values, so that each is within 2^-20 (2 + S) of itself (the bar above),
+    # scores of normed rows at most 128 / sqrt(128) log2(e) = 16.4 (of keys off by 1/254 or 1/16 of themselves, 17.4)
+    assert bool(((outs[0] - outs[1] * 2.0 ** 108).abs() <= 2 * 2.0 ** -20 * 19.4 * outs[0]).all())
