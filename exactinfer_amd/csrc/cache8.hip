@@ -816,8 +816,7 @@ __device__ __forceinline__ void few8_walk(const Cache8Args& a, const List& list,
 // e4m3) 188 us against 144.
 constexpr int kK8RowB = 2 * kHeadDim + 16, kK8Tile = kKT * kK8RowB;  // [32 keys][128 d], rows spread over banks
 constexpr int kV8RowB = 2 * kKT + 16, kV8Tile = kHeadDim * kV8RowB;  // [128 d][32 keys]
-constexpr int kBigAt8 = 2 * kKT * 4;  // after the scales of K and V: the largest big one (of K, of V)
-constexpr int kScales8 = kBigAt8 + 16;
+constexpr int kScales8 = 2 * kKT * 4;                                // of K, of V
 constexpr int kBuf8 = kK8Tile + kV8Tile + kScales8;                 // one tile of a group
 static_assert(kBuf8 % 16 == 0, "16-byte pieces");
 template <int kS>
@@ -919,14 +918,12 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
         *reinterpret_cast<u32x2*>(d) = u32x2{pair_f16<kInt8, 0>(lo), pair_f16<kInt8, 0>(hi)};
         *reinterpret_cast<u32x2*>(d + kV8RowB) = u32x2{pair_f16<kInt8, 1>(lo), pair_f16<kInt8, 1>(hi)};
     };
-    // (the upper half of the wave writes the largest big one)
-    // (no branch: a spill among the instructions of one side would save half of the lanes)
-    const uint32_t to_scales = kK8Tile + kV8Tile + 4 * kKT * (hw & 1) + 4 * col +
-                               hh * (kBigAt8 + 4 * (hw & 1) - 4 * kKT * (hw & 1) - 4 * col);
+    // (both halves of the wave write the same.  A big scale of V, whichever rows see it, takes the pass to pass_again:
+    // F lowered for it would cost the rows that do not see it their bits)
+    const uint32_t to_scales = kK8Tile + kV8Tile + 4 * kKT * (hw & 1) + 4 * col;
     auto store_scales = [&](int i) {
-        float big = 0.f;
-        if (__builtin_amdgcn_ballot_w64(__builtin_fabsf(ts) > kBigScale)) big = wave_max(big_scale(ts));
-        *reinterpret_cast<float*>(buf(i) + to_scales) = hh ? big : ts;
+        if ((hw & 1) && __builtin_amdgcn_ballot_w64(__builtin_fabsf(ts) > kBigScale)) *again = 1;
+        *reinterpret_cast<float*>(buf(i) + to_scales) = ts;
     };
     auto store_all_k = [&](int i) {
 #pragma unroll
@@ -1046,7 +1043,6 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
         f32x4 f[4];
 #pragma unroll
         for (int c = 0; c < 4; ++c) f[c] = *reinterpret_cast<const f32x4*>(sc + 8 * c);
-        const float big = *reinterpret_cast<const float*>(buf(i) + kK8Tile + kV8Tile + kBigAt8 + 4);
         read_k(i + 1, 0), read_k(i + 1, 1);
         fence();
 #pragma unroll
@@ -1082,11 +1078,6 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
             if (__builtin_amdgcn_ballot_w64(fn - fe != up)) scale_sums(pow2(fn - fe - up));
             fe = fn;
             m = mn;
-        }
-        if (uniform(big) != 0.f) {
-            const int fn = min(fe, most_f(big));
-            scale_sums(pow2(fn - fe));
-            fe = fn;
         }
         // ---- weights times scales times F
         const float nb = m == -INFINITY ? 0.f : (float)fe - m;

@@ -114,3 +114,43 @@ def test_tiny_values_as_stored(gpu, kind):
     # The same codes, in two arithmetics: positive values, so that each is within 2^-20 (2 + S) of itself (the bar above),
     # scores of normed rows at most 128 / sqrt(128) log2(e) = 16.4 (of keys off by 1/254 or 1/16 of themselves, 17.4)
     assert bool(((outs[0] - outs[1] * 2.0 ** 108).abs() <= 2 * 2.0 ** -20 * 19.4 * outs[0]).all())
+
+
+# ------------------------------------------------------------------ scales that a row does not see
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("power", [60, 100, 117])
+@pytest.mark.parametrize("tree", [False, True])
+@pytest.mark.parametrize("n", [4, 15, 40])
+def test_huge_values_that_a_row_does_not_see(gpu, kind, power, tree, n):
+    """Finite huge values at new keys that some rows see and others do not, beside scales of some 2^-20: rows that do not
+    see them keep their bits.  Eight sequences of eight KV heads, so that a workgroup takes several tiles of one; nearly
+    all weight is at the new keys, which share their tiles with the huge ones."""
+    H, HKV, past, seqs = 32, 8, 990, 8
+    total = past + n
+    b = Batch(gpu, H, HKV, [n] * seqs, [total] * seqs, 32, seed=11)
+    cache = fill_cache(gpu, kind, b.n_blocks, 32, HKV, 12, spread=0.2)
+    cache.k.copy_(torch.ones(cache.k.shape, device="cuda").to(cache.k.dtype))
+    cache.v_scale.mul_(2.0 ** -14)
+    huge = sorted({total - 1, past + n // 2})
+    t = torch.arange(total, device="cuda")
+    for s in range(seqs):
+        page = i32(b.table_np[s]).long()[t // 32]
+        score = torch.where(t < past, -30.0, 0.1 * (t % 7)).float() * (math.log(2.0) / SCALE / D)
+        cache.k_scale[page, :, t % 32] = score[:, None]
+        for h in huge:
+            cache.v_scale[page[h], :, h % 32] = 2.0 ** power
+    q = 1 + 0.1 * _normal(13, b.rows, H * D)
+    mask, bits, _ = b.trees(width=3) if tree else (None, None, None)
+    out = gpu.attn_packed_cache8(q, cache, b.table, b.plan, b.shape, mask=mask)
+    for s in range(seqs):
+        r = b.rows_of(s)
+        k, v = cached64(cache, b.table_np[s], total)
+        seen = sees(n, total, None if bits is None else bits[r])
+        for rows in (~seen[:, huge].any(1), seen[:, huge].any(1)):
+            at = rows.cuda()
+            if not bool(rows.any()):
+                continue
+            for h in (0, 5):
+                heads = slice(h * (H // HKV), (h + 1) * (H // HKV))
+                q64 = q[r].view(n, H, D).double()[at][:, heads]
+                assert _worst(q64, k[:, h:h + 1], v[:, h:h + 1], seen[rows], out[r][at][:, heads]) < 1, (s, h)
