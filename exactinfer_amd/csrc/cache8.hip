@@ -360,13 +360,7 @@ constexpr int kTopF = 96;                              // log2 F at most
 constexpr float kTopW = 0x1p15f;                       // p s_v F at most
 constexpr int kAgain = 64;                              // flags of passes to be done again
 constexpr float kLazy8 = 8.f;                          // the reference moves when a score passes it by more
-// Scales of values in between (larger ones are not provided for) keep F so low that p s_v F stays finite.
-constexpr float kBigScale = 0x1p20f, kMostScale = 0x1p118f;
-__device__ __forceinline__ float big_scale(float s) {  // s if it is one, else 0
-    s = __builtin_fabsf(s);
-    return s > kBigScale && s <= kMostScale ? s : 0.f;
-}
-__device__ __forceinline__ int most_f(float big) { return 127 + 118 - (int)(__float_as_uint(big) >> 23); }
+constexpr float kBigScale = 0x1p20f;                   // larger scales of values: pass_again
 __device__ __forceinline__ float pow2(int e) { return __builtin_amdgcn_ldexpf(1.f, e); }
 
 // The streaming cache policy of a buffer load, for codes that are read once: 60000 keys 27 us, without it 29.
@@ -646,15 +640,12 @@ __device__ __forceinline__ void few8_walk(const Cache8Args& a, const List& list,
             float big = 0.f;
 #pragma unroll
             for (int r = 0; r < 8; ++r) big = fmaxf(big, __builtin_fabsf(t.vs[r >> 2][r & 3]));
-            if (__builtin_amdgcn_ballot_w64(big > kBigScale)) {
+            if (__builtin_amdgcn_ballot_w64(big > kBigScale)) {  // (pages behind the last key may hold anything)
                 big = 0.f;
 #pragma unroll
                 for (int r = 0; r < 8; ++r)
-                    if (seen(r)) big = fmaxf(big, big_scale(t.vs[r >> 2][r & 3]));
-                big = row_max(big);
-                const int fn = big > 0.f ? min(fe, most_f(big)) : fe;
-                scale_sums(pow2(fn - fe));
-                fe = fn;
+                    if (seen(r)) big = fmaxf(big, __builtin_fabsf(t.vs[r >> 2][r & 3]));
+                if (__builtin_amdgcn_ballot_w64(big > kBigScale)) again[min(turn, kAgain - 1)] = 1;
             }
             const float nb = m == -INFINITY ? 0.f : (float)fe - m;
             float sum = 0.f, wm = 0.f;

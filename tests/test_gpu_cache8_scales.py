@@ -154,3 +154,44 @@ def test_huge_values_that_a_row_does_not_see(gpu, kind, power, tree, n):
                 heads = slice(h * (H // HKV), (h + 1) * (H // HKV))
                 q64 = q[r].view(n, H, D).double()[at][:, heads]
                 assert _worst(q64, k[:, h:h + 1], v[:, h:h + 1], seen[rows], out[r][at][:, heads]) < 1, (s, h)
+
+
+# ------------------------------------------------------------------ huge values
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("lens,past", BATCHES + [([1], [20000])])
+@pytest.mark.parametrize("power", [60, 100, 118])
+def test_huge_values_of_one_sign(gpu, kind, lens, past, power):
+    """Sums over the keys would pass fp32's range long before they are divided; the outputs do not."""
+    b = _batch(gpu, lens, past, 14)
+    cache = fill_cache(gpu, kind, b.n_blocks, 32, 1, 15, spread=0.2)
+    cache.v.view(torch.int8).bitwise_and_(0x7F) if kind == "e4m3" else cache.v.copy_(cache.v.abs())
+    cache.v_scale.fill_(2.0 ** power)
+    q = _normal(16, b.rows, 4 * D)
+    _check(b, cache, q, gpu.attn_packed_cache8(q, cache, b.table, b.plan, b.shape))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("lens,past", BATCHES + [([1], [20000])])
+def test_small_weights_of_huge_values(gpu, kind, lens, past):
+    """A key with nearly all the weight, and many with 2^-25 of it each."""
+    b = _batch(gpu, lens, past, 17)
+    cache = _keys_of_ones(gpu, kind, b, 18, lambda t: torch.where(t == 100, 25.0, 0.0))
+    cache.v_scale.mul_(2.0 ** 121)
+    for s in range(len(lens)):  # the values of that key are zero in half of the columns
+        cache.v[int(b.table_np[s][3]), 0, 4].view(torch.int8)[:64] = 0
+    q = torch.ones((b.rows, 4 * D), device="cuda")
+    _check(b, cache, q, gpu.attn_packed_cache8(q, cache, b.table, b.plan, b.shape))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("lens,past", BATCHES)
+def test_huge_values_without_weight(gpu, kind, lens, past):
+    """Huge values at keys that have next to no weight beside tiny ones at the others."""
+    b = _batch(gpu, lens, past, 19)
+    cache = _keys_of_ones(gpu, kind, b, 20, lambda t: torch.where(t % 50 == 7, -300.0, 0.0))
+    for s, total in enumerate(b.totals):
+        t = torch.arange(total, device="cuda")
+        cache.v_scale[i32(b.table_np[s]).long()[t // 32], 0, t % 32] = \
+            torch.where(t % 50 == 7, 2.0 ** 117, 2.0 ** -90 * (1 + 0.01 * (t % 32))).float()
+    q = torch.ones((b.rows, 4 * D), device="cuda")
+    _check(b, cache, q, gpu.attn_packed_cache8(q, cache, b.table, b.plan, b.shape))
