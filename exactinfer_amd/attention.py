@@ -536,7 +536,8 @@ _CACHE_KINDS = {"e4m3": (1, torch.float8_e4m3fn), "int8": (2, torch.int8)}
 class Cache8:
     """A paged pool of 8-bit keys and values (include/ei_cache8.h): codes k, v [n_blocks, HKV, block_size, 128]
     (float8_e4m3fn or int8) and scales k_scale, v_scale [n_blocks, HKV, block_size]; a code stands for
-    code * scale.  Made empty (zeros), or of tensors that a program has already."""
+    code * scale.  Made empty (zeros), or of tensors that a program has already; calls read the tensors' addresses each
+    time, the tensors themselves stay those it was made of."""
 
     def __init__(self, n_blocks: int, block_size: int, n_head_kv: int, kind: str = "e4m3", device="cuda"):
         if kind not in _CACHE_KINDS:
@@ -564,14 +565,25 @@ class Cache8:
             if t.dtype is not dtype or t.shape != shape or not t.is_contiguous() or t.device != k.device:
                 raise ValueError(f"{name} must be a contiguous {dtype} tensor {tuple(shape)} on {k.device}, got "
                                  f"{t.dtype} {tuple(t.shape)} on {t.device}")
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
-        self.kind, number = kinds[k.dtype]
-        self.n_blocks, self.n_head_kv, self.block_size = k.shape[:3]
         import ctypes
-        self._c = _capi.Cache8C(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), number,
-                                self.n_blocks, self.block_size)
-        self._at = ctypes.addressof(self._c)
+        self._tensors = k, v, k_scale, v_scale
+        self._kind, number = kinds[k.dtype]
+        self._shape = n_blocks, _, block_size = k.shape[:3]
+        self._at = k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr()
+        self._c = _capi.Cache8C(*self._at, number, n_blocks, block_size)
+        self._c_at = ctypes.addressof(self._c)
         self._device = k.get_device()
+
+    k, v, k_scale, v_scale = (property(lambda self, i=i: self._tensors[i]) for i in range(4))
+    n_blocks, n_head_kv, block_size = (property(lambda self, i=i: self._shape[i]) for i in range(3))
+    kind = property(lambda self: self._kind)
+
+    def _address(self) -> int:
+        """Of the ei_cache8 that the tensors are now."""
+        k, v, k_scale, v_scale = self._tensors
+        if (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr()) != self._at:
+            self._take(k, v, k_scale, v_scale)
+        return self._c_at
 
 
 # (A call's launch takes 4 us of host time; its checks, with a function and a message for each, took as much again.  So
@@ -607,7 +619,8 @@ def _out_of(batch: PackedBatch, out: torch.Tensor | None, dev: int) -> torch.Ten
 
 
 def _cache8_args(cache: Cache8, block_table: torch.Tensor, batch: PackedBatch, n_head_kv: int, dev: int) -> tuple:
-    if cache.n_head_kv != n_head_kv:
+    at = cache._address()
+    if cache._shape[1] != n_head_kv:
         raise ValueError(f"the cache holds {cache.n_head_kv} KV heads, the call has {n_head_kv}")
     if cache._device != dev:
         _refuse("the cache", cache.k, cache.k.dtype)
@@ -616,7 +629,7 @@ def _cache8_args(cache: Cache8, block_table: torch.Tensor, batch: PackedBatch, n
             shape[0] < batch.n_seq or not block_table.is_contiguous()):
         _need_contiguous("block_table", block_table, torch.int32)
         raise ValueError(f"block_table must be [{batch.n_seq}, blocks], got {tuple(shape)}")
-    return cache._at, block_table.data_ptr(), shape[1]
+    return at, block_table.data_ptr(), shape[1]
 
 
 def _pool_of(kc: torch.Tensor, vc: torch.Tensor, block_table: torch.Tensor, block_size: int, batch: PackedBatch,
