@@ -56,7 +56,7 @@ __device__ __forceinline__ size_t head_row(int page, int HKV, int kvh, int shift
 // grid (rows, ceil((H + 2 HKV) / 16)).
 //
 // Bound by memory: 7644 rows of H 32 / HKV 8 (333 MB) 59 to 64 us, 5.2 to 5.6 TB/s, above a large copy's 4.7; with four
-// bytes a lane instead of sixteen 83 us.  48 rows of H 16 / HKV 8 take 5 us: looking up a row's owner and its page.
+// bytes a lane instead of sixteen 83 us.  48 rows of H 16 / HKV 8 take 4 us: looking up a row's owner and its page.
 template <bool kInt8, bool kVec>
 __global__ __launch_bounds__(256) void k_cache8_store(const float* __restrict__ qkv, long row_stride,
                                                       float* __restrict__ q_out, Cache8Args a,
@@ -363,8 +363,9 @@ constexpr float kLazy8 = 8.f;                          // the reference moves wh
 constexpr float kBigScale = 0x1p20f;                   // larger scales of values: pass_again
 __device__ __forceinline__ float pow2(int e) { return __builtin_amdgcn_ldexpf(1.f, e); }
 
-// The streaming cache policy of a buffer load, for codes that are read once: 60000 keys 27 us, without it 29.
-// (Where 24 sequences share all their keys it costs 2%.)
+// The streaming cache policy of a buffer load, for codes that a workgroup reads once: 60000 keys of single tokens, with
+// merge and host, 34.6 us, without it 37.3.  Units of 17 to 32 rows read theirs twice, by two waves, and pay 3 to 9%
+// (32 drafts of 5 after 1000 keys 29.4 us, without it 26.7), 24 sequences that share all their keys 2%.
 constexpr int kOnce = 2;
 
 // ---- sixteen rows of a wave, a tile at a time: each lane its row l % 16 and quarter l / 16
@@ -516,7 +517,7 @@ __device__ __forceinline__ void put_nans(const Rsrc& rv, uint32_t bits, int quar
 // Bound by reading the codes, two tiles of each wave in flight.  A pass is short where sequences are: the next unit
 // and its pages are looked up during a pass, its queries and first tiles fetched before the waves' sums meet.
 // H 32 / HKV 8, pages of 64, e4m3: 60000 keys of one sequence (127 MB) 27 us, as 24 of 2500 keys 29.6, as 96 of 625
-// 32.4 (one pass after another 34.3 and 41.6); 130000 keys 49 us, 5.6 TB/s, or 6.9 past the 8 us that a call over 31
+// 32.4 (one pass after another 34.3 and 41.6); 130000 keys 49 us, 5.6 TB/s, or 6.7 past the 8 us that a call over 31
 // keys takes: launch, plan, unit, page and codes one after another.
 template <bool kInt8, bool kTree>
 __device__ __forceinline__ void few8_walk(const Cache8Args& a, const List& list, int4 sh, int share, int kvh,
@@ -799,16 +800,16 @@ __device__ __forceinline__ void few8_walk(const Cache8Args& a, const List& list,
 // weights' planes between those of P . V, by hand, since the compiler would put each kind together (and every LDS
 // read right before its use).
 //
-// Bound by the matrix unit and its power: 1024 rows after 12000 keys (H 32 / HKV 8, int8) 407 to 423 us, 500 to 517
-// TFLOP/s, 1.0 PFLOP/s over the two plane products, 82 to 85% of what a large fp16 product reaches; the matrix unit is
-// busy 48% of the cycles at 2.0 GHz of 2.4, vector instructions 54%, beside each other.  With the softmax between the
-// products instead of among them 464 us, a barrier for every tile and lanes' addresses made anew 456.  Units of 33 to
-// 64 rows in two groups of four waves, half of them idle: 16 trees of 48 tokens (G 4, 192 rows: units of 128 and 64,
+// Bound by the matrix unit and its power: 1024 rows after 12000 keys (H 32 / HKV 8, int8) 407 to 465 us by box, 455 to
+// 517 TFLOP/s, 0.9 to 1.0 PFLOP/s over the two plane products, 75 to 85% of what a large fp16 product reaches; the
+// matrix unit is busy 48% of the cycles at 2.0 GHz of 2.4, vector instructions 54%, beside each other.  Where it takes
+// 407 us: with the softmax between the products instead of among them 464, a barrier for every tile and lanes'
+// addresses made anew 456.  Units of 33 to 64 rows in two groups of four waves, half of them idle: 16 trees of 48 tokens (G 4, 192 rows: units of 128 and 64,
 // e4m3) 188 us against 144.
 constexpr int kK8RowB = 2 * kHeadDim + 16, kK8Tile = kKT * kK8RowB;  // [32 keys][128 d], rows spread over banks
 constexpr int kV8RowB = 2 * kKT + 16, kV8Tile = kHeadDim * kV8RowB;  // [128 d][32 keys]
 constexpr int kScales8 = 2 * kKT * 4;                                // of K, of V
-constexpr int kBuf8 = kK8Tile + kV8Tile + kScales8;                 // one tile of a group
+constexpr int kBuf8 = kK8Tile + kV8Tile + kScales8;                  // one tile of a group
 static_assert(kBuf8 % 16 == 0, "16-byte pieces");
 template <int kS>
 struct Wide8 {
@@ -822,7 +823,7 @@ struct Wide8 {
     static constexpr int kF = kEnd > kTilesF ? kEnd : kTilesF;
 };
 constexpr int kNanAt8 = Wide8<4>::kF > Wide8<2>::kF ? Wide8<4>::kF : Wide8<2>::kF;  // a word: NaN codes were met
-// Flags of the passes to be done again, a byte each: 64 of the wide ones, 64 of the few-row ones (from the 64th on one).
+// Flags of passes to be done again, a byte each: 64 of the wide ones, 64 of the few-row ones (one from the 64th on).
 constexpr int kAgainAt8 = kNanAt8 + 4;
 constexpr int kLds8 = 4 * kAgainAt8 + 2 * kAgain;
 static_assert(kLds8 <= 160 * 1024 && 2 * kFew8F <= kNanAt8, "LDS budget");
@@ -1291,11 +1292,12 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
 }
 
 // ---- sixteen rows with two references
-// Where F could not serve, a pass is done again when the workgroup is through with the others: sixteen rows for each wave,
-// which takes all tiles, with two references, both whole numbers: m of the weights' sum, and u of the products' sums, the
-// largest log2 of a weight times its value's scale, rounded up.  The operand is (the scale's fraction)
-// 2^(s + its exponent - u + 14), so that no scale overflows or underflows, whatever stands beside it; a key that the row
-// does not see is in neither.  One tile after the other, nothing in flight.
+// Where F could not serve, a pass is done again when the workgroup is through with the others: sixteen rows for each
+// wave, which takes all tiles, with two references, both whole numbers: m of the weights' sum, and u of the products'
+// sums, the largest log2 of a weight times its value's scale, rounded up.  The operand is (the scale's fraction)
+// 2^(s + its exponent - u + 14), so that no scale overflows or underflows, whatever stands beside it; a key that the
+// row does not see is in neither.  One tile after the other, nothing in flight: three to five times slower (24 tokens over
+// 60251 keys 147 us instead of 36, 1024 rows after 12000 keys 1436 instead of 465).
 template <bool kInt8, bool kTree, bool kFew>
 __device__ __forceinline__ void pass_again(const Cache8Args& a, const Pass& p, int kvh, FastDiv fG, float sl2) {
     constexpr int D = kHeadDim;
@@ -1368,8 +1370,8 @@ __device__ __forceinline__ void pass_again(const Cache8Args& a, const Pass& p, i
             if (nans) put_nans(codes_rsrc(a.v8, at.row, at.there), bits, quarter, o);
         }
     }
-    // The weights' sum goes to 1/2 .. 1 (to 2^-17 where values may be near fp32's largest: parts are added), the sums of
-    // products with it.
+    // The weights' sum goes to 1/2 .. 1 (to 2^-17 where values may be near fp32's largest: parts are added), the sums
+    // of products with it.
     const float sum = half_sum(l + lane_xor16(l)), up = fminf(fmaxf(u - m, -400.f), 400.f);
     const int down = __builtin_amdgcn_frexp_expf(sum) + (up > 64.f ? 16 : 0);
     l = __builtin_amdgcn_ldexpf(l, -down);

@@ -1,6 +1,7 @@
 // packed.h — what the attention kernels over batches of several sequences share (packed.hip, cache8.hip): the
-// layout of the plan that k_packed_plan makes, the walk over a workgroup's share of it, the parts of units that its
-// cuts divide, masks of drafted trees, binary16 planes.
+// layout of the plan that k_packed_plan makes, the walk over a workgroup's share of it (cache8.hip's; packed.hip and
+// the pipelined walk over few-row units, few8_walk, each read the plan by the same rules in a loop of their own), the
+// parts of units that its cuts divide, masks of drafted trees, binary16 planes.
 #pragma once
 
 #include "common.h"

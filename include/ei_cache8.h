@@ -7,8 +7,11 @@
  * and whose decode takes one token at a time (:1648-1658).
  *
  * Every call is over a batch that ei_packed_plan laid out with kv_len: rows cu_rows[s] .. cu_rows[s+1] - 1 are the n
- * new rows of sequence s, row i of them stands at slot kv_len[s] - n + i of its cache, and rows past the last
- * sequence's are neither read nor written.  A call whose n_seq, rows or heads differ from the plan's writes nothing.
+ * new rows of sequence s, row i of them stands at slot kv_len[s] - n + i of its cache; of rows past the last
+ * sequence's nothing is used, and nothing is written for them.  A call whose n_seq, rows or heads differ from the
+ * plan's writes nothing.  Lengths must not pass the plan's max_kv: attention takes a longer sequence as ei_packed.h
+ * says, as one of max_kv keys, the last n of which count as its new rows (masks too), while rows at slots from max_kv
+ * on are not stored and ei_cache_keep moves what those slots hold.
  * A call whose outputs, workspace or pools overlap anything else that it reads or writes is refused.
  */
 #ifndef EI_CACHE8_H
@@ -31,8 +34,8 @@ extern "C" {
  *   EI_CACHE_INT8  scale a / 127, codes rint(y * (127 / a)), signed bytes
  *   EI_CACHE_E4M3  scale a / 448, codes y * (448 / a) rounded to the nearest e4m3 (4 exponent bits of bias 7, 3 of
  *                  fraction, no infinities, 0x7F and 0xFF are NaN), ties to even
- * each operation in fp32, rounded once: off by at most a/254 and by half a step of e4m3.  a < 2^-110: scale and codes
- * 0.  a not finite: scale NaN, codes 0 (every value of that head row reads as NaN).
+ * each operation in fp32, rounded once: off by a/254 or half a step of e4m3, and by those roundings.  a < 2^-110:
+ * scale and codes 0.  a not finite: scale NaN, codes 0 (every value of that head row reads as NaN).
  * 264 bytes per key and KV head, against 1024 of the fp32 pool. */
 enum { EI_CACHE_E4M3 = 1, EI_CACHE_INT8 = 2 };
 typedef struct ei_cache8 {
@@ -89,12 +92,14 @@ int ei_tree_step_paged(ei_stream_t stream, const float* qkv, long row_stride, fl
  * of a block whose entry is not in [0, n_blocks), count as zeros: nothing is read there.
  *
  * Codes are exact in binary16; q and the weights, each times the value's scale, are two binary16 planes, which keep
- * 22 bits of 24 down to 2^-39 of a query's largest value and of a row's largest weight times scale so far.  Sums and
- * softmax in fp32.  Scales of keys up to 2^96 and of values up to 2^118 are provided for (larger ones give infinities
- * and NaN; beside scales of values above 2^90 smaller ones keep fewer bits).  Key and value rows that a row does not
- * see never reach it, whatever they hold; a NaN scale that it does see makes its output NaN, a NaN code of a key too,
- * and one of a value that column of it.  A batch called twice gives the same bits; they differ in the last ones with
- * the batch a sequence is in. */
+ * 22 bits of 24 down to 2^-39 of a query's largest value and of a row's largest weight times scale so far (2^-38 where
+ * keys are taken again).  Sums and softmax in fp32; weights below 2^-116 of a row's largest may count as zero.  Scales
+ * of keys up to 2^96 are provided for (larger ones give infinities and NaN), and all that values can have.  Where a
+ * scale above 2^20 is among the values, or none of a row's weights times scales reaches 2^-82, the workgroup takes
+ * those keys again, three to five times slower.  Key and value rows that a row does not see never reach it, whatever
+ * they hold; a NaN scale that it does see makes its output NaN, a NaN code of a key too, and one of a value that
+ * column of it.  A batch called twice gives the same bits; they differ in the last ones with the batch a sequence is
+ * in. */
 int ei_attn_packed_cache8(ei_stream_t stream, const float* q, long q_stride, float* out, const ei_cache8* cache,
                           const int* block_table, int max_blocks, int n_seq, int rows, int n_head, int n_head_kv,
                           int head_dim, const uint64_t* mask, int mask_words, float scale, const void* plan,

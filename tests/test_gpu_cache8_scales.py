@@ -111,8 +111,8 @@ def test_tiny_values_as_stored(gpu, kind):
         qkv[:, 12 * D:] = (1 + qkv[:, 12 * D:].abs()) * 2.0 ** power
         cache, ones = A.Cache8(b.n_blocks, 32, 4, kind), torch.ones(D, device="cuda")
         outs.append(A.packed_step_cache8(qkv, cache, b.table, b.plan, b.shape, ones, ones, A.rope_table(64)))
-    # The same codes, in two arithmetics: positive values, so that each is within 2^-20 (2 + S) of itself (the bar above),
-    # scores of normed rows at most 128 / sqrt(128) log2(e) = 16.4 (of keys off by 1/254 or 1/16 of themselves, 17.4)
+    # The same codes, in two arithmetics: positive values, so that each is within 2^-20 (2 + S) of itself (the bar
+    # above), scores of normed rows at most 128 / sqrt(128) log2(e) = 16.4 (of keys off by 1/254 or 1/16 of themselves, 17.4)
     assert bool(((outs[0] - outs[1] * 2.0 ** 108).abs() <= 2 * 2.0 ** -20 * 19.4 * outs[0]).all())
 
 
@@ -122,8 +122,8 @@ def test_tiny_values_as_stored(gpu, kind):
 @pytest.mark.parametrize("tree", [False, True])
 @pytest.mark.parametrize("n", [4, 15, 40])
 def test_huge_values_that_a_row_does_not_see(gpu, kind, power, tree, n):
-    """Finite huge values at new keys that some rows see and others do not, beside scales of some 2^-20: rows that do not
-    see them keep their bits.  Eight sequences of eight KV heads, so that a workgroup takes several tiles of one; nearly
+    """Finite huge values at new keys that some rows see and others do not, beside scales of some 2^-20: rows that do
+    not see them keep their bits.  Eight sequences of eight KV heads, so that a workgroup takes several tiles of one; nearly
     all weight is at the new keys, which share their tiles with the huge ones."""
     H, HKV, past, seqs = 32, 8, 990, 8
     total = past + n
