@@ -1358,8 +1358,9 @@ __device__ __forceinline__ void pass_again(const Cache8Args& a, const Pass& p, i
         for (int r = 0; r < 8; ++r) {
             const float e = (float)(14 + __builtin_amdgcn_frexp_expf(scale[r]));
             sum += __builtin_amdgcn_exp2f(mn == -INFINITY ? score[r] : score[r] - mn);
-            w[r] = __builtin_amdgcn_frexp_mantf(scale[r]) *
-                   __builtin_amdgcn_exp2f(score[r] + (un == -INFINITY ? e : e - un));
+            const float y = __builtin_amdgcn_frexp_mantf(scale[r]) *
+                            __builtin_amdgcn_exp2f(score[r] + (un == -INFINITY ? e : e - un));
+            w[r] = scale[r] == 0.f ? 0.f : y;  // (its score has not met u, and may be far above)
         }
         l += sum;
         if constexpr (kInt8) {

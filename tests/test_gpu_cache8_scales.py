@@ -116,6 +116,24 @@ def test_tiny_values_as_stored(gpu, kind):
     assert bool(((outs[0] - outs[1] * 2.0 ** 108).abs() <= 2 * 2.0 ** -20 * 19.4 * outs[0]).all())
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("lens,past", BATCHES)
+@pytest.mark.parametrize("score,power", [(0.0, -110), (60.0, -50)])
+def test_zeros_beside_tiny_values(gpu, kind, lens, past, score, power):
+    """Values that are zero (and a page that is not there) with as much weight as tiny ones, or much more."""
+    b = _batch(gpu, lens, past, 8)
+    cache = _keys_of_ones(gpu, kind, b, 9, lambda t: torch.where(t % 5 == 2, score, 0.0))
+    cache.v_scale.mul_(2.0 ** power)
+    table = b.table_np.copy()
+    for s, total in enumerate(b.totals):
+        t = torch.arange(2, total, 5, device="cuda")
+        cache.v_scale[i32(table[s]).long()[t // 32], 0, t % 32] = 0.0
+        table[s, 1] = -1
+    b.table_np = table
+    q = torch.ones((b.rows, 4 * D), device="cuda")
+    _check(b, cache, q, gpu.attn_packed_cache8(q, cache, i32(table), b.plan, b.shape))
+
+
 # ------------------------------------------------------------------ scales that a row does not see
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("power", [60, 100, 117])
