@@ -1444,6 +1444,7 @@ __global__ __launch_bounds__(64 * kWaves) void k_cache8_attn(Cache8Args a, int s
     if (threadIdx.x < 2 * kAgain) again[threadIdx.x] = 0;
     int n = 0;
     walk_share<false>(a, pv.wide, wide, rounds, shares, share, kvh, fG, wide_parts, [&](const Pass& p) {
+        if (n == 0) lds_barrier();  // the flags are clear before a wave sets one
         uint8_t* const flag = again + min(n++, kAgain - 1);
         if (p.nflat - kUnitRows * p.u > 2 * kQB) wide8_pass<kInt8, kTree, 4>(a, p, kvh, fG, sl2, smem, flag);
         else wide8_pass<kInt8, kTree, 2>(a, p, kvh, fG, sl2, smem, flag);
