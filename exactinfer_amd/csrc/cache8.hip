@@ -1295,8 +1295,8 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
 // Where F could not serve, a pass is done again when the workgroup is through with the others: sixteen rows for each
 // wave, which takes all tiles, with two references, both whole numbers: m of the weights' sum, and u of the products'
 // sums, the largest log2 of a weight times its value's scale, rounded up.  The operand is (the scale's fraction)
-// 2^(s + its exponent - u + 14), so that no scale overflows or underflows, whatever stands beside it; a key that the
-// row does not see is in neither.  One tile after the other, nothing in flight: three to five times slower (24 tokens over
+// 2^(s + its exponent - u + 15), so that no scale overflows or underflows, whatever stands beside it; a key that the
+// row does not see is in neither.  The row's largest operand lies between 2^13 and 2^15.  One tile after the other, nothing in flight: three to five times slower (24 tokens over
 // 60251 keys 147 us instead of 36, 1024 rows after 12000 keys 1436 instead of 465).
 template <bool kInt8, bool kTree, bool kFew>
 __device__ __forceinline__ void pass_again(const Cache8Args& a, const Pass& p, int kvh, FastDiv fG, float sl2) {
@@ -1356,7 +1356,7 @@ __device__ __forceinline__ void pass_again(const Cache8Args& a, const Pass& p, i
         float w[8], sum = 0.f;
 #pragma unroll
         for (int r = 0; r < 8; ++r) {
-            const float e = (float)(14 + __builtin_amdgcn_frexp_expf(scale[r]));
+            const float e = (float)(15 + __builtin_amdgcn_frexp_expf(scale[r]));
             sum += __builtin_amdgcn_exp2f(mn == -INFINITY ? score[r] : score[r] - mn);
             const float y = __builtin_amdgcn_frexp_mantf(scale[r]) *
                             __builtin_amdgcn_exp2f(score[r] + (un == -INFINITY ? e : e - un));
@@ -1380,7 +1380,7 @@ __device__ __forceinline__ void pass_again(const Cache8Args& a, const Pass& p, i
 #pragma unroll
     for (int y = 0; y < 8; ++y)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) o[y][r] = __builtin_amdgcn_ldexpf(o[y][r], (int)up - 14 - down);
+        for (int r = 0; r < 4; ++r) o[y][r] = __builtin_amdgcn_ldexpf(o[y][r], (int)up - 15 - down);
     if (m == -INFINITY) {  // (scores of -infinity beside infinite values; parts without weights are left out)
         float z = 0.f;
 #pragma unroll
