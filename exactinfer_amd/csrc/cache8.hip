@@ -804,8 +804,8 @@ __device__ __forceinline__ void few8_walk(const Cache8Args& a, const List& list,
 // 517 TFLOP/s, 0.9 to 1.0 PFLOP/s over the two plane products, 75 to 85% of what a large fp16 product reaches; the
 // matrix unit is busy 48% of the cycles at 2.0 GHz of 2.4, vector instructions 54%, beside each other.  Where it takes
 // 407 us: with the softmax between the products instead of among them 464, a barrier for every tile and lanes'
-// addresses made anew 456.  Units of 33 to 64 rows in two groups of four waves, half of them idle: 16 trees of 48 tokens (G 4, 192 rows: units of 128 and 64,
-// e4m3) 188 us against 144.
+// addresses made anew 456.  Units of 33 to 64 rows in two groups of four waves, half of them idle: 16 trees of 48
+// tokens (G 4, 192 rows: units of 128 and 64, e4m3) 188 us against 144.
 constexpr int kK8RowB = 2 * kHeadDim + 16, kK8Tile = kKT * kK8RowB;  // [32 keys][128 d], rows spread over banks
 constexpr int kV8RowB = 2 * kKT + 16, kV8Tile = kHeadDim * kV8RowB;  // [128 d][32 keys]
 constexpr int kScales8 = 2 * kKT * 4;                                // of K, of V
@@ -1296,8 +1296,9 @@ __device__ __forceinline__ void wide8_pass(const Cache8Args& a, const Pass& p, i
 // wave, which takes all tiles, with two references, both whole numbers: m of the weights' sum, and u of the products'
 // sums, the largest log2 of a weight times its value's scale, rounded up.  The operand is (the scale's fraction)
 // 2^(s + its exponent - u + 15), so that no scale overflows or underflows, whatever stands beside it; a key that the
-// row does not see is in neither.  The row's largest operand lies between 2^13 and 2^15.  One tile after the other, nothing in flight: three to five times slower (24 tokens over
-// 60251 keys 147 us instead of 36, 1024 rows after 12000 keys 1436 instead of 465).
+// row does not see is in neither.  The row's largest operand lies between 2^13 and 2^15.  One tile after the other,
+// nothing in flight: three to five times slower (24 tokens over 60251 keys 147 us instead of 36, 1024 rows after 12000
+// keys 1436 instead of 465).
 template <bool kInt8, bool kTree, bool kFew>
 __device__ __forceinline__ void pass_again(const Cache8Args& a, const Pass& p, int kvh, FastDiv fG, float sl2) {
     constexpr int D = kHeadDim;

@@ -96,10 +96,10 @@ int ei_tree_step_paged(ei_stream_t stream, const float* qkv, long row_stride, fl
  * keys are taken again).  Sums and softmax in fp32; weights below 2^-116 of a row's largest may count as zero, and
  * outputs below fp32's normal numbers.  Scales of keys up to 2^96 are provided for (larger ones give infinities and
  * NaN), and all that values can have.  Where a scale above 2^20 is among the values, or none of a row's weights times
- * scales reaches 2^-82, the workgroup takes those keys again, three to five times slower.  Key and value rows that a row
- * does not see never reach it, whatever they hold; a NaN scale that it does see makes its output NaN, a NaN code of a
- * key too, and one of a value that column of it.  A batch called twice gives the same bits; they differ in the last ones
- * with the batch a sequence is in. */
+ * scales reaches 2^-82, the workgroup takes those keys again, three to five times slower.  Key and value rows that a
+ * row does not see never reach it, whatever they hold; a NaN scale that it does see makes its output NaN, a NaN code of
+ * a key too, and one of a value that column of it.  A batch called twice gives the same bits; they differ in the last
+ * ones with the batch a sequence is in. */
 int ei_attn_packed_cache8(ei_stream_t stream, const float* q, long q_stride, float* out, const ei_cache8* cache,
                           const int* block_table, int max_blocks, int n_seq, int rows, int n_head, int n_head_kv,
                           int head_dim, const uint64_t* mask, int mask_words, float scale, const void* plan,
